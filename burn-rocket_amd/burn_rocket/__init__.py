@@ -69,6 +69,14 @@ SIGNATURES = {
     "rk_attention_dev_noalloc": (_i, [_p, _p, _p, _i64, _i64, _i, _i, _i, _f, _f, _i, _i64, _i64, _i64, _p, _p]),
     "rk_flash_attn_f16": (_i, [_i64, _i64, _i, _i, _i, _i, _f, _f, _i, _i64, _i64, _i64, _p, _p, _p, _p]),
     "rk_flash_attn_f16_masked": (_i, [_i64, _i64, _i, _i, _i, _i, _f, _f, _p, _p, _p, _p, _p]),
+    "rk_packed_plan_create": (_i, [_p, _i64, _i, _i, _i, _i, _i64, _p]),
+    "rk_paged_plan_create": (_i, [_p, _p, _p, _i64, _i64, _i64, _i, _i, _i, _i, _i, _i64, _p]),
+    "rk_packed_plan_update": (_i, [_p, _p, _i64, _p]),
+    "rk_paged_plan_update": (_i, [_p, _p, _p, _p, _i64, _i64, _p]),
+    "rk_seq_plan_destroy": (_i, [_p]),
+    "rk_attention_packed_dev": (_i, [_p, _p, _i64, _p, _i64, _p, _i64, _f, _f, _p, _i64, _i, _p]),
+    "rk_attention_paged_dev": (_i, [_p, _p, _i64, _p, _p, _f, _f, _p, _i64, _i, _p]),
+    "rk_paged_append_dev": (_i, [_p, _p, _i64, _p, _p, _c.c_double, _p, _p, _i, _i64, _p, _i64, _p, _p, _i, _p]),
     "rk_moe_route": (_i, [_p, _i64, _i, _i, _i, _p, _p]),
     "rk_pack_moe_q8_0": (_i, [_p, _p, _p, _i, _i64, _i64, _p]),
     "rk_pack_moe_f32": (_i, [_p, _p, _p, _i, _i64, _i64, _p]),
@@ -505,6 +513,146 @@ def flash_attn_f16(q, k, v, n_q, n_kv, head_dim, n_head, n_kv_heads, scale, soft
                                   float(softcap), mode, window, q0, k0, _ptr(q16), _ptr(k16), _ptr(v16),
                                   _ptr(out)), "rocket_flash_attn_fp16_ctx", n_q, n_kv, head_dim)
     return out.view(np.float16).reshape(n_head, n_q, dv)
+
+
+# ---------------------------------------------- batches of sequences, paged KV
+def _lens(a):
+    a = np.asarray(a)
+    if a.size and (a.dtype.kind not in "iu" or a.min() < -2**31 or a.max() >= 2**31):
+        _shape_error("plan", "lengths and page ids are whole numbers of 32 bits")
+    return np.ascontiguousarray(a, dtype=np.int32)
+
+
+class SeqPlan:
+    """A plan of rk_packed_plan_create or rk_paged_plan_create (`ptr`): what a batch of
+    sequences looks like. Freed with the object, or by `destroy`."""
+
+    def __init__(self, ptr, n_tokens, heads, page_size=0):
+        self.ptr, self.n_tokens, self.page_size = ptr, n_tokens, page_size
+        self.n_head, self.n_kv_heads, self.head_dim = heads
+
+    def update(self, q_lens, kv_lens=None, page_table=None, stream=None):
+        """Another batch with the same heads, mask and pages; ordered on `stream`."""
+        q = _lens(q_lens)
+        st = ctypes.c_void_p(stream) if stream else None
+        if self.page_size == 0:
+            _check(_lib.rk_packed_plan_update(self.ptr, _ptr(q), q.size, st), "packed_plan_update")
+        else:
+            kv, table = _lens(kv_lens), _lens(page_table)
+            if kv.size != q.size or table.ndim != 2 or table.shape[0] != q.size:
+                _shape_error("paged_plan_update", "q_lens, kv_lens [n] and page_table [n, pages]")
+            _check(_lib.rk_paged_plan_update(self.ptr, _ptr(q), _ptr(kv), _ptr(table), table.shape[1], q.size, st),
+                   "paged_plan_update")
+        self.n_tokens = int(q.sum(dtype=np.int64))
+
+    def destroy(self):
+        if self.ptr:
+            _check(_lib.rk_seq_plan_destroy(self.ptr), "seq_plan_destroy")
+            self.ptr = None
+
+    def __del__(self):
+        try:
+            if self.ptr and _lib is not None:
+                _lib.rk_seq_plan_destroy(self.ptr)
+        except Exception:
+            pass
+
+
+def packed_plan(q_lens, n_head, n_kv_heads, head_dim, mode=MASK_CAUSAL, window=-1):
+    """The plan of sequences of q_lens tokens that lie one behind the other."""
+    load_library()
+    q, out = _lens(q_lens), ctypes.c_void_p()
+    _check(_lib.rk_packed_plan_create(_ptr(q), q.size, n_head, n_kv_heads, head_dim, mode, window, ctypes.byref(out)),
+           "packed_plan")
+    return SeqPlan(out.value, int(q.sum(dtype=np.int64)), (n_head, n_kv_heads, head_dim))
+
+
+def paged_plan(q_lens, kv_lens, page_table, n_pages, page_size, n_head, n_kv_heads, head_dim, mode=MASK_CAUSAL,
+               window=-1):
+    """The plan of sequences whose kv_lens keys (the last q_lens of them new) lie in the pages that the rows of
+    page_table [n, pages] name, in a cache [n_pages, n_kv_heads, page_size, head_dim]."""
+    load_library()
+    q, kv, table, out = _lens(q_lens), _lens(kv_lens), _lens(page_table), ctypes.c_void_p()
+    if kv.size != q.size or table.ndim != 2 or table.shape[0] != q.size:
+        _shape_error("paged_plan", "q_lens, kv_lens [n] and page_table [n, pages]")
+    _check(_lib.rk_paged_plan_create(_ptr(q), _ptr(kv), _ptr(table), table.shape[1], q.size, n_pages, page_size, n_head,
+                                     n_kv_heads, head_dim, mode, window, ctypes.byref(out)), "paged_plan")
+    return SeqPlan(out.value, int(q.sum(dtype=np.int64)), (n_head, n_kv_heads, head_dim), page_size)
+
+
+def attention_packed(q, k, v, q_lens, n_head, n_kv_heads, head_dim, scale, softcap=None, mode=MASK_CAUSAL, window=-1,
+                     bf16=False):
+    """Masked GQA attention of sequences of q_lens tokens that lie one behind the other: q [tokens, H*D], k and v
+    [tokens, KV*D] fp16 (or bf16 bits with bf16=True); returned in q's type."""
+    q, k, v = np.asarray(q), np.asarray(k), np.asarray(v)
+    dt = _float_dtype(q, bf16, "rocket_attention_packed")
+    plan = packed_plan(q_lens, n_head, n_kv_heads, head_dim, mode, window)
+    try:
+        w, kw = n_head * head_dim, n_kv_heads * head_dim
+        assert q.shape == (plan.n_tokens, w), "q must be [tokens, H*D]"
+        assert k.shape == v.shape == (plan.n_tokens, kw), "k and v must be [tokens, KV*D]"
+        assert k.dtype == v.dtype == q.dtype, "q, k and v must share a type"
+        if plan.n_tokens == 0:
+            return q.copy()
+        return _run_dev("rk_attention_packed_dev", "rocket_attention_packed", q, [q, k, v],
+                        lambda p, o: (plan.ptr, p[0], w, p[1], kw, p[2], kw, float(scale), float(softcap or 0.0), o, w,
+                                      dt, None))
+    finally:
+        plan.destroy()
+
+
+class PagedCache:
+    """K and V of many sequences in pages of device memory, and the calls of a step on them:
+    `append` a fused projection's rows, then `attention`. Which pages a sequence holds is the
+    caller's (the page table that the plan was made with)."""
+
+    def __init__(self, n_pages, page_size, n_kv_heads, head_dim, bf16=False):
+        self.shape, self.bf16 = (n_pages, n_kv_heads, page_size, head_dim), bf16
+        self.dtype = DTYPE_BF16 if bf16 else DTYPE_F16
+        nbytes = 2 * n_pages * n_kv_heads * page_size * head_dim
+        self.k, self.v = DeviceBuffer(nbytes), DeviceBuffer(nbytes)
+
+    def plan(self, q_lens, kv_lens, page_table, n_head, mode=MASK_CAUSAL, window=-1):
+        n_pages, kv, ps, d = self.shape
+        return paged_plan(q_lens, kv_lens, page_table, n_pages, ps, n_head, kv, d, mode, window)
+
+    def _mine(self, plan, a, width, op):
+        if (plan.n_kv_heads, plan.page_size, plan.head_dim) != self.shape[1:]:
+            _shape_error(op, "the plan is of another cache's heads or pages")
+        _float_dtype(a, self.bf16, op)
+        if a.dtype != (np.uint16 if self.bf16 else np.float16) or a.shape != (plan.n_tokens, width):
+            _shape_error(op, f"rows must be [{plan.n_tokens}, {width}] in the cache's type")
+
+    def append(self, plan, qkv, cos, sin, q_norm_w=None, k_norm_w=None, eps=1e-6):
+        """q|k|v rows [tokens, (H + 2 KV)*D] into the cache; returns the rotated q [tokens, H*D]. cos and sin
+        [positions, D/2] and the norm weights [D] in the cache's type (the tables in f32 too)."""
+        qkv, cos, sin = np.asarray(qkv), np.asarray(cos), np.asarray(sin)
+        h, kv, d = plan.n_head, plan.n_kv_heads, plan.head_dim
+        self._mine(plan, qkv, (h + 2 * kv) * d, "rocket_paged_append")
+        ct = DTYPE_F32 if cos.dtype == np.float32 else self.dtype
+        if cos.ndim != 2 or cos.shape[1] != d // 2 or sin.shape != cos.shape or sin.dtype != cos.dtype:
+            _shape_error("rocket_paged_append", "cos and sin must be [positions, D/2]")
+        if ct == self.dtype:
+            _float_dtype(cos, self.bf16, "rocket_paged_append")
+        norms = [] if q_norm_w is None else [np.asarray(q_norm_w), np.asarray(k_norm_w)]
+        if any(w.shape != (d,) or w.dtype != qkv.dtype for w in norms):
+            _shape_error("rocket_paged_append", "the norm weights must be [D] in the cache's type")
+        out = np.empty((plan.n_tokens, h * d), qkv.dtype)
+        if plan.n_tokens == 0:
+            return out
+        return _run_dev("rk_paged_append_dev", "rocket_paged_append", out, [qkv, cos, sin] + norms,
+                        lambda p, o: (plan.ptr, p[0], (h + 2 * kv) * d, *(p[3:5] if norms else (None, None)), float(eps),
+                                      p[1], p[2], ct, cos.shape[0], o, h * d, self.k.ptr, self.v.ptr, self.dtype, None))
+
+    def attention(self, plan, q, scale, softcap=None):
+        """The plan's new tokens q [tokens, H*D] over the cache; returned in q's type."""
+        q, w = np.asarray(q), plan.n_head * plan.head_dim
+        self._mine(plan, q, w, "rocket_attention_paged")
+        if plan.n_tokens == 0:
+            return q.copy()
+        return _run_dev("rk_attention_paged_dev", "rocket_attention_paged", q, [q],
+                        lambda p, o: (plan.ptr, p[0], w, self.k.ptr, self.v.ptr, float(scale), float(softcap or 0.0), o, w,
+                                      self.dtype, None))
 
 
 def moe_route(logits, top_k, norm_topk=True):

@@ -32,6 +32,18 @@ __device__ __forceinline__ void vis_range(int mode, int64_t w, int64_t t, int64_
   }
 }
 
+// The same for a query of a batch of sequences (32-bit positions and windows),
+// clipped to the sequence's keys. Where no row sees a key (a.uniform) every key.
+__device__ __forceinline__ void seq_visible(const SeqAttnArgs &a, int t, int kv_len, int &lo, int &hi) {
+  lo = 0;
+  hi = kv_len - 1;
+  if (a.uniform) return;
+  if (a.mask_mode == RK_MASK_CAUSAL || a.mask_mode == RK_MASK_CAUSAL_WINDOW) hi = min(hi, t);
+  if (a.mask_mode == RK_MASK_WINDOW) hi = min(hi, t + a.window);
+  if (a.mask_mode == RK_MASK_WINDOW) lo = max(0, t - a.window);
+  if (a.mask_mode == RK_MASK_CAUSAL_WINDOW) lo = max(0, t - a.window + 1);
+}
+
 // x - f32(h) for the low / high fp16 half of h in one v_fma_mix_f32 (the f16
 // operand is widened exactly and the difference of a value and its
 // truncation to fp16 is exact in f32), instead of a convert and a subtract.

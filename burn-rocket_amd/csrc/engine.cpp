@@ -21,6 +21,7 @@
 
 #include "../../include/burn_rocket_amd.h"
 #include "kernels.hpp"
+#include "seq_plan.hpp"
 #include "stage.hpp"
 
 static inline int64_t round_up_i(int64_t a, int64_t b) { return (a + b - 1) / b * b; }
@@ -104,6 +105,22 @@ struct Weight {
   int gu_ws_stride = 0, dn_ws_stride = 0;
 };
 
+// A batch of sequences (rk_packed_plan_create, rk_paged_plan_create): the lists
+// the kernels read and the partial states of split rows, in buffers of its own.
+// Both are fenced like scratch: a call on another stream waits for the last one.
+struct SeqPlan {
+  SeqGeom geom;
+  SeqLists lists;        // as last built (the device holds items, merges, toks, table)
+  int64_t n_seqs = 0;
+  DevBuf block, part;
+  size_t off_merges = 0, off_toks = 0, off_table = 0;  // byte offsets in block (items at 0)
+  size_t cap_items = 0, cap_merges = 0, cap_toks = 0, cap_table = 0;
+  uint8_t *pin = nullptr;      // page-locked image of block, made by the first update
+  hipEvent_t pin_ev = nullptr;  // its last upload
+  bool captured = false;       // a graph holds these buffers: they are not replaced
+  int64_t captured_pos = INT64_MAX;  // rows of the shortest cos/sin tables that a captured append reads
+};
+
 struct Engine {
   int device = 0;
   hipStream_t stream = nullptr;
@@ -121,6 +138,7 @@ struct Engine {
   uint8_t *moe_pin = nullptr;
   size_t moe_pin_bytes = 0;
   uint64_t epoch = 0;        // rk_trim_scratch: scratch not used since the last trim goes
+  std::unordered_set<SeqPlan *> seq_plans;
 };
 
 std::mutex g_mu;
@@ -2421,6 +2439,402 @@ extern "C" int rk_attention_qkv_dev(void *qkv, int64_t s, int64_t row_stride, in
   g_eng->calls++;
   return RK_OK;
 }
+// =========================================================================
+// Batches of sequences: packed, or over a paged KV cache
+// =========================================================================
+namespace {
+size_t align16(size_t b) { return (b + 15) / 16 * 16; }
+
+void seq_buf_free(DevBuf &b) {
+  if (b.p) (void)hipFree(b.p);
+  if (b.ev) (void)hipEventDestroy(b.ev);
+  b = DevBuf{};
+}
+
+// The end of a buffer's last use, awaited by the host.
+int seq_buf_wait(DevBuf &b, const char *op) {
+  if (!b.ev) return RK_OK;
+  RK_TRY(fence_point(b, op));
+  if (b.recorded) HIP_TRY(hipEventSynchronize(b.ev), op);
+  b.recorded = false;
+  return RK_OK;
+}
+
+// A plan's buffer in a call: ordered after its last use on another stream, as
+// scratch is. In a capture nothing is awaited or recorded: the order between a
+// graph's replays and other uses of its plan is the caller's.
+int seq_buf_use(CallScope &cs, DevBuf &b, bool capturing, const char *op) {
+  if (capturing || !b.p) return RK_OK;
+  if (!b.ev) HIP_TRY(hipEventCreateWithFlags(&b.ev, hipEventDisableTiming), op);
+  if ((b.recorded || b.pending) && b.ev_stream != cs.st) {
+    RK_TRY(fence_point(b, op));
+    HIP_TRY(hipStreamWaitEvent(cs.st, b.ev, 0), op);
+  }
+  cs.used.push_back(&b);
+  return RK_OK;
+}
+
+int is_capturing(hipStream_t st, bool *yes, const char *op) {
+  hipStreamCaptureStatus s = hipStreamCaptureStatusNone;
+  HIP_TRY(hipStreamIsCapturing(st, &s), op);
+  *yes = s != hipStreamCaptureStatusNone;
+  return RK_OK;
+}
+
+size_t seq_part_bytes(const SeqPlan &p) {
+  return (size_t)p.lists.n_parts * p.geom.n_kv_heads * SEQ_ROWS * (p.geom.head_dim + 2) * 4;
+}
+
+// Writes the plan's lists, padded to its capacities, in the layout of its block.
+void seq_image(const SeqPlan &p, uint8_t *to) {
+  std::memset(to, 0, p.block.bytes);
+  const SeqLists &l = p.lists;
+  if (!l.items.empty()) std::memcpy(to, l.items.data(), l.items.size() * sizeof(SeqItem));
+  if (!l.merges.empty()) std::memcpy(to + p.off_merges, l.merges.data(), l.merges.size() * sizeof(SeqMerge));
+  if (!l.toks.empty()) std::memcpy(to + p.off_toks, l.toks.data(), l.toks.size() * sizeof(SeqTok));
+  SeqTok *toks = (SeqTok *)(to + p.off_toks);
+  for (size_t i = l.toks.size(); i < p.cap_toks; ++i) toks[i].page = -1;  // goes nowhere
+  if (!l.table.empty()) std::memcpy(to + p.off_table, l.table.data(), l.table.size() * 4);
+}
+
+// Buffers that hold the lists (new ones, or the old where they are large enough).
+int seq_reserve(SeqPlan &p, const char *op) {
+  const SeqLists &l = p.lists;
+  const bool fits = p.block.p && l.items.size() <= p.cap_items && l.merges.size() <= p.cap_merges &&
+                    l.toks.size() <= p.cap_toks && l.table.size() <= p.cap_table;
+  if (!fits) {
+    RK_TRY(seq_buf_wait(p.block, op));
+    if (p.block.p) HIP_TRY(hipFree(p.block.p), op);
+    p.block.p = nullptr;
+    if (p.pin) HIP_TRY(hipHostFree(p.pin), op);
+    p.pin = nullptr;
+    p.cap_items = std::max(p.cap_items, l.items.size());
+    p.cap_merges = std::max(p.cap_merges, l.merges.size());
+    p.cap_toks = std::max(p.cap_toks, l.toks.size());
+    p.cap_table = std::max(p.cap_table, l.table.size());
+    p.off_merges = align16(p.cap_items * sizeof(SeqItem));
+    p.off_toks = p.off_merges + align16(p.cap_merges * sizeof(SeqMerge));
+    p.off_table = p.off_toks + align16(p.cap_toks * sizeof(SeqTok));
+    p.block.bytes = std::max<size_t>(p.off_table + align16(p.cap_table * 4), 256);
+    HIP_TRY(hipMalloc(&p.block.p, p.block.bytes), op);
+  }
+  const size_t part = seq_part_bytes(p);
+  if (part > p.part.bytes) {
+    RK_TRY(seq_buf_wait(p.part, op));
+    if (p.part.p) HIP_TRY(hipFree(p.part.p), op);
+    p.part.p = nullptr;
+    p.part.bytes = 0;
+    HIP_TRY(hipMalloc(&p.part.p, part), op);
+    p.part.bytes = part;
+  }
+  return RK_OK;
+}
+
+// The lists grow with the batch: a failed host allocation is a status here.
+template <typename F>
+int no_throw(const char *op, F &&f) {
+  try {
+    return f();
+  } catch (const std::bad_alloc &) {
+    return fail(RK_E_NOMEM, op, "host lists");
+  } catch (const std::exception &e) {
+    return fail(RK_E_NOMEM, op, e.what());
+  }
+}
+
+int seq_plan_create(SeqGeom g, const SeqBatch &b, void **plan, const char *op) {
+  if (!plan) return fail(RK_E_SHAPE, op, "null output");
+  *plan = nullptr;
+  bool unsupported;
+  std::string bad = seq_check_geom(g, &unsupported);
+  if (!bad.empty()) return fail(unsupported ? RK_E_UNSUPPORTED : RK_E_SHAPE, op, bad);
+  bad = seq_check_batch(g, b);
+  if (!bad.empty()) return fail(RK_E_SHAPE, op, bad);
+  std::lock_guard<std::mutex> lk(g_mu);
+  RK_TRY(ensure(op));
+  SeqPlan *p = new SeqPlan;
+  const int rc = no_throw(op, [&]() -> int {
+    p->geom = g;
+    p->n_seqs = b.n_seqs;
+    seq_build(g, b, g_eng->num_cus, &p->lists);
+    RK_TRY(seq_reserve(*p, op));
+    std::vector<uint8_t> image(p->block.bytes);
+    seq_image(*p, image.data());
+    HIP_TRY(hipMemcpy(p->block.p, image.data(), image.size(), hipMemcpyHostToDevice), op);
+    g_eng->seq_plans.insert(p);
+    return RK_OK;
+  });
+  if (rc != RK_OK) {
+    seq_buf_free(p->block);
+    seq_buf_free(p->part);
+    delete p;
+    return rc;
+  }
+  *plan = p;
+  return RK_OK;
+}
+
+// A live plan of the asked kind.
+int seq_plan_get(const void *plan, int paged, SeqPlan **out, const char *op) {
+  SeqPlan *p = (SeqPlan *)plan;
+  if (!p || !g_eng->seq_plans.count(p)) return fail(RK_E_SHAPE, op, "not a plan");
+  if (paged >= 0 && p->geom.paged != (paged == 1))
+    return fail(RK_E_SHAPE, op, p->geom.paged ? "the plan is one of a paged cache" : "the plan is one of packed sequences");
+  *out = p;
+  return RK_OK;
+}
+
+int seq_plan_update(void *plan, bool paged, const SeqBatch &b, rk_stream stream, const char *op) {
+  std::lock_guard<std::mutex> lk(g_mu);
+  RK_TRY(ensure(op));
+  SeqPlan *p;
+  RK_TRY(seq_plan_get(plan, paged, &p, op));
+  const std::string bad = seq_check_batch(p->geom, b);
+  if (!bad.empty()) return fail(RK_E_SHAPE, op, bad);
+  hipStream_t st = pick(stream);
+  bool capturing;
+  RK_TRY(is_capturing(st, &capturing, op));
+  if (capturing) return fail(RK_E_UNSUPPORTED, op, "a plan is not updated inside a capture: its lists come from the host");
+  SeqLists l;
+  seq_build(p->geom, b, g_eng->num_cus, &l);
+  if (p->captured) {
+    SeqPlan probe;
+    probe.geom = p->geom;
+    probe.lists.n_parts = l.n_parts;
+    if (l.items.size() > p->cap_items || l.merges.size() > p->cap_merges || l.toks.size() > p->cap_toks ||
+        l.table.size() > p->cap_table || seq_part_bytes(probe) > p->part.bytes)
+      return fail(RK_E_SHAPE, op, "a graph holds this plan, and the batch needs more than the one it was made for");
+    if (p->captured_pos != INT64_MAX && (l.clash || l.max_pos >= p->captured_pos))
+      return fail(RK_E_SHAPE, op, "a graph's append reads this plan: two new tokens in one slot, or past its cos/sin tables");
+  }
+  if (p->pin_ev) HIP_TRY(hipEventSynchronize(p->pin_ev), op);  // the image's last upload has left it
+  p->lists = std::move(l);
+  p->n_seqs = b.n_seqs;
+  int rc = seq_reserve(*p, op);
+  if (rc == RK_OK && !p->pin) {
+    const hipError_t e = hipHostMalloc((void **)&p->pin, p->block.bytes, hipHostMallocDefault);
+    if (e != hipSuccess) rc = hip_fail(e, op);
+  }
+  if (rc != RK_OK) {  // an empty batch rather than lists that the device does not hold
+    p->lists = SeqLists{};
+    p->n_seqs = 0;
+    return rc;
+  }
+  seq_image(*p, p->pin);
+  CallScope cs(st);
+  RK_TRY(seq_buf_use(cs, p->block, false, op));
+  HIP_TRY(rk_launch_upload(p->pin, p->block.p, p->block.bytes, st), op);
+  if (!p->pin_ev) HIP_TRY(hipEventCreateWithFlags(&p->pin_ev, hipEventDisableTiming), op);
+  HIP_TRY(hipEventRecord(p->pin_ev, st), op);
+  return RK_OK;
+}
+
+int seq_rows_check(const void *p, int64_t stride, int64_t width, const char *what, const char *op) {
+  if (!p) return fail(RK_E_SHAPE, op, std::string("null ") + what);
+  if (stride < width) return fail(RK_E_SHAPE, op, std::string(what) + ": the token stride is shorter than the token's heads");
+  if (stride % 8 != 0 || ((uintptr_t)p & 15) != 0)
+    return fail(RK_E_SHAPE, op, std::string(what) + ": needs a token stride of a multiple of 8 values and a 16-byte aligned buffer");
+  return RK_OK;
+}
+
+int seq_attention(const void *plan, bool paged, const void *q, int64_t q_stride, const void *k, int64_t k_stride,
+                  const void *v, int64_t v_stride, float scale, float softcap, void *out, int64_t out_stride,
+                  int dtype, rk_stream stream, const char *op) {
+  std::lock_guard<std::mutex> lk(g_mu);
+  RK_TRY(ensure(op));
+  SeqPlan *p;
+  RK_TRY(seq_plan_get(plan, paged, &p, op));
+  const SeqGeom &g = p->geom;
+  if (dtype != RK_DTYPE_F16 && dtype != RK_DTYPE_BF16) return fail(RK_E_UNSUPPORTED, op, "dtype must be fp16 or bf16");
+  hipStream_t st = pick(stream);
+  bool capturing;
+  RK_TRY(is_capturing(st, &capturing, op));
+  if (p->lists.n_tokens == 0 && !capturing) return RK_OK;
+  const int64_t qw = (int64_t)g.n_head * g.head_dim, kw = (int64_t)g.n_kv_heads * g.head_dim;
+  RK_TRY(seq_rows_check(q, q_stride, qw, "q", op));
+  RK_TRY(seq_rows_check(out, out_stride, qw, "out", op));
+  RK_TRY(seq_rows_check(k, paged ? kw : k_stride, kw, paged ? "k_cache" : "k", op));
+  RK_TRY(seq_rows_check(v, paged ? kw : v_stride, kw, paged ? "v_cache" : "v", op));
+  CallScope cs(st);
+  RK_TRY(seq_buf_use(cs, p->block, capturing, op));
+  RK_TRY(seq_buf_use(cs, p->part, capturing, op));
+  SeqAttnArgs a{};
+  const uint8_t *block = (const uint8_t *)p->block.p;
+  a.q = q;
+  a.k = k;
+  a.v = v;
+  a.out = out;
+  a.q_stride = q_stride;
+  a.k_stride = k_stride;
+  a.v_stride = v_stride;
+  a.out_stride = out_stride;
+  a.items = (const SeqItem *)block;
+  a.table = (const int32_t *)(block + p->off_table);
+  a.part = (float *)p->part.p;
+  a.n_head = g.n_head;
+  a.n_kv_heads = g.n_kv_heads;
+  a.head_dim = g.head_dim;
+  while (paged && (1 << a.page_log2) < g.page_size) ++a.page_log2;
+  a.scale = scale;
+  a.softcap = softcap;
+  a.mask_mode = g.mask_mode;
+  a.window = (int)g.window;
+  a.uniform = g.uniform;
+  // A captured launch has a workgroup for every item that an update may list.
+  const size_t n = capturing ? p->cap_items : p->lists.items.size();
+  if (n == 0) return RK_OK;
+  if (capturing) p->captured = true;
+  HIP_TRY(rk_launch_attention_seqs(a, (int)n, paged, dtype, st), op);
+  g_eng->calls++;
+  return RK_OK;
+}
+}  // namespace
+
+extern "C" int rk_packed_plan_create(const int32_t *q_lens, int64_t n_seqs, int n_head, int n_kv_heads, int head_dim,
+                                     int mask_mode, int64_t window, void **plan) {
+  SeqGeom g;
+  g.n_head = n_head;
+  g.n_kv_heads = n_kv_heads;
+  g.head_dim = head_dim;
+  g.mask_mode = mask_mode;
+  g.window = window;
+  SeqBatch b;
+  b.q_lens = q_lens;
+  b.n_seqs = n_seqs;
+  return no_throw("rk_packed_plan_create", [&] {
+    return seq_plan_create(g, b, plan, "rk_packed_plan_create");
+  });
+}
+extern "C" int rk_paged_plan_create(const int32_t *q_lens, const int32_t *kv_lens, const int32_t *page_table,
+                                    int64_t table_stride, int64_t n_seqs, int64_t n_pages, int page_size, int n_head,
+                                    int n_kv_heads, int head_dim, int mask_mode, int64_t window, void **plan) {
+  SeqGeom g;
+  g.paged = true;
+  g.n_head = n_head;
+  g.n_kv_heads = n_kv_heads;
+  g.head_dim = head_dim;
+  g.mask_mode = mask_mode;
+  g.window = window;
+  g.n_pages = n_pages;
+  g.page_size = page_size;
+  return no_throw("rk_paged_plan_create", [&] {
+    return seq_plan_create(g, SeqBatch{q_lens, kv_lens, page_table, table_stride, n_seqs}, plan, "rk_paged_plan_create");
+  });
+}
+extern "C" int rk_packed_plan_update(void *plan, const int32_t *q_lens, int64_t n_seqs, rk_stream stream) {
+  SeqBatch b;
+  b.q_lens = q_lens;
+  b.n_seqs = n_seqs;
+  return no_throw("rk_packed_plan_update", [&] {
+    return seq_plan_update(plan, false, b, stream, "rk_packed_plan_update");
+  });
+}
+extern "C" int rk_paged_plan_update(void *plan, const int32_t *q_lens, const int32_t *kv_lens,
+                                    const int32_t *page_table, int64_t table_stride, int64_t n_seqs, rk_stream stream) {
+  return no_throw("rk_paged_plan_update", [&] {
+    return seq_plan_update(plan, true, SeqBatch{q_lens, kv_lens, page_table, table_stride, n_seqs}, stream,
+                         "rk_paged_plan_update");
+  });
+}
+extern "C" int rk_seq_plan_destroy(void *plan) {
+  const char *op = "rk_seq_plan_destroy";
+  std::lock_guard<std::mutex> lk(g_mu);
+  RK_TRY(ensure(op));
+  if (!plan) return RK_OK;
+  SeqPlan *p;
+  RK_TRY(seq_plan_get(plan, -1, &p, op));
+  // Calls and uploads that read its buffers end first; replays of a graph that
+  // holds them are known to the device alone.
+  if (p->captured) HIP_TRY(hipDeviceSynchronize(), op);
+  RK_TRY(seq_buf_wait(p->block, op));
+  RK_TRY(seq_buf_wait(p->part, op));
+  if (p->pin_ev) {
+    HIP_TRY(hipEventSynchronize(p->pin_ev), op);
+    (void)hipEventDestroy(p->pin_ev);
+  }
+  if (p->pin) (void)hipHostFree(p->pin);
+  seq_buf_free(p->block);
+  seq_buf_free(p->part);
+  g_eng->seq_plans.erase(p);
+  delete p;
+  return RK_OK;
+}
+extern "C" int rk_attention_packed_dev(const void *plan, const void *q, int64_t q_stride, const void *k,
+                                       int64_t k_stride, const void *v, int64_t v_stride, float scale, float softcap,
+                                       void *out, int64_t out_stride, int dtype, rk_stream stream) {
+  return seq_attention(plan, false, q, q_stride, k, k_stride, v, v_stride, scale, softcap, out, out_stride, dtype,
+                       stream, "rk_attention_packed_dev");
+}
+extern "C" int rk_attention_paged_dev(const void *plan, const void *q, int64_t q_stride, const void *k_cache,
+                                      const void *v_cache, float scale, float softcap, void *out, int64_t out_stride,
+                                      int dtype, rk_stream stream) {
+  return seq_attention(plan, true, q, q_stride, k_cache, 0, v_cache, 0, scale, softcap, out, out_stride, dtype, stream,
+                       "rk_attention_paged_dev");
+}
+extern "C" int rk_paged_append_dev(const void *plan, const void *qkv, int64_t row_stride, const void *q_norm_w,
+                                   const void *k_norm_w, double eps, const void *cos, const void *sin, int cs_dtype,
+                                   int64_t n_pos, void *q_out, int64_t q_out_stride, void *k_cache, void *v_cache,
+                                   int dtype, rk_stream stream) {
+  const char *op = "rk_paged_append_dev";
+  std::lock_guard<std::mutex> lk(g_mu);
+  RK_TRY(ensure(op));
+  SeqPlan *p;
+  RK_TRY(seq_plan_get(plan, 1, &p, op));
+  const SeqGeom &g = p->geom;
+  if (dtype != RK_DTYPE_F16 && dtype != RK_DTYPE_BF16) return fail(RK_E_UNSUPPORTED, op, "dtype must be fp16 or bf16");
+  if (cs_dtype != dtype && cs_dtype != RK_DTYPE_F32)
+    return fail(RK_E_UNSUPPORTED, op, "cos/sin must have the element type of qkv or be f32");
+  if ((q_norm_w == nullptr) != (k_norm_w == nullptr)) return fail(RK_E_SHAPE, op, "give both norm weights or neither");
+  hipStream_t st = pick(stream);
+  bool capturing;
+  RK_TRY(is_capturing(st, &capturing, op));
+  if (p->lists.n_tokens == 0 && !capturing) return RK_OK;
+  const int heads = g.n_head + 2 * g.n_kv_heads;
+  RK_TRY(seq_rows_check(qkv, row_stride, (int64_t)heads * g.head_dim, "qkv", op));
+  RK_TRY(seq_rows_check(q_out, q_out_stride, (int64_t)g.n_head * g.head_dim, "q_out", op));
+  if (q_out == qkv && q_out_stride != row_stride)
+    return fail(RK_E_SHAPE, op, "q_out on qkv itself needs the same token stride");
+  for (const void *b : {(const void *)k_cache, (const void *)v_cache, cos, sin})
+    if (!b || ((uintptr_t)b & 15) != 0) return fail(RK_E_SHAPE, op, "k_cache, v_cache, cos and sin must be 16-byte aligned buffers");
+  if ((((uintptr_t)q_norm_w | (uintptr_t)k_norm_w) & 15) != 0) return fail(RK_E_SHAPE, op, "norm weights must be 16-byte aligned");
+  if (p->lists.max_pos >= n_pos)
+    return fail(RK_E_SHAPE, op, "the tables have " + std::to_string(n_pos) + " rows, the last new token is at " +
+                                    std::to_string(p->lists.max_pos));
+  if (p->lists.clash) return fail(RK_E_SHAPE, op, "two new tokens of the batch go to one slot of a page");
+  const int64_t n = capturing ? (int64_t)p->cap_toks : p->lists.n_tokens;
+  if (n * heads > INT32_MAX) return fail(RK_E_SHAPE, op, "2^31 or more head rows");
+  CallScope cs(st);
+  RK_TRY(seq_buf_use(cs, p->block, capturing, op));
+  PagedAppendArgs a{};
+  a.qkv = qkv;
+  a.row_stride = row_stride;
+  a.q_norm_w = q_norm_w;
+  a.k_norm_w = k_norm_w;
+  a.eps = (float)eps;
+  a.cos = cos;
+  a.sin = sin;
+  a.q_out = q_out;
+  a.q_out_stride = q_out_stride;
+  a.k_cache = k_cache;
+  a.v_cache = v_cache;
+  a.toks = (const SeqTok *)((const uint8_t *)p->block.p + p->off_toks);
+  a.n_tokens = (int)n;
+  a.n_head = g.n_head;
+  a.n_kv_heads = g.n_kv_heads;
+  a.head_dim = g.head_dim;
+  while ((1 << a.page_log2) < g.page_size) ++a.page_log2;
+  if (n == 0) return RK_OK;
+  if (capturing) {
+    p->captured = true;
+    p->captured_pos = std::min(p->captured_pos, n_pos);
+  }
+  HIP_TRY(rk_launch_paged_append(a, dtype, cs_dtype, st), op);
+  return RK_OK;
+}
+
+// =========================================================================
+// RMSNorm with the int8 quantizer, host forms of the norms and RoPE
+// =========================================================================
 extern "C" int rk_rms_norm_quantize_dev(const void *x, const void *w, int w_dtype, int64_t rows,
                                         int64_t d, double eps, int dtype, int8_t *q,
                                         float *q_scale, rk_stream stream) {
@@ -2526,6 +2940,9 @@ extern "C" int rk_stream_destroy(rk_stream stream) {
   HIP_TRY(hipStreamSynchronize(st), "rk_stream_destroy");
   for (auto &kv : g_eng->scratch)
     if (kv.second.ev_stream == st) kv.second.pending = kv.second.recorded = false;
+  for (SeqPlan *p : g_eng->seq_plans)
+    for (DevBuf *b : {&p->block, &p->part})
+      if (b->ev_stream == st) b->pending = b->recorded = false;
   HIP_TRY(hipStreamDestroy(st), "rk_stream_destroy");
   g_eng->own_streams.erase(st);
   return RK_OK;

@@ -5,6 +5,8 @@
 #include <stdint.h>
 #include <stdlib.h>
 
+#include "seq_plan.hpp"
+
 // Integer tuning knob from the environment (read at every call, like the
 // reference's ROCKET_* knobs); `dflt` when unset or not a number.
 static inline int rk_knob(const char *name, int dflt) {
@@ -209,6 +211,34 @@ bool rk_attn_rows_fits(const AttnArgs &a, const void *v, int64_t v_tok_stride);
 void rk_attn_rows_workspace(const AttnArgs &a, size_t *part_bytes, size_t *n_cnt);
 hipError_t rk_launch_attention_rows(const AttnArgs &a, const void *v, int64_t v_tok_stride, int64_t v_head_stride,
                                     hipStream_t st);
+
+// Batches of sequences (seq_plan.hpp). The lists are in device memory.
+struct SeqAttnArgs {
+  const void *q, *k, *v;  // k, v: packed rows, or the cache [page][kv head][page_size][head_dim]
+  void *out;
+  int64_t q_stride, k_stride, v_stride, out_stride;  // values between tokens (k, v: packed only)
+  const SeqItem *items;
+  const int32_t *table;  // page ids (paged)
+  float *part;           // partial softmax states
+  int n_head, n_kv_heads, head_dim, page_log2;
+  float scale, softcap;
+  int mask_mode, window, uniform;
+};
+hipError_t rk_launch_attention_seqs(const SeqAttnArgs &a, int n_items, bool paged, int dtype, hipStream_t st);
+
+struct PagedAppendArgs {
+  const void *qkv;  // [n_tokens] rows: q heads, k heads, v heads
+  int64_t row_stride;
+  const void *q_norm_w, *k_norm_w;  // both null: no norm
+  float eps;
+  const void *cos, *sin;
+  void *q_out;
+  int64_t q_out_stride;
+  void *k_cache, *v_cache;
+  const SeqTok *toks;
+  int n_tokens, n_head, n_kv_heads, head_dim, page_log2;
+};
+hipError_t rk_launch_paged_append(const PagedAppendArgs &a, int dtype, int cs_dtype, hipStream_t st);
 
 // MoE helpers.
 struct MoeTile {

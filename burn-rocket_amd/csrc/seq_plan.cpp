@@ -1,0 +1,132 @@
+// Host side of the batches of sequences (seq_plan.hpp): checks and schedules.
+#include "seq_plan.hpp"
+
+#include <algorithm>
+#include <numeric>
+
+#include "../../include/burn_rocket_amd.h"
+
+namespace {
+constexpr int64_t MAX_KEYS = (int64_t)1 << 30;  // positions and windows stay inside 32 bits
+
+int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+// First and last key that the query at position t sees, clipped to the sequence.
+void visible(const SeqGeom &g, int64_t t, int64_t kv_len, int64_t *lo, int64_t *hi) {
+  *lo = 0;
+  *hi = kv_len - 1;
+  if (g.uniform) return;
+  if (g.mask_mode == RK_MASK_CAUSAL || g.mask_mode == RK_MASK_CAUSAL_WINDOW) *hi = std::min(*hi, t);
+  if (g.mask_mode == RK_MASK_WINDOW) *hi = std::min(*hi, t + g.window);
+  if (g.mask_mode == RK_MASK_WINDOW) *lo = std::max<int64_t>(0, t - g.window);
+  if (g.mask_mode == RK_MASK_CAUSAL_WINDOW) *lo = std::max<int64_t>(0, t - g.window + 1);
+}
+
+int64_t kv_of(const SeqBatch &b, int64_t i) { return b.kv_lens ? b.kv_lens[i] : b.q_lens[i]; }
+}  // namespace
+
+std::string seq_check_geom(SeqGeom &g, bool *unsupported) {
+  *unsupported = false;
+  if (g.n_head <= 0 || g.n_kv_heads <= 0 || g.n_head % g.n_kv_heads != 0)
+    return "n_head must be a positive multiple of n_kv_heads";
+  if (g.n_head / g.n_kv_heads > 128) return "GQA group above 128";
+  switch (g.head_dim) {
+    case 32: case 48: case 64: case 72: case 80: case 96: case 112: case 128: case 256: break;
+    default:
+      *unsupported = true;
+      return "head_dim " + std::to_string(g.head_dim) + " (supported: 32, 48, 64, 72, 80, 96, 112, 128, 256)";
+  }
+  if (g.mask_mode < RK_MASK_NONE || g.mask_mode > RK_MASK_CAUSAL_WINDOW) return "unknown mask mode";
+  // window < 0 disables the window (ext.rs:99-126).
+  if (g.mask_mode == RK_MASK_WINDOW && g.window < 0) g.mask_mode = RK_MASK_NONE;
+  if (g.mask_mode == RK_MASK_CAUSAL_WINDOW && g.window < 0) g.mask_mode = RK_MASK_CAUSAL;
+  g.window = std::min(g.window, MAX_KEYS);
+  g.uniform = g.mask_mode == RK_MASK_CAUSAL_WINDOW && g.window == 0;
+  if (g.paged) {
+    if (g.page_size < 16 || g.page_size > 256 || (g.page_size & (g.page_size - 1)))
+      return "page_size must be 16, 32, 64, 128 or 256";
+    if (g.n_pages <= 0 || g.n_pages > INT32_MAX) return "n_pages must be in [1, 2^31)";
+  }
+  return "";
+}
+
+std::string seq_check_batch(const SeqGeom &g, const SeqBatch &b) {
+  if (b.n_seqs < 0 || b.n_seqs > INT32_MAX) return "n_seqs must be in [0, 2^31)";
+  if (b.n_seqs == 0) return "";
+  if (!b.q_lens || (g.paged && (!b.kv_lens || !b.page_table))) return "null list";
+  const int64_t G = g.n_head / g.n_kv_heads;
+  int64_t toks = 0, ids = 0;
+  for (int64_t i = 0; i < b.n_seqs; ++i) {
+    const std::string at = "sequence " + std::to_string(i) + ": ";
+    const int64_t q = b.q_lens[i], kv = kv_of(b, i);
+    if (q < 0 || kv < q) return at + "needs 0 <= q_len <= kv_len";
+    if (kv > MAX_KEYS) return at + "more than 2^30 keys";
+    if (q * G > INT32_MAX) return at + "q_len·(n_head/n_kv_heads) of 2^31 or more";
+    toks += q;
+    if (toks > INT32_MAX) return "2^31 or more new tokens";
+    if (!g.paged || q == 0) continue;
+    const int64_t pages = ceil_div(kv, g.page_size);
+    if (pages > b.table_stride) return at + "its keys need more pages than a table row holds";
+    ids += pages;
+    if (ids > INT32_MAX) return "2^31 or more page ids";
+    int64_t lo, hi;
+    visible(g, kv - q, kv, &lo, &hi);
+    for (int64_t p = lo / g.page_size; p < pages; ++p) {
+      const int32_t id = b.page_table[i * b.table_stride + p];
+      if (id < 0 || id >= g.n_pages)
+        return at + "page " + std::to_string(p) + " has id " + std::to_string(id) + " of " + std::to_string(g.n_pages);
+    }
+  }
+  // items and merges are counted with 32 bits, a launch's workgroups too
+  if ((toks * G / 16 + b.n_seqs + 4096) * g.n_kv_heads > INT32_MAX) return "2^31 or more row tiles";
+  return "";
+}
+
+void seq_build(const SeqGeom &g, const SeqBatch &b, int num_cus, SeqLists *out) {
+  (void)num_cus;
+  *out = SeqLists{};
+  const int64_t G = g.n_head / g.n_kv_heads;
+  struct Piece {
+    int32_t page, off, end;
+  };
+  std::vector<Piece> pieces;  // where new tokens go: slots [off, end) of a page
+  for (int64_t i = 0; i < b.n_seqs; ++i) {
+    const int64_t q = b.q_lens[i], kv = kv_of(b, i), pos0 = kv - q;
+    if (q == 0) continue;
+    SeqItem it{};
+    it.tok0 = (int32_t)out->n_tokens;
+    it.pos0 = (int32_t)pos0;
+    it.rows = (int32_t)(q * G);
+    it.kv_len = (int32_t)kv;
+    it.table = (int32_t)out->table.size();
+    it.part = -1;
+    for (int64_t r = 0; r < q * G; r += SEQ_ROWS) {
+      int64_t lo, hi, lo2, hi2;
+      visible(g, pos0 + r / G, kv, &lo, &hi);
+      visible(g, pos0 + (std::min(r + SEQ_ROWS, q * G) - 1) / G, kv, &lo2, &hi2);
+      it.row0 = (int32_t)r;
+      it.k_lo = (int32_t)lo;
+      it.k_begin = (int32_t)(lo / SEQ_KEY_TILE * SEQ_KEY_TILE);
+      it.k_end = (int32_t)(hi2 + 1);
+      out->items.push_back(it);
+    }
+    out->n_tokens += q;
+    out->max_pos = std::max(out->max_pos, kv - 1);
+    if (!g.paged) continue;
+    int64_t lo, hi;
+    visible(g, pos0, kv, &lo, &hi);
+    const int32_t *row = b.page_table + i * b.table_stride;
+    const int64_t ps = g.page_size;
+    for (int64_t p = 0; p < ceil_div(kv, ps); ++p) out->table.push_back(p < lo / ps ? 0 : row[p]);
+    for (int64_t t = pos0; t < kv; ++t) out->toks.push_back(SeqTok{row[t / ps], (int32_t)t});
+    for (int64_t t = pos0; t < kv;) {
+      const int64_t e = std::min(kv, (t / ps + 1) * ps);
+      pieces.push_back(Piece{row[t / ps], (int32_t)(t % ps), (int32_t)((e - 1) % ps + 1)});
+      t = e;
+    }
+  }
+  std::sort(pieces.begin(), pieces.end(),
+            [](const Piece &x, const Piece &y) { return x.page != y.page ? x.page < y.page : x.off < y.off; });
+  for (size_t i = 1; i < pieces.size(); ++i)
+    out->clash |= pieces[i].page == pieces[i - 1].page && pieces[i].off < pieces[i - 1].end;
+}

@@ -1,0 +1,79 @@
+// Batches of sequences: the lists that the kernels on packed sequences and on a
+// paged KV cache read, made and checked on the host.
+//
+// A sequence of a batch has q_len new tokens, the last of its kv_len keys (packed
+// sequences: all of them). Its query rows are the pairs r = q·G + g of new token
+// q and head g of a kv head's group of G: consecutive rows are the heads that
+// read the same keys, so any group size fills a tile of rows without gaps. An
+// item is a tile of rows of one sequence with a range of its keys; each runs once
+// for every kv head. A tile whose keys are split between several items has as
+// many partial softmax states, which a merge joins in ascending key order.
+#pragma once
+
+#include <stdint.h>
+
+#include <string>
+#include <vector>
+
+struct SeqItem {
+  int32_t tok0;     // row of the sequence's first new token in q and out (packed: in k and v too)
+  int32_t pos0;     // key index of that token
+  int32_t rows;     // query rows of the sequence, q_len·G; 0: the item is empty
+  int32_t row0;     // first row of the tile
+  int32_t kv_len;   // keys of the sequence
+  int32_t k_begin;  // the item's keys [k_begin, k_end); k_begin is a multiple of SEQ_KEY_TILE
+  int32_t k_end;
+  int32_t k_lo;     // lowest key that a row of the tile sees: blocks of 16 keys below it are not read
+  int32_t table;    // paged: where the sequence's page ids start in the table list
+  int32_t part;     // >= 0: slot of its partial state (the slot of kv head g is part·n_kv_heads + g)
+  int32_t pad[2];
+};
+
+// A row tile whose states are joined: slots part0 .. part0 + n_parts - 1.
+struct SeqMerge {
+  int32_t tok0, rows, row0, part0, n_parts;
+  int32_t pad[3];
+};
+
+// Where a new token goes: its page and its key index.
+struct SeqTok {
+  int32_t page, pos;
+};
+
+constexpr int SEQ_ROWS = 128;     // query rows of a tile
+constexpr int SEQ_KEY_TILE = 64;  // keys of the kernels' steps; ranges start at multiples of it
+
+struct SeqGeom {
+  bool paged = false;
+  int n_head = 0, n_kv_heads = 0, head_dim = 0;
+  int mask_mode = 0;
+  int64_t window = -1;
+  int64_t n_pages = 0;
+  int page_size = 0;
+  bool uniform = false;  // no row sees a key (a causal window of 0): every row averages V
+};
+
+struct SeqBatch {
+  const int32_t *q_lens = nullptr, *kv_lens = nullptr;
+  const int32_t *page_table = nullptr;
+  int64_t table_stride = 0, n_seqs = 0;
+};
+
+struct SeqLists {
+  int64_t n_tokens = 0;
+  int64_t max_pos = -1;   // largest key index of a new token
+  bool clash = false;     // two new tokens go to one slot of a page
+  int n_parts = 0;        // partial states (per kv head)
+  std::vector<SeqItem> items;
+  std::vector<SeqMerge> merges;
+  std::vector<SeqTok> toks;
+  std::vector<int32_t> table;
+};
+
+// Checks without a device: "" or what is wrong. seq_check_geom also resolves
+// negative windows (mask_mode) and `uniform`; *unsupported: the head dim is one
+// that the kernels do not have.
+std::string seq_check_geom(SeqGeom &g, bool *unsupported);
+std::string seq_check_batch(const SeqGeom &g, const SeqBatch &b);
+// The lists of a checked batch for a GPU of num_cus CUs.
+void seq_build(const SeqGeom &g, const SeqBatch &b, int num_cus, SeqLists *out);

@@ -162,6 +162,39 @@ unsafe extern "C" {
         scale: f32, softcap: f32, mask: *const u16, q: *const u16, k: *const u16, v: *const u16,
         out: *mut u16
     ) -> c_int;
+    pub fn rk_packed_plan_create(
+        q_lens: *const i32, n_seqs: i64, n_head: c_int, n_kv_heads: c_int, head_dim: c_int,
+        mask_mode: c_int, window: i64, plan: *mut *mut c_void
+    ) -> c_int;
+    pub fn rk_paged_plan_create(
+        q_lens: *const i32, kv_lens: *const i32, page_table: *const i32, table_stride: i64,
+        n_seqs: i64, n_pages: i64, page_size: c_int, n_head: c_int, n_kv_heads: c_int,
+        head_dim: c_int, mask_mode: c_int, window: i64, plan: *mut *mut c_void
+    ) -> c_int;
+    pub fn rk_packed_plan_update(
+        plan: *mut c_void, q_lens: *const i32, n_seqs: i64, stream: Stream
+    ) -> c_int;
+    pub fn rk_paged_plan_update(
+        plan: *mut c_void, q_lens: *const i32, kv_lens: *const i32, page_table: *const i32,
+        table_stride: i64, n_seqs: i64, stream: Stream
+    ) -> c_int;
+    pub fn rk_seq_plan_destroy(plan: *mut c_void) -> c_int;
+    pub fn rk_attention_packed_dev(
+        plan: *const c_void, q: *const c_void, q_stride: i64, k: *const c_void, k_stride: i64,
+        v: *const c_void, v_stride: i64, scale: f32, softcap: f32, out: *mut c_void,
+        out_stride: i64, dtype: c_int, stream: Stream
+    ) -> c_int;
+    pub fn rk_attention_paged_dev(
+        plan: *const c_void, q: *const c_void, q_stride: i64, k_cache: *const c_void,
+        v_cache: *const c_void, scale: f32, softcap: f32, out: *mut c_void, out_stride: i64,
+        dtype: c_int, stream: Stream
+    ) -> c_int;
+    pub fn rk_paged_append_dev(
+        plan: *const c_void, qkv: *const c_void, row_stride: i64, q_norm_w: *const c_void,
+        k_norm_w: *const c_void, eps: f64, cos: *const c_void, sin: *const c_void,
+        cs_dtype: c_int, n_pos: i64, q_out: *mut c_void, q_out_stride: i64,
+        k_cache: *mut c_void, v_cache: *mut c_void, dtype: c_int, stream: Stream
+    ) -> c_int;
     pub fn rk_moe_route(
         logits: *const f32, s: i64, n_experts: c_int, top_k: c_int, norm_topk: c_int,
         ids: *mut u32, wts: *mut f32

@@ -402,6 +402,89 @@ int rk_flash_attn_f16_masked(int64_t n_q, int64_t n_kv, int head_dim, int dv, in
                              const uint16_t *q, const uint16_t *k, const uint16_t *v, uint16_t *out);
 
 /* ======================================================================== *
+ * Batches of sequences: packed, and over a paged KV cache                   *
+ * ======================================================================== */
+
+/* No counterpart in the reference, whose attention takes one sequence a call
+ * (batch 1, ext.rs:1680-1710) with its keys in one piece. A plan holds what a
+ * batch of sequences looks like and how its work is shared out; it is made on
+ * the host from the scheduler's lists, checked there, and serves all layers of a
+ * step that have its heads and mask.
+ *
+ * Sequence b has q_lens[b] new tokens, the last of its kv_lens[b] keys: token i
+ * is at key index t = kv_lens[b] - q_lens[b] + i. The new tokens of all sequences
+ * lie one behind the other, in order, in q, out and q|k|v rows; q_lens[b] = 0 is
+ * a sequence without work. Rows past the last sequence are neither read nor
+ * written. Packed sequences are their new tokens alone (kv_lens = q_lens).
+ *
+ * The cache: k_cache, v_cache [n_pages][n_kv_heads][page_size][head_dim], page
+ * size 16, 32, 64, 128 or 256. Key j of sequence b is row j % page_size of page
+ * page_table[b·table_stride + j / page_size]. Sequences may share pages that
+ * they only read. Entries past a sequence's last key, or before the first key
+ * that any of its tokens sees (windows), are not looked at; every other one has
+ * to be in [0, n_pages) or the plan is refused (RK_E_SHAPE). Slots of a page
+ * past a sequence's last key may hold anything.
+ *
+ * Masks are those of rk_attention_dev with query position t and key position
+ * j. A causal window of 0 leaves no key visible: such rows average V over the
+ * sequence's keys, as there.
+ *
+ * The lists are copied: the caller's arrays may go when a call returns. An
+ * update gives the plan another batch of the same heads, mask and pages; it is
+ * ordered on `stream` after the calls that used the plan, waits on the host for
+ * the upload of the update before it, and is refused inside a stream capture.
+ *
+ * Streams: calls on one plan from different streams run one after another. Under
+ * a stream capture nothing is allocated and launches have room for every batch
+ * of an update that needs no more tokens, sequences and pages than the plan was
+ * made with; larger updates are then refused (RK_E_SHAPE). The buffers of a
+ * captured call must have room for as many tokens as the plan was made with.
+ * The caller orders the replays of graphs that share a plan, and other calls
+ * and updates of a captured plan, after one another. A plan is destroyed after its
+ * graphs. */
+int rk_packed_plan_create(const int32_t *q_lens, int64_t n_seqs, int n_head, int n_kv_heads, int head_dim,
+                          int mask_mode, int64_t window, void **plan);
+int rk_paged_plan_create(const int32_t *q_lens, const int32_t *kv_lens, const int32_t *page_table,
+                         int64_t table_stride, int64_t n_seqs, int64_t n_pages, int page_size, int n_head,
+                         int n_kv_heads, int head_dim, int mask_mode, int64_t window, void **plan);
+int rk_packed_plan_update(void *plan, const int32_t *q_lens, int64_t n_seqs, rk_stream stream);
+int rk_paged_plan_update(void *plan, const int32_t *q_lens, const int32_t *kv_lens,
+                         const int32_t *page_table, int64_t table_stride, int64_t n_seqs, rk_stream stream);
+int rk_seq_plan_destroy(void *plan);
+
+/* Attention of every sequence of a packed batch over its own tokens: q [tokens]
+ * rows of n_head·head_dim values q_stride apart, k and v likewise with n_kv_heads
+ * heads (column ranges of one q|k|v row, for instance), out as q. dtype fp16 or
+ * bf16 (RK_DTYPE_*), strides multiples of 8 values, buffers 16-byte aligned, head
+ * dims as rk_attention_dev without the padded ones. Scores and softmax in f32,
+ * probabilities rounded to nearest in dtype for the product with V, sums in f32,
+ * one rounding at the end. The split of a row's keys between workgroups depends on
+ * the whole batch: a sequence's result can differ in rounding between batches,
+ * equal batches give equal bits. A non-finite value of V reaches every row of its
+ * sequence that is computed in a tile with a row that sees it. */
+int rk_attention_packed_dev(const void *plan, const void *q, int64_t q_stride, const void *k, int64_t k_stride,
+                            const void *v, int64_t v_stride, float scale, float softcap, void *out,
+                            int64_t out_stride, int dtype, rk_stream stream);
+/* The new tokens of a paged batch (one a sequence, chunks, or both) over the
+ * cache, which already holds their own keys; otherwise as the packed form. */
+int rk_attention_paged_dev(const void *plan, const void *q, int64_t q_stride, const void *k_cache,
+                           const void *v_cache, float scale, float softcap, void *out, int64_t out_stride,
+                           int dtype, rk_stream stream);
+/* The prologue in front of it, on a fused q|k|v projection of the new tokens
+ * (rows row_stride apart: q heads, k heads, v heads): RMSNorm over head_dim with
+ * q_norm_w / k_norm_w [head_dim] (both NULL: none), then rotate-half RoPE with
+ * row t of cos/sin [n_pos, head_dim/2] for the token at key index t, q to q_out
+ * rows, k and v to the tokens' slots of the cache. All in f32, rounded once at the
+ * store (rk_qk_norm_rope_dev rounds the norm's result too). q_out may be qkv with
+ * the same stride (q in place). dtype fp16 or bf16, the norm weights too; cos/sin
+ * of dtype or f32. RK_E_SHAPE when n_pos rows do not reach the last token, or two
+ * new tokens of the batch go to one slot of a page. */
+int rk_paged_append_dev(const void *plan, const void *qkv, int64_t row_stride, const void *q_norm_w,
+                        const void *k_norm_w, double eps, const void *cos, const void *sin, int cs_dtype,
+                        int64_t n_pos, void *q_out, int64_t q_out_stride, void *k_cache, void *v_cache,
+                        int dtype, rk_stream stream);
+
+/* ======================================================================== *
  * MoE experts                                                               *
  * ======================================================================== */
 
