@@ -73,6 +73,7 @@ SIGNATURES = {
     "rk_paged_plan_create": (_i, [_p, _p, _p, _i64, _i64, _i64, _i, _i, _i, _i, _i, _i64, _p]),
     "rk_packed_plan_update": (_i, [_p, _p, _i64, _p]),
     "rk_paged_plan_update": (_i, [_p, _p, _p, _p, _i64, _i64, _p]),
+    "rk_seq_plan_reserve": (_i, [_p, _i64]),
     "rk_seq_plan_destroy": (_i, [_p]),
     "rk_attention_packed_dev": (_i, [_p, _p, _i64, _p, _i64, _p, _i64, _f, _f, _p, _i64, _i, _p]),
     "rk_attention_paged_dev": (_i, [_p, _p, _i64, _p, _p, _f, _f, _p, _i64, _i, _p]),
@@ -544,6 +545,10 @@ class SeqPlan:
             _check(_lib.rk_paged_plan_update(self.ptr, _ptr(q), _ptr(kv), _ptr(table), table.shape[1], q.size, st),
                    "paged_plan_update")
         self.n_tokens = int(q.sum(dtype=np.int64))
+
+    def reserve(self, max_q_len=0):
+        """Room for every batch of no more sequences, tokens and pages than this one, for a graph capture."""
+        _check(_lib.rk_seq_plan_reserve(self.ptr, max_q_len), "seq_plan_reserve")
 
     def destroy(self):
         if self.ptr:

@@ -106,18 +106,31 @@ struct Weight {
 };
 
 // A batch of sequences (rk_packed_plan_create, rk_paged_plan_create): the lists
-// the kernels read and the partial states of split rows, in buffers of its own.
-// Both are fenced like scratch: a call on another stream waits for the last one.
+// the kernels read (one block of device memory) and the workspace of split rows
+// (arrival counts, which start at zero and which every launch leaves at zero, then
+// partial states). Both are fenced like scratch: a call on another stream waits for
+// the last one.
 struct SeqPlan {
+  // What block and workspace hold, or have room for. Offsets are in bytes.
+  struct Room {
+    size_t rows = 0, tiles = 0, toks = 0, table = 0;  // entries of the lists
+    size_t row_parts = 0, tile_parts = 0;             // partial states per kv head
+    bool holds(const Room &o) const {
+      return o.rows <= rows && o.tiles <= tiles && o.toks <= toks && o.table <= table && o.row_parts <= row_parts &&
+             o.tile_parts <= tile_parts;
+    }
+  };
   SeqGeom geom;
-  SeqLists lists;        // as last built (the device holds items, merges, toks, table)
+  SeqLists lists;  // as last built; the device holds them
   int64_t n_seqs = 0;
-  DevBuf block, part;
-  size_t off_merges = 0, off_toks = 0, off_table = 0;  // byte offsets in block (items at 0)
-  size_t cap_items = 0, cap_merges = 0, cap_toks = 0, cap_table = 0;
-  uint8_t *pin = nullptr;      // page-locked image of block, made by the first update
+  Room room;
+  DevBuf block, work;
+  size_t off_tiles = 0, off_toks = 0, off_table = 0;      // in block (row items at 0)
+  size_t off_tile_cnt = 0, off_rows = 0, off_tile_part = 0;  // in work (row counts at 0)
+  uint8_t *pin = nullptr;       // page-locked image of block, made by the first update
   hipEvent_t pin_ev = nullptr;  // its last upload
-  bool captured = false;       // a graph holds these buffers: they are not replaced
+  int64_t reserved_q = 0;       // > 0: rk_seq_plan_reserve'd, for q_lens up to this
+  bool captured = false;        // a graph holds these buffers: they are not replaced
   int64_t captured_pos = INT64_MAX;  // rows of the shortest cos/sin tables that a captured append reads
 };
 
@@ -2481,52 +2494,62 @@ int is_capturing(hipStream_t st, bool *yes, const char *op) {
   return RK_OK;
 }
 
-size_t seq_part_bytes(const SeqPlan &p) {
-  return (size_t)p.lists.n_parts * p.geom.n_kv_heads * SEQ_ROWS * (p.geom.head_dim + 2) * 4;
+SeqPlan::Room seq_room(const SeqLists &l) {
+  SeqPlan::Room r;
+  r.rows = l.rows.items.size();
+  r.tiles = l.tiles.items.size();
+  r.toks = l.toks.size();
+  r.table = l.table.size();
+  r.row_parts = (size_t)l.rows.n_parts;
+  r.tile_parts = (size_t)l.tiles.n_parts;
+  return r;
 }
 
-// Writes the plan's lists, padded to its capacities, in the layout of its block.
+// Writes the plan's lists, padded to its room, in the layout of its block.
 void seq_image(const SeqPlan &p, uint8_t *to) {
   std::memset(to, 0, p.block.bytes);
   const SeqLists &l = p.lists;
-  if (!l.items.empty()) std::memcpy(to, l.items.data(), l.items.size() * sizeof(SeqItem));
-  if (!l.merges.empty()) std::memcpy(to + p.off_merges, l.merges.data(), l.merges.size() * sizeof(SeqMerge));
-  if (!l.toks.empty()) std::memcpy(to + p.off_toks, l.toks.data(), l.toks.size() * sizeof(SeqTok));
+  const auto put = [&](size_t off, const void *src, size_t bytes) {
+    if (bytes) std::memcpy(to + off, src, bytes);
+  };
+  put(0, l.rows.items.data(), l.rows.items.size() * sizeof(SeqItem));
+  put(p.off_tiles, l.tiles.items.data(), l.tiles.items.size() * sizeof(SeqItem));
+  put(p.off_toks, l.toks.data(), l.toks.size() * sizeof(SeqTok));
+  put(p.off_table, l.table.data(), l.table.size() * 4);
   SeqTok *toks = (SeqTok *)(to + p.off_toks);
-  for (size_t i = l.toks.size(); i < p.cap_toks; ++i) toks[i].page = -1;  // goes nowhere
-  if (!l.table.empty()) std::memcpy(to + p.off_table, l.table.data(), l.table.size() * 4);
+  for (size_t i = l.toks.size(); i < p.room.toks; ++i) toks[i].page = -1;  // goes nowhere
 }
 
-// Buffers that hold the lists (new ones, or the old where they are large enough).
-int seq_reserve(SeqPlan &p, const char *op) {
-  const SeqLists &l = p.lists;
-  const bool fits = p.block.p && l.items.size() <= p.cap_items && l.merges.size() <= p.cap_merges &&
-                    l.toks.size() <= p.cap_toks && l.table.size() <= p.cap_table;
-  if (!fits) {
-    RK_TRY(seq_buf_wait(p.block, op));
-    if (p.block.p) HIP_TRY(hipFree(p.block.p), op);
-    p.block.p = nullptr;
-    if (p.pin) HIP_TRY(hipHostFree(p.pin), op);
-    p.pin = nullptr;
-    p.cap_items = std::max(p.cap_items, l.items.size());
-    p.cap_merges = std::max(p.cap_merges, l.merges.size());
-    p.cap_toks = std::max(p.cap_toks, l.toks.size());
-    p.cap_table = std::max(p.cap_table, l.table.size());
-    p.off_merges = align16(p.cap_items * sizeof(SeqItem));
-    p.off_toks = p.off_merges + align16(p.cap_merges * sizeof(SeqMerge));
-    p.off_table = p.off_toks + align16(p.cap_toks * sizeof(SeqTok));
-    p.block.bytes = std::max<size_t>(p.off_table + align16(p.cap_table * 4), 256);
-    HIP_TRY(hipMalloc(&p.block.p, p.block.bytes), op);
-  }
-  const size_t part = seq_part_bytes(p);
-  if (part > p.part.bytes) {
-    RK_TRY(seq_buf_wait(p.part, op));
-    if (p.part.p) HIP_TRY(hipFree(p.part.p), op);
-    p.part.p = nullptr;
-    p.part.bytes = 0;
-    HIP_TRY(hipMalloc(&p.part.p, part), op);
-    p.part.bytes = part;
-  }
+// Buffers with room for `want` (new ones, or the old where they are large enough).
+// The block's contents are lost where it is replaced.
+int seq_reserve(SeqPlan &p, const SeqPlan::Room &want, const char *op) {
+  if (p.block.p && p.room.holds(want)) return RK_OK;
+  RK_TRY(seq_buf_wait(p.block, op));
+  RK_TRY(seq_buf_wait(p.work, op));
+  if (p.block.p) HIP_TRY(hipFree(p.block.p), op);
+  p.block.p = nullptr;
+  if (p.work.p) HIP_TRY(hipFree(p.work.p), op);
+  p.work.p = nullptr;
+  if (p.pin) HIP_TRY(hipHostFree(p.pin), op);
+  p.pin = nullptr;
+  SeqPlan::Room &r = p.room;
+  r = SeqPlan::Room{std::max(r.rows, want.rows),   std::max(r.tiles, want.tiles),
+                    std::max(r.toks, want.toks),   std::max(r.table, want.table),
+                    std::max(r.row_parts, want.row_parts), std::max(r.tile_parts, want.tile_parts)};
+  p.off_tiles = align16(r.rows * sizeof(SeqItem));
+  p.off_toks = p.off_tiles + align16(r.tiles * sizeof(SeqItem));
+  p.off_table = p.off_toks + align16(r.toks * sizeof(SeqTok));
+  p.block.bytes = std::max<size_t>(p.off_table + align16(r.table * 4), 256);
+  HIP_TRY(hipMalloc(&p.block.p, p.block.bytes), op);
+  if (r.row_parts + r.tile_parts == 0) return RK_OK;
+  const size_t kv = (size_t)p.geom.n_kv_heads;
+  p.off_tile_cnt = r.row_parts * kv * 4;
+  p.off_rows = (p.off_tile_cnt + r.tile_parts * kv * 4 + 255) / 256 * 256;
+  p.off_tile_part = p.off_rows + r.row_parts * kv * rk_seq_slot_bytes(p.geom.head_dim, true);
+  p.work.bytes = p.off_tile_part + r.tile_parts * kv * rk_seq_slot_bytes(p.geom.head_dim, false);
+  HIP_TRY(hipMalloc(&p.work.p, p.work.bytes), op);
+  HIP_TRY(hipMemset(p.work.p, 0, p.off_rows), op);
+  HIP_TRY(hipDeviceSynchronize(), op);
   return RK_OK;
 }
 
@@ -2557,7 +2580,7 @@ int seq_plan_create(SeqGeom g, const SeqBatch &b, void **plan, const char *op) {
     p->geom = g;
     p->n_seqs = b.n_seqs;
     seq_build(g, b, g_eng->num_cus, &p->lists);
-    RK_TRY(seq_reserve(*p, op));
+    RK_TRY(seq_reserve(*p, seq_room(p->lists), op));
     std::vector<uint8_t> image(p->block.bytes);
     seq_image(*p, image.data());
     HIP_TRY(hipMemcpy(p->block.p, image.data(), image.size(), hipMemcpyHostToDevice), op);
@@ -2566,7 +2589,7 @@ int seq_plan_create(SeqGeom g, const SeqBatch &b, void **plan, const char *op) {
   });
   if (rc != RK_OK) {
     seq_buf_free(p->block);
-    seq_buf_free(p->part);
+    seq_buf_free(p->work);
     delete p;
     return rc;
   }
@@ -2598,19 +2621,15 @@ int seq_plan_update(void *plan, bool paged, const SeqBatch &b, rk_stream stream,
   SeqLists l;
   seq_build(p->geom, b, g_eng->num_cus, &l);
   if (p->captured) {
-    SeqPlan probe;
-    probe.geom = p->geom;
-    probe.lists.n_parts = l.n_parts;
-    if (l.items.size() > p->cap_items || l.merges.size() > p->cap_merges || l.toks.size() > p->cap_toks ||
-        l.table.size() > p->cap_table || seq_part_bytes(probe) > p->part.bytes)
-      return fail(RK_E_SHAPE, op, "a graph holds this plan, and the batch needs more than the one it was made for");
+    if (!p->room.holds(seq_room(l)) || l.max_q > p->reserved_q)
+      return fail(RK_E_SHAPE, op, "a graph holds this plan, and the batch needs more than was reserved");
     if (p->captured_pos != INT64_MAX && (l.clash || l.max_pos >= p->captured_pos))
       return fail(RK_E_SHAPE, op, "a graph's append reads this plan: two new tokens in one slot, or past its cos/sin tables");
   }
   if (p->pin_ev) HIP_TRY(hipEventSynchronize(p->pin_ev), op);  // the image's last upload has left it
   p->lists = std::move(l);
   p->n_seqs = b.n_seqs;
-  int rc = seq_reserve(*p, op);
+  int rc = seq_reserve(*p, seq_room(p->lists), op);
   if (rc == RK_OK && !p->pin) {
     const hipError_t e = hipHostMalloc((void **)&p->pin, p->block.bytes, hipHostMallocDefault);
     if (e != hipSuccess) rc = hip_fail(e, op);
@@ -2649,15 +2668,18 @@ int seq_attention(const void *plan, bool paged, const void *q, int64_t q_stride,
   hipStream_t st = pick(stream);
   bool capturing;
   RK_TRY(is_capturing(st, &capturing, op));
+  if (capturing && p->reserved_q == 0) return fail(RK_E_UNSUPPORTED, op, "capture needs rk_seq_plan_reserve first");
   if (p->lists.n_tokens == 0 && !capturing) return RK_OK;
   const int64_t qw = (int64_t)g.n_head * g.head_dim, kw = (int64_t)g.n_kv_heads * g.head_dim;
   RK_TRY(seq_rows_check(q, q_stride, qw, "q", op));
   RK_TRY(seq_rows_check(out, out_stride, qw, "out", op));
   RK_TRY(seq_rows_check(k, paged ? kw : k_stride, kw, paged ? "k_cache" : "k", op));
   RK_TRY(seq_rows_check(v, paged ? kw : v_stride, kw, paged ? "v_cache" : "v", op));
+  if (!paged && std::max(k_stride, v_stride) >= SEQ_MAX_STRIDE)
+    return fail(RK_E_SHAPE, op, "k and v strides must be below 2^26 values");
   CallScope cs(st);
   RK_TRY(seq_buf_use(cs, p->block, capturing, op));
-  RK_TRY(seq_buf_use(cs, p->part, capturing, op));
+  RK_TRY(seq_buf_use(cs, p->work, capturing, op));
   SeqAttnArgs a{};
   const uint8_t *block = (const uint8_t *)p->block.p;
   a.q = q;
@@ -2668,9 +2690,7 @@ int seq_attention(const void *plan, bool paged, const void *q, int64_t q_stride,
   a.k_stride = k_stride;
   a.v_stride = v_stride;
   a.out_stride = out_stride;
-  a.items = (const SeqItem *)block;
   a.table = (const int32_t *)(block + p->off_table);
-  a.part = (float *)p->part.p;
   a.n_head = g.n_head;
   a.n_kv_heads = g.n_kv_heads;
   a.head_dim = g.head_dim;
@@ -2681,10 +2701,22 @@ int seq_attention(const void *plan, bool paged, const void *q, int64_t q_stride,
   a.window = (int)g.window;
   a.uniform = g.uniform;
   // A captured launch has a workgroup for every item that an update may list.
-  const size_t n = capturing ? p->cap_items : p->lists.items.size();
-  if (n == 0) return RK_OK;
+  const size_t n_rows = capturing ? p->room.rows : p->lists.rows.items.size();
+  const size_t n_tiles = capturing ? p->room.tiles : p->lists.tiles.items.size();
   if (capturing) p->captured = true;
-  HIP_TRY(rk_launch_attention_seqs(a, (int)n, paged, dtype, st), op);
+  uint8_t *work = (uint8_t *)p->work.p;
+  if (n_tiles) {
+    a.items = (const SeqItem *)(block + p->off_tiles);
+    a.cnt = (unsigned *)(work + p->off_tile_cnt);
+    a.part = work + p->off_tile_part;
+    HIP_TRY(rk_launch_attention_seqs(a, (int)n_tiles, false, paged, dtype, st), op);
+  }
+  if (n_rows) {
+    a.items = (const SeqItem *)block;
+    a.cnt = (unsigned *)work;
+    a.part = work + p->off_rows;
+    HIP_TRY(rk_launch_attention_seqs(a, (int)n_rows, true, paged, dtype, st), op);
+  }
   g_eng->calls++;
   return RK_OK;
 }
@@ -2736,6 +2768,35 @@ extern "C" int rk_paged_plan_update(void *plan, const int32_t *q_lens, const int
                          "rk_paged_plan_update");
   });
 }
+extern "C" int rk_seq_plan_reserve(void *plan, int64_t max_q_len) {
+  const char *op = "rk_seq_plan_reserve";
+  return no_throw(op, [&]() -> int {
+    std::lock_guard<std::mutex> lk(g_mu);
+    RK_TRY(ensure(op));
+    SeqPlan *p;
+    RK_TRY(seq_plan_get(plan, -1, &p, op));
+    if (p->captured) return fail(RK_E_UNSUPPORTED, op, "a graph holds this plan");
+    const int64_t G = p->geom.n_head / p->geom.n_kv_heads;
+    const int64_t longest = std::max<int64_t>({max_q_len, p->lists.max_q, 1});
+    if (longest > INT32_MAX / G) return fail(RK_E_SHAPE, op, "max_q_len·(n_head/n_kv_heads) of 2^31 or more");
+    SeqBound rows, tiles;
+    seq_bound(p->geom, p->n_seqs, p->lists.n_tokens, longest, g_eng->num_cus, &rows, &tiles);
+    SeqPlan::Room want = seq_room(p->lists);
+    want.rows = (size_t)rows.items;
+    want.row_parts = (size_t)rows.parts;
+    want.tiles = (size_t)tiles.items;
+    want.tile_parts = (size_t)tiles.parts;
+    // (a list that would be lost with its buffers is written again)
+    RK_TRY(seq_buf_wait(p->block, op));
+    RK_TRY(seq_buf_wait(p->work, op));
+    RK_TRY(seq_reserve(*p, want, op));
+    std::vector<uint8_t> image(p->block.bytes);
+    seq_image(*p, image.data());
+    HIP_TRY(hipMemcpy(p->block.p, image.data(), image.size(), hipMemcpyHostToDevice), op);
+    p->reserved_q = longest;
+    return RK_OK;
+  });
+}
 extern "C" int rk_seq_plan_destroy(void *plan) {
   const char *op = "rk_seq_plan_destroy";
   std::lock_guard<std::mutex> lk(g_mu);
@@ -2747,14 +2808,14 @@ extern "C" int rk_seq_plan_destroy(void *plan) {
   // holds them are known to the device alone.
   if (p->captured) HIP_TRY(hipDeviceSynchronize(), op);
   RK_TRY(seq_buf_wait(p->block, op));
-  RK_TRY(seq_buf_wait(p->part, op));
+  RK_TRY(seq_buf_wait(p->work, op));
   if (p->pin_ev) {
     HIP_TRY(hipEventSynchronize(p->pin_ev), op);
     (void)hipEventDestroy(p->pin_ev);
   }
   if (p->pin) (void)hipHostFree(p->pin);
   seq_buf_free(p->block);
-  seq_buf_free(p->part);
+  seq_buf_free(p->work);
   g_eng->seq_plans.erase(p);
   delete p;
   return RK_OK;
@@ -2788,6 +2849,7 @@ extern "C" int rk_paged_append_dev(const void *plan, const void *qkv, int64_t ro
   hipStream_t st = pick(stream);
   bool capturing;
   RK_TRY(is_capturing(st, &capturing, op));
+  if (capturing && p->reserved_q == 0) return fail(RK_E_UNSUPPORTED, op, "capture needs rk_seq_plan_reserve first");
   if (p->lists.n_tokens == 0 && !capturing) return RK_OK;
   const int heads = g.n_head + 2 * g.n_kv_heads;
   RK_TRY(seq_rows_check(qkv, row_stride, (int64_t)heads * g.head_dim, "qkv", op));
@@ -2801,7 +2863,7 @@ extern "C" int rk_paged_append_dev(const void *plan, const void *qkv, int64_t ro
     return fail(RK_E_SHAPE, op, "the tables have " + std::to_string(n_pos) + " rows, the last new token is at " +
                                     std::to_string(p->lists.max_pos));
   if (p->lists.clash) return fail(RK_E_SHAPE, op, "two new tokens of the batch go to one slot of a page");
-  const int64_t n = capturing ? (int64_t)p->cap_toks : p->lists.n_tokens;
+  const int64_t n = capturing ? (int64_t)p->room.toks : p->lists.n_tokens;
   if (n * heads > INT32_MAX) return fail(RK_E_SHAPE, op, "2^31 or more head rows");
   CallScope cs(st);
   RK_TRY(seq_buf_use(cs, p->block, capturing, op));
@@ -2941,7 +3003,7 @@ extern "C" int rk_stream_destroy(rk_stream stream) {
   for (auto &kv : g_eng->scratch)
     if (kv.second.ev_stream == st) kv.second.pending = kv.second.recorded = false;
   for (SeqPlan *p : g_eng->seq_plans)
-    for (DevBuf *b : {&p->block, &p->part})
+    for (DevBuf *b : {&p->block, &p->work})
       if (b->ev_stream == st) b->pending = b->recorded = false;
   HIP_TRY(hipStreamDestroy(st), "rk_stream_destroy");
   g_eng->own_streams.erase(st);

@@ -219,12 +219,21 @@ struct SeqAttnArgs {
   int64_t q_stride, k_stride, v_stride, out_stride;  // values between tokens (k, v: packed only)
   const SeqItem *items;
   const int32_t *table;  // page ids (paged)
-  float *part;           // partial softmax states
+  void *part;            // partial softmax states
+  unsigned *cnt;         // arrival counts of split tiles: zero between launches
   int n_head, n_kv_heads, head_dim, page_log2;
   float scale, softcap;
   int mask_mode, window, uniform;
 };
-hipError_t rk_launch_attention_seqs(const SeqAttnArgs &a, int n_items, bool paged, int dtype, hipStream_t st);
+// Launches over n_items items of a.items; few: those of the list of few rows.
+hipError_t rk_launch_attention_seqs(const SeqAttnArgs &a, int n_items, bool few, bool paged, int dtype, hipStream_t st);
+size_t rk_seq_slot_bytes(int head_dim, bool few);  // one partial state
+hipError_t rk_launch_seq_rows_f16(const SeqAttnArgs &a, int n_items, bool paged, hipStream_t st);
+hipError_t rk_launch_seq_rows_bf16(const SeqAttnArgs &a, int n_items, bool paged, hipStream_t st);
+hipError_t rk_launch_seq_tiles_f16(const SeqAttnArgs &a, int n_items, bool paged, hipStream_t st);
+hipError_t rk_launch_seq_tiles_bf16(const SeqAttnArgs &a, int n_items, bool paged, hipStream_t st);
+hipError_t rk_launch_seq_tiles_f16_cap(const SeqAttnArgs &a, int n_items, bool paged, hipStream_t st);
+hipError_t rk_launch_seq_tiles_bf16_cap(const SeqAttnArgs &a, int n_items, bool paged, hipStream_t st);
 
 struct PagedAppendArgs {
   const void *qkv;  // [n_tokens] rows: q heads, k heads, v heads

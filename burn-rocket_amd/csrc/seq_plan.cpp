@@ -82,9 +82,57 @@ std::string seq_check_batch(const SeqGeom &g, const SeqBatch &b) {
   return "";
 }
 
+namespace {
+// Workgroups of a kernel that the GPU holds at once, per kv head (at least one).
+int64_t slots_per_head(const SeqGeom &g, int num_cus, bool few) {
+  // LDS leaves one workgroup per CU, two of the first kernel for heads up to 64.
+  const int64_t slots = (int64_t)std::max(1, num_cus) * (few && g.head_dim <= 64 ? 2 : 1);
+  return std::max<int64_t>(1, slots / g.n_kv_heads);
+}
+
+// Splits the keys of the longest tiles so that no item is longer than an even share
+// of the work (and none shorter than `least` steps), then sorts longest first: the
+// short ones fill the last round.
+void split(std::vector<SeqItem> &tiles, int step, int64_t slots, int64_t least, SeqList *out) {
+  const auto steps = [&](const SeqItem &t) { return ceil_div(t.k_end - t.k_begin, step); };
+  int64_t total = 0;
+  for (const SeqItem &t : tiles) total += steps(t);
+  const int64_t quota = std::max(least, ceil_div(total, slots));
+  for (SeqItem &t : tiles) {
+    const int64_t n = steps(t), parts = std::min<int64_t>(ceil_div(n, quota), SEQ_MAX_PARTS);
+    t.n_parts = (int32_t)parts;
+    t.part0 = out->n_parts;
+    if (parts > 1) out->n_parts += (int)parts;
+    const int32_t k0 = t.k_begin, k1 = t.k_end;
+    for (int64_t i = 0; i < parts; ++i) {
+      t.sp = (int32_t)i;
+      t.k_begin = (int32_t)(k0 + n * i / parts * step);
+      t.k_end = i + 1 == parts ? k1 : (int32_t)(k0 + n * (i + 1) / parts * step);
+      out->items.push_back(t);
+    }
+  }
+  std::stable_sort(out->items.begin(), out->items.end(),
+                   [&](const SeqItem &x, const SeqItem &y) { return steps(x) > steps(y); });
+}
+constexpr int64_t ROWS_LEAST = 8, TILES_LEAST = 4;  // steps of an item that its own cost allows
+}  // namespace
+
+void seq_bound(const SeqGeom &g, int64_t n_seqs, int64_t n_tokens, int64_t max_q, int num_cus, SeqBound *rows,
+               SeqBound *tiles) {
+  // Splits add at most total / quota <= slots items; a split tile's states are at
+  // most twice what its split added.
+  const int64_t G = g.n_head / g.n_kv_heads, tr = seq_tile_rows(g.head_dim);
+  const int64_t s0 = slots_per_head(g, num_cus, true), s1 = slots_per_head(g, num_cus, false);
+  n_seqs = std::min(n_seqs, n_tokens);  // those with new tokens
+  *rows = SeqBound{n_seqs + s0, 2 * s0};
+  *tiles = SeqBound{};
+  if (max_q * G > SEQ_FEW_ROWS)
+    *tiles = SeqBound{n_tokens * G / tr + std::min(n_seqs, n_tokens * G / (SEQ_FEW_ROWS + 1)) + s1, 2 * s1};
+}
+
 void seq_build(const SeqGeom &g, const SeqBatch &b, int num_cus, SeqLists *out) {
-  (void)num_cus;
   *out = SeqLists{};
+  std::vector<SeqItem> rows, tiles;
   const int64_t G = g.n_head / g.n_kv_heads;
   struct Piece {
     int32_t page, off, end;
@@ -99,18 +147,20 @@ void seq_build(const SeqGeom &g, const SeqBatch &b, int num_cus, SeqLists *out) 
     it.rows = (int32_t)(q * G);
     it.kv_len = (int32_t)kv;
     it.table = (int32_t)out->table.size();
-    it.part = -1;
-    for (int64_t r = 0; r < q * G; r += SEQ_ROWS) {
+    const bool few = q * G <= SEQ_FEW_ROWS;
+    const int64_t tr = few ? 16 : seq_tile_rows(g.head_dim), step = few ? SEQ_ROWS_CHUNK : SEQ_KEY_TILE;
+    for (int64_t r = 0; r < q * G; r += tr) {
       int64_t lo, hi, lo2, hi2;
       visible(g, pos0 + r / G, kv, &lo, &hi);
-      visible(g, pos0 + (std::min(r + SEQ_ROWS, q * G) - 1) / G, kv, &lo2, &hi2);
+      visible(g, pos0 + (std::min(r + tr, q * G) - 1) / G, kv, &lo2, &hi2);
       it.row0 = (int32_t)r;
       it.k_lo = (int32_t)lo;
-      it.k_begin = (int32_t)(lo / SEQ_KEY_TILE * SEQ_KEY_TILE);
+      it.k_begin = (int32_t)(lo / step * step);
       it.k_end = (int32_t)(hi2 + 1);
-      out->items.push_back(it);
+      (few ? rows : tiles).push_back(it);
     }
     out->n_tokens += q;
+    out->max_q = std::max(out->max_q, q);
     out->max_pos = std::max(out->max_pos, kv - 1);
     if (!g.paged) continue;
     int64_t lo, hi;
@@ -125,6 +175,8 @@ void seq_build(const SeqGeom &g, const SeqBatch &b, int num_cus, SeqLists *out) 
       t = e;
     }
   }
+  split(rows, SEQ_ROWS_CHUNK, slots_per_head(g, num_cus, true), ROWS_LEAST, &out->rows);
+  split(tiles, SEQ_KEY_TILE, slots_per_head(g, num_cus, false), TILES_LEAST, &out->tiles);
   std::sort(pieces.begin(), pieces.end(),
             [](const Piece &x, const Piece &y) { return x.page != y.page ? x.page < y.page : x.off < y.off; });
   for (size_t i = 1; i < pieces.size(); ++i)

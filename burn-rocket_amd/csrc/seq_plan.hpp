@@ -21,18 +21,13 @@ struct SeqItem {
   int32_t rows;     // query rows of the sequence, q_len·G; 0: the item is empty
   int32_t row0;     // first row of the tile
   int32_t kv_len;   // keys of the sequence
-  int32_t k_begin;  // the item's keys [k_begin, k_end); k_begin is a multiple of SEQ_KEY_TILE
+  int32_t k_begin;  // the item's keys [k_begin, k_end); k_begin is a multiple of the list's step
   int32_t k_end;
   int32_t k_lo;     // lowest key that a row of the tile sees: blocks of 16 keys below it are not read
   int32_t table;    // paged: where the sequence's page ids start in the table list
-  int32_t part;     // >= 0: slot of its partial state (the slot of kv head g is part·n_kv_heads + g)
-  int32_t pad[2];
-};
-
-// A row tile whose states are joined: slots part0 .. part0 + n_parts - 1.
-struct SeqMerge {
-  int32_t tok0, rows, row0, part0, n_parts;
-  int32_t pad[3];
+  int32_t n_parts;  // items of this tile
+  int32_t sp;       // which of them, in key order
+  int32_t part0;    // n_parts > 1: slot of the first one's state (of kv head g: part0·n_kv_heads + g)
 };
 
 // Where a new token goes: its page and its key index.
@@ -40,8 +35,15 @@ struct SeqTok {
   int32_t page, pos;
 };
 
-constexpr int SEQ_ROWS = 128;     // query rows of a tile
-constexpr int SEQ_KEY_TILE = 64;  // keys of the kernels' steps; ranges start at multiples of it
+// Two kernels take the items: tiles of 16 rows with their keys over the waves of a
+// workgroup (seq_rows.hpp) for sequences of at most SEQ_FEW_ROWS query rows, tiles of
+// seq_tile_rows (seq_tiles.hpp) for the others.
+constexpr int SEQ_FEW_ROWS = 16;
+constexpr int SEQ_ROWS_CHUNK = 32;  // keys of a step of the first, ranges start at multiples
+constexpr int SEQ_KEY_TILE = 64;    // and of the second
+constexpr int seq_tile_rows(int head_dim) { return head_dim <= 128 ? 128 : 64; }
+constexpr int SEQ_MAX_PARTS = 32;
+constexpr int64_t SEQ_MAX_STRIDE = (int64_t)1 << 26;  // values between packed tokens: 16 of them stay below 2 GiB
 
 struct SeqGeom {
   bool paged = false;
@@ -59,13 +61,16 @@ struct SeqBatch {
   int64_t table_stride = 0, n_seqs = 0;
 };
 
+struct SeqList {
+  std::vector<SeqItem> items;  // longest first
+  int n_parts = 0;             // partial states (per kv head)
+};
 struct SeqLists {
   int64_t n_tokens = 0;
+  int64_t max_q = 0;      // longest q_len
   int64_t max_pos = -1;   // largest key index of a new token
   bool clash = false;     // two new tokens go to one slot of a page
-  int n_parts = 0;        // partial states (per kv head)
-  std::vector<SeqItem> items;
-  std::vector<SeqMerge> merges;
+  SeqList rows, tiles;
   std::vector<SeqTok> toks;
   std::vector<int32_t> table;
 };
@@ -77,3 +82,10 @@ std::string seq_check_geom(SeqGeom &g, bool *unsupported);
 std::string seq_check_batch(const SeqGeom &g, const SeqBatch &b);
 // The lists of a checked batch for a GPU of num_cus CUs.
 void seq_build(const SeqGeom &g, const SeqBatch &b, int num_cus, SeqLists *out);
+// The most items and partial states that seq_build lists for any batch of at most
+// n_seqs sequences and n_tokens new tokens, none longer than max_q.
+struct SeqBound {
+  int64_t items = 0, parts = 0;
+};
+void seq_bound(const SeqGeom &g, int64_t n_seqs, int64_t n_tokens, int64_t max_q, int num_cus, SeqBound *rows,
+               SeqBound *tiles);

@@ -178,6 +178,7 @@ unsafe extern "C" {
         plan: *mut c_void, q_lens: *const i32, kv_lens: *const i32, page_table: *const i32,
         table_stride: i64, n_seqs: i64, stream: Stream
     ) -> c_int;
+    pub fn rk_seq_plan_reserve(plan: *mut c_void, max_q_len: i64) -> c_int;
     pub fn rk_seq_plan_destroy(plan: *mut c_void) -> c_int;
     pub fn rk_attention_packed_dev(
         plan: *const c_void, q: *const c_void, q_stride: i64, k: *const c_void, k_stride: i64,

@@ -434,14 +434,15 @@ int rk_flash_attn_f16_masked(int64_t n_q, int64_t n_kv, int head_dim, int dv, in
  * ordered on `stream` after the calls that used the plan, waits on the host for
  * the upload of the update before it, and is refused inside a stream capture.
  *
- * Streams: calls on one plan from different streams run one after another. Under
- * a stream capture nothing is allocated and launches have room for every batch
- * of an update that needs no more tokens, sequences and pages than the plan was
- * made with; larger updates are then refused (RK_E_SHAPE). The buffers of a
- * captured call must have room for as many tokens as the plan was made with.
- * The caller orders the replays of graphs that share a plan, and other calls
- * and updates of a captured plan, after one another. A plan is destroyed after its
- * graphs. */
+ * Streams: calls on one plan from different streams run one after another. Before
+ * a call is captured into a graph, rk_seq_plan_reserve gives the plan room for any
+ * later batch of no more sequences, tokens and pages than its present one, with
+ * q_lens up to max_q_len (below the present longest: that one); nothing is allocated
+ * in the capture, launches have room for all of it, and updates that need more are
+ * then refused (RK_E_SHAPE). The q, out and q|k|v buffers of a captured call must
+ * have room for the present number of tokens. The caller orders the replays of
+ * graphs that share a plan, and other calls and updates of a captured plan, after
+ * one another. A plan is destroyed after its graphs. */
 int rk_packed_plan_create(const int32_t *q_lens, int64_t n_seqs, int n_head, int n_kv_heads, int head_dim,
                           int mask_mode, int64_t window, void **plan);
 int rk_paged_plan_create(const int32_t *q_lens, const int32_t *kv_lens, const int32_t *page_table,
@@ -450,6 +451,7 @@ int rk_paged_plan_create(const int32_t *q_lens, const int32_t *kv_lens, const in
 int rk_packed_plan_update(void *plan, const int32_t *q_lens, int64_t n_seqs, rk_stream stream);
 int rk_paged_plan_update(void *plan, const int32_t *q_lens, const int32_t *kv_lens,
                          const int32_t *page_table, int64_t table_stride, int64_t n_seqs, rk_stream stream);
+int rk_seq_plan_reserve(void *plan, int64_t max_q_len);
 int rk_seq_plan_destroy(void *plan);
 
 /* Attention of every sequence of a packed batch over its own tokens: q [tokens]

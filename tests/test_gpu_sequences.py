@@ -517,7 +517,7 @@ class Graph:
 def test_captured_step_replays_with_updates(rk):
     """Append and attention in one graph, replayed on later steps of a batch that shrinks and grows again."""
     note("graph capture")
-    h, kv, d, ps, n_pos = 8, 2, 64, 16, 4096
+    h, kv, d, ps, n_pos = 16, 2, 64, 16, 4096
     rng = np.random.default_rng(30)
     pg = ref.Pages(rng, [3000, 900, 64], ps)
     shape, xs = (pg.n_pages, kv, ps, d), (4, (h + 2 * kv) * d)
@@ -534,8 +534,14 @@ def test_captured_step_replays_with_updates(rk):
         ok(rk, lib.rk_attention_paged_dev(plan.ptr, q.ptr, h * d, k.ptr, v.ptr, 0.1, 0.0, o.ptr, h * d, rk.DTYPE_F16, st))
 
     plan = rk.paged_plan([2, 1, 1], [3000, 900, 64], pg.table, pg.n_pages, ps, h, kv, d)
+    refused = []
+    Graph(st, lambda: refused.append(lib.rk_attention_paged_dev(plan.ptr, mine[3].ptr, h * d, mine[0].ptr, mine[1].ptr, 0.1, 0.0,
+                                                                mine[4].ptr, h * d, rk.DTYPE_F16, st))).destroy()
+    assert refused == [rk.RK_E_UNSUPPORTED]  # nothing is reserved yet
+    plan.reserve(4)
     g = Graph(st, lambda: step(plan, *mine))
-    batches = [([2, 1, 1], [3000, 900, 64]), ([1], [1234]), ([1, 1, 1], [2048, 16, 60]), ([2, 2], [500, 899]), ([1, 0, 1], [2999, 5, 1])]
+    batches = [([2, 1, 1], [3000, 900, 64]), ([1], [1234]), ([1, 1, 1], [2048, 16, 60]), ([2, 2], [500, 899]), ([4], [3000]),
+               ([1, 0, 1], [2999, 5, 1])]
     for i, (q_lens, kv_lens) in enumerate(batches):
         n, x = sum(q_lens), rows(rng, "f16", *xs)
         table = pg.table[:len(q_lens)]
@@ -558,6 +564,8 @@ def test_captured_step_replays_with_updates(rk):
         now = want[:2]
     with pytest.raises(rk.RocketError):  # five tokens: more than the graph has room for
         plan.update([2, 2, 1], [10, 10, 10], pg.table, stream=st)
+    with pytest.raises(rk.RocketError):  # a longer chunk than was reserved for
+        plan.update([5], [10], pg.table[:1], stream=st)
     with pytest.raises(rk.RocketError):  # past the tables that the graph reads
         plan.update([1], [4097], np.zeros((1, 300), np.int32), stream=st)
     g.destroy()
