@@ -186,7 +186,7 @@ def prepare(case, seed):
     if "table" in t:
         s["table"] = torch.from_numpy(t["table"].astype(np.int64)).cuda()
     if own:
-        rk = _rk()
+        rk = s["rk"] = _rk()
         rk.init(0)
         modes = {"none": rk.MASK_NONE, "causal": rk.MASK_CAUSAL, "window": rk.MASK_WINDOW, "causal_window": rk.MASK_CAUSAL_WINDOW}
         heads = (c["h"], c["kv"], c["d"], modes[c.get("mode", "causal")], c.get("window", -1))
@@ -221,7 +221,7 @@ def run(state):
 
 
 def _own(s):
-    c, t, rk = s["c"], s["t"], _rk()
+    c, t, rk = s["c"], s["t"], s["rk"]
     lib, h, kv, d = rk.lib(), c["h"], c["kv"], c["d"]
     types = {"f32": rk.DTYPE_F32, "f16": rk.DTYPE_F16, "bf16": rk.DTYPE_BF16}
     dt, plan, p = types[c["dtype"]], s["plan"].ptr, torch.Tensor.data_ptr
