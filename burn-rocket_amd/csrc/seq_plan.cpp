@@ -1,8 +1,9 @@
 // Host side of the batches of sequences (seq_plan.hpp): checks and schedules.
 #include "seq_plan.hpp"
 
+#include <stdlib.h>
+
 #include <algorithm>
-#include <numeric>
 
 #include "../../include/burn_rocket_amd.h"
 
@@ -121,7 +122,7 @@ void seq_bound(const SeqGeom &g, int64_t n_seqs, int64_t n_tokens, int64_t max_q
                SeqBound *tiles) {
   // Splits add at most total / quota <= slots items; a split tile's states are at
   // most twice what its split added.
-  const int64_t G = g.n_head / g.n_kv_heads, tr = seq_tile_rows(g.head_dim);
+  const int64_t G = g.n_head / g.n_kv_heads, tr = seq_tile_rows(g.head_dim, false);
   const int64_t s0 = slots_per_head(g, num_cus, true), s1 = slots_per_head(g, num_cus, false);
   n_seqs = std::min(n_seqs, n_tokens);  // those with new tokens
   *rows = SeqBound{n_seqs + s0, 2 * s0};
@@ -130,25 +131,31 @@ void seq_bound(const SeqGeom &g, int64_t n_seqs, int64_t n_tokens, int64_t max_q
     *tiles = SeqBound{n_tokens * G / tr + std::min(n_seqs, n_tokens * G / (SEQ_FEW_ROWS + 1)) + s1, 2 * s1};
 }
 
-void seq_build(const SeqGeom &g, const SeqBatch &b, int num_cus, SeqLists *out) {
-  *out = SeqLists{};
-  std::vector<SeqItem> rows, tiles;
+void seq_items(const SeqGeom &g, int num_cus, bool may_wide, SeqLists *l) {
   const int64_t G = g.n_head / g.n_kv_heads;
-  struct Piece {
-    int32_t page, off, end;
-  };
-  std::vector<Piece> pieces;  // where new tokens go: slots [off, end) of a page
-  for (int64_t i = 0; i < b.n_seqs; ++i) {
-    const int64_t q = b.q_lens[i], kv = kv_of(b, i), pos0 = kv - q;
+  const size_t n = l->q_lens.size();
+  std::vector<SeqItem> rows, tiles;
+  l->rows = l->tiles = SeqList{};
+  l->wide = false;
+  if (may_wide) {
+    int64_t t = 0;
+    for (const int64_t q : l->q_lens)
+      if (q * G > SEQ_FEW_ROWS) t += ceil_div(q * G, seq_tile_rows(g.head_dim, true));
+    l->wide = t * g.n_kv_heads >= 2 * num_cus;
+    if (const char *e = getenv("RK_SEQ_WIDE")) l->wide = atoi(e) != 0;
+  }
+  int64_t tok = 0, ids = 0;
+  for (size_t i = 0; i < n; ++i) {
+    const int64_t q = l->q_lens[i], kv = l->kv_lens[i], pos0 = kv - q;
     if (q == 0) continue;
     SeqItem it{};
-    it.tok0 = (int32_t)out->n_tokens;
+    it.tok0 = (int32_t)tok;
     it.pos0 = (int32_t)pos0;
     it.rows = (int32_t)(q * G);
     it.kv_len = (int32_t)kv;
-    it.table = (int32_t)out->table.size();
+    it.table = (int32_t)ids;
     const bool few = q * G <= SEQ_FEW_ROWS;
-    const int64_t tr = few ? 16 : seq_tile_rows(g.head_dim), step = few ? SEQ_ROWS_CHUNK : SEQ_KEY_TILE;
+    const int64_t tr = few ? 16 : seq_tile_rows(g.head_dim, l->wide), step = few ? SEQ_ROWS_CHUNK : SEQ_KEY_TILE;
     for (int64_t r = 0; r < q * G; r += tr) {
       int64_t lo, hi, lo2, hi2;
       visible(g, pos0 + r / G, kv, &lo, &hi);
@@ -159,6 +166,24 @@ void seq_build(const SeqGeom &g, const SeqBatch &b, int num_cus, SeqLists *out) 
       it.k_end = (int32_t)(hi2 + 1);
       (few ? rows : tiles).push_back(it);
     }
+    tok += q;
+    if (g.paged) ids += ceil_div(kv, g.page_size);
+  }
+  split(rows, SEQ_ROWS_CHUNK, slots_per_head(g, num_cus, true), ROWS_LEAST, &l->rows);
+  split(tiles, SEQ_KEY_TILE, slots_per_head(g, num_cus, false), TILES_LEAST, &l->tiles);
+}
+
+void seq_build(const SeqGeom &g, const SeqBatch &b, int num_cus, bool may_wide, SeqLists *out) {
+  *out = SeqLists{};
+  struct Piece {
+    int32_t page, off, end;
+  };
+  std::vector<Piece> pieces;  // where new tokens go: slots [off, end) of a page
+  for (int64_t i = 0; i < b.n_seqs; ++i) {
+    const int64_t q = b.q_lens[i], kv = kv_of(b, i), pos0 = kv - q;
+    if (q == 0) continue;
+    out->q_lens.push_back((int32_t)q);
+    out->kv_lens.push_back((int32_t)kv);
     out->n_tokens += q;
     out->max_q = std::max(out->max_q, q);
     out->max_pos = std::max(out->max_pos, kv - 1);
@@ -175,8 +200,7 @@ void seq_build(const SeqGeom &g, const SeqBatch &b, int num_cus, SeqLists *out) 
       t = e;
     }
   }
-  split(rows, SEQ_ROWS_CHUNK, slots_per_head(g, num_cus, true), ROWS_LEAST, &out->rows);
-  split(tiles, SEQ_KEY_TILE, slots_per_head(g, num_cus, false), TILES_LEAST, &out->tiles);
+  seq_items(g, num_cus, may_wide, out);
   std::sort(pieces.begin(), pieces.end(),
             [](const Piece &x, const Piece &y) { return x.page != y.page ? x.page < y.page : x.off < y.off; });
   for (size_t i = 1; i < pieces.size(); ++i)

@@ -1,13 +1,15 @@
 // Attention of sequences with many query rows (prompts, chunks of prompts) on
 // gfx950: an online softmax over key tiles that K and V reach through LDS.
 //
-// A workgroup has a tile of 4·16·QB query rows of one kv head (128; 64 for head dim
-// 256) and an item's key range. Its 8 waves are two key groups of 4; wave w of a
-// group has rows 16·QB·w .., and the groups walk alternate key tiles of TK keys.
-// Their work alternates between a slot of matrix products (P·V of one tile, then
-// K·Qᵀ of the next) and a slot of softmax, one group a slot behind the other, so
-// that a SIMD multiplies for one wave while it exponentiates for the other.
-// Barriers separate the slots.
+// A workgroup's 8 waves are two groups of 4; a wave has 16·QB query rows of one kv
+// head. With KG = 1 all 8 have rows of their own (a tile of 256 rows, 128 for head dim
+// 256) and walk the item's key tiles together; with KG = 2 the groups have the same
+// 128 (64) rows and walk alternate key tiles, and their states meet at the end. KG = 1
+// copies half as much to LDS per product, KG = 2 leaves finer tiles for
+// batches that do not fill the GPU. The work of a group alternates between a slot of
+// matrix products (P·V of one tile, then K·Qᵀ of the next) and a slot of softmax, one
+// group a slot behind the other, so that a SIMD multiplies for one wave while it
+// exponentiates for the other. Barriers separate the slots.
 //
 // Per wave and tile (v_mfma_f32_16x16x32):
 //   Sᵀ = K·Qᵀ   K rows from LDS, Q in registers; a lane owns one query of each
@@ -19,11 +21,17 @@
 // The LDS fragment reads feed QB products each; with 32 rows per wave they take
 // the whole read rate of a CU (128 bytes a clock) while the products run.
 //
-// LDS: per group two buffers of K (rows of KPC 16-byte pieces, piece c of row r at
-// c ^ (r & (KPC-1))) and two of V (16-key blocks; 32-byte pairs swizzled by the
-// key where rows are a power of two). Copies go to LDS directly, one 16-key block
-// per buffer descriptor: a block lies in one page, so that its address is scalar
-// work and rows past the sequence's keys read as zeros.
+// Row sums come from the same products (a row of ones), which takes their additions
+// off the softmax slot and counts the probabilities as rounded.
+//
+// LDS: K rows of KPC 16-byte pieces (piece c of row r at c ^ (r & (KPC-1))), V as
+// 16-key blocks (32-byte pairs swizzled by the key where rows are a power of two).
+// KG = 2: two buffers of each per group, a group copies its own. KG = 1: three of K,
+// copied by group 1, and two of V, copied by group 0. Copies go to LDS directly, one
+// 16-key block per buffer descriptor: a block lies in one page, and rows past the
+// sequence's keys read as zeros. They start with a slot of softmax and have landed at
+// its end; started three slots ahead (four and three buffers) they cost the same, so it is not their
+// latency that counts but what they take from the LDS reads.
 //
 // Items that are one of n_parts of their tile leave their state in the plan's
 // workspace; the last to arrive merges the parts in key order.
@@ -32,13 +40,16 @@
 #include "seq_attn.hpp"
 
 namespace {
+// LDS fragments read ahead of their products: 2 and 4 to 8 and 8 measured alike.
+constexpr int AHEAD_V = 3, AHEAD_K = 4;
 constexpr float RESCALE = 8.0f;  // with P_BIAS: probabilities stay below 2^14
 
-template <int D>
+template <int D, int KG>
 struct SeqTilesGeom {
   static constexpr int QB = D <= 128 ? 2 : 1;       // 16-query blocks per wave
   static constexpr int TK = D <= 128 ? 64 : 32;     // keys per tile
-  static constexpr int ROWS = 64 * QB;              // query rows per workgroup
+  static constexpr int NW = 8 / KG;                 // waves with rows of their own
+  static constexpr int ROWS = NW * 16 * QB;         // query rows per workgroup
   static constexpr int NQC = (D + 31) / 32;         // 32-wide d chunks of QKᵀ
   static constexpr int NDB = (D + 15) / 16;         // 16-row d blocks of Oᵀ
   static constexpr int CH = D / 8;                  // 16-byte pieces of a row
@@ -52,21 +63,24 @@ struct SeqTilesGeom {
   static constexpr int VB = VI * 1024;              // bytes of a V block
   static constexpr bool POW2 = (D & (D - 1)) == 0;
   static constexpr int VSW = POW2 ? (CH / 2 < 8 ? CH / 2 : 8) - 1 : 0;
-  static constexpr int K_BYTES = TK * KROW;
-  static constexpr int BUF = K_BYTES + NB * VB;
-  static constexpr int XCH = (2 * QB + NDB * QB * 4) * 256;  // a wave's state in the exchange of the groups
-  static constexpr int SMEM = 4 * BUF > 4 * XCH ? 4 * BUF : 4 * XCH;
+  static constexpr int K_BYTES = TK * KROW, V_BYTES = NB * VB;
+  static constexpr int V_AT = (KG == 2 ? 4 : 3) * K_BYTES;  // the V buffers, behind those of K
+  static constexpr int BUFS = V_AT + (KG == 2 ? 4 : 2) * V_BYTES;
+  static constexpr int CK = KI * NB / 4, CV = VI * NB / 4;  // copies per wave and tile
+  static_assert(KI * NB % 4 == 0 && VI * NB % 4 == 0, "every wave copies alike");
+  static constexpr int XCH = (2 * QB + NDB * QB * 4) * 256;  // a wave's state in the exchange of the groups (KG = 2)
+  static constexpr int SMEM = BUFS > 4 * XCH || KG == 1 ? BUFS : 4 * XCH;
   static constexpr int NJ = 1 + NDB * QB;           // 1 KB pieces of a wave's state in the workspace
-  static constexpr int SLOT_BYTES = 4 * NJ * 1024;
+  static constexpr int SLOT_BYTES = NW * NJ * 1024;
   static_assert(SMEM <= 160 * 1024, "LDS");
 };
 }  // namespace
 
-template <int DT, int D, bool PAGED, bool SOFTCAP>
+template <int DT, int D, int KG, bool PAGED, bool SOFTCAP>
 __global__ __launch_bounds__(512, 2) void seq_tiles_kernel(SeqAttnArgs a) {
-  using Gm = SeqTilesGeom<D>;
+  using Gm = SeqTilesGeom<D, KG>;
   constexpr int QB = Gm::QB, TK = Gm::TK, NQC = Gm::NQC, NDB = Gm::NDB, NB = Gm::NB, NC2 = Gm::NC2;
-  constexpr int KI = Gm::KI, VI = Gm::VI, CH = Gm::CH, KPC = Gm::KPC, KROW = Gm::KROW, BUF = Gm::BUF;
+  constexpr int KI = Gm::KI, VI = Gm::VI, CH = Gm::CH, KPC = Gm::KPC, KROW = Gm::KROW;
   extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
 
   const int KV = a.n_kv_heads, G = a.n_head / KV;
@@ -77,15 +91,18 @@ __global__ __launch_bounds__(512, 2) void seq_tiles_kernel(SeqAttnArgs a) {
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int grp = wave >> 2, wq = wave & 3;
   const int l16 = lane & 15, lg = lane >> 4;
+  const int wr = KG == 1 ? wave : wq;  // which of the waves with rows
 
-  // ---- this lane's rows and what they see
+  // ---- this lane's rows and what they see. A negative scale is a sign of Q.
+  const uint32_t flip = a.scale < 0.f ? 0x80008000u : 0u;
+  const float scale = fabsf(a.scale);
   bool rok[QB];
   int klo[QB], khi[QB];
   uintx4 qf[QB][NQC];
   f16 *orow[QB];
 #pragma unroll
   for (int qb = 0; qb < QB; ++qb) {
-    const int r = it.row0 + wq * 16 * QB + qb * 16 + l16;
+    const int r = it.row0 + wr * 16 * QB + qb * 16 + l16;
     rok[qb] = r < it.rows;
     const int q = rok[qb] ? r / G : 0, h = kvh * G + (rok[qb] ? r % G : 0);
     seq_visible(a, it.pos0 + q, it.kv_len, klo[qb], khi[qb]);
@@ -94,29 +111,32 @@ __global__ __launch_bounds__(512, 2) void seq_tiles_kernel(SeqAttnArgs a) {
 #pragma unroll
     for (int c = 0; c < NQC; ++c) {
       const int d0 = 32 * c + 8 * lg;
-      qf[qb][c] = (rok[qb] && d0 < D) ? *(const uintx4 *)(qrow + d0) : uintx4{};
+      qf[qb][c] = ((rok[qb] && d0 < D) ? *(const uintx4 *)(qrow + d0) : uintx4{}) ^ flip;
     }
     orow[qb] = (f16 *)a.out + (int64_t)(it.tok0 + q) * a.out_stride + (int64_t)h * D;
   }
-  // Keys that every row of the tile sees, from its first and last row (the ends of
+  // Keys that every row of the wave sees, from its first and last row (the ends of
   // a row's keys never decrease with the row).
   int full_lo, full_hi, skip;
-  seq_visible(a, it.pos0 + it.row0 / G, it.kv_len, skip, full_hi);
-  seq_visible(a, it.pos0 + (min(it.row0 + Gm::ROWS, it.rows) - 1) / G, it.kv_len, full_lo, skip);
+  const int w_row0 = min(it.row0 + wr * 16 * QB, it.rows - 1);
+  seq_visible(a, it.pos0 + w_row0 / G, it.kv_len, skip, full_hi);
+  seq_visible(a, it.pos0 + min(w_row0 + 16 * QB - 1, it.rows - 1) / G, it.kv_len, full_lo, skip);
   // (a scale of 0 must leave hidden scores at -inf)
-  const float C = SOFTCAP ? LOG2E : a.scale != 0.f ? a.scale * LOG2E : 1e-30f;
+  const float C = SOFTCAP ? LOG2E : scale != 0.f ? scale * LOG2E : 1e-30f;
 
   // ---- copies
   const uint32_t ks = (uint32_t)((PAGED ? D : a.k_stride) * 2), vs = (uint32_t)((PAGED ? D : a.v_stride) * 2);
   const int kt_begin = it.k_begin / TK, n_tiles = (it.k_end + TK - 1) / TK - kt_begin;
-  const int nj = (n_tiles - grp + 1) / 2, nj_max = (n_tiles + 1) / 2;
+  // The group's tiles, numbered j = 0 .. nj - 1: tile kt_begin + KG·j (+ grp).
+  const int nj = KG == 2 ? (n_tiles - grp + 1) / 2 : n_tiles, nj_max = (n_tiles + KG - 1) / KG;
+  const int kt0 = kt_begin + (KG == 2 ? grp : 0);
   // Blocks of the group's tiles: lane l holds block l % NB of tile l / NB of a window
-  // of WIN tiles, kb of tile j + 1's window and vb of tile j's; ids: page ids of the
-  // window that kb turns to next (fetched a window ahead).
+  // of WIN tiles; kb and vb: of the windows that the next copies of K and V lie in;
+  // ids: page ids of the window that comes next (fetched a window ahead).
   constexpr int WIN = 64 / NB;
   KeyBlocks kb, vb;
   int ids = 0;
-  auto key_of = [&](int w) ALWAYS_INLINE { return (kt_begin + 2 * (w * WIN + lane / NB) + grp) * TK + 16 * (lane % NB); };
+  auto key_of = [&](int w) ALWAYS_INLINE { return (kt0 + KG * (w * WIN + lane / NB)) * TK + 16 * (lane % NB); };
   auto fetch_ids = [&](int w) ALWAYS_INLINE {
     if constexpr (PAGED) ids = a.table[it.table + (min(key_of(w), it.kv_len - 1) >> a.page_log2)];
   };
@@ -125,12 +145,12 @@ __global__ __launch_bounds__(512, 2) void seq_tiles_kernel(SeqAttnArgs a) {
   auto turn_v = [&](int w) ALWAYS_INLINE { vb = key_blocks<PAGED>(a, it, a.v, a.v_stride, kvh, key_of(w), end, ids); };
   // Wave wq's share of the copies of the group's tile j: pieces s of its 16-key
   // blocks b, in the order s + KI·b.
+  auto k_buf = [&](int j) ALWAYS_INLINE { return smem + (KG == 2 ? grp * 2 + (j & 1) : (int)((unsigned)j % 3)) * Gm::K_BYTES; };
+  auto v_buf = [&](int j) ALWAYS_INLINE { return smem + Gm::V_AT + ((KG == 2 ? grp * 2 : 0) + (j & 1)) * Gm::V_BYTES; };
   auto copy_k = [&](int j) ALWAYS_INLINE {
-    uint8_t *const to = smem + (grp * 2 + (j & 1)) * BUF;
-    static_for<(KI * NB + 3) / 4>([&](auto i_c) ALWAYS_INLINE {
-      const int c = wq + 4 * decltype(i_c)::value;
-      if (KI * NB % 4 && c >= KI * NB) return;
-      const int b = c / KI, s = c % KI;
+    uint8_t *const to = k_buf(j);
+    static_for<Gm::CK>([&](auto i_c) ALWAYS_INLINE {
+      const int c = wq + 4 * decltype(i_c)::value, b = c / KI, s = c % KI;
       const rsrc_t rk = block_rsrc(kb, (j % WIN) * NB + b);
       const int p = 64 * s + lane, row = p / KPC;
       const int ch = (p % KPC) ^ (row & Gm::KSW);  // logical piece of this slot
@@ -138,11 +158,9 @@ __global__ __launch_bounds__(512, 2) void seq_tiles_kernel(SeqAttnArgs a) {
     });
   };
   auto copy_v = [&](int j) ALWAYS_INLINE {
-    uint8_t *const to = smem + (grp * 2 + (j & 1)) * BUF + Gm::K_BYTES;
-    static_for<(VI * NB + 3) / 4>([&](auto i_c) ALWAYS_INLINE {
-      const int c = wq + 4 * decltype(i_c)::value;
-      if (VI * NB % 4 && c >= VI * NB) return;
-      const int b = c / VI, s = c % VI;
+    uint8_t *const to = v_buf(j);
+    static_for<Gm::CV>([&](auto i_c) ALWAYS_INLINE {
+      const int c = wq + 4 * decltype(i_c)::value, b = c / VI, s = c % VI;
       const rsrc_t rv = block_rsrc(vb, (j % WIN) * NB + b);
       const int p = 64 * s + lane, row = p / CH, ch = p % CH;
       const int lch = Gm::VSW ? ch ^ ((row & Gm::VSW) << 1) : ch;
@@ -156,43 +174,51 @@ __global__ __launch_bounds__(512, 2) void seq_tiles_kernel(SeqAttnArgs a) {
 #pragma unroll
   for (int c = 0; c < NQC; ++c) k_off[c] = (uint32_t)(l16 * KROW + (((4 * c + lg) ^ (l16 & Gm::KSW)) << 4));
   const int vkey = 4 * lg + (l16 >> 2);
-  const uint32_t v_row = (uint32_t)(Gm::K_BYTES + vkey * (D * 2) + (l16 & 3) * 8);
+  const uint32_t v_row = (uint32_t)(vkey * (D * 2) + (l16 & 3) * 8);
   const int vsw = vkey & Gm::VSW;
 
   floatx4 o[NDB][QB], s[NB][QB];
   uintx4 p[NC2][QB];
-  float m_run[QB], l_run[QB];
+  float m_run[QB];
+  floatx4 l_run[QB];  // (every row of the product with ones is the row sum)
+  const uint32_t one2 = DT == RK_DTYPE_F16 ? 0x3c003c00u : 0x3f803f80u;
+  const uintx4 ones = {one2, one2, one2, one2};
 #pragma unroll
   for (int qb = 0; qb < QB; ++qb) {
     m_run[qb] = -INFINITY;
-    l_run[qb] = 0.f;
+    l_run[qb] = floatx4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int db = 0; db < NDB; ++db) o[db][qb] = floatx4{0.f, 0.f, 0.f, 0.f};
   }
 
   auto mfma_slot = [&](int j) ALWAYS_INLINE {
+    __builtin_amdgcn_s_setprio(1);  // products first: what they leave of the issue slots is enough for a softmax
     if (j >= 1 && j - 1 < nj) {
-      const uint8_t *vb = smem + (grp * 2 + ((j - 1) & 1)) * BUF + v_row;
+      const uint8_t *vt = v_buf(j - 1) + v_row;
 #pragma unroll
-      for (int c2 = 0; c2 < NC2; ++c2)
+      for (int c2 = 0; c2 < NC2; ++c2) {
+#pragma unroll
+        for (int qb = 0; qb < QB; ++qb) l_run[qb] = mfma16<DT>(ones, p[c2][qb], l_run[qb]);
 #pragma unroll
         for (int db = 0; db < NDB; ++db) {
-          const uint8_t *at = vb + 2 * c2 * Gm::VB + ((db ^ vsw) << 5);
+          const uint8_t *at = vt + 2 * c2 * Gm::VB + ((db ^ vsw) << 5);
           const uintx4 vf = join8(lds_read_tr16(at), lds_read_tr16(at + Gm::VB));
 #pragma unroll
           for (int qb = 0; qb < QB; ++qb) o[db][qb] = mfma16<DT>(vf, p[c2][qb], o[db][qb]);
         }
+      }
+      // Each fragment (two reads) AHEAD_V fragments ahead of its products.
+      constexpr int NF = NC2 * NDB, AV = AHEAD_V < NF ? AHEAD_V : NF;
+      __builtin_amdgcn_sched_group_barrier(0x100, 2 * AV, 0);
+      static_for<NF - AV>([&](auto) ALWAYS_INLINE {
+        __builtin_amdgcn_sched_group_barrier(0x008, QB, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+      });
+      __builtin_amdgcn_sched_group_barrier(0x008, QB * (AV + NC2), 0);
     }
     __builtin_amdgcn_sched_barrier(0);  // P dies before S is made
     if (j < nj) {
-      // The copies come after the transposing reads: the compiler holds those until
-      // every copy in flight has landed.
-      if ((j + 1) % WIN == 0) turn_k(j / WIN + 1);
-      if (j % WIN == 0) turn_v(j / WIN);
-      copy_k(j + 1);  // (past the last tile: zeros)
-      copy_v(j);
-      if (j % WIN == 0) fetch_ids(j / WIN + 1);  // (lands with the copies)
-      const uint8_t *kt = smem + (grp * 2 + (j & 1)) * BUF;
+      const uint8_t *kt = k_buf(j);
 #pragma unroll
       for (int b = 0; b < NB; ++b)
 #pragma unroll
@@ -205,18 +231,39 @@ __global__ __launch_bounds__(512, 2) void seq_tiles_kernel(SeqAttnArgs a) {
 #pragma unroll
           for (int qb = 0; qb < QB; ++qb) s[b][qb] = mfma16<DT>(kf, qf[qb][c], s[b][qb]);
         }
+      constexpr int NR = NB * NQC, AK = AHEAD_K < NR ? AHEAD_K : NR;
+      __builtin_amdgcn_sched_group_barrier(0x100, AK, 1);
+      static_for<NR - AK>([&](auto) ALWAYS_INLINE {
+        __builtin_amdgcn_sched_group_barrier(0x008, QB, 1);
+        __builtin_amdgcn_sched_group_barrier(0x100, 1, 1);
+      });
+      __builtin_amdgcn_sched_group_barrier(0x008, QB * AK, 1);
     }
   };
   auto softmax_slot = [&](int j) ALWAYS_INLINE {
+    __builtin_amdgcn_s_setprio(0);
     if (j >= nj) return;
-    const int key0 = (kt_begin + 2 * j + grp) * TK;
+    // The copies: between products they hold those up, and this slot is the shorter one.
+    // Past the last tile they are of zeros; page ids land with them.
+    if (KG == 2 || grp == 1) {
+      constexpr int KD = KG == 2 ? 1 : 2;  // (KG = 1: K(j + 1) is what group 0 multiplies meanwhile)
+      if ((j + KD) % WIN == 0) turn_k((j + KD) / WIN);
+      copy_k(j + KD);
+      if (KG == 1 && (j + KD) % WIN == 0) fetch_ids((j + KD) / WIN + 1);
+    }
+    if (KG == 2 || grp == 0) {
+      if (j % WIN == 0) turn_v(j / WIN);
+      copy_v(j);
+      if (j % WIN == 0) fetch_ids(j / WIN + 1);
+    }
+    const int key0 = (kt0 + KG * j) * TK;
     if constexpr (SOFTCAP) {
 #pragma unroll
       for (int b = 0; b < NB; ++b)
 #pragma unroll
         for (int qb = 0; qb < QB; ++qb)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) s[b][qb][e] = a.softcap * tanhf(s[b][qb][e] * a.scale / a.softcap);
+          for (int e = 0; e < 4; ++e) s[b][qb][e] = a.softcap * tanhf(s[b][qb][e] * scale / a.softcap);
     }
     if (a.uniform || key0 < full_lo || key0 + TK - 1 > full_hi) {
 #pragma unroll
@@ -227,21 +274,20 @@ __global__ __launch_bounds__(512, 2) void seq_tiles_kernel(SeqAttnArgs a) {
           for (int e = 0; e < 4; ++e) {
             const int key = key0 + 16 * b + 4 * lg + e;
             const float v = a.uniform ? 0.f : s[b][qb][e];
-            // (hidden below: the sign of C decides which infinity becomes 0)
-            s[b][qb][e] = key < klo[qb] || key > khi[qb] ? (C < 0.f ? INFINITY : -INFINITY) : v;
+            s[b][qb][e] = key < klo[qb] || key > khi[qb] ? -INFINITY : v;
           }
     }
     float mt[QB];
     bool up = false;
 #pragma unroll
     for (int qb = 0; qb < QB; ++qb) {
-      float m = s[0][qb][0] * C;
+      float m = s[0][qb][0];
 #pragma unroll
       for (int b = 0; b < NB; ++b)
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-          if (b | e) m = fmaxf(m, s[b][qb][e] * C);
-      mt[qb] = max4groups(m);
+          if (b | e) m = __builtin_elementwise_maximum(m, s[b][qb][e]);  // (v_maximum3; fmaxf canonicalizes first)
+      mt[qb] = max4groups(m) * C;
       up |= mt[qb] > m_run[qb] + RESCALE;
     }
     if (__builtin_amdgcn_ballot_w64(up) != 0) {
@@ -258,7 +304,6 @@ __global__ __launch_bounds__(512, 2) void seq_tiles_kernel(SeqAttnArgs a) {
 #pragma unroll
     for (int qb = 0; qb < QB; ++qb) {
       const float nm = m_run[qb] == -INFINITY ? 0.f : P_BIAS - m_run[qb];
-      float lsum = 0.f;
 #pragma unroll
       for (int c2 = 0; c2 < NC2; ++c2)
 #pragma unroll
@@ -266,18 +311,28 @@ __global__ __launch_bounds__(512, 2) void seq_tiles_kernel(SeqAttnArgs a) {
           const int b = 2 * c2 + (i >> 1), e = 2 * (i & 1);
           const float e0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][qb][e], C, nm));
           const float e1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][qb][e + 1], C, nm));
-          lsum += e0 + e1;
           p[c2][qb][i] = pack2<DT>(e0, e1);
         }
-      l_run[qb] += lsum;
     }
+    // P is made here: left alone, the compiler moves the exponentials to their use, into
+    // the slot of products.
+#pragma unroll
+    for (int c2 = 0; c2 < NC2; ++c2)
+#pragma unroll
+      for (int qb = 0; qb < QB; ++qb) asm volatile("" : "+v"(p[c2][qb]));
     __builtin_amdgcn_sched_barrier(0);
-    WAIT_VMCNT(0);  // K(j+1) and V(j) land before the next slot of products
+    WAIT_VMCNT(0);
   };
 
   fetch_ids(0);
-  turn_k(0);
-  copy_k(0);
+  if (KG == 2 || grp == 1) {
+    turn_k(0);
+    copy_k(0);
+    if constexpr (KG == 1) {
+      copy_k(1);
+      fetch_ids(1);
+    }
+  }
   WAIT_VMCNT(0);
   BARRIER();
   // One loop per group, so that only S (group 1) or only P (group 0) lives across
@@ -302,38 +357,44 @@ __global__ __launch_bounds__(512, 2) void seq_tiles_kernel(SeqAttnArgs a) {
   }
   WAIT_VMCNT(0);
 
-  // ---- the groups' states meet in LDS: group 1 writes, group 0 merges
-  BARRIER();  // the K and V buffers are free
-  float *const xch = (float *)(smem + wq * Gm::XCH) + lane;
-  float lt[QB], m_all[QB], l_all[QB];
+  // ---- KG = 2: the groups' states meet in LDS: group 1 writes, group 0 merges
+  float m_all[QB], l_all[QB];
 #pragma unroll
-  for (int qb = 0; qb < QB; ++qb) lt[qb] = sum4groups(l_run[qb]);
-  if (grp == 1) {
-#pragma unroll
-    for (int qb = 0; qb < QB; ++qb) {
-      xch[(2 * qb) * 64] = m_run[qb];
-      xch[(2 * qb + 1) * 64] = lt[qb];
-#pragma unroll
-      for (int db = 0; db < NDB; ++db)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) xch[(2 * QB + (db * QB + qb) * 4 + e) * 64] = o[db][qb][e];
-    }
-    WAIT_LGKMCNT0();
+  for (int qb = 0; qb < QB; ++qb) {
+    m_all[qb] = m_run[qb];
+    l_all[qb] = l_run[qb][0];
   }
-  BARRIER();
-  if (grp == 0) {
+  const bool mine = KG == 1 || grp == 0;  // whether this wave has the rows' state now
+  if constexpr (KG == 2) {
+    BARRIER();  // the K and V buffers are free
+    float *const xch = (float *)(smem + wq * Gm::XCH) + lane;
+    if (grp == 1) {
 #pragma unroll
-    for (int qb = 0; qb < QB; ++qb) {
-      const float m1 = xch[(2 * qb) * 64], l1 = xch[(2 * qb + 1) * 64];
-      m_all[qb] = fmaxf(m_run[qb], m1);
-      const float mu = m_all[qb] == -INFINITY ? 0.f : m_all[qb];
-      const float a0 = __builtin_amdgcn_exp2f(m_run[qb] - mu), a1 = __builtin_amdgcn_exp2f(m1 - mu);
-      l_all[qb] = lt[qb] * a0 + l1 * a1;
+      for (int qb = 0; qb < QB; ++qb) {
+        xch[(2 * qb) * 64] = m_all[qb];
+        xch[(2 * qb + 1) * 64] = l_all[qb];
 #pragma unroll
-      for (int db = 0; db < NDB; ++db)
+        for (int db = 0; db < NDB; ++db)
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          o[db][qb][e] = o[db][qb][e] * a0 + xch[(2 * QB + (db * QB + qb) * 4 + e) * 64] * a1;
+          for (int e = 0; e < 4; ++e) xch[(2 * QB + (db * QB + qb) * 4 + e) * 64] = o[db][qb][e];
+      }
+      WAIT_LGKMCNT0();
+    }
+    BARRIER();
+    if (grp == 0) {
+#pragma unroll
+      for (int qb = 0; qb < QB; ++qb) {
+        const float m1 = xch[(2 * qb) * 64], l1 = xch[(2 * qb + 1) * 64];
+        m_all[qb] = fmaxf(m_run[qb], m1);
+        const float mu = m_all[qb] == -INFINITY ? 0.f : m_all[qb];
+        const float a0 = __builtin_amdgcn_exp2f(m_run[qb] - mu), a1 = __builtin_amdgcn_exp2f(m1 - mu);
+        l_all[qb] = l_all[qb] * a0 + l1 * a1;
+#pragma unroll
+        for (int db = 0; db < NDB; ++db)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            o[db][qb][e] = o[db][qb][e] * a0 + xch[(2 * QB + (db * QB + qb) * 4 + e) * 64] * a1;
+      }
     }
   }
   auto store_o = [&](const floatx4 ov, int db, int qb, float inv) ALWAYS_INLINE {
@@ -343,7 +404,7 @@ __global__ __launch_bounds__(512, 2) void seq_tiles_kernel(SeqAttnArgs a) {
   };
   const int S = it.n_parts;
   if (S == 1) {
-    if (grp == 0) {
+    if (mine) {
 #pragma unroll
       for (int qb = 0; qb < QB; ++qb) {
         const float inv = 1.0f / l_all[qb];
@@ -354,24 +415,24 @@ __global__ __launch_bounds__(512, 2) void seq_tiles_kernel(SeqAttnArgs a) {
     return;
   }
   // ---- one of several parts: the state to its slot, with device-coherent (sc1)
-  // accesses; slot: [wave wq][piece][lane] 16 bytes, piece 0 the (m, l) pairs, piece
+  // accesses; slot: [wave][piece][lane] 16 bytes, piece 0 the (m, l) pairs, piece
   // 1 + db·QB + qb the Oᵀ block.
   constexpr int SC1 = 16;
   constexpr int NJ = Gm::NJ;
   const uint32_t slot_step = (uint32_t)KV * Gm::SLOT_BYTES;
   const rsrc_t rp = make_rsrc((const uint8_t *)a.part + ((int64_t)it.part0 * KV + kvh) * Gm::SLOT_BYTES,
                               (int64_t)(S - 1) * slot_step + Gm::SLOT_BYTES);
-  const uint32_t lane_at = (uint32_t)((wq * NJ * 64 + lane) * 16);
-  if (grp == 0) {
-    const uint32_t mine = lane_at + (uint32_t)it.sp * slot_step;
+  const uint32_t lane_at = (uint32_t)((wr * NJ * 64 + lane) * 16);
+  if (mine) {
+    const uint32_t to = lane_at + (uint32_t)it.sp * slot_step;
     const floatx4 ml = {m_all[0], l_all[0], m_all[QB - 1], l_all[QB - 1]};
-    __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(uintx4, ml), rp, mine, 0, SC1);
+    __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(uintx4, ml), rp, to, 0, SC1);
 #pragma unroll
     for (int db = 0; db < NDB; ++db)
 #pragma unroll
       for (int qb = 0; qb < QB; ++qb)
         __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(uintx4, o[db][qb]), rp,
-                                               mine + (uint32_t)((1 + db * QB + qb) * 1024), 0, SC1);
+                                               to + (uint32_t)((1 + db * QB + qb) * 1024), 0, SC1);
     WAIT_VMCNT(0);  // stored before the arrival count
   }
   BARRIER();  // (the exchange area is free)
@@ -385,8 +446,9 @@ __global__ __launch_bounds__(512, 2) void seq_tiles_kernel(SeqAttnArgs a) {
   }
   BARRIER();
   if (!*flag) return;
-  // The parts in key order; the groups share the d blocks.
-  constexpr int HB = (NDB + 1) / 2;
+  // The parts in key order; with KG = 2 the groups share the d blocks.
+  constexpr int HB = (NDB + KG - 1) / KG;
+  const int db0 = KG == 2 ? grp * HB : 0;
   float m[QB], l[QB];
   floatx4 acc[HB][QB];
 #pragma unroll
@@ -404,7 +466,7 @@ __global__ __launch_bounds__(512, 2) void seq_tiles_kernel(SeqAttnArgs a) {
     for (int i = 0; i < HB; ++i)
 #pragma unroll
       for (int qb = 0; qb < QB; ++qb) {
-        const int db = grp * HB + i;
+        const int db = db0 + i;
         x[i][qb] = __builtin_bit_cast(floatx4, __builtin_amdgcn_raw_buffer_load_b128(
                                                    rp, db < NDB ? at + (uint32_t)((1 + db * QB + qb) * 1024) : OOB_OFFSET, 0, SC1));
       }
@@ -424,16 +486,16 @@ __global__ __launch_bounds__(512, 2) void seq_tiles_kernel(SeqAttnArgs a) {
     const float inv = 1.0f / l[qb];
 #pragma unroll
     for (int i = 0; i < HB; ++i)
-      if (grp * HB + i < NDB) store_o(acc[i][qb], grp * HB + i, qb, inv);
+      if (db0 + i < NDB) store_o(acc[i][qb], db0 + i, qb, inv);
   }
 }
 
 namespace {
-template <int DT, int D, bool PAGED, bool SOFTCAP>
-hipError_t launch_seq_tiles(const SeqAttnArgs &a, int n_items, hipStream_t st) {
-  using Gm = SeqTilesGeom<D>;
-  static_assert(Gm::ROWS == seq_tile_rows(D) && SEQ_KEY_TILE % Gm::TK == 0, "the plan's tiles");
-  auto kern = seq_tiles_kernel<DT, D, PAGED, SOFTCAP>;
+template <int DT, int D, int KG, bool PAGED, bool SOFTCAP>
+hipError_t launch_seq_tiles_kg(const SeqAttnArgs &a, int n_items, hipStream_t st) {
+  using Gm = SeqTilesGeom<D, KG>;
+  static_assert(Gm::ROWS == seq_tile_rows(D, KG == 1) && SEQ_KEY_TILE % Gm::TK == 0, "the plan's tiles");
+  auto kern = seq_tiles_kernel<DT, D, KG, PAGED, SOFTCAP>;
   static bool attr_set = false;
   if (!attr_set) {
     hipError_t e = hipFuncSetAttribute((const void *)kern, hipFuncAttributeMaxDynamicSharedMemorySize, Gm::SMEM);
@@ -443,19 +505,24 @@ hipError_t launch_seq_tiles(const SeqAttnArgs &a, int n_items, hipStream_t st) {
   hipLaunchKernelGGL(kern, dim3((unsigned)(n_items * a.n_kv_heads)), dim3(512), Gm::SMEM, st, a);
   return hipGetLastError();
 }
+template <int DT, int D, bool PAGED, bool SOFTCAP>
+hipError_t launch_seq_tiles(const SeqAttnArgs &a, int n_items, bool wide, hipStream_t st) {
+  return wide ? launch_seq_tiles_kg<DT, D, 1, PAGED, SOFTCAP>(a, n_items, st)
+              : launch_seq_tiles_kg<DT, D, 2, PAGED, SOFTCAP>(a, n_items, st);
+}
 
 template <int DT, bool PAGED, bool SOFTCAP>
-hipError_t launch_seq_tiles_d(const SeqAttnArgs &a, int n_items, hipStream_t st) {
+hipError_t launch_seq_tiles_d(const SeqAttnArgs &a, int n_items, bool wide, hipStream_t st) {
   switch (a.head_dim) {
-    case 32: return launch_seq_tiles<DT, 32, PAGED, SOFTCAP>(a, n_items, st);
-    case 48: return launch_seq_tiles<DT, 48, PAGED, SOFTCAP>(a, n_items, st);
-    case 64: return launch_seq_tiles<DT, 64, PAGED, SOFTCAP>(a, n_items, st);
-    case 72: return launch_seq_tiles<DT, 72, PAGED, SOFTCAP>(a, n_items, st);
-    case 80: return launch_seq_tiles<DT, 80, PAGED, SOFTCAP>(a, n_items, st);
-    case 96: return launch_seq_tiles<DT, 96, PAGED, SOFTCAP>(a, n_items, st);
-    case 112: return launch_seq_tiles<DT, 112, PAGED, SOFTCAP>(a, n_items, st);
-    case 128: return launch_seq_tiles<DT, 128, PAGED, SOFTCAP>(a, n_items, st);
-    case 256: return launch_seq_tiles<DT, 256, PAGED, SOFTCAP>(a, n_items, st);
+    case 32: return launch_seq_tiles<DT, 32, PAGED, SOFTCAP>(a, n_items, wide, st);
+    case 48: return launch_seq_tiles<DT, 48, PAGED, SOFTCAP>(a, n_items, wide, st);
+    case 64: return launch_seq_tiles<DT, 64, PAGED, SOFTCAP>(a, n_items, wide, st);
+    case 72: return launch_seq_tiles<DT, 72, PAGED, SOFTCAP>(a, n_items, wide, st);
+    case 80: return launch_seq_tiles<DT, 80, PAGED, SOFTCAP>(a, n_items, wide, st);
+    case 96: return launch_seq_tiles<DT, 96, PAGED, SOFTCAP>(a, n_items, wide, st);
+    case 112: return launch_seq_tiles<DT, 112, PAGED, SOFTCAP>(a, n_items, wide, st);
+    case 128: return launch_seq_tiles<DT, 128, PAGED, SOFTCAP>(a, n_items, wide, st);
+    case 256: return launch_seq_tiles<DT, 256, PAGED, SOFTCAP>(a, n_items, wide, st);
   }
   return hipErrorInvalidValue;
 }
