@@ -114,11 +114,10 @@ struct SeqPlan {
   // What block and workspace hold, or have room for. Offsets are in bytes.
   struct Room {
     size_t rows = 0, tiles = 0, toks = 0, table = 0;  // entries of the lists
-    size_t row_parts = 0, tile_bytes = 0;             // partial states per kv head (of tiles: in bytes)
-    size_t tile_cnt = 0;                              // and tiles' arrival counts per kv head
+    size_t row_parts = 0, tile_parts = 0;             // partial states per kv head
     bool holds(const Room &o) const {
       return o.rows <= rows && o.tiles <= tiles && o.toks <= toks && o.table <= table && o.row_parts <= row_parts &&
-             o.tile_bytes <= tile_bytes && o.tile_cnt <= tile_cnt;
+             o.tile_parts <= tile_parts;
     }
   };
   SeqGeom geom;
@@ -2495,15 +2494,14 @@ int is_capturing(hipStream_t st, bool *yes, const char *op) {
   return RK_OK;
 }
 
-SeqPlan::Room seq_room(const SeqGeom &g, const SeqLists &l) {
+SeqPlan::Room seq_room(const SeqLists &l) {
   SeqPlan::Room r;
   r.rows = l.rows.items.size();
   r.tiles = l.tiles.items.size();
   r.toks = l.toks.size();
   r.table = l.table.size();
   r.row_parts = (size_t)l.rows.n_parts;
-  r.tile_cnt = (size_t)l.tiles.n_parts;
-  r.tile_bytes = r.tile_cnt * rk_seq_slot_bytes(g.head_dim, l.wide ? SEQ_WIDE : SEQ_TILES);
+  r.tile_parts = (size_t)l.tiles.n_parts;
   return r;
 }
 
@@ -2537,19 +2535,18 @@ int seq_reserve(SeqPlan &p, const SeqPlan::Room &want, const char *op) {
   SeqPlan::Room &r = p.room;
   r = SeqPlan::Room{std::max(r.rows, want.rows),   std::max(r.tiles, want.tiles),
                     std::max(r.toks, want.toks),   std::max(r.table, want.table),
-                    std::max(r.row_parts, want.row_parts), std::max(r.tile_bytes, want.tile_bytes),
-                    std::max(r.tile_cnt, want.tile_cnt)};
+                    std::max(r.row_parts, want.row_parts), std::max(r.tile_parts, want.tile_parts)};
   p.off_tiles = align16(r.rows * sizeof(SeqItem));
   p.off_toks = p.off_tiles + align16(r.tiles * sizeof(SeqItem));
   p.off_table = p.off_toks + align16(r.toks * sizeof(SeqTok));
   p.block.bytes = std::max<size_t>(p.off_table + align16(r.table * 4), 256);
   HIP_TRY(hipMalloc(&p.block.p, p.block.bytes), op);
-  if (r.row_parts + r.tile_cnt == 0) return RK_OK;
+  if (r.row_parts + r.tile_parts == 0) return RK_OK;
   const size_t kv = (size_t)p.geom.n_kv_heads;
   p.off_tile_cnt = r.row_parts * kv * 4;
-  p.off_rows = (p.off_tile_cnt + r.tile_cnt * kv * 4 + 255) / 256 * 256;
+  p.off_rows = (p.off_tile_cnt + r.tile_parts * kv * 4 + 255) / 256 * 256;
   p.off_tile_part = p.off_rows + r.row_parts * kv * rk_seq_slot_bytes(p.geom.head_dim, SEQ_ROWS);
-  p.work.bytes = p.off_tile_part + r.tile_bytes * kv;
+  p.work.bytes = p.off_tile_part + r.tile_parts * kv * rk_seq_slot_bytes(p.geom.head_dim, SEQ_TILES);
   HIP_TRY(hipMalloc(&p.work.p, p.work.bytes), op);
   HIP_TRY(hipMemset(p.work.p, 0, p.off_rows), op);
   HIP_TRY(hipDeviceSynchronize(), op);
@@ -2582,8 +2579,8 @@ int seq_plan_create(SeqGeom g, const SeqBatch &b, void **plan, const char *op) {
   const int rc = no_throw(op, [&]() -> int {
     p->geom = g;
     p->n_seqs = b.n_seqs;
-    seq_build(g, b, g_eng->num_cus, true, &p->lists);
-    RK_TRY(seq_reserve(*p, seq_room(p->geom, p->lists), op));
+    seq_build(g, b, g_eng->num_cus, &p->lists);
+    RK_TRY(seq_reserve(*p, seq_room(p->lists), op));
     std::vector<uint8_t> image(p->block.bytes);
     seq_image(*p, image.data());
     HIP_TRY(hipMemcpy(p->block.p, image.data(), image.size(), hipMemcpyHostToDevice), op);
@@ -2622,9 +2619,9 @@ int seq_plan_update(void *plan, bool paged, const SeqBatch &b, rk_stream stream,
   RK_TRY(is_capturing(st, &capturing, op));
   if (capturing) return fail(RK_E_UNSUPPORTED, op, "a plan is not updated inside a capture: its lists come from the host");
   SeqLists l;
-  seq_build(p->geom, b, g_eng->num_cus, p->reserved_q == 0, &l);
+  seq_build(p->geom, b, g_eng->num_cus, &l);
   if (p->captured) {
-    if (!p->room.holds(seq_room(p->geom, l)) || l.max_q > p->reserved_q)
+    if (!p->room.holds(seq_room(l)) || l.max_q > p->reserved_q)
       return fail(RK_E_SHAPE, op, "a graph holds this plan, and the batch needs more than was reserved");
     if (p->captured_pos != INT64_MAX && (l.clash || l.max_pos >= p->captured_pos))
       return fail(RK_E_SHAPE, op, "a graph's append reads this plan: two new tokens in one slot, or past its cos/sin tables");
@@ -2632,7 +2629,7 @@ int seq_plan_update(void *plan, bool paged, const SeqBatch &b, rk_stream stream,
   if (p->pin_ev) HIP_TRY(hipEventSynchronize(p->pin_ev), op);  // the image's last upload has left it
   p->lists = std::move(l);
   p->n_seqs = b.n_seqs;
-  int rc = seq_reserve(*p, seq_room(p->geom, p->lists), op);
+  int rc = seq_reserve(*p, seq_room(p->lists), op);
   if (rc == RK_OK && !p->pin) {
     const hipError_t e = hipHostMalloc((void **)&p->pin, p->block.bytes, hipHostMallocDefault);
     if (e != hipSuccess) rc = hip_fail(e, op);
@@ -2712,7 +2709,7 @@ int seq_attention(const void *plan, bool paged, const void *q, int64_t q_stride,
     a.items = (const SeqItem *)(block + p->off_tiles);
     a.cnt = (unsigned *)(work + p->off_tile_cnt);
     a.part = work + p->off_tile_part;
-    HIP_TRY(rk_launch_attention_seqs(a, (int)n_tiles, p->lists.wide ? SEQ_WIDE : SEQ_TILES, paged, dtype, st), op);
+    HIP_TRY(rk_launch_attention_seqs(a, (int)n_tiles, SEQ_TILES, paged, dtype, st), op);
   }
   if (n_rows) {
     a.items = (const SeqItem *)block;
@@ -2784,14 +2781,11 @@ extern "C" int rk_seq_plan_reserve(void *plan, int64_t max_q_len) {
     if (longest > INT32_MAX / G) return fail(RK_E_SHAPE, op, "max_q_len·(n_head/n_kv_heads) of 2^31 or more");
     SeqBound rows, tiles;
     seq_bound(p->geom, p->n_seqs, p->lists.n_tokens, longest, g_eng->num_cus, &rows, &tiles);
-    // From now on no wide tiles: a captured launch is of one kind of tile.
-    seq_items(p->geom, g_eng->num_cus, false, &p->lists);
-    SeqPlan::Room want = seq_room(p->geom, p->lists);
+    SeqPlan::Room want = seq_room(p->lists);
     want.rows = (size_t)rows.items;
     want.row_parts = (size_t)rows.parts;
     want.tiles = (size_t)tiles.items;
-    want.tile_cnt = (size_t)tiles.parts;
-    want.tile_bytes = want.tile_cnt * rk_seq_slot_bytes(p->geom.head_dim, SEQ_TILES);
+    want.tile_parts = (size_t)tiles.parts;
     RK_TRY(seq_buf_wait(p->block, op));
     RK_TRY(seq_buf_wait(p->work, op));
     RK_TRY(seq_reserve(*p, want, op));

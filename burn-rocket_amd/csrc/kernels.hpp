@@ -230,10 +230,10 @@ hipError_t rk_launch_attention_seqs(const SeqAttnArgs &a, int n_items, SeqKind k
 size_t rk_seq_slot_bytes(int head_dim, SeqKind kind);  // one partial state
 hipError_t rk_launch_seq_rows_f16(const SeqAttnArgs &a, int n_items, bool paged, hipStream_t st);
 hipError_t rk_launch_seq_rows_bf16(const SeqAttnArgs &a, int n_items, bool paged, hipStream_t st);
-hipError_t rk_launch_seq_tiles_f16(const SeqAttnArgs &a, int n_items, bool wide, bool paged, hipStream_t st);
-hipError_t rk_launch_seq_tiles_bf16(const SeqAttnArgs &a, int n_items, bool wide, bool paged, hipStream_t st);
-hipError_t rk_launch_seq_tiles_f16_cap(const SeqAttnArgs &a, int n_items, bool wide, bool paged, hipStream_t st);
-hipError_t rk_launch_seq_tiles_bf16_cap(const SeqAttnArgs &a, int n_items, bool wide, bool paged, hipStream_t st);
+hipError_t rk_launch_seq_tiles_f16(const SeqAttnArgs &a, int n_items, bool paged, hipStream_t st);
+hipError_t rk_launch_seq_tiles_bf16(const SeqAttnArgs &a, int n_items, bool paged, hipStream_t st);
+hipError_t rk_launch_seq_tiles_f16_cap(const SeqAttnArgs &a, int n_items, bool paged, hipStream_t st);
+hipError_t rk_launch_seq_tiles_bf16_cap(const SeqAttnArgs &a, int n_items, bool paged, hipStream_t st);
 
 struct PagedAppendArgs {
   const void *qkv;  // [n_tokens] rows: q heads, k heads, v heads

@@ -1,8 +1,6 @@
 // Host side of the batches of sequences (seq_plan.hpp): checks and schedules.
 #include "seq_plan.hpp"
 
-#include <stdlib.h>
-
 #include <algorithm>
 
 #include "../../include/burn_rocket_amd.h"
@@ -86,19 +84,37 @@ std::string seq_check_batch(const SeqGeom &g, const SeqBatch &b) {
 namespace {
 // Workgroups of a kernel that the GPU holds at once, per kv head (at least one).
 int64_t slots_per_head(const SeqGeom &g, int num_cus, bool few) {
-  // LDS leaves one workgroup per CU, two of the first kernel for heads up to 64.
-  const int64_t slots = (int64_t)std::max(1, num_cus) * (few && g.head_dim <= 64 ? 2 : 1);
+  // Registers and LDS leave two workgroups per CU, one of the first kernel for heads above 64.
+  const int64_t slots = (int64_t)std::max(1, num_cus) * (few && g.head_dim > 64 ? 1 : 2);
   return std::max<int64_t>(1, slots / g.n_kv_heads);
 }
 
-// Splits the keys of the longest tiles so that no item is longer than an even share
-// of the work (and none shorter than `least` steps), then sorts longest first: the
-// short ones fill the last round.
-void split(std::vector<SeqItem> &tiles, int step, int64_t slots, int64_t least, SeqList *out) {
+// Splits the keys of the longest tiles where that shortens the launch, then sorts
+// longest first: the short ones fill the last round. Fewer tiles than the GPU holds at
+// once: items of equal length, as many as it holds (one more than that is another
+// round: 512 query rows against 16901 keys, 128 tiles, took 152 us in 512 items and
+// 206 in 516 on MI355X). More: only tiles longer than 5/4 of an even share. None where
+// the longest would shrink by less than `cost` steps, which is what states to
+// store and merge take (about 20 us for tiles of 128 rows).
+void split(std::vector<SeqItem> &tiles, int step, int64_t slots, int64_t cost, SeqList *out) {
   const auto steps = [&](const SeqItem &t) { return ceil_div(t.k_end - t.k_begin, step); };
-  int64_t total = 0;
-  for (const SeqItem &t : tiles) total += steps(t);
-  const int64_t quota = std::max(least, ceil_div(total, slots));
+  int64_t total = 0, longest = 0;
+  for (const SeqItem &t : tiles) {
+    total += steps(t);
+    longest = std::max(longest, steps(t));
+  }
+  int64_t quota = std::max<int64_t>(1, ceil_div(total, slots));
+  if ((int64_t)tiles.size() < slots) {
+    const auto items = [&](int64_t q) {
+      int64_t n = 0;
+      for (const SeqItem &t : tiles) n += std::min<int64_t>(ceil_div(steps(t), q), SEQ_MAX_PARTS);
+      return n;
+    };
+    while (items(quota) > slots) quota += 1 + quota / 64;
+  } else {
+    quota = ceil_div(5 * total, 4 * slots);
+  }
+  if (longest - quota < cost) quota = std::max<int64_t>(longest, 1);
   for (SeqItem &t : tiles) {
     const int64_t n = steps(t), parts = std::min<int64_t>(ceil_div(n, quota), SEQ_MAX_PARTS);
     t.n_parts = (int32_t)parts;
@@ -115,14 +131,15 @@ void split(std::vector<SeqItem> &tiles, int step, int64_t slots, int64_t least, 
   std::stable_sort(out->items.begin(), out->items.end(),
                    [&](const SeqItem &x, const SeqItem &y) { return steps(x) > steps(y); });
 }
-constexpr int64_t ROWS_LEAST = 8, TILES_LEAST = 4;  // steps of an item that its own cost allows
+constexpr int64_t ROWS_COST = 8, TILES_COST = 12;  // steps that a split costs
 }  // namespace
 
 void seq_bound(const SeqGeom &g, int64_t n_seqs, int64_t n_tokens, int64_t max_q, int num_cus, SeqBound *rows,
                SeqBound *tiles) {
-  // Splits add at most total / quota <= slots items; a split tile's states are at
+  // A tile of n steps has at most n / quota + 1 items, and quota is at least an even
+  // share of the steps: splits add at most `slots` items. A split tile's states are at
   // most twice what its split added.
-  const int64_t G = g.n_head / g.n_kv_heads, tr = seq_tile_rows(g.head_dim, false);
+  const int64_t G = g.n_head / g.n_kv_heads, tr = seq_tile_rows(g.head_dim);
   const int64_t s0 = slots_per_head(g, num_cus, true), s1 = slots_per_head(g, num_cus, false);
   n_seqs = std::min(n_seqs, n_tokens);  // those with new tokens
   *rows = SeqBound{n_seqs + s0, 2 * s0};
@@ -131,31 +148,25 @@ void seq_bound(const SeqGeom &g, int64_t n_seqs, int64_t n_tokens, int64_t max_q
     *tiles = SeqBound{n_tokens * G / tr + std::min(n_seqs, n_tokens * G / (SEQ_FEW_ROWS + 1)) + s1, 2 * s1};
 }
 
-void seq_items(const SeqGeom &g, int num_cus, bool may_wide, SeqLists *l) {
+void seq_build(const SeqGeom &g, const SeqBatch &b, int num_cus, SeqLists *out) {
+  *out = SeqLists{};
   const int64_t G = g.n_head / g.n_kv_heads;
-  const size_t n = l->q_lens.size();
   std::vector<SeqItem> rows, tiles;
-  l->rows = l->tiles = SeqList{};
-  l->wide = false;
-  if (may_wide) {
-    int64_t t = 0;
-    for (const int64_t q : l->q_lens)
-      if (q * G > SEQ_FEW_ROWS) t += ceil_div(q * G, seq_tile_rows(g.head_dim, true));
-    l->wide = t * g.n_kv_heads >= 2 * num_cus;
-    if (const char *e = getenv("RK_SEQ_WIDE")) l->wide = atoi(e) != 0;
-  }
-  int64_t tok = 0, ids = 0;
-  for (size_t i = 0; i < n; ++i) {
-    const int64_t q = l->q_lens[i], kv = l->kv_lens[i], pos0 = kv - q;
+  struct Piece {
+    int32_t page, off, end;
+  };
+  std::vector<Piece> pieces;  // where new tokens go: slots [off, end) of a page
+  for (int64_t i = 0; i < b.n_seqs; ++i) {
+    const int64_t q = b.q_lens[i], kv = kv_of(b, i), pos0 = kv - q;
     if (q == 0) continue;
     SeqItem it{};
-    it.tok0 = (int32_t)tok;
+    it.tok0 = (int32_t)out->n_tokens;
     it.pos0 = (int32_t)pos0;
     it.rows = (int32_t)(q * G);
     it.kv_len = (int32_t)kv;
-    it.table = (int32_t)ids;
+    it.table = (int32_t)out->table.size();
     const bool few = q * G <= SEQ_FEW_ROWS;
-    const int64_t tr = few ? 16 : seq_tile_rows(g.head_dim, l->wide), step = few ? SEQ_ROWS_CHUNK : SEQ_KEY_TILE;
+    const int64_t tr = few ? 16 : seq_tile_rows(g.head_dim), step = few ? SEQ_ROWS_CHUNK : SEQ_KEY_TILE;
     for (int64_t r = 0; r < q * G; r += tr) {
       int64_t lo, hi, lo2, hi2;
       visible(g, pos0 + r / G, kv, &lo, &hi);
@@ -166,24 +177,6 @@ void seq_items(const SeqGeom &g, int num_cus, bool may_wide, SeqLists *l) {
       it.k_end = (int32_t)(hi2 + 1);
       (few ? rows : tiles).push_back(it);
     }
-    tok += q;
-    if (g.paged) ids += ceil_div(kv, g.page_size);
-  }
-  split(rows, SEQ_ROWS_CHUNK, slots_per_head(g, num_cus, true), ROWS_LEAST, &l->rows);
-  split(tiles, SEQ_KEY_TILE, slots_per_head(g, num_cus, false), TILES_LEAST, &l->tiles);
-}
-
-void seq_build(const SeqGeom &g, const SeqBatch &b, int num_cus, bool may_wide, SeqLists *out) {
-  *out = SeqLists{};
-  struct Piece {
-    int32_t page, off, end;
-  };
-  std::vector<Piece> pieces;  // where new tokens go: slots [off, end) of a page
-  for (int64_t i = 0; i < b.n_seqs; ++i) {
-    const int64_t q = b.q_lens[i], kv = kv_of(b, i), pos0 = kv - q;
-    if (q == 0) continue;
-    out->q_lens.push_back((int32_t)q);
-    out->kv_lens.push_back((int32_t)kv);
     out->n_tokens += q;
     out->max_q = std::max(out->max_q, q);
     out->max_pos = std::max(out->max_pos, kv - 1);
@@ -200,7 +193,8 @@ void seq_build(const SeqGeom &g, const SeqBatch &b, int num_cus, bool may_wide, 
       t = e;
     }
   }
-  seq_items(g, num_cus, may_wide, out);
+  split(rows, SEQ_ROWS_CHUNK, slots_per_head(g, num_cus, true), ROWS_COST, &out->rows);
+  split(tiles, SEQ_KEY_TILE, slots_per_head(g, num_cus, false), TILES_COST, &out->tiles);
   std::sort(pieces.begin(), pieces.end(),
             [](const Piece &x, const Piece &y) { return x.page != y.page ? x.page < y.page : x.off < y.off; });
   for (size_t i = 1; i < pieces.size(); ++i)

@@ -37,12 +37,12 @@ struct SeqTok {
 
 // Kinds of items: tiles of 16 rows with their keys over the waves of a workgroup
 // (seq_rows.hpp) for sequences of at most SEQ_FEW_ROWS query rows; for the others
-// tiles of seq_tile_rows rows (seq_tiles.hpp), all of a batch wide or none.
-enum SeqKind { SEQ_ROWS, SEQ_TILES, SEQ_WIDE };
+// tiles of seq_tile_rows rows (seq_tiles.hpp).
+enum SeqKind { SEQ_ROWS, SEQ_TILES };
 constexpr int SEQ_FEW_ROWS = 16;
 constexpr int SEQ_ROWS_CHUNK = 32;  // keys of a step of the first, ranges start at multiples
 constexpr int SEQ_KEY_TILE = 64;    // and of the second
-constexpr int seq_tile_rows(int head_dim, bool wide) { return (head_dim <= 128 ? 128 : 64) * (wide ? 2 : 1); }
+constexpr int seq_tile_rows(int head_dim) { return head_dim <= 128 ? 128 : 64; }
 constexpr int SEQ_MAX_PARTS = 32;
 constexpr int64_t SEQ_MAX_STRIDE = (int64_t)1 << 26;  // values between packed tokens: 16 of them stay below 2 GiB
 
@@ -71,9 +71,7 @@ struct SeqLists {
   int64_t max_q = 0;      // longest q_len
   int64_t max_pos = -1;   // largest key index of a new token
   bool clash = false;     // two new tokens go to one slot of a page
-  bool wide = false;      // the tiles are SEQ_WIDE
   SeqList rows, tiles;
-  std::vector<int32_t> q_lens, kv_lens;
   std::vector<SeqTok> toks;
   std::vector<int32_t> table;
 };
@@ -83,13 +81,10 @@ struct SeqLists {
 // that the kernels do not have.
 std::string seq_check_geom(SeqGeom &g, bool *unsupported);
 std::string seq_check_batch(const SeqGeom &g, const SeqBatch &b);
-// The lists of a checked batch for a GPU of num_cus CUs. may_wide: whether its tiles may
-// be SEQ_WIDE.
-void seq_build(const SeqGeom &g, const SeqBatch &b, int num_cus, bool may_wide, SeqLists *out);
-// Its items alone, again, from the lengths that the lists keep.
-void seq_items(const SeqGeom &g, int num_cus, bool may_wide, SeqLists *l);
+// The lists of a checked batch for a GPU of num_cus CUs.
+void seq_build(const SeqGeom &g, const SeqBatch &b, int num_cus, SeqLists *out);
 // The most items and partial states that seq_build lists for any batch of at most
-// n_seqs sequences and n_tokens new tokens, none longer than max_q, without SEQ_WIDE.
+// n_seqs sequences and n_tokens new tokens, none longer than max_q.
 struct SeqBound {
   int64_t items = 0, parts = 0;
 };

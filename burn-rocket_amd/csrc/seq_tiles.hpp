@@ -1,15 +1,11 @@
 // Attention of sequences with many query rows (prompts, chunks of prompts) on
 // gfx950: an online softmax over key tiles that K and V reach through LDS.
 //
-// A workgroup's 8 waves are two groups of 4; a wave has 16·QB query rows of one kv
-// head. With KG = 1 all 8 have rows of their own (a tile of 256 rows, 128 for head dim
-// 256) and walk the item's key tiles together; with KG = 2 the groups have the same
-// 128 (64) rows and walk alternate key tiles, and their states meet at the end. KG = 1
-// copies half as much to LDS per product, KG = 2 leaves finer tiles for
-// batches that do not fill the GPU. The work of a group alternates between a slot of
-// matrix products (P·V of one tile, then K·Qᵀ of the next) and a slot of softmax, one
-// group a slot behind the other, so that a SIMD multiplies for one wave while it
-// exponentiates for the other. Barriers separate the slots.
+// A workgroup's 4 waves have 16·QB query rows of one kv head each (a tile of 128, 64 for
+// head dim 256) and walk the item's key tiles of TK keys together: products (P·V of one
+// tile, then K·Qᵀ of the next), then the softmax. Two workgroups share a CU, so that
+// a SIMD multiplies for a wave of one while it exponentiates for one of the other, and
+// so that one's start and end hide behind the other's tiles. One barrier per tile.
 //
 // Per wave and tile (v_mfma_f32_16x16x32):
 //   Sᵀ = K·Qᵀ   K rows from LDS, Q in registers; a lane owns one query of each
@@ -26,12 +22,10 @@
 //
 // LDS: K rows of KPC 16-byte pieces (piece c of row r at c ^ (r & (KPC-1))), V as
 // 16-key blocks (32-byte pairs swizzled by the key where rows are a power of two).
-// KG = 2: two buffers of each per group, a group copies its own. KG = 1: three of K,
-// copied by group 1, and two of V, copied by group 0. Copies go to LDS directly, one
-// 16-key block per buffer descriptor: a block lies in one page, and rows past the
-// sequence's keys read as zeros. They start with a slot of softmax and have landed at
-// its end; started three slots ahead (four and three buffers) they cost the same, so it is not their
-// latency that counts but what they take from the LDS reads.
+// Two buffers of each. Copies go to LDS directly, one 16-key block per buffer
+// descriptor: a block lies in one page, and rows past the sequence's keys read as
+// zeros. They start with the softmax, which their latency hides behind; issued between
+// products they held those up.
 //
 // Items that are one of n_parts of their tile leave their state in the plan's
 // workspace; the last to arrive merges the parts in key order.
@@ -44,12 +38,11 @@ namespace {
 constexpr int AHEAD_V = 3, AHEAD_K = 4;
 constexpr float RESCALE = 8.0f;  // with P_BIAS: probabilities stay below 2^14
 
-template <int D, int KG>
+template <int D>
 struct SeqTilesGeom {
   static constexpr int QB = D <= 128 ? 2 : 1;       // 16-query blocks per wave
   static constexpr int TK = D <= 128 ? 64 : 32;     // keys per tile
-  static constexpr int NW = 8 / KG;                 // waves with rows of their own
-  static constexpr int ROWS = NW * 16 * QB;         // query rows per workgroup
+  static constexpr int ROWS = 64 * QB;              // query rows per workgroup
   static constexpr int NQC = (D + 31) / 32;         // 32-wide d chunks of QKᵀ
   static constexpr int NDB = (D + 15) / 16;         // 16-row d blocks of Oᵀ
   static constexpr int CH = D / 8;                  // 16-byte pieces of a row
@@ -64,21 +57,19 @@ struct SeqTilesGeom {
   static constexpr bool POW2 = (D & (D - 1)) == 0;
   static constexpr int VSW = POW2 ? (CH / 2 < 8 ? CH / 2 : 8) - 1 : 0;
   static constexpr int K_BYTES = TK * KROW, V_BYTES = NB * VB;
-  static constexpr int V_AT = (KG == 2 ? 4 : 3) * K_BYTES;  // the V buffers, behind those of K
-  static constexpr int BUFS = V_AT + (KG == 2 ? 4 : 2) * V_BYTES;
+  static constexpr int V_AT = 2 * K_BYTES;          // the V buffers, behind those of K
+  static constexpr int SMEM = V_AT + 2 * V_BYTES;
   static constexpr int CK = KI * NB / 4, CV = VI * NB / 4;  // copies per wave and tile
   static_assert(KI * NB % 4 == 0 && VI * NB % 4 == 0, "every wave copies alike");
-  static constexpr int XCH = (2 * QB + NDB * QB * 4) * 256;  // a wave's state in the exchange of the groups (KG = 2)
-  static constexpr int SMEM = BUFS > 4 * XCH || KG == 1 ? BUFS : 4 * XCH;
   static constexpr int NJ = 1 + NDB * QB;           // 1 KB pieces of a wave's state in the workspace
-  static constexpr int SLOT_BYTES = NW * NJ * 1024;
-  static_assert(SMEM <= 160 * 1024, "LDS");
+  static constexpr int SLOT_BYTES = 4 * NJ * 1024;
+  static_assert(2 * SMEM <= 160 * 1024, "two workgroups per CU");
 };
 }  // namespace
 
-template <int DT, int D, int KG, bool PAGED, bool SOFTCAP>
-__global__ __launch_bounds__(512, 2) void seq_tiles_kernel(SeqAttnArgs a) {
-  using Gm = SeqTilesGeom<D, KG>;
+template <int DT, int D, bool PAGED, bool SOFTCAP>
+__global__ __launch_bounds__(256, 2) void seq_tiles_kernel(SeqAttnArgs a) {
+  using Gm = SeqTilesGeom<D>;
   constexpr int QB = Gm::QB, TK = Gm::TK, NQC = Gm::NQC, NDB = Gm::NDB, NB = Gm::NB, NC2 = Gm::NC2;
   constexpr int KI = Gm::KI, VI = Gm::VI, CH = Gm::CH, KPC = Gm::KPC, KROW = Gm::KROW;
   extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
@@ -89,9 +80,7 @@ __global__ __launch_bounds__(512, 2) void seq_tiles_kernel(SeqAttnArgs a) {
   if (it.rows == 0) return;
   const int lane = lane_id();
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int grp = wave >> 2, wq = wave & 3;
   const int l16 = lane & 15, lg = lane >> 4;
-  const int wr = KG == 1 ? wave : wq;  // which of the waves with rows
 
   // ---- this lane's rows and what they see. A negative scale is a sign of Q.
   const uint32_t flip = a.scale < 0.f ? 0x80008000u : 0u;
@@ -102,7 +91,7 @@ __global__ __launch_bounds__(512, 2) void seq_tiles_kernel(SeqAttnArgs a) {
   f16 *orow[QB];
 #pragma unroll
   for (int qb = 0; qb < QB; ++qb) {
-    const int r = it.row0 + wr * 16 * QB + qb * 16 + l16;
+    const int r = it.row0 + wave * 16 * QB + qb * 16 + l16;
     rok[qb] = r < it.rows;
     const int q = rok[qb] ? r / G : 0, h = kvh * G + (rok[qb] ? r % G : 0);
     seq_visible(a, it.pos0 + q, it.kv_len, klo[qb], khi[qb]);
@@ -118,7 +107,7 @@ __global__ __launch_bounds__(512, 2) void seq_tiles_kernel(SeqAttnArgs a) {
   // Keys that every row of the wave sees, from its first and last row (the ends of
   // a row's keys never decrease with the row).
   int full_lo, full_hi, skip;
-  const int w_row0 = min(it.row0 + wr * 16 * QB, it.rows - 1);
+  const int w_row0 = min(it.row0 + wave * 16 * QB, it.rows - 1);
   seq_visible(a, it.pos0 + w_row0 / G, it.kv_len, skip, full_hi);
   seq_visible(a, it.pos0 + min(w_row0 + 16 * QB - 1, it.rows - 1) / G, it.kv_len, full_lo, skip);
   // (a scale of 0 must leave hidden scores at -inf)
@@ -126,31 +115,28 @@ __global__ __launch_bounds__(512, 2) void seq_tiles_kernel(SeqAttnArgs a) {
 
   // ---- copies
   const uint32_t ks = (uint32_t)((PAGED ? D : a.k_stride) * 2), vs = (uint32_t)((PAGED ? D : a.v_stride) * 2);
-  const int kt_begin = it.k_begin / TK, n_tiles = (it.k_end + TK - 1) / TK - kt_begin;
-  // The group's tiles, numbered j = 0 .. nj - 1: tile kt_begin + KG·j (+ grp).
-  const int nj = KG == 2 ? (n_tiles - grp + 1) / 2 : n_tiles, nj_max = (n_tiles + KG - 1) / KG;
-  const int kt0 = kt_begin + (KG == 2 ? grp : 0);
-  // Blocks of the group's tiles: lane l holds block l % NB of tile l / NB of a window
+  const int kt_begin = it.k_begin / TK, nj = (it.k_end + TK - 1) / TK - kt_begin;  // tiles kt_begin + j
+  // Blocks of the item's tiles: lane l holds block l % NB of tile l / NB of a window
   // of WIN tiles; kb and vb: of the windows that the next copies of K and V lie in;
   // ids: page ids of the window that comes next (fetched a window ahead).
   constexpr int WIN = 64 / NB;
   KeyBlocks kb, vb;
   int ids = 0;
-  auto key_of = [&](int w) ALWAYS_INLINE { return (kt0 + KG * (w * WIN + lane / NB)) * TK + 16 * (lane % NB); };
+  auto key_of = [&](int w) ALWAYS_INLINE { return (kt_begin + w * WIN + lane / NB) * TK + 16 * (lane % NB); };
   auto fetch_ids = [&](int w) ALWAYS_INLINE {
     if constexpr (PAGED) ids = a.table[it.table + (min(key_of(w), it.kv_len - 1) >> a.page_log2)];
   };
-  const int end = (kt_begin + n_tiles) * TK;
+  const int end = (kt_begin + nj) * TK;
   auto turn_k = [&](int w) ALWAYS_INLINE { kb = key_blocks<PAGED>(a, it, a.k, a.k_stride, kvh, key_of(w), end, ids); };
   auto turn_v = [&](int w) ALWAYS_INLINE { vb = key_blocks<PAGED>(a, it, a.v, a.v_stride, kvh, key_of(w), end, ids); };
-  // Wave wq's share of the copies of the group's tile j: pieces s of its 16-key
+  // The wave's share of the copies of tile j: pieces s of its 16-key
   // blocks b, in the order s + KI·b.
-  auto k_buf = [&](int j) ALWAYS_INLINE { return smem + (KG == 2 ? grp * 2 + (j & 1) : (int)((unsigned)j % 3)) * Gm::K_BYTES; };
-  auto v_buf = [&](int j) ALWAYS_INLINE { return smem + Gm::V_AT + ((KG == 2 ? grp * 2 : 0) + (j & 1)) * Gm::V_BYTES; };
+  auto k_buf = [&](int j) ALWAYS_INLINE { return smem + (j & 1) * Gm::K_BYTES; };
+  auto v_buf = [&](int j) ALWAYS_INLINE { return smem + Gm::V_AT + (j & 1) * Gm::V_BYTES; };
   auto copy_k = [&](int j) ALWAYS_INLINE {
     uint8_t *const to = k_buf(j);
     static_for<Gm::CK>([&](auto i_c) ALWAYS_INLINE {
-      const int c = wq + 4 * decltype(i_c)::value, b = c / KI, s = c % KI;
+      const int c = wave + 4 * decltype(i_c)::value, b = c / KI, s = c % KI;
       const rsrc_t rk = block_rsrc(kb, (j % WIN) * NB + b);
       const int p = 64 * s + lane, row = p / KPC;
       const int ch = (p % KPC) ^ (row & Gm::KSW);  // logical piece of this slot
@@ -160,7 +146,7 @@ __global__ __launch_bounds__(512, 2) void seq_tiles_kernel(SeqAttnArgs a) {
   auto copy_v = [&](int j) ALWAYS_INLINE {
     uint8_t *const to = v_buf(j);
     static_for<Gm::CV>([&](auto i_c) ALWAYS_INLINE {
-      const int c = wq + 4 * decltype(i_c)::value, b = c / VI, s = c % VI;
+      const int c = wave + 4 * decltype(i_c)::value, b = c / VI, s = c % VI;
       const rsrc_t rv = block_rsrc(vb, (j % WIN) * NB + b);
       const int p = 64 * s + lane, row = p / CH, ch = p % CH;
       const int lch = Gm::VSW ? ch ^ ((row & Gm::VSW) << 1) : ch;
@@ -191,7 +177,7 @@ __global__ __launch_bounds__(512, 2) void seq_tiles_kernel(SeqAttnArgs a) {
     for (int db = 0; db < NDB; ++db) o[db][qb] = floatx4{0.f, 0.f, 0.f, 0.f};
   }
 
-  auto mfma_slot = [&](int j) ALWAYS_INLINE {
+  auto products = [&](int j) ALWAYS_INLINE {
     __builtin_amdgcn_s_setprio(1);  // products first: what they leave of the issue slots is enough for a softmax
     if (j >= 1 && j - 1 < nj) {
       const uint8_t *vt = v_buf(j - 1) + v_row;
@@ -240,23 +226,16 @@ __global__ __launch_bounds__(512, 2) void seq_tiles_kernel(SeqAttnArgs a) {
       __builtin_amdgcn_sched_group_barrier(0x008, QB * AK, 1);
     }
   };
-  auto softmax_slot = [&](int j) ALWAYS_INLINE {
+  auto softmax = [&](int j) ALWAYS_INLINE {
     __builtin_amdgcn_s_setprio(0);
-    if (j >= nj) return;
-    // The copies: between products they hold those up, and this slot is the shorter one.
-    // Past the last tile they are of zeros; page ids land with them.
-    if (KG == 2 || grp == 1) {
-      constexpr int KD = KG == 2 ? 1 : 2;  // (KG = 1: K(j + 1) is what group 0 multiplies meanwhile)
-      if ((j + KD) % WIN == 0) turn_k((j + KD) / WIN);
-      copy_k(j + KD);
-      if (KG == 1 && (j + KD) % WIN == 0) fetch_ids((j + KD) / WIN + 1);
-    }
-    if (KG == 2 || grp == 0) {
-      if (j % WIN == 0) turn_v(j / WIN);
-      copy_v(j);
-      if (j % WIN == 0) fetch_ids(j / WIN + 1);
-    }
-    const int key0 = (kt0 + KG * j) * TK;
+    // The copies (past the last tile of zeros; page ids land with them). Their buffers
+    // were last read before the barrier that every wave has passed.
+    if ((j + 1) % WIN == 0) turn_k(j / WIN + 1);
+    if (j % WIN == 0) turn_v(j / WIN);
+    copy_k(j + 1);
+    copy_v(j);
+    if (j % WIN == 0) fetch_ids(j / WIN + 1);
+    const int key0 = (kt_begin + j) * TK;
     if constexpr (SOFTCAP) {
 #pragma unroll
       for (int b = 0; b < NB; ++b)
@@ -315,7 +294,7 @@ __global__ __launch_bounds__(512, 2) void seq_tiles_kernel(SeqAttnArgs a) {
         }
     }
     // P is made here: left alone, the compiler moves the exponentials to their use, into
-    // the slot of products.
+    // the products.
 #pragma unroll
     for (int c2 = 0; c2 < NC2; ++c2)
 #pragma unroll
@@ -325,78 +304,20 @@ __global__ __launch_bounds__(512, 2) void seq_tiles_kernel(SeqAttnArgs a) {
   };
 
   fetch_ids(0);
-  if (KG == 2 || grp == 1) {
-    turn_k(0);
-    copy_k(0);
-    if constexpr (KG == 1) {
-      copy_k(1);
-      fetch_ids(1);
-    }
-  }
+  turn_k(0);
+  copy_k(0);
   WAIT_VMCNT(0);
   BARRIER();
-  // One loop per group, so that only S (group 1) or only P (group 0) lives across
-  // an iteration; both make 2·nj_max + 2 barriers.
-  if (grp == 0) {
-    for (int j = 0; j <= nj_max; ++j) {
-      mfma_slot(j);
-      BARRIER();
-      softmax_slot(j);
-      BARRIER();
-    }
-  } else {
+  for (int j = 0; j < nj; ++j) {
+    products(j);
+    softmax(j);
     BARRIER();
-    mfma_slot(0);
-    BARRIER();
-    for (int j = 0; j < nj_max; ++j) {
-      softmax_slot(j);
-      BARRIER();
-      mfma_slot(j + 1);
-      BARRIER();
-    }
   }
+  products(nj);
   WAIT_VMCNT(0);
-
-  // ---- KG = 2: the groups' states meet in LDS: group 1 writes, group 0 merges
-  float m_all[QB], l_all[QB];
+  float l_all[QB];
 #pragma unroll
-  for (int qb = 0; qb < QB; ++qb) {
-    m_all[qb] = m_run[qb];
-    l_all[qb] = l_run[qb][0];
-  }
-  const bool mine = KG == 1 || grp == 0;  // whether this wave has the rows' state now
-  if constexpr (KG == 2) {
-    BARRIER();  // the K and V buffers are free
-    float *const xch = (float *)(smem + wq * Gm::XCH) + lane;
-    if (grp == 1) {
-#pragma unroll
-      for (int qb = 0; qb < QB; ++qb) {
-        xch[(2 * qb) * 64] = m_all[qb];
-        xch[(2 * qb + 1) * 64] = l_all[qb];
-#pragma unroll
-        for (int db = 0; db < NDB; ++db)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) xch[(2 * QB + (db * QB + qb) * 4 + e) * 64] = o[db][qb][e];
-      }
-      WAIT_LGKMCNT0();
-    }
-    BARRIER();
-    if (grp == 0) {
-#pragma unroll
-      for (int qb = 0; qb < QB; ++qb) {
-        const float m1 = xch[(2 * qb) * 64], l1 = xch[(2 * qb + 1) * 64];
-        m_all[qb] = fmaxf(m_run[qb], m1);
-        const float mu = m_all[qb] == -INFINITY ? 0.f : m_all[qb];
-        const float a0 = __builtin_amdgcn_exp2f(m_run[qb] - mu), a1 = __builtin_amdgcn_exp2f(m1 - mu);
-        l_all[qb] = l_all[qb] * a0 + l1 * a1;
-#pragma unroll
-        for (int db = 0; db < NDB; ++db)
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            o[db][qb][e] = o[db][qb][e] * a0 + xch[(2 * QB + (db * QB + qb) * 4 + e) * 64] * a1;
-      }
-    }
-  }
+  for (int qb = 0; qb < QB; ++qb) l_all[qb] = l_run[qb][0];
   auto store_o = [&](const floatx4 ov, int db, int qb, float inv) ALWAYS_INLINE {
     const int d0 = db * 16 + 4 * lg;
     if (rok[qb] && d0 < D)
@@ -404,13 +325,11 @@ __global__ __launch_bounds__(512, 2) void seq_tiles_kernel(SeqAttnArgs a) {
   };
   const int S = it.n_parts;
   if (S == 1) {
-    if (mine) {
 #pragma unroll
-      for (int qb = 0; qb < QB; ++qb) {
-        const float inv = 1.0f / l_all[qb];
+    for (int qb = 0; qb < QB; ++qb) {
+      const float inv = 1.0f / l_all[qb];
 #pragma unroll
-        for (int db = 0; db < NDB; ++db) store_o(o[db][qb], db, qb, inv);
-      }
+      for (int db = 0; db < NDB; ++db) store_o(o[db][qb], db, qb, inv);
     }
     return;
   }
@@ -422,20 +341,18 @@ __global__ __launch_bounds__(512, 2) void seq_tiles_kernel(SeqAttnArgs a) {
   const uint32_t slot_step = (uint32_t)KV * Gm::SLOT_BYTES;
   const rsrc_t rp = make_rsrc((const uint8_t *)a.part + ((int64_t)it.part0 * KV + kvh) * Gm::SLOT_BYTES,
                               (int64_t)(S - 1) * slot_step + Gm::SLOT_BYTES);
-  const uint32_t lane_at = (uint32_t)((wr * NJ * 64 + lane) * 16);
-  if (mine) {
-    const uint32_t to = lane_at + (uint32_t)it.sp * slot_step;
-    const floatx4 ml = {m_all[0], l_all[0], m_all[QB - 1], l_all[QB - 1]};
-    __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(uintx4, ml), rp, to, 0, SC1);
+  const uint32_t lane_at = (uint32_t)((wave * NJ * 64 + lane) * 16);
+  const uint32_t to = lane_at + (uint32_t)it.sp * slot_step;
+  const floatx4 ml_all = {m_run[0], l_all[0], m_run[QB - 1], l_all[QB - 1]};
+  __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(uintx4, ml_all), rp, to, 0, SC1);
 #pragma unroll
-    for (int db = 0; db < NDB; ++db)
+  for (int db = 0; db < NDB; ++db)
 #pragma unroll
-      for (int qb = 0; qb < QB; ++qb)
-        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(uintx4, o[db][qb]), rp,
-                                               to + (uint32_t)((1 + db * QB + qb) * 1024), 0, SC1);
-    WAIT_VMCNT(0);  // stored before the arrival count
-  }
-  BARRIER();  // (the exchange area is free)
+    for (int qb = 0; qb < QB; ++qb)
+      __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(uintx4, o[db][qb]), rp,
+                                             to + (uint32_t)((1 + db * QB + qb) * 1024), 0, SC1);
+  WAIT_VMCNT(0);  // stored before the arrival count
+  BARRIER();  // (the K and V buffers are free)
   unsigned *flag = (unsigned *)smem;
   if (threadIdx.x == 0) {
     unsigned *cnt = a.cnt + (int64_t)it.part0 * KV + kvh;
@@ -446,30 +363,26 @@ __global__ __launch_bounds__(512, 2) void seq_tiles_kernel(SeqAttnArgs a) {
   }
   BARRIER();
   if (!*flag) return;
-  // The parts in key order; with KG = 2 the groups share the d blocks.
-  constexpr int HB = (NDB + KG - 1) / KG;
-  const int db0 = KG == 2 ? grp * HB : 0;
+  // The parts in key order.
   float m[QB], l[QB];
-  floatx4 acc[HB][QB];
+  floatx4 acc[NDB][QB];
 #pragma unroll
   for (int qb = 0; qb < QB; ++qb) {
     m[qb] = -INFINITY;
     l[qb] = 0.f;
 #pragma unroll
-    for (int i = 0; i < HB; ++i) acc[i][qb] = floatx4{0.f, 0.f, 0.f, 0.f};
+    for (int db = 0; db < NDB; ++db) acc[db][qb] = floatx4{0.f, 0.f, 0.f, 0.f};
   }
   for (int sp = 0; sp < S; ++sp) {
     const uint32_t at = lane_at + (uint32_t)sp * slot_step;
     const floatx4 ml = __builtin_bit_cast(floatx4, __builtin_amdgcn_raw_buffer_load_b128(rp, at, 0, SC1));
-    floatx4 x[HB][QB];
+    floatx4 x[NDB][QB];
 #pragma unroll
-    for (int i = 0; i < HB; ++i)
+    for (int db = 0; db < NDB; ++db)
 #pragma unroll
-      for (int qb = 0; qb < QB; ++qb) {
-        const int db = db0 + i;
-        x[i][qb] = __builtin_bit_cast(floatx4, __builtin_amdgcn_raw_buffer_load_b128(
-                                                   rp, db < NDB ? at + (uint32_t)((1 + db * QB + qb) * 1024) : OOB_OFFSET, 0, SC1));
-      }
+      for (int qb = 0; qb < QB; ++qb)
+        x[db][qb] = __builtin_bit_cast(floatx4, __builtin_amdgcn_raw_buffer_load_b128(
+                                                    rp, at + (uint32_t)((1 + db * QB + qb) * 1024), 0, SC1));
 #pragma unroll
     for (int qb = 0; qb < QB; ++qb) {
       const float m1 = qb ? ml[2] : ml[0], l1 = qb ? ml[3] : ml[1];
@@ -478,51 +391,45 @@ __global__ __launch_bounds__(512, 2) void seq_tiles_kernel(SeqAttnArgs a) {
       m[qb] = mn;
       l[qb] = l[qb] * a0 + l1 * a1;
 #pragma unroll
-      for (int i = 0; i < HB; ++i) acc[i][qb] = acc[i][qb] * a0 + x[i][qb] * a1;
+      for (int db = 0; db < NDB; ++db) acc[db][qb] = acc[db][qb] * a0 + x[db][qb] * a1;
     }
   }
 #pragma unroll
   for (int qb = 0; qb < QB; ++qb) {
     const float inv = 1.0f / l[qb];
 #pragma unroll
-    for (int i = 0; i < HB; ++i)
-      if (db0 + i < NDB) store_o(acc[i][qb], db0 + i, qb, inv);
+    for (int db = 0; db < NDB; ++db) store_o(acc[db][qb], db, qb, inv);
   }
 }
 
 namespace {
-template <int DT, int D, int KG, bool PAGED, bool SOFTCAP>
-hipError_t launch_seq_tiles_kg(const SeqAttnArgs &a, int n_items, hipStream_t st) {
-  using Gm = SeqTilesGeom<D, KG>;
-  static_assert(Gm::ROWS == seq_tile_rows(D, KG == 1) && SEQ_KEY_TILE % Gm::TK == 0, "the plan's tiles");
-  auto kern = seq_tiles_kernel<DT, D, KG, PAGED, SOFTCAP>;
+template <int DT, int D, bool PAGED, bool SOFTCAP>
+hipError_t launch_seq_tiles(const SeqAttnArgs &a, int n_items, hipStream_t st) {
+  using Gm = SeqTilesGeom<D>;
+  static_assert(Gm::ROWS == seq_tile_rows(D) && SEQ_KEY_TILE % Gm::TK == 0, "the plan's tiles");
+  auto kern = seq_tiles_kernel<DT, D, PAGED, SOFTCAP>;
   static bool attr_set = false;
   if (!attr_set) {
     hipError_t e = hipFuncSetAttribute((const void *)kern, hipFuncAttributeMaxDynamicSharedMemorySize, Gm::SMEM);
     if (e != hipSuccess) return e;
     attr_set = true;
   }
-  hipLaunchKernelGGL(kern, dim3((unsigned)(n_items * a.n_kv_heads)), dim3(512), Gm::SMEM, st, a);
+  hipLaunchKernelGGL(kern, dim3((unsigned)(n_items * a.n_kv_heads)), dim3(256), Gm::SMEM, st, a);
   return hipGetLastError();
-}
-template <int DT, int D, bool PAGED, bool SOFTCAP>
-hipError_t launch_seq_tiles(const SeqAttnArgs &a, int n_items, bool wide, hipStream_t st) {
-  return wide ? launch_seq_tiles_kg<DT, D, 1, PAGED, SOFTCAP>(a, n_items, st)
-              : launch_seq_tiles_kg<DT, D, 2, PAGED, SOFTCAP>(a, n_items, st);
 }
 
 template <int DT, bool PAGED, bool SOFTCAP>
-hipError_t launch_seq_tiles_d(const SeqAttnArgs &a, int n_items, bool wide, hipStream_t st) {
+hipError_t launch_seq_tiles_d(const SeqAttnArgs &a, int n_items, hipStream_t st) {
   switch (a.head_dim) {
-    case 32: return launch_seq_tiles<DT, 32, PAGED, SOFTCAP>(a, n_items, wide, st);
-    case 48: return launch_seq_tiles<DT, 48, PAGED, SOFTCAP>(a, n_items, wide, st);
-    case 64: return launch_seq_tiles<DT, 64, PAGED, SOFTCAP>(a, n_items, wide, st);
-    case 72: return launch_seq_tiles<DT, 72, PAGED, SOFTCAP>(a, n_items, wide, st);
-    case 80: return launch_seq_tiles<DT, 80, PAGED, SOFTCAP>(a, n_items, wide, st);
-    case 96: return launch_seq_tiles<DT, 96, PAGED, SOFTCAP>(a, n_items, wide, st);
-    case 112: return launch_seq_tiles<DT, 112, PAGED, SOFTCAP>(a, n_items, wide, st);
-    case 128: return launch_seq_tiles<DT, 128, PAGED, SOFTCAP>(a, n_items, wide, st);
-    case 256: return launch_seq_tiles<DT, 256, PAGED, SOFTCAP>(a, n_items, wide, st);
+    case 32: return launch_seq_tiles<DT, 32, PAGED, SOFTCAP>(a, n_items, st);
+    case 48: return launch_seq_tiles<DT, 48, PAGED, SOFTCAP>(a, n_items, st);
+    case 64: return launch_seq_tiles<DT, 64, PAGED, SOFTCAP>(a, n_items, st);
+    case 72: return launch_seq_tiles<DT, 72, PAGED, SOFTCAP>(a, n_items, st);
+    case 80: return launch_seq_tiles<DT, 80, PAGED, SOFTCAP>(a, n_items, st);
+    case 96: return launch_seq_tiles<DT, 96, PAGED, SOFTCAP>(a, n_items, st);
+    case 112: return launch_seq_tiles<DT, 112, PAGED, SOFTCAP>(a, n_items, st);
+    case 128: return launch_seq_tiles<DT, 128, PAGED, SOFTCAP>(a, n_items, st);
+    case 256: return launch_seq_tiles<DT, 256, PAGED, SOFTCAP>(a, n_items, st);
   }
   return hipErrorInvalidValue;
 }
