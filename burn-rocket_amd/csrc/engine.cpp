@@ -2709,13 +2709,13 @@ int seq_attention(const void *plan, bool paged, const void *q, int64_t q_stride,
     a.items = (const SeqItem *)(block + p->off_tiles);
     a.cnt = (unsigned *)(work + p->off_tile_cnt);
     a.part = work + p->off_tile_part;
-    HIP_TRY(rk_launch_attention_seqs(a, (int)n_tiles, SEQ_TILES, paged, dtype, st), op);
+    HIP_TRY(rk_launch_attention_seqs(a, (int)n_tiles, SEQ_TILES, p->lists.tiles.longest, paged, dtype, st), op);
   }
   if (n_rows) {
     a.items = (const SeqItem *)block;
     a.cnt = (unsigned *)work;
     a.part = work + p->off_rows;
-    HIP_TRY(rk_launch_attention_seqs(a, (int)n_rows, SEQ_ROWS, paged, dtype, st), op);
+    HIP_TRY(rk_launch_attention_seqs(a, (int)n_rows, SEQ_ROWS, p->lists.rows.longest, paged, dtype, st), op);
   }
   g_eng->calls++;
   return RK_OK;

@@ -225,11 +225,13 @@ struct SeqAttnArgs {
   float scale, softcap;
   int mask_mode, window, uniform;
 };
-// Launches over n_items items of a.items, a list of SEQ_* kind.
-hipError_t rk_launch_attention_seqs(const SeqAttnArgs &a, int n_items, SeqKind kind, bool paged, int dtype, hipStream_t st);
+// Launches over n_items items of a.items, a list of SEQ_* kind. longest: the keys of its
+// longest item (it decides how a launch is made, not whether it is right).
+hipError_t rk_launch_attention_seqs(const SeqAttnArgs &a, int n_items, SeqKind kind, int longest, bool paged, int dtype,
+                                    hipStream_t st);
 size_t rk_seq_slot_bytes(int head_dim, SeqKind kind);  // one partial state
-hipError_t rk_launch_seq_rows_f16(const SeqAttnArgs &a, int n_items, bool paged, hipStream_t st);
-hipError_t rk_launch_seq_rows_bf16(const SeqAttnArgs &a, int n_items, bool paged, hipStream_t st);
+hipError_t rk_launch_seq_rows_f16(const SeqAttnArgs &a, int n_items, bool brief, bool paged, hipStream_t st);
+hipError_t rk_launch_seq_rows_bf16(const SeqAttnArgs &a, int n_items, bool brief, bool paged, hipStream_t st);
 hipError_t rk_launch_seq_tiles_f16(const SeqAttnArgs &a, int n_items, bool paged, hipStream_t st);
 hipError_t rk_launch_seq_tiles_bf16(const SeqAttnArgs &a, int n_items, bool paged, hipStream_t st);
 hipError_t rk_launch_seq_tiles_f16_cap(const SeqAttnArgs &a, int n_items, bool paged, hipStream_t st);

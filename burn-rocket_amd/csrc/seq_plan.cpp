@@ -96,27 +96,29 @@ int64_t slots_per_head(const SeqGeom &g, int num_cus, bool few) {
 // 206 in 516 on MI355X). More: only tiles longer than 5/4 of an even share. None where
 // the longest would shrink by less than `cost` steps, which is what states to
 // store and merge take (about 20 us for tiles of 128 rows).
-void split(std::vector<SeqItem> &tiles, int step, int64_t slots, int64_t cost, SeqList *out) {
+void split(std::vector<SeqItem> &tiles, int step, int64_t slots, int64_t least, int64_t cost, SeqList *out) {
   const auto steps = [&](const SeqItem &t) { return ceil_div(t.k_end - t.k_begin, step); };
   int64_t total = 0, longest = 0;
   for (const SeqItem &t : tiles) {
     total += steps(t);
     longest = std::max(longest, steps(t));
   }
-  int64_t quota = std::max<int64_t>(1, ceil_div(total, slots));
+  // (16 states are merged in one pass)
+  const int64_t max_parts = longest <= 32 * 16 ? 16 : SEQ_MAX_PARTS;
+  int64_t quota = std::max(least, ceil_div(total, slots));
   if ((int64_t)tiles.size() < slots) {
     const auto items = [&](int64_t q) {
       int64_t n = 0;
-      for (const SeqItem &t : tiles) n += std::min<int64_t>(ceil_div(steps(t), q), SEQ_MAX_PARTS);
+      for (const SeqItem &t : tiles) n += std::min(ceil_div(steps(t), q), max_parts);
       return n;
     };
     while (items(quota) > slots) quota += 1 + quota / 64;
   } else {
-    quota = ceil_div(5 * total, 4 * slots);
+    quota = std::max(least, ceil_div(5 * total, 4 * slots));
   }
   if (longest - quota < cost) quota = std::max<int64_t>(longest, 1);
   for (SeqItem &t : tiles) {
-    const int64_t n = steps(t), parts = std::min<int64_t>(ceil_div(n, quota), SEQ_MAX_PARTS);
+    const int64_t n = steps(t), parts = std::min(ceil_div(n, quota), max_parts);
     t.n_parts = (int32_t)parts;
     t.part0 = out->n_parts;
     if (parts > 1) out->n_parts += (int)parts;
@@ -128,10 +130,12 @@ void split(std::vector<SeqItem> &tiles, int step, int64_t slots, int64_t cost, S
       out->items.push_back(t);
     }
   }
+  for (const SeqItem &t : out->items) out->longest = std::max(out->longest, t.k_end - t.k_begin);
   std::stable_sort(out->items.begin(), out->items.end(),
                    [&](const SeqItem &x, const SeqItem &y) { return steps(x) > steps(y); });
 }
-constexpr int64_t ROWS_COST = 8, TILES_COST = 12;  // steps that a split costs
+// Steps of an item at least (a chunk for each wave), and steps that a split costs.
+constexpr int64_t ROWS_LEAST = 8, ROWS_COST = 8, TILES_LEAST = 4, TILES_COST = 12;
 }  // namespace
 
 void seq_bound(const SeqGeom &g, int64_t n_seqs, int64_t n_tokens, int64_t max_q, int num_cus, SeqBound *rows,
@@ -142,7 +146,9 @@ void seq_bound(const SeqGeom &g, int64_t n_seqs, int64_t n_tokens, int64_t max_q
   const int64_t G = g.n_head / g.n_kv_heads, tr = seq_tile_rows(g.head_dim);
   const int64_t s0 = slots_per_head(g, num_cus, true), s1 = slots_per_head(g, num_cus, false);
   n_seqs = std::min(n_seqs, n_tokens);  // those with new tokens
-  *rows = SeqBound{n_seqs + s0, 2 * s0};
+  // (a small batch has at most four tiles of 16 rows per CU and all heads)
+  const int64_t few = std::min(n_tokens * G / 16 + n_seqs, ceil_div(4 * (int64_t)num_cus, g.n_kv_heads));
+  *rows = SeqBound{(max_q * G > SEQ_FEW_ROWS ? std::max(n_seqs, few) : n_seqs) + s0, 2 * s0};
   *tiles = SeqBound{};
   if (max_q * G > SEQ_FEW_ROWS)
     *tiles = SeqBound{n_tokens * G / tr + std::min(n_seqs, n_tokens * G / (SEQ_FEW_ROWS + 1)) + s1, 2 * s1};
@@ -156,6 +162,19 @@ void seq_build(const SeqGeom &g, const SeqBatch &b, int num_cus, SeqLists *out) 
     int32_t page, off, end;
   };
   std::vector<Piece> pieces;  // where new tokens go: slots [off, end) of a page
+  // A small batch goes to the kernel of few rows whole: at most four tiles of 16 rows
+  // per CU with few keys (each is a short wait there), or one per CU with 4096 keys (past
+  // that the tiles' own reads of K and V cost more than what the other kernel's shared
+  // ones wait for). MI355X, 32/4 heads of 128, rows -> tiles: 256 rows on 4096 keys 18.1
+  // us, 35.7; 128 rows on 30000 41.8, 50.9; 256 rows on 30000 73, 52; 16 times 64 rows
+  // on 2000 25.2, 29.8; on 8000 78, 60; 16 times 96 rows on 300 14.6, 11.9.
+  int64_t n16 = 0, n16_keys = 0;
+  for (int64_t i = 0; i < b.n_seqs; ++i) {
+    const int64_t t = ceil_div(b.q_lens[i] * G, 16) * g.n_kv_heads;
+    n16 += t;
+    n16_keys += t * kv_of(b, i);
+  }
+  const bool small = n16_keys <= 4096ll * num_cus && (n16 <= num_cus || (n16 <= 4 * num_cus && n16_keys <= 128 * n16));
   for (int64_t i = 0; i < b.n_seqs; ++i) {
     const int64_t q = b.q_lens[i], kv = kv_of(b, i), pos0 = kv - q;
     if (q == 0) continue;
@@ -165,7 +184,7 @@ void seq_build(const SeqGeom &g, const SeqBatch &b, int num_cus, SeqLists *out) 
     it.rows = (int32_t)(q * G);
     it.kv_len = (int32_t)kv;
     it.table = (int32_t)out->table.size();
-    const bool few = q * G <= SEQ_FEW_ROWS;
+    const bool few = small || q * G <= SEQ_FEW_ROWS;
     const int64_t tr = few ? 16 : seq_tile_rows(g.head_dim), step = few ? SEQ_ROWS_CHUNK : SEQ_KEY_TILE;
     for (int64_t r = 0; r < q * G; r += tr) {
       int64_t lo, hi, lo2, hi2;
@@ -193,8 +212,8 @@ void seq_build(const SeqGeom &g, const SeqBatch &b, int num_cus, SeqLists *out) 
       t = e;
     }
   }
-  split(rows, SEQ_ROWS_CHUNK, slots_per_head(g, num_cus, true), ROWS_COST, &out->rows);
-  split(tiles, SEQ_KEY_TILE, slots_per_head(g, num_cus, false), TILES_COST, &out->tiles);
+  split(rows, SEQ_ROWS_CHUNK, slots_per_head(g, num_cus, true), ROWS_LEAST, ROWS_COST, &out->rows);
+  split(tiles, SEQ_KEY_TILE, slots_per_head(g, num_cus, false), TILES_LEAST, TILES_COST, &out->tiles);
   std::sort(pieces.begin(), pieces.end(),
             [](const Piece &x, const Piece &y) { return x.page != y.page ? x.page < y.page : x.off < y.off; });
   for (size_t i = 1; i < pieces.size(); ++i)

@@ -36,8 +36,8 @@ struct SeqTok {
 };
 
 // Kinds of items: tiles of 16 rows with their keys over the waves of a workgroup
-// (seq_rows.hpp) for sequences of at most SEQ_FEW_ROWS query rows; for the others
-// tiles of seq_tile_rows rows (seq_tiles.hpp).
+// (seq_rows.hpp) for sequences of at most SEQ_FEW_ROWS query rows, or for all of a small
+// batch; for the others tiles of seq_tile_rows rows (seq_tiles.hpp).
 enum SeqKind { SEQ_ROWS, SEQ_TILES };
 constexpr int SEQ_FEW_ROWS = 16;
 constexpr int SEQ_ROWS_CHUNK = 32;  // keys of a step of the first, ranges start at multiples
@@ -65,6 +65,7 @@ struct SeqBatch {
 struct SeqList {
   std::vector<SeqItem> items;  // longest first
   int n_parts = 0;             // partial states (per kv head)
+  int longest = 0;             // keys of the longest item
 };
 struct SeqLists {
   int64_t n_tokens = 0;

@@ -29,11 +29,9 @@
 
 namespace {
 constexpr int CK = SEQ_ROWS_CHUNK;  // keys per chunk
-__host__ __device__ constexpr int seq_rows_waves(int d) { return d <= 128 ? 8 : 4; }
 
-template <int D>
+template <int D, int RW>
 struct SeqRowsGeom {
-  static constexpr int RW = seq_rows_waves(D);
   static constexpr int NQC = (D + 31) / 32;  // 32-wide d chunks of QKᵀ
   static constexpr int NDB = (D + 15) / 16;  // 16-row d blocks of Oᵀ
   static constexpr int CH = D / 8;           // 16-byte pieces per V row
@@ -48,11 +46,11 @@ struct SeqRowsGeom {
 };
 }  // namespace
 
-template <int DT, int D, bool PAGED>
-__global__ __launch_bounds__(seq_rows_waves(D) * 64, 2) void seq_rows_kernel(SeqAttnArgs a) {
-  using Gm = SeqRowsGeom<D>;
+template <int DT, int D, int RW, bool PAGED>
+__global__ __launch_bounds__(RW * 64, 2) void seq_rows_kernel(SeqAttnArgs a) {
+  using Gm = SeqRowsGeom<D, RW>;
   constexpr int KBUF = D > 128 ? 1 : 2;  // K register sets (two of head dim 256 spill)
-  constexpr int NQC = Gm::NQC, NDB = Gm::NDB, CH = Gm::CH, VB_INS = Gm::VB_INS, KL = Gm::KL, RW = Gm::RW;
+  constexpr int NQC = Gm::NQC, NDB = Gm::NDB, CH = Gm::CH, VB_INS = Gm::VB_INS, KL = Gm::KL;
   // The two V buffers of the waves, objects of their own: the compiler then knows that
   // a copy into one is not what a read of the other waits for.
   __shared__ __attribute__((aligned(16))) uint8_t v_even[RW * Gm::V_BYTES];
@@ -320,24 +318,34 @@ __global__ __launch_bounds__(seq_rows_waves(D) * 64, 2) void seq_rows_kernel(Seq
 
 namespace {
 template <int DT, int D, bool PAGED>
-hipError_t launch_seq_rows(const SeqAttnArgs &a, int n_items, hipStream_t st) {
-  using Gm = SeqRowsGeom<D>;
-  hipLaunchKernelGGL((seq_rows_kernel<DT, D, PAGED>), dim3((unsigned)(n_items * a.n_kv_heads)), dim3(Gm::RW * 64), 0, st, a);
+hipError_t launch_seq_rows(const SeqAttnArgs &a, int n_items, bool brief, hipStream_t st) {
+  const dim3 grid((unsigned)(n_items * a.n_kv_heads));
+  // Eight waves where their LDS fits; four where no item has more chunks than that
+  // half has to itself, as two such workgroups share a CU (24 sequences of 4 to 40
+  // tokens, 16/8 heads of 128: 8.2 us against 11.9; 64 sequences of up to 8000 keys the
+  // other way round: 197 against 186).
+  if constexpr (D <= 128) {
+    if (!brief) {
+      hipLaunchKernelGGL((seq_rows_kernel<DT, D, 8, PAGED>), grid, dim3(512), 0, st, a);
+      return hipGetLastError();
+    }
+  }
+  hipLaunchKernelGGL((seq_rows_kernel<DT, D, 4, PAGED>), grid, dim3(256), 0, st, a);
   return hipGetLastError();
 }
 
 template <int DT, bool PAGED>
-hipError_t launch_seq_rows_d(const SeqAttnArgs &a, int n_items, hipStream_t st) {
+hipError_t launch_seq_rows_d(const SeqAttnArgs &a, int n_items, bool brief, hipStream_t st) {
   switch (a.head_dim) {
-    case 32: return launch_seq_rows<DT, 32, PAGED>(a, n_items, st);
-    case 48: return launch_seq_rows<DT, 48, PAGED>(a, n_items, st);
-    case 64: return launch_seq_rows<DT, 64, PAGED>(a, n_items, st);
-    case 72: return launch_seq_rows<DT, 72, PAGED>(a, n_items, st);
-    case 80: return launch_seq_rows<DT, 80, PAGED>(a, n_items, st);
-    case 96: return launch_seq_rows<DT, 96, PAGED>(a, n_items, st);
-    case 112: return launch_seq_rows<DT, 112, PAGED>(a, n_items, st);
-    case 128: return launch_seq_rows<DT, 128, PAGED>(a, n_items, st);
-    case 256: return launch_seq_rows<DT, 256, PAGED>(a, n_items, st);
+    case 32: return launch_seq_rows<DT, 32, PAGED>(a, n_items, brief, st);
+    case 48: return launch_seq_rows<DT, 48, PAGED>(a, n_items, brief, st);
+    case 64: return launch_seq_rows<DT, 64, PAGED>(a, n_items, brief, st);
+    case 72: return launch_seq_rows<DT, 72, PAGED>(a, n_items, brief, st);
+    case 80: return launch_seq_rows<DT, 80, PAGED>(a, n_items, brief, st);
+    case 96: return launch_seq_rows<DT, 96, PAGED>(a, n_items, brief, st);
+    case 112: return launch_seq_rows<DT, 112, PAGED>(a, n_items, brief, st);
+    case 128: return launch_seq_rows<DT, 128, PAGED>(a, n_items, brief, st);
+    case 256: return launch_seq_rows<DT, 256, PAGED>(a, n_items, brief, st);
   }
   return hipErrorInvalidValue;
 }
