@@ -7,15 +7,17 @@ size_t rk_seq_slot_bytes(int head_dim, SeqKind kind) {
   return kind == SEQ_ROWS ? ndb * 1024 + 128 : 4 * (1 + ndb * qb) * 1024;
 }
 
-hipError_t rk_launch_attention_seqs(const SeqAttnArgs &a, int n_items, SeqKind kind, int longest, bool paged, int dtype,
-                                    hipStream_t st) {
+hipError_t rk_launch_attention_seqs(const SeqAttnArgs &a, int longest_row, bool paged, int dtype, hipStream_t st) {
   const bool f16 = dtype == RK_DTYPE_F16;
   if (!f16 && dtype != RK_DTYPE_BF16) return hipErrorInvalidValue;
-  if (kind == SEQ_ROWS) {
-    const bool brief = longest <= 4 * SEQ_ROWS_CHUNK;
-    return f16 ? rk_launch_seq_rows_f16(a, n_items, brief, paged, st) : rk_launch_seq_rows_bf16(a, n_items, brief, paged, st);
+  if (a.rows.n && (!a.tiles.n || !seq_one_launch(a.head_dim))) {
+    const bool brief = longest_row <= 4 * SEQ_ROWS_CHUNK;
+    const hipError_t e = f16 ? rk_launch_seq_rows_f16(a, brief, paged, st) : rk_launch_seq_rows_bf16(a, brief, paged, st);
+    if (e != hipSuccess) return e;
   }
-  if (a.softcap != 0.f)
-    return f16 ? rk_launch_seq_tiles_f16_cap(a, n_items, paged, st) : rk_launch_seq_tiles_bf16_cap(a, n_items, paged, st);
-  return f16 ? rk_launch_seq_tiles_f16(a, n_items, paged, st) : rk_launch_seq_tiles_bf16(a, n_items, paged, st);
+  if (!a.tiles.n) return hipSuccess;
+  SeqAttnArgs t = a;
+  if (!seq_one_launch(a.head_dim)) t.rows.n = 0;
+  if (a.softcap != 0.f) return f16 ? rk_launch_seq_tiles_f16_cap(t, paged, st) : rk_launch_seq_tiles_bf16_cap(t, paged, st);
+  return f16 ? rk_launch_seq_tiles_f16(t, paged, st) : rk_launch_seq_tiles_bf16(t, paged, st);
 }

@@ -17,6 +17,7 @@
 #include <string>
 #include <unordered_map>
 #include <unordered_set>
+#include <utility>
 #include <vector>
 
 #include "../../include/burn_rocket_amd.h"
@@ -2532,16 +2533,20 @@ int seq_reserve(SeqPlan &p, const SeqPlan::Room &want, const char *op) {
   p.work.p = nullptr;
   if (p.pin) HIP_TRY(hipHostFree(p.pin), op);
   p.pin = nullptr;
-  SeqPlan::Room &r = p.room;
-  r = SeqPlan::Room{std::max(r.rows, want.rows),   std::max(r.tiles, want.tiles),
-                    std::max(r.toks, want.toks),   std::max(r.table, want.table),
-                    std::max(r.row_parts, want.row_parts), std::max(r.tile_parts, want.tile_parts)};
+  // (p.room is none while a buffer is missing: a failed allocation is tried again)
+  const SeqPlan::Room had = std::exchange(p.room, SeqPlan::Room{});
+  const SeqPlan::Room r{std::max(had.rows, want.rows),   std::max(had.tiles, want.tiles),
+                        std::max(had.toks, want.toks),   std::max(had.table, want.table),
+                        std::max(had.row_parts, want.row_parts), std::max(had.tile_parts, want.tile_parts)};
   p.off_tiles = align16(r.rows * sizeof(SeqItem));
   p.off_toks = p.off_tiles + align16(r.tiles * sizeof(SeqItem));
   p.off_table = p.off_toks + align16(r.toks * sizeof(SeqTok));
   p.block.bytes = std::max<size_t>(p.off_table + align16(r.table * 4), 256);
   HIP_TRY(hipMalloc(&p.block.p, p.block.bytes), op);
-  if (r.row_parts + r.tile_parts == 0) return RK_OK;
+  if (r.row_parts + r.tile_parts == 0) {
+    p.room = r;
+    return RK_OK;
+  }
   const size_t kv = (size_t)p.geom.n_kv_heads;
   p.off_tile_cnt = r.row_parts * kv * 4;
   p.off_rows = (p.off_tile_cnt + r.tile_parts * kv * 4 + 255) / 256 * 256;
@@ -2550,6 +2555,7 @@ int seq_reserve(SeqPlan &p, const SeqPlan::Room &want, const char *op) {
   HIP_TRY(hipMalloc(&p.work.p, p.work.bytes), op);
   HIP_TRY(hipMemset(p.work.p, 0, p.off_rows), op);
   HIP_TRY(hipDeviceSynchronize(), op);
+  p.room = r;
   return RK_OK;
 }
 
@@ -2700,23 +2706,16 @@ int seq_attention(const void *plan, bool paged, const void *q, int64_t q_stride,
   a.mask_mode = g.mask_mode;
   a.window = (int)g.window;
   a.uniform = g.uniform;
-  // A captured launch has a workgroup for every item that an update may list.
+  // A captured launch has a workgroup for every item that an update may list, and is made
+  // for long ones.
   const size_t n_rows = capturing ? p->room.rows : p->lists.rows.items.size();
   const size_t n_tiles = capturing ? p->room.tiles : p->lists.tiles.items.size();
   if (capturing) p->captured = true;
   uint8_t *work = (uint8_t *)p->work.p;
-  if (n_tiles) {
-    a.items = (const SeqItem *)(block + p->off_tiles);
-    a.cnt = (unsigned *)(work + p->off_tile_cnt);
-    a.part = work + p->off_tile_part;
-    HIP_TRY(rk_launch_attention_seqs(a, (int)n_tiles, SEQ_TILES, p->lists.tiles.longest, paged, dtype, st), op);
-  }
-  if (n_rows) {
-    a.items = (const SeqItem *)block;
-    a.cnt = (unsigned *)work;
-    a.part = work + p->off_rows;
-    HIP_TRY(rk_launch_attention_seqs(a, (int)n_rows, SEQ_ROWS, p->lists.rows.longest, paged, dtype, st), op);
-  }
+  a.rows = SeqListArgs{(const SeqItem *)block, (int)n_rows, work + p->off_rows, (unsigned *)work};
+  a.tiles = SeqListArgs{(const SeqItem *)(block + p->off_tiles), (int)n_tiles, work + p->off_tile_part,
+                        (unsigned *)(work + p->off_tile_cnt)};
+  HIP_TRY(rk_launch_attention_seqs(a, capturing ? INT32_MAX : p->lists.rows.longest, paged, dtype, st), op);
   g_eng->calls++;
   return RK_OK;
 }

@@ -213,29 +213,33 @@ hipError_t rk_launch_attention_rows(const AttnArgs &a, const void *v, int64_t v_
                                     hipStream_t st);
 
 // Batches of sequences (seq_plan.hpp). The lists are in device memory.
+struct SeqListArgs {
+  const SeqItem *items;
+  int n;          // items
+  void *part;     // partial softmax states
+  unsigned *cnt;  // arrival counts of split tiles: zero between launches
+};
 struct SeqAttnArgs {
   const void *q, *k, *v;  // k, v: packed rows, or the cache [page][kv head][page_size][head_dim]
   void *out;
   int64_t q_stride, k_stride, v_stride, out_stride;  // values between tokens (k, v: packed only)
-  const SeqItem *items;
+  SeqListArgs rows, tiles;
   const int32_t *table;  // page ids (paged)
-  void *part;            // partial softmax states
-  unsigned *cnt;         // arrival counts of split tiles: zero between launches
   int n_head, n_kv_heads, head_dim, page_log2;
   float scale, softcap;
   int mask_mode, window, uniform;
 };
-// Launches over n_items items of a.items, a list of SEQ_* kind. longest: the keys of its
-// longest item (it decides how a launch is made, not whether it is right).
-hipError_t rk_launch_attention_seqs(const SeqAttnArgs &a, int n_items, SeqKind kind, int longest, bool paged, int dtype,
-                                    hipStream_t st);
+// Launches the items of both lists. longest_row: keys of the longest row item (it
+// decides how a launch is made, not whether it is right).
+hipError_t rk_launch_attention_seqs(const SeqAttnArgs &a, int longest_row, bool paged, int dtype, hipStream_t st);
 size_t rk_seq_slot_bytes(int head_dim, SeqKind kind);  // one partial state
-hipError_t rk_launch_seq_rows_f16(const SeqAttnArgs &a, int n_items, bool brief, bool paged, hipStream_t st);
-hipError_t rk_launch_seq_rows_bf16(const SeqAttnArgs &a, int n_items, bool brief, bool paged, hipStream_t st);
-hipError_t rk_launch_seq_tiles_f16(const SeqAttnArgs &a, int n_items, bool paged, hipStream_t st);
-hipError_t rk_launch_seq_tiles_bf16(const SeqAttnArgs &a, int n_items, bool paged, hipStream_t st);
-hipError_t rk_launch_seq_tiles_f16_cap(const SeqAttnArgs &a, int n_items, bool paged, hipStream_t st);
-hipError_t rk_launch_seq_tiles_bf16_cap(const SeqAttnArgs &a, int n_items, bool paged, hipStream_t st);
+hipError_t rk_launch_seq_rows_f16(const SeqAttnArgs &a, bool brief, bool paged, hipStream_t st);
+hipError_t rk_launch_seq_rows_bf16(const SeqAttnArgs &a, bool brief, bool paged, hipStream_t st);
+// (the items of a.tiles, with those of a.rows behind them)
+hipError_t rk_launch_seq_tiles_f16(const SeqAttnArgs &a, bool paged, hipStream_t st);
+hipError_t rk_launch_seq_tiles_bf16(const SeqAttnArgs &a, bool paged, hipStream_t st);
+hipError_t rk_launch_seq_tiles_f16_cap(const SeqAttnArgs &a, bool paged, hipStream_t st);
+hipError_t rk_launch_seq_tiles_bf16_cap(const SeqAttnArgs &a, bool paged, hipStream_t st);
 
 struct PagedAppendArgs {
   const void *qkv;  // [n_tokens] rows: q heads, k heads, v heads

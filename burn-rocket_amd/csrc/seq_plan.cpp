@@ -82,10 +82,10 @@ std::string seq_check_batch(const SeqGeom &g, const SeqBatch &b) {
 }
 
 namespace {
-// Workgroups of a kernel that the GPU holds at once, per kv head (at least one).
-int64_t slots_per_head(const SeqGeom &g, int num_cus, bool few) {
-  // Registers and LDS leave two workgroups per CU, one of the first kernel for heads above 64.
-  const int64_t slots = (int64_t)std::max(1, num_cus) * (few && g.head_dim > 64 ? 1 : 2);
+// Workgroups that the GPU holds at once, per kv head (at least one): registers and LDS
+// leave two per CU, one of those that take row items alone with heads above 64.
+int64_t slots_per_head(const SeqGeom &g, int num_cus, bool one) {
+  const int64_t slots = (int64_t)std::max(1, num_cus) * (one && g.head_dim > 64 ? 1 : 2);
   return std::max<int64_t>(1, slots / g.n_kv_heads);
 }
 
@@ -144,14 +144,14 @@ void seq_bound(const SeqGeom &g, int64_t n_seqs, int64_t n_tokens, int64_t max_q
   // share of the steps: splits add at most `slots` items. A split tile's states are at
   // most twice what its split added.
   const int64_t G = g.n_head / g.n_kv_heads, tr = seq_tile_rows(g.head_dim);
-  const int64_t s0 = slots_per_head(g, num_cus, true), s1 = slots_per_head(g, num_cus, false);
+  const int64_t slots = slots_per_head(g, num_cus, false);
   n_seqs = std::min(n_seqs, n_tokens);  // those with new tokens
   // (a small batch has at most four tiles of 16 rows per CU and all heads)
   const int64_t few = std::min(n_tokens * G / 16 + n_seqs, ceil_div(4 * (int64_t)num_cus, g.n_kv_heads));
-  *rows = SeqBound{(max_q * G > SEQ_FEW_ROWS ? std::max(n_seqs, few) : n_seqs) + s0, 2 * s0};
+  *rows = SeqBound{(max_q * G > SEQ_FEW_ROWS ? std::max(n_seqs, few) : n_seqs) + slots, 2 * slots};
   *tiles = SeqBound{};
   if (max_q * G > SEQ_FEW_ROWS)
-    *tiles = SeqBound{n_tokens * G / tr + std::min(n_seqs, n_tokens * G / (SEQ_FEW_ROWS + 1)) + s1, 2 * s1};
+    *tiles = SeqBound{n_tokens * G / tr + std::min(n_seqs, n_tokens * G / (SEQ_FEW_ROWS + 1)) + slots, 2 * slots};
 }
 
 void seq_build(const SeqGeom &g, const SeqBatch &b, int num_cus, SeqLists *out) {
@@ -212,7 +212,7 @@ void seq_build(const SeqGeom &g, const SeqBatch &b, int num_cus, SeqLists *out) 
       t = e;
     }
   }
-  split(rows, SEQ_ROWS_CHUNK, slots_per_head(g, num_cus, true), ROWS_LEAST, ROWS_COST, &out->rows);
+  split(rows, SEQ_ROWS_CHUNK, slots_per_head(g, num_cus, tiles.empty() || !seq_one_launch(g.head_dim)), ROWS_LEAST, ROWS_COST, &out->rows);
   split(tiles, SEQ_KEY_TILE, slots_per_head(g, num_cus, false), TILES_LEAST, TILES_COST, &out->tiles);
   std::sort(pieces.begin(), pieces.end(),
             [](const Piece &x, const Piece &y) { return x.page != y.page ? x.page < y.page : x.off < y.off; });

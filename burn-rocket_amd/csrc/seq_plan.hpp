@@ -43,6 +43,9 @@ constexpr int SEQ_FEW_ROWS = 16;
 constexpr int SEQ_ROWS_CHUNK = 32;  // keys of a step of the first, ranges start at multiples
 constexpr int SEQ_KEY_TILE = 64;    // and of the second
 constexpr int seq_tile_rows(int head_dim) { return head_dim <= 128 ? 128 : 64; }
+// Whether one launch takes both kinds of items: where the row items' buffers leave two
+// workgroups a CU.
+constexpr bool seq_one_launch(int head_dim) { return head_dim <= 128; }
 constexpr int SEQ_MAX_PARTS = 32;
 constexpr int64_t SEQ_MAX_STRIDE = (int64_t)1 << 26;  // values between packed tokens: 16 of them stay below 2 GiB
 

@@ -46,19 +46,19 @@ struct SeqRowsGeom {
 };
 }  // namespace
 
+// One item for one kv head: `block` counts the kv heads of one item, then the next item.
+// v_even, v_odd: the two V buffers of the waves, RW·V_BYTES each and objects of their
+// own: the compiler then knows that a copy into one is not what a read of the other
+// waits for.
 template <int DT, int D, int RW, bool PAGED>
-__global__ __launch_bounds__(RW * 64, 2) void seq_rows_kernel(SeqAttnArgs a) {
+__device__ __forceinline__ void seq_rows_item(const SeqAttnArgs &a, int block, uint8_t *v_even, uint8_t *v_odd) {
   using Gm = SeqRowsGeom<D, RW>;
   constexpr int KBUF = D > 128 ? 1 : 2;  // K register sets (two of head dim 256 spill)
   constexpr int NQC = Gm::NQC, NDB = Gm::NDB, CH = Gm::CH, VB_INS = Gm::VB_INS, KL = Gm::KL;
-  // The two V buffers of the waves, objects of their own: the compiler then knows that
-  // a copy into one is not what a read of the other waits for.
-  __shared__ __attribute__((aligned(16))) uint8_t v_even[RW * Gm::V_BYTES];
-  __shared__ __attribute__((aligned(16))) uint8_t v_odd[RW * Gm::V_BYTES];
 
   const int KV = a.n_kv_heads, G = a.n_head / KV;
-  const int kvh = blockIdx.x % KV;
-  const SeqItem it = a.items[blockIdx.x / KV];
+  const int kvh = block % KV;
+  const SeqItem it = a.rows.items[block / KV];
   if (it.rows == 0) return;
   const int lane = lane_id();
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -235,7 +235,7 @@ __global__ __launch_bounds__(RW * 64, 2) void seq_rows_kernel(SeqAttnArgs a) {
   constexpr int SC1 = 16;  // cache policy bit: device scope
   const int S = it.n_parts;
   const uint32_t slot_step = (uint32_t)KV * Gm::SLOT_BYTES;
-  const rsrc_t rp = make_rsrc((const uint8_t *)a.part + ((int64_t)it.part0 * KV + kvh) * Gm::SLOT_BYTES,
+  const rsrc_t rp = make_rsrc((const uint8_t *)a.rows.part + ((int64_t)it.part0 * KV + kvh) * Gm::SLOT_BYTES,
                               S > 1 ? (int64_t)(S - 1) * slot_step + Gm::SLOT_BYTES : 0);
   const uint32_t mine = (uint32_t)it.sp * slot_step;
   float wa[RW], m_all = -INFINITY, l_all = 0.f;
@@ -276,7 +276,7 @@ __global__ __launch_bounds__(RW * 64, 2) void seq_rows_kernel(SeqAttnArgs a) {
   __syncthreads();
   unsigned *flag = (unsigned *)v_odd;
   if (threadIdx.x == 0) {
-    unsigned *cnt = a.cnt + (int64_t)it.part0 * KV + kvh;
+    unsigned *cnt = a.rows.cnt + (int64_t)it.part0 * KV + kvh;
     const unsigned last = atomicAdd(cnt, 1u) == (unsigned)(S - 1);
     if (last) atomicExch(cnt, 0u);  // every part is in: reset for the next launch
     *flag = last;
@@ -316,10 +316,17 @@ __global__ __launch_bounds__(RW * 64, 2) void seq_rows_kernel(SeqAttnArgs a) {
   }
 }
 
+template <int DT, int D, int RW, bool PAGED>
+__global__ __launch_bounds__(RW * 64, 2) void seq_rows_kernel(SeqAttnArgs a) {
+  __shared__ __attribute__((aligned(16))) uint8_t v_even[RW * SeqRowsGeom<D, RW>::V_BYTES];
+  __shared__ __attribute__((aligned(16))) uint8_t v_odd[RW * SeqRowsGeom<D, RW>::V_BYTES];
+  seq_rows_item<DT, D, RW, PAGED>(a, blockIdx.x, v_even, v_odd);
+}
+
 namespace {
 template <int DT, int D, bool PAGED>
-hipError_t launch_seq_rows(const SeqAttnArgs &a, int n_items, bool brief, hipStream_t st) {
-  const dim3 grid((unsigned)(n_items * a.n_kv_heads));
+hipError_t launch_seq_rows(const SeqAttnArgs &a, bool brief, hipStream_t st) {
+  const dim3 grid((unsigned)(a.rows.n * a.n_kv_heads));
   // Eight waves where their LDS fits; four where no item has more chunks than that
   // half has to itself, as two such workgroups share a CU (24 sequences of 4 to 40
   // tokens, 16/8 heads of 128: 8.2 us against 11.9; 64 sequences of up to 8000 keys the
@@ -335,17 +342,17 @@ hipError_t launch_seq_rows(const SeqAttnArgs &a, int n_items, bool brief, hipStr
 }
 
 template <int DT, bool PAGED>
-hipError_t launch_seq_rows_d(const SeqAttnArgs &a, int n_items, bool brief, hipStream_t st) {
+hipError_t launch_seq_rows_d(const SeqAttnArgs &a, bool brief, hipStream_t st) {
   switch (a.head_dim) {
-    case 32: return launch_seq_rows<DT, 32, PAGED>(a, n_items, brief, st);
-    case 48: return launch_seq_rows<DT, 48, PAGED>(a, n_items, brief, st);
-    case 64: return launch_seq_rows<DT, 64, PAGED>(a, n_items, brief, st);
-    case 72: return launch_seq_rows<DT, 72, PAGED>(a, n_items, brief, st);
-    case 80: return launch_seq_rows<DT, 80, PAGED>(a, n_items, brief, st);
-    case 96: return launch_seq_rows<DT, 96, PAGED>(a, n_items, brief, st);
-    case 112: return launch_seq_rows<DT, 112, PAGED>(a, n_items, brief, st);
-    case 128: return launch_seq_rows<DT, 128, PAGED>(a, n_items, brief, st);
-    case 256: return launch_seq_rows<DT, 256, PAGED>(a, n_items, brief, st);
+    case 32: return launch_seq_rows<DT, 32, PAGED>(a, brief, st);
+    case 48: return launch_seq_rows<DT, 48, PAGED>(a, brief, st);
+    case 64: return launch_seq_rows<DT, 64, PAGED>(a, brief, st);
+    case 72: return launch_seq_rows<DT, 72, PAGED>(a, brief, st);
+    case 80: return launch_seq_rows<DT, 80, PAGED>(a, brief, st);
+    case 96: return launch_seq_rows<DT, 96, PAGED>(a, brief, st);
+    case 112: return launch_seq_rows<DT, 112, PAGED>(a, brief, st);
+    case 128: return launch_seq_rows<DT, 128, PAGED>(a, brief, st);
+    case 256: return launch_seq_rows<DT, 256, PAGED>(a, brief, st);
   }
   return hipErrorInvalidValue;
 }

@@ -31,7 +31,7 @@
 // workspace; the last to arrive merges the parts in key order.
 #pragma once
 
-#include "seq_attn.hpp"
+#include "seq_rows.hpp"
 
 namespace {
 // LDS fragments read ahead of their products: 2 and 4 to 8 and 8 measured alike.
@@ -57,26 +57,28 @@ struct SeqTilesGeom {
   static constexpr bool POW2 = (D & (D - 1)) == 0;
   static constexpr int VSW = POW2 ? (CH / 2 < 8 ? CH / 2 : 8) - 1 : 0;
   static constexpr int K_BYTES = TK * KROW, V_BYTES = NB * VB;
-  static constexpr int V_AT = 2 * K_BYTES;          // the V buffers, behind those of K
-  static constexpr int SMEM = V_AT + 2 * V_BYTES;
+  static constexpr bool WITH_ROWS = seq_one_launch(D);
+  static constexpr int ROW_BYTES = WITH_ROWS ? 4 * SeqRowsGeom<D, 4>::V_BYTES : 0;
+  static constexpr int K_SMEM = 2 * K_BYTES > ROW_BYTES ? 2 * K_BYTES : ROW_BYTES;
+  static constexpr int V_SMEM = 2 * V_BYTES > ROW_BYTES ? 2 * V_BYTES : ROW_BYTES;
   static constexpr int CK = KI * NB / 4, CV = VI * NB / 4;  // copies per wave and tile
   static_assert(KI * NB % 4 == 0 && VI * NB % 4 == 0, "every wave copies alike");
   static constexpr int NJ = 1 + NDB * QB;           // 1 KB pieces of a wave's state in the workspace
   static constexpr int SLOT_BYTES = 4 * NJ * 1024;
-  static_assert(2 * SMEM <= 160 * 1024, "two workgroups per CU");
+  static_assert(2 * (K_SMEM + V_SMEM) <= 160 * 1024, "two workgroups per CU");
 };
 }  // namespace
 
+// One item for one kv head, with the buffers of K and V.
 template <int DT, int D, bool PAGED, bool SOFTCAP>
-__global__ __launch_bounds__(256, 2) void seq_tiles_kernel(SeqAttnArgs a) {
+__device__ __forceinline__ void seq_tiles_item(const SeqAttnArgs &a, int block, uint8_t *k_smem, uint8_t *v_smem) {
   using Gm = SeqTilesGeom<D>;
   constexpr int QB = Gm::QB, TK = Gm::TK, NQC = Gm::NQC, NDB = Gm::NDB, NB = Gm::NB, NC2 = Gm::NC2;
   constexpr int KI = Gm::KI, VI = Gm::VI, CH = Gm::CH, KPC = Gm::KPC, KROW = Gm::KROW;
-  extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
 
   const int KV = a.n_kv_heads, G = a.n_head / KV;
-  const int kvh = blockIdx.x % KV;
-  const SeqItem it = a.items[blockIdx.x / KV];
+  const int kvh = block % KV;
+  const SeqItem it = a.tiles.items[block / KV];
   if (it.rows == 0) return;
   const int lane = lane_id();
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -131,8 +133,8 @@ __global__ __launch_bounds__(256, 2) void seq_tiles_kernel(SeqAttnArgs a) {
   auto turn_v = [&](int w) ALWAYS_INLINE { vb = key_blocks<PAGED>(a, it, a.v, a.v_stride, kvh, key_of(w), end, ids); };
   // The wave's share of the copies of tile j: pieces s of its 16-key
   // blocks b, in the order s + KI·b.
-  auto k_buf = [&](int j) ALWAYS_INLINE { return smem + (j & 1) * Gm::K_BYTES; };
-  auto v_buf = [&](int j) ALWAYS_INLINE { return smem + Gm::V_AT + (j & 1) * Gm::V_BYTES; };
+  auto k_buf = [&](int j) ALWAYS_INLINE { return k_smem + (j & 1) * Gm::K_BYTES; };
+  auto v_buf = [&](int j) ALWAYS_INLINE { return v_smem + (j & 1) * Gm::V_BYTES; };
   auto copy_k = [&](int j) ALWAYS_INLINE {
     uint8_t *const to = k_buf(j);
     static_for<Gm::CK>([&](auto i_c) ALWAYS_INLINE {
@@ -339,7 +341,7 @@ __global__ __launch_bounds__(256, 2) void seq_tiles_kernel(SeqAttnArgs a) {
   constexpr int SC1 = 16;
   constexpr int NJ = Gm::NJ;
   const uint32_t slot_step = (uint32_t)KV * Gm::SLOT_BYTES;
-  const rsrc_t rp = make_rsrc((const uint8_t *)a.part + ((int64_t)it.part0 * KV + kvh) * Gm::SLOT_BYTES,
+  const rsrc_t rp = make_rsrc((const uint8_t *)a.tiles.part + ((int64_t)it.part0 * KV + kvh) * Gm::SLOT_BYTES,
                               (int64_t)(S - 1) * slot_step + Gm::SLOT_BYTES);
   const uint32_t lane_at = (uint32_t)((wave * NJ * 64 + lane) * 16);
   const uint32_t to = lane_at + (uint32_t)it.sp * slot_step;
@@ -353,9 +355,9 @@ __global__ __launch_bounds__(256, 2) void seq_tiles_kernel(SeqAttnArgs a) {
                                              to + (uint32_t)((1 + db * QB + qb) * 1024), 0, SC1);
   WAIT_VMCNT(0);  // stored before the arrival count
   BARRIER();  // (the K and V buffers are free)
-  unsigned *flag = (unsigned *)smem;
+  unsigned *flag = (unsigned *)k_smem;
   if (threadIdx.x == 0) {
-    unsigned *cnt = a.cnt + (int64_t)it.part0 * KV + kvh;
+    unsigned *cnt = a.tiles.cnt + (int64_t)it.part0 * KV + kvh;
     const unsigned last = atomicAdd(cnt, 1u) == (unsigned)(S - 1);
     if (last) atomicExch(cnt, 0u);  // every part is in: reset for the next launch
     *flag = last;
@@ -402,34 +404,50 @@ __global__ __launch_bounds__(256, 2) void seq_tiles_kernel(SeqAttnArgs a) {
   }
 }
 
+// The tile items, then the batch's row items: those are bound by their reads of the
+// cache and run beside the products of the tiles, or where tiles have ended. MI355X, a
+// launch for each list against this one: 24 tokens on up to 2000 keys with a prompt
+// chunk of 256 on 2000, 16/4 heads of 64, 25.5 us, 16.8; 64 on up to 8000 with two
+// chunks of 1000, 32/4 heads of 128, 206, 147. Row items first: 20.1 and 161; both in
+// turns: 18.8 and 145. The most that it lost (64 on up to 8000 with a chunk of 512 on
+// 16901, 16/8 heads of 128; row items have half the waves here): 260, 270.
+template <int DT, int D, bool PAGED, bool SOFTCAP>
+__global__ __launch_bounds__(256, 2) void seq_tiles_kernel(SeqAttnArgs a) {
+  using Gm = SeqTilesGeom<D>;
+  __shared__ __attribute__((aligned(16))) uint8_t k_smem[Gm::K_SMEM];
+  __shared__ __attribute__((aligned(16))) uint8_t v_smem[Gm::V_SMEM];
+  const int n_tiles = a.tiles.n * a.n_kv_heads;
+  if constexpr (Gm::WITH_ROWS) {
+    if ((int)blockIdx.x >= n_tiles) {
+      seq_rows_item<DT, D, 4, PAGED>(a, blockIdx.x - n_tiles, k_smem, v_smem);
+      return;
+    }
+  }
+  seq_tiles_item<DT, D, PAGED, SOFTCAP>(a, blockIdx.x, k_smem, v_smem);
+}
+
 namespace {
 template <int DT, int D, bool PAGED, bool SOFTCAP>
-hipError_t launch_seq_tiles(const SeqAttnArgs &a, int n_items, hipStream_t st) {
+hipError_t launch_seq_tiles(const SeqAttnArgs &a, hipStream_t st) {
   using Gm = SeqTilesGeom<D>;
   static_assert(Gm::ROWS == seq_tile_rows(D) && SEQ_KEY_TILE % Gm::TK == 0, "the plan's tiles");
-  auto kern = seq_tiles_kernel<DT, D, PAGED, SOFTCAP>;
-  static bool attr_set = false;
-  if (!attr_set) {
-    hipError_t e = hipFuncSetAttribute((const void *)kern, hipFuncAttributeMaxDynamicSharedMemorySize, Gm::SMEM);
-    if (e != hipSuccess) return e;
-    attr_set = true;
-  }
-  hipLaunchKernelGGL(kern, dim3((unsigned)(n_items * a.n_kv_heads)), dim3(256), Gm::SMEM, st, a);
+  const dim3 grid((unsigned)((a.tiles.n + a.rows.n) * a.n_kv_heads));
+  hipLaunchKernelGGL((seq_tiles_kernel<DT, D, PAGED, SOFTCAP>), grid, dim3(256), 0, st, a);
   return hipGetLastError();
 }
 
 template <int DT, bool PAGED, bool SOFTCAP>
-hipError_t launch_seq_tiles_d(const SeqAttnArgs &a, int n_items, hipStream_t st) {
+hipError_t launch_seq_tiles_d(const SeqAttnArgs &a, hipStream_t st) {
   switch (a.head_dim) {
-    case 32: return launch_seq_tiles<DT, 32, PAGED, SOFTCAP>(a, n_items, st);
-    case 48: return launch_seq_tiles<DT, 48, PAGED, SOFTCAP>(a, n_items, st);
-    case 64: return launch_seq_tiles<DT, 64, PAGED, SOFTCAP>(a, n_items, st);
-    case 72: return launch_seq_tiles<DT, 72, PAGED, SOFTCAP>(a, n_items, st);
-    case 80: return launch_seq_tiles<DT, 80, PAGED, SOFTCAP>(a, n_items, st);
-    case 96: return launch_seq_tiles<DT, 96, PAGED, SOFTCAP>(a, n_items, st);
-    case 112: return launch_seq_tiles<DT, 112, PAGED, SOFTCAP>(a, n_items, st);
-    case 128: return launch_seq_tiles<DT, 128, PAGED, SOFTCAP>(a, n_items, st);
-    case 256: return launch_seq_tiles<DT, 256, PAGED, SOFTCAP>(a, n_items, st);
+    case 32: return launch_seq_tiles<DT, 32, PAGED, SOFTCAP>(a, st);
+    case 48: return launch_seq_tiles<DT, 48, PAGED, SOFTCAP>(a, st);
+    case 64: return launch_seq_tiles<DT, 64, PAGED, SOFTCAP>(a, st);
+    case 72: return launch_seq_tiles<DT, 72, PAGED, SOFTCAP>(a, st);
+    case 80: return launch_seq_tiles<DT, 80, PAGED, SOFTCAP>(a, st);
+    case 96: return launch_seq_tiles<DT, 96, PAGED, SOFTCAP>(a, st);
+    case 112: return launch_seq_tiles<DT, 112, PAGED, SOFTCAP>(a, st);
+    case 128: return launch_seq_tiles<DT, 128, PAGED, SOFTCAP>(a, st);
+    case 256: return launch_seq_tiles<DT, 256, PAGED, SOFTCAP>(a, st);
   }
   return hipErrorInvalidValue;
 }

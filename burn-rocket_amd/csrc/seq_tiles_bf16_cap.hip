@@ -1,7 +1,7 @@
 // seq_tiles.hpp for bf16, softcapped scores.
 #include "seq_tiles.hpp"
 
-hipError_t rk_launch_seq_tiles_bf16_cap(const SeqAttnArgs &a, int n_items, bool paged, hipStream_t st) {
-  return paged ? launch_seq_tiles_d<RK_DTYPE_BF16, true, true>(a, n_items, st)
-               : launch_seq_tiles_d<RK_DTYPE_BF16, false, true>(a, n_items, st);
+hipError_t rk_launch_seq_tiles_bf16_cap(const SeqAttnArgs &a, bool paged, hipStream_t st) {
+  return paged ? launch_seq_tiles_d<RK_DTYPE_BF16, true, true>(a, st)
+               : launch_seq_tiles_d<RK_DTYPE_BF16, false, true>(a, st);
 }

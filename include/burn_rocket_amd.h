@@ -461,9 +461,10 @@ int rk_seq_plan_destroy(void *plan);
  * dims as rk_attention_dev without the padded ones. Scores and softmax in f32,
  * probabilities rounded to nearest in dtype for the product with V, sums in f32,
  * one rounding at the end. The split of a row's keys between workgroups depends on
- * the whole batch: a sequence's result can differ in rounding between batches,
- * equal batches give equal bits. A non-finite value of V reaches every row of its
- * sequence that is computed in a tile with a row that sees it. */
+ * the whole batch: a sequence's result can differ in rounding between batches, and
+ * between a captured call (made for any batch of its plan's room) and one that is
+ * not. Equal batches give equal bits. A non-finite value of V reaches every row of
+ * its sequence that is computed in a tile with a row that sees it. */
 int rk_attention_packed_dev(const void *plan, const void *q, int64_t q_stride, const void *k, int64_t k_stride,
                             const void *v, int64_t v_stride, float scale, float softcap, void *out,
                             int64_t out_stride, int dtype, rk_stream stream);

@@ -549,11 +549,11 @@ def test_captured_step_replays_with_updates(rk):
         for b, a in zip(other, (*now, x, filled, filled)):
             b.upload(a)
         eager = rk.paged_plan(q_lens, kv_lens, table, pg.n_pages, ps, h, kv, d)
-        eager.reserve()  # the same kinds of tiles: equal bits
         step(eager, *other)
         rk.synchronize(st)
         want = [b.download(a.shape, np.uint16) for b, a in zip(other, (*now, x, filled, filled))]
-        assert (want[4][:n] != FILL).any() and (want[4][n:] == FILL).all()
+        keys = [[c[table[s, np.arange(m) // ps], :, np.arange(m) % ps] for s, m in enumerate(kv_lens)] for c in want[:2]]
+        outs = [want.pop()]
         for _ in range(3):
             for b, a in zip(mine, (*now, x, filled, filled)):
                 b.upload(a)
@@ -562,6 +562,11 @@ def test_captured_step_replays_with_updates(rk):
             rk.synchronize(st)
             for b, w in zip(mine, want):
                 assert (b.download(w.shape, np.uint16) == w).all(), f"batch {i}"
+            outs.append(mine[4].download(filled.shape, np.uint16))
+        for o in outs:
+            assert (o[n:] == FILL).all()
+            check_paged(o[:n], keys, want[3][:n], q_lens, kv_lens, h, kv, d, "f16", 0.1)
+        assert all((o == outs[1]).all() for o in outs[2:]), f"batch {i}"
         now = want[:2]
     with pytest.raises(rk.RocketError):  # five tokens: more than the graph has room for
         plan.update([2, 2, 1], [10, 10, 10], pg.table, stream=st)
