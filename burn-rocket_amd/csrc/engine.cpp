@@ -2797,99 +2797,107 @@ extern "C" int rk_seq_plan_reserve(void *plan, int64_t max_q_len) {
 }
 extern "C" int rk_seq_plan_destroy(void *plan) {
   const char *op = "rk_seq_plan_destroy";
-  std::lock_guard<std::mutex> lk(g_mu);
-  RK_TRY(ensure(op));
-  if (!plan) return RK_OK;
-  SeqPlan *p;
-  RK_TRY(seq_plan_get(plan, -1, &p, op));
-  // Calls and uploads that read its buffers end first; replays of a graph that
-  // holds them are known to the device alone.
-  if (p->captured) HIP_TRY(hipDeviceSynchronize(), op);
-  RK_TRY(seq_buf_wait(p->block, op));
-  RK_TRY(seq_buf_wait(p->work, op));
-  if (p->pin_ev) {
-    HIP_TRY(hipEventSynchronize(p->pin_ev), op);
-    (void)hipEventDestroy(p->pin_ev);
-  }
-  if (p->pin) (void)hipHostFree(p->pin);
-  seq_buf_free(p->block);
-  seq_buf_free(p->work);
-  g_eng->seq_plans.erase(p);
-  delete p;
-  return RK_OK;
+  return no_throw(op, [&]() -> int {
+    std::lock_guard<std::mutex> lk(g_mu);
+    RK_TRY(ensure(op));
+    if (!plan) return RK_OK;
+    SeqPlan *p;
+    RK_TRY(seq_plan_get(plan, -1, &p, op));
+    // Calls and uploads that read its buffers end first; replays of a graph that
+    // holds them are known to the device alone.
+    if (p->captured) HIP_TRY(hipDeviceSynchronize(), op);
+    RK_TRY(seq_buf_wait(p->block, op));
+    RK_TRY(seq_buf_wait(p->work, op));
+    if (p->pin_ev) {
+      HIP_TRY(hipEventSynchronize(p->pin_ev), op);
+      (void)hipEventDestroy(p->pin_ev);
+    }
+    if (p->pin) (void)hipHostFree(p->pin);
+    seq_buf_free(p->block);
+    seq_buf_free(p->work);
+    g_eng->seq_plans.erase(p);
+    delete p;
+    return RK_OK;
+  });
 }
 extern "C" int rk_attention_packed_dev(const void *plan, const void *q, int64_t q_stride, const void *k,
                                        int64_t k_stride, const void *v, int64_t v_stride, float scale, float softcap,
                                        void *out, int64_t out_stride, int dtype, rk_stream stream) {
-  return seq_attention(plan, false, q, q_stride, k, k_stride, v, v_stride, scale, softcap, out, out_stride, dtype,
-                       stream, "rk_attention_packed_dev");
+  return no_throw("rk_attention_packed_dev", [&] {
+    return seq_attention(plan, false, q, q_stride, k, k_stride, v, v_stride, scale, softcap, out, out_stride, dtype,
+                         stream, "rk_attention_packed_dev");
+  });
 }
 extern "C" int rk_attention_paged_dev(const void *plan, const void *q, int64_t q_stride, const void *k_cache,
                                       const void *v_cache, float scale, float softcap, void *out, int64_t out_stride,
                                       int dtype, rk_stream stream) {
-  return seq_attention(plan, true, q, q_stride, k_cache, 0, v_cache, 0, scale, softcap, out, out_stride, dtype, stream,
-                       "rk_attention_paged_dev");
+  return no_throw("rk_attention_paged_dev", [&] {
+    return seq_attention(plan, true, q, q_stride, k_cache, 0, v_cache, 0, scale, softcap, out, out_stride, dtype, stream,
+                         "rk_attention_paged_dev");
+  });
 }
 extern "C" int rk_paged_append_dev(const void *plan, const void *qkv, int64_t row_stride, const void *q_norm_w,
                                    const void *k_norm_w, double eps, const void *cos, const void *sin, int cs_dtype,
                                    int64_t n_pos, void *q_out, int64_t q_out_stride, void *k_cache, void *v_cache,
                                    int dtype, rk_stream stream) {
   const char *op = "rk_paged_append_dev";
-  std::lock_guard<std::mutex> lk(g_mu);
-  RK_TRY(ensure(op));
-  SeqPlan *p;
-  RK_TRY(seq_plan_get(plan, 1, &p, op));
-  const SeqGeom &g = p->geom;
-  if (dtype != RK_DTYPE_F16 && dtype != RK_DTYPE_BF16) return fail(RK_E_UNSUPPORTED, op, "dtype must be fp16 or bf16");
-  if (cs_dtype != dtype && cs_dtype != RK_DTYPE_F32)
-    return fail(RK_E_UNSUPPORTED, op, "cos/sin must have the element type of qkv or be f32");
-  if ((q_norm_w == nullptr) != (k_norm_w == nullptr)) return fail(RK_E_SHAPE, op, "give both norm weights or neither");
-  hipStream_t st = pick(stream);
-  bool capturing;
-  RK_TRY(is_capturing(st, &capturing, op));
-  if (capturing && p->reserved_q == 0) return fail(RK_E_UNSUPPORTED, op, "capture needs rk_seq_plan_reserve first");
-  if (p->lists.n_tokens == 0 && !capturing) return RK_OK;
-  const int heads = g.n_head + 2 * g.n_kv_heads;
-  RK_TRY(seq_rows_check(qkv, row_stride, (int64_t)heads * g.head_dim, "qkv", op));
-  RK_TRY(seq_rows_check(q_out, q_out_stride, (int64_t)g.n_head * g.head_dim, "q_out", op));
-  if (q_out == qkv && q_out_stride != row_stride)
-    return fail(RK_E_SHAPE, op, "q_out on qkv itself needs the same token stride");
-  for (const void *b : {(const void *)k_cache, (const void *)v_cache, cos, sin})
-    if (!b || ((uintptr_t)b & 15) != 0) return fail(RK_E_SHAPE, op, "k_cache, v_cache, cos and sin must be 16-byte aligned buffers");
-  if ((((uintptr_t)q_norm_w | (uintptr_t)k_norm_w) & 15) != 0) return fail(RK_E_SHAPE, op, "norm weights must be 16-byte aligned");
-  if (p->lists.max_pos >= n_pos)
-    return fail(RK_E_SHAPE, op, "the tables have " + std::to_string(n_pos) + " rows, the last new token is at " +
-                                    std::to_string(p->lists.max_pos));
-  if (p->lists.clash) return fail(RK_E_SHAPE, op, "two new tokens of the batch go to one slot of a page");
-  const int64_t n = capturing ? (int64_t)p->room.toks : p->lists.n_tokens;
-  if (n * heads > INT32_MAX) return fail(RK_E_SHAPE, op, "2^31 or more head rows");
-  CallScope cs(st);
-  RK_TRY(seq_buf_use(cs, p->block, capturing, op));
-  PagedAppendArgs a{};
-  a.qkv = qkv;
-  a.row_stride = row_stride;
-  a.q_norm_w = q_norm_w;
-  a.k_norm_w = k_norm_w;
-  a.eps = (float)eps;
-  a.cos = cos;
-  a.sin = sin;
-  a.q_out = q_out;
-  a.q_out_stride = q_out_stride;
-  a.k_cache = k_cache;
-  a.v_cache = v_cache;
-  a.toks = (const SeqTok *)((const uint8_t *)p->block.p + p->off_toks);
-  a.n_tokens = (int)n;
-  a.n_head = g.n_head;
-  a.n_kv_heads = g.n_kv_heads;
-  a.head_dim = g.head_dim;
-  while ((1 << a.page_log2) < g.page_size) ++a.page_log2;
-  if (n == 0) return RK_OK;
-  if (capturing) {
-    p->captured = true;
-    p->captured_pos = std::min(p->captured_pos, n_pos);
-  }
-  HIP_TRY(rk_launch_paged_append(a, dtype, cs_dtype, st), op);
-  return RK_OK;
+  return no_throw(op, [&]() -> int {
+    std::lock_guard<std::mutex> lk(g_mu);
+    RK_TRY(ensure(op));
+    SeqPlan *p;
+    RK_TRY(seq_plan_get(plan, 1, &p, op));
+    const SeqGeom &g = p->geom;
+    if (dtype != RK_DTYPE_F16 && dtype != RK_DTYPE_BF16) return fail(RK_E_UNSUPPORTED, op, "dtype must be fp16 or bf16");
+    if (cs_dtype != dtype && cs_dtype != RK_DTYPE_F32)
+      return fail(RK_E_UNSUPPORTED, op, "cos/sin must have the element type of qkv or be f32");
+    if ((q_norm_w == nullptr) != (k_norm_w == nullptr)) return fail(RK_E_SHAPE, op, "give both norm weights or neither");
+    hipStream_t st = pick(stream);
+    bool capturing;
+    RK_TRY(is_capturing(st, &capturing, op));
+    if (capturing && p->reserved_q == 0) return fail(RK_E_UNSUPPORTED, op, "capture needs rk_seq_plan_reserve first");
+    if (p->lists.n_tokens == 0 && !capturing) return RK_OK;
+    const int heads = g.n_head + 2 * g.n_kv_heads;
+    RK_TRY(seq_rows_check(qkv, row_stride, (int64_t)heads * g.head_dim, "qkv", op));
+    RK_TRY(seq_rows_check(q_out, q_out_stride, (int64_t)g.n_head * g.head_dim, "q_out", op));
+    if (q_out == qkv && q_out_stride != row_stride)
+      return fail(RK_E_SHAPE, op, "q_out on qkv itself needs the same token stride");
+    for (const void *b : {(const void *)k_cache, (const void *)v_cache, cos, sin})
+      if (!b || ((uintptr_t)b & 15) != 0) return fail(RK_E_SHAPE, op, "k_cache, v_cache, cos and sin must be 16-byte aligned buffers");
+    if ((((uintptr_t)q_norm_w | (uintptr_t)k_norm_w) & 15) != 0) return fail(RK_E_SHAPE, op, "norm weights must be 16-byte aligned");
+    if (p->lists.max_pos >= n_pos)
+      return fail(RK_E_SHAPE, op, "the tables have " + std::to_string(n_pos) + " rows, the last new token is at " +
+                                      std::to_string(p->lists.max_pos));
+    if (p->lists.clash) return fail(RK_E_SHAPE, op, "two new tokens of the batch go to one slot of a page");
+    const int64_t n = capturing ? (int64_t)p->room.toks : p->lists.n_tokens;
+    if (n * heads > INT32_MAX) return fail(RK_E_SHAPE, op, "2^31 or more head rows");
+    CallScope cs(st);
+    RK_TRY(seq_buf_use(cs, p->block, capturing, op));
+    PagedAppendArgs a{};
+    a.qkv = qkv;
+    a.row_stride = row_stride;
+    a.q_norm_w = q_norm_w;
+    a.k_norm_w = k_norm_w;
+    a.eps = (float)eps;
+    a.cos = cos;
+    a.sin = sin;
+    a.q_out = q_out;
+    a.q_out_stride = q_out_stride;
+    a.k_cache = k_cache;
+    a.v_cache = v_cache;
+    a.toks = (const SeqTok *)((const uint8_t *)p->block.p + p->off_toks);
+    a.n_tokens = (int)n;
+    a.n_head = g.n_head;
+    a.n_kv_heads = g.n_kv_heads;
+    a.head_dim = g.head_dim;
+    while ((1 << a.page_log2) < g.page_size) ++a.page_log2;
+    if (n == 0) return RK_OK;
+    if (capturing) {
+      p->captured = true;
+      p->captured_pos = std::min(p->captured_pos, n_pos);
+    }
+    HIP_TRY(rk_launch_paged_append(a, dtype, cs_dtype, st), op);
+    return RK_OK;
+  });
 }
 
 // =========================================================================

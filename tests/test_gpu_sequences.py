@@ -55,7 +55,19 @@ def check_packed(got, q, k, v, lens, h, kv, d, dtype, scale, softcap=0.0, mode=1
         at += n
 
 
+def crowd(h, kv):
+    """Sequences of one token that make a batch of these heads one with many tiles: its longer sequences go to the
+    kernel of many rows, not to that of few as in a small batch."""
+    return 1024 // (kv * -(-(h // kv) // 16)) + 1
+
+
 def packed_case(rk, seed, lens, h, kv, d, dtype, **kw):
+    one_packed_case(rk, seed, lens, h, kv, d, dtype, **kw)
+    if max(lens) * (h // kv) > 16:
+        one_packed_case(rk, seed, [*lens, *[1] * crowd(h, kv)], h, kv, d, dtype, **kw)
+
+
+def one_packed_case(rk, seed, lens, h, kv, d, dtype, **kw):
     rng, toks = np.random.default_rng(seed), sum(lens)
     q, k, v = (rows(rng, dtype, toks, n * d) for n in (h, kv, kv))
     got = packed(rk, q, k, v, lens, h, kv, d, dtype, d ** -0.5, extra=3, **kw)
@@ -117,31 +129,45 @@ def test_packed_reads_a_fused_projection_where_it_lies(rk):
 def test_packed_large_and_rising_scores(rk):
     """Scores in the hundreds that rise along the keys, and one key that outweighs the others."""
     note("packed, rising scores")
-    rng, n, h, kv, d = np.random.default_rng(7), 900, 4, 1, 128
+    rng, n, h, kv, d = np.random.default_rng(7), 1900, 4, 1, 128
     q, v = rows(rng, "f16", n, h * d), rows(rng, "f16", n, kv * d)
     k = ref.encode(rng.standard_normal((n, kv * d)) * np.linspace(0.1, 6, n)[:, None], "f16")
-    for mode in (0, 1):
-        check_packed(packed(rk, q, k, v, [n], h, kv, d, "f16", 1.0, mode=mode), q, k, v, [n], h, kv, d, "f16", 1.0, mode=mode)
+    for lens in ([n - more, *[1] * more] for more in (0, crowd(h, kv))):
+        for mode in (0, 1):
+            check_packed(packed(rk, q, k, v, lens, h, kv, d, "f16", 1.0, mode=mode), q, k, v, lens, h, kv, d, "f16", 1.0, mode=mode)
 
 
-def test_packed_hidden_keys_that_are_not_finite(rk):
+@pytest.mark.parametrize("many", [False, True])
+def test_packed_hidden_keys_that_are_not_finite(rk, many):
     """NaN and infinities in keys that a row does not see leave its scores alone; a value that no row of the
     sequence's other tiles sees does not reach them."""
     note("packed, NaN in hidden keys")
     rng, n, h, kv, d = np.random.default_rng(8), 300, 2, 1, 64
-    q, k, v = (rows(rng, "f16", n, m * d) for m in (h, kv, kv))
+    lens = [n, *[1] * crowd(h, kv) * many]
+    q, k, v = (rows(rng, "f16", sum(lens), m * d) for m in (h, kv, kv))
     bad = k.copy()
     bad[290] = 0x7E00  # NaN
     bad[295] = 0x7C00  # infinity
-    got = packed(rk, q, bad, v, [n], h, kv, d, "f16", d ** -0.5)
-    want = packed(rk, q, k, v, [n], h, kv, d, "f16", d ** -0.5)
-    assert (got[:290] == want[:290]).all()
+    got = packed(rk, q, bad, v, lens, h, kv, d, "f16", d ** -0.5)
+    want = packed(rk, q, k, v, lens, h, kv, d, "f16", d ** -0.5)
+    assert (got[:290] == want[:290]).all() and (got[n:] == want[n:]).all()
     # a NaN value beyond the window of every row of the first tiles
     badv = v.copy()
     badv[299] = 0x7E00
-    got = packed(rk, q, k, badv, [n], h, kv, d, "f16", d ** -0.5, mode=2, window=20)
-    want = packed(rk, q, k, v, [n], h, kv, d, "f16", d ** -0.5, mode=2, window=20)
-    assert (got[:128] == want[:128]).all()
+    got = packed(rk, q, k, badv, lens, h, kv, d, "f16", d ** -0.5, mode=2, window=20)
+    want = packed(rk, q, k, v, lens, h, kv, d, "f16", d ** -0.5, mode=2, window=20)
+    assert (got[:128] == want[:128]).all() and (got[n:] == want[n:]).all()
+
+
+@pytest.mark.parametrize("many", [False, True])
+@pytest.mark.parametrize("scale,softcap", [(0.0, 0.0), (-0.2, 0.0), (-0.2, 8.0), (0.0, 8.0)])
+def test_packed_scales_of_zero_and_below(rk, scale, softcap, many):
+    note(f"packed, scale {scale} softcap {softcap}")
+    rng, h, kv, d = np.random.default_rng(9), 4, 2, 96
+    lens = [170, 20, *[1] * crowd(h, kv) * many]
+    q, k, v = (rows(rng, "bf16", sum(lens), m * d) for m in (h, kv, kv))
+    got = packed(rk, q, k, v, lens, h, kv, d, "bf16", scale, softcap)
+    check_packed(got, q, k, v, lens, h, kv, d, "bf16", scale, softcap)
 
 
 # ------------------------------------------------------------------- paged ----
@@ -184,7 +210,20 @@ def check_paged(got, keys, q, q_lens, kv_lens, h, kv, d, dtype, scale, softcap=0
 
 
 def paged_case(rk, seed, q_lens, kv_lens, ps, h, kv, d, dtype, **kw):
+    one_paged_case(rk, seed, q_lens, kv_lens, ps, h, kv, d, dtype, 0, **kw)
+    if max(q_lens) * (h // kv) > 16:
+        one_paged_case(rk, seed, q_lens, kv_lens, ps, h, kv, d, dtype, crowd(h, kv), **kw)
+
+
+def one_paged_case(rk, seed, q_lens, kv_lens, ps, h, kv, d, dtype, more, **kw):
+    """`more` sequences of one token with two keys, all in one page that they share."""
+    q_lens, kv_lens = [*q_lens, *[1] * more], [*kv_lens, *[2] * min(more, 1)]
     pg, caches, keys, q = paged_inputs(seed, kv_lens, ps, h, kv, d, dtype, q_lens)
+    if more:
+        kv_lens += [2] * (more - 1)
+        pg.table = np.concatenate([pg.table, np.repeat(pg.table[-1:], more - 1, axis=0)])
+        for t in keys:
+            t += t[-1:] * (more - 1)
     got = paged(rk, pg, caches, q, q_lens, kv_lens, h, kv, d, dtype, d ** -0.5, **kw)
     check_paged(got, keys, q, q_lens, kv_lens, h, kv, d, dtype, d ** -0.5, **kw)
     assert (paged(rk, pg, caches, q, q_lens, kv_lens, h, kv, d, dtype, d ** -0.5, **kw) == got).all()
@@ -574,6 +613,64 @@ def test_captured_step_replays_with_updates(rk):
         plan.update([5], [10], pg.table[:1], stream=st)
     with pytest.raises(rk.RocketError):  # past the tables that the graph reads
         plan.update([1], [4097], np.zeros((1, 300), np.int32), stream=st)
+    g.destroy()
+    plan.destroy()
+    rk.destroy_stream(st)
+
+
+def test_captured_packed_batches_of_both_kinds(rk):
+    """One graph, replayed on batches that are small, that have long sequences among many short ones, and empty."""
+    note("graph capture, packed")
+    h, kv, d, n = 8, 2, 128, 1200
+    rng, lib, st = np.random.default_rng(31), rk.lib(), rk.new_stream()
+    q, k, v = (rows(rng, "bf16", n, m * d) for m in (h, kv, kv))
+    filled = np.full((n, h * d), FILL, np.uint16)
+    b = upload(rk, q, k, v, filled)
+    plan = rk.packed_plan([2] * 600, h, kv, d)
+    plan.reserve(500)
+    g = Graph(st, lambda: ok(rk, lib.rk_attention_packed_dev(plan.ptr, b[0].ptr, h * d, b[1].ptr, kv * d, b[2].ptr, kv * d, 0.1, 0.0,
+                                                             b[3].ptr, h * d, rk.DTYPE_BF16, st)))
+    for lens in ([2] * 600, [500, 3, 77], [400, *[1] * 520], [0, 0], [500, 200, *[1] * 500], [1]):
+        plan.update(lens, stream=st)
+        seen = []
+        for _ in range(3):
+            b[3].upload(filled)
+            g.replay()
+            rk.synchronize(st)
+            seen.append(b[3].download(filled.shape, np.uint16))
+        t = sum(lens)
+        assert all((o == seen[0]).all() for o in seen) and (seen[0][t:] == FILL).all()
+        check_packed(seen[0][:t], q, k, v, lens, h, kv, d, "bf16", 0.1)
+    g.destroy()
+    plan.destroy()
+    rk.destroy_stream(st)
+
+
+@pytest.mark.parametrize("h,kv,d,max_q", [(8, 2, 128, 1), (8, 2, 64, 40), (4, 4, 256, 400), (64, 1, 32, 64), (48, 48, 80, 7)])
+def test_a_reserved_plan_has_room_for_every_smaller_batch(rk, h, kv, d, max_q):
+    """A plan that a graph holds takes any batch of no more sequences, tokens and pages, short or long, few or many."""
+    note(f"reserve {h}/{kv} d={d} q_len {max_q}")
+    rng, ps, n_seqs, toks, n_pages = np.random.default_rng(d), 64, 40, 900, 4000
+    q = [max_q] * (toks // max_q) if max_q > 22 else [max_q] * n_seqs
+    q += [0] * (n_seqs - len(q))
+    toks = sum(q)
+    table = np.arange(n_seqs * 100, dtype=np.int32).reshape(n_seqs, 100)
+    plan, st = rk.paged_plan(q, [6400 if x else 0 for x in q], table, n_pages, ps, h, kv, d), rk.new_stream()
+    pages = 100 * sum(x > 0 for x in q)
+    plan.reserve(max_q)
+    (buf,) = upload(rk, np.zeros(64, np.uint16))  # (the graph is not launched)
+    g = Graph(st, lambda: ok(rk, rk.lib().rk_attention_paged_dev(plan.ptr, buf.ptr, h * d, buf.ptr, buf.ptr, 0.1, 0.0, buf.ptr, h * d,
+                                                                 rk.DTYPE_F16, st)))
+    for i in range(150):
+        n = int(rng.integers(1, n_seqs + 1))
+        left, held, ql, kl = toks, pages, [], []
+        for _ in range(n):
+            x = int(min(left, max_q, rng.choice([1, max_q, int(rng.integers(0, max_q + 1))])))
+            m = int(min(6400, held * ps, max(x, rng.choice([x, 100, 6400, int(rng.integers(1, 6401))])))) if x else 0
+            x = min(x, m)
+            left, held, ql, kl = left - x, held - -(-m // ps), [*ql, x], [*kl, m]
+        plan.update(ql, kl, table[:n], stream=st)
+    rk.synchronize(st)
     g.destroy()
     plan.destroy()
     rk.destroy_stream(st)
