@@ -162,19 +162,23 @@ void seq_build(const SeqGeom &g, const SeqBatch &b, int num_cus, SeqLists *out) 
     int32_t page, off, end;
   };
   std::vector<Piece> pieces;  // where new tokens go: slots [off, end) of a page
-  // A small batch goes to the kernel of few rows whole: at most four tiles of 16 rows
-  // per CU with few keys (each is a short wait there), or one per CU with 4096 keys (past
-  // that the tiles' own reads of K and V cost more than what the other kernel's shared
-  // ones wait for). MI355X, 32/4 heads of 128, rows -> tiles: 256 rows on 4096 keys 18.1
-  // us, 35.7; 128 rows on 30000 41.8, 50.9; 256 rows on 30000 73, 52; 16 times 64 rows
-  // on 2000 25.2, 29.8; on 8000 78, 60; 16 times 96 rows on 300 14.6, 11.9.
-  int64_t n16 = 0, n16_keys = 0;
+  // A small batch goes to the kernel of few rows whole: at most four tiles of 16 rows per
+  // CU whose products (each tile reads its K and V itself) take less than the other
+  // kernel's walk over the longest sequence. MI355X, rows -> tiles: 256 rows on 4096 keys,
+  // 32/4 heads of 128, 18 us, 36; 128 rows on 30000 42, 51; 256 rows on 30000 73, 52;
+  // 16 times 64 on 2000 25, 30; 16 times 96 on 300 14.6, 11.9. One prompt, causal: 300
+  // tokens of 16/8 heads of 128 9.6, 11.3; 600 19.3, 17.9; 800 of 12/12 heads of 64 11.3,
+  // 15.8; 1200 18.0, 15.6; 200 of 32/4 heads of 128 10.0, 9.8; 300 15.7, 11.4.
+  int64_t n16 = 0, n16_keys = 0, longest = 0;
   for (int64_t i = 0; i < b.n_seqs; ++i) {
+    if (b.q_lens[i] == 0) continue;
     const int64_t t = ceil_div(b.q_lens[i] * G, 16) * g.n_kv_heads;
     n16 += t;
     n16_keys += t * kv_of(b, i);
+    longest = std::max(longest, kv_of(b, i));
   }
-  const bool small = n16_keys <= 4096ll * num_cus && (n16 <= num_cus || (n16 <= 4 * num_cus && n16_keys <= 128 * n16));
+  const bool small = n16 <= 4 * num_cus && n16_keys <= 4096ll * num_cus &&
+                     n16_keys * g.head_dim <= num_cus * (14000 + 140 * longest);
   for (int64_t i = 0; i < b.n_seqs; ++i) {
     const int64_t q = b.q_lens[i], kv = kv_of(b, i), pos0 = kv - q;
     if (q == 0) continue;
