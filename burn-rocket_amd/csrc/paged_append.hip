@@ -12,6 +12,8 @@
 // the rotation needs no other lane and each lane has two loads in flight per
 // row; D/(2·CV) lanes make a row (rounded up to a power of two), the sum of
 // squares is a butterfly over them. V heads take the same lanes and are copied.
+// MI355X: six prompts of 900 to 2400 tokens, 32/4 heads of 128, norm, bf16: 30.8 us (184 MB,
+// 6.0 TB/s); 48 rows of 16/8 heads of 128 3.4 us, which is a launch and two trips to memory.
 #include <algorithm>
 
 #include "common.hpp"

@@ -18,6 +18,11 @@
 // its own: what lies past the sequence's keys reads as zeros without a branch. The
 // addresses of a wave's next 32 chunks wait in registers (lane l: block l).
 //
+// MI355X: 64 sequences of one token on 100 to 8000 keys, 16/8 heads of 128, 185 us (1.08
+// GB, 5.8 TB/s; a copy of 2 GiB moves 4.7); three on 60000 to 131072, 32/4
+// heads of 128, 102 us (5.4 TB/s); one token on 4097 keys, 32/4 heads of 128, 10.5
+// us: a launch, one trip for the lists, one for K and V, and three for the states.
+//
 // An item that is one of n_parts of its tile puts its state (Oᵀ unnormalised, m, l)
 // into the plan's workspace; the workgroup that arrives last merges all of them in
 // key order, whichever it is. Nothing waits on another workgroup.
