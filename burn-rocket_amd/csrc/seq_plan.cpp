@@ -56,16 +56,16 @@ std::string seq_check_batch(const SeqGeom &g, const SeqBatch &b) {
   const int64_t G = g.n_head / g.n_kv_heads;
   int64_t toks = 0, ids = 0;
   for (int64_t i = 0; i < b.n_seqs; ++i) {
-    const std::string at = "sequence " + std::to_string(i) + ": ";
+    const auto at = [&](const std::string &what) { return "sequence " + std::to_string(i) + ": " + what; };
     const int64_t q = b.q_lens[i], kv = kv_of(b, i);
-    if (q < 0 || kv < q) return at + "needs 0 <= q_len <= kv_len";
-    if (kv > MAX_KEYS) return at + "more than 2^30 keys";
-    if (q * G > INT32_MAX) return at + "q_len·(n_head/n_kv_heads) of 2^31 or more";
+    if (q < 0 || kv < q) return at("needs 0 <= q_len <= kv_len");
+    if (kv > MAX_KEYS) return at("more than 2^30 keys");
+    if (q * G > INT32_MAX) return at("q_len·(n_head/n_kv_heads) of 2^31 or more");
     toks += q;
     if (toks > INT32_MAX) return "2^31 or more new tokens";
     if (!g.paged || q == 0) continue;
     const int64_t pages = ceil_div(kv, g.page_size);
-    if (pages > b.table_stride) return at + "its keys need more pages than a table row holds";
+    if (pages > b.table_stride) return at("its keys need more pages than a table row holds");
     ids += pages;
     if (ids > INT32_MAX) return "2^31 or more page ids";
     int64_t lo, hi;
@@ -73,7 +73,7 @@ std::string seq_check_batch(const SeqGeom &g, const SeqBatch &b) {
     for (int64_t p = lo / g.page_size; p < pages; ++p) {
       const int32_t id = b.page_table[i * b.table_stride + p];
       if (id < 0 || id >= g.n_pages)
-        return at + "page " + std::to_string(p) + " has id " + std::to_string(id) + " of " + std::to_string(g.n_pages);
+        return at("page " + std::to_string(p) + " has id " + std::to_string(id) + " of " + std::to_string(g.n_pages));
     }
   }
   // items and merges are counted with 32 bits, a launch's workgroups too

@@ -126,6 +126,21 @@ def test_packed_reads_a_fused_projection_where_it_lies(rk):
     check_packed(got[:, :h * d], q, k, v, lens, h, kv, d, "bf16", 0.1)
 
 
+@pytest.mark.parametrize("lens,h,kv,d", [([1500], 8, 1, 64), ([5, 1, 700, *[1] * 300], 16, 4, 128), ([900, 40], 3, 1, 256),
+                                         ([20, 300], 4, 4, 72)])
+def test_packed_onto_the_queries(rk, lens, h, kv, d):
+    """out on q itself: the split tiles too read all of their queries before a row is stored."""
+    note(f"packed in place {h}/{kv} d={d}")
+    rng, toks = np.random.default_rng(d), sum(lens)
+    q, k, v = (rows(rng, "f16", toks, n * d) for n in (h, kv, kv))
+    want = packed(rk, q, k, v, lens, h, kv, d, "f16", 0.1)
+    plan, b = rk.packed_plan(lens, h, kv, d), upload(rk, q, k, v)
+    ok(rk, rk.lib().rk_attention_packed_dev(plan.ptr, b[0].ptr, h * d, b[1].ptr, kv * d, b[2].ptr, kv * d, 0.1, 0.0, b[0].ptr, h * d,
+                                            rk.DTYPE_F16, None))
+    rk.synchronize()
+    assert (b[0].download(want.shape, np.uint16) == want).all()
+
+
 def test_packed_large_and_rising_scores(rk):
     """Scores in the hundreds that rise along the keys, and one key that outweighs the others."""
     note("packed, rising scores")
@@ -618,10 +633,11 @@ def test_captured_step_replays_with_updates(rk):
     rk.destroy_stream(st)
 
 
-def test_captured_packed_batches_of_both_kinds(rk):
+@pytest.mark.parametrize("d", [128, 256])
+def test_captured_packed_batches_of_both_kinds(rk, d):
     """One graph, replayed on batches that are small, that have long sequences among many short ones, and empty."""
-    note("graph capture, packed")
-    h, kv, d, n = 8, 2, 128, 1200
+    note(f"graph capture, packed, d={d}")
+    h, kv, n = 8, 2, 1200
     rng, lib, st = np.random.default_rng(31), rk.lib(), rk.new_stream()
     q, k, v = (rows(rng, "bf16", n, m * d) for m in (h, kv, kv))
     filled = np.full((n, h * d), FILL, np.uint16)
