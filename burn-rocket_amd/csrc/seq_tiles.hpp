@@ -27,10 +27,10 @@
 // zeros. They start with the softmax, which their latency hides behind; issued between
 // products they held those up.
 //
-// MI355X: two prompts of 7000 tokens, 32/4 heads of 128, causal, bf16, 750-790 us (1.05-1.1
+// MI355X: two prompts of 7000 tokens, 32/4 heads of 128, causal, bf16, 735-790 us (1.05-1.13
 // PFLOP/s; the library's 8192³ product reaches 1.2), the matrix cores busy 53 % of the
-// clocks. 512 rows of 8 heads on 16901 keys 146 us (0.96 PFLOP/s, 17 us of it the states
-// of 4 parts a tile). 64 passages of 100 to 512 tokens 81 us (3 TB/s): items of three key
+// clocks. 512 rows of 8 heads on 16901 keys 138 us (1.01 PFLOP/s, 17 us of it the states
+// of 4 parts a tile). 64 passages of 100 to 512 tokens 76 us (3.2 TB/s): items of three key
 // tiles, whose first loads and last stores nothing hides. Head dim 256 has one 16-query
 // block per wave: every product reads its own 1 KB from LDS, twice the CU's rate. 45 us for
 // 9261 tokens, 3/1 heads, 512 keys to either side; 128 rows a workgroup, one per CU, 58.
@@ -254,18 +254,23 @@ __device__ __forceinline__ void seq_tiles_item(const SeqAttnArgs &a, int block, 
 #pragma unroll
           for (int e = 0; e < 4; ++e) s[b][qb][e] = a.softcap * tanhf(s[b][qb][e] * scale / a.softcap);
     }
-    if (a.uniform || key0 < full_lo || key0 + TK - 1 > full_hi) {
+    const auto each = [&](auto f) ALWAYS_INLINE {  // (s, its key from the lane's first of the tile on, query block)
 #pragma unroll
       for (int b = 0; b < NB; ++b)
 #pragma unroll
         for (int qb = 0; qb < QB; ++qb)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int key = key0 + 16 * b + 4 * lg + e;
-            const float v = a.uniform ? 0.f : s[b][qb][e];
-            s[b][qb][e] = key < klo[qb] || key > khi[qb] ? -INFINITY : v;
-          }
-    }
+          for (int e = 0; e < 4; ++e) s[b][qb][e] = f(s[b][qb][e], 16 * b + e, qb);
+    };
+    // One comparison an element, and only on the tiles that an end of the keys crosses: both
+    // ends and `uniform` tested at once took 80.4 us for the passages, 79.4 so, and 145 to 143
+    // for the 512 rows.
+    const int lane_key = key0 + 4 * lg;
+    if (a.uniform) each([](float, int, int) ALWAYS_INLINE { return 0.f; });
+    if (key0 + TK - 1 > full_hi)
+      each([&](float x, int k, int qb) ALWAYS_INLINE { return k > khi[qb] - lane_key ? -INFINITY : x; });
+    if (key0 < full_lo)
+      each([&](float x, int k, int qb) ALWAYS_INLINE { return k < klo[qb] - lane_key ? -INFINITY : x; });
     float mt[QB];
     bool up = false;
 #pragma unroll
