@@ -104,6 +104,22 @@ def test_packed_long(rk, lens, h, kv, d, dtype, mode):
     packed_case(rk, sum(lens), lens, h, kv, d, dtype, mode=mode)
 
 
+@pytest.mark.parametrize("lens,h,kv,d", [([1, 40, 300], 128, 1, 32), ([130, 1], 256, 2, 48), ([90, 3, 17], 300, 300, 32),
+                                         ([20, 1], 600, 600, 64)])
+def test_packed_widest_groups_and_many_kv_heads(rk, lens, h, kv, d):
+    note(f"packed {lens} {h}/{kv} d={d}")
+    packed_case(rk, h, lens, h, kv, d, "f16")
+
+
+def test_empty_batches(rk):
+    note("empty batches")
+    for plan in (rk.packed_plan([], 4, 2, 64), rk.paged_plan([], [], np.zeros((0, 0), np.int32), 1, 16, 4, 2, 64),
+                 rk.paged_plan([0, 0], [0, 9], np.full((2, 1), -1), 1, 16, 4, 2, 64)):
+        assert plan.n_tokens == 0
+        plan.reserve()
+        plan.destroy()
+
+
 def test_packed_many_short_sequences(rk):
     note("packed, 700 sequences")
     packed_case(rk, 3, [1 + i % 7 for i in range(700)], 4, 2, 64, "f16")
