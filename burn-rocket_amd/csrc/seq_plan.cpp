@@ -96,15 +96,17 @@ int64_t slots_per_head(const SeqGeom &g, int num_cus, bool one) {
 // 206 in 516 on MI355X). More: only tiles longer than 5/4 of an even share. None where
 // the longest would shrink by less than `cost` steps, which is what states to
 // store and merge take (about 20 us for tiles of 128 rows).
-void split(std::vector<SeqItem> &tiles, int step, int64_t slots, int64_t least, int64_t cost, SeqList *out) {
+void split(std::vector<SeqItem> &tiles, int step, int64_t slots, int64_t least, int64_t cost, int64_t most,
+           SeqList *out) {
   const auto steps = [&](const SeqItem &t) { return ceil_div(t.k_end - t.k_begin, step); };
   int64_t total = 0, longest = 0;
   for (const SeqItem &t : tiles) {
     total += steps(t);
     longest = std::max(longest, steps(t));
   }
-  // (16 states are merged in one pass)
-  const int64_t max_parts = longest <= 32 * 16 ? 16 : SEQ_MAX_PARTS;
+  // (16 states are merged in one pass: one token on 8000 keys, 4 kv heads of 128, 12.6 us with
+  // 16 parts, 13.7 with 32; on 16000 17.4, 16.0)
+  const int64_t max_parts = longest <= 32 * 16 ? 16 : most;
   int64_t quota = std::max(least, ceil_div(total, slots));
   if ((int64_t)tiles.size() < slots) {
     const auto items = [&](int64_t q) {
@@ -134,8 +136,11 @@ void split(std::vector<SeqItem> &tiles, int step, int64_t slots, int64_t least, 
   std::stable_sort(out->items.begin(), out->items.end(),
                    [&](const SeqItem &x, const SeqItem &y) { return steps(x) > steps(y); });
 }
-// Steps of an item at least (a chunk for each wave), and steps that a split costs.
-constexpr int64_t ROWS_LEAST = 8, ROWS_COST = 8, TILES_LEAST = 4, TILES_COST = 12;
+// Steps of an item at least, and steps that a split costs. (Row items of 4 chunks leave
+// half the waves idle, but none with a second: one token on 500 keys, 4 kv heads of 128,
+// 8.9 us, with 8 chunks 10.0.)
+constexpr int64_t ROWS_LEAST = 4, ROWS_COST = 8, TILES_LEAST = 4, TILES_COST = 12;
+constexpr int64_t PARTS = 32;  // of a tile at most
 }  // namespace
 
 void seq_bound(const SeqGeom &g, int64_t n_seqs, int64_t n_tokens, int64_t max_q, int num_cus, SeqBound *rows,
@@ -216,8 +221,12 @@ void seq_build(const SeqGeom &g, const SeqBatch &b, int num_cus, SeqLists *out) 
       t = e;
     }
   }
-  split(rows, SEQ_ROWS_CHUNK, slots_per_head(g, num_cus, tiles.empty() || !seq_one_launch(g.head_dim)), ROWS_LEAST, ROWS_COST, &out->rows);
-  split(tiles, SEQ_KEY_TILE, slots_per_head(g, num_cus, false), TILES_LEAST, TILES_COST, &out->tiles);
+  // Twice the parts where those leave three quarters of the CUs idle: one token on 60000
+  // keys, one kv head of 128, 27 us, 24; of 256 51, 45; with four heads of 128 28.8, 31.4.
+  const int64_t most = 4 * PARTS * (int64_t)rows.size() * g.n_kv_heads <= num_cus ? 2 * PARTS : PARTS;
+  split(rows, SEQ_ROWS_CHUNK, slots_per_head(g, num_cus, tiles.empty() || !seq_one_launch(g.head_dim)), ROWS_LEAST, ROWS_COST,
+        most, &out->rows);
+  split(tiles, SEQ_KEY_TILE, slots_per_head(g, num_cus, false), TILES_LEAST, TILES_COST, PARTS, &out->tiles);
   std::sort(pieces.begin(), pieces.end(),
             [](const Piece &x, const Piece &y) { return x.page != y.page ? x.page < y.page : x.off < y.off; });
   for (size_t i = 1; i < pieces.size(); ++i)

@@ -292,7 +292,7 @@ def test_paged_masks(rk, mode, window, softcap, h, kv, d):
 
 @pytest.mark.parametrize("q_lens,kv_lens,ps,h,kv,d,dtype", [
     ([1], [9001], 16, 32, 4, 128, "f16"), ([1], [20011], 64, 8, 8, 64, "bf16"), ([1, 1, 1], [6000, 33, 12345], 128, 4, 1, 256, "f16"),
-    ([64], [5000], 64, 8, 2, 128, "f16"), ([300], [3000], 16, 4, 4, 96, "f16"), ([200, 1, 1, 1], [2500, 2000, 70, 4100], 32, 16, 4, 64, "bf16")])
+    ([1], [40003], 64, 4, 1, 64, "f16"), ([64], [5000], 64, 8, 2, 128, "f16"), ([300], [3000], 16, 4, 4, 96, "f16"), ([200, 1, 1, 1], [2500, 2000, 70, 4100], 32, 16, 4, 64, "bf16")])
 def test_paged_long(rk, q_lens, kv_lens, ps, h, kv, d, dtype):
     note(f"paged long {q_lens} of {kv_lens}")
     paged_case(rk, sum(kv_lens), q_lens, kv_lens, ps, h, kv, d, dtype)
