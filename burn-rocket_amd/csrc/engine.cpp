@@ -2559,6 +2559,12 @@ int seq_reserve(SeqPlan &p, const SeqPlan::Room &want, const char *op) {
   return RK_OK;
 }
 
+// After a failure: an empty batch rather than lists that the device may not hold.
+void seq_forget(SeqPlan &p) {
+  p.lists = SeqLists{};
+  p.n_seqs = 0;
+}
+
 // The lists grow with the batch: a failed host allocation is a status here.
 template <typename F>
 int no_throw(const char *op, F &&f) {
@@ -2635,23 +2641,19 @@ int seq_plan_update(void *plan, bool paged, const SeqBatch &b, rk_stream stream,
   if (p->pin_ev) HIP_TRY(hipEventSynchronize(p->pin_ev), op);  // the image's last upload has left it
   p->lists = std::move(l);
   p->n_seqs = b.n_seqs;
-  int rc = seq_reserve(*p, seq_room(p->lists), op);
-  if (rc == RK_OK && !p->pin) {
-    const hipError_t e = hipHostMalloc((void **)&p->pin, p->block.bytes, hipHostMallocDefault);
-    if (e != hipSuccess) rc = hip_fail(e, op);
-  }
-  if (rc != RK_OK) {  // an empty batch rather than lists that the device does not hold
-    p->lists = SeqLists{};
-    p->n_seqs = 0;
-    return rc;
-  }
-  seq_image(*p, p->pin);
-  CallScope cs(st);
-  RK_TRY(seq_buf_use(cs, p->block, false, op));
-  HIP_TRY(rk_launch_upload(p->pin, p->block.p, p->block.bytes, st), op);
-  if (!p->pin_ev) HIP_TRY(hipEventCreateWithFlags(&p->pin_ev, hipEventDisableTiming), op);
-  HIP_TRY(hipEventRecord(p->pin_ev, st), op);
-  return RK_OK;
+  const int rc = [&]() -> int {
+    RK_TRY(seq_reserve(*p, seq_room(p->lists), op));
+    if (!p->pin) HIP_TRY(hipHostMalloc((void **)&p->pin, p->block.bytes, hipHostMallocDefault), op);
+    if (!p->pin_ev) HIP_TRY(hipEventCreateWithFlags(&p->pin_ev, hipEventDisableTiming), op);
+    seq_image(*p, p->pin);
+    CallScope cs(st);
+    RK_TRY(seq_buf_use(cs, p->block, false, op));
+    HIP_TRY(rk_launch_upload(p->pin, p->block.p, p->block.bytes, st), op);
+    HIP_TRY(hipEventRecord(p->pin_ev, st), op);
+    return RK_OK;
+  }();
+  if (rc != RK_OK) seq_forget(*p);
+  return rc;
 }
 
 int seq_rows_check(const void *p, int64_t stride, int64_t width, const char *what, const char *op) {
@@ -2787,12 +2789,18 @@ extern "C" int rk_seq_plan_reserve(void *plan, int64_t max_q_len) {
     want.tile_parts = (size_t)tiles.parts;
     RK_TRY(seq_buf_wait(p->block, op));
     RK_TRY(seq_buf_wait(p->work, op));
-    RK_TRY(seq_reserve(*p, want, op));
-    std::vector<uint8_t> image(p->block.bytes);
-    seq_image(*p, image.data());
-    HIP_TRY(hipMemcpy(p->block.p, image.data(), image.size(), hipMemcpyHostToDevice), op);
-    p->reserved_q = longest;
-    return RK_OK;
+    const int rc = no_throw(op, [&]() -> int {
+      RK_TRY(seq_reserve(*p, want, op));
+      std::vector<uint8_t> image(p->block.bytes);
+      seq_image(*p, image.data());
+      HIP_TRY(hipMemcpy(p->block.p, image.data(), image.size(), hipMemcpyHostToDevice), op);
+      return RK_OK;
+    });
+    if (rc == RK_OK)
+      p->reserved_q = longest;
+    else
+      seq_forget(*p);
+    return rc;
   });
 }
 extern "C" int rk_seq_plan_destroy(void *plan) {

@@ -432,7 +432,9 @@ int rk_flash_attn_f16_masked(int64_t n_q, int64_t n_kv, int head_dim, int dv, in
  * The lists are copied: the caller's arrays may go when a call returns. An
  * update gives the plan another batch of the same heads, mask and pages; it is
  * ordered on `stream` after the calls that used the plan, waits on the host for
- * the upload of the update before it, and is refused inside a stream capture.
+ * the upload of the update before it, and is refused inside a stream capture. A
+ * refused batch (RK_E_SHAPE) leaves the plan as it was; an update or a reserve that
+ * fails for want of memory leaves it with an empty batch.
  *
  * Streams: calls on one plan from different streams run one after another. Before
  * a call is captured into a graph, rk_seq_plan_reserve gives the plan room for any
