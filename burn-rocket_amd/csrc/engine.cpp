@@ -2559,10 +2559,12 @@ int seq_reserve(SeqPlan &p, const SeqPlan::Room &want, const char *op) {
   return RK_OK;
 }
 
-// After a failure: an empty batch rather than lists that the device may not hold.
+// After a failure: an empty batch rather than lists that the device may not hold, and no
+// capture of them before another reserve (a graph that has the buffers has their old lists).
 void seq_forget(SeqPlan &p) {
   p.lists = SeqLists{};
   p.n_seqs = 0;
+  if (!p.captured) p.reserved_q = 0;
 }
 
 // The lists grow with the batch: a failed host allocation is a status here.
