@@ -132,7 +132,8 @@ struct SeqPlan {
   hipEvent_t pin_ev = nullptr;  // its last upload
   int64_t reserved_q = 0;       // > 0: rk_seq_plan_reserve'd, for q_lens up to this
   bool captured = false;        // a graph holds these buffers: they are not replaced
-  int64_t captured_pos = INT64_MAX;  // rows of the shortest cos/sin tables that a captured append reads
+  int64_t captured_pos = INT64_MAX;   // rows of the shortest cos/sin tables that a captured append reads
+  int64_t captured_toks = INT64_MAX;  // tokens that every captured call's buffers have room for
 };
 
 struct Engine {
@@ -2637,6 +2638,9 @@ int seq_plan_update(void *plan, bool paged, const SeqBatch &b, rk_stream stream,
   if (p->captured) {
     if (!p->room.holds(seq_room(l)) || l.max_q > p->reserved_q)
       return fail(RK_E_SHAPE, op, "a graph holds this plan, and the batch needs more than was reserved");
+    if (l.n_tokens > p->captured_toks)
+      return fail(RK_E_SHAPE, op, "a graph holds this plan, and its buffers have room for " +
+                                      std::to_string(p->captured_toks) + " tokens");
     if (p->captured_pos != INT64_MAX && (l.clash || l.max_pos >= p->captured_pos))
       return fail(RK_E_SHAPE, op, "a graph's append reads this plan: two new tokens in one slot, or past its cos/sin tables");
   }
@@ -2714,7 +2718,10 @@ int seq_attention(const void *plan, bool paged, const void *q, int64_t q_stride,
   // for long ones.
   const size_t n_rows = capturing ? p->room.rows : p->lists.rows.items.size();
   const size_t n_tiles = capturing ? p->room.tiles : p->lists.tiles.items.size();
-  if (capturing) p->captured = true;
+  if (capturing) {
+    p->captured = true;
+    p->captured_toks = std::min(p->captured_toks, p->lists.n_tokens);
+  }
   uint8_t *work = (uint8_t *)p->work.p;
   a.rows = SeqListArgs{(const SeqItem *)block, (int)n_rows, work + p->off_rows, (unsigned *)work};
   a.tiles = SeqListArgs{(const SeqItem *)(block + p->off_tiles), (int)n_tiles, work + p->off_tile_part,
@@ -2904,6 +2911,7 @@ extern "C" int rk_paged_append_dev(const void *plan, const void *qkv, int64_t ro
     if (capturing) {
       p->captured = true;
       p->captured_pos = std::min(p->captured_pos, n_pos);
+      p->captured_toks = std::min(p->captured_toks, p->lists.n_tokens);
     }
     HIP_TRY(rk_launch_paged_append(a, dtype, cs_dtype, st), op);
     return RK_OK;

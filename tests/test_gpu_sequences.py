@@ -736,3 +736,52 @@ def test_numpy_helpers(rk):
     other = rk.paged_plan([1], [3], np.array([[1]]), 4, 32, h, kv, d)
     with pytest.raises(rk.RocketError):
         cache.attention(other, np.zeros((1, h * d), np.float16), 0.1)
+
+
+def test_a_captured_call_s_buffers_bound_later_batches(rk):
+    """A graph's buffers have room for the tokens at its capture. Room that a plan has beyond that (for splits, or from
+    a larger batch before) admits no more."""
+    note("tokens of a captured call")
+    lib, st, h, kv, d, ps = rk.lib(), rk.new_stream(), 8, 2, 64, 16
+    rng = np.random.default_rng(50)
+    q, k, v = (rows(rng, "f16", 10, n * d) for n in (h, kv, kv))
+    filled = np.full((12, h * d), FILL, np.uint16)
+    b = upload(rk, q, k, v, filled)
+    plan = rk.packed_plan([4], h, kv, d)
+    plan.reserve(1000)  # longer sequences, not more tokens
+    g = Graph(st, lambda: ok(rk, lib.rk_attention_packed_dev(plan.ptr, b[0].ptr, h * d, b[1].ptr, kv * d, b[2].ptr, kv * d, 0.1, 0.0,
+                                                             b[3].ptr, h * d, rk.DTYPE_F16, st)))
+    for lens in ([5], [1000], [2, 3], [1] * 5, [0, 4, 1]):
+        with pytest.raises(rk.RocketError) as e:
+            plan.update(lens, stream=st)
+        assert e.value.rc == rk.RK_E_SHAPE and "tokens" in str(e.value)
+    for lens in ([4], [1, 3], [2], [0, 0]):
+        plan.update(lens, stream=st)
+        b[3].upload(filled)
+        g.replay()
+        rk.synchronize(st)
+        got, t = b[3].download(filled.shape, np.uint16), sum(lens)
+        assert (got[t:] == FILL).all()
+        check_packed(got[:t], q, k, v, lens, h, kv, d, "f16", 0.1)
+    g.destroy()
+    plan.destroy()
+    # paged: the plan had a larger batch before; the append's tokens count as well
+    pg, caches, keys, q = paged_inputs(51, [64, 64], ps, h, kv, d, "f16", [6, 4])
+    x = rows(rng, "f16", 10, (h + 2 * kv) * d)
+    b = upload(rk, q, *caches, filled, x, np.ones((64, d // 2), np.float32))
+    for call in (lambda p: lib.rk_attention_paged_dev(p, b[0].ptr, h * d, b[1].ptr, b[2].ptr, 0.1, 0.0, b[3].ptr, h * d, rk.DTYPE_F16, st),
+                 lambda p: lib.rk_paged_append_dev(p, b[4].ptr, (h + 2 * kv) * d, None, None, 1e-6, b[5].ptr, b[5].ptr, rk.DTYPE_F32, 64,
+                                                   b[3].ptr, h * d, b[1].ptr, b[2].ptr, rk.DTYPE_F16, st)):
+        plan = rk.paged_plan([50, 50], [64, 64], pg.table, pg.n_pages, ps, h, kv, d)
+        plan.update([6, 4], [64, 64], pg.table, stream=st)
+        plan.reserve(50)
+        g = Graph(st, lambda: ok(rk, call(plan.ptr)))
+        for lens in ([6, 5], [50, 50], [11, 0]):
+            with pytest.raises(rk.RocketError) as e:
+                plan.update(lens, [64, 64], pg.table, stream=st)
+            assert e.value.rc == rk.RK_E_SHAPE
+        plan.update([10, 0], [64, 64], pg.table, stream=st)
+        rk.synchronize(st)
+        g.destroy()
+        plan.destroy()
+    rk.destroy_stream(st)
