@@ -528,8 +528,8 @@ class SeqPlan:
     """A plan of rk_packed_plan_create or rk_paged_plan_create (`ptr`): what a batch of
     sequences looks like. Freed with the object, or by `destroy`."""
 
-    def __init__(self, ptr, n_tokens, heads, page_size=0):
-        self.ptr, self.n_tokens, self.page_size = ptr, n_tokens, page_size
+    def __init__(self, ptr, n_tokens, heads, page_size=0, n_pages=0):
+        self.ptr, self.n_tokens, self.page_size, self.n_pages = ptr, n_tokens, page_size, n_pages
         self.n_head, self.n_kv_heads, self.head_dim = heads
 
     def update(self, q_lens, kv_lens=None, page_table=None, stream=None):
@@ -582,7 +582,7 @@ def paged_plan(q_lens, kv_lens, page_table, n_pages, page_size, n_head, n_kv_hea
         _shape_error("paged_plan", "q_lens, kv_lens [n] and page_table [n, pages]")
     _check(_lib.rk_paged_plan_create(_ptr(q), _ptr(kv), _ptr(table), table.shape[1], q.size, n_pages, page_size, n_head,
                                      n_kv_heads, head_dim, mode, window, ctypes.byref(out)), "paged_plan")
-    return SeqPlan(out.value, int(q.sum(dtype=np.int64)), (n_head, n_kv_heads, head_dim), page_size)
+    return SeqPlan(out.value, int(q.sum(dtype=np.int64)), (n_head, n_kv_heads, head_dim), page_size, n_pages)
 
 
 def attention_packed(q, k, v, q_lens, n_head, n_kv_heads, head_dim, scale, softcap=None, mode=MASK_CAUSAL, window=-1,
@@ -622,7 +622,7 @@ class PagedCache:
         return paged_plan(q_lens, kv_lens, page_table, n_pages, ps, n_head, kv, d, mode, window)
 
     def _mine(self, plan, a, width, op):
-        if (plan.n_kv_heads, plan.page_size, plan.head_dim) != self.shape[1:]:
+        if (plan.n_kv_heads, plan.page_size, plan.head_dim) != self.shape[1:] or plan.n_pages > self.shape[0]:
             _shape_error(op, "the plan is of another cache's heads or pages")
         _float_dtype(a, self.bf16, op)
         if a.dtype != (np.uint16 if self.bf16 else np.float16) or a.shape != (plan.n_tokens, width):

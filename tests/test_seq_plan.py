@@ -94,3 +94,24 @@ def test_binding_refuses_lengths_that_do_not_fit(lib):
         assert e.value.rc == rk.RK_E_SHAPE
     with pytest.raises(rk.RocketError):
         rk.paged_plan([1, 1], [1], np.zeros((2, 1)), 4, 16, 8, 2, 64)
+
+
+class FakeCache:
+    """A PagedCache's shape without its device memory."""
+
+    def __new__(cls, n_pages, ps, kv, d, bf16=False):
+        import burn_rocket as rk
+        c = rk.PagedCache.__new__(rk.PagedCache)
+        c.shape, c.bf16, c.dtype = (n_pages, kv, ps, d), bf16, rk.DTYPE_BF16 if bf16 else rk.DTYPE_F16
+        return c
+
+
+def test_a_cache_refuses_plans_that_name_pages_it_lacks():
+    import burn_rocket as rk
+    plan = rk.SeqPlan(None, 1, (4, 2, 64), 16, 9)
+    q, x, cs = np.zeros((1, 256), np.float16), np.zeros((1, 512), np.float16), np.zeros((9, 32), np.float32)
+    for cache in (FakeCache(8, 16, 2, 64), FakeCache(9, 32, 2, 64), FakeCache(9, 16, 4, 64), FakeCache(9, 16, 2, 32)):
+        for call in (lambda: cache.attention(plan, q, 0.1), lambda: cache.append(plan, x, cs, cs)):
+            with pytest.raises(rk.RocketError) as e:
+                call()
+            assert e.value.rc == rk.RK_E_SHAPE and "pages" in str(e.value)
