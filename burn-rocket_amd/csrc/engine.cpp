@@ -2687,6 +2687,7 @@ int seq_attention(const void *plan, bool paged, const void *q, int64_t q_stride,
   const int64_t qw = (int64_t)g.n_head * g.head_dim, kw = (int64_t)g.n_kv_heads * g.head_dim;
   RK_TRY(seq_rows_check(q, q_stride, qw, "q", op));
   RK_TRY(seq_rows_check(out, out_stride, qw, "out", op));
+  if (out == q && out_stride != q_stride) return fail(RK_E_SHAPE, op, "out on q itself needs the same token stride");
   RK_TRY(seq_rows_check(k, paged ? kw : k_stride, kw, paged ? "k_cache" : "k", op));
   RK_TRY(seq_rows_check(v, paged ? kw : v_stride, kw, paged ? "v_cache" : "v", op));
   if (!paged && std::max(k_stride, v_stride) >= SEQ_MAX_STRIDE)

@@ -785,3 +785,15 @@ def test_a_captured_call_s_buffers_bound_later_batches(rk):
         g.destroy()
         plan.destroy()
     rk.destroy_stream(st)
+
+
+def test_out_on_the_queries_with_another_stride_is_refused(rk):
+    note("out on q, another stride")
+    lib, b = rk.lib(), rk.DeviceBuffer(1 << 16)
+    x, a, p = b.ptr, rk.packed_plan([4, 5], 4, 2, 64), rk.paged_plan([1], [20], np.array([[1, 2]]), 4, 16, 4, 2, 64)
+    for qs, os_ in ((256, 264), (512, 256)):
+        assert lib.rk_attention_packed_dev(a.ptr, x, qs, x + 16384, 128, x + 16384, 128, 0.1, 0.0, x, os_, rk.DTYPE_F16, None) == rk.RK_E_SHAPE
+        assert b"stride" in lib.rk_last_error()
+        assert lib.rk_attention_paged_dev(p.ptr, x, qs, x + 16384, x + 16384, 0.1, 0.0, x, os_, rk.DTYPE_F16, None) == rk.RK_E_SHAPE
+    assert lib.rk_attention_packed_dev(a.ptr, x, 264, x + 16384, 128, x + 16384, 128, 0.1, 0.0, x, 264, rk.DTYPE_F16, None) == 0
+    rk.synchronize()
