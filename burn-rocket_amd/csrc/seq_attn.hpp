@@ -42,17 +42,18 @@ __device__ __forceinline__ uintx4 join8(shortx4 a, shortx4 b) {
 }
 
 // Where the 16-key blocks of an item's keys lie, for one kv head: a lane knows one
-// block, and a wave that needs block i takes its descriptor from lane i. Rows past
-// the sequence's keys, blocks that no row of the item sees and blocks from `end` on
-// read as zeros.
+// block, and a wave that needs block i takes its descriptor from lane i. Keys from the
+// item's end on (which no row of its tile sees, or another part has) and blocks below
+// the first key that one sees read as zeros. V's keys below it in its own block do too
+// (hidden_below): a probability of 0 times a NaN or an infinity would reach every row.
 struct KeyBlocks {
   uint32_t lo, hi, bytes;
 };
 // The block from key key0 on; page: its page id (paged).
 template <bool PAGED>
 __device__ __forceinline__ KeyBlocks key_blocks(const SeqAttnArgs &a, const SeqItem &it, const void *base,
-                                                int64_t tok_stride, int kvh, int key0, int end, int page) {
-  const int rows = key0 + 15 < it.k_lo || key0 >= end ? 0 : max(0, min(16, it.kv_len - key0));
+                                                int64_t tok_stride, int kvh, int key0, int page) {
+  const int rows = key0 + 15 < it.k_lo ? 0 : max(0, min(16, it.k_end - key0));
   const int D = a.head_dim;
   int64_t at;
   KeyBlocks b;  // (strides are below SEQ_MAX_STRIDE)
@@ -68,6 +69,9 @@ __device__ __forceinline__ KeyBlocks key_blocks(const SeqAttnArgs &a, const SeqI
   b.hi = (uint32_t)(addr >> 32) & 0xffff;
   return b;
 }
+// Whether row `row` of the block from key key0 on lies below the first key that a row of
+// the item's tile sees.
+__device__ __forceinline__ bool hidden_below(const SeqItem &it, int key0, int row) { return row < it.k_lo - key0; }
 __device__ __forceinline__ rsrc_t block_rsrc(const KeyBlocks &b, int i) {
   const uint32_t lo = __builtin_amdgcn_readlane(b.lo, i), hi = __builtin_amdgcn_readlane(b.hi, i);
   return __builtin_amdgcn_make_buffer_rsrc((void *)((uint64_t)hi << 32 | lo), (short)0, __builtin_amdgcn_readlane(b.bytes, i),

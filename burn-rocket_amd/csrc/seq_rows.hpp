@@ -99,8 +99,8 @@ __device__ __forceinline__ void seq_rows_item(const SeqAttnArgs &a, int block, u
   auto turn = [&](int from) ALWAYS_INLINE {
     const int key0 = (from + (lane >> 1) * RW) * CK + 16 * (lane & 1);
     const int page = PAGED ? a.table[it.table + (min(key0, it.kv_len - 1) >> a.page_log2)] : 0;
-    kb = key_blocks<PAGED>(a, it, a.k, a.k_stride, kvh, key0, c_end * CK, page);
-    vb = key_blocks<PAGED>(a, it, a.v, a.v_stride, kvh, key0, c_end * CK, page);
+    kb = key_blocks<PAGED>(a, it, a.k, a.k_stride, kvh, key0, page);
+    vb = key_blocks<PAGED>(a, it, a.v, a.v_stride, kvh, key0, page);
     win_c = from;
   };
   auto load_k = [&](uintx4(&kf)[2][NQC], int cc) ALWAYS_INLINE {
@@ -127,6 +127,15 @@ __device__ __forceinline__ void seq_rows_item(const SeqAttnArgs &a, int block, u
         bdma16(rv, to, (uint32_t)row * vs + (uint32_t)(lch * 16), 0);
       }
     }
+  };
+  // Zeros over the rows of chunk cc that lie below the item's first key.
+  auto cut_v = [&](auto buf_c, int cc) ALWAYS_INLINE {
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+#pragma unroll
+      for (int i = 0; i < VB_INS; ++i)
+        if (hidden_below(it, cc * CK + 16 * b, (64 * i + lane) / CH))
+          *(uintx4 *)((decltype(buf_c)::value ? v_odd : v_even) + (v_wave + b * Gm::VB_BYTES + i * 1024 + lane * 16)) = uintx4{};
   };
   // Transposing reads: this lane's 8 bytes of key 4·lg + l16/4 of a block, columns
   // 16·db + 4·(l16%4)..; the swizzle moves 32-byte pairs.
@@ -207,6 +216,7 @@ __device__ __forceinline__ void seq_rows_item(const SeqAttnArgs &a, int block, u
       scores(kf[0]);
       load_k(kf[0], nx);
     }
+    if (c * CK < it.k_lo) cut_v(cur_c, c);
     softmax_pv(cur_c, c);
     WAIT_LGKMCNT0();  // the V buffer's reads are done before it is refilled
     asm volatile("" ::: "memory");

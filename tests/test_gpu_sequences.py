@@ -797,3 +797,54 @@ def test_out_on_the_queries_with_another_stride_is_refused(rk):
         assert lib.rk_attention_paged_dev(p.ptr, x, qs, x + 16384, x + 16384, 0.1, 0.0, x, os_, rk.DTYPE_F16, None) == rk.RK_E_SHAPE
     assert lib.rk_attention_packed_dev(a.ptr, x, 264, x + 16384, 128, x + 16384, 128, 0.1, 0.0, x, 264, rk.DTYPE_F16, None) == 0
     rk.synchronize()
+
+
+def tokens_of_a_tile(small, g, d):
+    """New tokens of the rows that are computed together."""
+    return (16 if small else 128 if d <= 128 else 64) // g
+
+
+@pytest.mark.parametrize("n,many", [(300, False), (300, True), (2000, True)])
+@pytest.mark.parametrize("h,kv,d", [(8, 1, 64), (1, 1, 128), (4, 2, 80), (8, 1, 256)])
+def test_values_that_no_row_of_a_tile_sees_do_not_reach_it(rk, n, many, h, kv, d):
+    """A NaN or infinity in V just behind the last key that any row of a tile sees, or just before the first one,
+    leaves the tile's results as they are, bit for bit."""
+    note(f"hidden values, n={n} many={many} {h}/{kv} d={d}")
+    rng, tile = np.random.default_rng(60), tokens_of_a_tile(not many, h // kv, d)
+    lens = [n, *[1] * crowd(h, kv) * many]
+    q, k, v = (rows(rng, "f16", sum(lens), m * d) for m in (h, kv, kv))
+    tok = np.arange(n)
+    first, last = tok // tile * tile, np.minimum(tok // tile * tile + tile, n) - 1  # of each token's tile
+    for mode, window in ((1, -1), (3, 50), (2, 37), (3, 130)):
+        want = packed(rk, q, k, v, lens, h, kv, d, "f16", 0.1, mode=mode, window=window)
+        lo = first - {1: n, 2: window, 3: window - 1}[mode]
+        hi, hidden = last + (window if mode == 2 else 0), 0
+        for at, bits in ((tile, 0x7E00), (tile + 1, 0x7C00), (2 * tile + 4, 0xFC00), (100, 0x7E00), (n // 2 + 1, 0x7E00), (n - 2, 0x7E00)):
+            bad = v.copy()
+            bad[at] = bits
+            got = packed(rk, q, k, bad, lens, h, kv, d, "f16", 0.1, mode=mode, window=window)
+            clean = (at < lo) | (at > hi)
+            hidden += clean.sum()  # (none of a key in a causal prompt's first tile)
+            wrong = np.flatnonzero((got[:n] != want[:n]).any(1) & clean)
+            assert wrong.size == 0, f"mode {mode} window {window}: key {at} reached tokens {wrong[:4]}"
+            assert (got[n:] == want[n:]).all()
+        assert hidden > 0
+
+
+@pytest.mark.parametrize("h,kv,d", [(8, 2, 64), (32, 4, 128), (3, 1, 256)])
+@pytest.mark.parametrize("n,m", [(1, 400), (1, 7000), (5, 333), (40, 6000)])
+def test_paged_values_beside_the_window_do_not_reach_the_tokens(rk, h, kv, d, n, m):
+    """The keys on either side of what the new tokens see: of a page that the sequence still holds, or of later slots."""
+    note(f"paged, hidden values, {n} of {m} {h}/{kv} d={d}")
+    ps = 32
+    pg, caches, keys, q = paged_inputs(61, [m], ps, h, kv, d, "f16", [n])
+    for window in (50, 64, 333):
+        want = paged(rk, pg, caches, q, [n], [m], h, kv, d, "f16", 0.1, mode=3, window=window)
+        assert np.isfinite(ref.decode(want, "f16")).all()
+        first = m - n - window + 1
+        if first <= 0:
+            continue
+        bad = [caches[0], caches[1].copy()]
+        for at in range(max(0, first - 40), first):
+            bad[1][pg.table[0, at // ps], :, at % ps] = 0x7E00
+        assert (paged(rk, pg, bad, q, [n], [m], h, kv, d, "f16", 0.1, mode=3, window=window) == want).all(), f"window {window}"
