@@ -28,6 +28,22 @@ __device__ __forceinline__ uint32_t pack2(float x, float y) {
   else
     return __builtin_bit_cast(uint32_t, bf16x2{(__bf16)x, (__bf16)y});
 }
+// Two probabilities as two values of the type each: cut off to the type, and what that
+// leaves. Together they hold 2^-16 of the value (bf16; fp16 2^-20): with one value, as
+// accurate as a result's own rounding, results of rows with few keys that nearly cancel
+// were off by up to 9e-2 (bf16) and 1.1e-2 (fp16) of their size, above the 1e-2 that the
+// single-sequence attention is held to.
+template <int DT>
+__device__ __forceinline__ void split2(float x, float y, uint32_t &hi, uint32_t &lo) {
+  if constexpr (DT == RK_DTYPE_F16) {
+    hi = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(x, y));
+    lo = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(minus_half_lo(hi, x), minus_half_hi(hi, y)));
+  } else {
+    const uint32_t a = __float_as_uint(x), b = __float_as_uint(y);
+    hi = __builtin_amdgcn_perm(b, a, 0x07060302);  // the upper halves
+    lo = pack2<DT>(x - __uint_as_float(a & 0xffff0000u), y - __uint_as_float(b & 0xffff0000u));
+  }
+}
 // Probabilities are kept times 2^P_BIAS: fp16's smallest normal value is then
 // 2^-20 of the largest one, the sums have the same factor.
 constexpr float P_BIAS = 6.0f;

@@ -11,7 +11,8 @@
 //   Sᵀ = K·Qᵀ   a lane owns one query row (lane % 16) and keys 4·(lane/16)+e of
 //               each 16-key block, so that the row maximum is in the lane and two
 //               lane swaps;
-//   P           exp2 in f32 against the running maximum, rounded once to the type;
+//   P           exp2 in f32 against the running maximum, held as two values of the
+//               type (the second product costs nothing beside the reads);
 //   Oᵀ += Vᵀ·Pᵀ V read back through the transposing LDS read, which hands a lane
 //               the keys of P's registers: V needs no rearranging pass.
 // A chunk is two 16-key blocks, each inside one page, with a buffer descriptor of
@@ -181,17 +182,22 @@ __device__ __forceinline__ void seq_rows_item(const SeqAttnArgs &a, int block, u
       for (int db = 0; db < NDB; ++db) o[db] *= alpha;
     }
     m_run = m_new;
-    uintx4 p;
+    uintx4 p, p_lo;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const float e0 = __builtin_amdgcn_exp2f(x[2 * i] - (mu - P_BIAS)), e1 = __builtin_amdgcn_exp2f(x[2 * i + 1] - (mu - P_BIAS));
       l_run += e0 + e1;
-      p[i] = pack2<DT>(e0, e1);
+      uint32_t hi, lo;
+      split2<DT>(e0, e1, hi, lo);
+      p[i] = hi;
+      p_lo[i] = lo;
     }
 #pragma unroll
     for (int db = 0; db < NDB; ++db) {
       const uint8_t *const at = (decltype(buf_c)::value ? v_odd : v_even) + (v_wave + (int)v_row + ((db ^ vsw) << 5));
-      o[db] = mfma16<DT>(join8(lds_read_tr16(at), lds_read_tr16(at + Gm::VB_BYTES)), p, o[db]);
+      const uintx4 vf = join8(lds_read_tr16(at), lds_read_tr16(at + Gm::VB_BYTES));
+      o[db] = mfma16<DT>(vf, p, o[db]);
+      o[db] = mfma16<DT>(vf, p_lo, o[db]);
     }
   };
 

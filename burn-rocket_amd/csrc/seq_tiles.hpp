@@ -11,14 +11,15 @@
 //   Sᵀ = K·Qᵀ   K rows from LDS, Q in registers; a lane owns one query of each
 //               16-query block and keys 4·(lane/16)+e of each 16-key block;
 //   P           exp2 against a maximum that is only raised when a score passes it
-//               by 2^RESCALE, rounded once to the type;
+//               by 2^RESCALE, held as two values of the type (split2), which takes half
+//               as many products again;
 //   Oᵀ += Vᵀ·Pᵀ V rows from LDS as they lie in memory, through the transposing
 //               read, in the order of P's registers.
 // The LDS fragment reads feed QB products each; with 32 rows per wave they take
 // the whole read rate of a CU (128 bytes a clock) while the products run.
 //
 // Row sums come from the same products (a row of ones), which takes their additions
-// off the softmax slot and counts the probabilities as rounded.
+// off the softmax slot and counts the probabilities as they are held.
 //
 // LDS: K rows of KPC 16-byte pieces (piece c of row r at c ^ (r & (KPC-1))), V as
 // 16-key blocks (32-byte pairs swizzled by the key where rows are a power of two).
@@ -27,13 +28,14 @@
 // zeros. They start with the softmax, which their latency hides behind; issued between
 // products they held those up.
 //
-// MI355X: two prompts of 7000 tokens, 32/4 heads of 128, causal, bf16, 735-790 us (1.05-1.13
-// PFLOP/s; the library's 8192³ product reaches 1.2), the matrix cores busy 53 % of the
-// clocks. 512 rows of 8 heads on 16901 keys 138 us (1.01 PFLOP/s, 17 us of it the states
-// of 4 parts a tile). 64 passages of 100 to 512 tokens 76 us (3.2 TB/s): items of three key
+// MI355X: two prompts of 7000 tokens, 32/4 heads of 128, causal, bf16, 996 us: 0.83 PFLOP/s,
+// with the second half of P and the row sums 1.35 issued (the library's 8192³ product reaches
+// 1.2). With P as one value it took 742. 512 rows of 8 heads on 16901 keys 187 us (one value:
+// 147). 64 passages of 100 to 512 tokens 88 us (79): items of three key
 // tiles, whose first loads and last stores nothing hides. Head dim 256 has one 16-query
-// block per wave: every product reads its own 1 KB from LDS, twice the CU's rate. 45 us for
-// 9261 tokens, 3/1 heads, 512 keys to either side; 128 rows a workgroup, one per CU, 58.
+// block per wave: every product reads its own 1 KB from LDS, twice the CU's rate. 58 us for
+// 9261 tokens, 3/1 heads, 512 keys to either side (one value of P: 52; 128 rows a workgroup, one
+// per CU, a quarter more).
 //
 // Items that are one of n_parts of their tile leave their state in the plan's
 // workspace; the last to arrive merges the parts in key order.
@@ -183,7 +185,7 @@ __device__ __forceinline__ void seq_tiles_item(const SeqAttnArgs &a, int block, 
   const int vsw = vkey & Gm::VSW;
 
   floatx4 o[NDB][QB], s[NB][QB];
-  uintx4 p[NC2][QB];
+  uintx4 p[NC2][QB], p_lo[NC2][QB];
   float m_run[QB];
   floatx4 l_run[QB];  // (every row of the product with ones is the row sum)
   const uint32_t one2 = DT == RK_DTYPE_F16 ? 0x3c003c00u : 0x3f803f80u;
@@ -203,23 +205,28 @@ __device__ __forceinline__ void seq_tiles_item(const SeqAttnArgs &a, int block, 
 #pragma unroll
       for (int c2 = 0; c2 < NC2; ++c2) {
 #pragma unroll
-        for (int qb = 0; qb < QB; ++qb) l_run[qb] = mfma16<DT>(ones, p[c2][qb], l_run[qb]);
+        for (int qb = 0; qb < QB; ++qb) {
+          l_run[qb] = mfma16<DT>(ones, p[c2][qb], l_run[qb]);
+          l_run[qb] = mfma16<DT>(ones, p_lo[c2][qb], l_run[qb]);
+        }
 #pragma unroll
         for (int db = 0; db < NDB; ++db) {
           const uint8_t *at = vt + 2 * c2 * Gm::VB + ((db ^ vsw) << 5);
           const uintx4 vf = join8(lds_read_tr16(at), lds_read_tr16(at + Gm::VB));
 #pragma unroll
           for (int qb = 0; qb < QB; ++qb) o[db][qb] = mfma16<DT>(vf, p[c2][qb], o[db][qb]);
+#pragma unroll
+          for (int qb = 0; qb < QB; ++qb) o[db][qb] = mfma16<DT>(vf, p_lo[c2][qb], o[db][qb]);
         }
       }
       // Each fragment (two reads) AHEAD_V fragments ahead of its products.
       constexpr int NF = NC2 * NDB, AV = AHEAD_V < NF ? AHEAD_V : NF;
       __builtin_amdgcn_sched_group_barrier(0x100, 2 * AV, 0);
       static_for<NF - AV>([&](auto) ALWAYS_INLINE {
-        __builtin_amdgcn_sched_group_barrier(0x008, QB, 0);
+        __builtin_amdgcn_sched_group_barrier(0x008, 2 * QB, 0);
         __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
       });
-      __builtin_amdgcn_sched_group_barrier(0x008, QB * (AV + NC2), 0);
+      __builtin_amdgcn_sched_group_barrier(0x008, 2 * QB * (AV + NC2), 0);
     }
     __builtin_amdgcn_sched_barrier(0);  // P dies before S is made
     if (j < nj) {
@@ -314,7 +321,10 @@ __device__ __forceinline__ void seq_tiles_item(const SeqAttnArgs &a, int block, 
           const int b = 2 * c2 + (i >> 1), e = 2 * (i & 1);
           const float e0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][qb][e], C, nm));
           const float e1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][qb][e + 1], C, nm));
-          p[c2][qb][i] = pack2<DT>(e0, e1);
+          uint32_t hi, lo;
+          split2<DT>(e0, e1, hi, lo);
+          p[c2][qb][i] = hi;
+          p_lo[c2][qb][i] = lo;
         }
     }
     // P is made here: left alone, the compiler moves the exponentials to their use, into
@@ -322,7 +332,7 @@ __device__ __forceinline__ void seq_tiles_item(const SeqAttnArgs &a, int block, 
 #pragma unroll
     for (int c2 = 0; c2 < NC2; ++c2)
 #pragma unroll
-      for (int qb = 0; qb < QB; ++qb) asm volatile("" : "+v"(p[c2][qb]));
+      for (int qb = 0; qb < QB; ++qb) asm volatile("" : "+v"(p[c2][qb]), "+v"(p_lo[c2][qb]));
     __builtin_amdgcn_sched_barrier(0);
     WAIT_VMCNT(0);
   };

@@ -462,8 +462,8 @@ int rk_seq_plan_destroy(void *plan);
  * heads (column ranges of one q|k|v row, for instance), out as q, or q itself with
  * the same stride. dtype fp16 or bf16 (RK_DTYPE_*), strides multiples of 8 values,
  * buffers 16-byte aligned, head dims as rk_attention_dev without the padded ones.
- * Scores and softmax in f32, probabilities rounded to nearest in dtype for the
- * product with V, sums in f32, one rounding at the end. The split of a row's keys between workgroups depends on
+ * Scores and softmax in f32, probabilities as two values of dtype for the product
+ * with V (2^-16 of each is left), sums in f32, one rounding at the end. The split of a row's keys between workgroups depends on
  * the whole batch: a sequence's result can differ in rounding between batches, and
  * between a captured call (made for any batch of its plan's room) and one that is
  * not. Equal batches give equal bits. A non-finite value of V reaches every row of

@@ -848,3 +848,56 @@ def test_paged_values_beside_the_window_do_not_reach_the_tokens(rk, h, kv, d, n,
         for at in range(max(0, first - 40), first):
             bad[1][pg.table[0, at // ps], :, at % ps] = 0x7E00
         assert (paged(rk, pg, bad, q, [n], [m], h, kv, d, "f16", 0.1, mode=3, window=window) == want).all(), f"window {window}"
+
+
+# ----------------------------------------------------------- probabilities ----
+# A probability is held as two values of the type: what the second leaves is 2^-16 of it at most (bf16: 2^-7 of it is
+# the second one's range, 2^-9 of that its rounding; fp16: 2^-10 and 2^-10).
+P_LEFT = 2.0 ** -16
+
+
+def close_once_rounded(got, q, k, v, pos, scale, softcap, mode, window, dtype, what):
+    """`got` is the exact result but for its own rounding and f32 arithmetic."""
+    want, rest = ref.attention(q, k, v, pos, scale, softcap, mode, window, P_LEFT)
+    ref.close(got, want, rest + 1.01 * ref.HALF[dtype] * np.abs(want), what)
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("many", [False, True])
+@pytest.mark.parametrize("h,kv,d,mode,window,softcap", [(4, 2, 64, 1, -1, 0.0), (16, 8, 128, 1, -1, 0.0), (2, 2, 72, 0, -1, 0.0),
+                                                        (3, 1, 256, 2, 40, 0.0), (8, 1, 32, 1, -1, 20.0), (4, 4, 96, 3, 70, 30.0)])
+def test_packed_rounds_the_result_alone(rk, dtype, many, h, kv, d, mode, window, softcap):
+    note(f"packed, once rounded, {dtype} many={many} {h}/{kv} d={d}")
+    rng = np.random.default_rng(70)
+    lens = [150, 7, *[1] * crowd(h, kv) * many]
+    q, k, v = (rows(rng, dtype, sum(lens), m * d) for m in (h, kv, kv))
+    got = packed(rk, q, k, v, lens, h, kv, d, dtype, d ** -0.5, softcap, mode, window)
+    for at, n in ((0, 150), (150, 7)):
+        a = [ref.decode(t[at:at + n], dtype).reshape(n, -1, d) for t in (got, q, k, v)]
+        close_once_rounded(*a, np.arange(n), d ** -0.5, softcap, mode, window, dtype, f"sequence of {n}")
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("q_lens,kv_lens,h,kv,d", [([1, 1], [4097, 33], 32, 4, 128), ([40, 1], [900, 700], 16, 4, 64), ([200], [1500], 8, 1, 128),
+                                                   ([1], [3000], 4, 1, 256)])
+def test_paged_rounds_the_result_alone(rk, dtype, q_lens, kv_lens, h, kv, d):
+    note(f"paged, once rounded, {dtype} {q_lens} of {kv_lens} {h}/{kv} d={d}")
+    pg, caches, keys, q = paged_inputs(71, kv_lens, 32, h, kv, d, dtype, q_lens)
+    got, at = paged(rk, pg, caches, q, q_lens, kv_lens, h, kv, d, dtype, d ** -0.5), 0
+    for i, (n, m) in enumerate(zip(q_lens, kv_lens)):
+        a = [ref.decode(t[at:at + n], dtype).reshape(n, h, d) for t in (got, q)]
+        close_once_rounded(*a, *(ref.decode(t[i], dtype) for t in keys), np.arange(m - n, m), d ** -0.5, 0.0, 1, -1, dtype, f"{n} of {m}")
+        at += n
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("n,h,kv,d,mode", [(1024, 16, 8, 128, 1), (2116, 16, 16, 72, 0), (24, 16, 8, 128, 1)])
+def test_packed_meets_the_gate_of_the_single_sequence_attention(rk, orc, dtype, n, h, kv, d, mode):
+    """Cosine 0.9999 and max-rel 1e-2, which rk_attention_dev is held to, at its sizes."""
+    note(f"packed, parity gate, {dtype} n={n} {h}/{kv} d={d}")
+    rng = np.random.default_rng(72)
+    x = [rng.standard_normal((n, m * d)) for m in (h, kv, kv)]
+    x = [ref.encode(np.where(np.abs(a) < 2.0 ** -6, 0.0, a), dtype) for a in x]  # (bf16 values of this range are fp16 values)
+    got = ref.decode(packed(rk, *x, [n], h, kv, d, dtype, d ** -0.5, mode=mode), dtype)
+    want = orc.attention_ref(*(ref.decode(a, dtype).astype(np.float16) for a in x), h, kv, d, d ** -0.5, 0.0, mode)
+    assert orc.cosine(got, want) >= 0.9999 and orc.max_rel(got, want) <= 1e-2, (orc.cosine(got, want), orc.max_rel(got, want))
