@@ -422,6 +422,12 @@ extern "C" int rk_mem_stats(rk_mem_stats_t *out) {
       out->attention_bytes += kv.second.bytes;
   }
   out->host_bytes = g_eng->stage.pinned_bytes() + g_eng->moe_pin_bytes;
+  for (const SeqPlan *p : g_eng->seq_plans) {
+    const uint64_t held = (p->block.p ? p->block.bytes : 0) + (p->work.p ? p->work.bytes : 0);
+    out->scratch_bytes += held;
+    out->attention_bytes += held;
+    if (p->pin) out->host_bytes += p->block.bytes;  // an image of the block
+  }
   return RK_OK;
 }
 

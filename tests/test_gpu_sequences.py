@@ -901,3 +901,23 @@ def test_packed_meets_the_gate_of_the_single_sequence_attention(rk, orc, dtype, 
     got = ref.decode(packed(rk, *x, [n], h, kv, d, dtype, d ** -0.5, mode=mode), dtype)
     want = orc.attention_ref(*(ref.decode(a, dtype).astype(np.float16) for a in x), h, kv, d, d ** -0.5, 0.0, mode)
     assert orc.cosine(got, want) >= 0.9999 and orc.max_rel(got, want) <= 1e-2, (orc.cosine(got, want), orc.max_rel(got, want))
+
+
+def test_mem_stats_count_live_plans(rk):
+    note("mem_stats of plans")
+    h, kv, d = 8, 1, 128
+    before = rk.mem_stats()
+    plan = rk.paged_plan([1], [30000], np.arange(2000, dtype=np.int32)[None], 2000, 16, h, kv, d)
+    made = rk.mem_stats()
+    held = made.scratch_bytes - before.scratch_bytes
+    # page ids, and a state of 16 rows for each part of a tile that is split
+    assert held >= 4 * 1875 + 16 * 16 * d * 4 and made.attention_bytes - before.attention_bytes == held
+    assert made.host_bytes == before.host_bytes and made.n_scratch == before.n_scratch
+    plan.update([1], [29999], np.arange(2000, dtype=np.int32)[None])
+    now = rk.mem_stats()
+    assert now.host_bytes - before.host_bytes >= 4 * 1875 and now.scratch_bytes - before.scratch_bytes == held
+    plan.reserve(300)
+    assert rk.mem_stats().scratch_bytes > now.scratch_bytes
+    plan.destroy()
+    after = rk.mem_stats()
+    assert (after.scratch_bytes, after.attention_bytes, after.host_bytes) == (before.scratch_bytes, before.attention_bytes, before.host_bytes)
