@@ -128,7 +128,7 @@ struct SeqPlan {
   DevBuf block, work;
   size_t off_tiles = 0, off_toks = 0, off_table = 0;      // in block (row items at 0)
   size_t off_tile_cnt = 0, off_rows = 0, off_tile_part = 0;  // in work (row counts at 0)
-  uint8_t *pin = nullptr;       // page-locked image of block, made by the first update
+  uint8_t *pin = nullptr;       // page-locked image of block, made by the first update or reserve
   hipEvent_t pin_ev = nullptr;  // its last upload
   int64_t reserved_q = 0;       // > 0: rk_seq_plan_reserve'd, for q_lens up to this
   bool captured = false;        // a graph holds these buffers: they are not replaced
@@ -2566,12 +2566,20 @@ int seq_reserve(SeqPlan &p, const SeqPlan::Room &want, const char *op) {
   return RK_OK;
 }
 
+// What an update uploads from, for the block as it is.
+int seq_pin(SeqPlan &p, const char *op) {
+  if (!p.pin) HIP_TRY(hipHostMalloc((void **)&p.pin, p.block.bytes, hipHostMallocDefault), op);
+  if (!p.pin_ev) HIP_TRY(hipEventCreateWithFlags(&p.pin_ev, hipEventDisableTiming), op);
+  return RK_OK;
+}
+
 // After a failure: an empty batch rather than lists that the device may not hold, and no
-// capture of them before another reserve (a graph that has the buffers has their old lists).
+// capture of them before another reserve. (Updates of a captured plan allocate nothing: one
+// that fails has lost the device, and the plan takes no other.)
 void seq_forget(SeqPlan &p) {
   p.lists = SeqLists{};
   p.n_seqs = 0;
-  if (!p.captured) p.reserved_q = 0;
+  p.reserved_q = 0;
 }
 
 // The lists grow with the batch: a failed host allocation is a status here.
@@ -2655,8 +2663,7 @@ int seq_plan_update(void *plan, bool paged, const SeqBatch &b, rk_stream stream,
   p->n_seqs = b.n_seqs;
   const int rc = [&]() -> int {
     RK_TRY(seq_reserve(*p, seq_room(p->lists), op));
-    if (!p->pin) HIP_TRY(hipHostMalloc((void **)&p->pin, p->block.bytes, hipHostMallocDefault), op);
-    if (!p->pin_ev) HIP_TRY(hipEventCreateWithFlags(&p->pin_ev, hipEventDisableTiming), op);
+    RK_TRY(seq_pin(*p, op));
     seq_image(*p, p->pin);
     CallScope cs(st);
     RK_TRY(seq_buf_use(cs, p->block, false, op));
@@ -2807,6 +2814,7 @@ extern "C" int rk_seq_plan_reserve(void *plan, int64_t max_q_len) {
     RK_TRY(seq_buf_wait(p->work, op));
     const int rc = no_throw(op, [&]() -> int {
       RK_TRY(seq_reserve(*p, want, op));
+      RK_TRY(seq_pin(*p, op));
       std::vector<uint8_t> image(p->block.bytes);
       seq_image(*p, image.data());
       HIP_TRY(hipMemcpy(p->block.p, image.data(), image.size(), hipMemcpyHostToDevice), op);

@@ -442,10 +442,10 @@ int rk_flash_attn_f16_masked(int64_t n_q, int64_t n_kv, int head_dim, int dv, in
  * a call is captured into a graph, rk_seq_plan_reserve gives the plan room for any
  * later batch of no more sequences, tokens and pages than its present one, with
  * q_lens up to max_q_len (below the present longest: that one); nothing is allocated
- * in the capture, launches have room for all of it, and updates that need more are
- * then refused (RK_E_SHAPE). The q, out and q|k|v buffers of a captured call must
- * have room for the tokens of the batch that the plan holds when the call is captured;
- * updates to a batch of more tokens are refused too. The caller orders the replays of
+ * in the capture or by later updates, launches have room for all of it, and updates
+ * that need more are then refused (RK_E_SHAPE). The q, out and q|k|v buffers of a
+ * captured call must have room for the tokens of the batch that the plan holds when
+ * the call is captured; updates to a batch of more tokens are refused too. The caller orders the replays of
  * graphs that share a plan, and other calls and updates of a captured plan, after
  * one another. A plan is destroyed after its graphs. */
 int rk_packed_plan_create(const int32_t *q_lens, int64_t n_seqs, int n_head, int n_kv_heads, int head_dim,

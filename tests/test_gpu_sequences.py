@@ -921,3 +921,25 @@ def test_mem_stats_count_live_plans(rk):
     plan.destroy()
     after = rk.mem_stats()
     assert (after.scratch_bytes, after.attention_bytes, after.host_bytes) == (before.scratch_bytes, before.attention_bytes, before.host_bytes)
+
+
+def test_updates_of_a_captured_plan_allocate_nothing(rk):
+    """All that they need is there with the reserve: none can fail for want of memory and leave a graph with lists that
+    the plan no longer knows."""
+    note("updates of a captured plan")
+    h, kv, d, n = 8, 2, 64, 40
+    st, b = rk.new_stream(), rk.DeviceBuffer(n * (h + 2 * kv) * d * 2)
+    plan, before = rk.packed_plan([1] * n, h, kv, d), rk.mem_stats()
+    plan.reserve(n)
+    held = rk.mem_stats()
+    assert held.host_bytes > before.host_bytes
+    g = Graph(st, lambda: ok(rk, rk.lib().rk_attention_packed_dev(plan.ptr, b.ptr, h * d, b.ptr, kv * d, b.ptr, kv * d, 0.1, 0.0, b.ptr,
+                                                                  h * d, rk.DTYPE_F16, st)))
+    for lens in ([n], [1], [n // 2] * 2, [], [1] * n):
+        plan.update(lens, stream=st)
+        now = rk.mem_stats()
+        assert (now.host_bytes, now.scratch_bytes) == (held.host_bytes, held.scratch_bytes)
+    rk.synchronize(st)
+    g.destroy()
+    plan.destroy()
+    rk.destroy_stream(st)
