@@ -639,6 +639,8 @@ class PagedCache:
             _shape_error("rocket_paged_append", "cos and sin must be [positions, D/2]")
         if ct == self.dtype:
             _float_dtype(cos, self.bf16, "rocket_paged_append")
+        if (q_norm_w is None) != (k_norm_w is None):
+            _shape_error("rocket_paged_append", "give both norm weights or neither")
         norms = [] if q_norm_w is None else [np.asarray(q_norm_w), np.asarray(k_norm_w)]
         if any(w.shape != (d,) or w.dtype != qkv.dtype for w in norms):
             _shape_error("rocket_paged_append", "the norm weights must be [D] in the cache's type")

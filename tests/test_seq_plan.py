@@ -115,3 +115,13 @@ def test_a_cache_refuses_plans_that_name_pages_it_lacks():
             with pytest.raises(rk.RocketError) as e:
                 call()
             assert e.value.rc == rk.RK_E_SHAPE and "pages" in str(e.value)
+
+
+def test_append_refuses_one_norm_weight_alone():
+    import burn_rocket as rk
+    plan, cache = rk.SeqPlan(None, 1, (4, 2, 64), 16, 8), FakeCache(8, 16, 2, 64)
+    x, cs, w = np.zeros((1, 512), np.float16), np.zeros((9, 32), np.float32), np.ones(64, np.float16)
+    for norms in ((w, None), (None, w)):
+        with pytest.raises(rk.RocketError) as e:
+            cache.append(plan, x, cs, cs, *norms)
+        assert e.value.rc == rk.RK_E_SHAPE and "both" in str(e.value)
