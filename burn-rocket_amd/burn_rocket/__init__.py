@@ -537,6 +537,8 @@ class SeqPlan:
         q = _lens(q_lens)
         st = ctypes.c_void_p(stream) if stream else None
         if self.page_size == 0:
+            if kv_lens is not None or page_table is not None:
+                _shape_error("packed_plan_update", "packed sequences have no kv_lens or page_table")
             _check(_lib.rk_packed_plan_update(self.ptr, _ptr(q), q.size, st), "packed_plan_update")
         else:
             kv, table = _lens(kv_lens), _lens(page_table)

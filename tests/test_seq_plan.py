@@ -125,3 +125,12 @@ def test_append_refuses_one_norm_weight_alone():
         with pytest.raises(rk.RocketError) as e:
             cache.append(plan, x, cs, cs, *norms)
         assert e.value.rc == rk.RK_E_SHAPE and "both" in str(e.value)
+
+
+def test_an_update_of_packed_sequences_refuses_cached_keys():
+    import burn_rocket as rk
+    plan = rk.SeqPlan(None, 1, (4, 2, 64))
+    for extra in (dict(kv_lens=[5]), dict(page_table=[[0]]), dict(kv_lens=[5], page_table=[[0]])):
+        with pytest.raises(rk.RocketError) as e:
+            plan.update([1], **extra)
+        assert e.value.rc == rk.RK_E_SHAPE and "packed" in str(e.value)
