@@ -539,18 +539,24 @@ class SeqPlan:
         if self.page_size == 0:
             if kv_lens is not None or page_table is not None:
                 _shape_error("packed_plan_update", "packed sequences have no kv_lens or page_table")
-            _check(_lib.rk_packed_plan_update(self.ptr, _ptr(q), q.size, st), "packed_plan_update")
+            self._changed(_lib.rk_packed_plan_update(self.ptr, _ptr(q), q.size, st), "packed_plan_update")
         else:
             kv, table = _lens(kv_lens), _lens(page_table)
             if kv.size != q.size or table.ndim != 2 or table.shape[0] != q.size:
                 _shape_error("paged_plan_update", "q_lens, kv_lens [n] and page_table [n, pages]")
-            _check(_lib.rk_paged_plan_update(self.ptr, _ptr(q), _ptr(kv), _ptr(table), table.shape[1], q.size, st),
-                   "paged_plan_update")
+            self._changed(_lib.rk_paged_plan_update(self.ptr, _ptr(q), _ptr(kv), _ptr(table), table.shape[1], q.size, st),
+                          "paged_plan_update")
         self.n_tokens = int(q.sum(dtype=np.int64))
 
     def reserve(self, max_q_len=0):
         """Room for every batch of no more sequences, tokens and pages than this one, for a graph capture."""
-        _check(_lib.rk_seq_plan_reserve(self.ptr, max_q_len), "seq_plan_reserve")
+        self._changed(_lib.rk_seq_plan_reserve(self.ptr, max_q_len), "seq_plan_reserve")
+
+    def _changed(self, rc, op):
+        """A refused change leaves the plan as it was, one that failed leaves an empty batch."""
+        if rc not in (0, RK_E_SHAPE, RK_E_UNSUPPORTED):
+            self.n_tokens = 0
+        _check(rc, op)
 
     def destroy(self):
         if self.ptr:

@@ -134,3 +134,20 @@ def test_an_update_of_packed_sequences_refuses_cached_keys():
         with pytest.raises(rk.RocketError) as e:
             plan.update([1], **extra)
         assert e.value.rc == rk.RK_E_SHAPE and "packed" in str(e.value)
+
+
+@pytest.mark.parametrize("rc,left", [(-1, 3), (-5, 3), (-3, 0), (-4, 0)])
+def test_a_plan_whose_change_failed_has_no_tokens(monkeypatch, rc, left):
+    """Calls on such a plan write nothing: the binding expects no rows of them then."""
+    import burn_rocket as rk
+
+    class Failing:
+        rk_packed_plan_update = rk_paged_plan_update = rk_seq_plan_reserve = staticmethod(lambda *a: rc)
+        rk_last_error = staticmethod(lambda: b"planted")
+
+    monkeypatch.setattr(rk, "_lib", Failing)
+    for plan, change in ((rk.SeqPlan(None, 3, (4, 2, 64)), lambda p: p.update([2])), (rk.SeqPlan(None, 3, (4, 2, 64)), lambda p: p.reserve(9)),
+                         (rk.SeqPlan(None, 3, (4, 2, 64), 16, 8), lambda p: p.update([2], [9], [[1]]))):
+        with pytest.raises(rk.RocketError) as e:
+            change(plan)
+        assert e.value.rc == rc and plan.n_tokens == left
