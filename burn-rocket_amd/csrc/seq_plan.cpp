@@ -169,18 +169,22 @@ void seq_build(const SeqGeom &g, const SeqBatch &b, int num_cus, SeqLists *out) 
   std::vector<Piece> pieces;  // where new tokens go: slots [off, end) of a page
   // A small batch goes to the kernel of few rows whole: at most four tiles of 16 rows per
   // CU whose products (each tile reads its K and V itself) take less than the other
-  // kernel's walk over the longest sequence. MI355X, rows -> tiles: 256 rows on 4096 keys,
-  // 32/4 heads of 128, 18 us, 36; 128 rows on 30000 42, 51; 256 rows on 30000 73, 52;
-  // 16 times 64 on 2000 25, 30; 16 times 96 on 300 14.6, 11.9. One prompt, causal: 300
-  // tokens of 16/8 heads of 128 9.6, 11.3; 600 19.3, 17.9; 800 of 12/12 heads of 64 11.3,
-  // 15.8; 1200 18.0, 15.6; 200 of 32/4 heads of 128 10.0, 9.8; 300 15.7, 11.4.
+  // kernel's walk over the longest sequence, both over the keys that its new tokens see.
+  // MI355X, rows -> tiles: 256 rows on 4096 keys, 32/4 heads of 128, 18.8 us, 27.3; 128 rows on
+  // 30000 41.6, 68; 256 rows on 30000 73, 68; 16 times 64 on 2000 25, 30; 16 times 96 on 300
+  // 14.5, 13.2. One prompt, causal: 300 tokens of 16/8 heads of 128 9.8, 13.0; 600 19.8, 21.1;
+  // 800 of 12/12 heads of 64 11.5, 18.8; 1200 18.1, 16.5; 200 of 32/4 heads of 128 10.2, 11.2;
+  // 300 15.9, 13.3. 64 tokens of 16/4 heads of 64, window 512, behind 2000 to 100000 keys 8.0, 15-17.
   int64_t n16 = 0, n16_keys = 0, longest = 0;
   for (int64_t i = 0; i < b.n_seqs; ++i) {
     if (b.q_lens[i] == 0) continue;
-    const int64_t t = ceil_div(b.q_lens[i] * G, 16) * g.n_kv_heads;
+    const int64_t t = ceil_div(b.q_lens[i] * G, 16) * g.n_kv_heads, kv = kv_of(b, i);
+    int64_t lo, hi, skip;
+    visible(g, kv - b.q_lens[i], kv, &lo, &skip);
+    visible(g, kv - 1, kv, &skip, &hi);
     n16 += t;
-    n16_keys += t * kv_of(b, i);
-    longest = std::max(longest, kv_of(b, i));
+    n16_keys += t * (hi + 1 - lo);
+    longest = std::max(longest, hi + 1 - lo);
   }
   const bool small = n16 <= 4 * num_cus && n16_keys <= 4096ll * num_cus &&
                      n16_keys * g.head_dim <= num_cus * (14000 + 140 * longest);

@@ -943,3 +943,10 @@ def test_updates_of_a_captured_plan_allocate_nothing(rk):
     g.destroy()
     plan.destroy()
     rk.destroy_stream(st)
+
+
+@pytest.mark.parametrize("q,kv_len", [(64, 2000), (64, 20000), (200, 60000)])
+@pytest.mark.parametrize("mode,window", [(3, 512), (2, 100)])
+def test_windowed_chunks_behind_long_prefixes(rk, q, kv_len, mode, window):
+    note(f"paged, chunk of {q} of {kv_len}, mode {mode} window {window}")
+    paged_case(rk, q + window, [q, 1], [kv_len, 90], 64, 16, 4, 64, "bf16", mode=mode, window=window)
