@@ -89,14 +89,17 @@ int64_t slots_per_head(const SeqGeom &g, int num_cus, bool one) {
   return std::max<int64_t>(1, slots / g.n_kv_heads);
 }
 
+constexpr int64_t PARTS = 32, PARTS_LONG = 1024;
+
 // Splits the keys of the longest tiles where that shortens the launch, then sorts
 // longest first: the short ones fill the last round. Fewer tiles than the GPU holds at
 // once: items of equal length, as many as it holds (one more than that is another
 // round: 512 query rows against 16901 keys, 128 tiles, took 152 us in 512 items and
 // 206 in 516 on MI355X). More: only tiles longer than 5/4 of an even share. None where
 // the longest would shrink by less than `cost` steps, which is what states to
-// store and merge take (about 20 us for tiles of 128 rows).
-void split(std::vector<SeqItem> &tiles, int step, int64_t slots, int64_t least, int64_t cost, int64_t most,
+// store and merge take (about 20 us for tiles of 128 rows). A tile has 16 parts at most up
+// to `merged` steps, then PARTS, from PARTS_LONG steps on `most`.
+void split(std::vector<SeqItem> &tiles, int step, int64_t slots, int64_t least, int64_t cost, int64_t merged, int64_t most,
            SeqList *out) {
   const auto steps = [&](const SeqItem &t) { return ceil_div(t.k_end - t.k_begin, step); };
   int64_t total = 0, longest = 0;
@@ -104,9 +107,7 @@ void split(std::vector<SeqItem> &tiles, int step, int64_t slots, int64_t least, 
     total += steps(t);
     longest = std::max(longest, steps(t));
   }
-  // (16 states are merged in one pass: one token on 8000 keys, 4 kv heads of 128, 12.6 us with
-  // 16 parts, 13.7 with 32; on 16000 17.4, 16.0)
-  const int64_t max_parts = longest <= 32 * 16 ? 16 : most;
+  const int64_t max_parts = longest <= merged ? 16 : longest <= PARTS_LONG ? PARTS : most;
   int64_t quota = std::max(least, ceil_div(total, slots));
   if ((int64_t)tiles.size() < slots) {
     const auto items = [&](int64_t q) {
@@ -140,7 +141,6 @@ void split(std::vector<SeqItem> &tiles, int step, int64_t slots, int64_t least, 
 // half the waves idle, but none with a second: one token on 500 keys, 4 kv heads of 128,
 // 8.9 us, with 8 chunks 10.0.)
 constexpr int64_t ROWS_LEAST = 4, ROWS_COST = 8, TILES_LEAST = 4, TILES_COST = 12;
-constexpr int64_t PARTS = 32;  // of a tile at most
 }  // namespace
 
 void seq_bound(const SeqGeom &g, int64_t n_seqs, int64_t n_tokens, int64_t max_q, int num_cus, SeqBound *rows,
@@ -225,12 +225,22 @@ void seq_build(const SeqGeom &g, const SeqBatch &b, int num_cus, SeqLists *out) 
       t = e;
     }
   }
+  // Row items merge 16 states in one pass, which pays up to 13000 keys, or 16000 where
+  // those parts give half the CUs work. MI355X, one token, heads of 128, 16 parts -> 32: one kv
+  // head, 12000 keys 14.7 us, 14.0, 14000 16.0, 14.9, 20000 19.1, 16.4; four, 12000 14.9, 15.0, 14000 16.5,
+  // 15.8, 20000 20.0, 17.5; eight, 14000 17.5, 19.5, 20000 20.9, 22.0.
+  const int64_t row_heads = (int64_t)rows.size() * g.n_kv_heads;
+  const int64_t row_merged = 64 * row_heads <= num_cus ? 416 : 512;
+  // Tiles merge one state at a time, beside much more work: 128 rows on 8000 keys 31.7, 36.9; 16000
+  // 44.7, 43.2; 24000 57.8, 49.2; heads of 64 on 16000 34.1, 37.4; 24000 43.2, 43.5; of 256 on 12000 44.5,
+  // 42.6; 24000 70.7, 56.4.
+  const int64_t tile_merged = g.head_dim <= 64 ? 384 : 256;
   // Twice the parts where those leave three quarters of the CUs idle: one token on 60000
-  // keys, one kv head of 128, 27 us, 24; of 256 51, 45; with four heads of 128 28.8, 31.4.
-  const int64_t most = 4 * PARTS * (int64_t)rows.size() * g.n_kv_heads <= num_cus ? 2 * PARTS : PARTS;
+  // keys, one kv head of 128, 27 us, 24.6 (on 20000 16.4, 18.4); of 256 51, 45; with four heads of 128 29.0, 31.8.
+  const int64_t most = 4 * PARTS * row_heads <= num_cus ? 2 * PARTS : PARTS;
   split(rows, SEQ_ROWS_CHUNK, slots_per_head(g, num_cus, tiles.empty() || !seq_one_launch(g.head_dim)), ROWS_LEAST, ROWS_COST,
-        most, &out->rows);
-  split(tiles, SEQ_KEY_TILE, slots_per_head(g, num_cus, false), TILES_LEAST, TILES_COST, PARTS, &out->tiles);
+        row_merged, most, &out->rows);
+  split(tiles, SEQ_KEY_TILE, slots_per_head(g, num_cus, false), TILES_LEAST, TILES_COST, tile_merged, PARTS, &out->tiles);
   std::sort(pieces.begin(), pieces.end(),
             [](const Piece &x, const Piece &y) { return x.page != y.page ? x.page < y.page : x.off < y.off; });
   for (size_t i = 1; i < pieces.size(); ++i)

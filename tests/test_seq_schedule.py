@@ -56,3 +56,18 @@ def test_a_longer_hidden_prefix_changes_no_kernel(host, h, kv, d, mode, window):
             r, t, counts = plan(host, geom(h, kv, d, mode, window, 64), q, [prefix + x for x in q])
             shapes.add((tuple(counts[:4]), counts[6], *((tuple(i["k_end"] - i["k_begin"]), tuple(i["n_parts"])) for i in (r, t))))
         assert len(shapes) == 1, f"{q}: {[s[0] for s in shapes]}"
+
+
+def test_parts_of_a_tile_follow_its_keys(host):
+    """16 states are merged in one pass, which pays up to a length that depends on the kind of items."""
+    def parts(kv, n, q=1, g=8, d=128):
+        r, t, _ = plan(host, geom(kv * g, kv, d, ps=64), [q], [n])
+        return [int(i["n_parts"].max(initial=0)) for i in (r, t)]
+
+    for kv in (1, 4):
+        assert parts(kv, 8000)[0] == 16 and parts(kv, 12000)[0] == 16
+        assert parts(kv, 16000)[0] == 32 and parts(kv, 30000)[0] == 32 and parts(kv, 60000)[0] == (64 if kv == 1 else 32)
+    assert parts(8, 16000)[0] == 16 and parts(8, 20000)[0] == 32  # (every CU has work with 16)
+    # tiles, of batches that are too large for the kernel of few rows
+    assert parts(1, 12000, 256)[1] == 16 and parts(1, 24000, 128)[1] == 32 and parts(4, 24000, 32)[1] == 32
+    assert parts(1, 20000, 256, d=64)[1] == 16
