@@ -950,3 +950,99 @@ def test_updates_of_a_captured_plan_allocate_nothing(rk):
 def test_windowed_chunks_behind_long_prefixes(rk, q, kv_len, mode, window):
     note(f"paged, chunk of {q} of {kv_len}, mode {mode} window {window}")
     paged_case(rk, q + window, [q, 1], [kv_len, 90], 64, 16, 4, 64, "bf16", mode=mode, window=window)
+
+
+class CallerStream:
+    """A stream that the library did not make."""
+
+    def __init__(self):
+        with open("/proc/self/maps") as f:
+            self.hip = ctypes.CDLL(next(line.split()[-1] for line in f if "libamdhip64" in line))
+        s = ctypes.c_void_p()
+        assert self.hip.hipStreamCreateWithFlags(ctypes.byref(s), 1) == 0  # non-blocking
+        self.ptr = s.value
+
+    def destroy(self):
+        assert self.hip.hipStreamDestroy(ctypes.c_void_p(self.ptr)) == 0
+
+
+def two_streams(rk, own):
+    made = [None if own else CallerStream() for _ in range(2)]
+    sts = [rk.new_stream() if own else m.ptr for m in made]
+
+    def done():
+        for st, m in zip(sts, made):
+            rk.synchronize(st)
+            rk.destroy_stream(st) if own else m.destroy()
+
+    return sts, done
+
+
+@pytest.mark.parametrize("own", [True, False])
+def test_a_plan_s_batches_on_two_streams_each_see_their_own(rk, own):
+    """Updates alternate between two batches, each on its own stream, with nothing waited for between them: neither's
+    lists reach the other's call."""
+    note(f"two batches on two streams, the library's own: {own}")
+    h, kv, d, ps = 32, 4, 128, 16
+    pg, caches, keys, q = paged_inputs(80, [60000, 3000], ps, h, kv, d, "f16", [1, 1])
+    other = pg.table.copy()
+    other[[0, 1]] = other[[1, 0]]
+    batches = [([1, 1], [60000, 2900], pg.table), ([1, 1], [70, 41000], other)]
+    want = []
+    for ql, kl, table in batches:
+        plan = rk.paged_plan(ql, kl, table, pg.n_pages, ps, h, kv, d)
+        want.append(paged(rk, pg, caches, q, ql, kl, h, kv, d, "f16", 0.1, plan=plan))
+    check_paged(want[0], [[t[0], t[1][:2900]] for t in keys], q, [1, 1], batches[0][1], h, kv, d, "f16", 0.1)
+    check_paged(want[1], [[t[1][:70], t[0][:41000]] for t in keys], q, [1, 1], batches[1][1], h, kv, d, "f16", 0.1)
+    assert (want[0] != want[1]).any(1).all()
+    b = upload(rk, q, *caches)
+    outs = [rk.DeviceBuffer(q.nbytes) for _ in range(12)]
+    plan = rk.paged_plan(*batches[0], pg.n_pages, ps, h, kv, d)
+    plan.update(*batches[1])  # (room for both: no later update waits to allocate)
+    sts, done = two_streams(rk, own)
+    for i, o in enumerate(outs):
+        plan.update(*batches[i % 2], stream=sts[i % 2])
+        for _ in range(3):
+            ok(rk, rk.lib().rk_attention_paged_dev(plan.ptr, b[0].ptr, h * d, b[1].ptr, b[2].ptr, 0.1, 0.0, o.ptr, h * d, rk.DTYPE_F16,
+                                                   sts[i % 2]))
+    done()
+    for i, o in enumerate(outs):
+        assert (o.download(q.shape, np.uint16) == want[i % 2]).all(), f"call {i}"
+    plan.destroy()
+
+
+@pytest.mark.parametrize("own", [True, False])
+def test_an_update_that_grows_a_plan_in_use_waits_for_it(rk, own):
+    """The lists and states of a call that still runs on another stream are not given back under it."""
+    note(f"growth in use, the library's own streams: {own}")
+    rng, h, kv, d = np.random.default_rng(81), 8, 1, 128
+    small, large = [3000], [2500, *[3] * 500]
+    toks = sum(large)
+    q, k, v = (rows(rng, "bf16", toks, n * d) for n in (h, kv, kv))
+    want = [packed(rk, *(a[:sum(lens)] for a in (q, k, v)), lens, h, kv, d, "bf16", 0.1) for lens in (small, large)]
+    b = upload(rk, q, k, v)
+    sts, done = two_streams(rk, own)
+    for i in range(4):
+        plan, outs = rk.packed_plan(small, h, kv, d), [rk.DeviceBuffer(q.nbytes) for _ in range(2)]
+
+        def call(o, st):
+            ok(rk, rk.lib().rk_attention_packed_dev(plan.ptr, b[0].ptr, h * d, b[1].ptr, kv * d, b[2].ptr, kv * d, 0.1, 0.0, o.ptr, h * d,
+                                                    rk.DTYPE_BF16, st))
+
+        for _ in range(5):
+            call(outs[0], sts[0])
+        plan.update(large, stream=sts[1])
+        call(outs[1], sts[1])
+        for st in sts:
+            rk.synchronize(st)
+        for o, w in zip(outs, want):
+            assert (o.download(w.shape, np.uint16) == w).all()
+        plan.destroy()
+    done()
+
+
+@pytest.mark.parametrize("mode,window", [(1, -1), (3, 200), (0, -1)])
+@pytest.mark.parametrize("h,kv,d", [(8, 2, 64), (16, 2, 128), (3, 1, 256), (4, 4, 72)])
+def test_paged_softcap_in_bf16(rk, mode, window, h, kv, d):
+    note(f"paged, bf16, softcap, mode {mode} {h}/{kv} d={d}")
+    paged_case(rk, 82, [1, 150, 20], [700, 600, 20], 32, h, kv, d, "bf16", mode=mode, window=window, softcap=20.0)
