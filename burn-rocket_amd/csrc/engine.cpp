@@ -2472,6 +2472,25 @@ void seq_buf_free(DevBuf &b) {
   b = DevBuf{};
 }
 
+int is_capturing(hipStream_t st, bool *yes, const char *op) {
+  hipStreamCaptureStatus s = hipStreamCaptureStatusNone;
+  HIP_TRY(hipStreamIsCapturing(st, &s), op);
+  *yes = s != hipStreamCaptureStatusNone;
+  return RK_OK;
+}
+
+// Refuses what has to wait for a plan's last call while that call's stream is captured: an
+// event recorded there now would belong to the graph, and a stream that waits for it to the
+// capture. (Calls on `st` itself wait for nothing.)
+int seq_fenceable(const SeqPlan &p, hipStream_t st, const char *op) {
+  for (const DevBuf *b : {&p.block, &p.work}) {
+    bool capturing = false;
+    if (b->pending && b->ev_stream != st) RK_TRY(is_capturing(b->ev_stream, &capturing, op));
+    if (capturing) return fail(RK_E_UNSUPPORTED, op, "the stream of the plan's last call is being captured");
+  }
+  return RK_OK;
+}
+
 // The end of a buffer's last use, awaited by the host.
 int seq_buf_wait(DevBuf &b, const char *op) {
   if (!b.ev) return RK_OK;
@@ -2492,13 +2511,6 @@ int seq_buf_use(CallScope &cs, DevBuf &b, bool capturing, const char *op) {
     HIP_TRY(hipStreamWaitEvent(cs.st, b.ev, 0), op);
   }
   cs.used.push_back(&b);
-  return RK_OK;
-}
-
-int is_capturing(hipStream_t st, bool *yes, const char *op) {
-  hipStreamCaptureStatus s = hipStreamCaptureStatusNone;
-  HIP_TRY(hipStreamIsCapturing(st, &s), op);
-  *yes = s != hipStreamCaptureStatusNone;
   return RK_OK;
 }
 
@@ -2647,6 +2659,7 @@ int seq_plan_update(void *plan, bool paged, const SeqBatch &b, rk_stream stream,
   bool capturing;
   RK_TRY(is_capturing(st, &capturing, op));
   if (capturing) return fail(RK_E_UNSUPPORTED, op, "a plan is not updated inside a capture: its lists come from the host");
+  RK_TRY(seq_fenceable(*p, st, op));
   SeqLists l;
   seq_build(p->geom, b, g_eng->num_cus, &l);
   if (p->captured) {
@@ -2705,6 +2718,7 @@ int seq_attention(const void *plan, bool paged, const void *q, int64_t q_stride,
   RK_TRY(seq_rows_check(v, paged ? kw : v_stride, kw, paged ? "v_cache" : "v", op));
   if (!paged && std::max(k_stride, v_stride) >= SEQ_MAX_STRIDE)
     return fail(RK_E_SHAPE, op, "k and v strides must be below 2^26 values");
+  if (!capturing) RK_TRY(seq_fenceable(*p, st, op));
   CallScope cs(st);
   RK_TRY(seq_buf_use(cs, p->block, capturing, op));
   RK_TRY(seq_buf_use(cs, p->work, capturing, op));
@@ -2800,6 +2814,7 @@ extern "C" int rk_seq_plan_reserve(void *plan, int64_t max_q_len) {
     SeqPlan *p;
     RK_TRY(seq_plan_get(plan, -1, &p, op));
     if (p->captured) return fail(RK_E_UNSUPPORTED, op, "a graph holds this plan");
+    RK_TRY(seq_fenceable(*p, nullptr, op));
     const int64_t G = p->geom.n_head / p->geom.n_kv_heads;
     const int64_t longest = std::max<int64_t>({max_q_len, p->lists.max_q, 1});
     if (longest > INT32_MAX / G) return fail(RK_E_SHAPE, op, "max_q_len·(n_head/n_kv_heads) of 2^31 or more");
@@ -2835,6 +2850,7 @@ extern "C" int rk_seq_plan_destroy(void *plan) {
     if (!plan) return RK_OK;
     SeqPlan *p;
     RK_TRY(seq_plan_get(plan, -1, &p, op));
+    RK_TRY(seq_fenceable(*p, nullptr, op));
     // Calls and uploads that read its buffers end first; replays of a graph that
     // holds them are known to the device alone.
     if (p->captured) HIP_TRY(hipDeviceSynchronize(), op);
@@ -2902,6 +2918,7 @@ extern "C" int rk_paged_append_dev(const void *plan, const void *qkv, int64_t ro
     if (p->lists.clash) return fail(RK_E_SHAPE, op, "two new tokens of the batch go to one slot of a page");
     const int64_t n = capturing ? (int64_t)p->room.toks : p->lists.n_tokens;
     if (n * heads > INT32_MAX) return fail(RK_E_SHAPE, op, "2^31 or more head rows");
+    if (!capturing) RK_TRY(seq_fenceable(*p, st, op));
     CallScope cs(st);
     RK_TRY(seq_buf_use(cs, p->block, capturing, op));
     PagedAppendArgs a{};

@@ -438,7 +438,9 @@ int rk_flash_attn_f16_masked(int64_t n_q, int64_t n_kv, int head_dim, int dv, in
  * refused batch (RK_E_SHAPE) leaves the plan as it was; an update or a reserve that
  * fails for want of memory leaves it with an empty batch.
  *
- * Streams: calls on one plan from different streams run one after another. Before
+ * Streams: calls on one plan from different streams run one after another; while the
+ * stream of its last call is captured, whatever would have to wait for that call is
+ * refused (RK_E_UNSUPPORTED). Before
  * a call is captured into a graph, rk_seq_plan_reserve gives the plan room for any
  * later batch of no more sequences, tokens and pages than its present one, with
  * q_lens up to max_q_len (below the present longest: that one); nothing is allocated

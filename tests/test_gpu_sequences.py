@@ -1046,3 +1046,45 @@ def test_an_update_that_grows_a_plan_in_use_waits_for_it(rk, own):
 def test_paged_softcap_in_bf16(rk, mode, window, h, kv, d):
     note(f"paged, bf16, softcap, mode {mode} {h}/{kv} d={d}")
     paged_case(rk, 82, [1, 150, 20], [700, 600, 20], 32, h, kv, d, "bf16", mode=mode, window=window, softcap=20.0)
+
+
+def test_other_streams_are_refused_while_the_last_call_s_stream_is_captured(rk):
+    """A plan's last call ran on a stream that is then captured: a call elsewhere, which has to wait for it, does not
+    become part of the capture, and works afterwards."""
+    note("another stream beside a capture")
+    rng, lib, h, kv, d, lens = np.random.default_rng(83), rk.lib(), 8, 2, 64, [40, 1, 9]
+    q, k, v = (rows(rng, "f16", 50, n * d) for n in (h, kv, kv))
+    b, outs = upload(rk, q, k, v), [rk.DeviceBuffer(q.nbytes) for _ in range(2)]
+    plan, sts, seen = rk.packed_plan(lens, h, kv, d), [rk.new_stream(), rk.new_stream()], []
+    plan.reserve(50)
+
+    def call(i):
+        return lib.rk_attention_packed_dev(plan.ptr, b[0].ptr, h * d, b[1].ptr, kv * d, b[2].ptr, kv * d, 0.1, 0.0, outs[i].ptr, h * d,
+                                           rk.DTYPE_F16, sts[i])
+
+    ok(rk, call(0))  # a warm-up, as programs make before they capture
+
+    def step():
+        ok(rk, call(0))
+        seen.append(call(1))
+        for change in (lambda: plan.update([50], stream=sts[1]), lambda: plan.destroy()):
+            with pytest.raises(rk.RocketError) as e:
+                change()
+            seen.append(e.value.rc)
+
+    g = Graph(sts[0], step)
+    assert seen == [rk.RK_E_UNSUPPORTED] * 3
+    ok(rk, call(1))
+    for _ in range(3):
+        rk.synchronize(sts[1])  # (the order of replays and other calls is the caller's)
+        outs[0].upload(np.full(q.shape, FILL, np.uint16))
+        g.replay()
+        rk.synchronize(sts[0])
+        ok(rk, call(1))
+        rk.synchronize(sts[1])
+        for o in outs:
+            check_packed(o.download(q.shape, np.uint16), q, k, v, lens, h, kv, d, "f16", 0.1)
+    g.destroy()
+    plan.destroy()
+    for st in sts:
+        rk.destroy_stream(st)
