@@ -15,8 +15,8 @@
 //               as many products again;
 //   Oᵀ += Vᵀ·Pᵀ V rows from LDS as they lie in memory, through the transposing
 //               read, in the order of P's registers.
-// The LDS fragment reads feed QB products each; with 32 rows per wave they take
-// the whole read rate of a CU (128 bytes a clock) while the products run.
+// An LDS fragment of K feeds QB products, one of V 2·QB; with 32 rows per wave K's take
+// the whole read rate of a CU (128 bytes a clock) while the scores' products run.
 //
 // Row sums come from the same products (a row of ones), which takes their additions
 // off the softmax slot and counts the probabilities as they are held.
@@ -33,9 +33,11 @@
 // 1.2). With P as one value it took 742. 512 rows of 8 heads on 16901 keys 187 us (one value:
 // 147). 64 passages of 100 to 512 tokens 88 us (79): items of three key
 // tiles, whose first loads and last stores nothing hides. Head dim 256 has one 16-query
-// block per wave: every product reads its own 1 KB from LDS, twice the CU's rate. 58 us for
-// 9261 tokens, 3/1 heads, 512 keys to either side (one value of P: 52; 128 rows a workgroup, one
-// per CU, a quarter more).
+// block per wave: every score's product reads its own 1 KB from LDS, twice the CU's rate. 49 to 58 us
+// for 9261 tokens, 3/1 heads, 512 keys to either side (one value of P: 44 to 52; 128 rows a workgroup,
+// one per CU, a quarter more).
+//
+// Times beside the code that compare two forms were taken with P as one value.
 //
 // Items that are one of n_parts of their tile leave their state in the plan's
 // workspace; the last to arrive merges the parts in key order.

@@ -434,22 +434,25 @@ int rk_flash_attn_f16_masked(int64_t n_q, int64_t n_kv, int head_dim, int dv, in
  * The lists are copied: the caller's arrays may go when a call returns. An
  * update gives the plan another batch of the same heads, mask and pages; it is
  * ordered on `stream` after the calls that used the plan, waits on the host for
- * the upload of the update before it, and is refused inside a stream capture. A
- * refused batch (RK_E_SHAPE) leaves the plan as it was; an update or a reserve that
- * fails for want of memory leaves it with an empty batch.
+ * the upload of the update before it (with the library's lock held), and is refused
+ * inside a stream capture. One that needs more room than the plan has had so far
+ * (more items, tokens, page ids or split rows) reallocates: it waits for the calls that
+ * used the plan, and for the device. A plan made with the largest batch to come, or
+ * reserved on it, does not grow. A refused batch (RK_E_SHAPE) leaves the plan as it
+ * was; an update or a reserve that fails for want of memory leaves it with an empty batch.
  *
  * Streams: calls on one plan from different streams run one after another; while the
  * stream of its last call is captured, whatever would have to wait for that call is
- * refused (RK_E_UNSUPPORTED). Before
- * a call is captured into a graph, rk_seq_plan_reserve gives the plan room for any
- * later batch of no more sequences, tokens and pages than its present one, with
- * q_lens up to max_q_len (below the present longest: that one); nothing is allocated
- * in the capture or by later updates, launches have room for all of it, and updates
- * that need more are then refused (RK_E_SHAPE). The q, out and q|k|v buffers of a
- * captured call must have room for the tokens of the batch that the plan holds when
- * the call is captured; updates to a batch of more tokens are refused too. The caller orders the replays of
- * graphs that share a plan, and other calls and updates of a captured plan, after
- * one another. A plan is destroyed after its graphs. */
+ * refused (RK_E_UNSUPPORTED). Before a call is captured into a graph, rk_seq_plan_reserve
+ * gives the plan room for any later batch of no more sequences, tokens and pages than
+ * its present one, with q_lens up to max_q_len (below the present longest: that one);
+ * nothing is allocated in the capture or by later updates, launches have room for all
+ * of it, and updates that need more are then refused (RK_E_SHAPE). The q, out and q|k|v
+ * buffers of a captured call must have room for the tokens of the batch that the plan
+ * holds when the call is captured; updates to a batch of more tokens are refused too.
+ * The caller orders the replays of graphs that share a plan, and other calls and updates
+ * of a captured plan, after one another. A plan is destroyed after its graphs. Creating,
+ * reserving, growing and destroying plans is not for captures of any stream. */
 int rk_packed_plan_create(const int32_t *q_lens, int64_t n_seqs, int n_head, int n_kv_heads, int head_dim,
                           int mask_mode, int64_t window, void **plan);
 int rk_paged_plan_create(const int32_t *q_lens, const int32_t *kv_lens, const int32_t *page_table,
@@ -467,11 +470,12 @@ int rk_seq_plan_destroy(void *plan);
  * the same stride. dtype fp16 or bf16 (RK_DTYPE_*), strides multiples of 8 values,
  * buffers 16-byte aligned, head dims as rk_attention_dev without the padded ones.
  * Scores and softmax in f32, probabilities as two values of dtype for the product
- * with V (2^-16 of each is left), sums in f32, one rounding at the end. The split of a row's keys between workgroups depends on
- * the whole batch: a sequence's result can differ in rounding between batches, and
+ * with V (2^-16 of each is left), sums in f32, one rounding at the end: the parity
+ * of rk_attention_dev. The split of a row's keys between workgroups depends on the
+ * whole batch: a sequence's result can differ in rounding between batches, and
  * between a captured call (made for any batch of its plan's room) and one that is
  * not. Equal batches give equal bits. A non-finite value of V reaches every row of
- * its sequence that is computed in a tile with a row that sees it. */
+ * its sequence that is computed in a tile with a row that sees it, and no other. */
 int rk_attention_packed_dev(const void *plan, const void *q, int64_t q_stride, const void *k, int64_t k_stride,
                             const void *v, int64_t v_stride, float scale, float softcap, void *out,
                             int64_t out_stride, int dtype, rk_stream stream);
