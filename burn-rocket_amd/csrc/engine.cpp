@@ -2817,7 +2817,7 @@ extern "C" int rk_seq_plan_reserve(void *plan, int64_t max_q_len) {
     RK_TRY(seq_fenceable(*p, nullptr, op));
     const int64_t G = p->geom.n_head / p->geom.n_kv_heads;
     const int64_t longest = std::max<int64_t>({max_q_len, p->lists.max_q, 1});
-    if (longest > INT32_MAX / G) return fail(RK_E_SHAPE, op, "max_q_len·(n_head/n_kv_heads) of 2^31 or more");
+    if (longest > SEQ_MAX_ROWS / G) return fail(RK_E_SHAPE, op, "max_q_len·(n_head/n_kv_heads) above 2^31 - 129");
     SeqBound rows, tiles;
     seq_bound(p->geom, p->n_seqs, p->lists.n_tokens, longest, g_eng->num_cus, &rows, &tiles);
     SeqPlan::Room want = seq_room(p->lists);

@@ -60,7 +60,7 @@ std::string seq_check_batch(const SeqGeom &g, const SeqBatch &b) {
     const int64_t q = b.q_lens[i], kv = kv_of(b, i);
     if (q < 0 || kv < q) return at("needs 0 <= q_len <= kv_len");
     if (kv > MAX_KEYS) return at("more than 2^30 keys");
-    if (q * G > INT32_MAX) return at("q_len·(n_head/n_kv_heads) of 2^31 or more");
+    if (q * G > SEQ_MAX_ROWS) return at("q_len·(n_head/n_kv_heads) above 2^31 - 129");
     toks += q;
     if (toks > INT32_MAX) return "2^31 or more new tokens";
     if (!g.paged || q == 0) continue;

@@ -46,6 +46,7 @@ constexpr int seq_tile_rows(int head_dim) { return head_dim <= 128 ? 128 : 64; }
 // Whether one launch takes both kinds of items: where the row items' buffers leave two
 // workgroups a CU.
 constexpr bool seq_one_launch(int head_dim) { return head_dim <= 128; }
+constexpr int64_t SEQ_MAX_ROWS = INT32_MAX - 128;  // query rows of a sequence: a tile's last row stays inside 32 bits
 constexpr int64_t SEQ_MAX_STRIDE = (int64_t)1 << 26;  // values between packed tokens: 16 of them stay below 2 GiB
 
 struct SeqGeom {

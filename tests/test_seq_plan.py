@@ -151,3 +151,10 @@ def test_a_plan_whose_change_failed_has_no_tokens(monkeypatch, rc, left):
         with pytest.raises(rk.RocketError) as e:
             change(plan)
         assert e.value.rc == rc and plan.n_tokens == left
+
+
+def test_query_rows_stay_inside_32_bits(lib):
+    """A sequence of nearly 2^31 query rows: its last tile's rows are counted past the end."""
+    from burn_rocket import RK_E_DEVICE, RK_E_SHAPE
+    for q, rc in (((2**31 - 129) // 127, RK_E_DEVICE), ((2**31 - 129) // 127 + 1, RK_E_SHAPE), ((2**31 - 1) // 127, RK_E_SHAPE)):
+        assert packed(lib, i32(q), h=127, kv=1, d=32)[0] == rc, q
