@@ -170,11 +170,13 @@ void seq_build(const SeqGeom &g, const SeqBatch &b, int num_cus, SeqLists *out) 
   // A small batch goes to the kernel of few rows whole: at most four tiles of 16 rows per
   // CU whose products (each tile reads its K and V itself) take less than the other
   // kernel's walk over the longest sequence, both over the keys that its new tokens see.
-  // MI355X, rows -> tiles: 256 rows on 4096 keys, 32/4 heads of 128, 18.8 us, 27.3; 128 rows on
-  // 30000 41.6, 68; 256 rows on 30000 73, 68; 16 times 64 on 2000 25, 30; 16 times 96 on 300
-  // 14.5, 13.2. One prompt, causal: 300 tokens of 16/8 heads of 128 9.8, 13.0; 600 19.8, 21.1;
-  // 800 of 12/12 heads of 64 11.5, 18.8; 1200 18.1, 16.5; 200 of 32/4 heads of 128 10.2, 11.2;
-  // 300 15.9, 13.3. 64 tokens of 16/4 heads of 64, window 512, behind 2000 to 100000 keys 8.0, 15-17.
+  // The constants fit 497 batches on MI355X, of which 29 take more than 1.05 times the faster
+  // kernel. Rows -> tiles in us: 256 rows on 4096 keys, 32/4 heads of 128, 18.8, 27.3; 128 rows on
+  // 30000 41.6, 68; 256 rows on 30000 73, 68; 16 times 64 on 2000 25, 30; 256 rows of 8/2 heads of 256 on 8000
+  // 48.7, 38.3. One prompt, causal: 300 tokens of 16/8 heads of 128 9.8, 13.0; 400 12.5, 16.3; 500 15.0, 18.2 (tiles
+  // by the rule); 800 of 14/2 heads of 80 17.1, 22.4; 800 of 12/12 heads of 64 11.5, 18.8; 1000 15.8, 14.2 (rows by
+  // the rule); 200 of 32/4 heads of 128 10.2, 11.2; 300 15.9, 13.3. 64 tokens of 16/4 heads of 64, window 512, behind
+  // 2000 to 100000 keys 8.0, 15-17.
   int64_t n16 = 0, n16_keys = 0, longest = 0;
   for (int64_t i = 0; i < b.n_seqs; ++i) {
     if (b.q_lens[i] == 0) continue;
@@ -186,8 +188,7 @@ void seq_build(const SeqGeom &g, const SeqBatch &b, int num_cus, SeqLists *out) 
     n16_keys += t * (hi + 1 - lo);
     longest = std::max(longest, hi + 1 - lo);
   }
-  const bool small = n16 <= 4 * num_cus && n16_keys <= 4096ll * num_cus &&
-                     n16_keys * g.head_dim <= num_cus * (14000 + 140 * longest);
+  const bool small = n16 <= 4 * num_cus && n16_keys * g.head_dim <= num_cus * std::min(8000 + 220 * longest, (int64_t)393216);
   for (int64_t i = 0; i < b.n_seqs; ++i) {
     const int64_t q = b.q_lens[i], kv = kv_of(b, i), pos0 = kv - q;
     if (q == 0) continue;
