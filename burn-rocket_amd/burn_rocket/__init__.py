@@ -23,7 +23,7 @@ LIB_PATH = os.path.join(os.path.dirname(_HERE), "lib", "libburn_rocket_amd.so")
 RK_OK = 0
 RK_E_SHAPE, RK_E_TILING, RK_E_NOMEM, RK_E_DEVICE = -1, -2, -3, -4
 RK_E_UNSUPPORTED, RK_E_RANGE, RK_E_IO = -5, -6, -7
-RK_WEIGHT_F16, RK_WEIGHT_I8, RK_WEIGHT_QAT = 1, 2, 3
+RK_WEIGHT_F16, RK_WEIGHT_I8, RK_WEIGHT_QAT, RK_WEIGHT_FP8 = 1, 2, 3, 4
 MASK_NONE, MASK_CAUSAL, MASK_WINDOW, MASK_CAUSAL_WINDOW = 0, 1, 2, 3
 NOALLOC_SCRATCH_BYTES = 32 << 20  # RK_NOALLOC_SCRATCH_BYTES
 DTYPE_F32, DTYPE_F16, DTYPE_BF16 = 0, 1, 2
@@ -64,6 +64,11 @@ SIGNATURES = {
     "rk_matmul_w8a8_f16out_dev": (_i, [_u64, _p, _p, _i64, _i64, _i64, _p, _p]),
     "rk_matmul_i8_raw_dev": (_i, [_u64, _p, _i64, _i64, _p, _p]),
     "rk_matmul_i8_partials_dev": (_i, [_u64, _p, _i64, _i64, _p, _p]),
+    "rk_pack_fp8": (_i, [_p, _p, _i64, _i64, _p]),
+    "rk_pack_fp8_f32": (_i, [_p, _i64, _i64, _p]),
+    "rk_quantize_fp8_dev": (_i, [_p, _i, _i64, _i64, _p, _p, _p]),
+    "rk_matmul_fp8_codes_dev": (_i, [_u64, _p, _p, _i64, _i64, _p, _i, _p]),
+    "rk_matmul_fp8_dev": (_i, [_u64, _p, _i, _i64, _i64, _p, _i, _p]),
     "rk_attention": (_i, [_p, _p, _p, _i64, _i64, _i, _i, _i, _f, _f, _i, _i64, _i64, _i64, _p]),
     "rk_attention_dev": (_i, [_p, _p, _p, _i64, _i64, _i, _i, _i, _f, _f, _i, _i64, _i64, _i64, _p, _p]),
     "rk_attention_dev_noalloc": (_i, [_p, _p, _p, _i64, _i64, _i, _i, _i, _f, _f, _i, _i64, _i64, _i64, _p, _p]),
@@ -318,6 +323,58 @@ def pack_qat(codes, w_scale, n, k, in_scale, out_scale):
     _check(_lib.rk_pack_qat(_ptr(codes), _ptr(w_scale), n, k, in_scale, out_scale, ctypes.byref(out)),
            "rocket_i8_weights_pack", 0, k, n)
     return WeightId(out.value)
+
+
+def _blocks(n):
+    return -(-n // 128)
+
+
+def pack_fp8(codes, scales):
+    """Resident fp8 weight from e4m3 codes [N, K] (their bytes) and one f32 scale per 128 x 128 block
+    [ceil(N/128), ceil(K/128)]."""
+    codes, scales = np.ascontiguousarray(codes, dtype=np.uint8), _f32(scales)
+    n, k = codes.shape
+    if scales.shape != (_blocks(n), _blocks(k)):
+        _shape_error("pack_fp8", f"scales must be [{_blocks(n)}, {_blocks(k)}]")
+    out = ctypes.c_uint64()
+    _check(load_library().rk_pack_fp8(_ptr(codes), _ptr(scales), n, k, ctypes.byref(out)), "pack_fp8", 0, k, n)
+    return WeightId(out.value)
+
+
+def pack_fp8_f32(w):
+    """Resident fp8 weight from f32 [N, K], quantized per 128 x 128 block on the device."""
+    wf = _f32(w)
+    n, k = wf.shape
+    out = ctypes.c_uint64()
+    _check(load_library().rk_pack_fp8_f32(_ptr(wf), n, k, ctypes.byref(out)), "pack_fp8", 0, k, n)
+    return WeightId(out.value)
+
+
+def quantize_fp8(x, bf16=False):
+    """Rows of x [M, K] as e4m3 codes (uint8 [M, K]) and scales f32 [M, ceil(K/128)]. f32, float16, or bf16 bits in
+    uint16 with bf16=True."""
+    x = np.ascontiguousarray(x)
+    dt = _float_dtype(x, bf16, "quantize_fp8")
+    m, k = x.shape
+    q, s = np.empty((m, k), np.uint8), np.empty((m, _blocks(k)), np.float32)
+    if m == 0:
+        return q, s
+    bufs = [DeviceBuffer.from_array(x), DeviceBuffer(q.nbytes), DeviceBuffer(s.nbytes)]
+    _check(_lib.rk_quantize_fp8_dev(bufs[0].ptr, dt, m, k, bufs[1].ptr, bufs[2].ptr, None), "quantize_fp8", m, k)
+    synchronize()
+    return bufs[1].download(q.shape, q.dtype), bufs[2].download(s.shape, s.dtype)
+
+
+def matmul_fp8(x, wid, bf16=False):
+    """x [M, K] through an fp8 weight, quantized on the way; returned in x's type (as `quantize_fp8` takes it)."""
+    x = np.ascontiguousarray(x)
+    dt = _float_dtype(x, bf16, "matmul_fp8")
+    m, k = x.shape
+    n = weight_info(wid)[1]
+    out = np.empty((m, n), x.dtype)
+    if m == 0:
+        return out
+    return _run_dev("rk_matmul_fp8_dev", "matmul_fp8", out, [x], lambda p, o: (int(wid), p[0], dt, m, k, o, dt, None))
 
 
 def weight_info(wid):

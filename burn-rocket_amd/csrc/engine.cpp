@@ -104,6 +104,7 @@ struct Weight {
   int8_t *gu_codes = nullptr, *dn_codes = nullptr;
   float *gu_scales = nullptr, *dn_scales = nullptr;
   int gu_ws_stride = 0, dn_ws_stride = 0;
+  // RK_WEIGHT_FP8: codes in the resident layout of fp8.hpp, scales [ceil(n/128), ws_stride], ws_stride = ceil(k/128)
 };
 
 // A batch of sequences (rk_packed_plan_create, rk_paged_plan_create): the lists
@@ -272,6 +273,13 @@ int64_t stage_chunk_rows(int64_t rows, size_t in_row, size_t out_row) {
   c = std::max<int64_t>(c, (rows + rkstage::HostStage::kMaxChunks - 1) / rkstage::HostStage::kMaxChunks);
   c = round_up_i(c, 16);
   return std::min<int64_t>(c, std::max<int64_t>(rows, 1));
+}
+
+int is_capturing(hipStream_t st, bool *yes, const char *op) {
+  hipStreamCaptureStatus s = hipStreamCaptureStatusNone;
+  HIP_TRY(hipStreamIsCapturing(st, &s), op);
+  *yes = s != hipStreamCaptureStatusNone;
+  return RK_OK;
 }
 
 Weight *find(uint64_t id) {
@@ -889,6 +897,41 @@ int gemm_f16_run(CallScope &cs, const void *a, const void *b, void *c, int64_t m
   return RK_OK;
 }
 
+// c = codes · Wᵀ for an fp8 weight. Results that stay f32 take the products with f32 sums (fp8.hpp).
+int fp8_product_run(const Weight &w, const uint8_t *a, const float *as, int64_t m, void *c, int c_dtype, hipStream_t st,
+                    const char *op) {
+  const bool exact = c_dtype == RK_DTYPE_F32;
+  if (rk_fp8_few_fits_codes(m)) {
+    Fp8FewArgs g{};
+    g.x = a;
+    g.as = as;
+    g.m = (int)m;
+    g.n = (int)w.n;
+    g.k = (int)w.k;
+    g.kt = w.ws_stride;
+    g.w = (const uint8_t *)w.codes;
+    g.ws = w.scales;
+    g.c = c;
+    g.c_dtype = c_dtype;
+    HIP_TRY(rk_launch_fp8_few(g, 3, exact, st), op);
+    return RK_OK;
+  }
+  Fp8GemmArgs g{};
+  g.a = a;
+  g.as = as;
+  g.m = m;
+  g.n = (int)w.n;
+  g.k = (int)w.k;
+  g.kt = w.ws_stride;
+  g.w = (const uint8_t *)w.codes;
+  g.ws = w.scales;
+  g.c = c;
+  g.c_dtype = c_dtype;
+  g.num_cus = g_eng->num_cus;
+  HIP_TRY(rk_launch_gemm_fp8(g, exact, st), op);
+  return RK_OK;
+}
+
 int check_m(int64_t m, int64_t k, const Weight *w, const char *op) {
   if (!w) return fail(RK_E_SHAPE, op, "weight id is not packed");
   if (m < 0) return fail(RK_E_SHAPE, op, "M must not be negative");
@@ -940,6 +983,16 @@ extern "C" int rk_matmul(rk_weight_id id, const float *x, int64_t m, int64_t k, 
               "rk_matmul");
       return launch_i8(*w, q + r0 * k, s + r0 * ng, (int)ng, (int)(w->group / 32), I8_PER_GROUP, false,
                        r1 - r0, y32 + r0 * n, st, "rk_matmul_int8_gw");
+    };
+  } else if (w->kind == RK_WEIGHT_FP8) {
+    uint8_t *q;
+    float *s;
+    const int64_t ks = w->ws_stride;
+    RK_TRY(scratch(cs, "mm_q", (size_t)m * k, (void **)&q));
+    RK_TRY(scratch(cs, "mm_s", (size_t)m * ks * 4, (void **)&s));
+    compute = [=](int64_t r0, int64_t r1) {
+      HIP_TRY(rk_launch_quantize_fp8(x32 + r0 * k, RK_DTYPE_F32, r1 - r0, (int)k, q + r0 * k, k, s + r0 * ks, st), "rk_matmul");
+      return fp8_product_run(*w, q + r0 * k, s + r0 * ks, r1 - r0, y32 + r0 * n, RK_DTYPE_F32, st, "rk_matmul_fp8");
     };
   } else {  // QAT
     int8_t *q;
@@ -2472,13 +2525,6 @@ void seq_buf_free(DevBuf &b) {
   b = DevBuf{};
 }
 
-int is_capturing(hipStream_t st, bool *yes, const char *op) {
-  hipStreamCaptureStatus s = hipStreamCaptureStatusNone;
-  HIP_TRY(hipStreamIsCapturing(st, &s), op);
-  *yes = s != hipStreamCaptureStatusNone;
-  return RK_OK;
-}
-
 // Refuses what has to wait for a plan's last call while that call's stream is captured: an
 // event recorded there now would belong to the graph, and a stream that waits for it to the
 // capture. (Calls on `st` itself wait for nothing.)
@@ -2948,6 +2994,162 @@ extern "C" int rk_paged_append_dev(const void *plan, const void *qkv, int64_t ro
     HIP_TRY(rk_launch_paged_append(a, dtype, cs_dtype, st), op);
     return RK_OK;
   });
+}
+
+// =========================================================================
+// Block-scaled fp8
+// =========================================================================
+namespace {
+bool fp8_float(int dtype) { return dtype >= RK_DTYPE_F32 && dtype <= RK_DTYPE_BF16; }
+
+// Offsets inside a tile's rows, and inside 256 rows of the weight, are 32-bit.
+int fp8_check_shape(int64_t n, int64_t k, const char *op) {
+  if (n <= 0 || k <= 0) return fail(RK_E_SHAPE, op, "empty weight");
+  if (k % 16 != 0) return fail(RK_E_SHAPE, op, "K must be a multiple of 16 (16-byte rows of codes)");
+  if (n > (1 << 22) || k > (1 << 22)) return fail(RK_E_SHAPE, op, "dimension above 2^22");
+  return RK_OK;
+}
+
+// A weight's buffers: codes with rows and K padded to 128 by zeros, scales.
+int fp8_alloc(Weight &w, int64_t n, int64_t k, const char *op) {
+  w.kind = RK_WEIGHT_FP8;
+  w.n = n;
+  w.k = k;
+  w.group = 128;
+  w.ws_stride = (int)((k + 127) / 128);
+  const int64_t nb = (n + 127) / 128;
+  const size_t codes = (size_t)nb * 128 * w.ws_stride * 128, scales = (size_t)nb * w.ws_stride * 4;
+  HIP_TRY(hipMalloc(&w.codes, codes), op);
+  HIP_TRY(hipMalloc((void **)&w.scales, scales), op);
+  HIP_TRY(hipMemsetAsync(w.codes, 0, codes, g_eng->stream), op);
+  w.bytes = codes + scales;
+  return RK_OK;
+}
+
+int fp8_rows_check(const void *p, const char *what, const char *op) {
+  if (!p) return fail(RK_E_SHAPE, op, std::string("null ") + what);
+  if ((uintptr_t)p & 15) return fail(RK_E_SHAPE, op, std::string(what) + " must be 16-byte aligned");
+  return RK_OK;
+}
+
+int fp8_weight(uint64_t id, int64_t m, int64_t k, Weight **w, const char *op) {
+  *w = find(id);
+  RK_TRY(check_m(m, k, *w, op));
+  if ((*w)->kind != RK_WEIGHT_FP8) return fail(RK_E_UNSUPPORTED, op, "weight is not fp8");
+  return RK_OK;
+}
+}  // namespace
+
+extern "C" int rk_pack_fp8(const uint8_t *codes, const float *scales, int64_t n, int64_t k, rk_weight_id *id) {
+  std::lock_guard<std::mutex> lk(g_mu);
+  const char *op = "rk_pack_fp8";
+  RK_TRY(ensure(op));
+  if (!codes || !scales || !id) return fail(RK_E_SHAPE, op, "null buffer");
+  RK_TRY(fp8_check_shape(n, k, op));
+  Weight w;
+  PackGuard guard(w);
+  RK_TRY(fp8_alloc(w, n, k, op));
+  CallScope cs(g_eng->stream);
+  void *dev;
+  RK_TRY(scratch(cs, "pack_blk", (size_t)n * k, &dev));
+  HIP_TRY(hipMemcpyAsync(dev, codes, (size_t)n * k, hipMemcpyHostToDevice, cs.st), op);
+  HIP_TRY(rk_launch_fp8_layout((const uint8_t *)dev, n, (int)k, 32, 0, (uint8_t *)w.codes, cs.st), op);
+  HIP_TRY(hipMemcpyAsync(w.scales, scales, (size_t)((n + 127) / 128) * w.ws_stride * 4, hipMemcpyHostToDevice, cs.st), op);
+  HIP_TRY(hipStreamSynchronize(cs.st), op);
+  *id = guard.register_weight();
+  return RK_OK;
+}
+
+extern "C" int rk_pack_fp8_f32(const float *w32, int64_t n, int64_t k, rk_weight_id *id) {
+  std::lock_guard<std::mutex> lk(g_mu);
+  const char *op = "rk_pack_fp8_f32";
+  RK_TRY(ensure(op));
+  if (!w32 || !id) return fail(RK_E_SHAPE, op, "null buffer");
+  RK_TRY(fp8_check_shape(n, k, op));
+  Weight w;
+  PackGuard guard(w);
+  RK_TRY(fp8_alloc(w, n, k, op));
+  CallScope cs(g_eng->stream);
+  void *dev;
+  RK_TRY(scratch(cs, "pack_f32", (size_t)n * k * 4, &dev));
+  HIP_TRY(hipMemcpyAsync(dev, w32, (size_t)n * k * 4, hipMemcpyHostToDevice, cs.st), op);
+  HIP_TRY(rk_launch_fp8_pack((const float *)dev, n, (int)k, 32, 0, (uint8_t *)w.codes, w.scales, cs.st), op);
+  HIP_TRY(hipStreamSynchronize(cs.st), op);
+  *id = guard.register_weight();
+  return RK_OK;
+}
+
+extern "C" int rk_quantize_fp8_dev(const void *x, int x_dtype, int64_t m, int64_t k, uint8_t *q, float *scale, rk_stream stream) {
+  std::lock_guard<std::mutex> lk(g_mu);
+  const char *op = "rk_quantize_fp8_dev";
+  RK_TRY(ensure(op));
+  if (m < 0 || m > INT32_MAX) return fail(RK_E_SHAPE, op, "M must be in [0, 2^31)");
+  RK_TRY(fp8_check_shape(1, k, op));
+  if (!fp8_float(x_dtype)) return fail(RK_E_SHAPE, op, "unknown dtype");
+  if (m == 0) return RK_OK;
+  RK_TRY(fp8_rows_check(x, "x", op));
+  RK_TRY(fp8_rows_check(q, "q", op));
+  if (!scale) return fail(RK_E_SHAPE, op, "null scale buffer");
+  HIP_TRY(rk_launch_quantize_fp8(x, x_dtype, m, (int)k, q, k, scale, pick(stream)), op);
+  return RK_OK;
+}
+
+extern "C" int rk_matmul_fp8_codes_dev(rk_weight_id id, const uint8_t *a, const float *a_scale, int64_t m, int64_t k, void *c,
+                                       int c_dtype, rk_stream stream) {
+  std::lock_guard<std::mutex> lk(g_mu);
+  const char *op = "rk_matmul_fp8_codes_dev";
+  RK_TRY(ensure(op));
+  Weight *w;
+  RK_TRY(fp8_weight(id, m, k, &w, op));
+  if (!fp8_float(c_dtype)) return fail(RK_E_SHAPE, op, "unknown dtype");
+  if (m == 0) return RK_OK;
+  RK_TRY(fp8_rows_check(a, "a", op));
+  RK_TRY(fp8_rows_check(c, "c", op));
+  if (!a_scale) return fail(RK_E_SHAPE, op, "null scale buffer");
+  RK_TRY(fp8_product_run(*w, a, a_scale, m, c, c_dtype, pick(stream), op));
+  g_eng->calls++;
+  return RK_OK;
+}
+
+extern "C" int rk_matmul_fp8_dev(rk_weight_id id, const void *x, int x_dtype, int64_t m, int64_t k, void *c, int c_dtype,
+                                 rk_stream stream) {
+  std::lock_guard<std::mutex> lk(g_mu);
+  const char *op = "rk_matmul_fp8_dev";
+  RK_TRY(ensure(op));
+  Weight *w;
+  RK_TRY(fp8_weight(id, m, k, &w, op));
+  if (!fp8_float(x_dtype) || !fp8_float(c_dtype)) return fail(RK_E_SHAPE, op, "unknown dtype");
+  if (m == 0) return RK_OK;
+  RK_TRY(fp8_rows_check(x, "x", op));
+  RK_TRY(fp8_rows_check(c, "c", op));
+  hipStream_t st = pick(stream);
+  if (rk_fp8_few_fits_x(m, w->ws_stride)) {  // one launch, nothing in library memory
+    Fp8FewArgs g{};
+    g.x = x;
+    g.m = (int)m;
+    g.n = (int)w->n;
+    g.k = (int)k;
+    g.kt = w->ws_stride;
+    g.w = (const uint8_t *)w->codes;
+    g.ws = w->scales;
+    g.c = c;
+    g.c_dtype = c_dtype;
+    HIP_TRY(rk_launch_fp8_few(g, x_dtype, c_dtype == RK_DTYPE_F32, st), op);
+  } else {
+    bool capturing;
+    RK_TRY(is_capturing(st, &capturing, op));
+    if (capturing)
+      return fail(RK_E_UNSUPPORTED, op, "these rows are quantized into library memory, which a graph must not hold: capture "
+                                        "rk_quantize_fp8_dev and rk_matmul_fp8_codes_dev");
+    CallScope cs(st);
+    void *q, *s;
+    RK_TRY(scratch(cs, "fp8_q", (size_t)m * k, &q));
+    RK_TRY(scratch(cs, "fp8_s", (size_t)m * w->ws_stride * 4, &s));
+    HIP_TRY(rk_launch_quantize_fp8(x, x_dtype, m, (int)k, (uint8_t *)q, k, (float *)s, st), op);
+    RK_TRY(fp8_product_run(*w, (const uint8_t *)q, (const float *)s, m, c, c_dtype, st, op));
+  }
+  g_eng->calls++;
+  return RK_OK;
 }
 
 // =========================================================================

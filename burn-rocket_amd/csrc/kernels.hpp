@@ -293,6 +293,45 @@ hipError_t rk_launch_moe_gemm_down(int tile_rows, int max_rows, const int8_t *aq
                                    int N, int K, const float *row_w, float *yb, const MoeCombine &cmb,
                                    hipStream_t st);
 
+// Block-scaled fp8 (fp8.hpp). Weights are in the resident layout; kt = ceil(K / 128).
+hipError_t rk_launch_quantize_fp8(const void *x, int dtype, int64_t m, int k, uint8_t *q, int64_t q_stride, float *scale,
+                                  hipStream_t st);
+hipError_t rk_launch_fp8_layout(const uint8_t *codes, int64_t n, int k, int grp_stride, int grp_off, uint8_t *out, hipStream_t st);
+hipError_t rk_launch_fp8_pack(const float *w, int64_t n, int k, int grp_stride, int grp_off, uint8_t *out, float *scale,
+                              hipStream_t st);
+// Few rows (fp8_few.hip): x [m, k] of a float type, or codes [m, k] with scales [m, kt] (x_dtype 3).
+struct Fp8FewArgs {
+  const void *x;
+  const float *as;    // scales of codes
+  int m, n, k, kt;    // rows (dense), outputs, K
+  const uint8_t *w;
+  const float *ws;
+  void *c;            // [rows, n] of c_dtype
+  int c_dtype;
+  // experts: grid.y is a tile
+  const MoeTile *tiles;
+  const int32_t *tok;           // row of x of each bucket row (first product)
+  const float *row_w;           // router weight of each bucket row (second product)
+  int64_t w_stride, ws_stride;  // bytes and scales per expert
+  int64_t up_scales;            // scales from a gate block's to its up block's
+};
+bool rk_fp8_few_fits_x(int64_t m, int kt);
+bool rk_fp8_few_fits_codes(int64_t m);
+hipError_t rk_launch_fp8_few(const Fp8FewArgs &g, int x_dtype, bool exact, hipStream_t st);
+// Any rows (gemm_fp8.hip): codes [m, k] with scales [m, kt].
+struct Fp8GemmArgs {
+  const uint8_t *a;
+  const float *as;
+  int64_t m;
+  int n, k, kt;
+  const uint8_t *w;
+  const float *ws;
+  void *c;
+  int c_dtype;
+  int num_cus;
+};
+hipError_t rk_launch_gemm_fp8(const Fp8GemmArgs &g, bool exact, hipStream_t st);
+
 // The static device scratch of rk_attention_dev_noalloc (noalloc.hip):
 // rk_noalloc_setup looks up the array's address on `device`, which must be
 // current, once; rk_noalloc_scratch returns it (null before setup).

@@ -32,6 +32,7 @@ pub const RK_E_IO: c_int = -7;
 pub const RK_WEIGHT_F16: c_int = 1;
 pub const RK_WEIGHT_I8: c_int = 2;
 pub const RK_WEIGHT_QAT: c_int = 3;
+pub const RK_WEIGHT_FP8: c_int = 4;
 
 pub const RK_MASK_NONE: c_int = 0;
 pub const RK_MASK_CAUSAL: c_int = 1;
@@ -130,6 +131,19 @@ unsafe extern "C" {
     ) -> c_int;
     pub fn rk_matmul_i8_partials_dev(
         id: WeightId, a: *const i8, m: i64, k: i64, p: *mut i32, stream: Stream
+    ) -> c_int;
+    pub fn rk_pack_fp8(codes: *const u8, scales: *const f32, n: i64, k: i64, id: *mut WeightId) -> c_int;
+    pub fn rk_pack_fp8_f32(w: *const f32, n: i64, k: i64, id: *mut WeightId) -> c_int;
+    pub fn rk_quantize_fp8_dev(
+        x: *const c_void, x_dtype: c_int, m: i64, k: i64, q: *mut u8, scale: *mut f32, stream: Stream
+    ) -> c_int;
+    pub fn rk_matmul_fp8_codes_dev(
+        id: WeightId, a: *const u8, a_scale: *const f32, m: i64, k: i64, c: *mut c_void, c_dtype: c_int,
+        stream: Stream
+    ) -> c_int;
+    pub fn rk_matmul_fp8_dev(
+        id: WeightId, x: *const c_void, x_dtype: c_int, m: i64, k: i64, c: *mut c_void, c_dtype: c_int,
+        stream: Stream
     ) -> c_int;
     pub fn rk_attention(
         q: *const f32, k: *const f32, v: *const f32, n_q: i64, n_kv: i64, n_head: c_int,

@@ -51,6 +51,7 @@ extern "C" {
 #define RK_WEIGHT_F16 1 /* resident fp16 [N, K] */
 #define RK_WEIGHT_I8 2  /* resident int8 codes [N, K] + f32 scales [N, K/group] */
 #define RK_WEIGHT_QAT 3 /* resident per-channel int8 codes + w_scale [N] */
+#define RK_WEIGHT_FP8 4 /* resident e4m3 codes [N, K] + f32 scales [N/128, K/128] */
 
 /* ---- attention mask modes (ext.rs:1643-1666 `MaskMode`) ------------------ *
  * With absolute query position t = q0 + i and key position j = k0 + jj:
@@ -305,6 +306,43 @@ int rk_matmul_i8_raw_dev(rk_weight_id id, const int8_t *a, int64_t m, int64_t k,
  * per-K-tile partials of `drain`, int8.rs:708-746). */
 int rk_matmul_i8_partials_dev(rk_weight_id id, const int8_t *a, int64_t m,
                               int64_t k, int32_t *p, rk_stream stream);
+
+/* ---- block-scaled fp8 ----------------------------------------------------- *
+ * No counterpart in the reference, which has no fp8. Weights as block-scaled
+ * checkpoints hold them: e4m3 codes (OCP, no infinities) [N, K] with one f32 scale
+ * per 128 × 128 block, scales [ceil(N/128), ceil(K/128)]; a weight is its codes
+ * times their block's scale. Activations: e4m3 codes [M, K] with one f32 scale per
+ * row and 128 values, [M, ceil(K/128)]. N and M are any, K a multiple of 16; the
+ * last blocks may be short. Device buffers are 16-byte aligned (scales: 4).
+ *
+ *   c[m, n] = Σ_b as[m, b]·ws[n/128, b]·P_b[m, n],  P_b the product of block b's codes
+ *
+ * with the blocks summed in f32. P_b: with f32 results in f32; with fp16 and bf16 results by
+ * the fp8 matrix instructions, whose sums keep about 2^-16 of a result. The order of
+ * the sums depends on M, N, K and the types: a row's result can differ in rounding
+ * between calls of different M. Equal calls give equal bits. NaN codes, and rows of
+ * activations that hold an infinity or a NaN, give NaN results in their rows alone. */
+
+/* Weight from codes and scales on the host. */
+int rk_pack_fp8(const uint8_t *codes, const float *scales, int64_t n, int64_t k, rk_weight_id *id);
+/* Weight from f32 [N, K] on the host, quantized on the device: per block the scale
+ * max(amax/448, 1e-12), codes w / scale (an f32 number) rounded to nearest even. */
+int rk_pack_fp8_f32(const float *w, int64_t n, int64_t k, rk_weight_id *id);
+/* Rows of x [M, K] of type x_dtype (RK_DTYPE_*) to codes q [M, K] and scales
+ * [M, ceil(K/128)] by the same rule per row and block. A block that holds an
+ * infinity has an infinite scale; a NaN is the code NaN and does not enter its
+ * block's scale. */
+int rk_quantize_fp8_dev(const void *x, int x_dtype, int64_t m, int64_t k, uint8_t *q, float *scale, rk_stream stream);
+/* c [M, N] of type c_dtype = codes · Wᵀ, for codes that several weights share. */
+int rk_matmul_fp8_codes_dev(rk_weight_id id, const uint8_t *a, const float *a_scale, int64_t m, int64_t k, void *c,
+                            int c_dtype, rk_stream stream);
+/* x quantized on the way, then the product: the results of the two calls above up to
+ * the order of sums. Up to 32 rows of at most 64 KB of codes in all are one launch that uses no library
+ * memory; other sizes hold the codes in library scratch, and are refused inside a stream
+ * capture (RK_E_UNSUPPORTED): capture the two calls instead. rk_matmul takes fp8
+ * weights too. */
+int rk_matmul_fp8_dev(rk_weight_id id, const void *x, int x_dtype, int64_t m, int64_t k, void *c, int c_dtype,
+                      rk_stream stream);
 
 /* ======================================================================== *
  * Attention                                                                 *
