@@ -28,6 +28,7 @@ MASK_NONE, MASK_CAUSAL, MASK_WINDOW, MASK_CAUSAL_WINDOW = 0, 1, 2, 3
 NOALLOC_SCRATCH_BYTES = 32 << 20  # RK_NOALLOC_SCRATCH_BYTES
 DTYPE_F32, DTYPE_F16, DTYPE_BF16 = 0, 1, 2
 GLU_SILU, GLU_GELU = 1, 2
+ROUTE_SOFTMAX, ROUTE_SIGMOID = 0, 1
 
 # Every entry point of include/burn_rocket_amd.h with its ctypes signature.
 _c = ctypes
@@ -84,6 +85,11 @@ SIGNATURES = {
     "rk_attention_paged_dev": (_i, [_p, _p, _i64, _p, _p, _f, _f, _p, _i64, _i, _p]),
     "rk_paged_append_dev": (_i, [_p, _p, _i64, _p, _p, _c.c_double, _p, _p, _i, _i64, _p, _i64, _p, _p, _i, _p]),
     "rk_moe_route": (_i, [_p, _i64, _i, _i, _i, _p, _p]),
+    "rk_moe_route_dev": (_i, [_p, _i, _i64, _i, _i, _i, _p, _i, _i, _i, _f, _p, _p, _p]),
+    "rk_moe_routed_plan_create": (_i, [_u64, _i64, _i, _p]),
+    "rk_moe_plan_route_dev": (_i, [_p, _i64, _p, _p, _p]),
+    "rk_pack_moe_fp8": (_i, [_p, _p, _p, _p, _p, _p, _i, _i64, _i64, _p]),
+    "rk_moe_experts_fp8_dev": (_i, [_u64, _p, _p, _p, _i, _i, _p]),
     "rk_pack_moe_q8_0": (_i, [_p, _p, _p, _i, _i64, _i64, _p]),
     "rk_pack_moe_f32": (_i, [_p, _p, _p, _i, _i64, _i64, _p]),
     "rk_moe_experts_dev": (_i, [_u64, _p, _i64, _i, _p, _p, _p, _p]),
@@ -989,6 +995,90 @@ class I8Context:
 
     def clear_scratch(self):
         clear_scratch()
+
+
+def route_experts(logits, top_k, score=ROUTE_SOFTMAX, bias=None, n_groups=1, top_groups=1, norm_topk=True, scale=1.0,
+                  bf16=False):
+    """The router on the GPU (rk_moe_route_dev): softmax or sigmoid scores, chosen with an optional bias among the
+    experts of the top_groups best groups. logits [s, E] f32, float16 or bf16 bits; ids u32 [s, k], weights f32 [s, k]."""
+    logits = np.ascontiguousarray(logits)
+    dt = _float_dtype(logits, bf16, "route_experts")
+    s, e = logits.shape
+    if bias is not None and np.shape(bias) != (e,):
+        _shape_error("route_experts", "bias must be [n_experts]")
+    ids, wts = np.empty((s, top_k), np.uint32), np.empty((s, top_k), np.float32)
+    bufs = [DeviceBuffer.from_array(logits), DeviceBuffer(ids.nbytes), DeviceBuffer(wts.nbytes)]
+    if bias is not None:
+        bufs.append(DeviceBuffer.from_array(_f32(bias)))
+    _check(_lib.rk_moe_route_dev(bufs[0].ptr, dt, s, e, top_k, score, bufs[3].ptr if bias is not None else None, n_groups,
+                                 top_groups, int(norm_topk), float(scale), bufs[1].ptr, bufs[2].ptr, None), "route_experts")
+    synchronize()
+    return bufs[1].download(ids.shape, ids.dtype), bufs[2].download(wts.shape, wts.dtype)
+
+
+def pack_moe_fp8(gate, gate_scales, up, up_scales, down, down_scales):
+    """Expert stack of block-scaled fp8: codes gate and up [E, I, H], down [E, H, I] (bytes), scales
+    [E, ceil(rows/128), ceil(K/128)]."""
+    g, u, d = (np.ascontiguousarray(a, dtype=np.uint8) for a in (gate, up, down))
+    gs, us, ds = (_f32(a) for a in (gate_scales, up_scales, down_scales))
+    E, I, H = g.shape
+    if u.shape != (E, I, H) or d.shape != (E, H, I):
+        _shape_error("pack_moe_fp8", "gate and up [E, I, H], down [E, H, I]")
+    if gs.shape != (E, _blocks(I), _blocks(H)) or us.shape != gs.shape or ds.shape != (E, _blocks(H), _blocks(I)):
+        _shape_error("pack_moe_fp8", "scales [E, ceil(rows/128), ceil(K/128)]")
+    out = ctypes.c_uint64()
+    _check(load_library().rk_pack_moe_fp8(_ptr(g), _ptr(gs), _ptr(u), _ptr(us), _ptr(d), _ptr(ds), E, H, I, ctypes.byref(out)),
+           "pack_moe_fp8")
+    return WeightId(out.value)
+
+
+class RoutedPlan:
+    """A plan of rk_moe_routed_plan_create (`ptr`): the lists of a batch of routed tokens, built on the GPU, and what the
+    experts' calls work in. Freed with the object, or by `destroy`."""
+
+    def __init__(self, ptr, wid, max_s, top_k):
+        self.ptr, self.wid, self.max_s, self.top_k = ptr, wid, max_s, top_k
+
+    def route(self, s, ids, wts, stream=None):
+        """The next batch: ids u32 and wts f32 [s, top_k] on the device; ordered on `stream`."""
+        _check(_lib.rk_moe_plan_route_dev(self.ptr, s, ids, wts, ctypes.c_void_p(stream) if stream else None), "moe_plan_route")
+
+    def destroy(self):
+        if self.ptr:
+            _check(_lib.rk_moe_plan_destroy(self.ptr), "moe_plan_destroy")
+            self.ptr = None
+
+    def __del__(self):
+        try:
+            if self.ptr and _lib is not None:
+                _lib.rk_moe_plan_destroy(self.ptr)
+        except Exception:
+            pass
+
+
+def routed_plan(wid, max_s, top_k):
+    """A routed plan of an expert stack with room for batches of up to max_s tokens."""
+    out = ctypes.c_void_p()
+    _check(load_library().rk_moe_routed_plan_create(int(wid), max_s, top_k, ctypes.byref(out)), "routed_plan")
+    return RoutedPlan(out.value, wid, max_s, top_k)
+
+
+def moe_layer(x, logits, wid, top_k, bf16=False, **router):
+    """A routed layer of fp8 experts on host arrays: x [s, H] by the experts that `route_experts` (its arguments in
+    `router`) chooses from logits [s, E] f32; returned in x's type."""
+    x, logits = np.ascontiguousarray(x), _f32(logits)
+    dt = _float_dtype(x, bf16, "moe_layer")
+    ids, wts = route_experts(logits, top_k, **router)
+    if len(x) == 0:
+        return x.copy()
+    plan = routed_plan(wid, len(x), top_k)
+    try:
+        def call(p, o):
+            plan.route(len(x), p[1], p[2])
+            return int(wid), plan.ptr, p[0], o, dt, 0, None
+        return _run_dev("rk_moe_experts_fp8_dev", "moe_layer", x, [x, ids, wts], call)
+    finally:
+        plan.destroy()
 
 
 # ------------------------------------------------------------- device buffers

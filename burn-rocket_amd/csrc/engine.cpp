@@ -99,6 +99,7 @@ struct Weight {
   size_t bytes = 0;
   // MoE expert stack (kind 0, moe = true)
   bool moe = false;
+  bool moe_fp8 = false;  // gu/dn_codes and scales in the fp8 layouts, strides in blocks of 128
   int n_experts = 0;
   int64_t hidden = 0, inter = 0;
   int8_t *gu_codes = nullptr, *dn_codes = nullptr;
@@ -137,6 +138,41 @@ struct SeqPlan {
   int64_t captured_toks = INT64_MAX;  // tokens that every captured call's buffers have room for
 };
 
+// Device-resident routing lists of one MoE call.
+struct MoePlan {
+  int64_t s = 0;
+  int top_k = 0;
+  int64_t rows = 0;
+  int n_tiles = 0;
+  int tile_rows = 128;        // rows per tile at most (the kernels' tile size)
+  int max_rows = 128;         // rows of the longest tile
+  int32_t *tok = nullptr;     // [rows] token of each bucket row
+  float *roww = nullptr;      // [rows] router weight of each bucket row
+  int32_t *slot = nullptr;    // [s, top_k] bucket rows of a token, ascending expert id
+  MoeTile *tiles = nullptr;   // [n_tiles] in expert order (down)
+  MoeTile *tiles_gu = nullptr;  // [n_tiles] the same tiles, longest first (gate|up)
+  void *block = nullptr;      // the lists' allocation, when the plan owns it
+  uint64_t weight = 0;        // expert stack the plan was made for
+  // Streams of the runs that read the lists: a library stream is
+  // synchronized when the plan is destroyed; a caller's stream gets an event
+  // recorded after each run there.
+  mutable std::vector<std::pair<hipStream_t, hipEvent_t>> uses;
+
+  // A plan whose lists are built on the GPU (rk_moe_routed_plan_create): one allocation holds the lists and
+  // everything its calls work in, fenced like a plan of sequences. s, rows, n_tiles, tile_rows and max_rows are
+  // those of the last batch; the offsets are for max_s tokens.
+  bool routed = false;
+  int64_t max_s = 0;
+  bool has_batch = false;       // rk_moe_plan_route_dev has been called
+  bool route_captured = false;  // its last call was captured: the device may not hold that batch yet
+  bool captured = false;        // a graph holds calls on the plan, of batches of s tokens
+  DevBuf mem;
+  int32_t *counts = nullptr, *n_valid = nullptr;
+  std::unordered_map<std::string, size_t> work;  // offsets of the calls' buffers, by the names of library scratch
+};
+
+
+
 struct Engine {
   int device = 0;
   hipStream_t stream = nullptr;
@@ -155,6 +191,7 @@ struct Engine {
   size_t moe_pin_bytes = 0;
   uint64_t epoch = 0;        // rk_trim_scratch: scratch not used since the last trim goes
   std::unordered_set<SeqPlan *> seq_plans;
+  std::unordered_set<MoePlan *> routed_plans;  // live plans of rk_moe_routed_plan_create
 };
 
 std::mutex g_mu;
@@ -279,6 +316,49 @@ int is_capturing(hipStream_t st, bool *yes, const char *op) {
   hipStreamCaptureStatus s = hipStreamCaptureStatusNone;
   HIP_TRY(hipStreamIsCapturing(st, &s), op);
   *yes = s != hipStreamCaptureStatusNone;
+  return RK_OK;
+}
+
+void seq_buf_free(DevBuf &b) {
+  if (b.p) (void)hipFree(b.p);
+  if (b.ev) (void)hipEventDestroy(b.ev);
+  b = DevBuf{};
+}
+
+// Refuses what has to wait for a plan's last call while that call's stream is captured: an
+// event recorded there now would belong to the graph, and a stream that waits for it to the
+// capture. (Calls on `st` itself wait for nothing.)
+int buf_fenceable(const DevBuf &b, hipStream_t st, const char *op) {
+  bool capturing = false;
+  if (b.pending && b.ev_stream != st) RK_TRY(is_capturing(b.ev_stream, &capturing, op));
+  if (capturing) return fail(RK_E_UNSUPPORTED, op, "the stream of the plan's last call is being captured");
+  return RK_OK;
+}
+int seq_fenceable(const SeqPlan &p, hipStream_t st, const char *op) {
+  RK_TRY(buf_fenceable(p.block, st, op));
+  return buf_fenceable(p.work, st, op);
+}
+
+// The end of a buffer's last use, awaited by the host.
+int seq_buf_wait(DevBuf &b, const char *op) {
+  if (!b.ev) return RK_OK;
+  RK_TRY(fence_point(b, op));
+  if (b.recorded) HIP_TRY(hipEventSynchronize(b.ev), op);
+  b.recorded = false;
+  return RK_OK;
+}
+
+// A plan's buffer in a call: ordered after its last use on another stream, as
+// scratch is. In a capture nothing is awaited or recorded: the order between a
+// graph's replays and other uses of its plan is the caller's.
+int seq_buf_use(CallScope &cs, DevBuf &b, bool capturing, const char *op) {
+  if (capturing || !b.p) return RK_OK;
+  if (!b.ev) HIP_TRY(hipEventCreateWithFlags(&b.ev, hipEventDisableTiming), op);
+  if ((b.recorded || b.pending) && b.ev_stream != cs.st) {
+    RK_TRY(fence_point(b, op));
+    HIP_TRY(hipStreamWaitEvent(cs.st, b.ev, 0), op);
+  }
+  cs.used.push_back(&b);
   return RK_OK;
 }
 
@@ -430,6 +510,7 @@ extern "C" int rk_mem_stats(rk_mem_stats_t *out) {
       out->attention_bytes += kv.second.bytes;
   }
   out->host_bytes = g_eng->stage.pinned_bytes() + g_eng->moe_pin_bytes;
+  for (const MoePlan *p : g_eng->routed_plans) out->scratch_bytes += p->mem.bytes;
   for (const SeqPlan *p : g_eng->seq_plans) {
     const uint64_t held = (p->block.p ? p->block.bytes : 0) + (p->work.p ? p->work.bytes : 0);
     out->scratch_bytes += held;
@@ -1801,6 +1882,9 @@ namespace {
 // multiple of 4, q8_code_offset in kernels.hpp).
 int64_t moe_gu_code_stride(const Weight &w) { return 2 * w.inter * w.gu_ws_stride * 32; }
 int64_t moe_dn_code_stride(const Weight &w) { return w.hidden * w.dn_ws_stride * 32; }
+// fp8 stacks: rows and K padded to 128.
+int64_t moe_fp8_gu_bytes(const Weight &w) { return 2 * round_up_i(w.inter, 128) * w.gu_ws_stride * 128; }
+int64_t moe_fp8_dn_bytes(const Weight &w) { return round_up_i(w.hidden, 128) * w.dn_ws_stride * 128; }
 
 }  // namespace
 
@@ -1908,27 +1992,6 @@ extern "C" int rk_pack_moe_f32(const float *gate, const float *up, const float *
 }
 
 namespace {
-// Device-resident routing lists of one MoE call.
-struct MoePlan {
-  int64_t s = 0;
-  int top_k = 0;
-  int64_t rows = 0;
-  int n_tiles = 0;
-  int tile_rows = 128;        // rows per tile at most (the kernels' tile size)
-  int max_rows = 128;         // rows of the longest tile
-  int32_t *tok = nullptr;     // [rows] token of each bucket row
-  float *roww = nullptr;      // [rows] router weight of each bucket row
-  int32_t *slot = nullptr;    // [s, top_k] bucket rows of a token, ascending expert id
-  MoeTile *tiles = nullptr;   // [n_tiles] in expert order (down)
-  MoeTile *tiles_gu = nullptr;  // [n_tiles] the same tiles, longest first (gate|up)
-  void *block = nullptr;      // the lists' allocation, when the plan owns it
-  uint64_t weight = 0;        // expert stack the plan was made for
-  // Streams of the runs that read the lists: a library stream is
-  // synchronized when the plan is destroyed; a caller's stream gets an event
-  // recorded after each run there.
-  mutable std::vector<std::pair<hipStream_t, hipEvent_t>> uses;
-};
-
 void plan_free(MoePlan *p) {
   if (!p) return;
   for (auto &u : p->uses)
@@ -1947,6 +2010,11 @@ struct MoeLists {
   size_t roww = 0, tiles = 0, tiles_gu = 0, slot = 0, bytes = 0;
 };
 
+// Rows of a tile of fp8 experts.
+int moe_fp8_tile_rows(const Weight &w, int64_t rows) {
+  return std::min(rk_fp8_few_rows(w.gu_ws_stride), rk_fp8_few_rows(w.dn_ws_stride));
+}
+
 // Checks the ids and sizes the lists: tiles of ≤ rk_moe_tile_rows() rows (two
 // tiles of one expert sit next to each other, so the second read of its
 // weights is mostly served from cache).
@@ -1955,7 +2023,7 @@ int moe_lists(const Weight &w, int64_t s, int top_k, const uint32_t *ids, MoeLis
   l->s = s;
   l->top_k = top_k;
   l->rows = s * top_k;
-  l->tile_rows = rk_moe_tile_rows();
+  l->tile_rows = w.moe_fp8 ? moe_fp8_tile_rows(w, l->rows) : rk_moe_tile_rows();
   l->off.assign(E + 1, 0);
   for (int64_t i = 0; i < l->rows; ++i) {
     if (ids[i] >= (uint32_t)E) return fail(RK_E_SHAPE, "rk_moe_plan", "expert id out of range");
@@ -2001,9 +2069,10 @@ void moe_fill_rows(const MoeLists &l, const uint32_t *ids, const float *wts, uin
   for (int e = 0; e + 1 < (int)l.off.size(); ++e)
     for (int64_t r = l.off[e]; r < l.off[e + 1]; r += l.tile_rows)
       tiles[n++] = MoeTile{e, (int)r, (int)std::min<int64_t>(l.tile_rows, l.off[e + 1] - r)};
-  for (int blocks = l.tile_rows / 32, m = 0; blocks >= 1; --blocks)
+  const int unit = l.tile_rows >= 64 ? 32 : std::max(l.tile_rows / 4, 1);
+  for (int blocks = l.tile_rows / unit, m = 0; blocks >= 1; --blocks)
     for (int i = 0; i < n; ++i)
-      if ((tiles[i].rows + 31) / 32 == blocks) gu[m++] = tiles[i];
+      if ((tiles[i].rows + unit - 1) / unit == blocks) gu[m++] = tiles[i];
 }
 
 // Each token's bucket rows for the combine. Rows of one expert are contiguous
@@ -2047,30 +2116,103 @@ int moe_plan(const Weight &w, int64_t s, int top_k, const uint32_t *ids, const f
   return RK_OK;
 }
 
+// A buffer of a call: the plan's own where its lists are built on the GPU, library scratch otherwise.
+int moe_buf(CallScope &cs, const MoePlan &plan, const char *name, size_t bytes, void **out, bool *fresh = nullptr) {
+  if (fresh) *fresh = false;
+  if (!plan.routed) return scratch(cs, name, bytes, out, fresh);
+  *out = (uint8_t *)plan.mem.p + plan.work.at(name);
+  return RK_OK;
+}
+
+// The buffers of a call on s tokens (`rows` pairs), and their bytes: what moe_run and moe_run_fp8 ask for.
+std::vector<std::pair<const char *, size_t>> moe_buffers(const Weight &w, int64_t s, int64_t rows) {
+  const size_t S = (size_t)s, R = (size_t)rows, H = (size_t)w.hidden, I = (size_t)w.inter;
+  if (w.moe_fp8) return {{"moe_act", R * I * 4}, {"moe_yb", R * H * 4}};
+  return {{"moe_xq", S * H},       {"moe_xs", S * (H / 32) * 4}, {"moe_act", R * I * 4}, {"moe_aq", R * I},
+          {"moe_as", R * (I / 32) * 4}, {"moe_yb", R * H * 4},        {"moe_cnt", S * ((H + 127) / 128) * 4}};
+}
+
+// fp8 experts. Tiles of few rows: each workgroup quantizes the rows it multiplies; silu(gate)·up goes to the second product
+// in f32. fp16 results: the first product has f32 sums, since a code of its results that flips is worth more than an fp16
+// rounding; f32 results: both have.
+int moe_run_fp8(CallScope &cs, const Weight &w, const MoePlan &plan, const void *x, void *y, int dtype, bool accumulate,
+                const std::function<int(int)> &lists = nullptr) {
+  const char *op = "rk_moe_experts_fp8_dev";
+  const int64_t H = w.hidden, I = w.inter, R = plan.rows;
+  hipStream_t st = cs.st;
+  void *act, *yb;
+  RK_TRY(moe_buf(cs, plan, "moe_act", (size_t)R * I * 4, &act));
+  RK_TRY(moe_buf(cs, plan, "moe_yb", (size_t)R * H * 4, &yb));
+  if (lists) {
+    RK_TRY(lists(0));
+    RK_TRY(lists(1));
+  }
+  Fp8FewArgs g{};
+  g.x = x;
+  g.n = (int)I;
+  g.k = (int)H;
+  g.kt = w.gu_ws_stride;
+  g.w = (const uint8_t *)w.gu_codes;
+  g.ws = w.gu_scales;
+  g.w_stride = moe_fp8_gu_bytes(w);
+  g.up_scales = (I + 127) / 128 * w.gu_ws_stride;
+  g.ws_stride = 2 * g.up_scales;
+  g.c = act;
+  g.c_dtype = RK_DTYPE_F32;
+  g.tiles = plan.tiles_gu;
+  g.n_tok = (int)plan.s;
+  g.tok = plan.tok;
+  HIP_TRY(rk_launch_fp8_few_gate_up(g, dtype, plan.tile_rows, plan.n_tiles, dtype != RK_DTYPE_BF16, st), op);
+  g.x = act;
+  g.n = (int)H;
+  g.k = (int)I;
+  g.kt = w.dn_ws_stride;
+  g.w = (const uint8_t *)w.dn_codes;
+  g.ws = w.dn_scales;
+  g.w_stride = moe_fp8_dn_bytes(w);
+  g.ws_stride = (H + 127) / 128 * w.dn_ws_stride;
+  g.c = yb;
+  g.tiles = plan.tiles;
+  g.row_w = plan.roww;
+  HIP_TRY(rk_launch_fp8_few_down(g, plan.tile_rows, plan.n_tiles, dtype == RK_DTYPE_F32, st), op);
+  CombineArgs c{};
+  c.rows = (const float *)yb;
+  c.slot = plan.slot;
+  c.n_valid = plan.n_valid;
+  c.y = y;
+  c.s = plan.s;
+  c.n = (int)H;
+  c.top_k = plan.top_k;
+  c.accumulate = accumulate;
+  HIP_TRY(rk_launch_moe_combine(c, dtype, st), op);
+  return RK_OK;
+}
+
 // lists (when given) enqueues the plan's lists: called with 0 before the launch
 // that reads all but `slot`, with 1 before the one that reads `slot`.
 int moe_run(CallScope &cs, const Weight &w, const MoePlan &plan, const float *x, float *y,
             float *act_out = nullptr, bool accumulate = false,
             const std::function<int(int)> &lists = nullptr) {
+  if (w.moe_fp8) return moe_run_fp8(cs, w, plan, x, y, RK_DTYPE_F32, accumulate, lists);
   hipStream_t st = cs.st;
   const int64_t H = w.hidden, I = w.inter, S = plan.s, R = std::max<int64_t>(plan.rows, 1);
   const int64_t KBh = H / 32, KBi = I / 32;  // 32-value activation groups per row
+  const char *op = "rk_moe_experts_dev";
   void *xq, *xs, *act, *aq, *as, *yb, *cnt;
-  RK_TRY(scratch(cs, "moe_xq", (size_t)S * H, &xq));
-  RK_TRY(scratch(cs, "moe_xs", (size_t)S * KBh * 4, &xs));
+  RK_TRY(moe_buf(cs, plan, "moe_xq", (size_t)S * H, &xq));
+  RK_TRY(moe_buf(cs, plan, "moe_xs", (size_t)S * KBh * 4, &xs));
   if (act_out)
     act = act_out;
   else
-    RK_TRY(scratch(cs, "moe_act", (size_t)R * I * 4, &act));
-  RK_TRY(scratch(cs, "moe_aq", (size_t)R * I, &aq));
-  RK_TRY(scratch(cs, "moe_as", (size_t)R * KBi * 4, &as));
-  RK_TRY(scratch(cs, "moe_yb", (size_t)R * H * 4, &yb));
+    RK_TRY(moe_buf(cs, plan, "moe_act", (size_t)R * I * 4, &act));
+  RK_TRY(moe_buf(cs, plan, "moe_aq", (size_t)R * I, &aq));
+  RK_TRY(moe_buf(cs, plan, "moe_as", (size_t)R * KBi * 4, &as));
+  RK_TRY(moe_buf(cs, plan, "moe_yb", (size_t)R * H * 4, &yb));
   // One arrival counter per (token, 128-column slice) for the combine in the
   // down launch. Each launch leaves them at zero; a new buffer is zeroed once.
   const size_t cnt_bytes = (size_t)S * ((H + 127) / 128) * 4;
   bool fresh = false;
-  RK_TRY(scratch(cs, "moe_cnt", cnt_bytes, &cnt, &fresh));
-  const char *op = "rk_moe_experts_dev";
+  RK_TRY(moe_buf(cs, plan, "moe_cnt", cnt_bytes, &cnt, &fresh));
   if (fresh) HIP_TRY(hipMemsetAsync(cnt, 0, std::max<size_t>(cnt_bytes, 256), st), op);
   // x and the silu·up rows are quantized per row per 32-value group, as the
   // reference's expert workers do (engine.rs:1005-1006, 1034-1035).
@@ -2113,6 +2255,22 @@ int plan_mark_used(const MoePlan &p, hipStream_t st) {
   return RK_OK;
 }
 
+// A routed plan's memory in a call: ordered after its last use on another stream; in a capture nothing is awaited or
+// recorded, and every later batch has this one's tokens.
+int moe_use(CallScope &cs, MoePlan &p, bool reads_lists, const char *op) {
+  if (!p.routed) return RK_OK;
+  bool capturing;
+  RK_TRY(is_capturing(cs.st, &capturing, op));
+  if (capturing) {
+    p.captured = true;
+    return RK_OK;
+  }
+  if (reads_lists && p.route_captured)
+    return fail(RK_E_UNSUPPORTED, op, "the plan's last rk_moe_plan_route_dev was captured: call it outside a capture first");
+  RK_TRY(buf_fenceable(p.mem, cs.st, op));
+  return seq_buf_use(cs, p.mem, false, op);
+}
+
 int moe_check(uint64_t id, int64_t s, int top_k, Weight **w, const char *op) {
   *w = find(id);
   if (!*w || !(*w)->moe) return fail(RK_E_SHAPE, op, "id is not an expert stack");
@@ -2127,6 +2285,19 @@ int moe_check(uint64_t id, int64_t s, int top_k, Weight **w, const char *op) {
     return fail(RK_E_SHAPE, op, "s·top_k·hidden f32 values must stay below 2^31 bytes");
   return RK_OK;
 }
+
+// fp8 stacks read and write their rows in pieces of 16 bytes.
+int moe_aligned(const Weight &w, const void *x, const void *y, const char *op) {
+  if (w.moe_fp8 && (((uintptr_t)x | (uintptr_t)y) & 15)) return fail(RK_E_SHAPE, op, "x and y must be 16-byte aligned");
+  return RK_OK;
+}
+
+int moe_planned_check(uint64_t id, const MoePlan &p, Weight **w, const char *op) {
+  if (p.routed && !p.has_batch) return fail(RK_E_SHAPE, op, "the plan has no batch yet: rk_moe_plan_route_dev");
+  RK_TRY(moe_check(id, p.s, p.top_k, w, op));
+  if (p.weight != id) return fail(RK_E_SHAPE, op, "plan was made for another expert stack");
+  return RK_OK;
+}
 }  // namespace
 
 namespace {
@@ -2137,6 +2308,7 @@ int moe_experts(rk_weight_id id, const float *x, int64_t s, int top_k, const uin
   Weight *w;
   RK_TRY(moe_check(id, s, top_k, &w, op));
   if (!x || !y || !ids || !wts) return fail(RK_E_SHAPE, op, "null buffer");
+  RK_TRY(moe_aligned(*w, x, y, op));
   hipStream_t st = pick(stream);
   CallScope cs(st);
   // The lists go from page-locked memory to scratch, long ones in two copies, so
@@ -2186,13 +2358,15 @@ int moe_experts_planned(rk_weight_id id, const void *plan, const float *x, float
   RK_TRY(ensure(op));
   const MoePlan *p = (const MoePlan *)plan;
   if (!p) return fail(RK_E_SHAPE, op, "null plan");
+  if (p->routed && p->weight == id && p->has_batch && p->s == 0) return RK_OK;
   if (!x || !y) return fail(RK_E_SHAPE, op, "null buffer");
   Weight *w;
-  RK_TRY(moe_check(id, p->s, p->top_k, &w, op));
-  if (p->weight != id) return fail(RK_E_SHAPE, op, "plan was made for another expert stack");
+  RK_TRY(moe_planned_check(id, *p, &w, op));
+  RK_TRY(moe_aligned(*w, x, y, op));
   CallScope cs(pick(stream));
+  RK_TRY(moe_use(cs, *(MoePlan *)p, true, op));
   RK_TRY(moe_run(cs, *w, *p, x, y, nullptr, accumulate));
-  RK_TRY(plan_mark_used(*p, cs.st));
+  if (!p->routed) RK_TRY(plan_mark_used(*p, cs.st));
   g_eng->calls++;
   return RK_OK;
 }
@@ -2243,13 +2417,14 @@ extern "C" int rk_moe_gate_up_dev(rk_weight_id id, const void *plan, const float
   RK_TRY(ensure("rk_moe_gate_up_dev"));
   const MoePlan *p = (const MoePlan *)plan;
   if (!p || !act) return fail(RK_E_SHAPE, "rk_moe_gate_up_dev", "null plan or output");
+  if (p->routed && p->weight == id && p->has_batch && p->s == 0) return RK_OK;
   Weight *w;
-  RK_TRY(moe_check(id, p->s, p->top_k, &w, "rk_moe_gate_up_dev"));
-  if (p->weight != id)
-    return fail(RK_E_SHAPE, "rk_moe_gate_up_dev", "plan was made for another expert stack");
+  RK_TRY(moe_planned_check(id, *p, &w, "rk_moe_gate_up_dev"));
+  if (w->moe_fp8) return fail(RK_E_UNSUPPORTED, "rk_moe_gate_up_dev", "an fp8 expert stack");
   CallScope cs(pick(stream));
+  RK_TRY(moe_use(cs, *(MoePlan *)p, true, "rk_moe_gate_up_dev"));
   RK_TRY(moe_run(cs, *w, *p, x, nullptr, act));
-  RK_TRY(plan_mark_used(*p, cs.st));
+  if (!p->routed) RK_TRY(plan_mark_used(*p, cs.st));
   return RK_OK;
 }
 
@@ -2257,6 +2432,15 @@ extern "C" int rk_moe_plan_destroy(void *plan) {
   std::lock_guard<std::mutex> lk(g_mu);
   RK_TRY(ensure("rk_moe_plan_destroy"));
   MoePlan *p = (MoePlan *)plan;
+  if (p && g_eng->routed_plans.count(p)) {
+    RK_TRY(buf_fenceable(p->mem, nullptr, "rk_moe_plan_destroy"));
+    if (p->captured) HIP_TRY(hipDeviceSynchronize(), "rk_moe_plan_destroy");  // replays are known to the device alone
+    RK_TRY(seq_buf_wait(p->mem, "rk_moe_plan_destroy"));
+    seq_buf_free(p->mem);
+    g_eng->routed_plans.erase(p);
+    plan_free(p);
+    return RK_OK;
+  }
   // Runs on any stream that read the plan's lists must have finished (a
   // library stream destroyed since was synchronized then).
   if (p)
@@ -2518,47 +2702,6 @@ extern "C" int rk_attention_qkv_dev(void *qkv, int64_t s, int64_t row_stride, in
 // =========================================================================
 namespace {
 size_t align16(size_t b) { return (b + 15) / 16 * 16; }
-
-void seq_buf_free(DevBuf &b) {
-  if (b.p) (void)hipFree(b.p);
-  if (b.ev) (void)hipEventDestroy(b.ev);
-  b = DevBuf{};
-}
-
-// Refuses what has to wait for a plan's last call while that call's stream is captured: an
-// event recorded there now would belong to the graph, and a stream that waits for it to the
-// capture. (Calls on `st` itself wait for nothing.)
-int seq_fenceable(const SeqPlan &p, hipStream_t st, const char *op) {
-  for (const DevBuf *b : {&p.block, &p.work}) {
-    bool capturing = false;
-    if (b->pending && b->ev_stream != st) RK_TRY(is_capturing(b->ev_stream, &capturing, op));
-    if (capturing) return fail(RK_E_UNSUPPORTED, op, "the stream of the plan's last call is being captured");
-  }
-  return RK_OK;
-}
-
-// The end of a buffer's last use, awaited by the host.
-int seq_buf_wait(DevBuf &b, const char *op) {
-  if (!b.ev) return RK_OK;
-  RK_TRY(fence_point(b, op));
-  if (b.recorded) HIP_TRY(hipEventSynchronize(b.ev), op);
-  b.recorded = false;
-  return RK_OK;
-}
-
-// A plan's buffer in a call: ordered after its last use on another stream, as
-// scratch is. In a capture nothing is awaited or recorded: the order between a
-// graph's replays and other uses of its plan is the caller's.
-int seq_buf_use(CallScope &cs, DevBuf &b, bool capturing, const char *op) {
-  if (capturing || !b.p) return RK_OK;
-  if (!b.ev) HIP_TRY(hipEventCreateWithFlags(&b.ev, hipEventDisableTiming), op);
-  if ((b.recorded || b.pending) && b.ev_stream != cs.st) {
-    RK_TRY(fence_point(b, op));
-    HIP_TRY(hipStreamWaitEvent(cs.st, b.ev, 0), op);
-  }
-  cs.used.push_back(&b);
-  return RK_OK;
-}
 
 SeqPlan::Room seq_room(const SeqLists &l) {
   SeqPlan::Room r;
@@ -3153,6 +3296,236 @@ extern "C" int rk_matmul_fp8_dev(rk_weight_id id, const void *x, int x_dtype, in
 }
 
 // =========================================================================
+// MoE layers routed on the GPU
+// =========================================================================
+extern "C" int rk_moe_route_dev(const void *logits, int dtype, int64_t s, int n_experts, int top_k, int score,
+                                const float *bias, int n_groups, int top_groups, int norm_topk, float scale, uint32_t *ids,
+                                float *wts, rk_stream stream) {
+  std::lock_guard<std::mutex> lk(g_mu);
+  const char *op = "rk_moe_route_dev";
+  RK_TRY(ensure(op));
+  if (s < 0 || s > INT32_MAX || n_experts <= 0 || top_k <= 0) return fail(RK_E_SHAPE, op, "need 0 <= s < 2^31, n_experts > 0, top_k > 0");
+  if (dtype < RK_DTYPE_F32 || dtype > RK_DTYPE_BF16) return fail(RK_E_SHAPE, op, "unknown dtype");
+  if (score != RK_ROUTE_SOFTMAX && score != RK_ROUTE_SIGMOID) return fail(RK_E_SHAPE, op, "unknown score");
+  if (n_groups <= 0 || n_experts % n_groups != 0 || top_groups <= 0 || top_groups > n_groups)
+    return fail(RK_E_SHAPE, op, "n_groups must divide n_experts, and top_groups be in [1, n_groups]");
+  if (top_k > n_experts / n_groups * top_groups) return fail(RK_E_SHAPE, op, "top_k above the experts of the chosen groups");
+  if (n_experts > RK_ROUTE_MAX_EXPERTS || top_k > RK_ROUTE_MAX_TOP || n_groups > RK_ROUTE_MAX_GROUPS)
+    return fail(RK_E_UNSUPPORTED, op, "up to 1024 experts, 64 choices and 64 groups");
+  if (s == 0) return RK_OK;
+  if (!logits || !ids || !wts) return fail(RK_E_SHAPE, op, "null buffer");
+  RouteArgs g{logits, dtype, s, n_experts, top_k, score, bias, n_groups, top_groups, norm_topk != 0, scale, ids, wts};
+  HIP_TRY(rk_launch_moe_route(g, pick(stream)), op);
+  return RK_OK;
+}
+
+namespace {
+constexpr int64_t kMaxRoutedRows = (int64_t)1 << 20;
+
+// Rows of a tile for a batch whose lists the host does not see. Q8_0 stacks: the kernel of few rows while an expert has few
+// on average, or has few at all; longer lists are more tiles of it.
+int routed_tile_rows(const Weight &w, int64_t s, int64_t rows) {
+  if (w.moe_fp8) return moe_fp8_tile_rows(w, rows);
+  if (rk_knob("RK_MOE_ROWS", 0) != 0) return rk_moe_tile_rows();
+  if (s <= 8) return 8;
+  if (s <= 16) return 16;
+  return rows <= 24 * (int64_t)w.n_experts ? 32 : 128;
+}
+// Tiles that `rows` pairs make at most: each bucket (an expert's, or that of no expert) ends with one that is not whole.
+int64_t routed_tiles(const Weight &w, int64_t rows, int tile_rows) {
+  return std::min<int64_t>(rows, w.n_experts + 1 + rows / tile_rows);
+}
+}  // namespace
+
+extern "C" int rk_moe_routed_plan_create(rk_weight_id id, int64_t max_s, int top_k, void **plan) {
+  const char *op = "rk_moe_routed_plan_create";
+  return no_throw(op, [&]() -> int {
+    std::lock_guard<std::mutex> lk(g_mu);
+    RK_TRY(ensure(op));
+    if (!plan) return fail(RK_E_SHAPE, op, "null output");
+    *plan = nullptr;
+    Weight *w;
+    RK_TRY(moe_check(id, max_s, top_k, &w, op));
+    if (w->n_experts > RK_ROUTE_MAX_EXPERTS) return fail(RK_E_UNSUPPORTED, op, "up to 1024 experts");
+    if (max_s > kMaxRoutedRows / top_k) return fail(RK_E_SHAPE, op, "max_s·top_k above 2^20");
+    const int64_t rows = max_s * top_k;
+    if (rows / routed_tile_rows(*w, max_s, rows) > 32768) return fail(RK_E_SHAPE, op, "more than 2^15 tiles");
+    size_t bytes = 0;
+    const auto take = [&](size_t n) {
+      const size_t at = bytes;
+      bytes += (n + 255) / 256 * 256;
+      return at;
+    };
+    const size_t tok = take(rows * 4), roww = take(rows * 4), slot = take(rows * 4), tiles = take(rows * sizeof(MoeTile)),
+                 tiles_gu = take(rows * sizeof(MoeTile)), valid = take(4),
+                 counts = take((size_t)rk_moe_lists_blocks(rows) * (w->n_experts + 1) * 4);
+    const size_t lists = bytes;
+    MoePlan *p = new MoePlan();
+    size_t cnt_at = 0, cnt_bytes = 0;
+    int rc = no_throw(op, [&]() -> int {
+      for (const auto &b : moe_buffers(*w, max_s, rows)) {
+        p->work[b.first] = take(b.second);
+        if (std::string(b.first) == "moe_cnt") {
+          cnt_at = p->work[b.first];
+          cnt_bytes = b.second;
+        }
+      }
+      HIP_TRY(hipMalloc(&p->mem.p, bytes), op);
+      p->mem.bytes = bytes;
+      // Lists of zeros name row 0 of token 0: what a call before their first building would read stays in bounds.
+      HIP_TRY(hipMemset(p->mem.p, 0, lists), op);
+      if (cnt_bytes) HIP_TRY(hipMemset((uint8_t *)p->mem.p + cnt_at, 0, cnt_bytes), op);
+      HIP_TRY(hipDeviceSynchronize(), op);
+      g_eng->routed_plans.insert(p);
+      return RK_OK;
+    });
+    if (rc != RK_OK) {
+      seq_buf_free(p->mem);
+      delete p;
+      return rc;
+    }
+    uint8_t *m = (uint8_t *)p->mem.p;
+    p->routed = true;
+    p->weight = id;
+    p->max_s = max_s;
+    p->top_k = top_k;
+    p->tok = (int32_t *)(m + tok);
+    p->roww = (float *)(m + roww);
+    p->slot = (int32_t *)(m + slot);
+    p->tiles = (MoeTile *)(m + tiles);
+    p->tiles_gu = (MoeTile *)(m + tiles_gu);
+    p->n_valid = (int32_t *)(m + valid);
+    p->counts = (int32_t *)(m + counts);
+    *plan = p;
+    return RK_OK;
+  });
+}
+
+extern "C" int rk_moe_plan_route_dev(void *plan, int64_t s, const uint32_t *ids, const float *wts, rk_stream stream) {
+  const char *op = "rk_moe_plan_route_dev";
+  return no_throw(op, [&]() -> int {
+    std::lock_guard<std::mutex> lk(g_mu);
+    RK_TRY(ensure(op));
+    MoePlan *p = (MoePlan *)plan;
+    if (!p || !g_eng->routed_plans.count(p)) return fail(RK_E_SHAPE, op, "not a plan of rk_moe_routed_plan_create");
+    if (s < 0 || s > p->max_s) return fail(RK_E_SHAPE, op, "the plan has room for " + std::to_string(p->max_s) + " tokens");
+    if (p->captured && s != p->s)
+      return fail(RK_E_SHAPE, op, "a graph holds this plan: its batches have " + std::to_string(p->s) + " tokens");
+    if (s > 0 && (!ids || !wts)) return fail(RK_E_SHAPE, op, "null buffer");
+    Weight *w = find(p->weight);
+    hipStream_t st = pick(stream);
+    bool capturing;
+    RK_TRY(is_capturing(st, &capturing, op));
+    CallScope cs(st);
+    RK_TRY(moe_use(cs, *p, false, op));
+    p->s = s;
+    p->has_batch = true;
+    p->route_captured = capturing;
+    p->rows = s * p->top_k;
+    if (s == 0) return RK_OK;
+    const int T = routed_tile_rows(*w, s, p->rows);
+    p->tile_rows = T;
+    p->max_rows = (int)std::min<int64_t>(T, p->rows);
+    p->n_tiles = (int)routed_tiles(*w, p->rows, T);
+    if (!w->moe_fp8 && T < 64) p->tile_rows = 128;  // (what the launches of the other kernels take; max_rows decides)
+    RouteListArgs g{};
+    g.ids = ids;
+    g.wts = wts;
+    g.rows = p->rows;
+    g.top_k = p->top_k;
+    g.n_experts = w->n_experts;
+    g.tile_rows = T;
+    g.max_tiles = p->n_tiles;
+    g.counts = p->counts;
+    g.n_valid = p->n_valid;
+    g.tok = p->tok;
+    g.row_w = p->roww;
+    g.slot = p->slot;
+    g.tiles = p->tiles;
+    g.tiles_gu = p->tiles_gu;
+    HIP_TRY(rk_launch_moe_lists(g, st), op);
+    return RK_OK;
+  });
+}
+
+extern "C" int rk_pack_moe_fp8(const uint8_t *gate, const float *gate_scales, const uint8_t *up, const float *up_scales,
+                               const uint8_t *down, const float *down_scales, int n_experts, int64_t hidden, int64_t inter,
+                               rk_weight_id *id) {
+  std::lock_guard<std::mutex> lk(g_mu);
+  const char *op = "rk_pack_moe_fp8";
+  RK_TRY(ensure(op));
+  if (n_experts <= 0 || hidden <= 0 || inter <= 0 || hidden % 16 || inter % 16 || hidden > 65536 || inter > 65536)
+    return fail(RK_E_SHAPE, op, "hidden and inter must be multiples of 16 up to 65536");
+  for (const void *b : {(const void *)gate, (const void *)gate_scales, (const void *)up, (const void *)up_scales,
+                        (const void *)down, (const void *)down_scales, (const void *)id})
+    if (!b) return fail(RK_E_SHAPE, op, "null buffer");
+  const int64_t E = n_experts, H = hidden, I = inter, Hb = (H + 127) / 128, Ib = (I + 127) / 128;
+  Weight w;
+  PackGuard guard(w);
+  w.moe = w.moe_fp8 = true;
+  w.n_experts = n_experts;
+  w.hidden = H;
+  w.inter = I;
+  w.n = H;
+  w.k = H;
+  w.group = 128;
+  w.gu_ws_stride = (int)Hb;
+  w.dn_ws_stride = (int)Ib;
+  const int64_t gu = moe_fp8_gu_bytes(w), dn = moe_fp8_dn_bytes(w), sc = Ib * Hb;
+  HIP_TRY(hipMalloc((void **)&w.gu_codes, (size_t)(E * gu)), op);
+  HIP_TRY(hipMalloc((void **)&w.dn_codes, (size_t)(E * dn)), op);
+  HIP_TRY(hipMalloc((void **)&w.gu_scales, (size_t)(E * 2 * sc) * 4), op);
+  HIP_TRY(hipMalloc((void **)&w.dn_scales, (size_t)(E * sc) * 4), op);
+  w.bytes = (size_t)(E * (gu + dn) + 3 * E * sc * 4);
+  CallScope cs(g_eng->stream);
+  hipStream_t st = cs.st;
+  HIP_TRY(hipMemsetAsync(w.gu_codes, 0, (size_t)(E * gu), st), op);  // the padding
+  HIP_TRY(hipMemsetAsync(w.dn_codes, 0, (size_t)(E * dn), st), op);
+  // An expert at a time: its three matrices up, then into their layouts (gate and up rows in turns of 32).
+  const size_t one = (size_t)(H * I);
+  uint8_t *dev;
+  RK_TRY(scratch(cs, "pack_blk", 3 * one, (void **)&dev));
+  for (int64_t e = 0; e < E; ++e) {
+    HIP_TRY(hipMemcpyAsync(dev, gate + e * one, one, hipMemcpyHostToDevice, st), op);
+    HIP_TRY(hipMemcpyAsync(dev + one, up + e * one, one, hipMemcpyHostToDevice, st), op);
+    HIP_TRY(hipMemcpyAsync(dev + 2 * one, down + e * one, one, hipMemcpyHostToDevice, st), op);
+    HIP_TRY(rk_launch_fp8_layout(dev, I, (int)H, 64, 0, (uint8_t *)w.gu_codes + e * gu, st), op);
+    HIP_TRY(rk_launch_fp8_layout(dev + one, I, (int)H, 64, 32, (uint8_t *)w.gu_codes + e * gu, st), op);
+    HIP_TRY(rk_launch_fp8_layout(dev + 2 * one, H, (int)I, 32, 0, (uint8_t *)w.dn_codes + e * dn, st), op);
+    HIP_TRY(hipMemcpyAsync(w.gu_scales + e * 2 * sc, gate_scales + e * sc, (size_t)sc * 4, hipMemcpyHostToDevice, st), op);
+    HIP_TRY(hipMemcpyAsync(w.gu_scales + e * 2 * sc + sc, up_scales + e * sc, (size_t)sc * 4, hipMemcpyHostToDevice, st), op);
+  }
+  HIP_TRY(hipMemcpyAsync(w.dn_scales, down_scales, (size_t)(E * sc) * 4, hipMemcpyHostToDevice, st), op);
+  HIP_TRY(hipStreamSynchronize(st), op);
+  *id = guard.register_weight();
+  return RK_OK;
+}
+
+extern "C" int rk_moe_experts_fp8_dev(rk_weight_id id, const void *plan, const void *x, void *y, int dtype, int accumulate,
+                                      rk_stream stream) {
+  const char *op = "rk_moe_experts_fp8_dev";
+  return no_throw(op, [&]() -> int {
+    std::lock_guard<std::mutex> lk(g_mu);
+    RK_TRY(ensure(op));
+    MoePlan *p = (MoePlan *)plan;
+    if (!p) return fail(RK_E_SHAPE, op, "null plan");
+    if (!fp8_float(dtype)) return fail(RK_E_SHAPE, op, "unknown dtype");
+    if (p->routed && p->weight == id && p->has_batch && p->s == 0) return RK_OK;
+    Weight *w;
+    RK_TRY(moe_planned_check(id, *p, &w, op));
+    if (!w->moe_fp8) return fail(RK_E_UNSUPPORTED, op, "not an fp8 expert stack");
+    RK_TRY(fp8_rows_check(x, "x", op));
+    RK_TRY(fp8_rows_check(y, "y", op));
+    CallScope cs(pick(stream));
+    RK_TRY(moe_use(cs, *p, true, op));
+    RK_TRY(moe_run_fp8(cs, *w, *p, x, y, dtype, accumulate != 0));
+    if (!p->routed) RK_TRY(plan_mark_used(*p, cs.st));
+    g_eng->calls++;
+    return RK_OK;
+  });
+}
+
+// =========================================================================
 // RMSNorm with the int8 quantizer, host forms of the norms and RoPE
 // =========================================================================
 extern "C" int rk_rms_norm_quantize_dev(const void *x, const void *w, int w_dtype, int64_t rows,
@@ -3263,6 +3636,8 @@ extern "C" int rk_stream_destroy(rk_stream stream) {
   for (SeqPlan *p : g_eng->seq_plans)
     for (DevBuf *b : {&p->block, &p->work})
       if (b->ev_stream == st) b->pending = b->recorded = false;
+  for (MoePlan *p : g_eng->routed_plans)
+    if (p->mem.ev_stream == st) p->mem.pending = p->mem.recorded = false;
   HIP_TRY(hipStreamDestroy(st), "rk_stream_destroy");
   g_eng->own_streams.erase(st);
   return RK_OK;

@@ -35,12 +35,14 @@ __global__ __launch_bounds__(FNW * 64, 2) void fp8_few_kernel(const Fp8FewArgs g
   const int lane = lane_id(), col = lane & 31, h = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int kt = g.kt;
-  int nb = blockIdx.x, rows = g.m;
+  // (a tile's workgroups one behind the other: they share its rows)
+  const int n_nb = (g.n + 31) / 32, nb = blockIdx.x % n_nb;
+  int rows = g.m;
   int64_t row0 = 0;
   const uint8_t *w = g.w;
   const float *ws = g.ws;
   if constexpr (MODE != FEW_DENSE) {
-    const MoeTile tile = g.tiles[blockIdx.y];
+    const MoeTile tile = g.tiles[blockIdx.x / n_nb];
     if (tile.rows <= 0 || tile.expert < 0) return;
     rows = tile.rows;
     row0 = tile.row0;
@@ -70,7 +72,7 @@ __global__ __launch_bounds__(FNW * 64, 2) void fp8_few_kernel(const Fp8FewArgs g
     const int sub = threadIdx.x & 15;
     for (int b = threadIdx.x / 16; b < rows * kt; b += FNW * 4) {
       const int r = b / kt, at = b - r * kt, c = at * 128 + sub * 8;
-      const int64_t src = MODE == FEW_GATE_UP ? (int64_t)g.tok[row0 + r] : row0 + r;
+      const int64_t src = MODE == FEW_GATE_UP ? (int64_t)min(g.tok[row0 + r], g.n_tok - 1) : row0 + r;
       float v[8];
       if (c < g.k) {
         if constexpr (XT == RK_DTYPE_F32) {
@@ -221,8 +223,28 @@ static hipError_t launch_few(const Fp8FewArgs &g, int rows, int n_tiles, hipStre
   }
   const size_t smem = few_smem<XT, NOUT>(rows, g.kt);
   if (smem > 160 * 1024) return hipErrorInvalidValue;
-  hipLaunchKernelGGL(kern, dim3((unsigned)((g.n + 31) / 32), (unsigned)n_tiles), dim3(FNW * 64), smem, st, g);
+  hipLaunchKernelGGL(kern, dim3((unsigned)((int64_t)(g.n + 31) / 32 * n_tiles)), dim3(FNW * 64), smem, st, g);
   return hipGetLastError();
+}
+
+// Rows of an expert tile that a workgroup has LDS for: a power of two of at most 32.
+int rk_fp8_few_rows(int kt) {
+  int rows = 32;
+  while (rows > 1 && few_smem<0, 2>(rows, kt) > 160 * 1024) rows /= 2;
+  return rows;
+}
+hipError_t rk_launch_fp8_few_gate_up(const Fp8FewArgs &g, int x_dtype, int tile_rows, int n_tiles, bool exact, hipStream_t st) {
+#define RK_FEW(XT) (exact ? launch_few<XT, FEW_GATE_UP, true, 1>(g, tile_rows, n_tiles, st) : launch_few<XT, FEW_GATE_UP, false, 1>(g, tile_rows, n_tiles, st))
+  switch (x_dtype) {
+    case RK_DTYPE_F32: return RK_FEW(RK_DTYPE_F32);
+    case RK_DTYPE_F16: return RK_FEW(RK_DTYPE_F16);
+    default: return RK_FEW(RK_DTYPE_BF16);
+  }
+#undef RK_FEW
+}
+hipError_t rk_launch_fp8_few_down(const Fp8FewArgs &g, int tile_rows, int n_tiles, bool exact, hipStream_t st) {
+  return exact ? launch_few<RK_DTYPE_F32, FEW_DOWN, true, 1>(g, tile_rows, n_tiles, st)
+               : launch_few<RK_DTYPE_F32, FEW_DOWN, false, 1>(g, tile_rows, n_tiles, st);
 }
 
 hipError_t rk_launch_fp8_few(const Fp8FewArgs &g, int x_dtype, bool exact, hipStream_t st) {

@@ -308,9 +308,10 @@ struct Fp8FewArgs {
   const float *ws;
   void *c;            // [rows, n] of c_dtype
   int c_dtype;
-  // experts: grid.y is a tile
+  // experts
   const MoeTile *tiles;
-  const int32_t *tok;           // row of x of each bucket row (first product)
+  int n_tok;                    // rows of x (first product)
+  const int32_t *tok;           // row of x of each bucket row
   const float *row_w;           // router weight of each bucket row (second product)
   int64_t w_stride, ws_stride;  // bytes and scales per expert
   int64_t up_scales;            // scales from a gate block's to its up block's
@@ -331,6 +332,50 @@ struct Fp8GemmArgs {
   int num_cus;
 };
 hipError_t rk_launch_gemm_fp8(const Fp8GemmArgs &g, bool exact, hipStream_t st);
+
+// Router and lists on the GPU (moe_route.hip).
+constexpr int RK_ROUTE_MAX_EXPERTS = 1024;
+constexpr int RK_ROUTE_MAX_TOP = 64, RK_ROUTE_MAX_GROUPS = 64;
+struct RouteArgs {
+  const void *logits;  // [s, n_experts] of dtype
+  int dtype;
+  int64_t s;
+  int n_experts, top_k, score;
+  const float *bias;   // [n_experts] or null
+  int n_groups, top_groups, norm;
+  float scale;
+  uint32_t *ids;       // [s, top_k]
+  float *wts;
+};
+hipError_t rk_launch_moe_route(const RouteArgs &g, hipStream_t st);
+struct RouteListArgs {
+  const uint32_t *ids;  // [rows] = [s, top_k]; ids past the last expert: no expert
+  const float *wts;
+  int64_t rows;
+  int top_k, n_experts, tile_rows, max_tiles;
+  int32_t *counts;      // [blocks][n_experts + 1], where there is more than one block
+  int32_t *n_valid;     // rows with an expert: the first ones
+  int32_t *tok;
+  float *row_w;
+  int32_t *slot;
+  MoeTile *tiles, *tiles_gu;  // [max_tiles]: rows without an expert are tiles of expert -1, unused ones have no rows
+};
+int rk_moe_lists_blocks(int64_t rows);
+hipError_t rk_launch_moe_lists(const RouteListArgs &g, hipStream_t st);
+struct CombineArgs {
+  const float *rows;     // [bucket rows, n], weighted
+  const int32_t *slot;   // [s, top_k]
+  const int32_t *n_valid;  // rows from this one on count for nothing (null: all count)
+  void *y;               // [s, n]
+  int64_t s;
+  int n, top_k, accumulate;  // n % 4 == 0
+};
+hipError_t rk_launch_moe_combine(const CombineArgs &g, int dtype, hipStream_t st);
+// fp8 experts on tiles of at most rk_fp8_few_rows(k) rows: x of x_dtype (first product, silu(gate)·up to f32 rows), or
+// f32 rows (second product, times their router weight).
+int rk_fp8_few_rows(int kt);
+hipError_t rk_launch_fp8_few_gate_up(const Fp8FewArgs &g, int x_dtype, int tile_rows, int n_tiles, bool exact, hipStream_t st);
+hipError_t rk_launch_fp8_few_down(const Fp8FewArgs &g, int tile_rows, int n_tiles, bool exact, hipStream_t st);
 
 // The static device scratch of rk_attention_dev_noalloc (noalloc.hip):
 // rk_noalloc_setup looks up the array's address on `device`, which must be

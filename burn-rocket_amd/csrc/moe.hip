@@ -242,6 +242,21 @@ __device__ __forceinline__ void moe_epilogue(const floatx16 (&facc)[NRB], const 
   }
 }
 
+// Tiles of expert -1, in lists built on the GPU: rows of tokens whose id named no expert. They count in the combine as rows
+// of zeros.
+template <int NW, int BM>
+__device__ __forceinline__ void moe_dead_tile(const MoeTile &tile, int64_t a_rows, int N, int n0, float *__restrict__ out,
+                                              int out_ld, const MoeCombine &cmb, float *s_rw, void *s_free) {
+  for (int row = threadIdx.x; row < BM; row += NW * 64) s_rw[row] = 0.f;
+  __syncthreads();
+  floatx16 facc[BM / 32];
+#pragma unroll
+  for (int i = 0; i < BM / 32; ++i)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) facc[i][r] = 0.f;
+  moe_epilogue<false, NW, BM / 32, 16>(facc, tile, a_rows, N, n0, s_rw, s_free, out, out_ld, cmb);
+}
+
 template <bool GU, int NW, int PD, int BM, int NRB>
 __device__ __forceinline__ void moe_body(
     const int8_t *__restrict__ A, const float *__restrict__ AS, int as_stride,
@@ -517,6 +532,13 @@ __global__ __launch_bounds__(NW * 64, 2) void moe_q8_kernel(
   const int L = t * n_col_tiles + jb % n_col_tiles;
   const MoeTile tile = tiles[L / n_col_tiles];
   const int n0 = (L % n_col_tiles) * 32 * NW;
+  if (tile.expert < 0) {  // no expert's rows, or an entry without rows (lists built on the GPU)
+    if constexpr (!GU) {
+      if (tile.rows > 0)
+        moe_dead_tile<NW, BM>(tile, a_rows, N, n0, out, out_ld, cmb, (float *)smem, (float *)smem + BM);
+    }
+    return;
+  }
   const int8_t *We = W + (int64_t)tile.expert * w_stride_e;
   const float *WSe = WS + (int64_t)tile.expert * ws_stride_e;
   // The body is instantiated per count of 32-row blocks holding rows; the
@@ -559,6 +581,12 @@ __global__ __launch_bounds__(256, 3) void moe_few_kernel(
   if (t >= cmb.n_tiles) return;
   const MoeTile tile = tiles[t];
   const int n0 = (jb % n_col_tiles) * 32 * NW;
+  if (tile.expert < 0) {  // as in moe_q8_kernel
+    if constexpr (!GU) {
+      if (tile.rows > 0) moe_dead_tile<NW, 32>(tile, a_rows, N, n0, out, out_ld, cmb, s_rw, s_free);
+    }
+    return;
+  }
   const int lane = lane_id();
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int fcol = lane & 31, fh = lane >> 5;

@@ -1,0 +1,349 @@
+// The router of a mixture of experts, and the lists of expert tiles that its choices make, both on the GPU: a routed layer
+// needs nothing from the host between its launches and can be captured into a graph.
+#include "common.hpp"
+#include "kernels.hpp"
+
+// ---------------------------------------------------------------------------
+// Router. A wave per token: expert v·64 + lane in register v of the lane. Choices are compared by the f64 score with its
+// bias, or, where there is none, by the logits themselves, which order the experts as their scores do: of two experts whose
+// f32 scores are a rounding apart the larger is taken, whatever the order of a sum. Equal ones go to the lower id; a NaN
+// ranks with -inf.
+namespace {
+struct Choice {
+  double key;
+  int id;  // INT_MAX: none
+};
+__device__ __forceinline__ bool before(const Choice &a, const Choice &b) { return a.key > b.key || (a.key == b.key && a.id < b.id); }
+// The first of the wave's choices, in all lanes.
+__device__ __forceinline__ Choice wave_first(Choice c) {
+#pragma unroll
+  for (int d = 32; d >= 1; d /= 2) {
+    const Choice o{__shfl_xor(c.key, d), __shfl_xor(c.id, d)};
+    if (before(o, c)) c = o;
+  }
+  return c;
+}
+constexpr int ROUTE_WAVES = 4;
+}  // namespace
+
+template <int V>
+__global__ __launch_bounds__(ROUTE_WAVES * 64) void moe_route_kernel(const RouteArgs g) {
+  const int lane = lane_id();
+  const int64_t t = (int64_t)blockIdx.x * ROUTE_WAVES + (threadIdx.x >> 6);
+  if (t >= g.s) return;
+  const int E = g.n_experts;
+  float p[V];
+  double key[V];
+  float mx = -INFINITY;
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    const int e = v * 64 + lane;
+    p[v] = e < E ? dt_load_any(g.logits, t * E + e, g.dtype) : -INFINITY;
+    key[v] = (double)p[v];
+    mx = fmaxf(mx, p[v]);
+  }
+  // Scores, in f32 as the weights are, and in f64 where they are compared.
+  if (g.score == RK_ROUTE_SOFTMAX) {
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) mx = fmaxf(mx, __shfl_xor(mx, d));
+    float sum = 0.f;
+    double sum64 = 0;
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      const bool in = v * 64 + lane < E;
+      if (g.bias) {
+        key[v] = in ? exp(key[v] - (double)mx) : 0;
+        sum64 += key[v];
+      }
+      p[v] = in ? expf(p[v] - mx) : 0.f;
+      sum += p[v];
+    }
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) sum += __shfl_xor(sum, d);
+    if (g.bias)
+#pragma unroll
+      for (int d = 1; d < 64; d *= 2) sum64 += __shfl_xor(sum64, d);
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      p[v] = p[v] / sum;
+      if (g.bias) key[v] = key[v] / sum64;
+    }
+  } else {
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      if (g.bias) key[v] = 1 / (1 + exp(-key[v]));
+      p[v] = 1.0f / (1.0f + expf(-p[v]));
+    }
+  }
+  unsigned open = 0;  // experts of the lane that may be chosen
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    const int e = v * 64 + lane;
+    if (e < E) {
+      if (g.bias) key[v] += (double)g.bias[e];
+      open |= 1u << v;
+    }
+    if (!(key[v] == key[v])) key[v] = -INFINITY;
+  }
+  auto best_of = [&](int lo, int hi, unsigned from) {
+    Choice c{-INFINITY, INT_MAX};
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      const int e = v * 64 + lane;
+      const Choice o{key[v], e};
+      if ((from >> v & 1) && e >= lo && e < hi && before(o, c)) c = o;
+    }
+    return wave_first(c);
+  };
+  auto close = [&](unsigned &mask, int id) {
+    if ((id & 63) == lane) mask &= ~(1u << (id >> 6));
+  };
+
+  // Groups: the score of one is its best choice, or with a bias the sum of its two best; experts of the others are closed.
+  if (g.n_groups > 1 && g.top_groups < g.n_groups) {
+    const int size = E / g.n_groups;
+    Choice mine{-INFINITY, INT_MAX};  // lane i: group i
+    for (int i = 0; i < g.n_groups; ++i) {
+      const Choice a = best_of(i * size, (i + 1) * size, open);
+      double s = a.key;
+      if (g.bias && size > 1) {
+        unsigned rest = open;
+        close(rest, a.id);
+        s += best_of(i * size, (i + 1) * size, rest).key;
+      }
+      if (!(s == s)) s = -INFINITY;  // (two infinities)
+      if (lane == i) mine = Choice{s, i};
+    }
+    unsigned keep = 0;
+    uint64_t kept = 0;
+    for (int j = 0; j < g.top_groups; ++j) {
+      const Choice c = wave_first(mine);
+      kept |= (uint64_t)1 << c.id;
+      if (lane == c.id) mine = Choice{-INFINITY, INT_MAX};
+    }
+#pragma unroll
+    for (int v = 0; v < V; ++v)
+      if ((open >> v & 1) && (kept >> ((v * 64 + lane) / size) & 1)) keep |= 1u << v;
+    open = keep;
+  }
+
+  // The top_k: lane j keeps choice j.
+  float w = 0.f, sum = 0.f;
+  int id = 0;
+  for (int j = 0; j < g.top_k; ++j) {
+    const Choice c = best_of(0, E, open);
+    close(open, c.id);
+    float mine = 0.f;
+#pragma unroll
+    for (int v = 0; v < V; ++v)
+      if (v == (c.id >> 6)) mine = p[v];
+    const float pw = __shfl(mine, c.id & 63);
+    sum += pw;
+    if (lane == j) {
+      w = pw;
+      id = c.id;
+    }
+  }
+  if (lane < g.top_k) {
+    if (g.norm) w = w / (sum + 1e-20f);
+    g.ids[t * g.top_k + lane] = (uint32_t)id;
+    g.wts[t * g.top_k + lane] = w * g.scale;
+  }
+}
+
+hipError_t rk_launch_moe_route(const RouteArgs &g, hipStream_t st) {
+  const int v = (g.n_experts + 63) / 64;
+  auto kern = v <= 1 ? moe_route_kernel<1> : v <= 2 ? moe_route_kernel<2> : v <= 4 ? moe_route_kernel<4> : v <= 8 ? moe_route_kernel<8> : moe_route_kernel<16>;
+  hipLaunchKernelGGL(kern, dim3((unsigned)((g.s + ROUTE_WAVES - 1) / ROUTE_WAVES)), dim3(ROUTE_WAVES * 64), 0, st, g);
+  return hipGetLastError();
+}
+
+// ---------------------------------------------------------------------------
+// Lists of a routed batch: the (token, slot) pairs sorted by expert, stably, which is the order that the host's lists have;
+// tiles of at most tile_rows rows; each token's rows in ascending expert id. Pairs whose id names no expert form a bucket
+// behind the last expert's, whose tiles have expert -1.
+//
+// Blocks of 1024 pairs. A pair's row is its expert's first row, plus the expert's pairs in earlier blocks (from the blocks'
+// counts, which a first launch leaves in memory where there are several), plus those of earlier waves of its block, plus
+// those of earlier lanes of its wave. No pair waits for another block's, and nothing depends on the order of atomics.
+namespace {
+constexpr int LB = 1024;       // pairs per block
+constexpr int LW = LB / 64;
+}  // namespace
+
+__global__ __launch_bounds__(LB) void moe_count_kernel(const RouteListArgs g) {
+  __shared__ int cnt[RK_ROUTE_MAX_EXPERTS + 1];
+  const int E = g.n_experts;
+  for (int e = threadIdx.x; e <= E; e += LB) cnt[e] = 0;
+  __syncthreads();
+  const int64_t i = (int64_t)blockIdx.x * LB + threadIdx.x;
+  if (i < g.rows) atomicAdd(&cnt[min(g.ids[i], (uint32_t)E)], 1);
+  __syncthreads();
+  for (int e = threadIdx.x; e <= E; e += LB) g.counts[(int64_t)blockIdx.x * (E + 1) + e] = cnt[e];
+}
+
+// Exclusive sums of x over the block's threads (fields of a word may be packed: none may carry).
+__device__ __forceinline__ uint64_t block_exclusive(uint64_t x, uint64_t *s_wave, uint64_t *total) {
+  const int lane = lane_id(), wave = threadIdx.x >> 6;
+  uint64_t inc = x;
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) {
+    const uint64_t o = __shfl_up(inc, d);
+    if (lane >= d) inc += o;
+  }
+  if (lane == 63) s_wave[wave] = inc;
+  __syncthreads();
+  uint64_t base = 0, all = 0;
+#pragma unroll
+  for (int w = 0; w < LW; ++w) {
+    const uint64_t o = s_wave[w];
+    if (w < wave) base += o;
+    all += o;
+  }
+  __syncthreads();
+  *total = all;
+  return base + inc - x;
+}
+
+__global__ __launch_bounds__(LB) void moe_lists_kernel(const RouteListArgs g, int n_blocks) {
+  constexpr int ME = RK_ROUTE_MAX_EXPERTS;
+  __shared__ int s_all[ME + 1], s_at[ME + 1];   // rows of each expert; the first row of this block's
+  __shared__ uint16_t s_cnt[LW][ME + 1];        // rows of each expert in each wave
+  __shared__ uint64_t s_wave[LW];
+  const int E = g.n_experts, tid = threadIdx.x, lane = lane_id(), wave = tid >> 6;
+  const int64_t i = (int64_t)blockIdx.x * LB + tid;
+  const bool in = i < g.rows;
+  const int e = in ? (int)min(g.ids[i], (uint32_t)E) : E + 1;
+  for (int x = tid; x <= E; x += LB) {
+    s_all[x] = 0;
+#pragma unroll
+    for (int w = 0; w < LW; ++w) s_cnt[w][x] = 0;
+  }
+  __syncthreads();
+  // Lanes of the wave with this pair's expert.
+  uint64_t peers = ~(uint64_t)0;
+  for (int b = 0; (E + 1) >> b != 0; ++b) {
+    const uint64_t has = __ballot(e >> b & 1);
+    peers &= (e >> b & 1) ? has : ~has;
+  }
+  const int rank = __popcll(peers & (((uint64_t)1 << lane) - 1));
+  if (in && rank == 0) s_cnt[wave][e] = (uint16_t)__popcll(peers);
+  if (n_blocks == 1) {
+    if (in && rank == 0) atomicAdd(&s_all[e], __popcll(peers));
+    __syncthreads();
+  }
+  // Rows of each expert in all blocks, and in those before this one. (E + 1 may be one more than the threads: the last
+  // bucket's count is not needed for the first rows.)
+  int all = 0, earlier = 0;
+  if (tid < E) {
+    if (n_blocks == 1) {
+      all = s_all[tid];
+    } else {
+      for (int b = 0; b < n_blocks; ++b) {
+        const int c = g.counts[(int64_t)b * (E + 1) + tid];
+        all += c;
+        if (b < (int)blockIdx.x) earlier += c;
+      }
+    }
+  }
+  uint64_t valid;
+  const int first = (int)block_exclusive((uint64_t)all, s_wave, &valid);
+  if (tid < E) s_at[tid] = first + earlier;
+  if (tid == 0) {
+    // The bucket without an expert: what this block and the earlier ones leave over.
+    int mine = 0;
+    if (n_blocks > 1)
+      for (int b = 0; b < (int)blockIdx.x; ++b) mine += g.counts[(int64_t)b * (E + 1) + E];
+    s_at[E] = (int)valid + mine;
+  }
+  __syncthreads();
+  if (in) {
+    int row = s_at[e] + rank;
+    for (int w = 0; w < wave; ++w) row += s_cnt[w][e];
+    const int64_t t = i / g.top_k;
+    const int j = (int)(i - t * g.top_k);
+    g.tok[row] = (int32_t)t;
+    g.row_w[row] = e < E ? g.wts[i] : 0.f;
+    int at = 0;
+    for (int o = 0; o < g.top_k; ++o) {
+      const int oe = (int)min(g.ids[t * g.top_k + o], (uint32_t)E);
+      if (oe < e || (oe == e && o < j)) ++at;
+    }
+    g.slot[t * g.top_k + at] = row;
+  }
+  if (blockIdx.x != 0) return;
+
+  // Tiles in expert order, and longest first: by quarters of tile_rows, in expert order within one. Thread x makes expert
+  // x's; four 16-bit counts (quarters 4, 3, 2, 1) share a word of the sums.
+  const int T = g.tile_rows, quarter = T / 4;
+  auto kinds = [&](int rows) -> uint64_t {
+    const int tail = rows % T;
+    uint64_t k = (uint64_t)(rows / T);
+    if (tail) k += (uint64_t)1 << (16 * (4 - (tail + quarter - 1) / quarter));
+    return k;
+  };
+  uint64_t total;
+  const uint64_t mine = kinds(all), base = block_exclusive(mine, s_wave, &total);
+  auto field = [](uint64_t x, int f) { return (int)(x >> (16 * f) & 0xffff); };
+  auto sum4 = [&](uint64_t x) { return field(x, 0) + field(x, 1) + field(x, 2) + field(x, 3); };
+  int start[4];
+  for (int f = 0, at = 0; f < 4; ++f) {
+    start[f] = at;
+    at += field(total, f);
+  }
+  const int n = sum4(total);
+  if (tid < E) {
+    int at = sum4(base), full = start[0] + field(base, 0);
+    for (int r = 0; r < all; r += T) {
+      const int rows = min(T, all - r), f = 4 - (rows + quarter - 1) / quarter;
+      const MoeTile tile{tid, first + r, rows};
+      g.tiles[at++] = tile;
+      // (an expert has any number of whole tiles, and one shorter one at most: whole ones first in their quarter)
+      g.tiles_gu[f == 0 ? full++ : start[f] + field(base, f)] = tile;
+    }
+  }
+  // Rows without an expert, and what no tile uses.
+  const int left = (int)g.rows - (int)valid, dead = (left + T - 1) / T;
+  for (int x = n + tid; x < g.max_tiles; x += LB) {
+    const int d = x - n, r = d * T;
+    const MoeTile tile = d < dead ? MoeTile{-1, (int)valid + r, min(T, left - r)} : MoeTile{-1, 0, 0};
+    g.tiles[x] = tile;
+    g.tiles_gu[x] = tile;
+  }
+  if (tid == 0) *g.n_valid = (int)valid;
+}
+
+hipError_t rk_launch_moe_lists(const RouteListArgs &g, hipStream_t st) {
+  const int nb = (int)((g.rows + LB - 1) / LB);
+  if (nb > 1) hipLaunchKernelGGL(moe_count_kernel, dim3(nb), dim3(LB), 0, st, g);
+  hipLaunchKernelGGL(moe_lists_kernel, dim3(nb), dim3(LB), 0, st, g, nb);
+  return hipGetLastError();
+}
+int rk_moe_lists_blocks(int64_t rows) { return (int)((rows + LB - 1) / LB); }
+
+// The weighted rows of each token to its result, in ascending expert id: y (+)= Σ rows. A thread per four values.
+template <int DT>
+__global__ __launch_bounds__(256) void moe_combine_kernel(const CombineArgs g) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, per = g.n / 4;
+  if (i >= g.s * per) return;
+  const int64_t t = i / per;
+  const int c = (int)(i - t * per) * 4;
+  float acc[4] = {0.f, 0.f, 0.f, 0.f};
+  if (g.accumulate) dt_load_vec<DT, 4>(g.y, t * g.n + c, acc);
+  const int valid = g.n_valid ? *g.n_valid : INT_MAX;
+  for (int j = 0; j < g.top_k; ++j) {
+    const int r = g.slot[t * g.top_k + j];
+    if (r >= valid) continue;
+    const floatx4 v = *(const floatx4 *)(g.rows + (int64_t)r * g.n + c);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) acc[e] += v[e];
+  }
+  dt_store_vec<DT, 4>(g.y, t * g.n + c, acc);
+}
+hipError_t rk_launch_moe_combine(const CombineArgs &g, int dtype, hipStream_t st) {
+  const unsigned grid = (unsigned)((g.s * (g.n / 4) + 255) / 256);
+  auto kern = dtype == RK_DTYPE_F32 ? moe_combine_kernel<RK_DTYPE_F32>
+              : dtype == RK_DTYPE_F16 ? moe_combine_kernel<RK_DTYPE_F16> : moe_combine_kernel<RK_DTYPE_BF16>;
+  hipLaunchKernelGGL(kern, dim3(grid), dim3(256), 0, st, g);
+  return hipGetLastError();
+}

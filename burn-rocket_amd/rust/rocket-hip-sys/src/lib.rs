@@ -33,6 +33,8 @@ pub const RK_WEIGHT_F16: c_int = 1;
 pub const RK_WEIGHT_I8: c_int = 2;
 pub const RK_WEIGHT_QAT: c_int = 3;
 pub const RK_WEIGHT_FP8: c_int = 4;
+pub const RK_ROUTE_SOFTMAX: c_int = 0;
+pub const RK_ROUTE_SIGMOID: c_int = 1;
 
 pub const RK_MASK_NONE: c_int = 0;
 pub const RK_MASK_CAUSAL: c_int = 1;
@@ -213,6 +215,23 @@ unsafe extern "C" {
     pub fn rk_moe_route(
         logits: *const f32, s: i64, n_experts: c_int, top_k: c_int, norm_topk: c_int,
         ids: *mut u32, wts: *mut f32
+    ) -> c_int;
+    pub fn rk_moe_route_dev(
+        logits: *const c_void, dtype: c_int, s: i64, n_experts: c_int, top_k: c_int, score: c_int,
+        bias: *const f32, n_groups: c_int, top_groups: c_int, norm_topk: c_int, scale: f32, ids: *mut u32,
+        wts: *mut f32, stream: Stream
+    ) -> c_int;
+    pub fn rk_moe_routed_plan_create(id: WeightId, max_s: i64, top_k: c_int, plan: *mut *mut c_void) -> c_int;
+    pub fn rk_moe_plan_route_dev(
+        plan: *mut c_void, s: i64, ids: *const u32, wts: *const f32, stream: Stream
+    ) -> c_int;
+    pub fn rk_pack_moe_fp8(
+        gate: *const u8, gate_scales: *const f32, up: *const u8, up_scales: *const f32, down: *const u8,
+        down_scales: *const f32, n_experts: c_int, hidden: i64, inter: i64, id: *mut WeightId
+    ) -> c_int;
+    pub fn rk_moe_experts_fp8_dev(
+        id: WeightId, plan: *const c_void, x: *const c_void, y: *mut c_void, dtype: c_int, accumulate: c_int,
+        stream: Stream
     ) -> c_int;
     pub fn rk_pack_moe_q8_0(
         gate: *const u8, up: *const u8, down: *const u8, n_experts: c_int, hidden: i64, inter: i64,

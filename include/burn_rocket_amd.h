@@ -77,6 +77,10 @@ extern "C" {
 #define RK_GLU_SILU 1
 #define RK_GLU_GELU 2
 
+/* Scores of a router (rk_moe_route_dev). */
+#define RK_ROUTE_SOFTMAX 0
+#define RK_ROUTE_SIGMOID 1
+
 typedef uint64_t rk_weight_id;
 typedef void *rk_stream; /* a hipStream_t; NULL selects the library stream */
 
@@ -118,7 +122,8 @@ int rk_stats_reset(void);
  * matmul_bo_bytes); host_bytes is the page-locked staging of the host-buffer
  * entries (its *_host_bytes) and the bucket lists of rk_moe_experts_dev. All three
  * count the lists and workspaces of live plans of sequences too, which go with
- * rk_seq_plan_destroy and not with the calls below (n_scratch does not count them). */
+ * rk_seq_plan_destroy and not with the calls below (n_scratch does not count them);
+ * scratch_bytes also the memory of live routed plans (rk_moe_routed_plan_create). */
 typedef struct {
   uint64_t weights_bytes;   /* resident weights */
   uint64_t scratch_bytes;   /* device scratch, all buffers */
@@ -609,6 +614,62 @@ int rk_moe_plan_destroy(void *plan);
  * within an expert, by token (the bucket order of engine.rs:292-305). */
 int rk_moe_gate_up_dev(rk_weight_id id, const void *plan, const float *x,
                        float *act, rk_stream stream);
+
+/* ---- routed on the GPU ----------------------------------------------------- *
+ * No counterpart in the reference, which routes and buckets on the host
+ * (src/clef/model.rs:462-489, src/clef/engine.rs:284-313). A layer is three calls
+ * on one stream, none of which copies or waits: route the tokens, build the lists,
+ * run the experts. */
+
+/* Router on device buffers: logits [s, n_experts] of type dtype to ids u32 [s, top_k]
+ * and wts f32 [s, top_k]. The scores p are the softmax of a token's logits or their
+ * sigmoid (score, RK_ROUTE_*). Experts are chosen by p + bias (f32 [n_experts], or
+ * NULL: by p), in descending order; the weights are p without the bias, divided by
+ * their sum + 1e-20 with norm_topk, times scale. n_groups > 1 (dividing n_experts)
+ * chooses among the experts of top_groups groups of n_experts / n_groups consecutive
+ * ones: a group's own score is the sum of its two largest p + bias, without a bias its
+ * largest p. Ties go to the lower id. Choices are compared in f64 (without a bias: by the logits,
+ * where rk_moe_route compares f32 probabilities, of which two may be equal); the weights are f32. A
+ * NaN ranks with -inf. 1 <= top_k <= 64 and at most the experts of the chosen groups;
+ * n_experts up to 1024, n_groups up to 64 (RK_E_UNSUPPORTED). s = 0 does nothing. */
+int rk_moe_route_dev(const void *logits, int dtype, int64_t s, int n_experts, int top_k, int score, const float *bias,
+                     int n_groups, int top_groups, int norm_topk, float scale, uint32_t *ids, float *wts, rk_stream stream);
+
+/* A plan of rk_moe_experts_planned_dev whose lists are built on the GPU, and that owns what
+ * its calls need: room for batches of up to max_s tokens. For stacks of up to 1024 experts
+ * and up to 2^20 rows max_s·top_k. The limits of rk_moe_experts_dev hold for max_s. Freed by
+ * rk_moe_plan_destroy, which waits for its calls; counted by rk_mem_stats as scratch. */
+int rk_moe_routed_plan_create(rk_weight_id id, int64_t max_s, int top_k, void **plan);
+/* The plan's next batch: ids [s, top_k] and wts [s, top_k] on the device, ordered on
+ * `stream` after the calls that used the plan. An id that names no expert (>= n_experts: an
+ * expert of another GPU, say) adds nothing to its token; a token of such ids alone gets
+ * zeros (with an accumulating call: nothing). An expert named twice counts twice. s = 0
+ * is a batch without tokens, on which the calls do nothing.
+ *
+ * HIP graphs: this call and the planned calls on such a plan allocate nothing and may be
+ * captured. Every later batch of the plan then has the captured s (RK_E_SHAPE): one plan per
+ * captured size. After a captured rk_moe_plan_route_dev, calls outside a capture need an
+ * rk_moe_plan_route_dev outside one first (RK_E_UNSUPPORTED). The caller orders the replays
+ * that share a plan, and other calls on it, after one another; while the stream of the
+ * plan's last call is captured, whatever would have to wait for that call is refused
+ * (RK_E_UNSUPPORTED). A plan is destroyed after its graphs. */
+int rk_moe_plan_route_dev(void *plan, int64_t s, const uint32_t *ids, const float *wts, rk_stream stream);
+
+/* Resident expert stack of block-scaled fp8 FFNs: codes gate and up [E, inter, hidden] and
+ * down [E, hidden, inter] with scales [E, ceil(rows/128), ceil(K/128)] each, on the host.
+ * hidden and inter are multiples of 16, up to 65536. rk_moe_experts_dev, the planned calls
+ * and their accumulating forms take it like a Q8_0 stack, with f32 x and y: x quantized as by
+ * rk_quantize_fp8_dev, silu(gate)·up in f32 quantized the same way, and the products of
+ * rk_matmul_fp8_dev in f32; tokens are summed in ascending expert id. rk_moe_gate_up_dev does
+ * not take it (RK_E_UNSUPPORTED). */
+int rk_pack_moe_fp8(const uint8_t *gate, const float *gate_scales, const uint8_t *up, const float *up_scales,
+                    const uint8_t *down, const float *down_scales, int n_experts, int64_t hidden, int64_t inter,
+                    rk_weight_id *id);
+/* The planned call on an fp8 stack with x and y of type dtype; accumulate: onto y. bf16: both
+ * products by the fp8 matrix instructions; fp16: the first one, whose results are quantized
+ * again, with f32 sums; f32: both with f32 sums. x and y are 16-byte aligned and may be the same buffer. */
+int rk_moe_experts_fp8_dev(rk_weight_id id, const void *plan, const void *x, void *y, int dtype, int accumulate,
+                           rk_stream stream);
 
 /* ======================================================================== *
  * MLP glue                                                                 *
