@@ -19,7 +19,7 @@ LIBDIR = os.path.join(HERE, "lib")
 LIB = os.path.join(LIBDIR, "libburn_rocket_amd.so")
 SOURCES = ["gemm_f16.hip", "gemm_i8.hip", "skinny.hip", "misc.hip", "norm.hip", "attention.hip", "attention_rows.hip", "moe.hip", "noalloc.hip",
            "attention_seqs.hip", "seq_tiles_f16.hip", "seq_tiles_bf16.hip", "seq_tiles_f16_cap.hip",
-           "seq_tiles_bf16_cap.hip", "seq_rows_f16.hip", "seq_rows_bf16.hip", "paged_append.hip", "fp8_quant.hip", "fp8_few.hip", "gemm_fp8.hip", "moe_route.hip", "engine.cpp", "stage.cpp", "seq_plan.cpp"]
+           "seq_tiles_bf16_cap.hip", "seq_rows_f16.hip", "seq_rows_bf16.hip", "paged_append.hip", "fp8_quant.hip", "fp8_few.hip", "gemm_fp8.hip", "moe_fp8.hip", "moe_route.hip", "engine.cpp", "stage.cpp", "seq_plan.cpp"]
 
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 ARCH = "gfx950"

@@ -2010,9 +2010,14 @@ struct MoeLists {
   size_t roww = 0, tiles = 0, tiles_gu = 0, slot = 0, bytes = 0;
 };
 
-// Rows of a tile of fp8 experts.
+// Rows of a tile of fp8 experts, by the rows that an expert has on average: the kernels of few rows, then tiles of 128 and
+// of 256 rows.
+int64_t moe_fp8_few_limit(const Weight &w) { return 16 * (int64_t)w.n_experts; }
 int moe_fp8_tile_rows(const Weight &w, int64_t rows) {
-  return std::min(rk_fp8_few_rows(w.gu_ws_stride), rk_fp8_few_rows(w.dn_ws_stride));
+  const int knob = rk_knob("RK_MOE_FP8_ROWS", 0);
+  if (knob == 128 || knob == 256) return knob;
+  if (rows <= moe_fp8_few_limit(w)) return std::min(rk_fp8_few_rows(w.gu_ws_stride), rk_fp8_few_rows(w.dn_ws_stride));
+  return rows >= 192 * (int64_t)w.n_experts ? 256 : 128;
 }
 
 // Checks the ids and sizes the lists: tiles of ≤ rk_moe_tile_rows() rows (two
@@ -2127,54 +2132,99 @@ int moe_buf(CallScope &cs, const MoePlan &plan, const char *name, size_t bytes, 
 // The buffers of a call on s tokens (`rows` pairs), and their bytes: what moe_run and moe_run_fp8 ask for.
 std::vector<std::pair<const char *, size_t>> moe_buffers(const Weight &w, int64_t s, int64_t rows) {
   const size_t S = (size_t)s, R = (size_t)rows, H = (size_t)w.hidden, I = (size_t)w.inter;
-  if (w.moe_fp8) return {{"moe_act", R * I * 4}, {"moe_yb", R * H * 4}};
+  if (w.moe_fp8) {
+    const size_t kh = (H + 127) / 128, ki = (I + 127) / 128, few = std::min(R, (size_t)moe_fp8_few_limit(w));
+    return {{"moe_xq", S * H}, {"moe_xs", S * kh * 4}, {"moe_act", std::max(few * I * 4, R * ki * 128)}, {"moe_as", R * ki * 4},
+            {"moe_yb", R * H * 4}};
+  }
   return {{"moe_xq", S * H},       {"moe_xs", S * (H / 32) * 4}, {"moe_act", R * I * 4}, {"moe_aq", R * I},
           {"moe_as", R * (I / 32) * 4}, {"moe_yb", R * H * 4},        {"moe_cnt", S * ((H + 127) / 128) * 4}};
 }
 
 // fp8 experts. Tiles of few rows: each workgroup quantizes the rows it multiplies; silu(gate)·up goes to the second product
-// in f32. fp16 results: the first product has f32 sums, since a code of its results that flips is worth more than an fp16
+// in f32. Others: the tokens are quantized once, and the first product quantizes its results. fp16 results: the first product has f32 sums, since a code of its results that flips is worth more than an fp16
 // rounding; f32 results: both have.
 int moe_run_fp8(CallScope &cs, const Weight &w, const MoePlan &plan, const void *x, void *y, int dtype, bool accumulate,
                 const std::function<int(int)> &lists = nullptr) {
   const char *op = "rk_moe_experts_fp8_dev";
   const int64_t H = w.hidden, I = w.inter, R = plan.rows;
   hipStream_t st = cs.st;
+  const bool few = plan.tile_rows < 128, exact1 = dtype != RK_DTYPE_BF16, exact2 = dtype == RK_DTYPE_F32;
+  const int64_t KTh = w.gu_ws_stride, KTi = w.dn_ws_stride;
   void *act, *yb;
-  RK_TRY(moe_buf(cs, plan, "moe_act", (size_t)R * I * 4, &act));
+  RK_TRY(moe_buf(cs, plan, "moe_act", few ? (size_t)R * I * 4 : (size_t)R * KTi * 128, &act));
   RK_TRY(moe_buf(cs, plan, "moe_yb", (size_t)R * H * 4, &yb));
-  if (lists) {
-    RK_TRY(lists(0));
-    RK_TRY(lists(1));
+  if (few) {
+    if (lists) {
+      RK_TRY(lists(0));
+      RK_TRY(lists(1));
+    }
+    Fp8FewArgs g{};
+    g.x = x;
+    g.n = (int)I;
+    g.k = (int)H;
+    g.kt = (int)KTh;
+    g.w = (const uint8_t *)w.gu_codes;
+    g.ws = w.gu_scales;
+    g.w_stride = moe_fp8_gu_bytes(w);
+    g.up_scales = KTi * KTh;
+    g.ws_stride = 2 * g.up_scales;
+    g.c = act;
+    g.c_dtype = RK_DTYPE_F32;
+    g.tiles = plan.tiles_gu;
+    g.n_tok = (int)plan.s;
+    g.tok = plan.tok;
+    HIP_TRY(rk_launch_fp8_few_gate_up(g, dtype, plan.tile_rows, plan.n_tiles, exact1, st), op);
+    g.x = act;
+    g.n = (int)H;
+    g.k = (int)I;
+    g.kt = (int)KTi;
+    g.w = (const uint8_t *)w.dn_codes;
+    g.ws = w.dn_scales;
+    g.w_stride = moe_fp8_dn_bytes(w);
+    g.ws_stride = KTh * KTi;
+    g.c = yb;
+    g.tiles = plan.tiles;
+    g.row_w = plan.roww;
+    HIP_TRY(rk_launch_fp8_few_down(g, plan.tile_rows, plan.n_tiles, exact2, st), op);
+  } else {
+    void *xq, *xs, *as;
+    RK_TRY(moe_buf(cs, plan, "moe_xq", (size_t)plan.s * H, &xq));
+    RK_TRY(moe_buf(cs, plan, "moe_xs", (size_t)plan.s * KTh * 4, &xs));
+    RK_TRY(moe_buf(cs, plan, "moe_as", (size_t)R * KTi * 4, &as));
+    HIP_TRY(rk_launch_quantize_fp8(x, dtype, plan.s, (int)H, (uint8_t *)xq, H, (float *)xs, st), op);
+    if (lists) RK_TRY(lists(0));
+    Fp8MoeArgs g{};
+    g.a = (const uint8_t *)xq;
+    g.as = (const float *)xs;
+    g.n_tok = (int)plan.s;
+    g.n = (int)I;
+    g.k = (int)H;
+    g.kt = (int)KTh;
+    g.w = (const uint8_t *)w.gu_codes;
+    g.ws = w.gu_scales;
+    g.w_stride = moe_fp8_gu_bytes(w);
+    g.tiles = plan.tiles_gu;
+    g.n_tiles = plan.n_tiles;
+    g.tile_rows = plan.tile_rows;
+    g.tok = plan.tok;
+    g.out = act;
+    g.out_s = (float *)as;
+    HIP_TRY(rk_launch_moe_fp8_gate_up(g, exact1, st), op);
+    if (lists) RK_TRY(lists(1));
+    g.a = (const uint8_t *)act;
+    g.as = (const float *)as;
+    g.n = (int)H;
+    g.k = (int)I;
+    g.kt = (int)KTi;
+    g.w = (const uint8_t *)w.dn_codes;
+    g.ws = w.dn_scales;
+    g.w_stride = moe_fp8_dn_bytes(w);
+    g.tiles = plan.tiles;
+    g.row_w = plan.roww;
+    g.out = yb;
+    HIP_TRY(rk_launch_moe_fp8_down(g, exact2, st), op);
   }
-  Fp8FewArgs g{};
-  g.x = x;
-  g.n = (int)I;
-  g.k = (int)H;
-  g.kt = w.gu_ws_stride;
-  g.w = (const uint8_t *)w.gu_codes;
-  g.ws = w.gu_scales;
-  g.w_stride = moe_fp8_gu_bytes(w);
-  g.up_scales = (I + 127) / 128 * w.gu_ws_stride;
-  g.ws_stride = 2 * g.up_scales;
-  g.c = act;
-  g.c_dtype = RK_DTYPE_F32;
-  g.tiles = plan.tiles_gu;
-  g.n_tok = (int)plan.s;
-  g.tok = plan.tok;
-  HIP_TRY(rk_launch_fp8_few_gate_up(g, dtype, plan.tile_rows, plan.n_tiles, dtype != RK_DTYPE_BF16, st), op);
-  g.x = act;
-  g.n = (int)H;
-  g.k = (int)I;
-  g.kt = w.dn_ws_stride;
-  g.w = (const uint8_t *)w.dn_codes;
-  g.ws = w.dn_scales;
-  g.w_stride = moe_fp8_dn_bytes(w);
-  g.ws_stride = (H + 127) / 128 * w.dn_ws_stride;
-  g.c = yb;
-  g.tiles = plan.tiles;
-  g.row_w = plan.roww;
-  HIP_TRY(rk_launch_fp8_few_down(g, plan.tile_rows, plan.n_tiles, dtype == RK_DTYPE_F32, st), op);
   CombineArgs c{};
   c.rows = (const float *)yb;
   c.slot = plan.slot;
@@ -3349,7 +3399,8 @@ extern "C" int rk_moe_routed_plan_create(rk_weight_id id, int64_t max_s, int top
     if (w->n_experts > RK_ROUTE_MAX_EXPERTS) return fail(RK_E_UNSUPPORTED, op, "up to 1024 experts");
     if (max_s > kMaxRoutedRows / top_k) return fail(RK_E_SHAPE, op, "max_s·top_k above 2^20");
     const int64_t rows = max_s * top_k;
-    if (rows / routed_tile_rows(*w, max_s, rows) > 32768) return fail(RK_E_SHAPE, op, "more than 2^15 tiles");
+    if (w->moe_fp8 && std::min(rows, moe_fp8_few_limit(*w)) / routed_tile_rows(*w, 1, 1) > 32768)
+      return fail(RK_E_SHAPE, op, "more than 2^15 tiles");
     size_t bytes = 0;
     const auto take = [&](size_t n) {
       const size_t at = bytes;

@@ -377,6 +377,24 @@ int rk_fp8_few_rows(int kt);
 hipError_t rk_launch_fp8_few_gate_up(const Fp8FewArgs &g, int x_dtype, int tile_rows, int n_tiles, bool exact, hipStream_t st);
 hipError_t rk_launch_fp8_few_down(const Fp8FewArgs &g, int tile_rows, int n_tiles, bool exact, hipStream_t st);
 
+// fp8 experts on tiles of up to 128 or 256 rows (moe_fp8.hip).
+struct Fp8MoeArgs {
+  const uint8_t *a;    // codes: tokens [n_tok, k] (first product), bucket rows [rows, kt·128] (second)
+  const float *as;     // [.., kt]
+  int n_tok, n, k, kt; // n: outputs (of the first product: of silu(gate)·up)
+  const uint8_t *w;
+  const float *ws;
+  int64_t w_stride;    // bytes per expert
+  const MoeTile *tiles;
+  int n_tiles, tile_rows;
+  const int32_t *tok;
+  const float *row_w;
+  void *out;           // codes [rows, ceil(n/128)·128], or f32 rows [rows, n]
+  float *out_s;        // scales of the codes
+};
+hipError_t rk_launch_moe_fp8_gate_up(const Fp8MoeArgs &g, bool exact, hipStream_t st);
+hipError_t rk_launch_moe_fp8_down(const Fp8MoeArgs &g, bool exact, hipStream_t st);
+
 // The static device scratch of rk_attention_dev_noalloc (noalloc.hip):
 // rk_noalloc_setup looks up the array's address on `device`, which must be
 // current, once; rk_noalloc_scratch returns it (null before setup).

@@ -1,0 +1,150 @@
+// Block-scaled fp8 experts on many rows: the two grouped products over tiles of bucket rows, on the K loop of the dense
+// product (fp8_tile.hpp). Few rows a tile: fp8_few.hip.
+//
+//   gate|up  rows gathered by their tokens; gate and up blocks of 32 weight rows lie in turns, so that a wave holds the gate
+//            and the up value of an output in one lane. A workgroup's 256 weight rows are 128 outputs: a whole block of the
+//            next product's activations, which it quantizes itself. act goes out as codes and scales, a quarter of f32's bytes
+//            and with no pass of its own.
+//   down     bucket rows as they lie, times their router weight, to f32 rows that the combine sums per token.
+#include "fp8_tile.hpp"
+#include "kernels.hpp"
+
+// Tile and column of a workgroup: tile t on XCD t mod 8, all its columns there, sharing its rows in that XCD's L2. Tiles
+// listed for more rows than the workgroup takes are `parts` tiles.
+__device__ __forceinline__ bool moe_fp8_place(const Fp8MoeArgs &g, int bm, int n_col, MoeTile &tile, int &nc) {
+  const int jb = blockIdx.x / 8, t = blockIdx.x % 8 + 8 * (jb / n_col), parts = g.tile_rows / bm;
+  if (t >= g.n_tiles * parts) return false;
+  tile = g.tiles[t / parts];
+  const int first = t % parts * bm;
+  tile.row0 += first;
+  tile.rows = min(tile.rows - first, bm);
+  nc = jb % n_col;
+  return tile.rows > 0 && tile.expert >= 0;
+}
+
+template <class T>
+__global__ __launch_bounds__(T::NT, 2) void moe_fp8_gate_up_kernel(const Fp8MoeArgs g) {
+  static_assert(T::BN == 256 && T::TN % 2 == 0, "128 outputs, gate and up in one wave");
+  constexpr int P = T::TN / 2;  // gate|up pairs of a wave
+  extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
+  MoeTile tile;
+  int nc;
+  const int KT = g.kt, ib = (g.n + 127) / 128;
+  if (!moe_fp8_place(g, T::BM, ib, tile, nc)) return;
+  const uint8_t *w = g.w + (int64_t)tile.expert * g.w_stride + (int64_t)nc * 8 * KT * 4096;
+  const float *ws = g.ws + (int64_t)tile.expert * 2 * ib * KT + (int64_t)nc * KT;
+  T t;
+  t.run(smem, g.a, (int64_t)g.n_tok * g.k, g.as, (int64_t)g.n_tok * KT * 4,
+        [&](int r) -> int64_t { return r < tile.rows ? (int64_t)g.tok[tile.row0 + r] : -1; }, tile.rows, w, (int64_t)8 * KT * 4096,
+        [&](int b) { return ws + (b & 1) * (int64_t)ib * KT; }, g.k, KT);
+
+  // act in place of the gate; the largest of a row's 128 over the lane's two halves and the workgroup's waves.
+  const int lane = lane_id(), col = lane & 31, h = lane >> 5;
+  const int wave = threadIdx.x >> 6, wm = wave / T::WN, wn = wave % T::WN;
+  float *s_max = (float *)smem;                                         // [WN][BM]
+  uint8_t *s_out = smem + T::WN * T::BM * 4;                            // [BM][144]: a row's codes
+  constexpr int ROW = 144;
+  static_assert(T::WN * T::BM * 4 + T::BM * ROW <= T::SMEM, "epilogue LDS");
+  __syncthreads();
+  float amax[T::TM];
+#pragma unroll
+  for (int j = 0; j < T::TM; ++j) {
+    amax[j] = 0.f;
+#pragma unroll
+    for (int p = 0; p < P; ++p)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const float v = fp8_silu_mul(t.acc[2 * p][j][r], t.acc[2 * p + 1][j][r]);
+        t.acc[2 * p][j][r] = v;
+        amax[j] = fmaxf(amax[j], fabsf(v));
+      }
+    amax[j] = fmaxf(amax[j], __shfl_xor(amax[j], 32));
+    if (h == 0) s_max[wn * T::BM + wm * T::WTM + j * 32 + col] = amax[j];
+  }
+  __syncthreads();
+#pragma unroll
+  for (int j = 0; j < T::TM; ++j) {
+    const int r = wm * T::WTM + j * 32 + col;
+    float m = 0.f;
+#pragma unroll
+    for (int x = 0; x < T::WN; ++x) m = fmaxf(m, s_max[x * T::BM + r]);
+    const float s = fp8_scale(m);
+    const Fp8Div div(s);
+#pragma unroll
+    for (int p = 0; p < P; ++p)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const floatx16 &v = t.acc[2 * p][j];
+        *(uint32_t *)(s_out + r * ROW + (wn * P + p) * 32 + q * 8 + h * 4) =
+            fp8_codes4(div(v[4 * q]), div(v[4 * q + 1]), div(v[4 * q + 2]), div(v[4 * q + 3]));
+      }
+    if (wn == 0 && h == 0 && r < tile.rows) g.out_s[((int64_t)tile.row0 + r) * ib + nc] = s;
+  }
+  __syncthreads();
+  for (int c = threadIdx.x; c < tile.rows * 8; c += T::NT) {
+    const int r = c >> 3, at = (c & 7) * 16;
+    *(uintx4 *)((uint8_t *)g.out + ((int64_t)tile.row0 + r) * ib * 128 + nc * 128 + at) = *(const uintx4 *)(s_out + r * ROW + at);
+  }
+}
+
+template <class T>
+__global__ __launch_bounds__(T::NT, 2) void moe_fp8_down_kernel(const Fp8MoeArgs g) {
+  extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
+  MoeTile tile;
+  int nc;
+  const int KT = g.kt, nblk = (g.n + 127) / 128 * 4;
+  if (!moe_fp8_place(g, T::BM, (g.n + T::BN - 1) / T::BN, tile, nc)) return;
+  const int nb0 = nc * (T::BN / 32), n0 = nc * T::BN;
+  const float *ws = g.ws + (int64_t)tile.expert * (nblk / 4) * KT;
+  T t;
+  t.run(smem, g.a + (int64_t)tile.row0 * KT * 128, (int64_t)tile.rows * KT * 128, g.as + (int64_t)tile.row0 * KT, (int64_t)tile.rows * KT * 4,
+        [&](int r) -> int64_t { return r < tile.rows ? r : -1; }, tile.rows, g.w + (int64_t)tile.expert * g.w_stride + (int64_t)nb0 * KT * 4096,
+        (int64_t)(nblk - nb0) * KT * 4096, [&](int b) { return ws + (int64_t)min((nb0 + b) / 4, nblk / 4 - 1) * KT; }, KT * 128, KT);
+  const int lane = lane_id(), col = lane & 31, h = lane >> 5;
+  const int wave = threadIdx.x >> 6, wm = wave / T::WN, wn = wave % T::WN;
+#pragma unroll
+  for (int j = 0; j < T::TM; ++j) {
+    const int r = wm * T::WTM + j * 32 + col;
+    if (r >= tile.rows) continue;
+    const float rw = g.row_w[tile.row0 + r];
+    float *to = (float *)g.out + ((int64_t)tile.row0 + r) * g.n;
+#pragma unroll
+    for (int i = 0; i < T::TN; ++i)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int n = n0 + wn * T::WTN + i * 32 + q * 8 + h * 4;
+        if (n < g.n)  // (a multiple of 16 outputs)
+          *(floatx4 *)(to + n) = floatx4{t.acc[i][j][4 * q] * rw, t.acc[i][j][4 * q + 1] * rw, t.acc[i][j][4 * q + 2] * rw, t.acc[i][j][4 * q + 3] * rw};
+      }
+  }
+}
+
+template <class T, bool GU>
+static hipError_t launch_moe_fp8(const Fp8MoeArgs &g, hipStream_t st) {
+  void (*kern)(const Fp8MoeArgs);
+  if constexpr (GU) kern = moe_fp8_gate_up_kernel<T>;
+  else kern = moe_fp8_down_kernel<T>;
+  static bool attr_set = false;
+  if (!attr_set) {
+    hipError_t e = hipFuncSetAttribute((const void *)kern, hipFuncAttributeMaxDynamicSharedMemorySize, T::SMEM);
+    if (e != hipSuccess) return e;
+    attr_set = true;
+  }
+  const int n_col = GU ? (g.n + 127) / 128 : (g.n + T::BN - 1) / T::BN;
+  hipLaunchKernelGGL(kern, dim3((unsigned)((g.n_tiles * (g.tile_rows / T::BM) + 7) / 8 * 8 * n_col)), dim3(T::NT), T::SMEM, st, g);
+  return hipGetLastError();
+}
+
+template <bool GU>
+static hipError_t launch_moe_fp8_any(const Fp8MoeArgs &g, bool exact, hipStream_t st) {
+  if (g.tile_rows != 128 && g.tile_rows != 256) return hipErrorInvalidValue;
+  if (exact) return launch_moe_fp8<Fp8Tile<128, 256, 2, 4, 2, true>, GU>(g, st);
+  if (g.tile_rows == 256) return launch_moe_fp8<Fp8Tile<256, 256, 4, 2, 2, false>, GU>(g, st);
+  return launch_moe_fp8<Fp8Tile<128, 256, 2, 4, 2, false>, GU>(g, st);
+}
+hipError_t rk_launch_moe_fp8_gate_up(const Fp8MoeArgs &g, bool exact, hipStream_t st) {
+  return launch_moe_fp8_any<true>(g, exact, st);
+}
+hipError_t rk_launch_moe_fp8_down(const Fp8MoeArgs &g, bool exact, hipStream_t st) {
+  return launch_moe_fp8_any<false>(g, exact, st);
+}

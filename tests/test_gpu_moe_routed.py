@@ -19,6 +19,13 @@ def ok(rk, rc):
     assert rc == 0, rk.lib().rk_last_error()
 
 
+@pytest.fixture(params=["by size", "128", "256"])
+def tiles(request, monkeypatch):
+    """fp8 experts on the tiles that the library picks for a batch, and on those of many rows."""
+    if request.param != "by size":
+        monkeypatch.setenv("RK_MOE_FP8_ROWS", request.param)
+
+
 # ------------------------------------------------------------------ router ----
 def route(logits, top_k, score="softmax", bias=None, groups=1, top_groups=1, norm=True, scale=1.0):
     """The definition in 64 bits, a token at a time."""
@@ -166,7 +173,7 @@ def choices(r, s, e, k, how):
 
 @pytest.mark.parametrize("kind", ["q8", "fp8"])
 @pytest.mark.parametrize("how", ["any", "one", "twice"])
-@pytest.mark.parametrize("s", [1, 7, 8, 9, 16, 17, 33, 255, 256, 257, 700, 1100])
+@pytest.mark.parametrize("s", [1, 7, 8, 9, 16, 17, 33, 255, 256, 257, 700, 1100, 2900])
 def test_lists_equal_those_of_the_host(rk, s, how, kind):
     """Bit for bit the results of the host's lists: one block of pairs, several, tiles of every size, one plan for
     batches of changing size."""
@@ -205,7 +212,7 @@ def test_lists_of_few_and_many_experts(rk, e, s, kind):
 
 @pytest.mark.parametrize("kind", ["q8", "fp8"])
 @pytest.mark.parametrize("s", [3, 40, 400])
-def test_ids_of_no_expert_add_nothing(rk, s, kind):
+def test_ids_of_no_expert_add_nothing(rk, tiles, s, kind):
     note(f"routed no expert s={s} {kind}")
     r = np.random.default_rng(s)
     e, k, h, i = 6, 4, 96, 64
@@ -328,7 +335,7 @@ EXPERTS = [(1, 5, 3, 144, 80), (2, 4, 1, 16, 16), (33, 4, 2, 256, 272), (70, 8, 
 
 @pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
 @pytest.mark.parametrize("s,e,k,h,i", EXPERTS)
-def test_fp8_experts(rk, s, e, k, h, i, dtype):
+def test_fp8_experts(rk, tiles, s, e, k, h, i, dtype):
     note(f"fp8 experts s={s} e={e} k={k} h={h} i={i} {dtype}")
     lib, r = rk.lib(), np.random.default_rng(s + h)
     stack = [ref.random_stack(r, e, n, kk) for n, kk in ((i, h), (i, h), (h, i))]
@@ -372,7 +379,7 @@ def test_bounds_of_the_expert_tests_are_tight(dtype, by):
 
 @pytest.mark.parametrize("router", [dict(), dict(score=1, bias=True, n_groups=4, top_groups=2, scale=2.5)])
 @pytest.mark.parametrize("s", [1, 50])
-def test_a_routed_layer(rk, s, router):
+def test_a_routed_layer(rk, tiles, s, router):
     """Logits to the layer's output: router, lists and experts one behind the other."""
     note(f"routed layer s={s} {router}")
     r = np.random.default_rng(s)
@@ -390,7 +397,7 @@ def test_a_routed_layer(rk, s, router):
     assert (np.abs(got - want) <= most * 1.001 + np.abs(want) * (ref.HALF["bf16"] * 1.001 + 40 * 2.0**-24)).all()
 
 
-def test_a_captured_layer_replays_on_new_inputs(rk):
+def test_a_captured_layer_replays_on_new_inputs(rk, tiles):
     """Router, lists and experts in one graph, replayed on new logits and rows with eager work on the plan in between."""
     note("routed layer, captured")
     from test_gpu_sequences import Graph
