@@ -79,29 +79,41 @@ struct Fp8Frag<true> {
     widen(4 * s + 3, j1[2], j1[3]);
   }
 };
-// The 32 × 32 product of two blocks' codes: rows 8·(r/4) + 4·(lane/32) + r%4 of `a` in register r, column lane%32 of `b`.
+// The 32 × 32 product of two blocks' codes, by halves of the block: rows 8·(r/4) + 4·(lane/32) + r%4 of `a` in register r, column lane%32 of `b`.
 // With the weight as `a` a lane holds one token's results for 16 outputs: one scale of its own, and one of the weight that
 // is the same for all.
-__device__ __forceinline__ floatx16 fp8_product(const Fp8Frag<false> &a, const Fp8Frag<false> &b) {
-  const floatx16 p = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a.f[0], b.f[0], floatx16{}, 0, 0, 0, 0, 0, 0);
-  return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a.f[1], b.f[1], p, 0, 0, 0, 0, 0, 0);
+__device__ __forceinline__ floatx16 fp8_half(const Fp8Frag<false> &a, const Fp8Frag<false> &b, int s, floatx16 p) {
+  return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a.f[s], b.f[s], p, 0, 0, 0, 0, 0, 0);
 }
-__device__ __forceinline__ floatx16 fp8_product(const Fp8Frag<true> &a, const Fp8Frag<true> &b) {
-  floatx16 p = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.f[0], b.f[0], floatx16{}, 0, 0, 0);
+__device__ __forceinline__ floatx16 fp8_half(const Fp8Frag<true> &a, const Fp8Frag<true> &b, int s, floatx16 p) {
 #pragma unroll
-  for (int i = 1; i < 8; ++i) p = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.f[i], b.f[i], p, 0, 0, 0);
+  for (int i = 0; i < 4; ++i) p = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.f[4 * s + i], b.f[4 * s + i], p, 0, 0, 0);
   return p;
+}
+template <bool EXACT>
+__device__ __forceinline__ floatx16 fp8_product(const Fp8Frag<EXACT> &a, const Fp8Frag<EXACT> &b) {
+  return fp8_half(a, b, 1, fp8_half(a, b, 0, floatx16{}));
 }
 
 // silu(g) · u in f32: g / (1 + e^-g) · u.
 __device__ __forceinline__ float fp8_silu_mul(float g, float u) { return g / (1.0f + expf(-g)) * u; }
 
+// Four f32 values to a type's bits, by the conversion instructions (nearest even; a NaN stays one).
+template <int DT>
+__device__ __forceinline__ void fp8_encode4(void *to, const float *v) {
+  if constexpr (DT == RK_DTYPE_BF16) {
+    typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+    *(bf16x4 *)to = bf16x4{(__bf16)v[0], (__bf16)v[1], (__bf16)v[2], (__bf16)v[3]};
+  } else {
+    dt_store_vec<DT, 4>(to, 0, v);
+  }
+}
 // Four consecutive values of a row of c (element type known at run time), `n` of them inside the row.
 __device__ __forceinline__ void fp8_store4(void *c, int dt, int64_t at, const float *v, int n, bool whole) {
   if (whole && n >= 4) {
     if (dt == RK_DTYPE_F32) dt_store_vec<RK_DTYPE_F32, 4>(c, at, v);
     else if (dt == RK_DTYPE_F16) dt_store_vec<RK_DTYPE_F16, 4>(c, at, v);
-    else dt_store_vec<RK_DTYPE_BF16, 4>(c, at, v);
+    else fp8_encode4<RK_DTYPE_BF16>((uint16_t *)c + at, v);
     return;
   }
 #pragma unroll

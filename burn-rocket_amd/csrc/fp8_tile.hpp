@@ -3,12 +3,25 @@
 
 #include "fp8.hpp"
 
+// The thread's index as a new value: what an epilogue computes from it is not kept in registers through the K loop.
+__device__ __forceinline__ int fresh_tid() {
+  int t = threadIdx.x;
+  asm volatile("" : "+v"(t));
+  return t;
+}
+
 // A workgroup takes BM rows × BN outputs and walks K in stages of 128, one block of both scales a stage. LDS slots are
 // filled by buffer→LDS copies a stage ahead: weights in the resident layout as they lie (a fragment is 1 KB in one piece,
 // free of bank conflicts), rows of activations with 16-byte chunk c of row r at c ^ ((r >> 1) & 7), and the rows' scales of
-// the stage behind them. The weight is the first operand, so that a lane holds 16 outputs of one row: a fold is one product
-// of two scales and 16 FMAs per 32 × 32 tile and stage, 64 cycles of the VALU for 128 of the matrix unit. Each tile's fold
-// is issued behind the next tile's products, so that the two units run side by side.
+// the stage and the blocks' behind them. The weight is the first operand, so that a lane holds 16 outputs of one row: a fold
+// is one product of two scales and 16 FMAs per 32 × 32 tile and stage, 64 cycles of the VALU for 128 of the matrix unit;
+// a SIMD's other wave has the matrix unit meanwhile. The barrier of a stage stands before its last row of tiles: by then its
+// fragments are in registers, so its slot is refilled and the next stage's first fragments are read under that row's
+// products.
+//
+// 16000 × 4096 × 4096 on MI355X, 256 × 256: 244 us, 2.2 PFLOP/s. Without the folds as much, without the copies 214, without
+// these and the stores 197. Tried: folds a tile behind in a second set of product registers (spills; 302 with fewer other
+// registers kept); the copies in one go behind the barrier (274) or all in the last row (265).
 template <int BM_, int BN_, int WM_, int WN_, int STAGES_, bool EXACT_>
 struct Fp8Tile {
   static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, STAGES = STAGES_;
@@ -17,120 +30,199 @@ struct Fp8Tile {
   static constexpr int WTM = BM / WM, WTN = BN / WN, TM = WTM / 32, TN = WTN / 32;
   static constexpr int QA = BM / 8, QB = BN / 8;  // 1 KB copies of a stage
   static constexpr int CA = QA / NW, CB = QB / NW, SI = BM / 64;  // per wave; copies of 64 row scales
-  static constexpr int SLOT = (BM + BN) * 128 + BM * 4;
+  static constexpr int WS_AT = (BM + BN) * 128 + BM * 4;  // the weight blocks' scales, [BN / 32]
+  static constexpr int SLOT = WS_AT + 256;
   static constexpr int SMEM = STAGES * SLOT;
   static_assert(SMEM <= 160 * 1024, "LDS per workgroup");
-  static_assert(CA * NW == QA && CB * NW == QB && SI <= NW && SI * 64 == BM, "copies per wave");
-  static_assert((TN * TM) % 2 == 0, "the two product registers alternate over stages too");
+  static_assert(CA * NW == QA && CB * NW == QB && SI < NW && SI * 64 == BM, "copies per wave");
+  static_assert((TN * TM) % 2 == 0 && TN % 2 == 0, "the two product registers and the two weight fragments alternate over stages too");
+  static_assert(STAGES == 2, "the slot of a stage is refilled for the one after the next");
 
   floatx16 acc[TN][TM];  // outputs 32·i + 8·(r/4) + 4·(lane/32) + r%4 of row 32·j + lane%32 of the wave's part
 
   // a: codes, rows k bytes apart, a_bytes in all from a; as: scales, rows KT apart. row_of(r): row of `a` for row r of the
-  // tile, or -1 (reads zeros). w: the first of the tile's weight blocks, w_bytes in all; ws(i): scales of the wave's block i.
-  // rows: of the tile (a wave without any only copies).
+  // tile, or -1 (reads zeros). w: the tile's weight blocks, as many as there are (a block past them
+  // reads the last one: its results are not stored); ws_of(i): of the scales `ws` (ws_bytes), the first one of the
+  // workgroup's block i. rows: of the tile (a wave without any only copies).
   template <typename RowOf, typename Scales>
   __device__ __forceinline__ void run(uint8_t *smem, const uint8_t *a, int64_t a_bytes, const float *as, int64_t as_bytes,
-                                      RowOf row_of, int rows, const uint8_t *w, int64_t w_bytes, Scales ws_of, int k, int KT) {
+                                      RowOf row_of, int rows, const uint8_t *w, int blocks, const float *ws, int64_t ws_bytes,
+                                      Scales ws_of, int k, int KT) {
     const int lane = lane_id(), col = lane & 31, h = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wm = wave / WN, wn = wave % WN;
-    const rsrc_t ra = make_rsrc(a, a_bytes), rs = make_rsrc(as, as_bytes), rw = make_rsrc(w, w_bytes);
-    // Whole offsets go into the vector part of a copy's address: that is what the range check sees.
+    const rsrc_t ra = make_rsrc(a, a_bytes), rw = make_rsrc(w, (int64_t)min(blocks, BN / 32) * KT * 4096);
+    // Rows past the tile's and lanes past K have vector offsets that every range check refuses; what the scalar part adds
+    // to the others stays inside a row, or inside the weight's blocks.
     const int r8 = lane >> 3, p8 = lane & 7;
-    uint32_t off[CA], ch[CA];
+    static_assert(NW % 2 == 0, "a wave's copies share their chunks' order");
+    const uint32_t ch = (uint32_t)((p8 ^ (((wave * 8 + r8) >> 1) & 7)) << 4);
+    uint32_t off[CA];
 #pragma unroll
     for (int i = 0; i < CA; ++i) {
-      const int r = (wave + i * NW) * 8 + r8;
-      const int64_t src = row_of(r);
-      ch[i] = (uint32_t)((p8 ^ ((r >> 1) & 7)) << 4);
-      off[i] = src < 0 ? OOB_OFFSET : (uint32_t)(src * k) + ch[i];
+      const int64_t src = row_of((wave + i * NW) * 8 + r8);
+      off[i] = src < 0 ? OOB_OFFSET : (uint32_t)(src * k) + ch;
     }
+    // One copy of scales a wave: of 64 rows, or (all others, to the same place) of the weight blocks.
+    const bool row_scales = wave < SI;
+    const rsrc_t rsc = row_scales ? make_rsrc(as, as_bytes) : make_rsrc(ws, ws_bytes);
+    const int sc_at = row_scales ? (QA + QB) * 1024 + wave * 256 : WS_AT;
     uint32_t soff = OOB_OFFSET;
-    if (wave < SI) {
+    if (row_scales) {
       const int64_t src = row_of(wave * 64 + lane);
       if (src >= 0) soff = (uint32_t)(src * KT * 4);
+    } else if (lane < BN / 32) {
+      soff = (uint32_t)(ws_of(lane) * 4);
     }
-    auto issue = [&](int slot, int kt) {
+    // Copies [FROM, TO) of a stage.
+    constexpr int CP = CA + CB + 1;
+    auto issue = [&](auto from_c, auto to_c, int slot, int kt) {
       uint8_t *sb = smem + slot * SLOT;
       const uint32_t k0 = (uint32_t)kt * 128;
-#pragma unroll
-      for (int i = 0; i < CA; ++i)
-        bdma16(ra, sb + (wave + i * NW) * 1024, k0 + ch[i] < (uint32_t)k ? off[i] + k0 : OOB_OFFSET, 0);
-#pragma unroll
-      for (int i = 0; i < CB; ++i) {
-        const int q = wave + i * NW;
-        bdma16(rw, sb + (QA + q) * 1024, lane * 16 + (uint32_t)(((q >> 2) * KT + kt) * 4096 + (q & 3) * 1024), 0);
-      }
-      if (wave < SI)
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, LDS_PTR(sb + (QA + QB) * 1024 + wave * 256), 4, soff + kt * 4, 0, 0, 0);
+      static_for<decltype(to_c)::value - decltype(from_c)::value>([&](auto c_c) {
+        constexpr int c = decltype(c_c)::value + decltype(from_c)::value;
+        if constexpr (c < CA) {
+          bdma16(ra, sb + (wave + c * NW) * 1024, k0 + ch < (uint32_t)k ? off[c] : OOB_OFFSET, k0);
+        } else if constexpr (c < CA + CB) {
+          const int q = wave + (c - CA) * NW;
+          bdma16(rw, sb + (QA + q) * 1024, lane * 16, (uint32_t)((min(q >> 2, blocks - 1) * KT + kt) * 4096 + (q & 3) * 1024));
+        } else {
+          __builtin_amdgcn_raw_ptr_buffer_load_lds(rsc, LDS_PTR(sb + sc_at), 4, soff, kt * 4, 0, 0);
+        }
+      });
+    };
+    // A stage's copies are dealt out over the tiles behind the barrier that frees their slot: the last row of tiles, and the
+    // next stage's first one if that leaves them a row's time to arrive. In one go they hold the waves up for a fifth of a
+    // stage (72 copies of 64 lanes through one address unit).
+    constexpr int SPREAD = TN > 2 ? 2 * TM : TM, QUOTA = (CP + SPREAD - 1) / SPREAD;
+    auto issue_at = [&](auto step_c, int slot, int kt) {
+      constexpr int f = decltype(step_c)::value * QUOTA, t = f + QUOTA;
+      if constexpr (decltype(step_c)::value < SPREAD && f < CP) issue(ic<f>{}, ic<(t < CP ? t : CP)>{}, slot, kt);
     };
 
     // A lane's fragment bytes: the row's chunks 4s + 2h + j, swizzled; the weight block's pieces.
     const int swz = (col >> 1) & 7;
-    uint32_t a_off[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      a_off[i] = (uint32_t)((wm * WTM + col) * 128 + (((4 * (i >> 1) + 2 * h + (i & 1)) ^ swz) << 4));
+    const uint32_t a_off = (uint32_t)((wm * WTM + col) * 128 + (((2 * h) ^ swz) << 4));  // (chunk bits 0 and 2: ^ 16, ^ 64)
     const uint32_t w_off = (uint32_t)(BM * 128 + wn * WTN * 128 + lane * 16);
     const uint32_t s_off = (uint32_t)((QA + QB) * 1024 + (wm * WTM + col) * 4);
-    const float *ws[TN];
-#pragma unroll
-    for (int i = 0; i < TN; ++i) ws[i] = ws_of(wn * TN + i);
 
-    floatx16 part[2];
 #pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      part[1][r] = 0.f;
+    for (int r = 0; r < 16; ++r)
 #pragma unroll
       for (int i = 0; i < TN; ++i)
 #pragma unroll
         for (int j = 0; j < TM; ++j) acc[i][j][r] = 0.f;
-    }
-    float pend = 0.f;  // scale of the tile whose fold is due
-    auto load_w = [&](Fp8Frag<EXACT> &f, const uint8_t *sb, int i) {
-      const uint8_t *p = sb + w_off + i * 4096;
+    Fp8Frag<EXACT> x[TM], wf[2];
+    float sa[TM], sw[TN];
+    auto load_w = [&](Fp8Frag<EXACT> &f, int slot, int i) {
+      const uint8_t *p = smem + slot * SLOT + w_off + i * 4096;
       f.set(0, *(const intx4 *)p, *(const intx4 *)(p + 1024));
       f.set(1, *(const intx4 *)(p + 2048), *(const intx4 *)(p + 3072));
     };
-    auto stage = [&](int slot, int kt) {
-      const uint8_t *sb = smem + slot * SLOT;
-      Fp8Frag<EXACT> x[TM], wf[2];
-      float sa[TM], sw[TN];
-#pragma unroll
-      for (int i = 0; i < TN; ++i) sw[i] = ws[i][kt];
-      load_w(wf[0], sb, 0);
-#pragma unroll
-      for (int j = 0; j < TM; ++j) {
-        const uint8_t *p = sb + j * 32 * 128;
-        x[j].set(0, *(const intx4 *)(p + a_off[0]), *(const intx4 *)(p + a_off[1]));
-        x[j].set(1, *(const intx4 *)(p + a_off[2]), *(const intx4 *)(p + a_off[3]));
-        sa[j] = *(const float *)(sb + s_off + j * 128);
-      }
-      static_for<TN>([&](auto i_c) {
-        constexpr int i = decltype(i_c)::value;
-        if constexpr (i + 1 < TN) load_w(wf[(i + 1) & 1], sb, i + 1);
-        static_for<TM>([&](auto j_c) {
-          constexpr int j = decltype(j_c)::value, u = i * TM + j, prev = (u + TN * TM - 1) % (TN * TM);
-          part[u & 1] = fp8_product(wf[i & 1], x[j]);
-          __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-          for (int r = 0; r < 16; ++r)
-            acc[prev / TM][prev % TM][r] = __builtin_fmaf(part[(u & 1) ^ 1][r], pend, acc[prev / TM][prev % TM][r]);
-          pend = sa[j] * sw[i];
-          __builtin_amdgcn_sched_barrier(0);
-        });
-      });
+    auto load_x = [&](int slot, int j) {
+      const uint8_t *p = smem + slot * SLOT + j * 32 * 128;
+      x[j].set(0, *(const intx4 *)(p + a_off), *(const intx4 *)(p + (a_off ^ 16)));
+      x[j].set(1, *(const intx4 *)(p + (a_off ^ 64)), *(const intx4 *)(p + (a_off ^ 80)));
     };
-    issue(0, 0);
-    for (int kt = 0; kt < KT; ++kt) {
+    // (the scales of the last row of tiles are used up before the next stage's are read)
+    auto load_s = [&](int slot) {
+#pragma unroll
+      for (int j = 0; j < TM; ++j) sa[j] = *(const float *)(smem + slot * SLOT + s_off + j * 128);
+#pragma unroll
+      for (int i = 0; i < TN; ++i) sw[i] = *(const float *)(smem + slot * SLOT + WS_AT + (wn * TN + i) * 4);
+    };
+    auto tile = [&](auto i_c, auto j_c) {
+      constexpr int i = decltype(i_c)::value, j = decltype(j_c)::value;
+      const floatx16 p = fp8_half(wf[i & 1], x[j], 1, fp8_half(wf[i & 1], x[j], 0, floatx16{}));
+      const float sc = sa[j] * sw[i];
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[i][j][r] = __builtin_fmaf(p[r], sc, acc[i][j][r]);
+      __builtin_amdgcn_sched_barrier(0);
+    };
+    auto arrived = [&] {
       WAIT_VMCNT(0);
       WAIT_LGKMCNT0();
       BARRIER();
-      if (kt + 1 < KT) issue((kt + 1) % STAGES, kt + 1);
-      if (wm * WTM < rows) stage(kt % STAGES, kt);
-    }
-    constexpr int last = TN * TM - 1;
+    };
+    issue(ic<0>{}, ic<CP>{}, 0, 0);
+    arrived();
+    if (wm * WTM >= rows) {  // a wave without rows copies for the others
+      for (int kt = 1; kt < KT; ++kt) {
+        issue(ic<0>{}, ic<CP>{}, kt & 1, kt);
+        arrived();
+      }
+    } else {
+      load_w(wf[0], 0, 0);
 #pragma unroll
-    for (int r = 0; r < 16; ++r) acc[TN - 1][TM - 1][r] = __builtin_fmaf(part[last & 1][r], pend, acc[TN - 1][TM - 1][r]);
+      for (int j = 0; j < TM; ++j) load_x(0, j);
+      load_s(0);
+      if (KT > 1) static_for<TM>([&](auto j_c) { issue_at(j_c, 1, 1); });
+      // more: a stage follows; most: one behind it too (no branches in the steady state)
+      auto stage = [&](int kt, auto more_c, auto most_c) {
+        constexpr bool more = decltype(more_c)::value, most = decltype(most_c)::value;
+        const int slot = kt & 1, next = slot ^ 1;
+        static_for<TN - 1>([&](auto i_c) {
+          load_w(wf[(decltype(i_c)::value + 1) & 1], slot, decltype(i_c)::value + 1);
+          static_for<TM>([&](auto j_c) {
+            tile(i_c, j_c);
+            if constexpr (more && decltype(i_c)::value == 0) issue_at(ic<TM + decltype(j_c)::value>{}, next, kt + 1);
+          });
+        });
+        if constexpr (more) {
+          arrived();
+          load_w(wf[0], next, 0);
+        }
+        static_for<TM>([&](auto j_c) {
+          tile(ic<TN - 1>{}, j_c);
+          if constexpr (most) issue_at(j_c, slot, kt + 2);
+          if constexpr (more) load_x(next, decltype(j_c)::value);
+        });
+        if constexpr (more) load_s(next);
+      };
+      for (int kt = 0; kt + 2 < KT; ++kt) stage(kt, ic<1>{}, ic<1>{});
+      if (KT > 1) stage(KT - 2, ic<1>{}, ic<0>{});
+      stage(KT - 1, ic<0>{}, ic<0>{});
+    }
+    __syncthreads();  // the slots may be used for something else
+  }
+
+  // The tile's results to rows of a matrix through LDS, so that a wave stores whole pieces of a row (its lanes hold four
+  // outputs of 32 rows each: 16-byte pieces of 32 lines, which cost a third of the vision layer's 4304 × 1152 product).
+  // value(i, j, r): the lane's result; to: the tile's first row, ld values apart; n: outputs from the tile's first on.
+  // Chunk c of 16 bytes of row r lies at c ^ (r mod 32) (16 of a narrow row): the rows that a store writes are on different banks.
+  template <int DT, typename Value>
+  __device__ __forceinline__ void store(uint8_t *smem, Value value, void *to, int64_t ld, int rows, int n) {
+    constexpr int ES = DT == RK_DTYPE_F32 ? 4 : 2, V = 16 / ES;  // values of a chunk
+    constexpr int ROWB = BN * ES, CH = ROWB / 16;                 // a row's bytes and chunks
+    constexpr int SW = CH < 32 ? CH - 1 : 31;
+    static_assert(BM * ROWB <= SMEM && (CH & (CH - 1)) == 0 && NT % CH == 0, "the tile in LDS");
+    const int tid = fresh_tid(), col = tid & 31, h = (tid >> 5) & 1;
+    const int wave = tid >> 6, wm = wave / WN, wn = wave % WN;
+#pragma unroll
+    for (int j = 0; j < TM; ++j)
+#pragma unroll
+      for (int i = 0; i < TN; ++i)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const float v[4] = {value(i, j, 4 * q), value(i, j, 4 * q + 1), value(i, j, 4 * q + 2), value(i, j, 4 * q + 3)};
+          const int r = wm * WTM + j * 32 + col, at = wn * WTN + i * 32 + q * 8 + h * 4;
+          fp8_encode4<DT>(smem + r * ROWB + (((at / V) ^ (r & SW)) * 16) + at % V * ES, v);
+        }
+    __syncthreads();
+    const int c = tid % CH, left = n - c * V;
+    if (left <= 0) return;
+    const bool whole = ld * ES % 16 == 0 && left >= V;
+    for (int r = tid / CH; r < rows; r += NT / CH) {
+      const uint8_t *p = smem + r * ROWB + ((c ^ (r & SW)) * 16);
+      uint8_t *o = (uint8_t *)to + (r * ld + c * V) * ES;
+      if (whole) {
+        *(uintx4 *)o = *(const uintx4 *)p;
+      } else {
+#pragma unroll
+        for (int e = 0; e < V; ++e)
+          if (e < left) ((dt_storage<DT> *)o)[e] = ((const dt_storage<DT> *)p)[e];
+      }
+    }
   }
 };

@@ -16,27 +16,19 @@ __global__ __launch_bounds__(T::NT, 2) void gemm_fp8_kernel(const Fp8GemmArgs g,
   const int n0 = tn * T::BN, KT = g.kt;
   const int64_t left = g.m - m0;
   const int rows = (int)min<int64_t>(left, T::BM);
-  const int nblk = (g.n + 127) / 128 * 4;  // (rows of the layout end on a multiple of 128: blocks past it read zeros)
+  const int nblk = (g.n + 127) / 128 * 4;
   T t;
   t.run(smem, g.a + m0 * g.k, left * g.k, g.as + m0 * KT, left * KT * 4, [&](int r) -> int64_t { return r < rows ? r : -1; }, rows,
-        g.w + (int64_t)(n0 / 32) * KT * 4096, (int64_t)(nblk - n0 / 32) * KT * 4096,
-        [&](int b) { return g.ws + (int64_t)min((n0 / 32 + b) / 4, nblk / 4 - 1) * KT; }, g.k, KT);
+        g.w + (int64_t)(n0 / 32) * KT * 4096, nblk - n0 / 32,
+        g.ws, (int64_t)(nblk / 4) * KT * 4, [&](int b) { return (int64_t)min((n0 / 32 + b) / 4, nblk / 4 - 1) * KT; }, g.k, KT);
 
-  const int lane = lane_id(), col = lane & 31, h = lane >> 5;
-  const int wave = threadIdx.x >> 6, wm = wave / T::WN, wn = wave % T::WN;
-  const bool whole = (g.n & 3) == 0;
-#pragma unroll
-  for (int j = 0; j < T::TM; ++j) {
-    const int r = wm * T::WTM + j * 32 + col;
-    if (r >= rows) continue;
-#pragma unroll
-    for (int i = 0; i < T::TN; ++i)
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const int n = n0 + wn * T::WTN + i * 32 + q * 8 + h * 4;
-        const float v[4] = {t.acc[i][j][4 * q], t.acc[i][j][4 * q + 1], t.acc[i][j][4 * q + 2], t.acc[i][j][4 * q + 3]};
-        fp8_store4(g.c, g.c_dtype, (m0 + r) * g.n + n, v, g.n - n, whole);
-      }
+  const auto value = [&](int i, int j, int r) { return t.acc[i][j][r]; };
+  const auto out = [&](int es) { return (uint8_t *)g.c + (m0 * g.n + n0) * es; };
+  if constexpr (T::EXACT) {
+    t.template store<RK_DTYPE_F32>(smem, value, out(4), g.n, rows, g.n - n0);
+  } else {
+    if (g.c_dtype == RK_DTYPE_F16) t.template store<RK_DTYPE_F16>(smem, value, out(2), g.n, rows, g.n - n0);
+    else t.template store<RK_DTYPE_BF16>(smem, value, out(2), g.n, rows, g.n - n0);
   }
 }
 
@@ -54,7 +46,9 @@ static hipError_t launch_fp8(const Fp8GemmArgs &g, hipStream_t st) {
   return hipGetLastError();
 }
 
+// exact: c f32; otherwise fp16 or bf16.
 hipError_t rk_launch_gemm_fp8(const Fp8GemmArgs &g, bool exact, hipStream_t st) {
+  if (exact != (g.c_dtype == RK_DTYPE_F32)) return hipErrorInvalidValue;
   if (exact) return launch_fp8<Fp8Tile<128, 128, 2, 2, 2, true>>(g, st);
   const int64_t big = (int64_t)((g.m + 255) / 256) * ((g.n + 255) / 256);
   if (big >= g.num_cus) return launch_fp8<Fp8Tile<256, 256, 4, 2, 2, false>>(g, st);

@@ -32,20 +32,19 @@ __global__ __launch_bounds__(T::NT, 2) void moe_fp8_gate_up_kernel(const Fp8MoeA
   const int KT = g.kt, ib = (g.n + 127) / 128;
   if (!moe_fp8_place(g, T::BM, ib, tile, nc)) return;
   const uint8_t *w = g.w + (int64_t)tile.expert * g.w_stride + (int64_t)nc * 8 * KT * 4096;
-  const float *ws = g.ws + (int64_t)tile.expert * 2 * ib * KT + (int64_t)nc * KT;
+  const float *ws = g.ws + (int64_t)tile.expert * 2 * ib * KT;
   T t;
   t.run(smem, g.a, (int64_t)g.n_tok * g.k, g.as, (int64_t)g.n_tok * KT * 4,
-        [&](int r) -> int64_t { return r < tile.rows ? (int64_t)g.tok[tile.row0 + r] : -1; }, tile.rows, w, (int64_t)8 * KT * 4096,
-        [&](int b) { return ws + (b & 1) * (int64_t)ib * KT; }, g.k, KT);
+        [&](int r) -> int64_t { return r < tile.rows ? (int64_t)g.tok[tile.row0 + r] : -1; }, tile.rows, w, 8, ws,
+        (int64_t)2 * ib * KT * 4, [&](int b) { return (int64_t)((b & 1) * ib + nc) * KT; }, g.k, KT);
 
   // act in place of the gate; the largest of a row's 128 over the lane's two halves and the workgroup's waves.
-  const int lane = lane_id(), col = lane & 31, h = lane >> 5;
-  const int wave = threadIdx.x >> 6, wm = wave / T::WN, wn = wave % T::WN;
+  const int tid = fresh_tid(), col = tid & 31, h = (tid >> 5) & 1;
+  const int wave = tid >> 6, wm = wave / T::WN, wn = wave % T::WN;
   float *s_max = (float *)smem;                                         // [WN][BM]
   uint8_t *s_out = smem + T::WN * T::BM * 4;                            // [BM][144]: a row's codes
   constexpr int ROW = 144;
   static_assert(T::WN * T::BM * 4 + T::BM * ROW <= T::SMEM, "epilogue LDS");
-  __syncthreads();
   float amax[T::TM];
 #pragma unroll
   for (int j = 0; j < T::TM; ++j) {
@@ -81,7 +80,7 @@ __global__ __launch_bounds__(T::NT, 2) void moe_fp8_gate_up_kernel(const Fp8MoeA
     if (wn == 0 && h == 0 && r < tile.rows) g.out_s[((int64_t)tile.row0 + r) * ib + nc] = s;
   }
   __syncthreads();
-  for (int c = threadIdx.x; c < tile.rows * 8; c += T::NT) {
+  for (int c = tid; c < tile.rows * 8; c += T::NT) {
     const int r = c >> 3, at = (c & 7) * 16;
     *(uintx4 *)((uint8_t *)g.out + ((int64_t)tile.row0 + r) * ib * 128 + nc * 128 + at) = *(const uintx4 *)(s_out + r * ROW + at);
   }
@@ -99,9 +98,9 @@ __global__ __launch_bounds__(T::NT, 2) void moe_fp8_down_kernel(const Fp8MoeArgs
   T t;
   t.run(smem, g.a + (int64_t)tile.row0 * KT * 128, (int64_t)tile.rows * KT * 128, g.as + (int64_t)tile.row0 * KT, (int64_t)tile.rows * KT * 4,
         [&](int r) -> int64_t { return r < tile.rows ? r : -1; }, tile.rows, g.w + (int64_t)tile.expert * g.w_stride + (int64_t)nb0 * KT * 4096,
-        (int64_t)(nblk - nb0) * KT * 4096, [&](int b) { return ws + (int64_t)min((nb0 + b) / 4, nblk / 4 - 1) * KT; }, KT * 128, KT);
-  const int lane = lane_id(), col = lane & 31, h = lane >> 5;
-  const int wave = threadIdx.x >> 6, wm = wave / T::WN, wn = wave % T::WN;
+        nblk - nb0, ws, (int64_t)(nblk / 4) * KT * 4, [&](int b) { return (int64_t)min((nb0 + b) / 4, nblk / 4 - 1) * KT; }, KT * 128, KT);
+  const int tid = fresh_tid(), col = tid & 31, h = (tid >> 5) & 1;
+  const int wave = tid >> 6, wm = wave / T::WN, wn = wave % T::WN;
 #pragma unroll
   for (int j = 0; j < T::TM; ++j) {
     const int r = wm * T::WTM + j * 32 + col;
