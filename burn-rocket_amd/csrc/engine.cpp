@@ -2135,7 +2135,7 @@ std::vector<std::pair<const char *, size_t>> moe_buffers(const Weight &w, int64_
   if (w.moe_fp8) {
     const size_t kh = (H + 127) / 128, ki = (I + 127) / 128, few = std::min(R, (size_t)moe_fp8_few_limit(w));
     return {{"moe_xq", S * H}, {"moe_xs", S * kh * 4}, {"moe_act", std::max(few * I * 4, R * ki * 128)}, {"moe_as", R * ki * 4},
-            {"moe_yb", R * H * 4}};
+            {"moe_yb", R * H * 4}, {"moe_ys", R * ((H + 63) / 64) * 4}};
   }
   return {{"moe_xq", S * H},       {"moe_xs", S * (H / 32) * 4}, {"moe_act", R * I * 4}, {"moe_aq", R * I},
           {"moe_as", R * (I / 32) * 4}, {"moe_yb", R * H * 4},        {"moe_cnt", S * ((H + 127) / 128) * 4}};
@@ -2151,7 +2151,7 @@ int moe_run_fp8(CallScope &cs, const Weight &w, const MoePlan &plan, const void 
   hipStream_t st = cs.st;
   const bool few = plan.tile_rows < 128, exact1 = dtype != RK_DTYPE_BF16, exact2 = dtype == RK_DTYPE_F32;
   const int64_t KTh = w.gu_ws_stride, KTi = w.dn_ws_stride;
-  void *act, *yb;
+  void *act, *yb, *ys = nullptr;
   RK_TRY(moe_buf(cs, plan, "moe_act", few ? (size_t)R * I * 4 : (size_t)R * KTi * 128, &act));
   RK_TRY(moe_buf(cs, plan, "moe_yb", (size_t)R * H * 4, &yb));
   if (few) {
@@ -2223,10 +2223,14 @@ int moe_run_fp8(CallScope &cs, const Weight &w, const MoePlan &plan, const void 
     g.tiles = plan.tiles;
     g.row_w = plan.roww;
     g.out = yb;
+    if (!exact2) RK_TRY(moe_buf(cs, plan, "moe_ys", (size_t)R * ((H + 63) / 64) * 4, &ys));
+    g.out_s = (float *)ys;
     HIP_TRY(rk_launch_moe_fp8_down(g, exact2, st), op);
   }
   CombineArgs c{};
-  c.rows = (const float *)yb;
+  c.rows = yb;
+  c.scales = (const float *)ys;
+  c.group = rk_moe_fp8_down_group(plan.tile_rows);
   c.slot = plan.slot;
   c.n_valid = plan.n_valid;
   c.y = y;

@@ -197,7 +197,7 @@ __global__ __launch_bounds__(FNW * 64, 2) void fp8_few_kernel(const Fp8FewArgs g
     const int n = nb * 32 + q * 8 + (l >> 5) * 4;
     if constexpr (MODE == FEW_GATE_UP) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) v[0][e] = fp8_silu_mul(v[0][e], v[1][e]);
+      for (int e = 0; e < 4; ++e) v[0][e] = fp8_silu_mul<EXACT>(v[0][e], v[1][e]);
     } else if constexpr (MODE == FEW_DOWN) {
       const float rw = g.row_w[row0 + r];
 #pragma unroll

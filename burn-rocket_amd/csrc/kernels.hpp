@@ -363,7 +363,9 @@ struct RouteListArgs {
 int rk_moe_lists_blocks(int64_t rows);
 hipError_t rk_launch_moe_lists(const RouteListArgs &g, hipStream_t st);
 struct CombineArgs {
-  const float *rows;     // [bucket rows, n], weighted
+  const void *rows;      // [bucket rows, n], weighted: f32, or fp16 with a scale per `group` outputs
+  const float *scales;   // [bucket rows, ceil(n / group)], or null: f32 rows
+  int group;
   const int32_t *slot;   // [s, top_k]
   const int32_t *n_valid;  // rows from this one on count for nothing (null: all count)
   void *y;               // [s, n]
@@ -389,10 +391,11 @@ struct Fp8MoeArgs {
   int n_tiles, tile_rows;
   const int32_t *tok;
   const float *row_w;
-  void *out;           // codes [rows, ceil(n/128)·128], or f32 rows [rows, n]
-  float *out_s;        // scales of the codes
+  void *out;           // codes [rows, ceil(n/128)·128]; second product: rows [rows, n], f32 (exact) or fp16
+  float *out_s;        // scales of the codes; of fp16 rows per rk_moe_fp8_down_group(tile_rows) outputs
 };
 hipError_t rk_launch_moe_fp8_gate_up(const Fp8MoeArgs &g, bool exact, hipStream_t st);
+int rk_moe_fp8_down_group(int tile_rows);
 hipError_t rk_launch_moe_fp8_down(const Fp8MoeArgs &g, bool exact, hipStream_t st);
 
 // The static device scratch of rk_attention_dev_noalloc (noalloc.hip):

@@ -5,7 +5,7 @@
 //            and the up value of an output in one lane. A workgroup's 256 weight rows are 128 outputs: a whole block of the
 //            next product's activations, which it quantizes itself. act goes out as codes and scales, a quarter of f32's bytes
 //            and with no pass of its own.
-//   down     bucket rows as they lie, times their router weight, to f32 rows that the combine sums per token.
+//   down     bucket rows as they lie, times their router weight, to rows that the combine sums per token.
 #include "fp8_tile.hpp"
 #include "kernels.hpp"
 
@@ -53,7 +53,7 @@ __global__ __launch_bounds__(T::NT, 2) void moe_fp8_gate_up_kernel(const Fp8MoeA
     for (int p = 0; p < P; ++p)
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
-        const float v = fp8_silu_mul(t.acc[2 * p][j][r], t.acc[2 * p + 1][j][r]);
+        const float v = fp8_silu_mul<T::EXACT>(t.acc[2 * p][j][r], t.acc[2 * p + 1][j][r]);
         t.acc[2 * p][j][r] = v;
         amax[j] = fmaxf(amax[j], fabsf(v));
       }
@@ -99,22 +99,51 @@ __global__ __launch_bounds__(T::NT, 2) void moe_fp8_down_kernel(const Fp8MoeArgs
   t.run(smem, g.a + (int64_t)tile.row0 * KT * 128, (int64_t)tile.rows * KT * 128, g.as + (int64_t)tile.row0 * KT, (int64_t)tile.rows * KT * 4,
         [&](int r) -> int64_t { return r < tile.rows ? r : -1; }, tile.rows, g.w + (int64_t)tile.expert * g.w_stride + (int64_t)nb0 * KT * 4096,
         nblk - nb0, ws, (int64_t)(nblk / 4) * KT * 4, [&](int b) { return (int64_t)min((nb0 + b) / 4, nblk / 4 - 1) * KT; }, KT * 128, KT);
+  // Rows times their router weight: f32, or fp16 under a power of two per row and wave (T::WTN outputs) that takes the
+  // largest to [2^14, 2^15): 2^-12 of a term, under what the sum is rounded to in the end, for half of the bytes that the
+  // combine reads back.
+  float *const to = (float *)g.out + (int64_t)tile.row0 * g.n + n0;
   const int tid = fresh_tid(), col = tid & 31, h = (tid >> 5) & 1;
   const int wave = tid >> 6, wm = wave / T::WN, wn = wave % T::WN;
+  float rw[T::TM];
 #pragma unroll
   for (int j = 0; j < T::TM; ++j) {
     const int r = wm * T::WTM + j * 32 + col;
-    if (r >= tile.rows) continue;
-    const float rw = g.row_w[tile.row0 + r];
-    float *to = (float *)g.out + ((int64_t)tile.row0 + r) * g.n;
+    rw[j] = r < tile.rows ? g.row_w[tile.row0 + r] : 0.f;
+    if constexpr (!T::EXACT) {
+      float amax = 0.f;
 #pragma unroll
-    for (int i = 0; i < T::TN; ++i)
+      for (int i = 0; i < T::TN; ++i)
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const int n = n0 + wn * T::WTN + i * 32 + q * 8 + h * 4;
-        if (n < g.n)  // (a multiple of 16 outputs)
-          *(floatx4 *)(to + n) = floatx4{t.acc[i][j][4 * q] * rw, t.acc[i][j][4 * q + 1] * rw, t.acc[i][j][4 * q + 2] * rw, t.acc[i][j][4 * q + 3] * rw};
-      }
+        for (int e = 0; e < 16; ++e) {
+          t.acc[i][j][e] *= rw[j];
+          amax = fmaxf(amax, fabsf(t.acc[i][j][e]));
+        }
+      amax = fmaxf(amax, __shfl_xor(amax, 32));
+      // exponent of the largest; nothing to scale in rows of zeros, nor by what is infinite
+      const int x = amax > 0.f && amax < INFINITY ? (int)(__float_as_uint(amax) >> 23) - 127 - 14 : 0;
+      rw[j] = ldexpf(1.f, -x);
+      if (h == 0 && r < tile.rows && n0 + wn * T::WTN < g.n)
+        g.out_s[((int64_t)tile.row0 + r) * ((g.n + T::WTN - 1) / T::WTN) + (n0 + wn * T::WTN) / T::WTN] = ldexpf(1.f, x);
+    }
+  }
+  const auto value = [&](int i, int j, int r) { return t.acc[i][j][r] * rw[j]; };
+  if constexpr (!T::EXACT) {
+    t.template store<RK_DTYPE_F16>(smem, value, (uint16_t *)g.out + (int64_t)tile.row0 * g.n + n0, g.n, tile.rows, g.n - n0);
+  } else {
+#pragma unroll
+    for (int j = 0; j < T::TM; ++j) {
+      const int r = wm * T::WTM + j * 32 + col;
+      if (r >= tile.rows) continue;
+#pragma unroll
+      for (int i = 0; i < T::TN; ++i)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int n = wn * T::WTN + i * 32 + q * 8 + h * 4;
+          if (n0 + n < g.n)  // (a multiple of 16 outputs)
+            *(floatx4 *)(to + (int64_t)r * g.n + n) = floatx4{value(i, j, 4 * q), value(i, j, 4 * q + 1), value(i, j, 4 * q + 2), value(i, j, 4 * q + 3)};
+        }
+    }
   }
 }
 
@@ -144,6 +173,8 @@ static hipError_t launch_moe_fp8_any(const Fp8MoeArgs &g, bool exact, hipStream_
 hipError_t rk_launch_moe_fp8_gate_up(const Fp8MoeArgs &g, bool exact, hipStream_t st) {
   return launch_moe_fp8_any<true>(g, exact, st);
 }
+// Outputs under one scale of the second product's fp16 rows.
+int rk_moe_fp8_down_group(int tile_rows) { return tile_rows == 256 ? 128 : 64; }
 hipError_t rk_launch_moe_fp8_down(const Fp8MoeArgs &g, bool exact, hipStream_t st) {
   return launch_moe_fp8_any<false>(g, exact, st);
 }

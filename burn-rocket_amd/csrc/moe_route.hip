@@ -321,29 +321,65 @@ hipError_t rk_launch_moe_lists(const RouteListArgs &g, hipStream_t st) {
 }
 int rk_moe_lists_blocks(int64_t rows) { return (int)((rows + LB - 1) / LB); }
 
-// The weighted rows of each token to its result, in ascending expert id: y (+)= Σ rows. A thread per four values.
-template <int DT>
+// The weighted rows of each token to its result, in ascending expert id: y (+)= Σ rows. A thread per eight values; a
+// token's rows are asked for four at a time. Bound by the rows' bytes.
+template <int DT, bool SCALED>
 __global__ __launch_bounds__(256) void moe_combine_kernel(const CombineArgs g) {
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, per = g.n / 4;
+  constexpr int V = 8;
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, per = g.n / V;
   if (i >= g.s * per) return;
   const int64_t t = i / per;
-  const int c = (int)(i - t * per) * 4;
-  float acc[4] = {0.f, 0.f, 0.f, 0.f};
-  if (g.accumulate) dt_load_vec<DT, 4>(g.y, t * g.n + c, acc);
-  const int valid = g.n_valid ? *g.n_valid : INT_MAX;
-  for (int j = 0; j < g.top_k; ++j) {
-    const int r = g.slot[t * g.top_k + j];
-    if (r >= valid) continue;
-    const floatx4 v = *(const floatx4 *)(g.rows + (int64_t)r * g.n + c);
+  const int c = (int)(i - t * per) * V, groups = SCALED ? (g.n + g.group - 1) / g.group : 0, at = SCALED ? c / g.group : 0;
+  float acc[V];
+  if (g.accumulate) {
+    if constexpr (DT == RK_DTYPE_F32) {
+      dt_load_vec<DT, 4>(g.y, t * g.n + c, acc);
+      dt_load_vec<DT, 4>(g.y, t * g.n + c + 4, acc + 4);
+    } else {
+      dt_load_vec<DT, V>(g.y, t * g.n + c, acc);
+    }
+  } else {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) acc[e] += v[e];
+    for (int e = 0; e < V; ++e) acc[e] = 0.f;
   }
-  dt_store_vec<DT, 4>(g.y, t * g.n + c, acc);
+  const int valid = g.n_valid ? *g.n_valid : INT_MAX;
+  const int32_t *slot = g.slot + t * g.top_k;
+  constexpr int U = 4;
+  for (int j0 = 0; j0 < g.top_k; j0 += U) {
+    float v[U][V], s[U];
+    bool has[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int r = j0 + u < g.top_k ? slot[j0 + u] : INT_MAX;
+      has[u] = r < valid && j0 + u < g.top_k;
+      const int64_t row = has[u] ? r : 0;
+      if constexpr (SCALED) {
+        dt_load_vec<RK_DTYPE_F16, V>(g.rows, row * g.n + c, v[u]);
+        s[u] = g.scales[row * groups + at];
+      } else {
+        dt_load_vec<RK_DTYPE_F32, 4>(g.rows, row * g.n + c, v[u]);
+        dt_load_vec<RK_DTYPE_F32, 4>(g.rows, row * g.n + c + 4, v[u] + 4);
+        s[u] = 1.f;
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (has[u])
+#pragma unroll
+        for (int e = 0; e < V; ++e) acc[e] += v[u][e] * s[u];  // (powers of two: the products are exact)
+  }
+  if constexpr (DT == RK_DTYPE_F32) {
+    dt_store_vec<DT, 4>(g.y, t * g.n + c, acc);
+    dt_store_vec<DT, 4>(g.y, t * g.n + c + 4, acc + 4);
+  } else {
+    dt_store_vec<DT, V>(g.y, t * g.n + c, acc);
+  }
 }
 hipError_t rk_launch_moe_combine(const CombineArgs &g, int dtype, hipStream_t st) {
-  const unsigned grid = (unsigned)((g.s * (g.n / 4) + 255) / 256);
-  auto kern = dtype == RK_DTYPE_F32 ? moe_combine_kernel<RK_DTYPE_F32>
-              : dtype == RK_DTYPE_F16 ? moe_combine_kernel<RK_DTYPE_F16> : moe_combine_kernel<RK_DTYPE_BF16>;
+  const unsigned grid = (unsigned)((g.s * (g.n / 8) + 255) / 256);
+#define RK_COMBINE(DT) (g.scales ? moe_combine_kernel<DT, true> : moe_combine_kernel<DT, false>)
+  auto kern = dtype == RK_DTYPE_F32 ? RK_COMBINE(RK_DTYPE_F32) : dtype == RK_DTYPE_F16 ? RK_COMBINE(RK_DTYPE_F16) : RK_COMBINE(RK_DTYPE_BF16);
+#undef RK_COMBINE
   hipLaunchKernelGGL(kern, dim3(grid), dim3(256), 0, st, g);
   return hipGetLastError();
 }
