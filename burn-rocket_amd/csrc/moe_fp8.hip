@@ -121,7 +121,7 @@ __global__ __launch_bounds__(T::NT, 2) void moe_fp8_down_kernel(const Fp8MoeArgs
         }
       amax = fmaxf(amax, __shfl_xor(amax, 32));
       // exponent of the largest; nothing to scale in rows of zeros, nor by what is infinite
-      const int x = amax > 0.f && amax < INFINITY ? (int)(__float_as_uint(amax) >> 23) - 127 - 14 : 0;
+      const int x = amax > 0.f && amax < INFINITY ? max((int)(__float_as_uint(amax) >> 23) - 127 - 14, -100) : 0;
       rw[j] = ldexpf(1.f, -x);
       if (h == 0 && r < tile.rows && n0 + wn * T::WTN < g.n)
         g.out_s[((int64_t)tile.row0 + r) * ((g.n + T::WTN - 1) / T::WTN) + (n0 + wn * T::WTN) / T::WTN] = ldexpf(1.f, x);

@@ -4,17 +4,73 @@
 #include "kernels.hpp"
 
 // ---------------------------------------------------------------------------
-// Router. A wave per token: expert v·64 + lane in register v of the lane. Choices are compared by the f64 score with its
-// bias, or, where there is none, by the logits themselves, which order the experts as their scores do: of two experts whose
+// Router. A wave per token: expert v·64 + lane in register v of the lane. Choices are those of the f64 scores with their
+// bias, or, where there is none, of the logits themselves, which order the experts as their scores do: of two experts whose
 // f32 scores are a rounding apart the larger is taken, whatever the order of a sum. Equal ones go to the lower id; a NaN
 // ranks with -inf.
+//
+// What bounds it is the picks, one maximum over the wave each: they go by 32-bit keys that order as the floats do (lane
+// exchanges inside the vector instruction, then two ballots' worth of scalar work). With a bias the f32 sums decide wherever
+// neighbours in the order are further apart than the sums can be off; a token where two are not (about one in a thousand) is
+// done again in f64. 16384 tokens, 256 experts, top 8 of 4 groups of 8 on MI355X: ROUTE_US.
 namespace {
+constexpr int ROUTE_WAVES = 4;
+
+// Floats to unsigned numbers in the same order, all above 0; -0 as 0, NaN as -inf.
+__device__ __forceinline__ uint32_t order_key(float x) {
+  if (!(x == x)) x = -INFINITY;
+  const uint32_t u = __float_as_uint(x + 0.f);
+  return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+__device__ __forceinline__ float key_value(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k); }
+
+template <int CTRL>
+__device__ __forceinline__ uint32_t max_dpp(uint32_t x) {
+  return max(x, (uint32_t)__builtin_amdgcn_update_dpp((int)x, (int)x, CTRL, 0xf, 0xf, false));
+}
+// The wave's largest key: lanes 1 and 2 apart, mirrored in 8 and 16, then rows into the next ones.
+__device__ __forceinline__ uint32_t wave_max(uint32_t x) {
+  x = max_dpp<0xB1>(x);
+  x = max_dpp<0x4E>(x);
+  x = max_dpp<0x141>(x);
+  x = max_dpp<0x140>(x);
+  x = max_dpp<0x142>(x);
+  x = max_dpp<0x143>(x);
+  return __builtin_amdgcn_readlane(x, 63);
+}
+
+// Keys of a token's experts (0: not to be chosen), and the picks from them.
+template <int V>
+struct Keys {
+  uint32_t k[V];
+  __device__ __forceinline__ uint32_t best() const {
+    uint32_t m = k[0];
+#pragma unroll
+    for (int v = 1; v < V; ++v) m = max(m, k[v]);
+    return wave_max(m);
+  }
+  // The lowest id with the key m.
+  __device__ __forceinline__ int find(uint32_t m) const {
+    int id = -1;
+#pragma unroll
+    for (int v = V - 1; v >= 0; --v) {
+      const uint64_t has = __ballot(k[v] == m);
+      if (has) id = v * 64 + __builtin_ctzll(has);
+    }
+    return id;
+  }
+  __device__ __forceinline__ void close(int id) {
+#pragma unroll
+    for (int v = 0; v < V; ++v) k[v] = v * 64 + lane_id() == id ? 0u : k[v];
+  }
+};
+
+// f64 form of the choices: (key, id) pairs by lane exchanges.
 struct Choice {
   double key;
   int id;  // INT_MAX: none
 };
 __device__ __forceinline__ bool before(const Choice &a, const Choice &b) { return a.key > b.key || (a.key == b.key && a.id < b.id); }
-// The first of the wave's choices, in all lanes.
 __device__ __forceinline__ Choice wave_first(Choice c) {
 #pragma unroll
   for (int d = 32; d >= 1; d /= 2) {
@@ -23,64 +79,34 @@ __device__ __forceinline__ Choice wave_first(Choice c) {
   }
   return c;
 }
-constexpr int ROUTE_WAVES = 4;
-}  // namespace
 
+// Ids of lane j's choice j, with a bias, in f64. x: the token's logits (what lies past the last expert is not looked at).
 template <int V>
-__global__ __launch_bounds__(ROUTE_WAVES * 64) void moe_route_kernel(const RouteArgs g) {
-  const int lane = lane_id();
-  const int64_t t = (int64_t)blockIdx.x * ROUTE_WAVES + (threadIdx.x >> 6);
-  if (t >= g.s) return;
-  const int E = g.n_experts;
-  float p[V];
-  double key[V];
-  float mx = -INFINITY;
+__device__ __forceinline__ int route_f64(const RouteArgs &g, int64_t t) {
+  const int lane = lane_id(), E = g.n_experts;
+  double key[V], mx = -INFINITY, sum = 0;
 #pragma unroll
   for (int v = 0; v < V; ++v) {
     const int e = v * 64 + lane;
-    p[v] = e < E ? dt_load_any(g.logits, t * E + e, g.dtype) : -INFINITY;
-    key[v] = (double)p[v];
-    mx = fmaxf(mx, p[v]);
+    key[v] = e < E ? (double)dt_load_any(g.logits, t * E + e, g.dtype) : -INFINITY;
+    mx = fmax(mx, key[v]);
   }
-  // Scores, in f32 as the weights are, and in f64 where they are compared.
   if (g.score == RK_ROUTE_SOFTMAX) {
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) mx = fmaxf(mx, __shfl_xor(mx, d));
-    float sum = 0.f;
-    double sum64 = 0;
+    for (int d = 1; d < 64; d *= 2) mx = fmax(mx, __shfl_xor(mx, d));
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-      const bool in = v * 64 + lane < E;
-      if (g.bias) {
-        key[v] = in ? exp(key[v] - (double)mx) : 0;
-        sum64 += key[v];
-      }
-      p[v] = in ? expf(p[v] - mx) : 0.f;
-      sum += p[v];
+      key[v] = v * 64 + lane < E ? exp(key[v] - mx) : 0;
+      sum += key[v];
     }
-#pragma unroll
     for (int d = 1; d < 64; d *= 2) sum += __shfl_xor(sum, d);
-    if (g.bias)
-#pragma unroll
-      for (int d = 1; d < 64; d *= 2) sum64 += __shfl_xor(sum64, d);
-#pragma unroll
-    for (int v = 0; v < V; ++v) {
-      p[v] = p[v] / sum;
-      if (g.bias) key[v] = key[v] / sum64;
-    }
-  } else {
-#pragma unroll
-    for (int v = 0; v < V; ++v) {
-      if (g.bias) key[v] = 1 / (1 + exp(-key[v]));
-      p[v] = 1.0f / (1.0f + expf(-p[v]));
-    }
   }
   unsigned open = 0;  // experts of the lane that may be chosen
 #pragma unroll
   for (int v = 0; v < V; ++v) {
     const int e = v * 64 + lane;
+    key[v] = g.score == RK_ROUTE_SOFTMAX ? key[v] / sum : 1 / (1 + exp(-key[v]));
     if (e < E) {
-      if (g.bias) key[v] += (double)g.bias[e];
+      key[v] += (double)g.bias[e];
       open |= 1u << v;
     }
     if (!(key[v] == key[v])) key[v] = -INFINITY;
@@ -98,15 +124,13 @@ __global__ __launch_bounds__(ROUTE_WAVES * 64) void moe_route_kernel(const Route
   auto close = [&](unsigned &mask, int id) {
     if ((id & 63) == lane) mask &= ~(1u << (id >> 6));
   };
-
-  // Groups: the score of one is its best choice, or with a bias the sum of its two best; experts of the others are closed.
-  if (g.n_groups > 1 && g.top_groups < g.n_groups) {
+  if (g.top_groups < g.n_groups) {
     const int size = E / g.n_groups;
     Choice mine{-INFINITY, INT_MAX};  // lane i: group i
     for (int i = 0; i < g.n_groups; ++i) {
       const Choice a = best_of(i * size, (i + 1) * size, open);
       double s = a.key;
-      if (g.bias && size > 1) {
+      if (size > 1) {
         unsigned rest = open;
         close(rest, a.id);
         s += best_of(i * size, (i + 1) * size, rest).key;
@@ -114,38 +138,140 @@ __global__ __launch_bounds__(ROUTE_WAVES * 64) void moe_route_kernel(const Route
       if (!(s == s)) s = -INFINITY;  // (two infinities)
       if (lane == i) mine = Choice{s, i};
     }
-    unsigned keep = 0;
     uint64_t kept = 0;
     for (int j = 0; j < g.top_groups; ++j) {
       const Choice c = wave_first(mine);
       kept |= (uint64_t)1 << c.id;
       if (lane == c.id) mine = Choice{-INFINITY, INT_MAX};
     }
+    unsigned keep = 0;
 #pragma unroll
     for (int v = 0; v < V; ++v)
       if ((open >> v & 1) && (kept >> ((v * 64 + lane) / size) & 1)) keep |= 1u << v;
     open = keep;
   }
-
-  // The top_k: lane j keeps choice j.
-  float w = 0.f, sum = 0.f;
   int id = 0;
   for (int j = 0; j < g.top_k; ++j) {
     const Choice c = best_of(0, E, open);
     close(open, c.id);
-    float mine = 0.f;
+    if (lane == j) id = c.id;
+  }
+  return id;
+}
+}  // namespace
+
+template <int V, bool BIAS>
+__global__ __launch_bounds__(ROUTE_WAVES * 64) void moe_route_kernel(const RouteArgs g) {
+  const int lane = lane_id();
+  const int64_t t = (int64_t)blockIdx.x * ROUTE_WAVES + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (t >= g.s) return;
+  const int E = g.n_experts;
+  const bool softmax = g.score == RK_ROUTE_SOFTMAX;
+  float x[V], mx = -INFINITY, sum = 1.f;
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    const int e = v * 64 + lane;
+    x[v] = e < E ? dt_load_any(g.logits, t * E + e, g.dtype) : -INFINITY;
+    mx = fmaxf(mx, x[v]);
+  }
+  if (softmax) {
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) mx = fmaxf(mx, __shfl_xor(mx, d));
+    sum = 0.f;
+#pragma unroll
+    for (int v = 0; v < V; ++v) sum += v * 64 + lane < E ? expf(x[v] - mx) : 0.f;
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) sum += __shfl_xor(sum, d);
+  }
+  auto score = [&](float l) { return softmax ? expf(l - mx) / sum : 1.0f / (1.0f + expf(-l)); };
+  Keys<V> keys;
+  float most = 1.f;  // the largest finite |score + bias|, at least 1
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    const int e = v * 64 + lane;
+    float by = x[v];
+    if constexpr (BIAS) {
+      by = score(x[v]) + (e < E ? g.bias[e] : 0.f);
+      if (fabsf(by) < INFINITY) most = fmaxf(most, fabsf(by));
+    }
+    keys.k[v] = e < E ? order_key(by) : 0u;
+  }
+  // A f32 sum is off by a few roundings of the score and one of its own: closer ones than this are not told apart.
+  float near = 0.f;
+  bool unsure = false;
+  if constexpr (BIAS) {
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) most = fmaxf(most, __shfl_xor(most, d));
+    near = most * 0x1p-20f;
+  }
+
+  // Groups: the score of one is its best choice, or with a bias the sum of its two best; experts of the others are closed.
+  if (g.top_groups < g.n_groups) {
+    const int size = E / g.n_groups;
+    uint32_t mine = 0;  // lane i: group i
+    int group[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) group[v] = (v * 64 + lane) / size;
+    for (int i = 0; i < g.n_groups; ++i) {
+      Keys<V> in;
+#pragma unroll
+      for (int v = 0; v < V; ++v) in.k[v] = group[v] == i ? keys.k[v] : 0u;
+      const uint32_t a = in.best();
+      float s = key_value(a);
+      if (BIAS && size > 1) {
+        in.close(in.find(a));
+        s += key_value(in.best());
+      }
+      if (lane == i) mine = order_key(s);
+    }
+    uint64_t kept = 0;
+    float last = 0.f;
+    for (int j = 0; j < g.top_groups + (BIAS ? 1 : 0); ++j) {
+      const uint32_t m = wave_max(mine);
+      if (BIAS && j == g.top_groups) {
+        unsure |= !(last - key_value(m) > 4 * near);
+        break;
+      }
+      const int i = __builtin_ctzll(__ballot(mine == m));
+      kept |= (uint64_t)1 << i;
+      if (lane == i) mine = 0;
+      last = key_value(m);
+    }
 #pragma unroll
     for (int v = 0; v < V; ++v)
-      if (v == (c.id >> 6)) mine = p[v];
-    const float pw = __shfl(mine, c.id & 63);
-    sum += pw;
-    if (lane == j) {
-      w = pw;
-      id = c.id;
+      if (!(kept >> (group[v] & 63) & 1)) keys.k[v] = 0u;
+  }
+
+  // The top_k: lane j keeps choice j. With a bias one more, to see how far the last one is from it.
+  int id = 0;
+  float last = INFINITY;
+  for (int j = 0; j < g.top_k + (BIAS ? 1 : 0); ++j) {
+    const uint32_t m = keys.best();
+    if constexpr (BIAS) {
+      if (j > 0 && m != 0) unsure |= !(last - key_value(m) > 2 * near);
+      last = key_value(m);
+      if (j == g.top_k) break;
     }
+    const int i = keys.find(m);
+    keys.close(i);
+    if (lane == j) id = i;
+  }
+  if (BIAS && unsure) id = route_f64<V>(g, t);
+  // Lane j's logit of its choice.
+  float w = 0.f;
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    const float l = __shfl(x[v], id & 63);
+    if (v == id >> 6) w = l;
+  }
+  w = lane < g.top_k ? score(w) : 0.f;
+  if (g.norm) {
+    float all = w;
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) all += __shfl_xor(all, d);
+    w = w / (all + 1e-20f);
   }
   if (lane < g.top_k) {
-    if (g.norm) w = w / (sum + 1e-20f);
     g.ids[t * g.top_k + lane] = (uint32_t)id;
     g.wts[t * g.top_k + lane] = w * g.scale;
   }
@@ -153,7 +279,9 @@ __global__ __launch_bounds__(ROUTE_WAVES * 64) void moe_route_kernel(const Route
 
 hipError_t rk_launch_moe_route(const RouteArgs &g, hipStream_t st) {
   const int v = (g.n_experts + 63) / 64;
-  auto kern = v <= 1 ? moe_route_kernel<1> : v <= 2 ? moe_route_kernel<2> : v <= 4 ? moe_route_kernel<4> : v <= 8 ? moe_route_kernel<8> : moe_route_kernel<16>;
+#define RK_ROUTE(V) (g.bias ? moe_route_kernel<V, true> : moe_route_kernel<V, false>)
+  auto kern = v <= 1 ? RK_ROUTE(1) : v <= 2 ? RK_ROUTE(2) : v <= 4 ? RK_ROUTE(4) : v <= 8 ? RK_ROUTE(8) : RK_ROUTE(16);
+#undef RK_ROUTE
   hipLaunchKernelGGL(kern, dim3((unsigned)((g.s + ROUTE_WAVES - 1) / ROUTE_WAVES)), dim3(ROUTE_WAVES * 64), 0, st, g);
   return hipGetLastError();
 }
