@@ -346,6 +346,7 @@ struct RouteArgs {
   float scale;
   uint32_t *ids;       // [s, top_k]
   float *wts;
+  int group_size = 0, group_shift = 0;  // set by the launcher
 };
 hipError_t rk_launch_moe_route(const RouteArgs &g, hipStream_t st);
 struct RouteListArgs {

@@ -4,15 +4,15 @@
 #include "kernels.hpp"
 
 // ---------------------------------------------------------------------------
-// Router. A wave per token: expert v·64 + lane in register v of the lane. Choices are those of the f64 scores with their
-// bias, or, where there is none, of the logits themselves, which order the experts as their scores do: of two experts whose
-// f32 scores are a rounding apart the larger is taken, whatever the order of a sum. Equal ones go to the lower id; a NaN
-// ranks with -inf.
+// Router. A wave per token, V consecutive experts a lane. Choices are those of the f64 scores with their bias, or, where
+// there is none, of the logits themselves, which order the experts as their scores do: of two experts whose f32 scores are a
+// rounding apart the larger is taken, whatever the order of a sum. Equal ones go to the lower id; a NaN ranks with -inf.
 //
-// What bounds it is the picks, one maximum over the wave each: they go by 32-bit keys that order as the floats do (lane
-// exchanges inside the vector instruction, then two ballots' worth of scalar work). With a bias the f32 sums decide wherever
-// neighbours in the order are further apart than the sums can be off; a token where two are not (about one in a thousand) is
-// done again in f64. 16384 tokens, 256 experts, top 8 of 4 groups of 8 on MI355X: ROUTE_US.
+// What bounds it is the picks, one maximum over the wave each. They go by 32-bit keys that order as the floats do: each lane
+// sorts its own, so that a pick is a maximum of the lanes' heads (lane exchanges inside the vector instruction), a ballot, and
+// a step of one lane's queue. With a bias the f32 sums decide wherever neighbours in the order are further apart than the
+// sums can be off; a token where two are not (about one in a thousand) is done again in f64. 16384 tokens, 256 experts, top 8
+// of 4 groups of 8 on MI355X: ROUTE_US (52 with a search of all registers per pick and two maxima per group, 95 in f64).
 namespace {
 constexpr int ROUTE_WAVES = 4;
 
@@ -24,247 +24,291 @@ __device__ __forceinline__ uint32_t order_key(float x) {
 }
 __device__ __forceinline__ float key_value(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k); }
 
-template <int CTRL>
-__device__ __forceinline__ uint32_t max_dpp(uint32_t x) {
-  return max(x, (uint32_t)__builtin_amdgcn_update_dpp((int)x, (int)x, CTRL, 0xf, 0xf, false));
+// x of other lanes, inside the vector instruction that uses it (0, which no maximum sees, where there is none): with the
+// neighbour, with the neighbouring pair, mirrored in 8 and in 16 lanes (after the two before them: with the other four, the
+// other eight); the last lane of a row of 16 to the next row, of the first two rows to the last two.
+template <int CTRL, int ROWS = 0xf>
+__device__ __forceinline__ uint32_t dpp(uint32_t x) {
+  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, ROWS, 0xf, false);
 }
-// The wave's largest key: lanes 1 and 2 apart, mirrored in 8 and 16, then rows into the next ones.
+constexpr int DPP_1 = 0xB1, DPP_2 = 0x4E, DPP_4 = 0x141, DPP_8 = 0x140, DPP_ROW1 = 0x142, DPP_ROW2 = 0x143;
+// The wave's largest key.
 __device__ __forceinline__ uint32_t wave_max(uint32_t x) {
-  x = max_dpp<0xB1>(x);
-  x = max_dpp<0x4E>(x);
-  x = max_dpp<0x141>(x);
-  x = max_dpp<0x140>(x);
-  x = max_dpp<0x142>(x);
-  x = max_dpp<0x143>(x);
+  x = max(x, dpp<DPP_1>(x));
+  x = max(x, dpp<DPP_2>(x));
+  x = max(x, dpp<DPP_4>(x));
+  x = max(x, dpp<DPP_8>(x));
+  x = max(x, dpp<DPP_ROW1, 0xa>(x));
+  x = max(x, dpp<DPP_ROW2, 0xc>(x));
   return __builtin_amdgcn_readlane(x, 63);
 }
-
-// Keys of a token's experts (0: not to be chosen), and the picks from them.
-template <int V>
-struct Keys {
-  uint32_t k[V];
-  __device__ __forceinline__ uint32_t best() const {
-    uint32_t m = k[0];
-#pragma unroll
-    for (int v = 1; v < V; ++v) m = max(m, k[v]);
-    return wave_max(m);
-  }
-  // The lowest id with the key m.
-  __device__ __forceinline__ int find(uint32_t m) const {
-    int id = -1;
-#pragma unroll
-    for (int v = V - 1; v >= 0; --v) {
-      const uint64_t has = __ballot(k[v] == m);
-      if (has) id = v * 64 + __builtin_ctzll(has);
-    }
-    return id;
-  }
-  __device__ __forceinline__ void close(int id) {
-#pragma unroll
-    for (int v = 0; v < V; ++v) k[v] = v * 64 + lane_id() == id ? 0u : k[v];
-  }
-};
-
-// f64 form of the choices: (key, id) pairs by lane exchanges.
-struct Choice {
-  double key;
-  int id;  // INT_MAX: none
-};
-__device__ __forceinline__ bool before(const Choice &a, const Choice &b) { return a.key > b.key || (a.key == b.key && a.id < b.id); }
-__device__ __forceinline__ Choice wave_first(Choice c) {
-#pragma unroll
-  for (int d = 32; d >= 1; d /= 2) {
-    const Choice o{__shfl_xor(c.key, d), __shfl_xor(c.id, d)};
-    if (before(o, c)) c = o;
-  }
-  return c;
+// The two largest of 2^n lanes, from the two of each.
+__device__ __forceinline__ void join2(uint32_t &a, uint32_t &b, uint32_t oa, uint32_t ob) {
+  b = max(min(a, oa), max(b, ob));
+  a = max(a, oa);
+}
+__device__ __forceinline__ void segment_top2(uint32_t &a, uint32_t &b, int lanes) {
+  if (lanes > 1) join2(a, b, dpp<DPP_1>(a), dpp<DPP_1>(b));
+  if (lanes > 2) join2(a, b, dpp<DPP_2>(a), dpp<DPP_2>(b));
+  if (lanes > 4) join2(a, b, dpp<DPP_4>(a), dpp<DPP_4>(b));
+  if (lanes > 8) join2(a, b, dpp<DPP_8>(a), dpp<DPP_8>(b));
+  if (lanes > 16) join2(a, b, __shfl_xor(a, 16), __shfl_xor(b, 16));
+  if (lanes > 32) join2(a, b, __shfl_xor(a, 32), __shfl_xor(b, 32));
 }
 
-// Ids of lane j's choice j, with a bias, in f64. x: the token's logits (what lies past the last expert is not looked at).
+// A lane's experts in the order they are chosen (key 0: none), by exchanges of neighbours: equal keys keep their order.
+template <int V, typename K>
+struct Queue {
+  K k[V];
+  int id[V];
+  __device__ __forceinline__ void sort() {
+#pragma unroll
+    for (int n = V - 1; n > 0; --n)
+#pragma unroll
+      for (int v = 0; v < n; ++v) {
+        const bool swap = k[v + 1] > k[v];
+        const K a = k[v], b = k[v + 1];
+        const int i = id[v], j = id[v + 1];
+        k[v] = swap ? b : a;
+        k[v + 1] = swap ? a : b;
+        id[v] = swap ? j : i;
+        id[v + 1] = swap ? i : j;
+      }
+  }
+  __device__ __forceinline__ void pop() {
+#pragma unroll
+    for (int v = 0; v + 1 < V; ++v) {
+      k[v] = k[v + 1];
+      id[v] = id[v + 1];
+    }
+    k[V - 1] = 0;
+  }
+};
+
+// The same of f64 numbers, by halves of 64-bit keys.
+__device__ __forceinline__ uint64_t order_key(double x) {
+  if (!(x == x)) x = -INFINITY;
+  const uint64_t u = (uint64_t)__double_as_longlong(x + 0.0);
+  return u >> 63 ? ~u : u | (uint64_t)1 << 63;
+}
+__device__ __forceinline__ double key_value(uint64_t k) {
+  return __longlong_as_double((long long)(k >> 63 ? k & ~((uint64_t)1 << 63) : ~k));
+}
+__device__ __forceinline__ uint64_t wave_max(uint64_t x) {
+  const uint32_t hi = wave_max((uint32_t)(x >> 32));
+  const uint32_t lo = wave_max((uint32_t)(x >> 32) == hi ? (uint32_t)x : 0u);
+  return (uint64_t)hi << 32 | lo;
+}
+
+// Lane j's choice j, with a bias, in f64. A token in a thousand comes here, but the launch waits for it: the same steps as
+// below on wider keys, where exchanges of (f64, id) pairs took 25 us.
 template <int V>
 __device__ __forceinline__ int route_f64(const RouteArgs &g, int64_t t) {
   const int lane = lane_id(), E = g.n_experts;
-  double key[V], mx = -INFINITY, sum = 0;
+  double p[V], mx = -INFINITY, sum = 0;
 #pragma unroll
   for (int v = 0; v < V; ++v) {
-    const int e = v * 64 + lane;
-    key[v] = e < E ? (double)dt_load_any(g.logits, t * E + e, g.dtype) : -INFINITY;
-    mx = fmax(mx, key[v]);
+    const int e = lane * V + v;
+    p[v] = e < E ? (double)dt_load_any(g.logits, t * E + e, g.dtype) : -INFINITY;
+    mx = fmax(mx, p[v]);
   }
   if (g.score == RK_ROUTE_SOFTMAX) {
     for (int d = 1; d < 64; d *= 2) mx = fmax(mx, __shfl_xor(mx, d));
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-      key[v] = v * 64 + lane < E ? exp(key[v] - mx) : 0;
-      sum += key[v];
+      p[v] = lane * V + v < E ? exp(p[v] - mx) : 0;
+      sum += p[v];
     }
     for (int d = 1; d < 64; d *= 2) sum += __shfl_xor(sum, d);
   }
-  unsigned open = 0;  // experts of the lane that may be chosen
+  Queue<V, uint64_t> q;
 #pragma unroll
   for (int v = 0; v < V; ++v) {
-    const int e = v * 64 + lane;
-    key[v] = g.score == RK_ROUTE_SOFTMAX ? key[v] / sum : 1 / (1 + exp(-key[v]));
-    if (e < E) {
-      key[v] += (double)g.bias[e];
-      open |= 1u << v;
-    }
-    if (!(key[v] == key[v])) key[v] = -INFINITY;
+    const int e = lane * V + v;
+    const double s = g.score == RK_ROUTE_SOFTMAX ? p[v] / sum : 1 / (1 + exp(-p[v]));
+    q.k[v] = e < E ? order_key(s + (double)g.bias[e]) : 0;
+    q.id[v] = e;
   }
-  auto best_of = [&](int lo, int hi, unsigned from) {
-    Choice c{-INFINITY, INT_MAX};
-#pragma unroll
-    for (int v = 0; v < V; ++v) {
-      const int e = v * 64 + lane;
-      const Choice o{key[v], e};
-      if ((from >> v & 1) && e >= lo && e < hi && before(o, c)) c = o;
-    }
-    return wave_first(c);
-  };
-  auto close = [&](unsigned &mask, int id) {
-    if ((id & 63) == lane) mask &= ~(1u << (id >> 6));
-  };
+  q.sort();
   if (g.top_groups < g.n_groups) {
-    const int size = E / g.n_groups;
-    Choice mine{-INFINITY, INT_MAX};  // lane i: group i
+    uint64_t mine = 0;  // lane i: group i
     for (int i = 0; i < g.n_groups; ++i) {
-      const Choice a = best_of(i * size, (i + 1) * size, open);
-      double s = a.key;
-      if (size > 1) {
-        unsigned rest = open;
-        close(rest, a.id);
-        s += best_of(i * size, (i + 1) * size, rest).key;
-      }
-      if (!(s == s)) s = -INFINITY;  // (two infinities)
-      if (lane == i) mine = Choice{s, i};
-    }
-    uint64_t kept = 0;
-    for (int j = 0; j < g.top_groups; ++j) {
-      const Choice c = wave_first(mine);
-      kept |= (uint64_t)1 << c.id;
-      if (lane == c.id) mine = Choice{-INFINITY, INT_MAX};
-    }
-    unsigned keep = 0;
+      uint64_t a = 0, b = 0;  // (sorted: the first two of the group)
 #pragma unroll
-    for (int v = 0; v < V; ++v)
-      if ((open >> v & 1) && (kept >> ((v * 64 + lane) / size) & 1)) keep |= 1u << v;
-    open = keep;
+      for (int v = V - 1; v >= 0; --v)
+        if (q.id[v] / g.group_size == i && q.k[v]) {
+          b = a;
+          a = q.k[v];
+        }
+      const uint64_t first = wave_max(a);
+      double s = key_value(first);
+      if (g.group_size > 1) {
+        const int at = __builtin_ctzll(__ballot(a == first));
+        s += key_value(wave_max(lane == at ? b : a));
+      }
+      if (lane == i) mine = order_key(s);
+    }
+    int rank = 0;
+    for (int i = 0; i < g.n_groups; ++i) {
+      const uint64_t o = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(mine >> 32), i) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)mine, i);
+      rank += o > mine || (o == mine && i < lane);
+    }
+    const uint64_t kept = __ballot(lane < g.n_groups && rank < g.top_groups);
+#pragma unroll
+    for (int v = 0; v < V; ++v) q.k[v] = kept >> min(q.id[v] / g.group_size, 63) & 1 ? q.k[v] : 0;
+    q.sort();
   }
   int id = 0;
   for (int j = 0; j < g.top_k; ++j) {
-    const Choice c = best_of(0, E, open);
-    close(open, c.id);
-    if (lane == j) id = c.id;
+    const uint64_t m = wave_max(q.k[0]);
+    const int at = __builtin_ctzll(__ballot(q.k[0] == m));
+    const int e = __builtin_amdgcn_readlane(q.id[0], at);
+    if (lane == at) q.pop();
+    if (lane == j) id = e;
   }
   return id;
 }
 }  // namespace
 
+template <int V>
+__device__ __forceinline__ void route_load(const RouteArgs &g, int64_t t, float (&x)[V]) {
+  const int e0 = lane_id() * V, E = g.n_experts;
+  constexpr int P = V < 4 ? V : 4;
+  auto pieces = [&](auto dt_c) {
+    constexpr int DT = decltype(dt_c)::value;
+#pragma unroll
+    for (int p = 0; p < V; p += P) {
+      if (E % P == 0 && e0 + p < E) {
+        dt_load_vec<DT, P>(g.logits, t * E + e0 + p, x + p);
+      } else {
+#pragma unroll
+        for (int v = p; v < p + P; ++v) x[v] = e0 + v < E ? dt_load<DT>(g.logits, t * E + e0 + v) : -INFINITY;
+      }
+    }
+  };
+  if (g.dtype == RK_DTYPE_F32) pieces(ic<RK_DTYPE_F32>{});
+  else if (g.dtype == RK_DTYPE_F16) pieces(ic<RK_DTYPE_F16>{});
+  else pieces(ic<RK_DTYPE_BF16>{});
+}
+
 template <int V, bool BIAS>
 __global__ __launch_bounds__(ROUTE_WAVES * 64) void moe_route_kernel(const RouteArgs g) {
-  const int lane = lane_id();
   const int64_t t = (int64_t)blockIdx.x * ROUTE_WAVES + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   if (t >= g.s) return;
-  const int E = g.n_experts;
+  const int lane = lane_id(), E = g.n_experts;
   const bool softmax = g.score == RK_ROUTE_SOFTMAX;
-  float x[V], mx = -INFINITY, sum = 1.f;
+  float x[V], bias[V], mx = -INFINITY, sum = 1.f;
+  route_load(g, t, x);
 #pragma unroll
-  for (int v = 0; v < V; ++v) {
-    const int e = v * 64 + lane;
-    x[v] = e < E ? dt_load_any(g.logits, t * E + e, g.dtype) : -INFINITY;
-    mx = fmaxf(mx, x[v]);
-  }
+  for (int v = 0; v < V; ++v) bias[v] = BIAS && lane * V + v < E ? g.bias[lane * V + v] : 0.f;
   if (softmax) {
+#pragma unroll
+    for (int v = 0; v < V; ++v) mx = fmaxf(mx, x[v]);
 #pragma unroll
     for (int d = 1; d < 64; d *= 2) mx = fmaxf(mx, __shfl_xor(mx, d));
     sum = 0.f;
 #pragma unroll
-    for (int v = 0; v < V; ++v) sum += v * 64 + lane < E ? expf(x[v] - mx) : 0.f;
+    for (int v = 0; v < V; ++v) sum += lane * V + v < E ? expf(x[v] - mx) : 0.f;
 #pragma unroll
     for (int d = 1; d < 64; d *= 2) sum += __shfl_xor(sum, d);
   }
-  auto score = [&](float l) { return softmax ? expf(l - mx) / sum : 1.0f / (1.0f + expf(-l)); };
-  Keys<V> keys;
-  float most = 1.f;  // the largest finite |score + bias|, at least 1
-#pragma unroll
-  for (int v = 0; v < V; ++v) {
-    const int e = v * 64 + lane;
-    float by = x[v];
-    if constexpr (BIAS) {
-      by = score(x[v]) + (e < E ? g.bias[e] : 0.f);
-      if (fabsf(by) < INFINITY) most = fmaxf(most, fabsf(by));
-    }
-    keys.k[v] = e < E ? order_key(by) : 0u;
-  }
-  // A f32 sum is off by a few roundings of the score and one of its own: closer ones than this are not told apart.
+  Queue<V, uint32_t> q;
+  // With a bias: no f32 sum is off by `near` (a few roundings of the score, one of its own), a 2^20th of the largest finite
+  // |score + bias| or of 1; closer ones are not told apart.
   float near = 0.f;
   bool unsure = false;
-  if constexpr (BIAS) {
 #pragma unroll
-    for (int d = 1; d < 64; d *= 2) most = fmaxf(most, __shfl_xor(most, d));
-    near = most * 0x1p-20f;
+  for (int v = 0; v < V; ++v) {
+    const int e = lane * V + v;
+    float by = x[v];
+    if constexpr (BIAS) {
+      const float p = softmax ? __builtin_amdgcn_exp2f((x[v] - mx) * 1.44269504f) * __builtin_amdgcn_rcpf(sum)
+                              : __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(x[v] * -1.44269504f));
+      by = p + bias[v];
+      near = fmaxf(near, fabsf(by) < INFINITY ? fabsf(by) : 0.f);
+    }
+    q.k[v] = e < E ? order_key(by) : 0u;
+    q.id[v] = e;
   }
+  q.sort();
+  if constexpr (BIAS) near = fmaxf(1.f, __uint_as_float(wave_max(__float_as_uint(near)))) * 0x1p-20f;  // (not negative: ordered as integers)
 
   // Groups: the score of one is its best choice, or with a bias the sum of its two best; experts of the others are closed.
   if (g.top_groups < g.n_groups) {
-    const int size = E / g.n_groups;
+    // Groups of 2^shift lanes side by side (-1: other ones).
+    const int shift = g.group_shift, lanes = 1 << max(shift, 0), size = g.group_size;
     uint32_t mine = 0;  // lane i: group i
-    int group[V];
+    if (shift >= 0) {
+      uint32_t a = q.k[0], b = V > 1 ? q.k[V > 1 ? 1 : 0] : 0u;
+      segment_top2(a, b, lanes);
+      const uint32_t s = BIAS && g.group_size > 1 ? order_key(key_value(a) + key_value(b)) : a;
+      mine = __shfl(s, lane * lanes & 63);
+      if (lane >= g.n_groups) mine = 0;
+    } else {
+      int by = size;
+      asm volatile("" : "+s"(by));  // (the divisions stay in this branch)
+      for (int i = 0; i < g.n_groups; ++i) {
+        uint32_t a = 0, b = 0;
 #pragma unroll
-    for (int v = 0; v < V; ++v) group[v] = (v * 64 + lane) / size;
+        for (int v = 0; v < V; ++v) {
+          const uint32_t k = q.id[v] / by == i ? q.k[v] : 0u;
+          join2(a, b, k, 0u);
+        }
+        segment_top2(a, b, 64);
+        if (lane == i) mine = BIAS && g.group_size > 1 ? order_key(key_value(a) + key_value(b)) : a;
+      }
+    }
+    // A group's rank: the groups before it.
+    int rank = 0;
     for (int i = 0; i < g.n_groups; ++i) {
-      Keys<V> in;
-#pragma unroll
-      for (int v = 0; v < V; ++v) in.k[v] = group[v] == i ? keys.k[v] : 0u;
-      const uint32_t a = in.best();
-      float s = key_value(a);
-      if (BIAS && size > 1) {
-        in.close(in.find(a));
-        s += key_value(in.best());
-      }
-      if (lane == i) mine = order_key(s);
+      const uint32_t o = __builtin_amdgcn_readlane(mine, i);
+      rank += o > mine || (o == mine && i < lane);
     }
-    uint64_t kept = 0;
-    float last = 0.f;
-    for (int j = 0; j < g.top_groups + (BIAS ? 1 : 0); ++j) {
-      const uint32_t m = wave_max(mine);
-      if (BIAS && j == g.top_groups) {
-        unsure |= !(last - key_value(m) > 4 * near);
-        break;
-      }
-      const int i = __builtin_ctzll(__ballot(mine == m));
-      kept |= (uint64_t)1 << i;
-      if (lane == i) mine = 0;
-      last = key_value(m);
+    const uint64_t kept = __ballot(lane < g.n_groups && rank < g.top_groups);
+    if constexpr (BIAS) {
+      const int in = __builtin_ctzll(__ballot(lane < g.n_groups && rank == g.top_groups - 1));
+      const int out = __builtin_ctzll(__ballot(lane < g.n_groups && rank == g.top_groups));
+      unsure = !(key_value((uint32_t)__builtin_amdgcn_readlane(mine, in)) - key_value((uint32_t)__builtin_amdgcn_readlane(mine, out)) > 4 * near);
     }
+    if (shift >= 0) {
+      const bool keep = kept >> (lane >> shift) & 1;
 #pragma unroll
-    for (int v = 0; v < V; ++v)
-      if (!(kept >> (group[v] & 63) & 1)) keys.k[v] = 0u;
+      for (int v = 0; v < V; ++v) q.k[v] = keep ? q.k[v] : 0u;
+    } else {  // (a lane may have experts of two groups)
+      int by = size;
+      asm volatile("" : "+s"(by));
+#pragma unroll
+      for (int v = 0; v < V; ++v) q.k[v] = kept >> min(q.id[v] / by, 63) & 1 ? q.k[v] : 0u;
+      q.sort();
+    }
   }
 
   // The top_k: lane j keeps choice j. With a bias one more, to see how far the last one is from it.
   int id = 0;
   float last = INFINITY;
   for (int j = 0; j < g.top_k + (BIAS ? 1 : 0); ++j) {
-    const uint32_t m = keys.best();
+    const uint32_t m = wave_max(q.k[0]);
     if constexpr (BIAS) {
-      if (j > 0 && m != 0) unsure |= !(last - key_value(m) > 2 * near);
-      last = key_value(m);
+      if (m == 0) break;  // (as many experts as choices)
+      const float c = key_value(m);
+      unsure |= j > 0 && !(last - c > 2 * near);
+      last = c;
       if (j == g.top_k) break;
     }
-    const int i = keys.find(m);
-    keys.close(i);
-    if (lane == j) id = i;
+    const int at = __builtin_ctzll(__ballot(q.k[0] == m));
+    const int e = __builtin_amdgcn_readlane(q.id[0], at);
+    if (lane == at) q.pop();
+    if (lane == j) id = e;
   }
   if (BIAS && unsure) id = route_f64<V>(g, t);
-  // Lane j's logit of its choice.
+  // Lane j's weight: the score of its choice's logit.
   float w = 0.f;
 #pragma unroll
   for (int v = 0; v < V; ++v) {
-    const float l = __shfl(x[v], id & 63);
-    if (v == id >> 6) w = l;
+    const float l = __shfl(x[v], id / V);
+    w = v == id % V ? l : w;
   }
-  w = lane < g.top_k ? score(w) : 0.f;
+  w = lane >= g.top_k ? 0.f : softmax ? expf(w - mx) / sum : 1.0f / (1.0f + expf(-w));
   if (g.norm) {
     float all = w;
 #pragma unroll
@@ -277,10 +321,15 @@ __global__ __launch_bounds__(ROUTE_WAVES * 64) void moe_route_kernel(const Route
   }
 }
 
-hipError_t rk_launch_moe_route(const RouteArgs &g, hipStream_t st) {
-  const int v = (g.n_experts + 63) / 64;
+hipError_t rk_launch_moe_route(const RouteArgs &args, hipStream_t st) {
+  RouteArgs g = args;
+  const int v = g.n_experts <= 64 ? 1 : g.n_experts <= 128 ? 2 : g.n_experts <= 256 ? 4 : g.n_experts <= 512 ? 8 : 16;
+  g.group_size = g.n_experts / g.n_groups;
+  g.group_shift = -1;
+  for (int sh = 0; sh <= 6; ++sh)
+    if (g.group_size == v << sh) g.group_shift = sh;
 #define RK_ROUTE(V) (g.bias ? moe_route_kernel<V, true> : moe_route_kernel<V, false>)
-  auto kern = v <= 1 ? RK_ROUTE(1) : v <= 2 ? RK_ROUTE(2) : v <= 4 ? RK_ROUTE(4) : v <= 8 ? RK_ROUTE(8) : RK_ROUTE(16);
+  auto kern = v == 1 ? RK_ROUTE(1) : v == 2 ? RK_ROUTE(2) : v == 4 ? RK_ROUTE(4) : v == 8 ? RK_ROUTE(8) : RK_ROUTE(16);
 #undef RK_ROUTE
   hipLaunchKernelGGL(kern, dim3((unsigned)((g.s + ROUTE_WAVES - 1) / ROUTE_WAVES)), dim3(ROUTE_WAVES * 64), 0, st, g);
   return hipGetLastError();
