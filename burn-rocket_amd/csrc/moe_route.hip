@@ -12,7 +12,7 @@
 // sorts its own, so that a pick is a maximum of the lanes' heads (lane exchanges inside the vector instruction), a ballot, and
 // a step of one lane's queue. With a bias the f32 sums decide wherever neighbours in the order are further apart than the
 // sums can be off; a token where two are not (about one in a thousand) is done again in f64. 16384 tokens, 256 experts, top 8
-// of 4 groups of 8 on MI355X: ROUTE_US (52 with a search of all registers per pick and two maxima per group, 95 in f64).
+// of 4 groups of 8 on MI355X: 22 us (52 with a search of all registers per pick and two maxima per group, 95 in f64).
 namespace {
 constexpr int ROUTE_WAVES = 4;
 
@@ -340,12 +340,14 @@ hipError_t rk_launch_moe_route(const RouteArgs &args, hipStream_t st) {
 // tiles of at most tile_rows rows; each token's rows in ascending expert id. Pairs whose id names no expert form a bucket
 // behind the last expert's, whose tiles have expert -1.
 //
-// Blocks of 1024 pairs. A pair's row is its expert's first row, plus the expert's pairs in earlier blocks (from the blocks'
-// counts, which a first launch leaves in memory where there are several), plus those of earlier waves of its block, plus
-// those of earlier lanes of its wave. No pair waits for another block's, and nothing depends on the order of atomics.
+// Blocks of 1024 pairs. A pair's row is its expert's first row, plus the expert's pairs in earlier blocks, plus those of
+// earlier waves of its block, plus those of earlier lanes of its wave. The pairs of other blocks are counted by each block
+// itself while there are few, and in a launch of their own that leaves the blocks' counts in memory. No pair waits for
+// another block's, and nothing depends on the order of atomics. Bound by the trips to memory one behind the other.
 namespace {
 constexpr int LB = 1024;       // pairs per block
 constexpr int LW = LB / 64;
+constexpr int COUNT_SELF = 8;  // blocks that count the others' pairs themselves
 }  // namespace
 
 __global__ __launch_bounds__(LB) void moe_count_kernel(const RouteListArgs g) {
@@ -384,15 +386,23 @@ __device__ __forceinline__ uint64_t block_exclusive(uint64_t x, uint64_t *s_wave
 
 __global__ __launch_bounds__(LB) void moe_lists_kernel(const RouteListArgs g, int n_blocks) {
   constexpr int ME = RK_ROUTE_MAX_EXPERTS;
-  __shared__ int s_all[ME + 1], s_at[ME + 1];   // rows of each expert; the first row of this block's
+  __shared__ int s_all[ME + 1], s_at[ME + 1];   // rows of each expert; those of earlier blocks, then the first row of this one's
   __shared__ uint16_t s_cnt[LW][ME + 1];        // rows of each expert in each wave
   __shared__ uint64_t s_wave[LW];
-  const int E = g.n_experts, tid = threadIdx.x, lane = lane_id(), wave = tid >> 6;
-  const int64_t i = (int64_t)blockIdx.x * LB + tid;
+  const int E = g.n_experts, tid = threadIdx.x, lane = lane_id(), wave = tid >> 6, block = blockIdx.x;
+  const bool counted = n_blocks > COUNT_SELF;
+  const int64_t i = (int64_t)block * LB + tid;
   const bool in = i < g.rows;
+  // Pairs of the other blocks, if they are counted here: on the way while the tables are cleared.
+  int other[COUNT_SELF];
+#pragma unroll
+  for (int b = 0; b < COUNT_SELF; ++b) {
+    const int64_t o = (int64_t)b * LB + tid;
+    other[b] = !counted && b < n_blocks && o < g.rows ? (int)min(g.ids[o], (uint32_t)E) : -1;
+  }
   const int e = in ? (int)min(g.ids[i], (uint32_t)E) : E + 1;
   for (int x = tid; x <= E; x += LB) {
-    s_all[x] = 0;
+    s_all[x] = s_at[x] = 0;
 #pragma unroll
     for (int w = 0; w < LW; ++w) s_cnt[w][x] = 0;
   }
@@ -405,47 +415,52 @@ __global__ __launch_bounds__(LB) void moe_lists_kernel(const RouteListArgs g, in
   }
   const int rank = __popcll(peers & (((uint64_t)1 << lane) - 1));
   if (in && rank == 0) s_cnt[wave][e] = (uint16_t)__popcll(peers);
-  if (n_blocks == 1) {
-    if (in && rank == 0) atomicAdd(&s_all[e], __popcll(peers));
-    __syncthreads();
-  }
-  // Rows of each expert in all blocks, and in those before this one. (E + 1 may be one more than the threads: the last
-  // bucket's count is not needed for the first rows.)
-  int all = 0, earlier = 0;
-  if (tid < E) {
-    if (n_blocks == 1) {
-      all = s_all[tid];
-    } else {
+  // Rows of each expert in all blocks, and in those before this one.
+  if (counted) {
+    for (int x = tid; x <= E; x += LB) {
+      int all = 0, before = 0;
+      const int32_t *c = g.counts + x;
+#pragma unroll 8
       for (int b = 0; b < n_blocks; ++b) {
-        const int c = g.counts[(int64_t)b * (E + 1) + tid];
-        all += c;
-        if (b < (int)blockIdx.x) earlier += c;
+        const int n = c[(int64_t)b * (E + 1)];
+        all += n;
+        before += b < block ? n : 0;
       }
+      s_all[x] = all;
+      s_at[x] = before;
     }
+  } else if (n_blocks == 1) {
+    if (in && rank == 0) atomicAdd(&s_all[e], __popcll(peers));
+  } else {
+#pragma unroll
+    for (int b = 0; b < COUNT_SELF; ++b)
+      if (other[b] >= 0) {
+        atomicAdd(&s_all[other[b]], 1);
+        if (b < block) atomicAdd(&s_at[other[b]], 1);
+      }
   }
+  __syncthreads();
+  const int all = tid < E ? s_all[tid] : 0;
   uint64_t valid;
   const int first = (int)block_exclusive((uint64_t)all, s_wave, &valid);
-  if (tid < E) s_at[tid] = first + earlier;
-  if (tid == 0) {
-    // The bucket without an expert: what this block and the earlier ones leave over.
-    int mine = 0;
-    if (n_blocks > 1)
-      for (int b = 0; b < (int)blockIdx.x; ++b) mine += g.counts[(int64_t)b * (E + 1) + E];
-    s_at[E] = (int)valid + mine;
-  }
+  if (tid < E) s_at[tid] += first;
+  if (tid == 0) s_at[E] += (int)valid;
   __syncthreads();
   if (in) {
     int row = s_at[e] + rank;
     for (int w = 0; w < wave; ++w) row += s_cnt[w][e];
     const int64_t t = i / g.top_k;
     const int j = (int)(i - t * g.top_k);
+    int at = 0;
+    for (int o0 = 0; o0 < g.top_k; o0 += 8) {
+      int oe[8];
+#pragma unroll
+      for (int o = 0; o < 8; ++o) oe[o] = o0 + o < g.top_k ? (int)min(g.ids[t * g.top_k + o0 + o], (uint32_t)E) : INT_MAX;
+#pragma unroll
+      for (int o = 0; o < 8; ++o) at += oe[o] < e || (oe[o] == e && o0 + o < j);
+    }
     g.tok[row] = (int32_t)t;
     g.row_w[row] = e < E ? g.wts[i] : 0.f;
-    int at = 0;
-    for (int o = 0; o < g.top_k; ++o) {
-      const int oe = (int)min(g.ids[t * g.top_k + o], (uint32_t)E);
-      if (oe < e || (oe == e && o < j)) ++at;
-    }
     g.slot[t * g.top_k + at] = row;
   }
   if (blockIdx.x != 0) return;
@@ -492,7 +507,7 @@ __global__ __launch_bounds__(LB) void moe_lists_kernel(const RouteListArgs g, in
 
 hipError_t rk_launch_moe_lists(const RouteListArgs &g, hipStream_t st) {
   const int nb = (int)((g.rows + LB - 1) / LB);
-  if (nb > 1) hipLaunchKernelGGL(moe_count_kernel, dim3(nb), dim3(LB), 0, st, g);
+  if (nb > COUNT_SELF) hipLaunchKernelGGL(moe_count_kernel, dim3(nb), dim3(LB), 0, st, g);
   hipLaunchKernelGGL(moe_lists_kernel, dim3(nb), dim3(LB), 0, st, g, nb);
   return hipGetLastError();
 }
