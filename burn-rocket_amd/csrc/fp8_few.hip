@@ -1,13 +1,15 @@
 // Products of few rows with a block-scaled fp8 weight: decode steps of a dense layer, and expert tiles of at most 32 rows.
 //
 // These are bound by the weight's bytes and, below a few MB, by latency: no wave may wait for another while it streams. A
-// workgroup takes one 32-row block of the weight (of an expert's first product: a gate and its up block) and its waves split
-// K: wave w reads the 4 KB blocks w, w + 8, .. of its row block in four 1 KB pieces, some of them ahead, straight into the
-// registers that a 32 × 32 product reads them from. The partial sums meet in LDS at the end, in wave order.
+// workgroup's eight waves are `groups` groups that take a 32-row block of the weight each (of an expert's first product: a
+// gate and its up block) and split its K among their waves: 4 KB blocks in four 1 KB pieces, straight into the registers
+// that a 32 × 32 product reads them from, the next ones on the way. The partial sums meet in LDS, in wave order. (Workgroups
+// that do several blocks one behind the other, asking for the next one's weights before they sum up the last, gain 2 % on 64
+// tokens of a 30B-A3B layer, and lose more on one.)
 //
 // The rows (32 columns of the products, most of them empty in a decode step) come as x itself: the workgroup quantizes them
-// into LDS while its first weights are on the way, so that a layer is one launch; or, where they do not fit LDS, as codes
-// that each wave reads from the caches, up to four column blocks a wave.
+// into LDS once, while its first weights are on the way, so that a layer is one launch; or, where they do not fit LDS, as
+// codes that each wave reads from the caches, up to four column blocks a wave.
 #include "fp8.hpp"
 #include "kernels.hpp"
 
@@ -18,52 +20,83 @@ constexpr int FEW_CODES = 3;  // x's type: codes and scales
 
 // Bytes of a quantized row in LDS: 16 more than its codes, which spreads the rows over the banks.
 __host__ __device__ constexpr int few_row(int kt) { return kt * 128 + 16; }
-template <int XT, int NOUT>
-size_t few_smem(int rows, int kt) {
-  const size_t red = (size_t)FNW * NOUT * 4096;
-  const size_t in = XT == FEW_CODES ? 0 : (size_t)rows * (few_row(kt) + kt * 4);
-  return red > in ? red : in;
+// Columns of the sums in LDS: a multiple of 8.
+__host__ __device__ constexpr int few_cols(int rows) { return rows >= 32 ? 32 : (rows + 7) / 8 * 8; }
+// Quantized rows with their scales, and the waves' sums behind them.
+__host__ __device__ constexpr size_t few_in(int xt, int rows, int kt) {
+  return xt == FEW_CODES ? 0 : ((size_t)rows * (few_row(kt) + kt * 4) + 15) / 16 * 16;
+}
+__host__ __device__ constexpr size_t few_smem(int xt, int nout, int rows, int kt) {
+  return few_in(xt, rows, kt) + (size_t)FNW * nout * 128 * few_cols(rows);
 }
 }  // namespace
 
 template <int XT, int MODE, bool EXACT, int TM>
 __global__ __launch_bounds__(FNW * 64, 2) void fp8_few_kernel(const Fp8FewArgs g) {
   constexpr int NB = MODE == FEW_GATE_UP ? 2 : 1;  // weight blocks
-  constexpr int D = NB == 2 || TM > 2 ? 2 : 4;     // blocks of K on the way, per wave
+  constexpr int D = XT == FEW_CODES ? 4 / TM : NB == 2 ? 2 : 4;  // blocks of K on the way, per wave
   static_assert(XT == FEW_CODES || TM == 1, "x in LDS: one column block");
   extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
   const int lane = lane_id(), col = lane & 31, h = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int kt = g.kt;
+  const int kt = g.kt, groups = g.groups, kw = FNW / groups;
+  const int grp = wave / kw, wk = wave - grp * kw;  // the wave's group, and its part of K
   // (a tile's workgroups one behind the other: they share its rows)
-  const int n_nb = (g.n + 31) / 32, nb = blockIdx.x % n_nb;
+  const int n_nb = (g.n + 31) / 32, per = (n_nb + groups - 1) / groups, nb0 = blockIdx.x % per * groups;
+  const int nb = min(nb0 + grp, n_nb - 1);  // (groups past the last block repeat it: they are not stored)
   int rows = g.m;
   int64_t row0 = 0;
   const uint8_t *w = g.w;
   const float *ws = g.ws;
   if constexpr (MODE != FEW_DENSE) {
-    const MoeTile tile = g.tiles[blockIdx.x / n_nb];
+    const MoeTile tile = g.tiles[blockIdx.x / per];
     if (tile.rows <= 0 || tile.expert < 0) return;
     rows = tile.rows;
     row0 = tile.row0;
     w += (int64_t)tile.expert * g.w_stride;
     ws += (int64_t)tile.expert * g.ws_stride;
+  } else {
+    row0 = (int64_t)(blockIdx.x / per) * 32 * TM;
+    rows = min((int)(g.m - row0), 32 * TM);
   }
 
-  // Weight blocks of this workgroup: consecutive in the layout. Scales: of the gate rows, then of the up rows.
-  const uint8_t *wb = w + (int64_t)nb * NB * kt * 4096 + lane * 16;
+  // Columns past the last row repeat it: they are not stored.
+  int row[TM];
+#pragma unroll
+  for (int j = 0; j < TM; ++j) row[j] = min(j * 32 + col, rows - 1);
+  // The wave's parts wk, wk + kw, .. of K, part `it` of them in registers it mod D. Weight blocks of a pair are consecutive
+  // in the layout; scales: of the gate rows, then of the up rows.
+  const int n_it = (kt - wk + kw - 1) / kw;  // (may be 0)
+  const uint8_t *wb = w + ((int64_t)nb * NB * kt + wk) * 4096 + lane * 16;
   const float *wsb = ws + (int64_t)(nb / 4) * kt;
-  intx4 ring[D][NB][4];
-  auto load = [&](auto d_c, int t) {
-    constexpr int d = decltype(d_c)::value;
+  struct Part {
+    intx4 w[NB][4], x[XT == FEW_CODES ? TM : 1][4];
+    float sw[NB], sa[TM];
+  } ring[D];
+  auto load = [&](auto d_c, int it) {
+    Part &r = ring[decltype(d_c)::value];
+    const int t = wk + kw * it;
 #pragma unroll
-    for (int b = 0; b < NB; ++b)
+    for (int b = 0; b < NB; ++b) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) ring[d][b][i] = *(const intx4 *)(wb + ((int64_t)b * kt + t) * 4096 + i * 1024);
+      for (int i = 0; i < 4; ++i) r.w[b][i] = *(const intx4 *)(wb + ((int64_t)b * kt + kw * it) * 4096 + i * 1024);
+      r.sw[b] = wsb[(int64_t)b * g.up_scales + t];
+    }
+    if constexpr (XT == FEW_CODES) {
+#pragma unroll
+      for (int j = 0; j < TM; ++j) {
+        const uint8_t *p = (const uint8_t *)g.x + (row0 + row[j]) * g.k;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int at = t * 128 + h * 32 + (i >> 1) * 64 + (i & 1) * 16;
+          r.x[j][i] = at < g.k ? *(const intx4 *)(p + at) : intx4{0, 0, 0, 0};
+        }
+        r.sa[j] = g.as[(row0 + row[j]) * kt + t];
+      }
+    }
   };
-  const int n_it = (kt - wave + FNW - 1) / FNW;  // (may be 0)
   static_for<D>([&](auto d_c) {
-    if (decltype(d_c)::value < n_it) load(d_c, wave + FNW * decltype(d_c)::value);
+    if (decltype(d_c)::value < n_it) load(d_c, decltype(d_c)::value);
   });
 
   // x to codes in LDS, [row][few_row], scales [row][kt] behind them.
@@ -108,93 +141,75 @@ __global__ __launch_bounds__(FNW * 64, 2) void fp8_few_kernel(const Fp8FewArgs g
     for (int j = 0; j < TM; ++j)
 #pragma unroll
       for (int r = 0; r < 16; ++r) acc[b][j][r] = 0.f;
-  // Columns past the last row repeat it: they are not stored.
-  int row[TM];
-#pragma unroll
-  for (int j = 0; j < TM; ++j) row[j] = min(j * 32 + col, rows - 1);
-  const uint8_t *codes = (const uint8_t *)g.x;
-  auto block = [&](auto d_c, int t) {
-    constexpr int d = decltype(d_c)::value;
-    Fp8Frag<EXACT> a[NB];
-#pragma unroll
-    for (int b = 0; b < NB; ++b) {
-      a[b].set(0, ring[d][b][0], ring[d][b][1]);
-      a[b].set(1, ring[d][b][2], ring[d][b][3]);
-    }
-    float sw[NB];
-#pragma unroll
-    for (int b = 0; b < NB; ++b) sw[b] = wsb[(int64_t)b * g.up_scales + t];
+  auto block = [&](const Part &p, int t) {
 #pragma unroll
     for (int j = 0; j < TM; ++j) {
       Fp8Frag<EXACT> x;
       float sa;
-      intx4 c[4];
       if constexpr (XT == FEW_CODES) {
-        const int64_t r = row0 + row[j];
-        const uint8_t *p = codes + r * g.k + t * 128 + h * 32;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int at = (i >> 1) * 64 + (i & 1) * 16;
-          c[i] = t * 128 + h * 32 + at < g.k ? *(const intx4 *)(p + at) : intx4{0, 0, 0, 0};
-        }
-        sa = g.as[r * kt + t];
+        x.set(0, p.x[j][0], p.x[j][1]);
+        x.set(1, p.x[j][2], p.x[j][3]);
+        sa = p.sa[j];
       } else {
-        const uint8_t *p = smem + (size_t)row[j] * few_row(kt) + t * 128 + h * 32;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) c[i] = *(const intx4 *)(p + (i >> 1) * 64 + (i & 1) * 16);
+        const uint8_t *q = smem + (size_t)row[j] * few_row(kt) + t * 128 + h * 32;
+        x.set(0, *(const intx4 *)q, *(const intx4 *)(q + 16));
+        x.set(1, *(const intx4 *)(q + 64), *(const intx4 *)(q + 80));
         sa = s_as[row[j] * kt + t];
       }
-      x.set(0, c[0], c[1]);
-      x.set(1, c[2], c[3]);
 #pragma unroll
       for (int b = 0; b < NB; ++b) {
-        const floatx16 p = fp8_product(a[b], x);
-        const float s = sa * sw[b];
+        Fp8Frag<EXACT> a;
+        a.set(0, p.w[b][0], p.w[b][1]);
+        a.set(1, p.w[b][2], p.w[b][3]);
+        const floatx16 c = fp8_product(a, x);
+        const float s = sa * p.sw[b];
 #pragma unroll
-        for (int r = 0; r < 16; ++r) acc[b][j][r] = __builtin_fmaf(p[r], s, acc[b][j][r]);
+        for (int r = 0; r < 16; ++r) acc[b][j][r] = __builtin_fmaf(c[r], s, acc[b][j][r]);
       }
     }
   };
   for (int it0 = 0; it0 < n_it; it0 += D)
     static_for<D>([&](auto d_c) {
-      const int it = it0 + decltype(d_c)::value;
+      constexpr int d = decltype(d_c)::value;
+      const int it = it0 + d;
       if (it < n_it) {
-        block(d_c, wave + FNW * it);
-        if (it + D < n_it) load(d_c, wave + FNW * (it + D));
+        block(ring[d], wk + kw * it);
+        if (it + D < n_it) load(d_c, it + D);
       }
     });
 
-  // The waves' sums: [wave][output][quarter][lane] of four values.
-  __syncthreads();
-  floatx4 *red = (floatx4 *)smem;
+  // Sums in LDS: [wave][output][quarter][half][column] of four values.
+  floatx4 *red = (floatx4 *)(smem + few_in(XT, rows, kt));
+  const int cols = few_cols(TM == 1 ? rows : 32);
+  if (col < cols)
 #pragma unroll
-  for (int b = 0; b < NB; ++b)
+    for (int b = 0; b < NB; ++b)
 #pragma unroll
-    for (int j = 0; j < TM; ++j)
+      for (int j = 0; j < TM; ++j)
 #pragma unroll
-      for (int q = 0; q < 4; ++q)
-        red[(((wave * NB + b) * TM + j) * 4 + q) * 64 + lane] =
-            floatx4{acc[b][j][4 * q], acc[b][j][4 * q + 1], acc[b][j][4 * q + 2], acc[b][j][4 * q + 3]};
+        for (int q = 0; q < 4; ++q)
+          red[((((wave * NB + b) * TM + j) * 4 + q) * 2 + h) * cols + col] =
+              floatx4{acc[b][j][4 * q], acc[b][j][4 * q + 1], acc[b][j][4 * q + 2], acc[b][j][4 * q + 3]};
   __syncthreads();
   const bool whole = (g.n & 3) == 0;
-  for (int o = threadIdx.x; o < TM * 256; o += FNW * 64) {
-    const int l = o & 63, q = (o >> 6) & 3, j = o >> 8;
-    const int r = j * 32 + (l & 31);
-    if (r >= rows) continue;
+  const int each = TM * 8 * cols;  // items of four values of a group
+  for (int o = threadIdx.x; o < groups * each; o += FNW * 64) {
+    const int gr = o / each, i = o - gr * each;
+    const int c = i % cols, hq = i / cols, hh = hq & 1, q = (hq >> 1) & 3, j = hq >> 3;
+    const int r = j * 32 + c, n = (nb0 + gr) * 32 + q * 8 + hh * 4;
+    if (r >= rows || n >= g.n) continue;
     float v[NB][4];
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
       floatx4 sum = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int k = 0; k < FNW; ++k) {
-        const floatx4 p = red[(((k * NB + b) * TM + j) * 4 + q) * 64 + l];
+      for (int k = 0; k < kw; ++k) {
+        const floatx4 p = red[(((((gr * kw + k) * NB + b) * TM + j) * 4 + q) * 2 + hh) * cols + c];
 #pragma unroll
         for (int e = 0; e < 4; ++e) sum[e] += p[e];
       }
 #pragma unroll
       for (int e = 0; e < 4; ++e) v[b][e] = sum[e];
     }
-    const int n = nb * 32 + q * 8 + (l >> 5) * 4;
     if constexpr (MODE == FEW_GATE_UP) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) v[0][e] = fp8_silu_mul<EXACT>(v[0][e], v[1][e]);
@@ -208,11 +223,17 @@ __global__ __launch_bounds__(FNW * 64, 2) void fp8_few_kernel(const Fp8FewArgs g
 }
 
 // Rows that a workgroup can quantize into its LDS (x itself as input), and those that it can take as codes.
-bool rk_fp8_few_fits_x(int64_t m, int kt) { return m <= 32 && few_smem<0, 1>((int)m, kt) <= 64 * 1024; }
+bool rk_fp8_few_fits_x(int64_t m, int kt) { return m <= 32 && few_in(0, (int)m, kt) <= 64 * 1024; }
 bool rk_fp8_few_fits_codes(int64_t m) { return m <= 128; }
+// Rows of an expert tile that a workgroup has LDS for: a power of two of at most 32.
+int rk_fp8_few_rows(int kt) {
+  int rows = 32;
+  while (rows > 1 && few_smem(0, 2, rows, kt) > 160 * 1024) rows /= 2;
+  return rows;
+}
 
 template <int XT, int MODE, bool EXACT, int TM>
-static hipError_t launch_few(const Fp8FewArgs &g, int rows, int n_tiles, hipStream_t st) {
+static hipError_t launch_few(Fp8FewArgs g, int rows, int n_tiles, hipStream_t st) {
   constexpr int NOUT = (MODE == FEW_GATE_UP ? 2 : 1) * TM;
   auto kern = fp8_few_kernel<XT, MODE, EXACT, TM>;
   static bool attr_set = false;
@@ -221,18 +242,18 @@ static hipError_t launch_few(const Fp8FewArgs &g, int rows, int n_tiles, hipStre
     if (e != hipSuccess) return e;
     attr_set = true;
   }
-  const size_t smem = few_smem<XT, NOUT>(rows, g.kt);
+  const size_t smem = few_smem(XT, NOUT, rows, g.kt);
   if (smem > 160 * 1024) return hipErrorInvalidValue;
-  hipLaunchKernelGGL(kern, dim3((unsigned)((int64_t)(g.n + 31) / 32 * n_tiles)), dim3(FNW * 64), smem, st, g);
+  // Blocks side by side in a workgroup: as many as leave a workgroup per CU, and a wave at most eight parts of K. Whole
+  // calls on a 30B-A3B layer, MI355X, with G of the first product's blocks and D of the second's: 64 tokens 171 us with 1
+  // and 1, 135 with 4 and 8; one token 28.2 with 1 and 1, 25.5 with 1 and 2, 25.9 with 2 and 4.
+  const int64_t n_nb = (g.n + 31) / 32;
+  g.groups = 1;
+  while (g.groups < FNW && (n_nb + 2 * g.groups - 1) / (2 * g.groups) * n_tiles >= 256 && g.kt * 2 * g.groups <= 8 * FNW) g.groups *= 2;
+  hipLaunchKernelGGL(kern, dim3((unsigned)((n_nb + g.groups - 1) / g.groups * n_tiles)), dim3(FNW * 64), smem, st, g);
   return hipGetLastError();
 }
 
-// Rows of an expert tile that a workgroup has LDS for: a power of two of at most 32.
-int rk_fp8_few_rows(int kt) {
-  int rows = 32;
-  while (rows > 1 && few_smem<0, 2>(rows, kt) > 160 * 1024) rows /= 2;
-  return rows;
-}
 hipError_t rk_launch_fp8_few_gate_up(const Fp8FewArgs &g, int x_dtype, int tile_rows, int n_tiles, bool exact, hipStream_t st) {
 #define RK_FEW(XT) (exact ? launch_few<XT, FEW_GATE_UP, true, 1>(g, tile_rows, n_tiles, st) : launch_few<XT, FEW_GATE_UP, false, 1>(g, tile_rows, n_tiles, st))
   switch (x_dtype) {
@@ -248,12 +269,19 @@ hipError_t rk_launch_fp8_few_down(const Fp8FewArgs &g, int tile_rows, int n_tile
 }
 
 hipError_t rk_launch_fp8_few(const Fp8FewArgs &g, int x_dtype, bool exact, hipStream_t st) {
-#define RK_FEW(XT, TM) (exact ? launch_few<XT, FEW_DENSE, true, TM>(g, g.m, 1, st) : launch_few<XT, FEW_DENSE, false, TM>(g, g.m, 1, st))
+  // Column blocks (32 rows) of a call, a wave's share of them: so many that a weight block's workgroups still fill the CUs.
+  // They read the weight once per share, which the caches serve.
+  const int cb = x_dtype == FEW_CODES ? (g.m + 31) / 32 : 1, n_nb = (g.n + 31) / 32;
+  int tm = 1;
+  while (tm < 4 && tm < cb && (int64_t)n_nb * ((cb + 2 * tm - 1) / (2 * tm)) >= 256) tm *= 2;
+  const int tiles = (cb + tm - 1) / tm;
+#define RK_FEW(XT, TM) \
+  (exact ? launch_few<XT, FEW_DENSE, true, TM>(g, g.m, tiles, st) : launch_few<XT, FEW_DENSE, false, TM>(g, g.m, tiles, st))
   switch (x_dtype) {
     case RK_DTYPE_F32: return RK_FEW(RK_DTYPE_F32, 1);
     case RK_DTYPE_F16: return RK_FEW(RK_DTYPE_F16, 1);
     case RK_DTYPE_BF16: return RK_FEW(RK_DTYPE_BF16, 1);
   }
-  return g.m <= 32 ? RK_FEW(FEW_CODES, 1) : g.m <= 64 ? RK_FEW(FEW_CODES, 2) : RK_FEW(FEW_CODES, 4);
+  return tm == 1 ? RK_FEW(FEW_CODES, 1) : tm == 2 ? RK_FEW(FEW_CODES, 2) : RK_FEW(FEW_CODES, 4);
 #undef RK_FEW
 }

@@ -315,6 +315,7 @@ struct Fp8FewArgs {
   const float *row_w;           // router weight of each bucket row (second product)
   int64_t w_stride, ws_stride;  // bytes and scales per expert
   int64_t up_scales;            // scales from a gate block's to its up block's
+  int groups;                   // set by the launcher: blocks of n side by side in a workgroup
 };
 bool rk_fp8_few_fits_x(int64_t m, int kt);
 bool rk_fp8_few_fits_codes(int64_t m);
