@@ -982,7 +982,7 @@ int gemm_f16_run(CallScope &cs, const void *a, const void *b, void *c, int64_t m
 int fp8_product_run(const Weight &w, const uint8_t *a, const float *as, int64_t m, void *c, int c_dtype, hipStream_t st,
                     const char *op) {
   const bool exact = c_dtype == RK_DTYPE_F32;
-  if (rk_fp8_few_fits_codes(m)) {
+  if (rk_fp8_few_fits_codes(m, w.n, exact, g_eng->num_cus)) {
     Fp8FewArgs g{};
     g.x = a;
     g.as = as;
@@ -3320,7 +3320,10 @@ extern "C" int rk_matmul_fp8_dev(rk_weight_id id, const void *x, int x_dtype, in
   RK_TRY(fp8_rows_check(x, "x", op));
   RK_TRY(fp8_rows_check(c, "c", op));
   hipStream_t st = pick(stream);
-  if (rk_fp8_few_fits_x(m, w->ws_stride)) {  // one launch, nothing in library memory
+  bool capturing;
+  RK_TRY(is_capturing(st, &capturing, op));
+  // one launch, nothing in library memory
+  if (rk_fp8_few_fits_x(m, w->ws_stride) && (capturing || rk_fp8_few_wants_x(m, w->ws_stride))) {
     Fp8FewArgs g{};
     g.x = x;
     g.m = (int)m;
@@ -3333,8 +3336,6 @@ extern "C" int rk_matmul_fp8_dev(rk_weight_id id, const void *x, int x_dtype, in
     g.c_dtype = c_dtype;
     HIP_TRY(rk_launch_fp8_few(g, x_dtype, c_dtype == RK_DTYPE_F32, st), op);
   } else {
-    bool capturing;
-    RK_TRY(is_capturing(st, &capturing, op));
     if (capturing)
       return fail(RK_E_UNSUPPORTED, op, "these rows are quantized into library memory, which a graph must not hold: capture "
                                         "rk_quantize_fp8_dev and rk_matmul_fp8_codes_dev");

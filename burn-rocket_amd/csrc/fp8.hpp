@@ -14,6 +14,18 @@ constexpr int FP8_BLOCK = 128;  // values per scale along K; rows per weight sca
 // its row's results NaN; a NaN does not reach amax and becomes the NaN code itself.
 __device__ __forceinline__ float fp8_scale(float amax) { return fmaxf(amax / 448.0f, 1e-12f); }
 
+// The largest of 16 neighbouring lanes' values, in all of them: rotations inside the vector instruction.
+template <int CTRL>
+__device__ __forceinline__ float fp8_rotated(float x) {
+  return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), CTRL, 0xf, 0xf, false));
+}
+__device__ __forceinline__ float fp8_max16(float x) {
+  x = fmaxf(x, fp8_rotated<0x121>(x));  // by 1, 2, 4 and 8 lanes
+  x = fmaxf(x, fp8_rotated<0x122>(x));
+  x = fmaxf(x, fp8_rotated<0x124>(x));
+  return fmaxf(x, fp8_rotated<0x128>(x));
+}
+
 // x / s as an f32 number, with the reciprocal of s taken once per block: the residual of the product with the reciprocal
 // corrects it to the rounded quotient. Codes are rounded from that number, so that they do not depend on how a division
 // is carried out: ties are common, since x and amax have few bits.

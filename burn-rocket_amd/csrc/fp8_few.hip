@@ -8,8 +8,8 @@
 // tokens of a 30B-A3B layer, and lose more on one.)
 //
 // The rows (32 columns of the products, most of them empty in a decode step) come as x itself: the workgroup quantizes them
-// into LDS once, while its first weights are on the way, so that a layer is one launch; or, where they do not fit LDS, as
-// codes that each wave reads from the caches, up to four column blocks a wave.
+// into LDS once, while its first weights are on the way, so that a layer is one launch; or, where they are more, as codes
+// that each wave reads from the caches, whole lines at a time, one or two column blocks a wave.
 #include "fp8.hpp"
 #include "kernels.hpp"
 
@@ -22,12 +22,12 @@ constexpr int FEW_CODES = 3;  // x's type: codes and scales
 __host__ __device__ constexpr int few_row(int kt) { return kt * 128 + 16; }
 // Columns of the sums in LDS: a multiple of 8.
 __host__ __device__ constexpr int few_cols(int rows) { return rows >= 32 ? 32 : (rows + 7) / 8 * 8; }
-// Quantized rows with their scales, and the waves' sums behind them.
-__host__ __device__ constexpr size_t few_in(int xt, int rows, int kt) {
-  return xt == FEW_CODES ? 0 : ((size_t)rows * (few_row(kt) + kt * 4) + 15) / 16 * 16;
-}
-__host__ __device__ constexpr size_t few_smem(int xt, int nout, int rows, int kt) {
-  return few_in(xt, rows, kt) + (size_t)FNW * nout * 128 * few_cols(rows);
+// Quantized rows with their scales, and the waves' sums behind them; or codes on their way to the operands, a part of K per
+// wave, where the sums go afterwards.
+__host__ __device__ constexpr size_t few_in(int rows, int kt) { return ((size_t)rows * (few_row(kt) + kt * 4) + 15) / 16 * 16; }
+__host__ __device__ constexpr size_t few_smem(int xt, int nout, int tm, int rows, int kt) {
+  const size_t red = (size_t)FNW * nout * 128 * few_cols(rows);
+  return xt != FEW_CODES ? few_in(rows, kt) + red : red > (size_t)FNW * tm * 4096 ? red : (size_t)FNW * tm * 4096;
 }
 }  // namespace
 
@@ -83,13 +83,14 @@ __global__ __launch_bounds__(FNW * 64, 2) void fp8_few_kernel(const Fp8FewArgs g
       r.sw[b] = wsb[(int64_t)b * g.up_scales + t];
     }
     if constexpr (XT == FEW_CODES) {
+      // whole lines: eight lanes a row of 128 codes
+      const int at = t * 128 + (lane & 7) * 16;
 #pragma unroll
       for (int j = 0; j < TM; ++j) {
-        const uint8_t *p = (const uint8_t *)g.x + (row0 + row[j]) * g.k;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const int at = t * 128 + h * 32 + (i >> 1) * 64 + (i & 1) * 16;
-          r.x[j][i] = at < g.k ? *(const intx4 *)(p + at) : intx4{0, 0, 0, 0};
+          const int64_t src = row0 + min(j * 32 + i * 8 + (lane >> 3), rows - 1);
+          r.x[j][i] = at < g.k ? *(const intx4 *)((const uint8_t *)g.x + src * g.k + at) : intx4{0, 0, 0, 0};
         }
         r.sa[j] = g.as[(row0 + row[j]) * kt + t];
       }
@@ -121,9 +122,7 @@ __global__ __launch_bounds__(FNW * 64, 2) void fp8_few_kernel(const Fp8FewArgs g
       float amax = 0.f;
 #pragma unroll
       for (int e = 0; e < 8; ++e) amax = fmaxf(amax, fabsf(v[e]));
-#pragma unroll
-      for (int d = 1; d < 16; d *= 2) amax = fmaxf(amax, __shfl_xor(amax, d));
-      const float s = fp8_scale(amax);
+      const float s = fp8_scale(fp8_max16(amax));
       const Fp8Div div(s);
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[e] = div(v[e]);
@@ -147,8 +146,16 @@ __global__ __launch_bounds__(FNW * 64, 2) void fp8_few_kernel(const Fp8FewArgs g
       Fp8Frag<EXACT> x;
       float sa;
       if constexpr (XT == FEW_CODES) {
-        x.set(0, p.x[j][0], p.x[j][1]);
-        x.set(1, p.x[j][2], p.x[j][3]);
+        // To operands through the wave's own LDS (its accesses run in order): chunk c of row r at c ^ ((r >> 1) & 7).
+        uint8_t *q = smem + (wave * TM + j) * 4096;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int r = i * 8 + (lane >> 3);
+          *(intx4 *)(q + r * 128 + (((lane & 7) ^ ((r >> 1) & 7)) << 4)) = p.x[j][i];
+        }
+        const uint32_t off = (uint32_t)(col * 128 + (((2 * h) ^ ((col >> 1) & 7)) << 4));  // (chunk bits 0 and 2: ^ 16, ^ 64)
+        x.set(0, *(const intx4 *)(q + off), *(const intx4 *)(q + (off ^ 16)));
+        x.set(1, *(const intx4 *)(q + (off ^ 64)), *(const intx4 *)(q + (off ^ 80)));
         sa = p.sa[j];
       } else {
         const uint8_t *q = smem + (size_t)row[j] * few_row(kt) + t * 128 + h * 32;
@@ -179,7 +186,8 @@ __global__ __launch_bounds__(FNW * 64, 2) void fp8_few_kernel(const Fp8FewArgs g
     });
 
   // Sums in LDS: [wave][output][quarter][half][column] of four values.
-  floatx4 *red = (floatx4 *)(smem + few_in(XT, rows, kt));
+  floatx4 *red = (floatx4 *)(smem + (XT == FEW_CODES ? 0 : few_in(rows, kt)));
+  if constexpr (XT == FEW_CODES) __syncthreads();
   const int cols = few_cols(TM == 1 ? rows : 32);
   if (col < cols)
 #pragma unroll
@@ -223,12 +231,22 @@ __global__ __launch_bounds__(FNW * 64, 2) void fp8_few_kernel(const Fp8FewArgs g
 }
 
 // Rows that a workgroup can quantize into its LDS (x itself as input), and those that it can take as codes.
-bool rk_fp8_few_fits_x(int64_t m, int kt) { return m <= 32 && few_in(0, (int)m, kt) <= 64 * 1024; }
-bool rk_fp8_few_fits_codes(int64_t m) { return m <= 128; }
+bool rk_fp8_few_fits_x(int64_t m, int kt) { return m <= 32 && few_in((int)m, kt) <= 64 * 1024; }
+// Where that is faster than a launch that quantizes once and a second one on codes: every workgroup takes 0.5 us for 32
+// blocks of x. us so and in two launches, MI355X: 8 × 4096 × 2048 6.6 and 7.1, 16 × 4096 × 2048 8.8 and 7.2, 16 × 1024 ×
+// 1024 5.7 and 6.2, 24 × 1024 × 1024 6.7 and 6.2, 4 × 4096 × 4096 8.1 and 8.8, 8 × 4096 × 4096 10.5 and 8.9.
+bool rk_fp8_few_wants_x(int64_t m, int kt) { return m * kt <= 160; }
+// Codes: while the grid is what is short, 32 outputs × 64 rows a workgroup, one per CU (two where the products are the
+// slow exact ones). us here and on 64 × 128 tiles, MI355X, 16-bit results: 128 × 4096 × 4096 10.1 and 15.4, 192 × 4096 ×
+// 4096 14.8 and 15.4, 256 × 4096 × 1024 7.3 and 6.5, 512 × 4096 × 4096 28 and 16; f32: 512 × 2048 × 2048 11.6 and 15.3,
+// 512 × 4096 × 2048 18 and 16.
+bool rk_fp8_few_fits_codes(int64_t m, int64_t n, bool exact, int num_cus) {
+  return m <= 32 || (n + 31) / 32 * ((m + 63) / 64) <= (exact ? 2 : 1) * (int64_t)num_cus;
+}
 // Rows of an expert tile that a workgroup has LDS for: a power of two of at most 32.
 int rk_fp8_few_rows(int kt) {
   int rows = 32;
-  while (rows > 1 && few_smem(0, 2, rows, kt) > 160 * 1024) rows /= 2;
+  while (rows > 1 && few_smem(0, 2, 1, rows, kt) > 160 * 1024) rows /= 2;
   return rows;
 }
 
@@ -242,15 +260,18 @@ static hipError_t launch_few(Fp8FewArgs g, int rows, int n_tiles, hipStream_t st
     if (e != hipSuccess) return e;
     attr_set = true;
   }
-  const size_t smem = few_smem(XT, NOUT, rows, g.kt);
+  const size_t smem = few_smem(XT, NOUT, TM, TM == 1 ? rows : 32, g.kt);
   if (smem > 160 * 1024) return hipErrorInvalidValue;
   // Blocks side by side in a workgroup: as many as leave a workgroup per CU, and a wave at most eight parts of K. Whole
   // calls on a 30B-A3B layer, MI355X, with G of the first product's blocks and D of the second's: 64 tokens 171 us with 1
-  // and 1, 135 with 4 and 8; one token 28.2 with 1 and 1, 25.5 with 1 and 2, 25.9 with 2 and 4.
+  // and 1, 135 with 4 and 8; one token 28.2 with 1 and 1, 25.5 with 1 and 2, 25.9 with 2 and 4. From codes a workgroup is a
+  // round of its CU: also where that leaves fewer (384 × 2048 × 2048 11.4 and 9.6 us).
   const int64_t n_nb = (g.n + 31) / 32;
+  const auto wgs = [&](int groups) { return (n_nb + groups - 1) / groups * n_tiles; };
   g.groups = 1;
-  while (g.groups < FNW && (n_nb + 2 * g.groups - 1) / (2 * g.groups) * n_tiles >= 256 && g.kt * 2 * g.groups <= 8 * FNW) g.groups *= 2;
-  hipLaunchKernelGGL(kern, dim3((unsigned)((n_nb + g.groups - 1) / g.groups * n_tiles)), dim3(FNW * 64), smem, st, g);
+  while (g.groups < FNW && (XT == FEW_CODES ? wgs(g.groups) > 256 : wgs(2 * g.groups) >= 256) && g.kt * 2 * g.groups <= 8 * FNW)
+    g.groups *= 2;
+  hipLaunchKernelGGL(kern, dim3((unsigned)wgs(g.groups)), dim3(FNW * 64), smem, st, g);
   return hipGetLastError();
 }
 
@@ -269,11 +290,10 @@ hipError_t rk_launch_fp8_few_down(const Fp8FewArgs &g, int tile_rows, int n_tile
 }
 
 hipError_t rk_launch_fp8_few(const Fp8FewArgs &g, int x_dtype, bool exact, hipStream_t st) {
-  // Column blocks (32 rows) of a call, a wave's share of them: so many that a weight block's workgroups still fill the CUs.
-  // They read the weight once per share, which the caches serve.
+  // Column blocks (32 rows) of a call, a wave's share of them: two where one each would be more than a round of workgroups
+  // (with four the registers do not do). They read the weight once per share, which the caches serve.
   const int cb = x_dtype == FEW_CODES ? (g.m + 31) / 32 : 1, n_nb = (g.n + 31) / 32;
-  int tm = 1;
-  while (tm < 4 && tm < cb && (int64_t)n_nb * ((cb + 2 * tm - 1) / (2 * tm)) >= 256) tm *= 2;
+  const int tm = (int64_t)n_nb * cb > 256 ? min(cb, 2) : 1;
   const int tiles = (cb + tm - 1) / tm;
 #define RK_FEW(XT, TM) \
   (exact ? launch_few<XT, FEW_DENSE, true, TM>(g, g.m, tiles, st) : launch_few<XT, FEW_DENSE, false, TM>(g, g.m, tiles, st))
@@ -282,6 +302,6 @@ hipError_t rk_launch_fp8_few(const Fp8FewArgs &g, int x_dtype, bool exact, hipSt
     case RK_DTYPE_F16: return RK_FEW(RK_DTYPE_F16, 1);
     case RK_DTYPE_BF16: return RK_FEW(RK_DTYPE_BF16, 1);
   }
-  return tm == 1 ? RK_FEW(FEW_CODES, 1) : tm == 2 ? RK_FEW(FEW_CODES, 2) : RK_FEW(FEW_CODES, 4);
+  return tm == 1 ? RK_FEW(FEW_CODES, 1) : RK_FEW(FEW_CODES, 2);
 #undef RK_FEW
 }

@@ -16,7 +16,7 @@ __global__ __launch_bounds__(QT) void quantize_fp8_kernel(const void *__restrict
   const int sub = threadIdx.x & 15;
   const int64_t step = (int64_t)gridDim.x * (QT / 16);
   for (int64_t b = (int64_t)blockIdx.x * (QT / 16) + threadIdx.x / 16; b < blocks; b += step) {
-    const int64_t row = b / kt;
+    const int64_t row = (uint32_t)b / (uint32_t)kt;  // (2^32 blocks do not fit the memory)
     const int at = (int)(b - row * kt), col = at * 128 + sub * 8;
     float v[8];
     const bool in = col < k;
@@ -34,9 +34,7 @@ __global__ __launch_bounds__(QT) void quantize_fp8_kernel(const void *__restrict
     float amax = 0.f;
 #pragma unroll
     for (int e = 0; e < 8; ++e) amax = fmaxf(amax, fabsf(v[e]));
-#pragma unroll
-    for (int d = 1; d < 16; d *= 2) amax = fmaxf(amax, __shfl_xor(amax, d));
-    const float s = fp8_scale(amax);
+    const float s = fp8_scale(fp8_max16(amax));
     const Fp8Div div(s);
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] = div(v[e]);

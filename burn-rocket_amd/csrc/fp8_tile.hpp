@@ -36,7 +36,7 @@ struct Fp8Tile {
   static_assert(SMEM <= 160 * 1024, "LDS per workgroup");
   static_assert(CA * NW == QA && CB * NW == QB && SI < NW && SI * 64 == BM, "copies per wave");
   static_assert((TN * TM) % 2 == 0 && TN % 2 == 0, "the two product registers and the two weight fragments alternate over stages too");
-  static_assert(STAGES == 2, "the slot of a stage is refilled for the one after the next");
+  static_assert(STAGES >= 2, "the slot of a stage is refilled for the one STAGES later");
 
   floatx16 acc[TN][TM];  // outputs 32·i + 8·(r/4) + 4·(lane/32) + r%4 of row 32·j + lane%32 of the wave's part
 
@@ -140,49 +140,63 @@ struct Fp8Tile {
       for (int r = 0; r < 16; ++r) acc[i][j][r] = __builtin_fmaf(p[r], sc, acc[i][j][r]);
       __builtin_amdgcn_sched_barrier(0);
     };
-    auto arrived = [&] {
-      WAIT_VMCNT(0);
+    // The copies of a wave's next stage have arrived when those of the `behind` ones after it are left (every wave issues CP a stage).
+    auto arrived = [&](auto behind_c) {
+      WAIT_VMCNT(decltype(behind_c)::value * CP);
       WAIT_LGKMCNT0();
       BARRIER();
     };
-    issue(ic<0>{}, ic<CP>{}, 0, 0);
-    arrived();
+    constexpr int AHEAD = STAGES - 2;  // stages in flight at a barrier behind the one that it waits for
+    static_assert(AHEAD * CP < 64, "copies that the wait can count");
+    const int pre = min(KT, STAGES - 1);
+    for (int kt = 0; kt < pre; ++kt) issue(ic<0>{}, ic<CP>{}, kt, kt);
+    if (KT > AHEAD) arrived(ic<AHEAD>{});
+    else arrived(ic<0>{});
+    auto after = [](int slot, int by) { return slot + by >= STAGES ? slot + by - STAGES : slot + by; };
+    int slot = 0;
     if (wm * WTM >= rows) {  // a wave without rows copies for the others
-      for (int kt = 1; kt < KT; ++kt) {
-        issue(ic<0>{}, ic<CP>{}, kt & 1, kt);
-        arrived();
+      for (int kt = 0; kt + 1 < KT; ++kt, slot = after(slot, 1)) {
+        if (kt + STAGES - 1 < KT) {
+          issue(ic<0>{}, ic<CP>{}, after(slot, STAGES - 1), kt + STAGES - 1);
+          arrived(ic<AHEAD>{});
+        } else {
+          arrived(ic<0>{});
+        }
       }
     } else {
       load_w(wf[0], 0, 0);
 #pragma unroll
       for (int j = 0; j < TM; ++j) load_x(0, j);
       load_s(0);
-      if (KT > 1) static_for<TM>([&](auto j_c) { issue_at(j_c, 1, 1); });
-      // more: a stage follows; most: one behind it too (no branches in the steady state)
-      auto stage = [&](int kt, auto more_c, auto most_c) {
-        constexpr bool more = decltype(more_c)::value, most = decltype(most_c)::value;
-        const int slot = kt & 1, next = slot ^ 1;
+      if (KT >= STAGES) static_for<TM>([&](auto j_c) { issue_at(j_c, STAGES - 1, STAGES - 1); });
+      // more: a stage follows; last: the stage STAGES - 1 later exists; most: the one STAGES later too (no branches in the steady state)
+      auto stage = [&](int kt, auto more_c, auto last_c, auto most_c) {
+        constexpr bool more = decltype(more_c)::value, last = decltype(last_c)::value, most = decltype(most_c)::value;
+        const int next = after(slot, 1);
         static_for<TN - 1>([&](auto i_c) {
           load_w(wf[(decltype(i_c)::value + 1) & 1], slot, decltype(i_c)::value + 1);
           static_for<TM>([&](auto j_c) {
             tile(i_c, j_c);
-            if constexpr (more && decltype(i_c)::value == 0) issue_at(ic<TM + decltype(j_c)::value>{}, next, kt + 1);
+            if constexpr (last && decltype(i_c)::value == 0) issue_at(ic<TM + decltype(j_c)::value>{}, after(slot, STAGES - 1), kt + STAGES - 1);
           });
         });
         if constexpr (more) {
-          arrived();
+          arrived(ic<last ? AHEAD : 0>{});
           load_w(wf[0], next, 0);
         }
         static_for<TM>([&](auto j_c) {
           tile(ic<TN - 1>{}, j_c);
-          if constexpr (most) issue_at(j_c, slot, kt + 2);
+          if constexpr (most) issue_at(j_c, slot, kt + STAGES);
           if constexpr (more) load_x(next, decltype(j_c)::value);
         });
         if constexpr (more) load_s(next);
+        slot = next;
       };
-      for (int kt = 0; kt + 2 < KT; ++kt) stage(kt, ic<1>{}, ic<1>{});
-      if (KT > 1) stage(KT - 2, ic<1>{}, ic<0>{});
-      stage(KT - 1, ic<0>{}, ic<0>{});
+      int kt = 0;
+      for (; kt + STAGES < KT; ++kt) stage(kt, ic<1>{}, ic<1>{}, ic<1>{});
+      if (kt + STAGES == KT) stage(kt++, ic<1>{}, ic<1>{}, ic<0>{});
+      for (; kt + 1 < KT; ++kt) stage(kt, ic<1>{}, ic<0>{}, ic<0>{});
+      stage(kt, ic<0>{}, ic<0>{}, ic<0>{});
     }
     __syncthreads();  // the slots may be used for something else
   }

@@ -49,8 +49,17 @@ static hipError_t launch_fp8(const Fp8GemmArgs &g, hipStream_t st) {
 // exact: c f32; otherwise fp16 or bf16.
 hipError_t rk_launch_gemm_fp8(const Fp8GemmArgs &g, bool exact, hipStream_t st) {
   if (exact != (g.c_dtype == RK_DTYPE_F32)) return hipErrorInvalidValue;
-  if (exact) return launch_fp8<Fp8Tile<128, 128, 2, 2, 2, true>>(g, st);
-  const int64_t big = (int64_t)((g.m + 255) / 256) * ((g.n + 255) / 256);
-  if (big >= g.num_cus) return launch_fp8<Fp8Tile<256, 256, 4, 2, 2, false>>(g, st);
+  // At most two 64 × 128 tiles per CU: a round of them ends sooner than one of 128 × 128 would. us so and with these, MI355X,
+  // 16-bit results: 3633 × 1024 × 2560 18.1 and 20.3, 512 × 4096 × 4096 16.4 and 26.7, 1024 × 4096 × 4096 (twice as many
+  // tiles) 26 and 30, 512 × 16384 × 2048 29 and 22; f32: 2048 × 1024 × 4096 29 and 40, 2048 × 4096 × 2048 42 and 37.
+  const bool small = (int64_t)((g.m + 63) / 64) * ((g.n + 127) / 128) <= 2 * g.num_cus;
+  if (exact) return small ? launch_fp8<Fp8Tile<64, 128, 2, 2, 3, true>>(g, st) : launch_fp8<Fp8Tile<128, 128, 2, 2, 2, true>>(g, st);
+  if (small) return launch_fp8<Fp8Tile<64, 128, 2, 2, 3, false>>(g, st);
+  // 256 × 256 where its rounds, one tile a CU, are less than two thirds of those of 128 × 128, two a CU: a round of them
+  // takes 47 to 60 us at K = 4096, one of these 34 to 38 (2560 × 4096: 54 and 63; 2048 × 4096: 51 and 38; 4608 × 4096: 100
+  // and 96).
+  const int64_t big = (int64_t)((g.m + 255) / 256) * ((g.n + 255) / 256), mid = (int64_t)((g.m + 127) / 128) * ((g.n + 127) / 128);
+  const auto rounds = [&](int64_t tiles, int64_t at_once) { return (tiles + at_once - 1) / at_once; };
+  if (3 * rounds(big, g.num_cus) < 2 * rounds(mid, 2 * g.num_cus)) return launch_fp8<Fp8Tile<256, 256, 4, 2, 2, false>>(g, st);
   return launch_fp8<Fp8Tile<128, 128, 2, 2, 2, false>>(g, st);
 }

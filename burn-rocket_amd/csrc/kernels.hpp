@@ -318,7 +318,8 @@ struct Fp8FewArgs {
   int groups;                   // set by the launcher: blocks of n side by side in a workgroup
 };
 bool rk_fp8_few_fits_x(int64_t m, int kt);
-bool rk_fp8_few_fits_codes(int64_t m);
+bool rk_fp8_few_wants_x(int64_t m, int kt);
+bool rk_fp8_few_fits_codes(int64_t m, int64_t n, bool exact, int num_cus);
 hipError_t rk_launch_fp8_few(const Fp8FewArgs &g, int x_dtype, bool exact, hipStream_t st);
 // Any rows (gemm_fp8.hip): codes [m, k] with scales [m, kt].
 struct Fp8GemmArgs {

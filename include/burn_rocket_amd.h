@@ -342,8 +342,9 @@ int rk_quantize_fp8_dev(const void *x, int x_dtype, int64_t m, int64_t k, uint8_
 int rk_matmul_fp8_codes_dev(rk_weight_id id, const uint8_t *a, const float *a_scale, int64_t m, int64_t k, void *c,
                             int c_dtype, rk_stream stream);
 /* x quantized on the way, then the product: the results of the two calls above up to
- * the order of sums. Up to 32 rows of at most 64 KB of codes in all are one launch that uses no library
- * memory; other sizes hold the codes in library scratch, and are refused inside a stream
+ * the order of sums. Up to 32 rows of at most 64 KB of codes in all can be captured:
+ * they need no library memory (while small, or inside a capture, they are one launch).
+ * Other sizes hold the codes in library scratch, and are refused inside a stream
  * capture (RK_E_UNSUPPORTED): capture the two calls instead. rk_matmul takes fp8
  * weights too. */
 int rk_matmul_fp8_dev(rk_weight_id id, const void *x, int x_dtype, int64_t m, int64_t k, void *c, int c_dtype,
