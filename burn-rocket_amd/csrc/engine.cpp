@@ -14,6 +14,7 @@
 #include <cstring>
 #include <functional>
 #include <mutex>
+#include <numeric>
 #include <string>
 #include <unordered_map>
 #include <unordered_set>
@@ -151,6 +152,7 @@ struct MoePlan {
   int32_t *slot = nullptr;    // [s, top_k] bucket rows of a token, ascending expert id
   MoeTile *tiles = nullptr;   // [n_tiles] in expert order (down)
   MoeTile *tiles_gu = nullptr;  // [n_tiles] the same tiles, longest first (gate|up)
+  bool pairs = false;         // (fp8) each row is a tile of its own, a token's consecutive, in ascending expert id
   void *block = nullptr;      // the lists' allocation, when the plan owns it
   uint64_t weight = 0;        // expert stack the plan was made for
   // Streams of the runs that read the lists: a library stream is
@@ -2006,6 +2008,7 @@ struct MoeLists {
   int top_k = 0;
   int64_t rows = 0;
   int n_tiles = 0, tile_rows = 128, max_rows = 0;
+  bool pairs = false;        // MoePlan::pairs
   std::vector<int64_t> off;  // [n_experts + 1] first bucket row of each expert
   size_t roww = 0, tiles = 0, tiles_gu = 0, slot = 0, bytes = 0;
 };
@@ -2019,6 +2022,12 @@ int moe_fp8_tile_rows(const Weight &w, int64_t rows) {
   if (rows <= moe_fp8_few_limit(w)) return std::min(rk_fp8_few_rows(w.gu_ws_stride), rk_fp8_few_rows(w.dn_ws_stride));
   return rows >= 192 * (int64_t)w.n_experts ? 256 : 128;
 }
+// Rows as tiles of their own, the second product with the sum over experts: while hardly two tokens share an expert, whose
+// weights are read for each. Router and experts of a layer of 128 experts (top 8), us in lists and so, MI355X: 1 token 28 and
+// 22, 4 tokens 51 and 43, 8 tokens 72 and 68, 12 tokens 82 and 93; of 8 wide ones (top 2): 2 tokens 30 and 23, 8 tokens 49 and 57.
+bool moe_fp8_pairs(const Weight &w, int64_t rows, int top_k) {
+  return rk_knob("RK_MOE_FP8_ROWS", 0) == 0 && 2 * rows <= w.n_experts && rk_fp8_token_fits(top_k, w.dn_ws_stride);
+}
 
 // Checks the ids and sizes the lists: tiles of ≤ rk_moe_tile_rows() rows (two
 // tiles of one expert sit next to each other, so the second read of its
@@ -2029,6 +2038,8 @@ int moe_lists(const Weight &w, int64_t s, int top_k, const uint32_t *ids, MoeLis
   l->top_k = top_k;
   l->rows = s * top_k;
   l->tile_rows = w.moe_fp8 ? moe_fp8_tile_rows(w, l->rows) : rk_moe_tile_rows();
+  l->pairs = w.moe_fp8 && moe_fp8_pairs(w, l->rows, top_k);
+  if (l->pairs) l->tile_rows = 1;
   l->off.assign(E + 1, 0);
   for (int64_t i = 0; i < l->rows; ++i) {
     if (ids[i] >= (uint32_t)E) return fail(RK_E_SHAPE, "rk_moe_plan", "expert id out of range");
@@ -2062,6 +2073,19 @@ int moe_lists(const Weight &w, int64_t s, int top_k, const uint32_t *ids, MoeLis
 void moe_fill_rows(const MoeLists &l, const uint32_t *ids, const float *wts, uint8_t *host) {
   int32_t *tok = (int32_t *)host;
   float *roww = (float *)(host + l.roww);
+  MoeTile *tiles = (MoeTile *)(host + l.tiles), *gu = (MoeTile *)(host + l.tiles_gu);
+  if (l.pairs) {
+    std::vector<int64_t> order(l.rows);
+    std::iota(order.begin(), order.end(), (int64_t)0);
+    for (int64_t t = 0; t < l.s; ++t)
+      std::stable_sort(order.begin() + t * l.top_k, order.begin() + (t + 1) * l.top_k, [&](int64_t a, int64_t b) { return ids[a] < ids[b]; });
+    for (int64_t row = 0; row < l.rows; ++row) {
+      tok[row] = (int32_t)(row / l.top_k);
+      roww[row] = wts[order[row]];
+      tiles[row] = gu[row] = MoeTile{(int)ids[order[row]], (int)row, 1};
+    }
+    return;
+  }
   std::vector<int64_t> fill(l.off.begin(), l.off.end() - 1);
   for (int64_t t = 0, i = 0; t < l.s; ++t)
     for (int j = 0; j < l.top_k; ++j, ++i) {
@@ -2069,7 +2093,6 @@ void moe_fill_rows(const MoeLists &l, const uint32_t *ids, const float *wts, uin
       tok[row] = (int32_t)t;
       roww[row] = wts[i];
     }
-  MoeTile *tiles = (MoeTile *)(host + l.tiles), *gu = (MoeTile *)(host + l.tiles_gu);
   int n = 0;
   for (int e = 0; e + 1 < (int)l.off.size(); ++e)
     for (int64_t r = l.off[e]; r < l.off[e + 1]; r += l.tile_rows)
@@ -2095,6 +2118,7 @@ void moe_bind(const MoeLists &l, uint8_t *dev, MoePlan *plan) {
   plan->top_k = l.top_k;
   plan->rows = l.rows;
   plan->n_tiles = l.n_tiles;
+  plan->pairs = l.pairs;
   plan->tile_rows = l.tile_rows;
   plan->max_rows = l.max_rows;
   plan->tok = (int32_t *)dev;
@@ -2186,6 +2210,14 @@ int moe_run_fp8(CallScope &cs, const Weight &w, const MoePlan &plan, const void 
     g.c = yb;
     g.tiles = plan.tiles;
     g.row_w = plan.roww;
+    if (plan.pairs) {
+      g.c = y;
+      g.c_dtype = dtype;
+      g.top_k = plan.top_k;
+      g.accumulate = accumulate;
+      HIP_TRY(rk_launch_fp8_token(g, plan.s, exact2, st), op);
+      return RK_OK;
+    }
     HIP_TRY(rk_launch_fp8_few_down(g, plan.tile_rows, plan.n_tiles, exact2, st), op);
   } else {
     void *xq, *xs, *as;
@@ -3480,6 +3512,7 @@ extern "C" int rk_moe_plan_route_dev(void *plan, int64_t s, const uint32_t *ids,
     p->rows = s * p->top_k;
     if (s == 0) return RK_OK;
     const int T = routed_tile_rows(*w, s, p->rows);
+    p->pairs = w->moe_fp8 && moe_fp8_pairs(*w, p->rows, p->top_k);
     p->tile_rows = T;
     p->max_rows = (int)std::min<int64_t>(T, p->rows);
     p->n_tiles = (int)routed_tiles(*w, p->rows, T);
@@ -3499,7 +3532,13 @@ extern "C" int rk_moe_plan_route_dev(void *plan, int64_t s, const uint32_t *ids,
     g.slot = p->slot;
     g.tiles = p->tiles;
     g.tiles_gu = p->tiles_gu;
-    HIP_TRY(rk_launch_moe_lists(g, st), op);
+    if (p->pairs) {
+      p->tile_rows = 1;
+      p->n_tiles = (int)p->rows;
+      HIP_TRY(rk_launch_moe_pairs(g, st), op);
+    } else {
+      HIP_TRY(rk_launch_moe_lists(g, st), op);
+    }
     return RK_OK;
   });
 }

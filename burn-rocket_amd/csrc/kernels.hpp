@@ -316,6 +316,7 @@ struct Fp8FewArgs {
   int64_t w_stride, ws_stride;  // bytes and scales per expert
   int64_t up_scales;            // scales from a gate block's to its up block's
   int groups;                   // set by the launcher: blocks of n side by side in a workgroup
+  int top_k, accumulate;        // rk_launch_fp8_token
 };
 bool rk_fp8_few_fits_x(int64_t m, int kt);
 bool rk_fp8_few_wants_x(int64_t m, int kt);
@@ -364,6 +365,8 @@ struct RouteListArgs {
   MoeTile *tiles, *tiles_gu;  // [max_tiles]: rows without an expert are tiles of expert -1, unused ones have no rows
 };
 int rk_moe_lists_blocks(int64_t rows);
+// Pairs as tiles of their own, a token's in ascending expert id: row t·top_k + .. and the tile of that index.
+hipError_t rk_launch_moe_pairs(const RouteListArgs &g, hipStream_t st);
 hipError_t rk_launch_moe_lists(const RouteListArgs &g, hipStream_t st);
 struct CombineArgs {
   const void *rows;      // [bucket rows, n], weighted: f32, or fp16 with a scale per `group` outputs
@@ -381,6 +384,9 @@ hipError_t rk_launch_moe_combine(const CombineArgs &g, int dtype, hipStream_t st
 int rk_fp8_few_rows(int kt);
 hipError_t rk_launch_fp8_few_gate_up(const Fp8FewArgs &g, int x_dtype, int tile_rows, int n_tiles, bool exact, hipStream_t st);
 hipError_t rk_launch_fp8_few_down(const Fp8FewArgs &g, int tile_rows, int n_tiles, bool exact, hipStream_t st);
+// Second product of s tokens, top_k f32 rows and tiles each, and their sum: c [s, n] of c_dtype.
+bool rk_fp8_token_fits(int top_k, int kt);
+hipError_t rk_launch_fp8_token(const Fp8FewArgs &g, int64_t s, bool exact, hipStream_t st);
 
 // fp8 experts on tiles of up to 128 or 256 rows (moe_fp8.hip).
 struct Fp8MoeArgs {

@@ -384,6 +384,19 @@ __device__ __forceinline__ uint64_t block_exclusive(uint64_t x, uint64_t *s_wave
   return base + inc - x;
 }
 
+// Where pair j of token t, of expert e, comes among the token's in ascending expert id (the same expert twice: in their order).
+__device__ __forceinline__ int place_in_token(const RouteListArgs &g, int64_t t, int e, int j) {
+  int at = 0;
+  for (int o0 = 0; o0 < g.top_k; o0 += 8) {
+    int oe[8];
+#pragma unroll
+    for (int o = 0; o < 8; ++o) oe[o] = o0 + o < g.top_k ? (int)min(g.ids[t * g.top_k + o0 + o], (uint32_t)g.n_experts) : INT_MAX;
+#pragma unroll
+    for (int o = 0; o < 8; ++o) at += oe[o] < e || (oe[o] == e && o0 + o < j);
+  }
+  return at;
+}
+
 __global__ __launch_bounds__(LB) void moe_lists_kernel(const RouteListArgs g, int n_blocks) {
   constexpr int ME = RK_ROUTE_MAX_EXPERTS;
   __shared__ int s_all[ME + 1], s_at[ME + 1];   // rows of each expert; those of earlier blocks, then the first row of this one's
@@ -450,15 +463,7 @@ __global__ __launch_bounds__(LB) void moe_lists_kernel(const RouteListArgs g, in
     int row = s_at[e] + rank;
     for (int w = 0; w < wave; ++w) row += s_cnt[w][e];
     const int64_t t = i / g.top_k;
-    const int j = (int)(i - t * g.top_k);
-    int at = 0;
-    for (int o0 = 0; o0 < g.top_k; o0 += 8) {
-      int oe[8];
-#pragma unroll
-      for (int o = 0; o < 8; ++o) oe[o] = o0 + o < g.top_k ? (int)min(g.ids[t * g.top_k + o0 + o], (uint32_t)E) : INT_MAX;
-#pragma unroll
-      for (int o = 0; o < 8; ++o) at += oe[o] < e || (oe[o] == e && o0 + o < j);
-    }
+    const int at = place_in_token(g, t, e, (int)(i - t * g.top_k));
     g.tok[row] = (int32_t)t;
     g.row_w[row] = e < E ? g.wts[i] : 0.f;
     g.slot[t * g.top_k + at] = row;
@@ -512,6 +517,21 @@ hipError_t rk_launch_moe_lists(const RouteListArgs &g, hipStream_t st) {
   return hipGetLastError();
 }
 int rk_moe_lists_blocks(int64_t rows) { return (int)((rows + LB - 1) / LB); }
+
+// Few tokens: no sorting over the batch, one trip to memory instead of four one behind the other (2 us instead of 6).
+__global__ __launch_bounds__(256) void moe_pairs_kernel(const RouteListArgs g) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= g.rows) return;
+  const int64_t t = i / g.top_k;
+  const int e = (int)min(g.ids[i], (uint32_t)g.n_experts), row = (int)(t * g.top_k) + place_in_token(g, t, e, (int)(i - t * g.top_k));
+  g.tok[row] = (int32_t)t;
+  g.row_w[row] = e < g.n_experts ? g.wts[i] : 0.f;
+  g.tiles[row] = g.tiles_gu[row] = MoeTile{e < g.n_experts ? e : -1, row, 1};
+}
+hipError_t rk_launch_moe_pairs(const RouteListArgs &g, hipStream_t st) {
+  hipLaunchKernelGGL(moe_pairs_kernel, dim3((unsigned)((g.rows + 255) / 256)), dim3(256), 0, st, g);
+  return hipGetLastError();
+}
 
 // The weighted rows of each token to its result, in ascending expert id: y (+)= Σ rows. A thread per eight values; a
 // token's rows are asked for four at a time. Bound by the rows' bytes.

@@ -475,3 +475,89 @@ def test_wide_experts(rk):
     want, most = experts(x, ids, wts, stack, "f32")
     for got in (run_routed(rk, wid, rk.routed_plan(wid, s, k), x, ids, wts), run_host(rk, wid, x, ids, wts)):
         assert (np.abs(got - want) <= most + np.abs(want) * 2.0**-23).all()
+
+
+# ------------------------------------------- few tokens: each pair by itself ----
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("s,e,k,h,i", [(1, 64, 8, 144, 80), (4, 64, 8, 272, 256), (3, 128, 16, 160, 144), (1, 70, 32, 64, 400),
+                                       (1, 70, 33, 48, 64), (8, 16, 1, 48, 1040), (1, 4, 2, 1040, 16), (1, 16, 8, 32, 8208)])
+def test_fp8_experts_of_few_tokens(rk, s, e, k, h, i, dtype):
+    """At most half as many pairs as experts; a top_k and an inter that are too large for that among them."""
+    test_fp8_experts(rk, None, s, e, k, h, i, dtype)
+
+
+@pytest.mark.parametrize("how", ["any", "one", "twice"])
+def test_few_tokens_without_some_experts(rk, how):
+    """A token's result is its own: that of the same token among many, up to the order of sums, and bit for bit that of
+    the host's lists. Ids that name no expert add nothing, whatever their weight."""
+    note(f"few tokens, no expert, {how}")
+    r = np.random.default_rng(21)
+    s, e, k, h, i = 5, 64, 6, 176, 144
+    stack = [ref.random_stack(r, e, n, kk) for n, kk in ((i, h), (i, h), (h, i))]
+    wid = rk.pack_moe_fp8(*stack[0], *stack[1], *stack[2])
+    x = r.standard_normal((s, h)).astype(np.float32)
+    ids, wts = choices(r, s, e, k, how)
+    plan = rk.routed_plan(wid, 40, k)
+    gone = r.random((s, k)) < 0.4
+    gone[0], gone[1] = False, True
+    for bad in (np.uint32(e), np.uint32(0xFFFFFFFF)):
+        mine, weights = np.where(gone, bad, ids).astype(np.uint32), np.where(gone, np.float32(np.nan), wts).astype(np.float32)
+        zero = np.where(gone, np.float32(0), wts).astype(np.float32)
+        got = run_routed(rk, wid, plan, x, mine, weights)
+        assert (got == run_host(rk, wid, x, ids, zero)).all() and (got[1] == 0).all()
+        y0 = r.standard_normal((s, h)).astype(np.float32)
+        got = run_routed(rk, wid, plan, x, mine, weights, y0, True)
+        assert (got == run_host(rk, wid, x, ids, zero, y0, True)).all() and (got[1] == y0[1]).all()
+    # the plan between small batches and large ones
+    many = np.repeat(x, 8, 0)
+    large = run_routed(rk, wid, plan, many, np.repeat(ids, 8, 0), np.repeat(wts, 8, 0))
+    want, most = experts(x, ids, wts, stack, "f32")
+    for n in range(s):
+        assert (run_routed(rk, wid, plan, x[n:n + 1], ids[n:n + 1], wts[n:n + 1]) == run_routed(rk, wid, plan, x, ids, wts)[n]).all()
+        assert (np.abs(large[8 * n] - want[n]) <= most[n] + np.abs(want[n]) * 2.0**-23).all()
+    plan.destroy()
+
+
+def test_few_tokens_with_non_finite_rows(rk):
+    """What is not finite in a token's rows or in an expert's weights stays with the tokens that it reaches."""
+    note("few tokens, not finite")
+    r = np.random.default_rng(22)
+    s, e, k, h, i = 4, 32, 3, 160, 144
+    stack = [ref.random_stack(r, e, n, kk) for n, kk in ((i, h), (i, h), (h, i))]
+    stack[2][0][5, 7, 9] = 127  # NaN in expert 5's second matrix
+    wid = rk.pack_moe_fp8(*stack[0], *stack[1], *stack[2])
+    x = r.standard_normal((s, h)).astype(np.float32)
+    x[1, 3], x[2, 130] = np.inf, np.nan
+    ids = np.array([[5, 1, 2], [6, 7, 8], [9, 10, 11], [12, 13, 14]], np.uint32)
+    wts = np.ones((s, k), np.float32)
+    got = run_routed(rk, wid, rk.routed_plan(wid, s, k), x, ids, wts)
+    clean, most = experts(np.where(np.isfinite(x), x, 0), ids, wts, [(np.where(c == 127, 0, c).astype(np.uint8), sc) for c, sc in stack], "f32")
+    assert np.isnan(got[0, 7]) and not np.isfinite(got[1]).any() and np.isnan(got[2]).all()
+    for n, cols in ((0, np.arange(h) != 7), (3, np.full(h, True))):
+        assert (np.abs(got[n] - clean[n])[cols] <= (most[n] + np.abs(clean[n]) * 2.0**-23)[cols]).all()
+
+
+def test_few_tokens_captured(rk):
+    note("few tokens, captured")
+    from test_gpu_sequences import Graph
+    lib, r = rk.lib(), np.random.default_rng(23)
+    e, k, h, i, s = 32, 4, 256, 160, 3
+    wid = int(rk.pack_moe_fp8(*ref.random_stack(r, e, i, h), *ref.random_stack(r, e, i, h), *ref.random_stack(r, e, h, i)))
+    plan, st = rk.routed_plan(wid, s, k), rk.new_stream()
+    b = [rk.DeviceBuffer.from_array(a) for a in (np.zeros((s, h), np.float32), np.zeros((s, k), np.uint32), np.zeros((s, k), np.float32), np.zeros((s, h), np.float32))]
+
+    def layer():
+        ok(rk, lib.rk_moe_plan_route_dev(plan.ptr, s, b[1].ptr, b[2].ptr, st))
+        ok(rk, lib.rk_moe_experts_planned_dev(wid, plan.ptr, b[0].ptr, b[3].ptr, st))
+    g = Graph(st, layer)
+    for n in range(4):
+        x = r.standard_normal((s, h)).astype(np.float32)
+        ids, wts = choices(r, s, e, k, "any")
+        for buf, a in zip(b, (x, ids, wts)):
+            buf.upload(a)
+        g.replay()
+        rk.synchronize(st)
+        assert (b[3].download((s, h), np.float32) == run_host(rk, wid, x, ids, wts)).all(), f"replay {n}"
+    g.destroy()
+    plan.destroy()
+    rk.destroy_stream(st)
