@@ -414,6 +414,9 @@ __global__ __launch_bounds__(LB) void moe_lists_kernel(const RouteListArgs g, in
     other[b] = !counted && b < n_blocks && o < g.rows ? (int)min(g.ids[o], (uint32_t)E) : -1;
   }
   const int e = in ? (int)min(g.ids[i], (uint32_t)E) : E + 1;
+  const int t = (int)(in ? i : 0) / g.top_k;
+  const float weight = in && e < E ? g.wts[i] : 0.f;
+  const int at = in ? place_in_token(g, t, e, (int)(i - (int64_t)t * g.top_k)) : 0;
   for (int x = tid; x <= E; x += LB) {
     s_all[x] = s_at[x] = 0;
 #pragma unroll
@@ -442,7 +445,7 @@ __global__ __launch_bounds__(LB) void moe_lists_kernel(const RouteListArgs g, in
       s_all[x] = all;
       s_at[x] = before;
     }
-  } else if (n_blocks == 1) {
+  } else if (n_blocks == 1 && block == 0) {
     if (in && rank == 0) atomicAdd(&s_all[e], __popcll(peers));
   } else {
 #pragma unroll
@@ -462,13 +465,11 @@ __global__ __launch_bounds__(LB) void moe_lists_kernel(const RouteListArgs g, in
   if (in) {
     int row = s_at[e] + rank;
     for (int w = 0; w < wave; ++w) row += s_cnt[w][e];
-    const int64_t t = i / g.top_k;
-    const int at = place_in_token(g, t, e, (int)(i - t * g.top_k));
-    g.tok[row] = (int32_t)t;
-    g.row_w[row] = e < E ? g.wts[i] : 0.f;
-    g.slot[t * g.top_k + at] = row;
+    g.tok[row] = t;
+    g.row_w[row] = weight;
+    g.slot[(int64_t)t * g.top_k + at] = row;
   }
-  if (blockIdx.x != 0) return;
+  if (block < n_blocks) return;
 
   // Tiles in expert order, and longest first: by quarters of tile_rows, in expert order within one. Thread x makes expert
   // x's; four 16-bit counts (quarters 4, 3, 2, 1) share a word of the sums.
@@ -513,7 +514,7 @@ __global__ __launch_bounds__(LB) void moe_lists_kernel(const RouteListArgs g, in
 hipError_t rk_launch_moe_lists(const RouteListArgs &g, hipStream_t st) {
   const int nb = (int)((g.rows + LB - 1) / LB);
   if (nb > COUNT_SELF) hipLaunchKernelGGL(moe_count_kernel, dim3(nb), dim3(LB), 0, st, g);
-  hipLaunchKernelGGL(moe_lists_kernel, dim3(nb), dim3(LB), 0, st, g, nb);
+  hipLaunchKernelGGL(moe_lists_kernel, dim3(nb + 1), dim3(LB), 0, st, g, nb);
   return hipGetLastError();
 }
 int rk_moe_lists_blocks(int64_t rows) { return (int)((rows + LB - 1) / LB); }
