@@ -980,10 +980,14 @@ int gemm_f16_run(CallScope &cs, const void *a, const void *b, void *c, int64_t m
   return RK_OK;
 }
 
-// c = codes · Wᵀ for an fp8 weight. Results that stay f32 take the products with f32 sums (fp8.hpp).
+// Whether a product takes the bf16 instructions (fp8.hpp): where its result keeps what the fp8 instructions cut (`wide`), and
+// where K is one block, whose few terms average too little of it out (2^-14 of Σ|terms| at K = 16). Such a product's time is its
+// results' bytes either way.
+bool fp8_exact(bool wide, int64_t kt) { return wide || kt == 1; }
+// c = codes · Wᵀ for an fp8 weight.
 int fp8_product_run(const Weight &w, const uint8_t *a, const float *as, int64_t m, void *c, int c_dtype, hipStream_t st,
                     const char *op) {
-  const bool exact = c_dtype == RK_DTYPE_F32;
+  const bool exact = fp8_exact(c_dtype == RK_DTYPE_F32, w.ws_stride);
   if (rk_fp8_few_fits_codes(m, w.n, exact, g_eng->num_cus)) {
     Fp8FewArgs g{};
     g.x = a;
@@ -2173,8 +2177,8 @@ int moe_run_fp8(CallScope &cs, const Weight &w, const MoePlan &plan, const void 
   const char *op = "rk_moe_experts_fp8_dev";
   const int64_t H = w.hidden, I = w.inter, R = plan.rows;
   hipStream_t st = cs.st;
-  const bool few = plan.tile_rows < 128, exact1 = dtype != RK_DTYPE_BF16, exact2 = dtype == RK_DTYPE_F32;
   const int64_t KTh = w.gu_ws_stride, KTi = w.dn_ws_stride;
+  const bool few = plan.tile_rows < 128, exact1 = fp8_exact(dtype != RK_DTYPE_BF16, KTh), exact2 = fp8_exact(dtype == RK_DTYPE_F32, KTi);
   void *act, *yb, *ys = nullptr;
   RK_TRY(moe_buf(cs, plan, "moe_act", few ? (size_t)R * I * 4 : (size_t)R * KTi * 128, &act));
   RK_TRY(moe_buf(cs, plan, "moe_yb", (size_t)R * H * 4, &yb));
@@ -3270,116 +3274,126 @@ int fp8_weight(uint64_t id, int64_t m, int64_t k, Weight **w, const char *op) {
 }  // namespace
 
 extern "C" int rk_pack_fp8(const uint8_t *codes, const float *scales, int64_t n, int64_t k, rk_weight_id *id) {
-  std::lock_guard<std::mutex> lk(g_mu);
   const char *op = "rk_pack_fp8";
-  RK_TRY(ensure(op));
-  if (!codes || !scales || !id) return fail(RK_E_SHAPE, op, "null buffer");
-  RK_TRY(fp8_check_shape(n, k, op));
-  Weight w;
-  PackGuard guard(w);
-  RK_TRY(fp8_alloc(w, n, k, op));
-  CallScope cs(g_eng->stream);
-  void *dev;
-  RK_TRY(scratch(cs, "pack_blk", (size_t)n * k, &dev));
-  HIP_TRY(hipMemcpyAsync(dev, codes, (size_t)n * k, hipMemcpyHostToDevice, cs.st), op);
-  HIP_TRY(rk_launch_fp8_layout((const uint8_t *)dev, n, (int)k, 32, 0, (uint8_t *)w.codes, cs.st), op);
-  HIP_TRY(hipMemcpyAsync(w.scales, scales, (size_t)((n + 127) / 128) * w.ws_stride * 4, hipMemcpyHostToDevice, cs.st), op);
-  HIP_TRY(hipStreamSynchronize(cs.st), op);
-  *id = guard.register_weight();
-  return RK_OK;
+  return no_throw(op, [&]() -> int {
+    std::lock_guard<std::mutex> lk(g_mu);
+    RK_TRY(ensure(op));
+    if (!codes || !scales || !id) return fail(RK_E_SHAPE, op, "null buffer");
+    RK_TRY(fp8_check_shape(n, k, op));
+    Weight w;
+    PackGuard guard(w);
+    RK_TRY(fp8_alloc(w, n, k, op));
+    CallScope cs(g_eng->stream);
+    void *dev;
+    RK_TRY(scratch(cs, "pack_blk", (size_t)n * k, &dev));
+    HIP_TRY(hipMemcpyAsync(dev, codes, (size_t)n * k, hipMemcpyHostToDevice, cs.st), op);
+    HIP_TRY(rk_launch_fp8_layout((const uint8_t *)dev, n, (int)k, 32, 0, (uint8_t *)w.codes, cs.st), op);
+    HIP_TRY(hipMemcpyAsync(w.scales, scales, (size_t)((n + 127) / 128) * w.ws_stride * 4, hipMemcpyHostToDevice, cs.st), op);
+    HIP_TRY(hipStreamSynchronize(cs.st), op);
+    *id = guard.register_weight();
+    return RK_OK;
+  });
 }
 
 extern "C" int rk_pack_fp8_f32(const float *w32, int64_t n, int64_t k, rk_weight_id *id) {
-  std::lock_guard<std::mutex> lk(g_mu);
   const char *op = "rk_pack_fp8_f32";
-  RK_TRY(ensure(op));
-  if (!w32 || !id) return fail(RK_E_SHAPE, op, "null buffer");
-  RK_TRY(fp8_check_shape(n, k, op));
-  Weight w;
-  PackGuard guard(w);
-  RK_TRY(fp8_alloc(w, n, k, op));
-  CallScope cs(g_eng->stream);
-  void *dev;
-  RK_TRY(scratch(cs, "pack_f32", (size_t)n * k * 4, &dev));
-  HIP_TRY(hipMemcpyAsync(dev, w32, (size_t)n * k * 4, hipMemcpyHostToDevice, cs.st), op);
-  HIP_TRY(rk_launch_fp8_pack((const float *)dev, n, (int)k, 32, 0, (uint8_t *)w.codes, w.scales, cs.st), op);
-  HIP_TRY(hipStreamSynchronize(cs.st), op);
-  *id = guard.register_weight();
-  return RK_OK;
+  return no_throw(op, [&]() -> int {
+    std::lock_guard<std::mutex> lk(g_mu);
+    RK_TRY(ensure(op));
+    if (!w32 || !id) return fail(RK_E_SHAPE, op, "null buffer");
+    RK_TRY(fp8_check_shape(n, k, op));
+    Weight w;
+    PackGuard guard(w);
+    RK_TRY(fp8_alloc(w, n, k, op));
+    CallScope cs(g_eng->stream);
+    void *dev;
+    RK_TRY(scratch(cs, "pack_f32", (size_t)n * k * 4, &dev));
+    HIP_TRY(hipMemcpyAsync(dev, w32, (size_t)n * k * 4, hipMemcpyHostToDevice, cs.st), op);
+    HIP_TRY(rk_launch_fp8_pack((const float *)dev, n, (int)k, 32, 0, (uint8_t *)w.codes, w.scales, cs.st), op);
+    HIP_TRY(hipStreamSynchronize(cs.st), op);
+    *id = guard.register_weight();
+    return RK_OK;
+  });
 }
 
 extern "C" int rk_quantize_fp8_dev(const void *x, int x_dtype, int64_t m, int64_t k, uint8_t *q, float *scale, rk_stream stream) {
-  std::lock_guard<std::mutex> lk(g_mu);
   const char *op = "rk_quantize_fp8_dev";
-  RK_TRY(ensure(op));
-  if (m < 0 || m > INT32_MAX) return fail(RK_E_SHAPE, op, "M must be in [0, 2^31)");
-  RK_TRY(fp8_check_shape(1, k, op));
-  if (!fp8_float(x_dtype)) return fail(RK_E_SHAPE, op, "unknown dtype");
-  if (m == 0) return RK_OK;
-  RK_TRY(fp8_rows_check(x, "x", op));
-  RK_TRY(fp8_rows_check(q, "q", op));
-  if (!scale) return fail(RK_E_SHAPE, op, "null scale buffer");
-  HIP_TRY(rk_launch_quantize_fp8(x, x_dtype, m, (int)k, q, k, scale, pick(stream)), op);
-  return RK_OK;
+  return no_throw(op, [&]() -> int {
+    std::lock_guard<std::mutex> lk(g_mu);
+    RK_TRY(ensure(op));
+    if (m < 0 || m > INT32_MAX) return fail(RK_E_SHAPE, op, "M must be in [0, 2^31)");
+    RK_TRY(fp8_check_shape(1, k, op));
+    if (!fp8_float(x_dtype)) return fail(RK_E_SHAPE, op, "unknown dtype");
+    if (m == 0) return RK_OK;
+    RK_TRY(fp8_rows_check(x, "x", op));
+    RK_TRY(fp8_rows_check(q, "q", op));
+    if (!scale) return fail(RK_E_SHAPE, op, "null scale buffer");
+    HIP_TRY(rk_launch_quantize_fp8(x, x_dtype, m, (int)k, q, k, scale, pick(stream)), op);
+    return RK_OK;
+  });
 }
 
 extern "C" int rk_matmul_fp8_codes_dev(rk_weight_id id, const uint8_t *a, const float *a_scale, int64_t m, int64_t k, void *c,
                                        int c_dtype, rk_stream stream) {
-  std::lock_guard<std::mutex> lk(g_mu);
   const char *op = "rk_matmul_fp8_codes_dev";
-  RK_TRY(ensure(op));
-  Weight *w;
-  RK_TRY(fp8_weight(id, m, k, &w, op));
-  if (!fp8_float(c_dtype)) return fail(RK_E_SHAPE, op, "unknown dtype");
-  if (m == 0) return RK_OK;
-  RK_TRY(fp8_rows_check(a, "a", op));
-  RK_TRY(fp8_rows_check(c, "c", op));
-  if (!a_scale) return fail(RK_E_SHAPE, op, "null scale buffer");
-  RK_TRY(fp8_product_run(*w, a, a_scale, m, c, c_dtype, pick(stream), op));
-  g_eng->calls++;
-  return RK_OK;
+  return no_throw(op, [&]() -> int {
+    std::lock_guard<std::mutex> lk(g_mu);
+    RK_TRY(ensure(op));
+    Weight *w;
+    RK_TRY(fp8_weight(id, m, k, &w, op));
+    if (!fp8_float(c_dtype)) return fail(RK_E_SHAPE, op, "unknown dtype");
+    if (m == 0) return RK_OK;
+    RK_TRY(fp8_rows_check(a, "a", op));
+    RK_TRY(fp8_rows_check(c, "c", op));
+    if (!a_scale) return fail(RK_E_SHAPE, op, "null scale buffer");
+    RK_TRY(fp8_product_run(*w, a, a_scale, m, c, c_dtype, pick(stream), op));
+    g_eng->calls++;
+    return RK_OK;
+  });
 }
 
 extern "C" int rk_matmul_fp8_dev(rk_weight_id id, const void *x, int x_dtype, int64_t m, int64_t k, void *c, int c_dtype,
                                  rk_stream stream) {
-  std::lock_guard<std::mutex> lk(g_mu);
   const char *op = "rk_matmul_fp8_dev";
-  RK_TRY(ensure(op));
-  Weight *w;
-  RK_TRY(fp8_weight(id, m, k, &w, op));
-  if (!fp8_float(x_dtype) || !fp8_float(c_dtype)) return fail(RK_E_SHAPE, op, "unknown dtype");
-  if (m == 0) return RK_OK;
-  RK_TRY(fp8_rows_check(x, "x", op));
-  RK_TRY(fp8_rows_check(c, "c", op));
-  hipStream_t st = pick(stream);
-  bool capturing;
-  RK_TRY(is_capturing(st, &capturing, op));
-  // one launch, nothing in library memory
-  if (rk_fp8_few_fits_x(m, w->ws_stride) && (capturing || rk_fp8_few_wants_x(m, w->ws_stride))) {
-    Fp8FewArgs g{};
-    g.x = x;
-    g.m = (int)m;
-    g.n = (int)w->n;
-    g.k = (int)k;
-    g.kt = w->ws_stride;
-    g.w = (const uint8_t *)w->codes;
-    g.ws = w->scales;
-    g.c = c;
-    g.c_dtype = c_dtype;
-    HIP_TRY(rk_launch_fp8_few(g, x_dtype, c_dtype == RK_DTYPE_F32, st), op);
-  } else {
-    if (capturing)
-      return fail(RK_E_UNSUPPORTED, op, "these rows are quantized into library memory, which a graph must not hold: capture "
-                                        "rk_quantize_fp8_dev and rk_matmul_fp8_codes_dev");
-    CallScope cs(st);
-    void *q, *s;
-    RK_TRY(scratch(cs, "fp8_q", (size_t)m * k, &q));
-    RK_TRY(scratch(cs, "fp8_s", (size_t)m * w->ws_stride * 4, &s));
-    HIP_TRY(rk_launch_quantize_fp8(x, x_dtype, m, (int)k, (uint8_t *)q, k, (float *)s, st), op);
-    RK_TRY(fp8_product_run(*w, (const uint8_t *)q, (const float *)s, m, c, c_dtype, st, op));
-  }
-  g_eng->calls++;
-  return RK_OK;
+  return no_throw(op, [&]() -> int {
+    std::lock_guard<std::mutex> lk(g_mu);
+    RK_TRY(ensure(op));
+    Weight *w;
+    RK_TRY(fp8_weight(id, m, k, &w, op));
+    if (!fp8_float(x_dtype) || !fp8_float(c_dtype)) return fail(RK_E_SHAPE, op, "unknown dtype");
+    if (m == 0) return RK_OK;
+    RK_TRY(fp8_rows_check(x, "x", op));
+    RK_TRY(fp8_rows_check(c, "c", op));
+    hipStream_t st = pick(stream);
+    bool capturing;
+    RK_TRY(is_capturing(st, &capturing, op));
+    // one launch, nothing in library memory
+    if (rk_fp8_few_fits_x(m, w->ws_stride) && (capturing || rk_fp8_few_wants_x(m, w->ws_stride))) {
+      Fp8FewArgs g{};
+      g.x = x;
+      g.m = (int)m;
+      g.n = (int)w->n;
+      g.k = (int)k;
+      g.kt = w->ws_stride;
+      g.w = (const uint8_t *)w->codes;
+      g.ws = w->scales;
+      g.c = c;
+      g.c_dtype = c_dtype;
+      HIP_TRY(rk_launch_fp8_few(g, x_dtype, fp8_exact(c_dtype == RK_DTYPE_F32, w->ws_stride), st), op);
+    } else {
+      if (capturing)
+        return fail(RK_E_UNSUPPORTED, op, "these rows are quantized into library memory, which a graph must not hold: capture "
+                                          "rk_quantize_fp8_dev and rk_matmul_fp8_codes_dev");
+      CallScope cs(st);
+      void *q, *s;
+      RK_TRY(scratch(cs, "fp8_q", (size_t)m * k, &q));
+      RK_TRY(scratch(cs, "fp8_s", (size_t)m * w->ws_stride * 4, &s));
+      HIP_TRY(rk_launch_quantize_fp8(x, x_dtype, m, (int)k, (uint8_t *)q, k, (float *)s, st), op);
+      RK_TRY(fp8_product_run(*w, (const uint8_t *)q, (const float *)s, m, c, c_dtype, st, op));
+    }
+    g_eng->calls++;
+    return RK_OK;
+  });
 }
 
 // =========================================================================
@@ -3388,22 +3402,24 @@ extern "C" int rk_matmul_fp8_dev(rk_weight_id id, const void *x, int x_dtype, in
 extern "C" int rk_moe_route_dev(const void *logits, int dtype, int64_t s, int n_experts, int top_k, int score,
                                 const float *bias, int n_groups, int top_groups, int norm_topk, float scale, uint32_t *ids,
                                 float *wts, rk_stream stream) {
-  std::lock_guard<std::mutex> lk(g_mu);
   const char *op = "rk_moe_route_dev";
-  RK_TRY(ensure(op));
-  if (s < 0 || s > INT32_MAX || n_experts <= 0 || top_k <= 0) return fail(RK_E_SHAPE, op, "need 0 <= s < 2^31, n_experts > 0, top_k > 0");
-  if (dtype < RK_DTYPE_F32 || dtype > RK_DTYPE_BF16) return fail(RK_E_SHAPE, op, "unknown dtype");
-  if (score != RK_ROUTE_SOFTMAX && score != RK_ROUTE_SIGMOID) return fail(RK_E_SHAPE, op, "unknown score");
-  if (n_groups <= 0 || n_experts % n_groups != 0 || top_groups <= 0 || top_groups > n_groups)
-    return fail(RK_E_SHAPE, op, "n_groups must divide n_experts, and top_groups be in [1, n_groups]");
-  if (top_k > n_experts / n_groups * top_groups) return fail(RK_E_SHAPE, op, "top_k above the experts of the chosen groups");
-  if (n_experts > RK_ROUTE_MAX_EXPERTS || top_k > RK_ROUTE_MAX_TOP || n_groups > RK_ROUTE_MAX_GROUPS)
-    return fail(RK_E_UNSUPPORTED, op, "up to 1024 experts, 64 choices and 64 groups");
-  if (s == 0) return RK_OK;
-  if (!logits || !ids || !wts) return fail(RK_E_SHAPE, op, "null buffer");
-  RouteArgs g{logits, dtype, s, n_experts, top_k, score, bias, n_groups, top_groups, norm_topk != 0, scale, ids, wts};
-  HIP_TRY(rk_launch_moe_route(g, pick(stream)), op);
-  return RK_OK;
+  return no_throw(op, [&]() -> int {
+    std::lock_guard<std::mutex> lk(g_mu);
+    RK_TRY(ensure(op));
+    if (s < 0 || s > INT32_MAX || n_experts <= 0 || top_k <= 0) return fail(RK_E_SHAPE, op, "need 0 <= s < 2^31, n_experts > 0, top_k > 0");
+    if (dtype < RK_DTYPE_F32 || dtype > RK_DTYPE_BF16) return fail(RK_E_SHAPE, op, "unknown dtype");
+    if (score != RK_ROUTE_SOFTMAX && score != RK_ROUTE_SIGMOID) return fail(RK_E_SHAPE, op, "unknown score");
+    if (n_groups <= 0 || n_experts % n_groups != 0 || top_groups <= 0 || top_groups > n_groups)
+      return fail(RK_E_SHAPE, op, "n_groups must divide n_experts, and top_groups be in [1, n_groups]");
+    if (top_k > n_experts / n_groups * top_groups) return fail(RK_E_SHAPE, op, "top_k above the experts of the chosen groups");
+    if (n_experts > RK_ROUTE_MAX_EXPERTS || top_k > RK_ROUTE_MAX_TOP || n_groups > RK_ROUTE_MAX_GROUPS)
+      return fail(RK_E_UNSUPPORTED, op, "up to 1024 experts, 64 choices and 64 groups");
+    if (s == 0) return RK_OK;
+    if (!logits || !ids || !wts) return fail(RK_E_SHAPE, op, "null buffer");
+    RouteArgs g{logits, dtype, s, n_experts, top_k, score, bias, n_groups, top_groups, norm_topk != 0, scale, ids, wts};
+    HIP_TRY(rk_launch_moe_route(g, pick(stream)), op);
+    return RK_OK;
+  });
 }
 
 namespace {
@@ -3546,54 +3562,56 @@ extern "C" int rk_moe_plan_route_dev(void *plan, int64_t s, const uint32_t *ids,
 extern "C" int rk_pack_moe_fp8(const uint8_t *gate, const float *gate_scales, const uint8_t *up, const float *up_scales,
                                const uint8_t *down, const float *down_scales, int n_experts, int64_t hidden, int64_t inter,
                                rk_weight_id *id) {
-  std::lock_guard<std::mutex> lk(g_mu);
   const char *op = "rk_pack_moe_fp8";
-  RK_TRY(ensure(op));
-  if (n_experts <= 0 || hidden <= 0 || inter <= 0 || hidden % 16 || inter % 16 || hidden > 65536 || inter > 65536)
-    return fail(RK_E_SHAPE, op, "hidden and inter must be multiples of 16 up to 65536");
-  for (const void *b : {(const void *)gate, (const void *)gate_scales, (const void *)up, (const void *)up_scales,
-                        (const void *)down, (const void *)down_scales, (const void *)id})
-    if (!b) return fail(RK_E_SHAPE, op, "null buffer");
-  const int64_t E = n_experts, H = hidden, I = inter, Hb = (H + 127) / 128, Ib = (I + 127) / 128;
-  Weight w;
-  PackGuard guard(w);
-  w.moe = w.moe_fp8 = true;
-  w.n_experts = n_experts;
-  w.hidden = H;
-  w.inter = I;
-  w.n = H;
-  w.k = H;
-  w.group = 128;
-  w.gu_ws_stride = (int)Hb;
-  w.dn_ws_stride = (int)Ib;
-  const int64_t gu = moe_fp8_gu_bytes(w), dn = moe_fp8_dn_bytes(w), sc = Ib * Hb;
-  HIP_TRY(hipMalloc((void **)&w.gu_codes, (size_t)(E * gu)), op);
-  HIP_TRY(hipMalloc((void **)&w.dn_codes, (size_t)(E * dn)), op);
-  HIP_TRY(hipMalloc((void **)&w.gu_scales, (size_t)(E * 2 * sc) * 4), op);
-  HIP_TRY(hipMalloc((void **)&w.dn_scales, (size_t)(E * sc) * 4), op);
-  w.bytes = (size_t)(E * (gu + dn) + 3 * E * sc * 4);
-  CallScope cs(g_eng->stream);
-  hipStream_t st = cs.st;
-  HIP_TRY(hipMemsetAsync(w.gu_codes, 0, (size_t)(E * gu), st), op);  // the padding
-  HIP_TRY(hipMemsetAsync(w.dn_codes, 0, (size_t)(E * dn), st), op);
-  // An expert at a time: its three matrices up, then into their layouts (gate and up rows in turns of 32).
-  const size_t one = (size_t)(H * I);
-  uint8_t *dev;
-  RK_TRY(scratch(cs, "pack_blk", 3 * one, (void **)&dev));
-  for (int64_t e = 0; e < E; ++e) {
-    HIP_TRY(hipMemcpyAsync(dev, gate + e * one, one, hipMemcpyHostToDevice, st), op);
-    HIP_TRY(hipMemcpyAsync(dev + one, up + e * one, one, hipMemcpyHostToDevice, st), op);
-    HIP_TRY(hipMemcpyAsync(dev + 2 * one, down + e * one, one, hipMemcpyHostToDevice, st), op);
-    HIP_TRY(rk_launch_fp8_layout(dev, I, (int)H, 64, 0, (uint8_t *)w.gu_codes + e * gu, st), op);
-    HIP_TRY(rk_launch_fp8_layout(dev + one, I, (int)H, 64, 32, (uint8_t *)w.gu_codes + e * gu, st), op);
-    HIP_TRY(rk_launch_fp8_layout(dev + 2 * one, H, (int)I, 32, 0, (uint8_t *)w.dn_codes + e * dn, st), op);
-    HIP_TRY(hipMemcpyAsync(w.gu_scales + e * 2 * sc, gate_scales + e * sc, (size_t)sc * 4, hipMemcpyHostToDevice, st), op);
-    HIP_TRY(hipMemcpyAsync(w.gu_scales + e * 2 * sc + sc, up_scales + e * sc, (size_t)sc * 4, hipMemcpyHostToDevice, st), op);
-  }
-  HIP_TRY(hipMemcpyAsync(w.dn_scales, down_scales, (size_t)(E * sc) * 4, hipMemcpyHostToDevice, st), op);
-  HIP_TRY(hipStreamSynchronize(st), op);
-  *id = guard.register_weight();
-  return RK_OK;
+  return no_throw(op, [&]() -> int {
+    std::lock_guard<std::mutex> lk(g_mu);
+    RK_TRY(ensure(op));
+    if (n_experts <= 0 || hidden <= 0 || inter <= 0 || hidden % 16 || inter % 16 || hidden > 65536 || inter > 65536)
+      return fail(RK_E_SHAPE, op, "hidden and inter must be multiples of 16 up to 65536");
+    for (const void *b : {(const void *)gate, (const void *)gate_scales, (const void *)up, (const void *)up_scales,
+                          (const void *)down, (const void *)down_scales, (const void *)id})
+      if (!b) return fail(RK_E_SHAPE, op, "null buffer");
+    const int64_t E = n_experts, H = hidden, I = inter, Hb = (H + 127) / 128, Ib = (I + 127) / 128;
+    Weight w;
+    PackGuard guard(w);
+    w.moe = w.moe_fp8 = true;
+    w.n_experts = n_experts;
+    w.hidden = H;
+    w.inter = I;
+    w.n = H;
+    w.k = H;
+    w.group = 128;
+    w.gu_ws_stride = (int)Hb;
+    w.dn_ws_stride = (int)Ib;
+    const int64_t gu = moe_fp8_gu_bytes(w), dn = moe_fp8_dn_bytes(w), sc = Ib * Hb;
+    HIP_TRY(hipMalloc((void **)&w.gu_codes, (size_t)(E * gu)), op);
+    HIP_TRY(hipMalloc((void **)&w.dn_codes, (size_t)(E * dn)), op);
+    HIP_TRY(hipMalloc((void **)&w.gu_scales, (size_t)(E * 2 * sc) * 4), op);
+    HIP_TRY(hipMalloc((void **)&w.dn_scales, (size_t)(E * sc) * 4), op);
+    w.bytes = (size_t)(E * (gu + dn) + 3 * E * sc * 4);
+    CallScope cs(g_eng->stream);
+    hipStream_t st = cs.st;
+    HIP_TRY(hipMemsetAsync(w.gu_codes, 0, (size_t)(E * gu), st), op);  // the padding
+    HIP_TRY(hipMemsetAsync(w.dn_codes, 0, (size_t)(E * dn), st), op);
+    // An expert at a time: its three matrices up, then into their layouts (gate and up rows in turns of 32).
+    const size_t one = (size_t)(H * I);
+    uint8_t *dev;
+    RK_TRY(scratch(cs, "pack_blk", 3 * one, (void **)&dev));
+    for (int64_t e = 0; e < E; ++e) {
+      HIP_TRY(hipMemcpyAsync(dev, gate + e * one, one, hipMemcpyHostToDevice, st), op);
+      HIP_TRY(hipMemcpyAsync(dev + one, up + e * one, one, hipMemcpyHostToDevice, st), op);
+      HIP_TRY(hipMemcpyAsync(dev + 2 * one, down + e * one, one, hipMemcpyHostToDevice, st), op);
+      HIP_TRY(rk_launch_fp8_layout(dev, I, (int)H, 64, 0, (uint8_t *)w.gu_codes + e * gu, st), op);
+      HIP_TRY(rk_launch_fp8_layout(dev + one, I, (int)H, 64, 32, (uint8_t *)w.gu_codes + e * gu, st), op);
+      HIP_TRY(rk_launch_fp8_layout(dev + 2 * one, H, (int)I, 32, 0, (uint8_t *)w.dn_codes + e * dn, st), op);
+      HIP_TRY(hipMemcpyAsync(w.gu_scales + e * 2 * sc, gate_scales + e * sc, (size_t)sc * 4, hipMemcpyHostToDevice, st), op);
+      HIP_TRY(hipMemcpyAsync(w.gu_scales + e * 2 * sc + sc, up_scales + e * sc, (size_t)sc * 4, hipMemcpyHostToDevice, st), op);
+    }
+    HIP_TRY(hipMemcpyAsync(w.dn_scales, down_scales, (size_t)(E * sc) * 4, hipMemcpyHostToDevice, st), op);
+    HIP_TRY(hipStreamSynchronize(st), op);
+    *id = guard.register_weight();
+    return RK_OK;
+  });
 }
 
 extern "C" int rk_moe_experts_fp8_dev(rk_weight_id id, const void *plan, const void *x, void *y, int dtype, int accumulate,

@@ -60,7 +60,7 @@ __host__ __device__ inline int64_t fp8_offset(int64_t r, int64_t k, int kt) {
 // exactly. The fp8 products (2·64 K-values) are twice as fast, but align the terms of a sum to the largest and cut them
 // there: 1.4e-5 of a result's size on normally distributed codes (2^-16), where the bf16 products' sums are those of f32.
 // That is far below a bf16 or fp16 rounding; results that stay f32, or that are quantized again in front of fp16 results
-// (a code that flips is a sixteenth of its value), take the bf16 products.
+// (a code that flips is a sixteenth of its value), take the bf16 products, and so do those of one block of K.
 template <bool EXACT>
 struct Fp8Frag;
 template <>

@@ -24,12 +24,10 @@ __global__ __launch_bounds__(T::NT, 2) void gemm_fp8_kernel(const Fp8GemmArgs g,
 
   const auto value = [&](int i, int j, int r) { return t.acc[i][j][r]; };
   const auto out = [&](int es) { return (uint8_t *)g.c + (m0 * g.n + n0) * es; };
-  if constexpr (T::EXACT) {
-    t.template store<RK_DTYPE_F32>(smem, value, out(4), g.n, rows, g.n - n0);
-  } else {
-    if (g.c_dtype == RK_DTYPE_F16) t.template store<RK_DTYPE_F16>(smem, value, out(2), g.n, rows, g.n - n0);
-    else t.template store<RK_DTYPE_BF16>(smem, value, out(2), g.n, rows, g.n - n0);
-  }
+  if constexpr (T::EXACT)
+    if (g.c_dtype == RK_DTYPE_F32) return t.template store<RK_DTYPE_F32>(smem, value, out(4), g.n, rows, g.n - n0);
+  if (g.c_dtype == RK_DTYPE_F16) t.template store<RK_DTYPE_F16>(smem, value, out(2), g.n, rows, g.n - n0);
+  else t.template store<RK_DTYPE_BF16>(smem, value, out(2), g.n, rows, g.n - n0);
 }
 
 template <class T>
@@ -46,9 +44,9 @@ static hipError_t launch_fp8(const Fp8GemmArgs &g, hipStream_t st) {
   return hipGetLastError();
 }
 
-// exact: c f32; otherwise fp16 or bf16.
+// f32 results take the exact products.
 hipError_t rk_launch_gemm_fp8(const Fp8GemmArgs &g, bool exact, hipStream_t st) {
-  if (exact != (g.c_dtype == RK_DTYPE_F32)) return hipErrorInvalidValue;
+  if (!exact && g.c_dtype == RK_DTYPE_F32) return hipErrorInvalidValue;
   // At most two 64 × 128 tiles per CU: a round of them ends sooner than one of 128 × 128 would. us so and with these, MI355X,
   // 16-bit results: 3633 × 1024 × 2560 18.1 and 20.3, 512 × 4096 × 4096 16.4 and 26.7, 1024 × 4096 × 4096 (twice as many
   // tiles) 26 and 30, 512 × 16384 × 2048 29 and 22; f32: 2048 × 1024 × 4096 29 and 40, 2048 × 4096 × 2048 42 and 37.

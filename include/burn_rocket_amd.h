@@ -322,8 +322,8 @@ int rk_matmul_i8_partials_dev(rk_weight_id id, const int8_t *a, int64_t m,
  *
  *   c[m, n] = Σ_b as[m, b]·ws[n/128, b]·P_b[m, n],  P_b the product of block b's codes
  *
- * with the blocks summed in f32. P_b: with f32 results in f32; with fp16 and bf16 results by
- * the fp8 matrix instructions, whose sums keep about 2^-16 of a result. The order of
+ * with the blocks summed in f32. P_b: with f32 results, and at K up to 128, in f32; with
+ * fp16 and bf16 results by the fp8 matrix instructions, whose sums keep about 2^-16 of a result. The order of
  * the sums depends on M, N, K and the types: a row's result can differ in rounding
  * between calls of different M. Equal calls give equal bits. NaN codes, and rows of
  * activations that hold an infinity or a NaN, give NaN results in their rows alone. */

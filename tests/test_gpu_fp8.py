@@ -189,3 +189,86 @@ def test_refusals(rk):
     assert lib.rk_matmul_f16_dev(wid, b.ptr, 2, 256, b.ptr, None) == rk.RK_E_UNSUPPORTED
     assert lib.rk_matmul_w8a8_dev(wid, b.ptr, b.ptr, 256, 2, 256, b.ptr, None) == rk.RK_E_UNSUPPORTED
     assert lib.rk_matmul_i8_raw_dev(wid, b.ptr, 2, 256, b.ptr, None) == rk.RK_E_UNSUPPORTED
+
+
+@pytest.mark.parametrize("k", [16, 144, 272, 400, 528, 1104])
+@pytest.mark.parametrize("m,n,c_dtype", [(260, 2100, "bf16"), (500, 2100, "f32"), (1100, 4100, "bf16"), (1100, 4100, "f32"), (2900, 4100, "f16")])
+def test_products_of_tiles(rk, m, n, k, c_dtype):
+    """Grids that are too large for the kernel of few rows, at one to nine blocks of K: 64 x 128 tiles in 16 and in 32 bits,
+    128 x 128 in both, 256 x 256."""
+    note(f"fp8 tiles m={m} n={n} k={k} {c_dtype}")
+    r = np.random.default_rng(m + n + k)
+    codes, scales = ref.random_weight(r, n, k)
+    x = rows(r, m, k).astype(np.float32)
+    got = product(rk, x, "f32", rk.pack_fp8(codes, scales), n, c_dtype, True)
+    q, s = ref.quantize(x)
+    some = np.unique(np.concatenate([r.integers(0, m, 150), [0, 63, 64, 127, 128, 255, 256, m - 1]]))
+    check(got[some], c_dtype, (q[some], s[some]), (codes, scales), k, "rows")
+    x64, w64 = ref.values(q, s), ref.weight_values(codes, scales)[-140:]
+    want, size = x64 @ w64.T, np.abs(x64) @ np.abs(w64).T
+    most = ref.sum_error(k, c_dtype) * size
+    most = most + (np.abs(want) + most) * ref.HALF[c_dtype] + (2.0**-25 if c_dtype == "f16" else 0)
+    assert (np.abs(ref.widen(got[:, -140:], c_dtype) - want) <= most).all(), "columns"
+
+
+def test_captured_calls(rk):
+    """Quantizer and product in a graph; small calls by one entry, one of them larger than it takes in one launch outside a
+    capture. Replayed on new rows, with calls of other sizes in between."""
+    note("fp8 captured")
+    from test_gpu_sequences import Graph
+    lib, r = rk.lib(), np.random.default_rng(31)
+    n, k = 200, 1040
+    codes, scales = ref.random_weight(r, n, k)
+    wid, st = int(rk.pack_fp8(codes, scales)), rk.new_stream()
+    sizes = (3, 32, 40, 700)
+    x = {m: rk.DeviceBuffer(m * k * 2) for m in sizes}
+    c = {m: rk.DeviceBuffer(m * n * 2) for m in sizes}
+    q, s = rk.DeviceBuffer(700 * k), rk.DeviceBuffer(700 * ref.blocks(k) * 4)
+    for m in sizes:
+        x[m].zero()
+
+    def step():
+        for m in (3, 32):
+            assert lib.rk_matmul_fp8_dev(wid, x[m].ptr, TYPES["bf16"], m, k, c[m].ptr, TYPES["bf16"], st) == 0
+        assert lib.rk_matmul_fp8_dev(wid, x[40].ptr, TYPES["bf16"], 40, k, c[40].ptr, TYPES["bf16"], st) == rk.RK_E_UNSUPPORTED
+        for m in (40, 700):
+            assert lib.rk_quantize_fp8_dev(x[m].ptr, TYPES["bf16"], m, k, q.ptr, s.ptr, st) == 0
+            assert lib.rk_matmul_fp8_codes_dev(wid, q.ptr, s.ptr, m, k, c[m].ptr, TYPES["bf16"], st) == 0
+    g = Graph(st, step)
+    for _ in range(4):
+        host = {}
+        for m in sizes:
+            host[m], v = ref.cast(rows(r, m, k), "bf16")
+            x[m].upload(host[m])
+            host[m] = (host[m], v)
+        g.replay()
+        rk.synchronize(st)
+        for m in sizes:
+            got = c[m].download((m, n), np.uint16)
+            check(got, "bf16", ref.quantize(host[m][1]), (codes, scales), k, f"captured m={m}")
+            if m != 32:
+                assert (got == product(rk, host[m][0], "bf16", wid, n, "bf16", m > 3)).all()
+    g.destroy()
+    rk.destroy_stream(st)
+
+
+def test_two_streams_share_the_codes_memory(rk):
+    """Calls in turn on two streams, larger ones after smaller ones: each waits for the codes of the last."""
+    note("fp8 two streams")
+    lib, r = rk.lib(), np.random.default_rng(32)
+    n, k = 300, 528
+    codes, scales = ref.random_weight(r, n, k)
+    wid, sts = int(rk.pack_fp8(codes, scales)), [rk.new_stream(), rk.new_stream()]
+    work = []
+    for i, m in enumerate((40, 700, 64, 1500, 33, 2000, 900, 50)):
+        x, v = ref.cast(rows(r, m, k), "f16")
+        work.append((v, rk.DeviceBuffer.from_array(x), rk.DeviceBuffer(m * n * 4)))
+    rk.synchronize()
+    for i, (v, x, c) in enumerate(work):
+        assert lib.rk_matmul_fp8_dev(wid, x.ptr, TYPES["f16"], len(v), k, c.ptr, TYPES["f32"], sts[i % 2]) == 0
+    for st in sts:
+        rk.synchronize(st)
+    for v, _, c in work:
+        check(c.download((len(v), n), np.float32), "f32", ref.quantize(v), (codes, scales), k, f"m={len(v)}")
+    for st in sts:
+        rk.destroy_stream(st)
