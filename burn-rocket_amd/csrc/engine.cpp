@@ -2178,7 +2178,8 @@ int moe_run_fp8(CallScope &cs, const Weight &w, const MoePlan &plan, const void 
   const int64_t H = w.hidden, I = w.inter, R = plan.rows;
   hipStream_t st = cs.st;
   const int64_t KTh = w.gu_ws_stride, KTi = w.dn_ws_stride;
-  const bool few = plan.tile_rows < 128, exact1 = fp8_exact(dtype != RK_DTYPE_BF16, KTh), exact2 = fp8_exact(dtype == RK_DTYPE_F32, KTi);
+  const bool few = plan.tile_rows < 128;
+  const bool exact1 = fp8_exact(few || dtype != RK_DTYPE_BF16, KTh), exact2 = fp8_exact(dtype == RK_DTYPE_F32, KTi);
   void *act, *yb, *ys = nullptr;
   RK_TRY(moe_buf(cs, plan, "moe_act", few ? (size_t)R * I * 4 : (size_t)R * KTi * 128, &act));
   RK_TRY(moe_buf(cs, plan, "moe_yb", (size_t)R * H * 4, &yb));

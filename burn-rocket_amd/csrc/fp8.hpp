@@ -59,8 +59,11 @@ __host__ __device__ inline int64_t fp8_offset(int64_t r, int64_t k, int kt) {
 // One operand of a 32-row, 128-value block: as it lies (products of fp8 codes), or widened to bf16, which holds every code
 // exactly. The fp8 products (2·64 K-values) are twice as fast, but align the terms of a sum to the largest and cut them
 // there: 1.4e-5 of a result's size on normally distributed codes (2^-16), where the bf16 products' sums are those of f32.
-// That is far below a bf16 or fp16 rounding; results that stay f32, or that are quantized again in front of fp16 results
-// (a code that flips is a sixteenth of its value), take the bf16 products, and so do those of one block of K.
+// That is far below a bf16 or fp16 rounding; results that stay f32 take the bf16 products, those of one block of K, and those
+// that are quantized again (a code that flips is a sixteenth of its value) in front of fp16 results or in tiles of few rows:
+// one token's result of 8 experts is then off by 1.6e-3 of its size, as the bf16 rounding alone has it, instead of 3.8e-3,
+// for 19.2 us instead of 18.1. In tiles of many rows, where the products are what bounds the time, the flips of a bf16
+// layer's codes stay: 2.3e-3 instead of 1.7e-3.
 template <bool EXACT>
 struct Fp8Frag;
 template <>

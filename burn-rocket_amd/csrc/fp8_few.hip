@@ -243,7 +243,7 @@ __global__ __launch_bounds__(FNW * 64, 2) void fp8_few_kernel(const Fp8FewArgs g
 // column p of the products, all others of its operand zeros, so that one accumulator holds them all.
 //
 // One token of a 30B-A3B layer, MI355X: 7.1 us (7.8 with eight waves), where the product and the combine of the lists' form
-// take 4.7 each; the whole call 17.9 instead of 24.5. Bound by the trips to memory one behind the other: 12.6 MB.
+// take 4.7 each; the whole call 19.2 instead of 25.8. Bound by the trips to memory one behind the other: 12.6 MB.
 constexpr int TNW = 16;  // waves
 template <bool EXACT>
 __global__ __launch_bounds__(TNW * 64) void fp8_token_kernel(const Fp8FewArgs g) {
