@@ -129,12 +129,20 @@ __device__ __forceinline__ void fp8_encode4(void *to, const float *v) {
     dt_store_vec<DT, 4>(to, 0, v);
   }
 }
-// Four consecutive values of a row of c (element type known at run time), `n` of them inside the row.
-__device__ __forceinline__ void fp8_store4(void *c, int dt, int64_t at, const float *v, int n, bool whole) {
-  if (whole && n >= 4) {
-    if (dt == RK_DTYPE_F32) dt_store_vec<RK_DTYPE_F32, 4>(c, at, v);
-    else if (dt == RK_DTYPE_F16) dt_store_vec<RK_DTYPE_F16, 4>(c, at, v);
-    else fp8_encode4<RK_DTYPE_BF16>((uint16_t *)c + at, v);
+// Four consecutive values of a row of c (element type known at run time), `n` of them inside the row. In one store at any
+// address, which gfx950 has: the rows of an odd length begin anywhere.
+__device__ __forceinline__ void fp8_store4(void *c, int dt, int64_t at, const float *v, int n) {
+  if (n >= 4) {
+    typedef uint32_t words4 __attribute__((ext_vector_type(4), aligned(4)));
+    typedef uint32_t words2 __attribute__((ext_vector_type(2), aligned(2)));
+    uint16_t h[4] __attribute__((aligned(8)));
+    if (dt == RK_DTYPE_F32) {
+      *(words4 *)((float *)c + at) = words4{__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3])};
+      return;
+    }
+    if (dt == RK_DTYPE_F16) fp8_encode4<RK_DTYPE_F16>(h, v);
+    else fp8_encode4<RK_DTYPE_BF16>(h, v);
+    *(words2 *)((uint16_t *)c + at) = __builtin_bit_cast(uintx2, h);
     return;
   }
 #pragma unroll

@@ -206,7 +206,6 @@ __global__ __launch_bounds__(FNW * 64, 2) void fp8_few_kernel(const Fp8FewArgs g
           red[((((wave * NB + b) * TM + j) * 4 + q) * 2 + h) * cols + col] =
               floatx4{acc[b][j][4 * q], acc[b][j][4 * q + 1], acc[b][j][4 * q + 2], acc[b][j][4 * q + 3]};
   __syncthreads();
-  const bool whole = (g.n & 3) == 0;
   const int each = TM * 8 * cols;  // items of four values of a group
   for (int o = threadIdx.x; o < groups * each; o += FNW * 64) {
     const int gr = o / each, i = o - gr * each;
@@ -233,7 +232,7 @@ __global__ __launch_bounds__(FNW * 64, 2) void fp8_few_kernel(const Fp8FewArgs g
 #pragma unroll
       for (int e = 0; e < 4; ++e) v[0][e] *= rw;
     }
-    fp8_store4(g.c, g.c_dtype, (row0 + r) * g.n + n, v[0], g.n - n, whole);
+    fp8_store4(g.c, g.c_dtype, (row0 + r) * g.n + n, v[0], g.n - n);
   }
 }
 

@@ -226,12 +226,15 @@ struct Fp8Tile {
     __syncthreads();
     const int c = tid % CH, left = n - c * V;
     if (left <= 0) return;
-    const bool whole = ld * ES % 16 == 0 && left >= V;
+    // (gfx950 stores 16 bytes at any address; a row of an odd length begins between two of its pieces. 3536 rows of 6780 at
+    // K = 384 value by value: 42 us instead of 22)
+    typedef uint32_t piece __attribute__((ext_vector_type(4), aligned(2)));
+    const bool whole = left >= V;
     for (int r = tid / CH; r < rows; r += NT / CH) {
       const uint8_t *p = smem + r * ROWB + ((c ^ (r & SW)) * 16);
       uint8_t *o = (uint8_t *)to + (r * ld + c * V) * ES;
       if (whole) {
-        *(uintx4 *)o = *(const uintx4 *)p;
+        *(piece *)o = *(const uintx4 *)p;
       } else {
 #pragma unroll
         for (int e = 0; e < V; ++e)
