@@ -2017,14 +2017,22 @@ struct MoeLists {
   size_t roww = 0, tiles = 0, tiles_gu = 0, slot = 0, bytes = 0;
 };
 
-// Rows of a tile of fp8 experts, by the rows that an expert has on average: the kernels of few rows, then tiles of 128 and
-// of 256 rows.
-int64_t moe_fp8_few_limit(const Weight &w) { return 16 * (int64_t)w.n_experts; }
+// Rows of a tile of fp8 experts. Up to 12 rows an expert on average the kernels of few rows, which stream weights and
+// quantize their rows themselves: a layer of 128 experts (2048 x 768, bf16) on 8 rows an expert 138 us with them and 139 on
+// tiles of 128 rows, 16 rows 153 and 144; 64 of 2048 x 1408 (fp16) 129 and 136, 148 and 138; 8 of 4096 x 1536 (bf16) 49 and 57,
+// 59 and 58. Then tiles of 256 rows where their rounds of the GPU (first product; half of an expert's last tile is empty)
+// take less than those of 128, one of which takes three quarters of the time: the 128 experts on 64 rows each 170 us on 128
+// and 189 on 256, on 128 rows 245 and 216, on 187 rows 325 and 249; the 8 on 192 rows 82 and 107, on 384 rows 147 and 122.
+int64_t moe_fp8_few_limit(const Weight &w) { return 12 * (int64_t)w.n_experts; }
 int moe_fp8_tile_rows(const Weight &w, int64_t rows) {
   const int knob = rk_knob("RK_MOE_FP8_ROWS", 0);
   if (knob == 128 || knob == 256) return knob;
   if (rows <= moe_fp8_few_limit(w)) return std::min(rk_fp8_few_rows(w.gu_ws_stride), rk_fp8_few_rows(w.dn_ws_stride));
-  return rows >= 192 * (int64_t)w.n_experts ? 256 : 128;
+  const auto rounds = [&](int tile) {
+    const int64_t tiles = std::max<int64_t>(w.n_experts, rows / tile + w.n_experts / 2);
+    return (tiles * w.dn_ws_stride + g_eng->num_cus - 1) / g_eng->num_cus;
+  };
+  return 4 * rounds(256) < 3 * rounds(128) ? 256 : 128;
 }
 // Rows as tiles of their own, the second product with the sum over experts: while hardly two tokens share an expert, whose
 // weights are read for each. Router and experts of a layer of 128 experts (top 8), us in lists and so, MI355X: 1 token 28 and
