@@ -666,9 +666,11 @@ int rk_moe_plan_route_dev(void *plan, int64_t s, const uint32_t *ids, const floa
 int rk_pack_moe_fp8(const uint8_t *gate, const float *gate_scales, const uint8_t *up, const float *up_scales,
                     const uint8_t *down, const float *down_scales, int n_experts, int64_t hidden, int64_t inter,
                     rk_weight_id *id);
-/* The planned call on an fp8 stack with x and y of type dtype; accumulate: onto y. bf16: both
- * products by the fp8 matrix instructions; fp16: the first one, whose results are quantized
- * again, with f32 sums; f32: both with f32 sums. x and y are 16-byte aligned and may be the same buffer. */
+/* The planned call on an fp8 stack with x and y of type dtype; accumulate: onto y. Products with
+ * f32 sums: both where the rows are f32; the first one, whose results are quantized again, also
+ * for fp16 rows, and for bf16 rows while there are few an expert; all others by the fp8 matrix
+ * instructions. x and y are 16-byte aligned and may be the same buffer. A token's result depends
+ * in its rounding on the batch that it is in; equal batches give equal bits. */
 int rk_moe_experts_fp8_dev(rk_weight_id id, const void *plan, const void *x, void *y, int dtype, int accumulate,
                            rk_stream stream);
 
