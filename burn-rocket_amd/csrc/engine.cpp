@@ -1912,11 +1912,13 @@ int moe_alloc(Weight &w, int n_experts, int64_t H, int64_t I, const char *op) {
   HIP_TRY(hipMalloc((void **)&w.dn_codes, dn_codes), op);
   HIP_TRY(hipMalloc((void **)&w.gu_scales, gu_sc * 4), op);
   HIP_TRY(hipMalloc((void **)&w.dn_scales, dn_sc * 4), op);
-  // Padding blocks of the fragment-major layout stay zero.
-  HIP_TRY(hipMemset(w.gu_codes, 0, gu_codes), op);
-  HIP_TRY(hipMemset(w.dn_codes, 0, dn_codes), op);
-  HIP_TRY(hipMemset(w.gu_scales, 0, gu_sc * 4), op);
-  HIP_TRY(hipMemset(w.dn_scales, 0, dn_sc * 4), op);
+  // Padding blocks of the fragment-major layout stay zero. On the stream that fills the rest: the library's streams do not
+  // wait for the null stream, on which a hipMemset may still run behind the first expert's codes.
+  hipStream_t st = g_eng->stream;
+  HIP_TRY(hipMemsetAsync(w.gu_codes, 0, gu_codes, st), op);
+  HIP_TRY(hipMemsetAsync(w.dn_codes, 0, dn_codes, st), op);
+  HIP_TRY(hipMemsetAsync(w.gu_scales, 0, gu_sc * 4, st), op);
+  HIP_TRY(hipMemsetAsync(w.dn_scales, 0, dn_sc * 4, st), op);
   w.bytes = gu_codes + dn_codes + (gu_sc + dn_sc) * 4;
   return RK_OK;
 }

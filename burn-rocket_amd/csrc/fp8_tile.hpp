@@ -117,7 +117,7 @@ struct Fp8Tile {
     auto load_w = [&](Fp8Frag<EXACT> &f, int slot, int i) {
       const uint8_t *p = smem + slot * SLOT + w_off + i * 4096;
       f.set(0, *(const intx4 *)p, *(const intx4 *)(p + 1024));
-      f.set(1, *(const intx4 *)(p + 2048), *(const intx4 *)(p + 3072));
+      f.set(1, *(const intx4 *)(p + 2048), *(const intx4 *)(p + 3 * 1024));
     };
     auto load_x = [&](int slot, int j) {
       const uint8_t *p = smem + slot * SLOT + j * 32 * 128;
