@@ -3728,6 +3728,7 @@ extern "C" int rk_memset_dev(void *dst, int value, size_t bytes) {
   std::lock_guard<std::mutex> lk(g_mu);
   RK_TRY(ensure("rk_memset_dev"));
   HIP_TRY(hipMemset(dst, value, bytes), "rk_memset_dev");
+  HIP_TRY(hipStreamSynchronize(nullptr), "rk_memset_dev");  // (calls on the library's streams do not wait for the null stream)
   return RK_OK;
 }
 extern "C" int rk_stream_get(rk_stream *stream) {
