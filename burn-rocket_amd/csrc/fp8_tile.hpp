@@ -1,4 +1,4 @@
-// The K loop that the dense and the expert products of many rows share (gemm_fp8.hip, moe_fp8.hip).
+// The K loops of the dense and the expert products of many rows (gemm_fp8.hip, moe_fp8.hip).
 #pragma once
 
 #include "fp8.hpp"
@@ -200,46 +200,174 @@ struct Fp8Tile {
     }
     __syncthreads();  // the slots may be used for something else
   }
+};
 
-  // The tile's results to rows of a matrix through LDS, so that a wave stores whole pieces of a row (its lanes hold four
-  // outputs of 32 rows each: 16-byte pieces of 32 lines, which cost a third of the vision layer's 4304 × 1152 product).
-  // value(i, j, r): the lane's result; to: the tile's first row, ld values apart; n: outputs from the tile's first on.
-  // Chunk c of 16 bytes of row r lies at c ^ (r mod 32) (16 of a narrow row): the rows that a store writes are on different banks.
-  template <int DT, typename Value>
-  __device__ __forceinline__ void store(uint8_t *smem, Value value, void *to, int64_t ld, int rows, int n) {
-    constexpr int ES = DT == RK_DTYPE_F32 ? 4 : 2, V = 16 / ES;  // values of a chunk
-    constexpr int ROWB = BN * ES, CH = ROWB / 16;                 // a row's bytes and chunks
-    constexpr int SW = CH < 32 ? CH - 1 : 31;
-    static_assert(BM * ROWB <= SMEM && (CH & (CH - 1)) == 0 && NT % CH == 0, "the tile in LDS");
-    const int tid = fresh_tid(), col = tid & 31, h = (tid >> 5) & 1;
-    const int wave = tid >> 6, wm = wave / WN, wn = wave % WN;
+// The tile's results to rows of a matrix through LDS, so that a wave stores whole pieces of a row (its lanes hold four
+// outputs of 32 rows each: 16-byte pieces of 32 lines, which cost a third of the vision layer's 4304 × 1152 product).
+// value(i, j, r): the lane's result; to: the tile's first row, ld values apart; n: outputs from the tile's first on.
+// Chunk c of 16 bytes of row r lies at c ^ (r mod 32) (16 of a narrow row): the rows that a store writes are on different banks.
+template <class T, int DT, typename Value>
+__device__ __forceinline__ void fp8_store_tile(uint8_t *smem, Value value, void *to, int64_t ld, int rows, int n) {
+  constexpr int BM = T::BM, BN = T::BN, WN = T::WN, WTM = T::WTM, WTN = T::WTN, TM = T::TM, TN = T::TN, NT = T::NT;
+  constexpr int ES = DT == RK_DTYPE_F32 ? 4 : 2, V = 16 / ES;  // values of a chunk
+  constexpr int ROWB = BN * ES, CH = ROWB / 16;                 // a row's bytes and chunks
+  constexpr int SW = CH < 32 ? CH - 1 : 31;
+  static_assert(BM * ROWB <= T::SMEM && (CH & (CH - 1)) == 0 && NT % CH == 0, "the tile in LDS");
+  const int tid = fresh_tid(), col = tid & 31, h = (tid >> 5) & 1;
+  const int wave = tid >> 6, wm = wave / WN, wn = wave % WN;
 #pragma unroll
-    for (int j = 0; j < TM; ++j)
+  for (int j = 0; j < TM; ++j)
+#pragma unroll
+    for (int i = 0; i < TN; ++i)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const float v[4] = {value(i, j, 4 * q), value(i, j, 4 * q + 1), value(i, j, 4 * q + 2), value(i, j, 4 * q + 3)};
+        const int r = wm * WTM + j * 32 + col, at = wn * WTN + i * 32 + q * 8 + h * 4;
+        fp8_encode4<DT>(smem + r * ROWB + (((at / V) ^ (r & SW)) * 16) + at % V * ES, v);
+      }
+  __syncthreads();
+  const int c = tid % CH, left = n - c * V;
+  if (left <= 0) return;
+  // (gfx950 stores 16 bytes at any address; a row of an odd length begins between two of its pieces. 3536 rows of 6780 at
+  // K = 384 value by value: 42 us instead of 22)
+  typedef uint32_t piece __attribute__((ext_vector_type(4), aligned(2)));
+  const bool whole = left >= V;
+  for (int r = tid / CH; r < rows; r += NT / CH) {
+    const uint8_t *p = smem + r * ROWB + ((c ^ (r & SW)) * 16);
+    uint8_t *o = (uint8_t *)to + (r * ld + c * V) * ES;
+    if (whole) {
+      *(piece *)o = *(const uintx4 *)p;
+    } else {
+#pragma unroll
+      for (int e = 0; e < V; ++e)
+        if (e < left) ((dt_storage<DT> *)o)[e] = ((const dt_storage<DT> *)p)[e];
+    }
+  }
+}
+
+// Smaller tiles, with the weights' fragments straight from memory to registers, as they lie: four waves of all BM rows and 32
+// outputs each, so that no two ask for the same weights, and LDS, which bounds such tiles otherwise, holds the rows alone.
+// STAGES - 1 stages of both are on the way. Two a CU of 64 × 128 move 15 TB/s out of the L2s.
+template <int TM_, int STAGES_, bool EXACT_>
+struct Fp8Flow {
+  static constexpr int TM = TM_, TN = 1, STAGES = STAGES_, WM = 1, WN = 4, NW = 4, NT = 256;
+  static constexpr bool EXACT = EXACT_;
+  static constexpr int BM = 32 * TM, BN = 128 * TN, WTM = BM, WTN = 32 * TN;
+  static constexpr int QA = BM / 8, CA = QA / NW, SI = BM / 64;
+  static constexpr int WS_AT = BM * 128 + BM * 4;
+  static constexpr int SLOT = WS_AT + 256;
+  static constexpr int OUT = BM * BN * (EXACT ? 4 : 2);
+  static constexpr int SMEM = STAGES * SLOT > OUT ? STAGES * SLOT : OUT;
+  static constexpr int OPS = CA + 1 + 4 * TN;  // memory operations of a wave and stage
+  static_assert(SI >= 1 && SI < NW && (STAGES - 2) * OPS < 64, "copies per wave");
+
+  floatx16 acc[TN][TM];
+
+  template <typename RowOf, typename Scales>
+  __device__ __forceinline__ void run(uint8_t *smem, const uint8_t *a, int64_t a_bytes, const float *as, int64_t as_bytes,
+                                      RowOf row_of, int rows, const uint8_t *w, int blocks, const float *ws, int64_t ws_bytes,
+                                      Scales ws_of, int k, int KT) {
+    const int lane = lane_id(), col = lane & 31, h = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const rsrc_t ra = make_rsrc(a, a_bytes), rw = make_rsrc(w, (int64_t)min(blocks, BN / 32) * KT * 4096);
+    const uint32_t ch = (uint32_t)(((lane & 7) ^ (((wave * 8 + (lane >> 3)) >> 1) & 7)) << 4);
+    uint32_t off[CA];
+#pragma unroll
+    for (int i = 0; i < CA; ++i) {
+      const int64_t src = row_of((wave + i * NW) * 8 + (lane >> 3));
+      off[i] = src < 0 ? OOB_OFFSET : (uint32_t)(src * k) + ch;
+    }
+    const bool row_scales = wave < SI;
+    const rsrc_t rsc = row_scales ? make_rsrc(as, as_bytes) : make_rsrc(ws, ws_bytes);
+    const int sc_at = row_scales ? BM * 128 + wave * 256 : WS_AT;
+    uint32_t soff = OOB_OFFSET;
+    if (row_scales) {
+      const int64_t src = row_of(wave * 64 + lane);
+      if (src >= 0) soff = (uint32_t)(src * KT * 4);
+    } else if (lane < BN / 32) {
+      soff = (uint32_t)(ws_of(lane) * 4);
+    }
+    intx4 wr[STAGES][TN][4];
+    // A stage's copies and loads. Between two barriers, all of them: the waits count them.
+    auto issue = [&](auto slot_c, int kt) {
+      constexpr int slot = decltype(slot_c)::value;
+      uint8_t *sb = smem + slot * SLOT;
+      const uint32_t k0 = (uint32_t)kt * 128;
+#pragma unroll
+      for (int c = 0; c < CA; ++c) bdma16(ra, sb + (wave + c * NW) * 1024, k0 + ch < (uint32_t)k ? off[c] : OOB_OFFSET, k0);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rsc, LDS_PTR(sb + sc_at), 4, soff, kt * 4, 0, 0);
 #pragma unroll
       for (int i = 0; i < TN; ++i)
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const float v[4] = {value(i, j, 4 * q), value(i, j, 4 * q + 1), value(i, j, 4 * q + 2), value(i, j, 4 * q + 3)};
-          const int r = wm * WTM + j * 32 + col, at = wn * WTN + i * 32 + q * 8 + h * 4;
-          fp8_encode4<DT>(smem + r * ROWB + (((at / V) ^ (r & SW)) * 16) + at % V * ES, v);
-        }
-    __syncthreads();
-    const int c = tid % CH, left = n - c * V;
-    if (left <= 0) return;
-    // (gfx950 stores 16 bytes at any address; a row of an odd length begins between two of its pieces. 3536 rows of 6780 at
-    // K = 384 value by value: 42 us instead of 22)
-    typedef uint32_t piece __attribute__((ext_vector_type(4), aligned(2)));
-    const bool whole = left >= V;
-    for (int r = tid / CH; r < rows; r += NT / CH) {
-      const uint8_t *p = smem + r * ROWB + ((c ^ (r & SW)) * 16);
-      uint8_t *o = (uint8_t *)to + (r * ld + c * V) * ES;
-      if (whole) {
-        *(piece *)o = *(const uintx4 *)p;
-      } else {
+        for (int q = 0; q < 4; ++q)
+          wr[slot][i][q] = __builtin_bit_cast(
+              intx4, __builtin_amdgcn_raw_buffer_load_b128(rw, lane * 16, (min(wave * TN + i, blocks - 1) * KT + kt) * 4096 + q * 1024, 0));
+    };
+    const int swz = (col >> 1) & 7;
+    const uint32_t a_off = (uint32_t)(col * 128 + (((2 * h) ^ swz) << 4));
 #pragma unroll
-        for (int e = 0; e < V; ++e)
-          if (e < left) ((dt_storage<DT> *)o)[e] = ((const dt_storage<DT> *)p)[e];
+    for (int i = 0; i < TN; ++i)
+#pragma unroll
+      for (int j = 0; j < TM; ++j) acc[i][j] = floatx16{};
+    auto stage = [&](auto slot_c) {
+      constexpr int slot = decltype(slot_c)::value;
+      const uint8_t *sb = smem + slot * SLOT;
+      Fp8Frag<EXACT> wf[TN], x[2];
+      float sa[TM], sw[TN];
+      auto load_x = [&](int j) {
+        const uint8_t *p = sb + j * 32 * 128;
+        x[j & 1].set(0, *(const intx4 *)(p + a_off), *(const intx4 *)(p + (a_off ^ 16)));
+        x[j & 1].set(1, *(const intx4 *)(p + (a_off ^ 64)), *(const intx4 *)(p + (a_off ^ 80)));
+      };
+      load_x(0);
+#pragma unroll
+      for (int j = 0; j < TM; ++j) sa[j] = *(const float *)(sb + BM * 128 + (j * 32 + col) * 4);
+#pragma unroll
+      for (int i = 0; i < TN; ++i) {
+        sw[i] = *(const float *)(sb + WS_AT + (wave * TN + i) * 4);
+        wf[i].set(0, wr[slot][i][0], wr[slot][i][1]);
+        wf[i].set(1, wr[slot][i][2], wr[slot][i][3]);
       }
-    }
+      static_for<TM>([&](auto j_c) {
+        constexpr int j = decltype(j_c)::value;
+        if constexpr (j + 1 < TM) load_x(j + 1);
+#pragma unroll
+        for (int i = 0; i < TN; ++i) {
+          const floatx16 p = fp8_product(wf[i], x[j & 1]);
+          const float sc = sa[j] * sw[i];
+#pragma unroll
+          for (int r = 0; r < 16; ++r) acc[i][j][r] = __builtin_fmaf(p[r], sc, acc[i][j][r]);
+        }
+      });
+    };
+    auto arrived = [&](auto behind_c) {
+      __builtin_amdgcn_sched_barrier(0);
+      WAIT_VMCNT(decltype(behind_c)::value * OPS);
+      WAIT_LGKMCNT0();
+      BARRIER();
+      __builtin_amdgcn_sched_barrier(0);
+    };
+    static_for<STAGES - 1>([&](auto d_c) {
+      if (decltype(d_c)::value < KT) issue(d_c, decltype(d_c)::value);
+    });
+    int kt = 0;
+    for (; kt + 2 * STAGES - 1 <= KT; kt += STAGES)
+      static_for<STAGES>([&](auto d_c) {
+        constexpr int d = decltype(d_c)::value;
+        arrived(ic<STAGES - 2>{});
+        issue(ic<(d + STAGES - 1) % STAGES>{}, kt + d + STAGES - 1);
+        stage(d_c);
+      });
+    for (; kt < KT; kt += STAGES)
+      static_for<STAGES>([&](auto d_c) {
+        constexpr int d = decltype(d_c)::value;
+        if (kt + d < KT) {
+          if (kt + d + STAGES - 2 < KT) arrived(ic<STAGES - 2>{});
+          else arrived(ic<0>{});
+          if (kt + d + STAGES - 1 < KT) issue(ic<(d + STAGES - 1) % STAGES>{}, kt + d + STAGES - 1);
+          stage(d_c);
+        }
+      });
+    __syncthreads();
   }
 };

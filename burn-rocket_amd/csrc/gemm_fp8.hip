@@ -25,9 +25,9 @@ __global__ __launch_bounds__(T::NT, 2) void gemm_fp8_kernel(const Fp8GemmArgs g,
   const auto value = [&](int i, int j, int r) { return t.acc[i][j][r]; };
   const auto out = [&](int es) { return (uint8_t *)g.c + (m0 * g.n + n0) * es; };
   if constexpr (T::EXACT)
-    if (g.c_dtype == RK_DTYPE_F32) return t.template store<RK_DTYPE_F32>(smem, value, out(4), g.n, rows, g.n - n0);
-  if (g.c_dtype == RK_DTYPE_F16) t.template store<RK_DTYPE_F16>(smem, value, out(2), g.n, rows, g.n - n0);
-  else t.template store<RK_DTYPE_BF16>(smem, value, out(2), g.n, rows, g.n - n0);
+    if (g.c_dtype == RK_DTYPE_F32) return fp8_store_tile<T, RK_DTYPE_F32>(smem, value, out(4), g.n, rows, g.n - n0);
+  if (g.c_dtype == RK_DTYPE_F16) fp8_store_tile<T, RK_DTYPE_F16>(smem, value, out(2), g.n, rows, g.n - n0);
+  else fp8_store_tile<T, RK_DTYPE_BF16>(smem, value, out(2), g.n, rows, g.n - n0);
 }
 
 template <class T>
@@ -47,17 +47,19 @@ static hipError_t launch_fp8(const Fp8GemmArgs &g, hipStream_t st) {
 // f32 results take the exact products.
 hipError_t rk_launch_gemm_fp8(const Fp8GemmArgs &g, bool exact, hipStream_t st) {
   if (!exact && g.c_dtype == RK_DTYPE_F32) return hipErrorInvalidValue;
-  // At most two 64 × 128 tiles per CU: a round of them ends sooner than one of 128 × 128 would. us so and with these, MI355X,
-  // 16-bit results: 3633 × 1024 × 2560 18.1 and 20.3, 512 × 4096 × 4096 16.4 and 26.7, 1024 × 4096 × 4096 (twice as many
-  // tiles) 26 and 30, 512 × 16384 × 2048 29 and 22; f32: 2048 × 1024 × 4096 29 and 40, 2048 × 4096 × 2048 42 and 37.
-  const bool small = (int64_t)((g.m + 63) / 64) * ((g.n + 127) / 128) <= 2 * g.num_cus;
-  if (exact) return small ? launch_fp8<Fp8Tile<64, 128, 2, 2, 3, true>>(g, st) : launch_fp8<Fp8Tile<128, 128, 2, 2, 2, true>>(g, st);
-  if (small) return launch_fp8<Fp8Tile<64, 128, 2, 2, 3, false>>(g, st);
+  const auto tiles = [&](int bm, int bn) { return (int64_t)((g.m + bm - 1) / bm) * ((g.n + bn - 1) / bn); };
+  const auto rounds = [&](int64_t n, int64_t at_once) { return (n + at_once - 1) / at_once; };
+  // At most one and a half 64 × 128 tiles per CU: a round of them ends sooner than one of 128 × 128 would. us so and with these,
+  // MI355X, 16-bit results: 2048 × 1024 × 4096 16.6 and 22, 512 × 4096 × 4096 16.0 and 21.8, 1024 × 4096 × 4096 (two per CU)
+  // 27.7 and 25.2, 3633 × 1024 × 2560 (1.8) 17.9 and 17.0; f32: 2048 × 1024 × 4096 24 and 35, 4096 × 1024 × 4096 39 and 40.
+  // (Fp8Tile with these sizes, weights through LDS: the six 18, 18, 27.4, 18.4; 30, 43; 4096 × 4096 × 4096 in f32 131 where
+  // this is 111.)
+  const bool small = 2 * tiles(64, 128) <= 3 * g.num_cus;
+  if (exact) return small ? launch_fp8<Fp8Flow<2, 3, true>>(g, st) : launch_fp8<Fp8Flow<4, 3, true>>(g, st);
+  if (small) return launch_fp8<Fp8Flow<2, 3, false>>(g, st);
   // 256 × 256 where its rounds, one tile a CU, are less than two thirds of those of 128 × 128, two a CU: a round of them
   // takes 47 to 60 us at K = 4096, one of these 34 to 38 (2560 × 4096: 54 and 63; 2048 × 4096: 51 and 38; 4608 × 4096: 100
   // and 96).
-  const int64_t big = (int64_t)((g.m + 255) / 256) * ((g.n + 255) / 256), mid = (int64_t)((g.m + 127) / 128) * ((g.n + 127) / 128);
-  const auto rounds = [&](int64_t tiles, int64_t at_once) { return (tiles + at_once - 1) / at_once; };
-  if (3 * rounds(big, g.num_cus) < 2 * rounds(mid, 2 * g.num_cus)) return launch_fp8<Fp8Tile<256, 256, 4, 2, 2, false>>(g, st);
-  return launch_fp8<Fp8Tile<128, 128, 2, 2, 2, false>>(g, st);
+  if (3 * rounds(tiles(256, 256), g.num_cus) < 2 * rounds(tiles(128, 128), 2 * g.num_cus)) return launch_fp8<Fp8Tile<256, 256, 4, 2, 2, false>>(g, st);
+  return launch_fp8<Fp8Flow<4, 3, false>>(g, st);
 }

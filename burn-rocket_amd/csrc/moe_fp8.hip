@@ -129,7 +129,7 @@ __global__ __launch_bounds__(T::NT, 2) void moe_fp8_down_kernel(const Fp8MoeArgs
   }
   const auto value = [&](int i, int j, int r) { return t.acc[i][j][r] * rw[j]; };
   if constexpr (!T::EXACT) {
-    t.template store<RK_DTYPE_F16>(smem, value, (uint16_t *)g.out + (int64_t)tile.row0 * g.n + n0, g.n, tile.rows, g.n - n0);
+    fp8_store_tile<T, RK_DTYPE_F16>(smem, value, (uint16_t *)g.out + (int64_t)tile.row0 * g.n + n0, g.n, tile.rows, g.n - n0);
   } else {
 #pragma unroll
     for (int j = 0; j < T::TM; ++j) {
