@@ -342,9 +342,9 @@ bool rk_fp8_few_fits_x(int64_t m, int kt) { return m <= 32 && few_in((int)m, kt)
 // 1024 5.7 and 6.2, 24 × 1024 × 1024 6.7 and 6.2, 4 × 4096 × 4096 8.1 and 8.8, 8 × 4096 × 4096 10.5 and 8.9.
 bool rk_fp8_few_wants_x(int64_t m, int kt) { return m * kt <= 160; }
 // Codes: while the grid is what is short, 32 outputs × 64 rows a workgroup, one per CU (two where the products are the
-// slow exact ones). us here and on 64 × 128 tiles, MI355X, 16-bit results: 128 × 4096 × 4096 10.1 and 15.4, 192 × 4096 ×
-// 4096 14.8 and 15.4, 256 × 4096 × 1024 7.3 and 6.5, 512 × 4096 × 4096 28 and 16; f32: 512 × 2048 × 2048 11.6 and 15.3,
-// 512 × 4096 × 2048 18 and 16.
+// slow exact ones). us here and on 64 × 128 tiles, MI355X, 16-bit results: 128 × 4096 × 4096 10.1 and 14.1, 256 × 2048 ×
+// 2048 7.0 and 9.0, 192 × 4096 × 4096 15.5 and 14.5, 256 × 4096 × 1024 7.2 and 6.0; f32: 512 × 2048 × 2048 12.0 and 13.6,
+// 768 × 2048 × 2048 18 and 14. Up to 32 rows a wave has one column block, and the weight streams: 32 × 16384 × 2048 9.7 and 10.2.
 bool rk_fp8_few_fits_codes(int64_t m, int64_t n, bool exact, int num_cus) {
   return m <= 32 || (n + 31) / 32 * ((m + 63) / 64) <= (exact ? 2 : 1) * (int64_t)num_cus;
 }
