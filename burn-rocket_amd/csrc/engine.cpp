@@ -2187,6 +2187,13 @@ int moe_run_fp8(CallScope &cs, const Weight &w, const MoePlan &plan, const void 
   const char *op = "rk_moe_experts_fp8_dev";
   const int64_t H = w.hidden, I = w.inter, R = plan.rows;
   hipStream_t st = cs.st;
+  if (!plan.routed) {
+    bool capturing;
+    RK_TRY(is_capturing(st, &capturing, op));
+    if (capturing)
+      return fail(RK_E_UNSUPPORTED, op, "a plan of host lists works in library memory, which a graph must not hold: capture calls on a "
+                                        "plan of rk_moe_routed_plan_create");
+  }
   const int64_t KTh = w.gu_ws_stride, KTi = w.dn_ws_stride;
   const bool few = plan.tile_rows < 128;
   const bool exact1 = fp8_exact(few || dtype != RK_DTYPE_BF16, KTh), exact2 = fp8_exact(dtype == RK_DTYPE_F32, KTi);

@@ -561,3 +561,32 @@ def test_few_tokens_captured(rk):
     g.destroy()
     plan.destroy()
     rk.destroy_stream(st)
+
+
+def test_host_lists_of_fp8_experts_are_refused_in_a_capture(rk):
+    note("fp8 host lists, captured")
+    from test_gpu_sequences import Graph
+    lib, r = rk.lib(), np.random.default_rng(24)
+    e, k, h, i, s = 4, 2, 64, 64, 8
+    wid = int(rk.pack_moe_fp8(*ref.random_stack(r, e, i, h), *ref.random_stack(r, e, i, h), *ref.random_stack(r, e, h, i)))
+    ids, wts = choices(r, s, e, k, "any")
+    plan, st = ctypes.c_void_p(), rk.new_stream()
+    ok(rk, lib.rk_moe_plan_create(wid, s, k, ids.ctypes.data, wts.ctypes.data, ctypes.byref(plan)))
+    x = rk.DeviceBuffer.from_array(r.standard_normal((s, h)).astype(np.float32))
+    y = rk.DeviceBuffer(s * h * 4)
+    y.zero()
+    for call in (lambda: lib.rk_moe_experts_fp8_dev(wid, plan, x.ptr, y.ptr, 0, 0, st),
+                 lambda: lib.rk_moe_experts_planned_dev(wid, plan, x.ptr, y.ptr, st)):
+        rcs = []
+
+        def step():
+            ok(rk, lib.rk_quantize_fp8_dev(x.ptr, 0, s, h, y.ptr, y.ptr + s * h, st))  # (a graph has to hold something)
+            rcs.append(call())
+        g = Graph(st, step)
+        assert rcs == [rk.RK_E_UNSUPPORTED]
+        g.destroy()
+        ok(rk, call())  # and outside of one
+        rk.synchronize(st)
+    assert (y.download((s, h), np.float32) == run_host(rk, wid, x.download((s, h), np.float32), ids, wts)).all()
+    ok(rk, lib.rk_moe_plan_destroy(plan))
+    rk.destroy_stream(st)
