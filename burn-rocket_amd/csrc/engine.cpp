@@ -2220,6 +2220,7 @@ int moe_run_fp8(CallScope &cs, const Weight &w, const MoePlan &plan, const void 
     g.tiles = plan.tiles_gu;
     g.n_tok = (int)plan.s;
     g.tok = plan.tok;
+    g.top_k = plan.pairs ? plan.top_k : 0;
     HIP_TRY(rk_launch_fp8_few_gate_up(g, dtype, plan.tile_rows, plan.n_tiles, exact1, st), op);
     g.x = act;
     g.n = (int)H;

@@ -32,33 +32,38 @@ __host__ __device__ constexpr size_t few_smem(int xt, int nout, int tm, int rows
 
 // Rows of x to codes in LDS, [row][few_row], by the whole workgroup: 16 lanes a block. Their scales [row][kt] are behind them.
 __device__ __forceinline__ float *few_scales(uint8_t *smem, int rows, int kt) { return (float *)(smem + (size_t)rows * few_row(kt)); }
+// Block b of the rows: the lane's eight values.
+template <int XT, typename RowOf>
+__device__ __forceinline__ void few_load(dt_raw<XT, 8> &raw, const void *x, int b, int rows, int k, int kt, RowOf row_of) {
+  const int r = b / kt, c = (b - r * kt) * 128 + (threadIdx.x & 15) * 8;
+#pragma unroll
+  for (int e = 0; e < raw.WORDS; ++e) raw.w[e] = 0;
+  if (r >= rows || c >= k) return;
+  const int64_t at = row_of(r) * k + c;
+  if constexpr (XT == RK_DTYPE_F32) {
+    *(uintx4 *)raw.w = *(const uintx4 *)((const float *)x + at);
+    *(uintx4 *)(raw.w + 4) = *(const uintx4 *)((const float *)x + at + 4);
+  } else {
+    *(uintx4 *)raw.w = *(const uintx4 *)((const uint16_t *)x + at);
+  }
+}
+// raw: the thread's first block, loaded by the caller (in front of the weights: what is asked for first comes first).
 template <int XT, int NW = FNW, typename RowOf>
-__device__ __forceinline__ void few_quantize(uint8_t *smem, const void *x, int rows, int k, int kt, RowOf row_of) {
+__device__ __forceinline__ void few_quantize(uint8_t *smem, dt_raw<XT, 8> &raw, const void *x, int rows, int k, int kt, RowOf row_of) {
   float *s_as = few_scales(smem, rows, kt);
   const int sub = threadIdx.x & 15;
   for (int b = threadIdx.x / 16; b < rows * kt; b += NW * 4) {
-    const int r = b / kt, at = b - r * kt, c = at * 128 + sub * 8;
-    const int64_t src = row_of(r);
-    float v[8];
-    if (c < k) {
-      if constexpr (XT == RK_DTYPE_F32) {
-        dt_load_vec<XT, 4>(x, src * k + c, v);
-        dt_load_vec<XT, 4>(x, src * k + c + 4, v + 4);
-      } else {
-        dt_load_vec<XT, 8>(x, src * k + c, v);
-      }
-    } else {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = 0.f;
-    }
-    float amax = 0.f;
+    const int r = b / kt, at = b - r * kt;
+    float v[8], amax = 0.f;
+    dt_decode_raw<XT, 8>(raw, v);
+    if (b + NW * 4 < rows * kt) few_load<XT>(raw, x, b + NW * 4, rows, k, kt, row_of);
 #pragma unroll
     for (int e = 0; e < 8; ++e) amax = fmaxf(amax, fabsf(v[e]));
     const float s = fp8_scale(fp8_max16(amax));
     const Fp8Div div(s);
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] = div(v[e]);
-    *(uintx2 *)(smem + (size_t)r * few_row(kt) + c) =
+    *(uintx2 *)(smem + (size_t)r * few_row(kt) + at * 128 + sub * 8) =
         uintx2{fp8_codes4(v[0], v[1], v[2], v[3]), fp8_codes4(v[4], v[5], v[6], v[7])};
     if (sub == 0) s_as[r * kt + at] = s;
   }
@@ -130,13 +135,27 @@ __global__ __launch_bounds__(FNW * 64, 2) void fp8_few_kernel(const Fp8FewArgs g
       }
     }
   };
+  // The first rows of x in front of the weights, unless their addresses come from memory too.
+  const auto row_of = [&](int r) -> int64_t {
+    if constexpr (MODE == FEW_GATE_UP) return g.top_k > 0 ? (row0 + r) / g.top_k : (int64_t)min(g.tok[row0 + r], g.n_tok - 1);
+    return row0 + r;
+  };
+  constexpr int XQ = XT == FEW_CODES ? RK_DTYPE_F16 : XT;
+  dt_raw<XQ, 8> raw;
+  const bool early = MODE != FEW_GATE_UP || g.top_k > 0;
+  if constexpr (XT != FEW_CODES) {
+    if (early) few_load<XQ>(raw, g.x, threadIdx.x / 16, rows, g.k, kt, row_of);
+    __builtin_amdgcn_sched_barrier(0);
+  }
   static_for<D>([&](auto d_c) {
     if (decltype(d_c)::value < n_it) load(d_c, decltype(d_c)::value);
   });
 
   const float *s_as = few_scales(smem, rows, kt);
   if constexpr (XT != FEW_CODES) {
-    few_quantize<XT>(smem, g.x, rows, g.k, kt, [&](int r) { return MODE == FEW_GATE_UP ? (int64_t)min(g.tok[row0 + r], g.n_tok - 1) : row0 + r; });
+    __builtin_amdgcn_sched_barrier(0);
+    if (!early) few_load<XQ>(raw, g.x, threadIdx.x / 16, rows, g.k, kt, row_of);
+    few_quantize<XQ>(smem, raw, g.x, rows, g.k, kt, row_of);
     __syncthreads();
   }
 
@@ -268,11 +287,16 @@ __global__ __launch_bounds__(TNW * 64) void fp8_token_kernel(const Fp8FewArgs g)
     for (int i = 0; i < 4; ++i) r.w[i] = *(const intx4 *)(w + i * 1024);
     r.sw = g.ws[e * g.ws_stride + (int64_t)(nb / 4) * kt + k];
   };
+  const auto row_of = [&](int r) { return row0 + r; };
+  dt_raw<RK_DTYPE_F32, 8> raw;
+  few_load<RK_DTYPE_F32>(raw, g.x, threadIdx.x / 16, rows, g.k, kt, row_of);
+  __builtin_amdgcn_sched_barrier(0);
   static_for<D>([&](auto d_c) {
     if (decltype(d_c)::value < n_it) load(d_c, decltype(d_c)::value);
   });
+  __builtin_amdgcn_sched_barrier(0);
   const float *s_as = few_scales(smem, rows, kt);
-  few_quantize<RK_DTYPE_F32, TNW>(smem, g.x, rows, g.k, kt, [&](int r) { return row0 + r; });
+  few_quantize<RK_DTYPE_F32, TNW>(smem, raw, g.x, rows, g.k, kt, row_of);
   __syncthreads();
 
   floatx16 acc = {};

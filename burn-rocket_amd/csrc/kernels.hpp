@@ -316,7 +316,8 @@ struct Fp8FewArgs {
   int64_t w_stride, ws_stride;  // bytes and scales per expert
   int64_t up_scales;            // scales from a gate block's to its up block's
   int groups;                   // set by the launcher: blocks of n side by side in a workgroup
-  int top_k, accumulate;        // rk_launch_fp8_token
+  int top_k;                    // tokens of top_k rows each, one behind the other (first product: or 0, by tok)
+  int accumulate;               // rk_launch_fp8_token
 };
 bool rk_fp8_few_fits_x(int64_t m, int kt);
 bool rk_fp8_few_wants_x(int64_t m, int kt);
