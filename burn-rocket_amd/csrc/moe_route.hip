@@ -75,13 +75,19 @@ struct Queue {
         id[v + 1] = swap ? i : j;
       }
   }
-  __device__ __forceinline__ void pop() {
+  // The ids (below 16: the expert's place in its lane), four bits each, so that a step of the queue moves them at once.
+  using Order = std::conditional_t<V <= 8, uint32_t, uint64_t>;
+  __device__ __forceinline__ Order order() const {
+    Order o = 0;
 #pragma unroll
-    for (int v = 0; v + 1 < V; ++v) {
-      k[v] = k[v + 1];
-      id[v] = id[v + 1];
-    }
+    for (int v = 0; v < V; ++v) o |= (Order)id[v] << (4 * v);
+    return o;
+  }
+  __device__ __forceinline__ void pop(Order &o) {
+#pragma unroll
+    for (int v = 0; v + 1 < V; ++v) k[v] = k[v + 1];
     k[V - 1] = 0;
+    o >>= 4;
   }
 };
 
@@ -127,7 +133,7 @@ __device__ __forceinline__ int route_f64(const RouteArgs &g, int64_t t) {
     const int e = lane * V + v;
     const double s = g.score == RK_ROUTE_SOFTMAX ? p[v] / sum : 1 / (1 + exp(-p[v]));
     q.k[v] = e < E ? order_key(s + (double)g.bias[e]) : 0;
-    q.id[v] = e;
+    q.id[v] = v;
   }
   q.sort();
   if (g.top_groups < g.n_groups) {
@@ -136,7 +142,7 @@ __device__ __forceinline__ int route_f64(const RouteArgs &g, int64_t t) {
       uint64_t a = 0, b = 0;  // (sorted: the first two of the group)
 #pragma unroll
       for (int v = V - 1; v >= 0; --v)
-        if (q.id[v] / g.group_size == i && q.k[v]) {
+        if ((lane * V + q.id[v]) / g.group_size == i && q.k[v]) {
           b = a;
           a = q.k[v];
         }
@@ -155,15 +161,16 @@ __device__ __forceinline__ int route_f64(const RouteArgs &g, int64_t t) {
     }
     const uint64_t kept = __ballot(lane < g.n_groups && rank < g.top_groups);
 #pragma unroll
-    for (int v = 0; v < V; ++v) q.k[v] = kept >> min(q.id[v] / g.group_size, 63) & 1 ? q.k[v] : 0;
+    for (int v = 0; v < V; ++v) q.k[v] = kept >> min((lane * V + q.id[v]) / g.group_size, 63) & 1 ? q.k[v] : 0;
     q.sort();
   }
   int id = 0;
+  auto order = q.order();
   for (int j = 0; j < g.top_k; ++j) {
     const uint64_t m = wave_max(q.k[0]);
     const int at = __builtin_ctzll(__ballot(q.k[0] == m));
-    const int e = __builtin_amdgcn_readlane(q.id[0], at);
-    if (lane == at) q.pop();
+    const int e = at * V + (__builtin_amdgcn_readlane((int)order, at) & 15);
+    if (lane == at) q.pop(order);
     if (lane == j) id = e;
   }
   return id;
@@ -228,7 +235,7 @@ __global__ __launch_bounds__(ROUTE_WAVES * 64) void moe_route_kernel(const Route
       near = fmaxf(near, fabsf(by) < INFINITY ? fabsf(by) : 0.f);
     }
     q.k[v] = e < E ? order_key(by) : 0u;
-    q.id[v] = e;
+    q.id[v] = v;
   }
   q.sort();
   if constexpr (BIAS) near = fmaxf(1.f, __uint_as_float(wave_max(__float_as_uint(near)))) * 0x1p-20f;  // (not negative: ordered as integers)
@@ -251,7 +258,7 @@ __global__ __launch_bounds__(ROUTE_WAVES * 64) void moe_route_kernel(const Route
         uint32_t a = 0, b = 0;
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-          const uint32_t k = q.id[v] / by == i ? q.k[v] : 0u;
+          const uint32_t k = (lane * V + q.id[v]) / by == i ? q.k[v] : 0u;
           join2(a, b, k, 0u);
         }
         segment_top2(a, b, 64);
@@ -278,27 +285,32 @@ __global__ __launch_bounds__(ROUTE_WAVES * 64) void moe_route_kernel(const Route
       int by = size;
       asm volatile("" : "+s"(by));
 #pragma unroll
-      for (int v = 0; v < V; ++v) q.k[v] = kept >> min(q.id[v] / by, 63) & 1 ? q.k[v] : 0u;
+      for (int v = 0; v < V; ++v) q.k[v] = kept >> min((lane * V + q.id[v]) / by, 63) & 1 ? q.k[v] : 0u;
       q.sort();
     }
   }
 
   // The top_k: lane j keeps choice j. With a bias one more, to see how far the last one is from it.
   int id = 0;
-  float last = INFINITY;
-  for (int j = 0; j < g.top_k + (BIAS ? 1 : 0); ++j) {
+  uint32_t key = 0;  // lane j: choice j's (none: 0)
+  auto order = q.order();
+  const int picks = g.top_k + (BIAS && g.top_k < 64 ? 1 : 0);
+  for (int j = 0; j < picks; ++j) {
     const uint32_t m = wave_max(q.k[0]);
-    if constexpr (BIAS) {
-      if (m == 0) break;  // (as many experts as choices)
-      const float c = key_value(m);
-      unsure |= j > 0 && !(last - c > 2 * near);
-      last = c;
-      if (j == g.top_k) break;
-    }
+    if (BIAS && m == 0) break;  // (as many experts as choices)
     const int at = __builtin_ctzll(__ballot(q.k[0] == m));
-    const int e = __builtin_amdgcn_readlane(q.id[0], at);
-    if (lane == at) q.pop();
-    if (lane == j) id = e;
+    const int e = at * V + (__builtin_amdgcn_readlane((int)order, at) & 15);
+    if (lane == at) q.pop(order);
+    if (lane == j) {
+      id = e;
+      if constexpr (BIAS) key = m;
+    }
+  }
+  if constexpr (BIAS) {
+    // Neighbours in the order: a lane's choice and the next one's.
+    const uint32_t behind = g.top_k == 64 ? wave_max(q.k[0]) : 0u, after = __shfl_down(key, 1);
+    const uint32_t next = lane < 63 ? after : behind;
+    unsure |= __ballot(lane < g.top_k && next != 0 && !(key_value(key) - key_value(next) > 2 * near)) != 0;
   }
   if (BIAS && unsure) id = route_f64<V>(g, t);
   // Lane j's weight: the score of its choice's logit.
@@ -311,8 +323,16 @@ __global__ __launch_bounds__(ROUTE_WAVES * 64) void moe_route_kernel(const Route
   w = lane >= g.top_k ? 0.f : softmax ? expf(w - mx) / sum : 1.0f / (1.0f + expf(-w));
   if (g.norm) {
     float all = w;
+    if (g.top_k <= 16) {  // all in one row of lanes
+      const auto turned = [&](auto by_c) { return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(all), decltype(by_c)::value, 0xf, 0xf, false)); };
+      all += turned(ic<0x121>{});  // rotations by 1, 2, 4 and 8 lanes
+      all += turned(ic<0x122>{});
+      all += turned(ic<0x124>{});
+      all += turned(ic<0x128>{});
+    } else {
 #pragma unroll
-    for (int d = 1; d < 64; d *= 2) all += __shfl_xor(all, d);
+      for (int d = 1; d < 64; d *= 2) all += __shfl_xor(all, d);
+    }
     w = w / (all + 1e-20f);
   }
   if (lane < g.top_k) {
