@@ -247,7 +247,9 @@ __device__ __forceinline__ void fp8_store_tile(uint8_t *smem, Value value, void 
 
 // Smaller tiles, with the weights' fragments straight from memory to registers, as they lie: four waves of all BM rows and 32
 // outputs each, so that no two ask for the same weights, and LDS, which bounds such tiles otherwise, holds the rows alone.
-// STAGES - 1 stages of both are on the way. Two a CU of 64 × 128 move 15 TB/s out of the L2s.
+// STAGES - 1 stages of both are on the way. A stage of 64 × 128 takes 0.4 us of
+// its CU on MI355X, whether one tile is there or two, of three stages or four, K split over two groups of waves or not: 24 KB, 60
+// GB/s out of the L2 for a CU, 15 TB/s for all.
 template <int TM_, int STAGES_, bool EXACT_>
 struct Fp8Flow {
   static constexpr int TM = TM_, TN = 1, STAGES = STAGES_, WM = 1, WN = 4, NW = 4, NT = 256;
