@@ -247,9 +247,10 @@ __device__ __forceinline__ void fp8_store_tile(uint8_t *smem, Value value, void 
 
 // Smaller tiles, with the weights' fragments straight from memory to registers, as they lie: four waves of all BM rows and 32
 // outputs each, so that no two ask for the same weights, and LDS, which bounds such tiles otherwise, holds the rows alone.
-// STAGES - 1 stages of both are on the way. A stage of 64 × 128 takes 0.4 us of
-// its CU on MI355X, whether one tile is there or two, of three stages or four, K split over two groups of waves or not: 24 KB, 60
-// GB/s out of the L2 for a CU, 15 TB/s for all.
+// STAGES - 1 stages of both are on the way. A stage of 64 × 128 takes 0.36 us of
+// its CU on MI355X, of two tiles there 0.54 both (products 0.12 and 0.24, the 24 KB of each 0.2 at what a CU reads out of its L2):
+// barrier, LDS, products and folds one behind the other, which three stages or four, or K split over two groups of waves,
+// change little.
 template <int TM_, int STAGES_, bool EXACT_>
 struct Fp8Flow {
   static constexpr int TM = TM_, TN = 1, STAGES = STAGES_, WM = 1, WN = 4, NW = 4, NT = 256;
