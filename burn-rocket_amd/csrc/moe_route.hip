@@ -12,7 +12,7 @@
 // sorts its own, so that a pick is a maximum of the lanes' heads (lane exchanges inside the vector instruction), a ballot, and
 // a step of one lane's queue. With a bias the f32 sums decide wherever neighbours in the order are further apart than the
 // sums can be off; a token where two are not (about one in a thousand) is done again in f64. 16384 tokens, 256 experts, top 8
-// of 4 groups of 8 on MI355X: 22 us (52 with a search of all registers per pick and two maxima per group, 95 in f64).
+// of 4 groups of 8 on MI355X: 21 us (52 with a search of all registers per pick and two maxima per group, 95 in f64).
 namespace {
 constexpr int ROUTE_WAVES = 4;
 
@@ -363,7 +363,8 @@ hipError_t rk_launch_moe_route(const RouteArgs &args, hipStream_t st) {
 // Blocks of 1024 pairs. A pair's row is its expert's first row, plus the expert's pairs in earlier blocks, plus those of
 // earlier waves of its block, plus those of earlier lanes of its wave. The pairs of other blocks are counted by each block
 // itself while there are few, and in a launch of their own that leaves the blocks' counts in memory. No pair waits for
-// another block's, and nothing depends on the order of atomics. Bound by the trips to memory one behind the other.
+// another block's, and nothing depends on the order of atomics. Bound by the trips to memory one behind the other: 8192 pairs
+// over 128 experts on MI355X 8.7 us, 49152 over 64 8.6 and 2.7 for the counts.
 namespace {
 constexpr int LB = 1024;       // pairs per block
 constexpr int LW = LB / 64;
@@ -555,7 +556,7 @@ hipError_t rk_launch_moe_pairs(const RouteListArgs &g, hipStream_t st) {
 }
 
 // The weighted rows of each token to its result, in ascending expert id: y (+)= Σ rows. A thread per eight values; a
-// token's rows are asked for four at a time. Bound by the rows' bytes.
+// token's rows are asked for four at a time. Bound by the rows' bytes: 49152 fp16 rows of 2048 on MI355X 46 us, 4.4 TB/s.
 template <int DT, bool SCALED>
 __global__ __launch_bounds__(256) void moe_combine_kernel(const CombineArgs g) {
   constexpr int V = 8;
