@@ -10,6 +10,9 @@
 // The rows (32 columns of the products, most of them empty in a decode step) come as x itself: the workgroup quantizes them
 // into LDS once, while its first weights are on the way, so that a layer is one launch; or, where they are more, as codes
 // that each wave reads from the caches, whole lines at a time, one or two column blocks a wave.
+//
+// MI355X: a row through 5120 × 2048 4.3 us (2.4 TB/s), through 16384 × 2048 8.0 (4.2); the experts' products of 64 tokens of that
+// layer 76 and 37 us (5.2 and 5.3 TB/s); codes of 48 rows through 2048 × 4096 6.9, of 333 through 1000 × 1104 in f32 6.0.
 #include "fp8.hpp"
 #include "kernels.hpp"
 
