@@ -11,8 +11,8 @@
 // What bounds it is the picks, one maximum over the wave each. They go by 32-bit keys that order as the floats do: each lane
 // sorts its own, so that a pick is a maximum of the lanes' heads (lane exchanges inside the vector instruction), a ballot, and
 // a step of one lane's queue. With a bias the f32 sums decide wherever neighbours in the order are further apart than the
-// sums can be off; a token where two are not (about one in a thousand) is done again in f64. 16384 tokens, 256 experts, top 8
-// of 4 groups of 8 on MI355X: 21 us (52 with a search of all registers per pick and two maxima per group, 95 in f64).
+// sums can be off; a token where two are not (about one in four thousand) is done again in f64. 16384 tokens, 256 experts, top 8
+// of 4 groups of 8 on MI355X: 20 us (52 with a search of all registers per pick and two maxima per group, 95 in f64).
 namespace {
 constexpr int ROUTE_WAVES = 4;
 
@@ -106,7 +106,7 @@ __device__ __forceinline__ uint64_t wave_max(uint64_t x) {
   return (uint64_t)hi << 32 | lo;
 }
 
-// Lane j's choice j, with a bias, in f64. A token in a thousand comes here, but the launch waits for it: the same steps as
+// Lane j's choice j, with a bias, in f64. Few tokens come here, but the launch waits for them: the same steps as
 // below on wider keys, where exchanges of (f64, id) pairs took 25 us.
 template <int V>
 __device__ __forceinline__ int route_f64(const RouteArgs &g, int64_t t) {
@@ -220,8 +220,11 @@ __global__ __launch_bounds__(ROUTE_WAVES * 64) void moe_route_kernel(const Route
     for (int d = 1; d < 64; d *= 2) sum += __shfl_xor(sum, d);
   }
   Queue<V, uint32_t> q;
-  // With a bias: no f32 sum is off by `near` (a few roundings of the score, one of its own), a 2^20th of the largest finite
-  // |score + bias| or of 1; closer ones are not told apart.
+  // With a bias: f32 sums further apart than 2·near (groups' sums of two: 4·near) are in the order of the exact ones. With m
+  // the largest finite |score + bias|, or 1: a sigmoid's sum is off by 3.9·2^-24·m at most (the reciprocal's and the sum's
+  // last bit 1 each, 1 + e^-x 1, e^-x 0.5 and its argument 0.33 times p(1 - p), the largest that |x|·p(1 - p) gets to), a sum of
+  // two by 9.8; near is 5 of these. A softmax's also has its sum's error, up to 21 roundings of V and 6 additions, in |p1 - p2|:
+  // near is 16.
   float near = 0.f;
   bool unsure = false;
 #pragma unroll
@@ -238,7 +241,7 @@ __global__ __launch_bounds__(ROUTE_WAVES * 64) void moe_route_kernel(const Route
     q.id[v] = v;
   }
   q.sort();
-  if constexpr (BIAS) near = fmaxf(1.f, __uint_as_float(wave_max(__float_as_uint(near)))) * 0x1p-20f;  // (not negative: ordered as integers)
+  if constexpr (BIAS) near = fmaxf(1.f, __uint_as_float(wave_max(__float_as_uint(near)))) * (softmax ? 0x1p-20f : 0x5p-24f);  // (not negative: ordered as integers)
 
   // Groups: the score of one is its best choice, or with a bias the sum of its two best; experts of the others are closed.
   if (g.top_groups < g.n_groups) {
