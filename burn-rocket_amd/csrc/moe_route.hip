@@ -2,6 +2,7 @@
 // needs nothing from the host between its launches and can be captured into a graph.
 #include "common.hpp"
 #include "kernels.hpp"
+#include "moe_tiles.hpp"
 
 // ---------------------------------------------------------------------------
 // Router. A wave per token, V consecutive experts a lane. Choices are those of the f64 scores with their bias, or, where
@@ -495,35 +496,15 @@ __global__ __launch_bounds__(LB) void moe_lists_kernel(const RouteListArgs g, in
   }
   if (block < n_blocks) return;
 
-  // Tiles in expert order, and longest first: by quarters of tile_rows, in expert order within one. Thread x makes expert
-  // x's; four 16-bit counts (quarters 4, 3, 2, 1) share a word of the sums.
-  const int T = g.tile_rows, quarter = T / 4;
-  auto kinds = [&](int rows) -> uint64_t {
-    const int tail = rows % T;
-    uint64_t k = (uint64_t)(rows / T);
-    if (tail) k += (uint64_t)1 << (16 * (4 - (tail + quarter - 1) / quarter));
-    return k;
-  };
+  // Tiles in expert order, and longest first. Thread x makes expert x's.
+  const int T = g.tile_rows;
   uint64_t total;
-  const uint64_t mine = kinds(all), base = block_exclusive(mine, s_wave, &total);
-  auto field = [](uint64_t x, int f) { return (int)(x >> (16 * f) & 0xffff); };
-  auto sum4 = [&](uint64_t x) { return field(x, 0) + field(x, 1) + field(x, 2) + field(x, 3); };
-  int start[4];
-  for (int f = 0, at = 0; f < 4; ++f) {
-    start[f] = at;
-    at += field(total, f);
-  }
-  const int n = sum4(total);
-  if (tid < E) {
-    int at = sum4(base), full = start[0] + field(base, 0);
-    for (int r = 0; r < all; r += T) {
-      const int rows = min(T, all - r), f = 4 - (rows + quarter - 1) / quarter;
-      const MoeTile tile{tid, first + r, rows};
-      g.tiles[at++] = tile;
-      // (an expert has any number of whole tiles, and one shorter one at most: whole ones first in their quarter)
-      g.tiles_gu[f == 0 ? full++ : start[f] + field(base, f)] = tile;
-    }
-  }
+  const uint64_t before = block_exclusive(moe_tile_counts(all, T), s_wave, &total);
+  const int n = moe_tile_sum(total);
+  if (tid < E)
+    moe_tile_places(all, T, before, total, [&](int at, int at_gu, int r, int rows) {
+      g.tiles[at] = g.tiles_gu[at_gu] = MoeTile{tid, first + r, rows};
+    });
   // Rows without an expert, and what no tile uses.
   const int left = (int)g.rows - (int)valid, dead = (left + T - 1) / T;
   for (int x = n + tid; x < g.max_tiles; x += LB) {
