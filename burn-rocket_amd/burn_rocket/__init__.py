@@ -1068,6 +1068,11 @@ def moe_layer(x, logits, wid, top_k, bf16=False, **router):
     `router`) chooses from logits [s, E] f32; returned in x's type."""
     x, logits = np.ascontiguousarray(x), _f32(logits)
     dt = _float_dtype(x, bf16, "moe_layer")
+    # the calls below are given pointers: rows that are missing or too short would be read behind their buffers
+    if x.ndim != 2 or logits.ndim != 2 or len(x) != len(logits):
+        _shape_error("moe_layer", f"x [s, H] and logits [s, E], not {x.shape} and {logits.shape}")
+    if x.shape[1] != weight_info(wid)[2]:
+        _shape_error("moe_layer", f"x of {x.shape[1]} values a row, a stack of {weight_info(wid)[2]}")
     ids, wts = route_experts(logits, top_k, **router)
     if len(x) == 0:
         return x.copy()
