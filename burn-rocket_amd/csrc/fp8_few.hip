@@ -362,8 +362,10 @@ hipError_t rk_launch_fp8_token(const Fp8FewArgs &g, int64_t s, bool exact, hipSt
   return hipGetLastError();
 }
 
-// Rows that a workgroup can quantize into its LDS (x itself as input), and those that it can take as codes.
-bool rk_fp8_few_fits_x(int64_t m, int kt) { return m <= 32 && few_in((int)m, kt) <= 64 * 1024; }
+// Rows that a workgroup can quantize into its LDS (x itself as input), and those that it can take as codes. Up to 32 rows of
+// 64 KB of codes in all always fit: with K padded to 128, the scales and 16 bytes a row they are 65536·132/128 + 32·(132 + 16)
+// bytes at most, and the sums behind them 32 KB.
+bool rk_fp8_few_fits_x(int64_t m, int kt) { return m <= 32 && few_in((int)m, kt) <= 72320; }
 // Where that is faster than a launch that quantizes once and a second one on codes: every workgroup takes 0.5 us for 32
 // blocks of x. us so and in two launches, MI355X: 8 × 4096 × 2048 6.6 and 7.1, 16 × 4096 × 2048 8.8 and 7.2, 16 × 1024 ×
 // 1024 5.7 and 6.2, 24 × 1024 × 1024 6.7 and 6.2, 4 × 4096 × 4096 8.1 and 8.8, 8 × 4096 × 4096 10.5 and 8.9.

@@ -272,3 +272,29 @@ def test_two_streams_share_the_codes_memory(rk):
         check(c.download((len(v), n), np.float32), "f32", ref.quantize(v), (codes, scales), k, f"m={len(v)}")
     for st in sts:
         rk.destroy_stream(st)
+
+
+@pytest.mark.parametrize("m,k", [(32, 2048), (1, 65536), (2, 32768), (3, 21840), (31, 2112), (5, 13104)])
+def test_captured_calls_up_to_64_kb_of_codes(rk, m, k):
+    """The largest calls that may be captured by one entry, K of whole blocks and not."""
+    note(f"fp8 captured m={m} k={k}")
+    from test_gpu_sequences import Graph
+    assert m * k <= 65536
+    lib, r = rk.lib(), np.random.default_rng(k)
+    n = 40
+    codes, scales = ref.random_weight(r, n, k)
+    wid, st = int(rk.pack_fp8(codes, scales)), rk.new_stream()
+    x, c = rk.DeviceBuffer(m * k * 2), rk.DeviceBuffer(m * n * 2)
+    x.zero()
+    rcs = []
+    g = Graph(st, lambda: rcs.append(lib.rk_matmul_fp8_dev(wid, x.ptr, TYPES["bf16"], m, k, c.ptr, TYPES["bf16"], st)))
+    assert rcs == [0], lib.rk_last_error()
+    for _ in range(3):
+        host, v = ref.cast(rows(r, m, k), "bf16")
+        x.upload(host)
+        g.replay()
+        rk.synchronize(st)
+        check(c.download((m, n), np.uint16), "bf16", ref.quantize(v), (codes, scales), k, f"captured m={m}")
+        product(rk, host, "bf16", wid, n, "bf16", False)  # and the call outside of one, in between
+    g.destroy()
+    rk.destroy_stream(st)
