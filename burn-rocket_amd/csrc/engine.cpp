@@ -2180,8 +2180,9 @@ std::vector<std::pair<const char *, size_t>> moe_buffers(const Weight &w, int64_
 }
 
 // fp8 experts. Tiles of few rows: each workgroup quantizes the rows it multiplies; silu(gate)·up goes to the second product
-// in f32. Others: the tokens are quantized once, and the first product quantizes its results. fp16 results: the first product has f32 sums, since a code of its results that flips is worth more than an fp16
-// rounding; f32 results: both have.
+// in f32. Others: the tokens are quantized once, and the first product quantizes its results. fp16 results: the first product
+// has f32 sums, since a code of its results that flips is worth more than an fp16 rounding; f32 results: both have. The rows
+// that are summed per token are f32 but in front of bf16 results on tiles of many rows (moe_fp8.hip).
 int moe_run_fp8(CallScope &cs, const Weight &w, const MoePlan &plan, const void *x, void *y, int dtype, bool accumulate,
                 const std::function<int(int)> &lists = nullptr) {
   const char *op = "rk_moe_experts_fp8_dev";
@@ -2278,7 +2279,7 @@ int moe_run_fp8(CallScope &cs, const Weight &w, const MoePlan &plan, const void 
     g.tiles = plan.tiles;
     g.row_w = plan.roww;
     g.out = yb;
-    if (!exact2) RK_TRY(moe_buf(cs, plan, "moe_ys", (size_t)R * ((H + 63) / 64) * 4, &ys));
+    if (dtype == RK_DTYPE_BF16 && !exact2) RK_TRY(moe_buf(cs, plan, "moe_ys", (size_t)R * ((H + 63) / 64) * 4, &ys));
     g.out_s = (float *)ys;
     HIP_TRY(rk_launch_moe_fp8_down(g, exact2, st), op);
   }

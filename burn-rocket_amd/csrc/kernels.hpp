@@ -401,8 +401,8 @@ struct Fp8MoeArgs {
   int n_tiles, tile_rows;
   const int32_t *tok;
   const float *row_w;
-  void *out;           // codes [rows, ceil(n/128)·128]; second product: rows [rows, n], f32 (exact) or fp16
-  float *out_s;        // scales of the codes; of fp16 rows per rk_moe_fp8_down_group(tile_rows) outputs
+  void *out;           // codes [rows, ceil(n/128)·128]; second product: rows [rows, n], f32, or fp16 with out_s
+  float *out_s;        // scales of the codes; of fp16 rows per rk_moe_fp8_down_group(tile_rows) outputs (null: f32 rows)
 };
 hipError_t rk_launch_moe_fp8_gate_up(const Fp8MoeArgs &g, bool exact, hipStream_t st);
 int rk_moe_fp8_down_group(int tile_rows);

@@ -86,7 +86,8 @@ __global__ __launch_bounds__(T::NT, 2) void moe_fp8_gate_up_kernel(const Fp8MoeA
   }
 }
 
-template <class T>
+// ROWS16: the weighted rows as fp16 under scales, for bf16 results; f32 otherwise.
+template <class T, bool ROWS16>
 __global__ __launch_bounds__(T::NT, 2) void moe_fp8_down_kernel(const Fp8MoeArgs g) {
   extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
   MoeTile tile;
@@ -99,9 +100,11 @@ __global__ __launch_bounds__(T::NT, 2) void moe_fp8_down_kernel(const Fp8MoeArgs
   t.run(smem, g.a + (int64_t)tile.row0 * KT * 128, (int64_t)tile.rows * KT * 128, g.as + (int64_t)tile.row0 * KT, (int64_t)tile.rows * KT * 4,
         [&](int r) -> int64_t { return r < tile.rows ? r : -1; }, tile.rows, g.w + (int64_t)tile.expert * g.w_stride + (int64_t)nb0 * KT * 4096,
         nblk - nb0, ws, (int64_t)(nblk / 4) * KT * 4, [&](int b) { return (int64_t)min((nb0 + b) / 4, nblk / 4 - 1) * KT; }, KT * 128, KT);
-  // Rows times their router weight: f32, or fp16 under a power of two per row and wave (T::WTN outputs) that takes the
-  // largest to [2^14, 2^15): 2^-12 of a term, under what the sum is rounded to in the end, for half of the bytes that the
-  // combine reads back.
+  // Rows times their router weight, in f32 for f32 and fp16 results: an fp16 row's rounding is as large as the result's own, and
+  // larger where experts cancel. In front of bf16 results (2^-8 of a result) fp16 rows, under a power of two per row and wave
+  // (T::WTN outputs) that takes the largest to [2^14, 2^15): 2^-11 of a term, and below 2^-29 of the largest 2^-40 of that,
+  // for half of the bytes (8192 tokens of a 64-expert layer, MI355X: this product and the combine 261 us, with f32 rows 351; the
+  // layer in fp16 1053 us, and 974 with fp16 rows).
   float *const to = (float *)g.out + (int64_t)tile.row0 * g.n + n0;
   const int tid = fresh_tid(), col = tid & 31, h = (tid >> 5) & 1;
   const int wave = tid >> 6, wm = wave / T::WN, wn = wave % T::WN;
@@ -110,7 +113,7 @@ __global__ __launch_bounds__(T::NT, 2) void moe_fp8_down_kernel(const Fp8MoeArgs
   for (int j = 0; j < T::TM; ++j) {
     const int r = wm * T::WTM + j * 32 + col;
     rw[j] = r < tile.rows ? g.row_w[tile.row0 + r] : 0.f;
-    if constexpr (!T::EXACT) {
+    if constexpr (ROWS16) {
       float amax = 0.f;
 #pragma unroll
       for (int i = 0; i < T::TN; ++i)
@@ -128,8 +131,10 @@ __global__ __launch_bounds__(T::NT, 2) void moe_fp8_down_kernel(const Fp8MoeArgs
     }
   }
   const auto value = [&](int i, int j, int r) { return t.acc[i][j][r] * rw[j]; };
-  if constexpr (!T::EXACT) {
+  if constexpr (ROWS16) {
     fp8_store_tile<T, RK_DTYPE_F16>(smem, value, (uint16_t *)g.out + (int64_t)tile.row0 * g.n + n0, g.n, tile.rows, g.n - n0);
+  } else if constexpr (T::BM * T::BN * 4 <= T::SMEM) {
+    fp8_store_tile<T, RK_DTYPE_F32>(smem, value, to, g.n, tile.rows, g.n - n0);
   } else {
 #pragma unroll
     for (int j = 0; j < T::TM; ++j) {
@@ -147,11 +152,11 @@ __global__ __launch_bounds__(T::NT, 2) void moe_fp8_down_kernel(const Fp8MoeArgs
   }
 }
 
-template <class T, bool GU>
+template <class T, bool GU, bool ROWS16 = false>
 static hipError_t launch_moe_fp8(const Fp8MoeArgs &g, hipStream_t st) {
   void (*kern)(const Fp8MoeArgs);
   if constexpr (GU) kern = moe_fp8_gate_up_kernel<T>;
-  else kern = moe_fp8_down_kernel<T>;
+  else kern = moe_fp8_down_kernel<T, ROWS16>;
   static bool attr_set = false;
   if (!attr_set) {
     hipError_t e = hipFuncSetAttribute((const void *)kern, hipFuncAttributeMaxDynamicSharedMemorySize, T::SMEM);
@@ -175,9 +180,12 @@ static hipError_t launch_moe_fp8_any(const Fp8MoeArgs &g, bool exact, hipStream_
     if (g.tile_rows == 256) return launch_moe_fp8<Fp8Tile<256, 256, 4, 2, 2, false>, GU>(g, st);
     return launch_moe_fp8<Fp8Tile<128, 256, 2, 4, 3, false>, GU>(g, st);
   } else {
-    if (exact) return launch_moe_fp8<Fp8Tile<128, 256, 2, 4, 2, true>, GU>(g, st);
-    if (g.tile_rows == 256) return launch_moe_fp8<Fp8Tile<256, 256, 4, 2, 2, false>, GU>(g, st);
-    return launch_moe_fp8<Fp8Tile<128, 128, 2, 2, 2, false>, GU>(g, st);
+    const bool rows16 = g.out_s != nullptr;
+    if (exact) return rows16 ? hipErrorInvalidValue : launch_moe_fp8<Fp8Tile<128, 256, 2, 4, 2, true>, GU>(g, st);
+    using Large = Fp8Tile<256, 256, 4, 2, 2, false>;
+    using Small = Fp8Tile<128, 128, 2, 2, 2, false>;
+    if (g.tile_rows == 256) return rows16 ? launch_moe_fp8<Large, GU, true>(g, st) : launch_moe_fp8<Large, GU>(g, st);
+    return rows16 ? launch_moe_fp8<Small, GU, true>(g, st) : launch_moe_fp8<Small, GU>(g, st);
   }
 }
 hipError_t rk_launch_moe_fp8_gate_up(const Fp8MoeArgs &g, bool exact, hipStream_t st) {

@@ -30,3 +30,53 @@ def test_tiles_of_two_and_four_rows(rk, h, i, s, how):
     want, most = experts(x, ids, wts, stack, "f32")
     assert (np.abs(got - want) <= most + np.abs(want) * 2.0**-23).all()
     plan.destroy()
+
+
+def run_fp8(rk, wid, x, ids, wts, dtype):
+    """rk_moe_experts_fp8_dev on rows of a 16-bit or 32-bit type."""
+    lib, s = rk.lib(), len(x)
+    plan = rk.routed_plan(wid, s, ids.shape[1])
+    bufs = [rk.DeviceBuffer.from_array(a) for a in (x, ids, wts, x)]
+    plan.route(s, bufs[1].ptr, bufs[2].ptr)
+    assert lib.rk_moe_experts_fp8_dev(int(wid), plan.ptr, bufs[0].ptr, bufs[3].ptr, {"f32": 0, "f16": 1, "bf16": 2}[dtype], 0, None) == 0
+    rk.synchronize()
+    got = ref.widen(bufs[3].download(x.shape, x.dtype), dtype)
+    plan.destroy()
+    return got
+
+
+def positive_weight(r, e, n, k):
+    """Codes of 1 to 2 in steps of a quarter: with rows of such values every product of codes is a multiple of 2^-10 of the
+    largest, which no instruction cuts."""
+    codes = ref.encode(1 + r.integers(0, 5, (e, n, k)) / 4)
+    return codes, (0.02 * (0.8 + 0.4 * r.random((e, ref.blocks(n), ref.blocks(k))))).astype(np.float32)
+
+
+def rows_error(ids, wts, stack, x, dtype):
+    """What bf16 layers on tiles of many rows may lose besides: each expert's weighted row as an fp16 number."""
+    if dtype != "bf16":
+        return 0
+    return 2.0**-11 * sum(np.abs(experts(x, ids[:, j:j + 1], wts[:, j:j + 1], stack, dtype)[0]) for j in range(ids.shape[1]))
+
+
+@pytest.mark.parametrize("rows", [128, 256])
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+def test_experts_that_nearly_cancel(rk, monkeypatch, rows, dtype):
+    """Two equal experts under weights of nearly the same size and opposite signs: what a token's rows lose before they are
+    summed is as large as the result."""
+    note(f"fp8 experts that cancel rows={rows} {dtype}")
+    monkeypatch.setenv("RK_MOE_FP8_ROWS", str(rows))
+    r = np.random.default_rng(rows)
+    s, h, i = 40, 256, 272
+    stack = [positive_weight(r, 1, n, k) for n, k in ((i, h), (i, h), (h, i))]
+    stack = [(np.repeat(c, 2, 0), np.repeat(sc, 2, 0)) for c, sc in stack]
+    wid = rk.pack_moe_fp8(*stack[0], *stack[1], *stack[2])
+    x, v = ref.cast(1 + r.random((s, h)), dtype)
+    ids = np.ascontiguousarray(np.tile([[0, 1]], (s, 1)), np.uint32)
+    w = r.uniform(0.5, 1, (s, 1))
+    wts = np.ascontiguousarray(np.concatenate([w, -w * (1 + 2.0**-9 * r.random((s, 1)))], 1), np.float32)
+    want, most = experts(v, ids, wts, stack, dtype)
+    most = most + rows_error(ids, wts, stack, v, dtype)
+    off = np.abs(run_fp8(rk, wid, x, ids, wts, dtype) - want)
+    bound = most + (np.abs(want) + most) * ref.HALF[dtype] + 2.0**-24 * np.abs(want)
+    assert (off <= bound).all(), f"{np.max(off / bound):.3g} times what it may be off"
