@@ -503,7 +503,9 @@ __global__ __launch_bounds__(LB) void moe_lists_kernel(const RouteListArgs g, in
   const int n = moe_tile_sum(total);
   if (tid < E)
     moe_tile_places(all, T, before, total, [&](int at, int at_gu, int r, int rows) {
-      g.tiles[at] = g.tiles_gu[at_gu] = MoeTile{tid, first + r, rows};
+      const MoeTile tile{tid, first + r, rows};
+      g.tiles[at] = tile;
+      g.tiles_gu[at_gu] = tile;
     });
   // Rows without an expert, and what no tile uses.
   const int left = (int)g.rows - (int)valid, dead = (left + T - 1) / T;

@@ -31,14 +31,11 @@ RK_TILES_FN int moe_tile_sum(uint64_t counts) {
 // whole tiles and one shorter one at most, behind the whole ones of its field.
 template <typename Put>
 RK_TILES_FN void moe_tile_places(int all, int T, uint64_t before, uint64_t total, Put put) {
-  int start[4];
-  for (int f = 0, at = 0; f < 4; ++f) {
-    start[f] = at + moe_tile_count(before, f);
-    at += moe_tile_count(total, f);
-  }
-  int at = moe_tile_sum(before);
-  for (int r = 0; r < all; r += T) {
-    const int rows = all - r < T ? all - r : T, f = moe_tile_field(rows, T);
-    put(at++, f == 0 ? start[0]++ : f == 1 ? start[1] : f == 2 ? start[2] : start[3], r, rows);
-  }
+  int at = moe_tile_sum(before), whole = moe_tile_count(before, 0), r = 0;
+  for (; r + T <= all; r += T) put(at++, whole++, r, T);
+  if (r == all) return;
+  const int f = moe_tile_field(all - r, T);
+  int place = f == 0 ? whole : moe_tile_count(before, f);
+  for (int longer = 0; longer < f; ++longer) place += moe_tile_count(total, longer);
+  put(at, place, r, all - r);
 }
