@@ -102,7 +102,7 @@ __global__ __launch_bounds__(T::NT, 2) void moe_fp8_down_kernel(const Fp8MoeArgs
         nblk - nb0, ws, (int64_t)(nblk / 4) * KT * 4, [&](int b) { return (int64_t)min((nb0 + b) / 4, nblk / 4 - 1) * KT; }, KT * 128, KT);
   // Rows times their router weight, in f32 for f32 and fp16 results: an fp16 row's rounding is as large as the result's own, and
   // larger where experts cancel. In front of bf16 results (2^-8 of a result) fp16 rows, under a power of two per row and wave
-  // (T::WTN outputs) that takes the largest to [2^14, 2^15): 2^-11 of a term, and below 2^-29 of the largest 2^-40 of that,
+  // (T::WTN outputs) that takes the largest to [2^14, 2^15): 2^-11 of a term, and below 2^-28 of the largest 2^-39 of that,
   // for half of the bytes (8192 tokens of a 64-expert layer, MI355X: this product and the combine 261 us, with f32 rows 351; the
   // layer in fp16 1053 us, and 974 with fp16 rows).
   float *const to = (float *)g.out + (int64_t)tile.row0 * g.n + n0;
@@ -123,8 +123,19 @@ __global__ __launch_bounds__(T::NT, 2) void moe_fp8_down_kernel(const Fp8MoeArgs
           amax = fmaxf(amax, fabsf(t.acc[i][j][e]));
         }
       amax = fmaxf(amax, __shfl_xor(amax, 32));
-      // exponent of the largest; nothing to scale in rows of zeros, nor by what is infinite
-      const int x = amax > 0.f && amax < INFINITY ? max((int)(__float_as_uint(amax) >> 23) - 127 - 14, -100) : 0;
+      if (amax == INFINITY) {  // the largest of the finite ones: an infinite one needs no scale
+        amax = 0.f;
+#pragma unroll
+        for (int i = 0; i < T::TN; ++i)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const float v = fabsf(t.acc[i][j][e]);
+            amax = fmaxf(amax, v < INFINITY ? v : 0.f);
+          }
+        amax = fmaxf(amax, __shfl_xor(amax, 32));  // (both lanes of a row are here)
+      }
+      // exponent of the largest; nothing to scale in rows of zeros
+      const int x = amax > 0.f ? max((int)(__float_as_uint(amax) >> 23) - 127 - 14, -100) : 0;
       rw[j] = ldexpf(1.f, -x);
       if (h == 0 && r < tile.rows && n0 + wn * T::WTN < g.n)
         g.out_s[((int64_t)tile.row0 + r) * ((g.n + T::WTN - 1) / T::WTN) + (n0 + wn * T::WTN) / T::WTN] = ldexpf(1.f, x);

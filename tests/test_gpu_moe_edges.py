@@ -80,3 +80,29 @@ def test_experts_that_nearly_cancel(rk, monkeypatch, rows, dtype):
     off = np.abs(run_fp8(rk, wid, x, ids, wts, dtype) - want)
     bound = most + (np.abs(want) + most) * ref.HALF[dtype] + 2.0**-24 * np.abs(want)
     assert (off <= bound).all(), f"{np.max(off / bound):.3g} times what it may be off"
+
+
+@pytest.mark.parametrize("rows", [128, 256])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_an_infinite_result_leaves_its_neighbours(rk, monkeypatch, rows, dtype):
+    """One output of a token beyond the largest f32; the others of its group are large but finite, and stay that."""
+    note(f"fp8 experts, an infinite result, rows={rows} {dtype}")
+    monkeypatch.setenv("RK_MOE_FP8_ROWS", str(rows))
+    r = np.random.default_rng(rows)
+    s, h, i, at = 40, 256, 272, 5
+    stack = [positive_weight(r, 2, n, k) for n, k in ((i, h), (i, h), (h, i))]
+    codes, scales = stack[2]
+    codes[:] = 1            # 2^-9
+    codes[:, at] = 126      # 448
+    scales[:] = np.float32(2.0**108)
+    wid = rk.pack_moe_fp8(*stack[0], *stack[1], *stack[2])
+    x, v = ref.cast(1 + r.random((s, h)), dtype)
+    ids, wts = choices(r, s, 2, 2, "any")
+    want, most = experts(v, ids, wts, stack, dtype)
+    most = most + rows_error(ids, wts, stack, v, dtype)
+    got = run_fp8(rk, wid, x, ids, wts, dtype)
+    rest = np.arange(h) != at
+    assert (want[:, at] > 2.0**128).all() and (want[:, rest] < 2.0**127).all()
+    assert (got[:, at] == np.inf).all()
+    off, bound = np.abs(got - want)[:, rest], (most + (np.abs(want) + most) * ref.HALF[dtype] + 2.0**-24 * np.abs(want))[:, rest]
+    assert (off <= bound).all(), f"{np.max(off / bound):.3g} times what it may be off"
