@@ -1,5 +1,7 @@
 // The router of a mixture of experts, and the lists of expert tiles that its choices make, both on the GPU: a routed layer
 // needs nothing from the host between its launches and can be captured into a graph.
+#include <cfloat>
+
 #include "common.hpp"
 #include "kernels.hpp"
 #include "moe_tiles.hpp"
@@ -13,7 +15,7 @@
 // sorts its own, so that a pick is a maximum of the lanes' heads (lane exchanges inside the vector instruction), a ballot, and
 // a step of one lane's queue. With a bias the f32 sums decide wherever neighbours in the order are further apart than the
 // sums can be off; a token where two are not (about one in four thousand) is done again in f64. 16384 tokens, 256 experts, top 8
-// of 4 groups of 8 on MI355X: 20 us (52 with a search of all registers per pick and two maxima per group, 95 in f64).
+// of 4 groups of 8 on MI355X: 18.4 us, 18.7 with a bias of -1e9 on every third expert (52 with a search of all registers per pick and two maxima per group, 95 in f64).
 namespace {
 constexpr int ROUTE_WAVES = 4;
 
@@ -221,12 +223,14 @@ __global__ __launch_bounds__(ROUTE_WAVES * 64) void moe_route_kernel(const Route
     for (int d = 1; d < 64; d *= 2) sum += __shfl_xor(sum, d);
   }
   Queue<V, uint32_t> q;
-  // With a bias: f32 sums further apart than 2·near (groups' sums of two: 4·near) are in the order of the exact ones. With m
-  // the largest finite |score + bias|, or 1: a sigmoid's sum is off by 3.9·2^-24·m at most (the reciprocal's and the sum's
+  // With a bias: f32 sums further apart than 2·near·m (groups' sums of two: 4·near·m) are in the order of the exact ones, m the
+  // larger magnitude of the compared ones, or 1: a sigmoid's sum is off by 3.9·2^-24·m at most (the reciprocal's and the sum's
   // last bit 1 each, 1 + e^-x 1, e^-x 0.5 and its argument 0.33 times p(1 - p), the largest that |x|·p(1 - p) gets to), a sum of
   // two by 9.8; near is 5 of these. A softmax's also has its sum's error, up to 21 roundings of V and 6 additions, in |p1 - p2|:
-  // near is 16.
-  float near = 0.f;
+  // near is 16. What lies further down is off by more only where it is lower by more, so that neighbours are all to look at,
+  // and an expert that a bias of -1e9 closes does not make the others unsure. (-inf is exact: its m is the largest finite number.)
+  const float near = softmax ? 0x1p-20f : 0x5p-24f;
+  float top = 0.f;
   bool unsure = false;
 #pragma unroll
   for (int v = 0; v < V; ++v) {
@@ -236,13 +240,12 @@ __global__ __launch_bounds__(ROUTE_WAVES * 64) void moe_route_kernel(const Route
       const float p = softmax ? __builtin_amdgcn_exp2f((x[v] - mx) * 1.44269504f) * __builtin_amdgcn_rcpf(sum)
                               : __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(x[v] * -1.44269504f));
       by = p + bias[v];
-      near = fmaxf(near, fabsf(by) < INFINITY ? fabsf(by) : 0.f);
+      top = fmaxf(top, by < INFINITY ? by : 0.f);
     }
     q.k[v] = e < E ? order_key(by) : 0u;
     q.id[v] = v;
   }
   q.sort();
-  if constexpr (BIAS) near = fmaxf(1.f, __uint_as_float(wave_max(__float_as_uint(near)))) * (softmax ? 0x1p-20f : 0x5p-24f);  // (not negative: ordered as integers)
 
   // Groups: the score of one is its best choice, or with a bias the sum of its two best; experts of the others are closed.
   if (g.top_groups < g.n_groups) {
@@ -279,7 +282,11 @@ __global__ __launch_bounds__(ROUTE_WAVES * 64) void moe_route_kernel(const Route
     if constexpr (BIAS) {
       const int in = __builtin_ctzll(__ballot(lane < g.n_groups && rank == g.top_groups - 1));
       const int out = __builtin_ctzll(__ballot(lane < g.n_groups && rank == g.top_groups));
-      unsure = !(key_value((uint32_t)__builtin_amdgcn_readlane(mine, in)) - key_value((uint32_t)__builtin_amdgcn_readlane(mine, out)) > 4 * near);
+      const float last = key_value((uint32_t)__builtin_amdgcn_readlane(mine, in)), first = key_value((uint32_t)__builtin_amdgcn_readlane(mine, out));
+      // What a sum of two, s, is made of is at most top, and where negative at least s - top, or s: magnitudes of up to
+      // max(top, 1) - min(s, 0). (Sums near the largest magnitude may be infinite in f32 alone.)
+      const float m = fmaxf(1.f, __uint_as_float(wave_max(__float_as_uint(top)))) + fminf(fmaxf(-first, 0.f), FLT_MAX);  // (top >= 0: ordered as an integer)
+      unsure = !(last - first > 4 * near * m) || last < -0x1p126f;
     }
     if (shift >= 0) {
       const bool keep = kept >> (lane >> shift) & 1;
@@ -314,7 +321,9 @@ __global__ __launch_bounds__(ROUTE_WAVES * 64) void moe_route_kernel(const Route
     // Neighbours in the order: a lane's choice and the next one's.
     const uint32_t behind = g.top_k == 64 ? wave_max(q.k[0]) : 0u, after = __shfl_down(key, 1);
     const uint32_t next = lane < 63 ? after : behind;
-    unsure |= __ballot(lane < g.top_k && next != 0 && !(key_value(key) - key_value(next) > 2 * near)) != 0;
+    const float mine = key_value(key), other = key_value(next);
+    const float m = fminf(fmaxf(fmaxf(1.f, fabsf(mine)), fabsf(other)), FLT_MAX);
+    unsure |= __ballot(lane < g.top_k && next != 0 && !(mine - other > 2 * near * m)) != 0;
   }
   if (BIAS && unsure) id = route_f64<V>(g, t);
   // Lane j's weight: the score of its choice's logit.
