@@ -2386,12 +2386,20 @@ int moe_check(uint64_t id, int64_t s, int top_k, Weight **w, const char *op) {
   if (!*w || !(*w)->moe) return fail(RK_E_SHAPE, op, "id is not an expert stack");
   if (s <= 0 || top_k <= 0 || top_k > (*w)->n_experts)
     return fail(RK_E_SHAPE, op, "need s > 0 and 0 < top_k <= n_experts");
+  const int64_t H = (*w)->hidden, I = (*w)->inter;
+  if (s > INT32_MAX) return fail(RK_E_SHAPE, op, "s must stay below 2^31");
+  if ((*w)->moe_fp8) {
+    // 32-bit offsets into the tokens' codes alone; bucket rows are addressed in 64 bits, their tiles times columns counted in 32.
+    if (s * H >= ((int64_t)1 << 31) || s * top_k > (((int64_t)1 << 33) - 1) / std::max(H, I))
+      return fail(RK_E_SHAPE, op, "s·hidden must stay below 2^31, s·top_k·hidden and s·top_k·inter below 2^33");
+    return RK_OK;
+  }
   // The expert kernels address the int8 activations (x [s, hidden], the
   // quantized silu·up rows [s·top_k, inter]) with 32-bit byte offsets.
-  if (s * (*w)->hidden >= ((int64_t)1 << 31) || s * top_k * (*w)->inter >= ((int64_t)1 << 31))
+  if (s * H >= ((int64_t)1 << 31) || s * top_k * I >= ((int64_t)1 << 31))
     return fail(RK_E_SHAPE, op, "s·hidden and s·top_k·inter must stay below 2^31");
   // The combine reads the per-slot f32 rows [s·top_k, hidden] the same way.
-  if (s * top_k * (*w)->hidden * 4 >= ((int64_t)1 << 31))
+  if (s * top_k * H * 4 >= ((int64_t)1 << 31))
     return fail(RK_E_SHAPE, op, "s·top_k·hidden f32 values must stay below 2^31 bytes");
   return RK_OK;
 }
@@ -3472,8 +3480,6 @@ extern "C" int rk_moe_routed_plan_create(rk_weight_id id, int64_t max_s, int top
     if (w->n_experts > RK_ROUTE_MAX_EXPERTS) return fail(RK_E_UNSUPPORTED, op, "up to 1024 experts");
     if (max_s > kMaxRoutedRows / top_k) return fail(RK_E_SHAPE, op, "max_s·top_k above 2^20");
     const int64_t rows = max_s * top_k;
-    if (w->moe_fp8 && std::min(rows, moe_fp8_few_limit(*w)) / routed_tile_rows(*w, 1, 1) > 32768)
-      return fail(RK_E_SHAPE, op, "more than 2^15 tiles");
     size_t bytes = 0;
     const auto take = [&](size_t n) {
       const size_t at = bytes;

@@ -638,8 +638,9 @@ int rk_moe_route_dev(const void *logits, int dtype, int64_t s, int n_experts, in
 
 /* A plan of rk_moe_experts_planned_dev whose lists are built on the GPU, and that owns what
  * its calls need: room for batches of up to max_s tokens. For stacks of up to 1024 experts
- * and up to 2^20 rows max_s·top_k. The limits of rk_moe_experts_dev hold for max_s. Freed by
- * rk_moe_plan_destroy, which waits for its calls; counted by rk_mem_stats as scratch. */
+ * and up to 2^20 rows max_s·top_k. The limits of the stack's calls (rk_moe_experts_dev,
+ * rk_pack_moe_fp8) hold for max_s. Freed by rk_moe_plan_destroy, which waits for its calls;
+ * counted by rk_mem_stats as scratch. */
 int rk_moe_routed_plan_create(rk_weight_id id, int64_t max_s, int top_k, void **plan);
 /* The plan's next batch: ids [s, top_k] and wts [s, top_k] on the device, ordered on
  * `stream` after the calls that used the plan. An id that names no expert (>= n_experts: an
@@ -661,8 +662,9 @@ int rk_moe_plan_route_dev(void *plan, int64_t s, const uint32_t *ids, const floa
  * hidden and inter are multiples of 16, up to 65536. rk_moe_experts_dev, the planned calls
  * and their accumulating forms take it like a Q8_0 stack, with f32 x and y: x quantized as by
  * rk_quantize_fp8_dev, silu(gate)·up in f32 quantized the same way, and the products of
- * rk_matmul_fp8_dev in f32; tokens are summed in ascending expert id. rk_moe_gate_up_dev does
- * not take it (RK_E_UNSUPPORTED). */
+ * rk_matmul_fp8_dev in f32; tokens are summed in ascending expert id. RK_E_SHAPE when s·hidden
+ * reaches 2^31, or s·top_k·hidden or s·top_k·inter 2^33. rk_moe_gate_up_dev does not take it
+ * (RK_E_UNSUPPORTED). */
 int rk_pack_moe_fp8(const uint8_t *gate, const float *gate_scales, const uint8_t *up, const float *up_scales,
                     const uint8_t *down, const float *down_scales, int n_experts, int64_t hidden, int64_t inter,
                     rk_weight_id *id);

@@ -1,4 +1,6 @@
 """Routed fp8 layers at the edges of their ranges: stacks whose rows fill LDS, and what the calls on them refuse."""
+import ctypes
+
 import numpy as np
 import pytest
 
@@ -106,3 +108,36 @@ def test_an_infinite_result_leaves_its_neighbours(rk, monkeypatch, rows, dtype):
     assert (got[:, at] == np.inf).all()
     off, bound = np.abs(got - want)[:, rest], (most + (np.abs(want) + most) * ref.HALF[dtype] + 2.0**-24 * np.abs(want))[:, rest]
     assert (off <= bound).all(), f"{np.max(off / bound):.3g} times what it may be off"
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+def test_batches_whose_rows_pass_2_31_bytes(rk, dtype):
+    """33000 tokens of 8 experts: bucket rows of 2048 f32 values end behind 2^31 bytes, those of fp16 behind 2^30."""
+    note(f"fp8 experts, many tokens {dtype}")
+    r = np.random.default_rng(3)
+    s, e, k, h, i = 33000, 16, 8, 2048, 144
+    stack, wid = random_layer(rk, r, e, h, i)
+    x, v = ref.cast(r.standard_normal((s, h), dtype=np.float32), dtype)
+    ids = np.ascontiguousarray(r.random((s, e)).argsort(1)[:, :k], np.uint32)
+    wts = np.ascontiguousarray(r.uniform(0.1, 1, (s, k)), np.float32)
+    got = run_fp8(rk, wid, x, ids, wts, dtype)
+    some = np.unique(np.concatenate([[0, 1, s - 2, s - 1], r.integers(0, s, 60)]))
+    want, most = experts(v[some], ids[some], wts[some], stack, dtype)
+    most = most + rows_error(ids[some], wts[some], stack, v[some], dtype)
+    off, bound = np.abs(got[some] - want), most + (np.abs(want) + most) * ref.HALF[dtype] + 2.0**-24 * np.abs(want) + (2.0**-25 if dtype == "f16" else 0)
+    assert (off <= bound).all(), f"{np.max(off / bound):.3g} times what it may be off"
+    assert np.isfinite(got).all()
+
+
+def test_batches_that_are_too_large(rk):
+    note("fp8 experts, too large")
+    lib, r = rk.lib(), np.random.default_rng(4)
+    out = ctypes.c_void_p()
+    make = lambda w, s, top: lib.rk_moe_routed_plan_create(int(w), s, top, ctypes.byref(out))  # noqa: E731
+    _, wid = random_layer(rk, r, 2, 16, 65536)
+    assert make(wid, 1 << 16, 2) == rk.RK_E_SHAPE       # s·top_k·inter
+    _, wid = random_layer(rk, r, 2, 2048, 16)
+    assert make(wid, 1 << 20, 1) == rk.RK_E_SHAPE       # s·hidden
+    assert make(wid, 1 << 60, 1) == rk.RK_E_SHAPE
+    q8 = rk.pack_moe_f32(*[np.zeros(n, np.float32) for n in ((2, 32, 2048), (2, 32, 2048), (2, 2048, 32))])
+    assert make(q8, 1 << 18, 1) == rk.RK_E_SHAPE        # its rows are addressed in 32 bits
