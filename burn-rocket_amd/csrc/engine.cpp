@@ -990,6 +990,7 @@ int fp8_product_run(const Weight &w, const uint8_t *a, const float *as, int64_t 
   const bool exact = fp8_exact(c_dtype == RK_DTYPE_F32, w.ws_stride);
   if (rk_fp8_few_fits_codes(m, w.n, exact, g_eng->num_cus)) {
     Fp8FewArgs g{};
+    g.num_cus = g_eng->num_cus;
     g.x = a;
     g.as = as;
     g.m = (int)m;
@@ -2207,6 +2208,7 @@ int moe_run_fp8(CallScope &cs, const Weight &w, const MoePlan &plan, const void 
       RK_TRY(lists(1));
     }
     Fp8FewArgs g{};
+    g.num_cus = g_eng->num_cus;
     g.x = x;
     g.n = (int)I;
     g.k = (int)H;
@@ -3398,6 +3400,7 @@ extern "C" int rk_matmul_fp8_dev(rk_weight_id id, const void *x, int x_dtype, in
     // one launch, nothing in library memory
     if (rk_fp8_few_fits_x(m, w->ws_stride) && (capturing || rk_fp8_few_wants_x(m, w->ws_stride))) {
       Fp8FewArgs g{};
+      g.num_cus = g_eng->num_cus;
       g.x = x;
       g.m = (int)m;
       g.n = (int)w->n;

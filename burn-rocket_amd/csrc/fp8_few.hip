@@ -403,7 +403,7 @@ static hipError_t launch_few(Fp8FewArgs g, int rows, int n_tiles, hipStream_t st
   const int64_t n_nb = (g.n + 31) / 32;
   const auto wgs = [&](int groups) { return (n_nb + groups - 1) / groups * n_tiles; };
   g.groups = 1;
-  while (g.groups < FNW && (XT == FEW_CODES ? wgs(g.groups) > 256 : wgs(2 * g.groups) >= 256) && g.kt * 2 * g.groups <= 8 * FNW)
+  while (g.groups < FNW && (XT == FEW_CODES ? wgs(g.groups) > g.num_cus : wgs(2 * g.groups) >= g.num_cus) && g.kt * 2 * g.groups <= 8 * FNW)
     g.groups *= 2;
   hipLaunchKernelGGL(kern, dim3((unsigned)wgs(g.groups)), dim3(FNW * 64), smem, st, g);
   return hipGetLastError();
@@ -427,7 +427,7 @@ hipError_t rk_launch_fp8_few(const Fp8FewArgs &g, int x_dtype, bool exact, hipSt
   // Column blocks (32 rows) of a call, a wave's share of them: two where one each would be more than a round of workgroups
   // (with four the registers do not do). They read the weight once per share, which the caches serve.
   const int cb = x_dtype == FEW_CODES ? (g.m + 31) / 32 : 1, n_nb = (g.n + 31) / 32;
-  const int tm = (int64_t)n_nb * cb > 256 ? min(cb, 2) : 1;
+  const int tm = (int64_t)n_nb * cb > g.num_cus ? min(cb, 2) : 1;
   const int tiles = (cb + tm - 1) / tm;
 #define RK_FEW(XT, TM) \
   (exact ? launch_few<XT, FEW_DENSE, true, TM>(g, g.m, tiles, st) : launch_few<XT, FEW_DENSE, false, TM>(g, g.m, tiles, st))

@@ -318,6 +318,7 @@ struct Fp8FewArgs {
   int groups;                   // set by the launcher: blocks of n side by side in a workgroup
   int top_k;                    // tokens of top_k rows each, one behind the other (first product: or 0, by tok)
   int accumulate;               // rk_launch_fp8_token
+  int num_cus;
 };
 bool rk_fp8_few_fits_x(int64_t m, int kt);
 bool rk_fp8_few_wants_x(int64_t m, int kt);
