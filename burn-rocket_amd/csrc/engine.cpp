@@ -2510,6 +2510,7 @@ extern "C" int rk_moe_plan_create(rk_weight_id id, int64_t s, int top_k, const u
   RK_TRY(ensure("rk_moe_plan_create"));
   Weight *w;
   RK_TRY(moe_check(id, s, top_k, &w, "rk_moe_plan_create"));
+  if (!ids || !wts || !plan) return fail(RK_E_SHAPE, "rk_moe_plan_create", "null buffer");
   MoePlan *p = new MoePlan();
   const int rc = moe_plan(*w, s, top_k, ids, wts, p, g_eng->stream);
   if (rc != RK_OK) {
@@ -2536,8 +2537,9 @@ extern "C" int rk_moe_gate_up_dev(rk_weight_id id, const void *plan, const float
   std::lock_guard<std::mutex> lk(g_mu);
   RK_TRY(ensure("rk_moe_gate_up_dev"));
   const MoePlan *p = (const MoePlan *)plan;
-  if (!p || !act) return fail(RK_E_SHAPE, "rk_moe_gate_up_dev", "null plan or output");
+  if (!p) return fail(RK_E_SHAPE, "rk_moe_gate_up_dev", "null plan");
   if (p->routed && p->weight == id && p->has_batch && p->s == 0) return RK_OK;
+  if (!x || !act) return fail(RK_E_SHAPE, "rk_moe_gate_up_dev", "null buffer");
   Weight *w;
   RK_TRY(moe_planned_check(id, *p, &w, "rk_moe_gate_up_dev"));
   if (w->moe_fp8) return fail(RK_E_UNSUPPORTED, "rk_moe_gate_up_dev", "an fp8 expert stack");

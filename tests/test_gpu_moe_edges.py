@@ -141,3 +141,28 @@ def test_batches_that_are_too_large(rk):
     assert make(wid, 1 << 60, 1) == rk.RK_E_SHAPE
     q8 = rk.pack_moe_f32(*[np.zeros(n, np.float32) for n in ((2, 32, 2048), (2, 32, 2048), (2, 2048, 32))])
     assert make(q8, 1 << 18, 1) == rk.RK_E_SHAPE        # its rows are addressed in 32 bits
+
+
+def test_null_buffers_and_empty_batches(rk):
+    """Null buffers are refused before anything reads them; a batch without tokens needs none."""
+    note("moe null buffers")
+    lib, r = rk.lib(), np.random.default_rng(5)
+    q8 = int(rk.pack_moe_f32(*[r.standard_normal(n).astype(np.float32) for n in ((4, 32, 64), (4, 32, 64), (4, 64, 32))]))
+    ids, wts, out = np.zeros((3, 2), np.uint32), np.ones((3, 2), np.float32), ctypes.c_void_p()
+    make = lambda i, w, o: lib.rk_moe_plan_create(q8, 3, 2, i, w, o)  # noqa: E731
+    assert make(None, wts.ctypes.data, ctypes.byref(out)) == rk.RK_E_SHAPE
+    assert make(ids.ctypes.data, None, ctypes.byref(out)) == rk.RK_E_SHAPE
+    assert make(ids.ctypes.data, wts.ctypes.data, None) == rk.RK_E_SHAPE
+    plan = rk.routed_plan(q8, 3, 2)
+    b = rk.DeviceBuffer(1 << 14)
+    b.zero()
+    plan.route(3, b.ptr, b.ptr)
+    assert lib.rk_moe_gate_up_dev(q8, plan.ptr, None, b.ptr, None) == rk.RK_E_SHAPE
+    assert lib.rk_moe_gate_up_dev(q8, plan.ptr, b.ptr, None, None) == rk.RK_E_SHAPE
+    plan.route(0, None, None)
+    assert lib.rk_moe_gate_up_dev(q8, plan.ptr, None, None, None) == 0
+    plan.destroy()
+    _, wid = random_layer(rk, r, 8, 64, 48)
+    ids, wts = rk.route_experts(np.zeros((0, 8), np.float32), 2)
+    assert ids.shape == wts.shape == (0, 2)
+    assert rk.moe_layer(np.zeros((0, 64), np.float16), np.zeros((0, 8), np.float32), wid, 2).shape == (0, 64)
