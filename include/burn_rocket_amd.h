@@ -671,12 +671,13 @@ int rk_pack_moe_fp8(const uint8_t *gate, const float *gate_scales, const uint8_t
 /* The planned call on an fp8 stack with x and y of type dtype; accumulate: onto y. Products with
  * f32 sums: both where the rows are f32; the first one, whose results are quantized again, also
  * for fp16 rows, and for bf16 rows while there are few an expert; all others by the fp8 matrix
- * instructions. A token's weighted rows are summed in f32; for bf16 rows beyond a few an expert
- * each is an fp16 number under a power of two per 64 outputs or more first (2^-11 of itself; below
- * 2^-28 of the largest of these 2^-39 of that). x and y are 16-byte aligned and may be the same
- * buffer. A token's result depends in its rounding on the batch that it is in; equal batches give
- * equal bits. In a stream capture a plan of host lists is refused (RK_E_UNSUPPORTED): its calls
- * work in library memory. */
+ * instructions (in a first product codes of silu(gate)·up next to a border between two flip:
+ * 1.5e-3 of a bf16 result's size, about its own rounding). A token's weighted rows are summed in
+ * f32; for bf16 rows beyond a few an expert each is an fp16 number under a power of two per 64
+ * outputs or more first (2^-11 of itself; below 2^-28 of the largest of these 2^-39 of that). x and
+ * y are 16-byte aligned and may be the same buffer. A token's result depends in its rounding on the
+ * batch that it is in; equal batches give equal bits. In a stream capture a plan of host lists is
+ * refused (RK_E_UNSUPPORTED): its calls work in library memory. */
 int rk_moe_experts_fp8_dev(rk_weight_id id, const void *plan, const void *x, void *y, int dtype, int accumulate,
                            rk_stream stream);
 
