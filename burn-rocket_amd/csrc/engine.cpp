@@ -2430,6 +2430,9 @@ int moe_experts(rk_weight_id id, const float *x, int64_t s, int top_k, const uin
   if (!x || !y || !ids || !wts) return fail(RK_E_SHAPE, op, "null buffer");
   RK_TRY(moe_aligned(*w, x, y, op));
   hipStream_t st = pick(stream);
+  bool capturing;
+  RK_TRY(is_capturing(st, &capturing, op));
+  if (capturing) return fail(RK_E_UNSUPPORTED, op, "waits for its stream, which would end the capture: capture calls on a plan");
   CallScope cs(st);
   // The lists go from page-locked memory to scratch, long ones in two copies, so
   // that the host fills them while the GPU works: the rows during the quantizer

@@ -585,7 +585,8 @@ int rk_pack_moe_f32(const float *gate, const float *up, const float *down,
  * combine runs inside the down-projection launch: the workgroup that
  * completes a token's top_k rows (an arrival count per token and column
  * slice) sums them in ascending expert id, so y does not depend on the
- * order the workgroups finish in. RK_E_SHAPE when s·hidden or
+ * order the workgroups finish in. The call waits for its stream, and is
+ * refused in a stream capture (RK_E_UNSUPPORTED). RK_E_SHAPE when s·hidden or
  * s·top_k·inter reaches 2^31, or s·top_k·hidden·4 bytes reaches 2^31. */
 int rk_moe_experts_dev(rk_weight_id id, const float *x, int64_t s, int top_k,
                        const uint32_t *ids, const float *wts, float *y,

@@ -166,3 +166,34 @@ def test_null_buffers_and_empty_batches(rk):
     ids, wts = rk.route_experts(np.zeros((0, 8), np.float32), 2)
     assert ids.shape == wts.shape == (0, 2)
     assert rk.moe_layer(np.zeros((0, 64), np.float16), np.zeros((0, 8), np.float32), wid, 2).shape == (0, 64)
+
+
+@pytest.mark.parametrize("kind", ["q8", "fp8"])
+def test_host_ids_are_refused_in_a_capture_that_goes_on(rk, kind):
+    """rk_moe_experts_dev waits for its stream; in a capture it is refused, and the capture holds what else was recorded."""
+    note(f"moe host ids, captured, {kind}")
+    from test_gpu_sequences import Graph
+    lib, r = rk.lib(), np.random.default_rng(6)
+    s, e, k, h, i = 5, 4, 2, 64, 64
+    wid = int(random_layer(rk, r, e, h, i)[1] if kind == "fp8" else
+              rk.pack_moe_f32(*[r.standard_normal(n).astype(np.float32) for n in ((e, i, h), (e, i, h), (e, h, i))]))
+    ids, wts = choices(r, s, e, k, "any")
+    st = rk.new_stream()
+    x, y = rk.DeviceBuffer.from_array(r.standard_normal((s, h)).astype(np.float32)), rk.DeviceBuffer(s * h * 4)
+    q, sc = rk.DeviceBuffer(s * h), rk.DeviceBuffer(s * 4)
+    call = lambda f: f(wid, x.ptr, s, k, ids.ctypes.data, wts.ctypes.data, y.ptr, st)  # noqa: E731
+    rcs = []
+
+    def step():
+        assert lib.rk_quantize_fp8_dev(x.ptr, 0, s, h, q.ptr, sc.ptr, st) == 0
+        rcs.extend(call(f) for f in (lib.rk_moe_experts_dev, lib.rk_moe_experts_acc_dev))
+    g = Graph(st, step)
+    assert rcs == [rk.RK_E_UNSUPPORTED] * 2
+    for _ in range(2):
+        q.zero()
+        g.replay()
+        rk.synchronize(st)
+        assert (q.download((s, h), np.uint8) == ref.quantize(x.download((s, h), np.float32))[0]).all()
+        assert call(lib.rk_moe_experts_dev) == 0
+    g.destroy()
+    rk.destroy_stream(st)
