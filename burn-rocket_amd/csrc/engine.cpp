@@ -54,6 +54,7 @@ int fail(int rc, const char *op, const std::string &detail) {
 int hip_fail(hipError_t e, const char *op) {
   const int rc = (e == hipErrorOutOfMemory || e == hipErrorMemoryAllocation) ? RK_E_NOMEM
                                                                              : RK_E_DEVICE;
+  (void)hipGetLastError();  // reported here: the next launch does not report it again
   return fail(rc, op, hipGetErrorString(e));
 }
 

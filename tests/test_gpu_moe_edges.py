@@ -197,3 +197,16 @@ def test_host_ids_are_refused_in_a_capture_that_goes_on(rk, kind):
         assert call(lib.rk_moe_experts_dev) == 0
     g.destroy()
     rk.destroy_stream(st)
+
+
+def test_an_error_is_reported_once(rk):
+    """A call that the device has no memory for fails; the next one knows nothing of it."""
+    note("an error is reported once")
+    lib, r = rk.lib(), np.random.default_rng(7)
+    x = r.standard_normal((3, 64)).astype(np.float32)
+    b, q, sc = rk.DeviceBuffer.from_array(x), rk.DeviceBuffer(3 * 64), rk.DeviceBuffer(12)
+    out = ctypes.c_void_p()
+    assert lib.rk_device_alloc(1 << 50, ctypes.byref(out)) == rk.RK_E_NOMEM
+    assert lib.rk_quantize_fp8_dev(b.ptr, 0, 3, 64, q.ptr, sc.ptr, None) == 0, lib.rk_last_error()
+    rk.synchronize()
+    assert (q.download((3, 64), np.uint8) == ref.quantize(x)[0]).all()
