@@ -2560,8 +2560,8 @@ extern "C" int rk_moe_plan_destroy(void *plan) {
   MoePlan *p = (MoePlan *)plan;
   if (p && g_eng->routed_plans.count(p)) {
     RK_TRY(buf_fenceable(p->mem, nullptr, "rk_moe_plan_destroy"));
-    if (p->captured) HIP_TRY(hipDeviceSynchronize(), "rk_moe_plan_destroy");  // replays are known to the device alone
     RK_TRY(seq_buf_wait(p->mem, "rk_moe_plan_destroy"));
+    // (replays are known to the device alone: hipFree waits for them, and leaves captures on other streams as they are)
     seq_buf_free(p->mem);
     g_eng->routed_plans.erase(p);
     plan_free(p);
@@ -3499,6 +3499,9 @@ extern "C" int rk_moe_routed_plan_create(rk_weight_id id, int64_t max_s, int top
                  tiles_gu = take(rows * sizeof(MoeTile)), valid = take(4),
                  counts = take((size_t)rk_moe_lists_blocks(rows) * (w->n_experts + 1) * 4);
     const size_t lists = bytes;
+    bool capturing;
+    RK_TRY(is_capturing(g_eng->stream, &capturing, op));
+    if (capturing) return fail(RK_E_UNSUPPORTED, op, "the library's stream, on which the lists are cleared, is being captured");
     MoePlan *p = new MoePlan();
     size_t cnt_at = 0, cnt_bytes = 0;
     int rc = no_throw(op, [&]() -> int {
@@ -3512,9 +3515,10 @@ extern "C" int rk_moe_routed_plan_create(rk_weight_id id, int64_t max_s, int top
       HIP_TRY(hipMalloc(&p->mem.p, bytes), op);
       p->mem.bytes = bytes;
       // Lists of zeros name row 0 of token 0: what a call before their first building would read stays in bounds.
-      HIP_TRY(hipMemset(p->mem.p, 0, lists), op);
-      if (cnt_bytes) HIP_TRY(hipMemset((uint8_t *)p->mem.p + cnt_at, 0, cnt_bytes), op);
-      HIP_TRY(hipDeviceSynchronize(), op);
+      // (On the library's stream: what waits for all streams ends a capture on any of them.)
+      HIP_TRY(hipMemsetAsync(p->mem.p, 0, lists, g_eng->stream), op);
+      if (cnt_bytes) HIP_TRY(hipMemsetAsync((uint8_t *)p->mem.p + cnt_at, 0, cnt_bytes, g_eng->stream), op);
+      HIP_TRY(hipStreamSynchronize(g_eng->stream), op);
       g_eng->routed_plans.insert(p);
       return RK_OK;
     });

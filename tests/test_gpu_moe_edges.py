@@ -210,3 +210,56 @@ def test_an_error_is_reported_once(rk):
     assert lib.rk_quantize_fp8_dev(b.ptr, 0, 3, 64, q.ptr, sc.ptr, None) == 0, lib.rk_last_error()
     rk.synchronize()
     assert (q.download((3, 64), np.uint8) == ref.quantize(x)[0]).all()
+
+
+def test_plans_come_and_go_during_a_capture(rk):
+    """A plan made, and one whose graph is gone destroyed, while another stream is captured: the capture goes on."""
+    note("routed plans during a capture")
+    from test_gpu_sequences import Graph
+    lib, r = rk.lib(), np.random.default_rng(8)
+    s, e, k, h, i = 40, 4, 2, 256, 128
+    _, wid = random_layer(rk, r, e, h, i)
+    x = r.standard_normal((s, h)).astype(np.float32)
+    ids, wts = choices(r, s, e, k, "any")
+    b = [rk.DeviceBuffer.from_array(a) for a in (x, ids, wts, x)]
+    sts = [rk.new_stream(), rk.new_stream()]
+
+    def layer(plan, st):
+        plan.route(s, b[1].ptr, b[2].ptr, st)
+        assert lib.rk_moe_experts_planned_dev(int(wid), plan.ptr, b[0].ptr, b[3].ptr, st) == 0
+    old, now, made = rk.routed_plan(wid, s, k), rk.routed_plan(wid, s, k), []
+    g = Graph(sts[0], lambda: layer(old, sts[0]))
+    for _ in range(20):
+        g.replay()  # still running when the graph goes
+    g.destroy()
+
+    def step():
+        layer(now, sts[1])
+        made.append(rk.routed_plan(wid, s, k))
+        old.destroy()
+    g = Graph(sts[1], step)
+    rk.synchronize(sts[0])
+    want = run_host(rk, wid, x, ids, wts)
+    for _ in range(3):
+        b[3].upload(np.zeros_like(x))
+        g.replay()
+        rk.synchronize(sts[1])
+        assert (b[3].download(x.shape, np.float32) == want).all()
+    assert (run_routed(rk, wid, made[0], x, ids, wts) == want).all()
+    g.destroy()
+    for p in (now, made[0]):
+        p.destroy()
+    # on the library's own stream it is refused, and the capture goes on too
+    rcs, out = [], ctypes.c_void_p()
+
+    def own():
+        assert lib.rk_quantize_fp8_dev(b[0].ptr, 0, s, h, b[3].ptr, b[3].ptr + s * h, None) == 0
+        rcs.append(lib.rk_moe_routed_plan_create(int(wid), s, k, ctypes.byref(out)))
+    g = Graph(rk.stream(), own)
+    assert rcs == [rk.RK_E_UNSUPPORTED]
+    g.replay()
+    rk.synchronize()
+    assert (b[3].download((s, h), np.uint8) == ref.quantize(x)[0]).all()
+    g.destroy()
+    for st in sts:
+        rk.destroy_stream(st)
