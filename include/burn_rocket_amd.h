@@ -641,7 +641,8 @@ int rk_moe_route_dev(const void *logits, int dtype, int64_t s, int n_experts, in
  * its calls need: room for batches of up to max_s tokens. For stacks of up to 1024 experts
  * and up to 2^20 rows max_s·top_k. The limits of the stack's calls (rk_moe_experts_dev,
  * rk_pack_moe_fp8) hold for max_s. Freed by rk_moe_plan_destroy, which waits for its calls;
- * counted by rk_mem_stats as scratch. */
+ * counted by rk_mem_stats as scratch. Waits for the library's stream, and is refused while that
+ * one is captured (RK_E_UNSUPPORTED); captures on other streams go on. */
 int rk_moe_routed_plan_create(rk_weight_id id, int64_t max_s, int top_k, void **plan);
 /* The plan's next batch: ids [s, top_k] and wts [s, top_k] on the device, ordered on
  * `stream` after the calls that used the plan. An id that names no expert (>= n_experts: an

@@ -298,3 +298,33 @@ def test_captured_calls_up_to_64_kb_of_codes(rk, m, k):
         product(rk, host, "bf16", wid, n, "bf16", False)  # and the call outside of one, in between
     g.destroy()
     rk.destroy_stream(st)
+
+
+@pytest.mark.parametrize("dtype", ["f16", "f32"])
+def test_rows_behind_2_31_bytes(rk, dtype):
+    """A million rows, whose codes and results each pass 2^31 bytes: the same rows over and over, the last of them as the first."""
+    note(f"fp8 past 2^31 bytes {dtype}")
+    lib, r = rk.lib(), np.random.default_rng(41)
+    m, n, k, part = (1 << 20) + 37, 1040, 2064, 8192 + 64
+    codes, scales = ref.random_weight(r, n, k)
+    wid = int(rk.pack_fp8(codes, scales))
+    x, v = ref.cast(rows(r, part, k), dtype)
+    width = x.itemsize
+    dx, dc = rk.DeviceBuffer(m * k * width), rk.DeviceBuffer(m * n * width)
+    dx.upload(x)
+    done = part
+    while done < m:
+        more = min(done, m - done)  # whole parts: rows of the same index modulo the part
+        assert lib.rk_memcpy_dtod(dx.ptr + done * k * width, dx.ptr, more * k * width, None) == 0
+        done += more
+    assert lib.rk_matmul_fp8_dev(wid, dx.ptr, TYPES[dtype], m, k, dc.ptr, TYPES[dtype], None) == 0, lib.rk_last_error()
+    rk.synchronize()
+    got = []
+    for at in (0, m - 500):
+        dst = rk.DeviceBuffer(500 * n * width)
+        assert lib.rk_memcpy_dtod(dst.ptr, dc.ptr + at * n * width, 500 * n * width, None) == 0
+        rk.synchronize()
+        got.append(dst.download((500, n), x.dtype))
+        of = np.arange(at, at + 500) % part
+        q, s = ref.quantize(v[of])
+        check(got[-1], dtype, (q, s), (codes, scales), k, f"rows from {at}")
